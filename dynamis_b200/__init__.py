@@ -1,7 +1,7 @@
 """dynamis_b200 — B200 (sm_100a) implementation of the Dynamis per-step data-parallel hot path.
 
 Radius graph, space-filling-curve partition, halo maps and halo exchange behind the reference's
-own Python-facing names.  The compute lives in ``libdynb.so`` (hand-written CUDA, C ABI in
+own Python-facing names, and the work of a message-passing layer between two exchanges.  The compute lives in ``libdynb.so`` (hand-written CUDA, C ABI in
 ``include/dynb.h``); there is no CPU or PyTorch fallback.
 """
 
@@ -27,6 +27,15 @@ from .exchange import (  # noqa: F401
     supports_fabric_handles,
 )
 from .halo import extract_halo_info, filter_edges_to_radius  # noqa: F401
+from .message import (  # noqa: F401
+    NeighborIndex,
+    TypeIndex,
+    distance_bias,
+    neighbor_attention,
+    neighbor_index,
+    type_index,
+    type_linear,
+)
 from .partition import (  # noqa: F401
     KDTreePartitioner,
     SFCCurveType,

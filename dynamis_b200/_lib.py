@@ -14,6 +14,8 @@ SO_PATH = os.path.join(_HERE, "libdynb.so")
 
 DYNB_F32 = 0
 DYNB_F64 = 1
+DYNB_F16 = 2
+DYNB_BF16 = 3
 
 RG_SRC_OVERFLOW = 1
 RG_BAD_TARGET = 2
@@ -72,6 +74,27 @@ class HaloCtx(ctypes.Structure):
         ("world_size", ctypes.c_int32),
         ("rank", ctypes.c_int32),
     ]
+
+
+class Attention(ctypes.Structure):
+    """dynb_attention"""
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("q_dev", "k_dev", "v_dev")]
+        + [(name, ctypes.c_int64) for name in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+        + [(name, ctypes.c_void_p) for name in ("bias_dev", "rows_dev", "row_start_dev", "src_dev")]
+        + [(name, ctypes.c_int64) for name in ("n_targets", "n_sources", "n_edges")]
+        + [(name, ctypes.c_int32) for name in ("heads", "kv_heads", "dim", "dtype")]
+        + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+    )
+
+
+class TypeLinear(ctypes.Structure):
+    """dynb_type_linear_args"""
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("weight_dev", "order_dev", "start_dev")]
+        + [("n_rows", ctypes.c_int64)]
+        + [(name, ctypes.c_int32) for name in ("types", "inner", "outer", "dtype")]
+    )
 
 
 # name -> (restype, argtypes); every symbol include/dynb.h declares must be listed here
@@ -139,6 +162,19 @@ SIGNATURES = {
     "dynb_kdtree_workspace_bytes": (_i32, [_i64, _i64, ctypes.POINTER(_i64)]),
     "dynb_kdtree_partition": (_i32, [_p, _i64, _p, _i64, _p, _i32, _p, _i64, _p]),
     "dynb_integrator_step": (_i32, [_i32, _p, _p, _p, _p, _p, _i64, _f64, _f64, _f64, _p, _p, _f64, _p, _p, _p]),
+    "dynb_neighbor_index_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "dynb_neighbor_index_plan": (_i32, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dynb_neighbor_index_fill": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p]),
+    "dynb_neighbor_attention": (_i32, [_p, _p, _p, _p, _p]),
+    "dynb_neighbor_attention_backward": (_i32, [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "dynb_distance_bias": (_i32, [_p, _i64, _p, _i32, _i32, _f64, _i32, _p, _p]),
+    "dynb_distance_bias_workspace_bytes": (_i32, [_i64, _i32, _i32, ctypes.POINTER(_i64)]),
+    "dynb_distance_bias_backward": (_i32, [_p, _i64, _p, _i32, _i32, _f64, _i32, _p, _p, _p, _p, _i64, _p]),
+    "dynb_type_index_workspace_bytes": (_i32, [_i64, ctypes.POINTER(_i64)]),
+    "dynb_type_index": (_i32, [_p, _i64, _i32, _p, _p, _p, _p, _i64, _p]),
+    "dynb_type_linear": (_i32, [_p, _p, _i64, _p, _p, _p]),
+    "dynb_type_linear_workspace_bytes": (_i32, [_p, ctypes.POINTER(_i64)]),
+    "dynb_type_linear_backward": (_i32, [_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p]),
     "dynb_sfc_static_max_atoms": (_i64, []),
     "dynb_sfc_partition_static": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p]),
 }

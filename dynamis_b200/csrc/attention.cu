@@ -1,0 +1,98 @@
+// C entry points of neighbour attention: checks of the arguments, then the kernels of attention_forward.cu and attention_backward.cu.
+
+#include "attention.cuh"
+
+namespace dynb {
+
+static int attn_args(const dynb_attention* in, AttnArgs* a)
+{
+    if (in == nullptr) return fail_arg("null pointer");
+    if (in->dtype != DYNB_F32 && in->dtype != DYNB_F16 && in->dtype != DYNB_BF16) return fail_arg("neighbor_attention: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
+    if (in->n_targets < 0 || in->n_sources < 0 || in->n_edges < 0) return fail_arg("neighbor_attention: sizes must be non-negative");
+    if (in->n_targets >= INT32_MAX || in->n_sources >= INT32_MAX || in->n_edges >= INT32_MAX) return fail_arg("neighbor_attention: sizes must be below 2^31 - 1");
+    if (in->heads < 1 || in->kv_heads < 1 || in->heads % in->kv_heads != 0 || in->heads > 65535) return fail_arg("neighbor_attention: heads must be a multiple of kv_heads");
+    if (in->dim < 1 || in->dim > DYNB_ATTENTION_MAX_DIM) return fail_arg("neighbor_attention: dim must lie in [1, 256]");
+    if (in->n_targets > 0 && (!in->rows_dev || !in->row_start_dev || !in->q_dev)) return fail_arg("null pointer");
+    if (in->n_edges > 0 && (!in->src_dev || !in->k_dev || !in->v_dev)) return fail_arg("null pointer");
+    *a = AttnArgs{};
+    a->q = {in->q_dev, in->q_row, in->q_head};
+    a->k = {in->k_dev, in->k_row, in->k_head};
+    a->v = {in->v_dev, in->v_row, in->v_head};
+    a->bias = in->bias_dev;
+    a->rows = in->rows_dev;
+    a->row_start = in->row_start_dev;
+    a->src = in->src_dev;
+    a->n_targets = in->n_targets;
+    a->n_sources = in->n_sources;
+    a->n_edges = in->n_targets > 0 && in->n_sources > 0 ? in->n_edges : 0;   // an edge has both ends
+    a->heads = in->heads;
+    a->kv_heads = in->kv_heads;
+    a->shared = in->heads / in->kv_heads;
+    a->dim = in->dim;
+    a->scale = in->scale;
+    return DYNB_OK;
+}
+
+// Whether every piece of 16 bytes of a head starts on 16 bytes.
+static bool attn_wide(const AttnRows& r, int size)
+{
+    return reinterpret_cast<uintptr_t>(r.at) % 16 == 0 && r.row * size % 16 == 0 && r.head * size % 16 == 0;
+}
+
+}  // namespace dynb
+
+using namespace dynb;
+
+extern "C" int dynb_neighbor_attention(const dynb_attention* args, void* out_dev, float* out32_dev, float* stats_dev, void* stream)
+{
+    AttnArgs a;
+    const int rc = attn_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (a.n_targets == 0) return DYNB_OK;
+    if (out_dev == nullptr) return fail_arg("null pointer");
+    const int size = args->dtype == DYNB_F32 ? 4 : 2;
+    a.out = out_dev;
+    a.out32_w = out32_dev;
+    a.stats_w = stats_dev;
+    a.wide = a.dim * size % 16 == 0 && attn_wide(a.q, size) && attn_wide(a.k, size) && attn_wide(a.v, size) && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0;
+    DYNB_CUDA_OK(attn_forward(a, args->dtype, static_cast<cudaStream_t>(stream)));
+    return DYNB_OK;
+}
+
+extern "C" int dynb_neighbor_attention_backward(const dynb_attention* args, const void* d_out_dev, int64_t d_out_row, int64_t d_out_head,
+                                                const float* out32_dev, const float* stats_dev, const int32_t* cols_dev, const int32_t* col_start_dev,
+                                                const int32_t* in_edge_dev, const int32_t* in_dst_dev, float* delta_dev, void* dq_dev, void* dk_dev,
+                                                void* dv_dev, float* d_bias_dev, void* stream)
+{
+    AttnArgs a;
+    const int rc = attn_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    const int size = args->dtype == DYNB_F32 ? 4 : 2;
+    a.d_out = {d_out_dev, d_out_row, d_out_head};
+    a.out32 = out32_dev;
+    a.stats = stats_dev;
+    a.delta = delta_dev;
+    a.cols = cols_dev;
+    a.col_start = col_start_dev;
+    a.in_edge = in_edge_dev;
+    a.in_dst = in_dst_dev;
+    a.dq = dq_dev;
+    a.dk = dk_dev;
+    a.dv = dv_dev;
+    a.d_bias = d_bias_dev;
+    if (d_bias_dev != nullptr && a.bias == nullptr) return fail_arg("neighbor_attention_backward: a gradient of a bias that is not there");
+    a.wide = a.dim * size % 16 == 0 && attn_wide(a.q, size) && attn_wide(a.k, size) && attn_wide(a.v, size) && attn_wide(a.d_out, size);
+    for (const void* p : {(const void*)dq_dev, (const void*)dk_dev, (const void*)dv_dev}) a.wide = a.wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool cols = (dk_dev != nullptr || dv_dev != nullptr) && a.n_sources > 0;
+    if (a.n_targets > 0) {   // also for the sources' gradients, which read delta
+        if (!d_out_dev || !out32_dev || !stats_dev || !delta_dev) return fail_arg("null pointer");
+        DYNB_CUDA_OK(attn_backward_rows(a, args->dtype, s));
+    }
+    if (cols) {
+        if (!cols_dev || !col_start_dev || (a.n_edges > 0 && (!in_edge_dev || !in_dst_dev))) return fail_arg("null pointer");
+        if (a.k.at == nullptr || a.v.at == nullptr) return fail_arg("null pointer");
+        DYNB_CUDA_OK(attn_backward_cols(a, args->dtype, s));
+    }
+    return DYNB_OK;
+}

@@ -1,0 +1,385 @@
+// Rows times the matrix of their type (no counterpart in the reference, whose models leave it to their libraries):
+//     y_i = x_i W[type_i] + b[type_i],   dx_i = dy_i W[type_i]^T,   dW[t] = sum over the rows i of type t of x_i^T dy_i,   db[t] = sum dy_i.
+// The rows are not moved: `order` lists them by type (ascending inside a type), `start` where every type begins, and a tile gathers its
+// rows as it loads them.  Products are summed in 32 bits and rounded once.  Sums over rows go in stretches of a fixed number of rows of a
+// type, joined in their order: no atomics.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "clear.cuh"
+
+namespace dynb {
+
+constexpr int TL_M = 64, TL_N = 64, TL_K = 16, TL_THREADS = 256;
+constexpr int TL_STRETCH = 4096;   // rows of a type whose products are summed by one block
+
+struct TlArgs {
+    const void *x, *w, *b, *dy;
+    void *y, *dx, *dw, *db;
+    float* partial;
+    const int32_t *order, *start;
+    int64_t n, x_row, dy_row;
+    int types, inner, outer;
+};
+
+__device__ __forceinline__ float tl_get(const float* p) { return *p; }
+__device__ __forceinline__ float tl_get(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float tl_get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void tl_put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void tl_put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void tl_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+struct TlTile { int type; int64_t begin, end; };   // places in `order`
+
+// The tile-th piece of `per` rows when every type's rows are cut into such pieces; type < 0 behind the last.  All lanes of a warp call it.
+__device__ __forceinline__ TlTile tl_tile(const TlArgs& a, int64_t tile, int per)
+{
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int t0 = 0; t0 < a.types; t0 += 32) {
+        const int t = t0 + lane;
+        const int64_t s0 = t < a.types ? max(a.start[t], 0) : 0, s1 = t < a.types ? min((int64_t)a.start[t + 1], a.n) : 0;
+        const int64_t rows = max(s1 - s0, (int64_t)0);
+        const int mine = (int)((rows + per - 1) / per);
+        int total;
+        const int excl = warp_excl_scan(mine, lane, &total);
+        const bool here = tile >= before + excl && tile < before + excl + mine;
+        const uint32_t found = __ballot_sync(0xffffffffu, here);
+        if (found != 0) {
+            const int from = __ffs(found) - 1;
+            const int64_t begin = s0 + (tile - before - excl) * per;
+            TlTile r;
+            r.type = t0 + from;
+            r.begin = __shfl_sync(0xffffffffu, begin, from);
+            r.end = min(r.begin + per, __shfl_sync(0xffffffffu, s1, from));
+            return r;
+        }
+        before += total;
+    }
+    return {-1, 0, 0};
+}
+
+// One tile of 64 gathered rows times 64 columns.  `back`: dx = dy W^T instead of y = x W + b.
+template <typename T>
+__global__ void __launch_bounds__(TL_THREADS)
+tl_rows_kernel(const TlArgs a, int back)
+{
+    __shared__ float sa[TL_K][TL_M + 4], sb[TL_K][TL_N + 4];
+    __shared__ int32_t rows[TL_M];
+    const TlTile tile = tl_tile(a, blockIdx.x, TL_M);
+    if (tile.type < 0) return;
+    const T* const in = static_cast<const T*>(back ? a.dy : a.x);
+    const T* const w = static_cast<const T*>(a.w) + (int64_t)tile.type * a.inner * a.outer;
+    T* const out = static_cast<T*>(back ? a.dx : a.y);
+    const int64_t in_row = back ? a.dy_row : a.x_row;
+    const int kk = back ? a.outer : a.inner, nn = back ? a.inner : a.outer;
+    if (threadIdx.x < TL_M) {
+        int32_t r = -1;
+        if (tile.begin + threadIdx.x < tile.end) {
+            r = a.order[tile.begin + threadIdx.x];
+            if ((uint32_t)r >= (uint64_t)a.n) r = -1;
+        }
+        rows[threadIdx.x] = r;
+    }
+    __syncthreads();
+    const int col0 = blockIdx.y * TL_N, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    float acc[4][4] = {};
+    for (int k0 = 0; k0 < kk; k0 += TL_K) {
+#pragma unroll
+        for (int i = threadIdx.x; i < TL_M * TL_K; i += TL_THREADS) {
+            const int m = i / TL_K, k = i % TL_K;
+            sa[k][m] = rows[m] >= 0 && k0 + k < kk ? tl_get(in + rows[m] * in_row + k0 + k) : 0.0f;
+        }
+#pragma unroll
+        for (int i = threadIdx.x; i < TL_N * TL_K; i += TL_THREADS) {
+            const int k = back ? i % TL_K : i / TL_N, n = back ? i / TL_K : i % TL_N;
+            const bool ok = k0 + k < kk && col0 + n < nn;
+            sb[k][n] = ok ? tl_get(back ? w + (int64_t)(col0 + n) * a.outer + k0 + k : w + (int64_t)(k0 + k) * a.outer + col0 + n) : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TL_K; k++) {
+            float fa[4], fb[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                fa[i] = sa[k][ty * 4 + i];
+                fb[i] = sb[k][tx * 4 + i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t r = rows[ty * 4 + i];
+        if (r < 0) continue;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int n = col0 + tx * 4 + j;
+            if (n >= nn) continue;
+            float v = acc[i][j];
+            if (!back && a.b != nullptr) v += tl_get(static_cast<const T*>(a.b) + (int64_t)tile.type * a.outer + n);
+            tl_put(out + (int64_t)r * nn + n, v);
+        }
+    }
+}
+
+// Products x^T dy (and sums of dy) of one stretch of rows of a type, 64 x 64 elements of the matrix.
+template <typename T>
+__global__ void __launch_bounds__(TL_THREADS)
+tl_weights_kernel(const TlArgs a)
+{
+    __shared__ float sa[TL_K][TL_M + 4], sb[TL_K][TL_N + 4];
+    __shared__ int32_t rows[TL_K];
+    const TlTile tile = tl_tile(a, blockIdx.x, TL_STRETCH);
+    if (tile.type < 0) return;
+    const int row0 = blockIdx.y * TL_M, col0 = blockIdx.z * TL_N, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    float acc[4][4] = {}, sum = 0.0f;
+    for (int64_t k0 = tile.begin; k0 < tile.end; k0 += TL_K) {
+        if (threadIdx.x < TL_K) {
+            int32_t r = -1;
+            if (k0 + threadIdx.x < tile.end) {
+                r = a.order[k0 + threadIdx.x];
+                if ((uint32_t)r >= (uint64_t)a.n) r = -1;
+            }
+            rows[threadIdx.x] = r;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = threadIdx.x; i < TL_M * TL_K; i += TL_THREADS) {
+            const int k = i / TL_M, m = i % TL_M;
+            sa[k][m] = rows[k] >= 0 && row0 + m < a.inner ? tl_get(static_cast<const T*>(a.x) + rows[k] * a.x_row + row0 + m) : 0.0f;
+            sb[k][m] = rows[k] >= 0 && col0 + m < a.outer ? tl_get(static_cast<const T*>(a.dy) + rows[k] * a.dy_row + col0 + m) : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < TL_K; k++) {
+            float fa[4], fb[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                fa[i] = sa[k][ty * 4 + i];
+                fb[i] = sb[k][tx * 4 + i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
+            if (threadIdx.x < TL_N) sum += sb[k][threadIdx.x];
+        }
+        __syncthreads();
+    }
+    const int64_t cells = (int64_t)a.inner * a.outer;
+    float* const mine = a.partial + blockIdx.x * (cells + a.outer);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int m = row0 + ty * 4 + i, n = col0 + tx * 4 + j;
+            if (m < a.inner && n < a.outer) mine[(int64_t)m * a.outer + n] = acc[i][j];
+        }
+    if (blockIdx.y == 0 && threadIdx.x < TL_N && col0 + threadIdx.x < a.outer) mine[cells + col0 + threadIdx.x] = sum;
+}
+
+// The stretches of a type joined: blockIdx.y is the type.
+template <typename T>
+__global__ void __launch_bounds__(TL_THREADS)
+tl_join_kernel(const TlArgs a, int64_t stretches)
+{
+    const int type = blockIdx.y;
+    __shared__ int64_t first_of, count_of;
+    if (threadIdx.x < 32) {   // stretches of the types before
+        int64_t first = 0;
+        for (int t = threadIdx.x; t < type; t += 32) {
+            const int64_t rows = min((int64_t)a.start[t + 1], a.n) - max(a.start[t], 0);
+            first += rows > 0 ? (rows + TL_STRETCH - 1) / TL_STRETCH : 0;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
+        if (threadIdx.x == 0) {
+            const int64_t rows = min((int64_t)a.start[type + 1], a.n) - max(a.start[type], 0);
+            first_of = first;
+            count_of = rows > 0 ? (rows + TL_STRETCH - 1) / TL_STRETCH : 0;
+        }
+    }
+    __syncthreads();
+    const int64_t cells = (int64_t)a.inner * a.outer, all = cells + a.outer, first = first_of, count = min(count_of, stretches - first_of);
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
+        float sum = 0.0f;
+        for (int64_t c = 0; c < count; c++) sum += a.partial[(first + c) * all + i];
+        if (i < cells) {
+            if (a.dw != nullptr) tl_put(static_cast<T*>(a.dw) + type * cells + i, sum);
+        } else if (a.db != nullptr) {
+            tl_put(static_cast<T*>(a.db) + (int64_t)type * a.outer + (i - cells), sum);
+        }
+    }
+}
+
+// Types as sort keys; bit 0 of `words` where one lies outside [0, types).
+__global__ void __launch_bounds__(TL_THREADS)
+tl_keys_kernel(const int64_t* types, int64_t n, int n_types, uint64_t* keys, uint32_t* order, uint32_t* word)
+{
+    chain_begin();
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        int64_t t = types[i];
+        if (t < 0 || t >= n_types) {
+            atomicOr(word, 1u);
+            t = 0;
+        }
+        keys[i] = (uint64_t)t;
+        order[i] = (uint32_t)i;
+    }
+}
+
+// Where every type begins in the sorted keys; the word to the host.
+__global__ void __launch_bounds__(TL_THREADS)
+tl_start_kernel(const uint64_t* keys, int64_t n, int n_types, int32_t* start, const uint32_t* word, int64_t* host)
+{
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i <= n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int from = i == 0 ? 0 : (int)keys[i - 1] + 1, to = i == n ? n_types : (int)keys[i];
+        for (int t = from; t <= to; t++) start[t] = (int32_t)i;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) host[0] = *word;
+}
+
+struct TiLayout { int64_t word, keys, sort, total; };
+static TiLayout ti_layout(int64_t n)
+{
+    int64_t sort = 0;
+    (void)dynb_radix_sort_workspace_bytes(n, &sort);
+    TiLayout l;
+    l.word = 0;
+    l.keys = 256;
+    l.sort = align_up(l.keys + 8 * n, 256);
+    l.total = l.sort + align_up(sort, 256);
+    return l;
+}
+
+static int tl_args(const dynb_type_linear_args* in, TlArgs* a)
+{
+    if (in == nullptr) return fail_arg("null pointer");
+    if (in->dtype != DYNB_F32 && in->dtype != DYNB_F16 && in->dtype != DYNB_BF16) return fail_arg("type_linear: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
+    if (in->n_rows < 0 || in->n_rows >= INT32_MAX) return fail_arg("type_linear: rows must lie in [0, 2^31 - 1)");
+    if (in->types < 1 || in->types > DYNB_TYPE_LINEAR_MAX_TYPES) return fail_arg("type_linear: types must lie in [1, 4096]");
+    if (in->inner < 1 || in->outer < 1 || in->inner > DYNB_TYPE_LINEAR_MAX_WIDTH || in->outer > DYNB_TYPE_LINEAR_MAX_WIDTH)
+        return fail_arg("type_linear: widths must lie in [1, 16384]");
+    if (!in->start_dev || !in->weight_dev || (in->n_rows > 0 && !in->order_dev)) return fail_arg("null pointer");
+    *a = TlArgs{};
+    a->w = in->weight_dev;
+    a->order = in->order_dev;
+    a->start = in->start_dev;
+    a->n = in->n_rows;
+    a->types = in->types;
+    a->inner = in->inner;
+    a->outer = in->outer;
+    return DYNB_OK;
+}
+
+template <typename T>
+static cudaError_t tl_rows(const TlArgs& a, int back, cudaStream_t s)
+{
+    const int nn = back ? a.inner : a.outer;
+    const dim3 grid((unsigned)((a.n + TL_M - 1) / TL_M + a.types), (nn + TL_N - 1) / TL_N);
+    tl_rows_kernel<T><<<grid, TL_THREADS, 0, s>>>(a, back);
+    return cudaGetLastError();
+}
+
+static int64_t tl_stretches(int64_t n, int types) { return (n + TL_STRETCH - 1) / TL_STRETCH + types; }
+
+template <typename T>
+static cudaError_t tl_weights(const TlArgs& a, cudaStream_t s)
+{
+    const int64_t stretches = tl_stretches(a.n, a.types);
+    const dim3 grid((unsigned)stretches, (a.inner + TL_M - 1) / TL_M, (a.outer + TL_N - 1) / TL_N);
+    tl_weights_kernel<T><<<grid, TL_THREADS, 0, s>>>(a);
+    const int64_t all = (int64_t)a.inner * a.outer + a.outer;
+    tl_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((all + TL_THREADS - 1) / TL_THREADS, 1024), a.types), TL_THREADS, 0, s>>>(a, stretches);
+    return cudaGetLastError();
+}
+
+}  // namespace dynb
+
+using namespace dynb;
+
+extern "C" int dynb_type_linear(const dynb_type_linear_args* args, const void* x_dev, int64_t x_row, const void* bias_dev, void* y_dev, void* stream)
+{
+    TlArgs a;
+    const int rc = tl_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (a.n == 0) return DYNB_OK;
+    if (!x_dev || !y_dev) return fail_arg("null pointer");
+    a.x = x_dev; a.x_row = x_row; a.b = bias_dev; a.y = y_dev;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    DYNB_CUDA_OK(args->dtype == DYNB_F32 ? tl_rows<float>(a, 0, s) : args->dtype == DYNB_F16 ? tl_rows<__half>(a, 0, s) : tl_rows<__nv_bfloat16>(a, 0, s));
+    return DYNB_OK;
+}
+
+extern "C" int dynb_type_linear_workspace_bytes(const dynb_type_linear_args* args, int64_t* bytes)
+{
+    TlArgs a;
+    const int rc = tl_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (bytes == nullptr) return fail_arg("null pointer");
+    *bytes = tl_stretches(a.n, a.types) * ((int64_t)a.inner * a.outer + a.outer) * 4;
+    return DYNB_OK;
+}
+
+extern "C" int dynb_type_linear_backward(const dynb_type_linear_args* args, const void* x_dev, int64_t x_row, const void* d_y_dev, int64_t d_y_row,
+                                         void* d_x_dev, void* d_weight_dev, void* d_bias_dev, void* workspace_dev, int64_t workspace_bytes,
+                                         void* stream)
+{
+    TlArgs a;
+    const int rc = tl_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (a.n > 0 && (!x_dev || !d_y_dev)) return fail_arg("null pointer");
+    a.x = x_dev; a.x_row = x_row; a.dy = d_y_dev; a.dy_row = d_y_row; a.dx = d_x_dev; a.dw = d_weight_dev; a.db = d_bias_dev;
+    a.partial = static_cast<float*>(workspace_dev);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (d_x_dev != nullptr && a.n > 0)
+        DYNB_CUDA_OK(args->dtype == DYNB_F32 ? tl_rows<float>(a, 1, s) : args->dtype == DYNB_F16 ? tl_rows<__half>(a, 1, s) : tl_rows<__nv_bfloat16>(a, 1, s));
+    if (d_weight_dev != nullptr || d_bias_dev != nullptr) {
+        int64_t need;
+        (void)dynb_type_linear_workspace_bytes(args, &need);
+        if (workspace_dev == nullptr || workspace_bytes < need) return fail_arg("workspace too small");
+        DYNB_CUDA_OK(args->dtype == DYNB_F32 ? tl_weights<float>(a, s) : args->dtype == DYNB_F16 ? tl_weights<__half>(a, s) : tl_weights<__nv_bfloat16>(a, s));
+    }
+    return DYNB_OK;
+}
+
+extern "C" int dynb_type_index_workspace_bytes(int64_t n_rows, int64_t* bytes)
+{
+    if (n_rows < 0 || n_rows >= INT32_MAX || bytes == nullptr) return fail_arg("type_index: rows must lie in [0, 2^31 - 1)");
+    *bytes = ti_layout(n_rows).total;
+    return DYNB_OK;
+}
+
+extern "C" int dynb_type_index(const int64_t* types_dev, int64_t n_rows, int types, int32_t* order_dev, int32_t* start_dev, int64_t* word_host,
+                               void* workspace_dev, int64_t workspace_bytes, void* stream)
+{
+    if (n_rows < 0 || n_rows >= INT32_MAX) return fail_arg("type_index: rows must lie in [0, 2^31 - 1)");
+    if (types < 1 || types > DYNB_TYPE_LINEAR_MAX_TYPES) return fail_arg("type_index: types must lie in [1, 4096]");
+    if (!start_dev || !workspace_dev || !word_host || (n_rows > 0 && (!types_dev || !order_dev))) return fail_arg("null pointer");
+    const TiLayout l = ti_layout(n_rows);
+    if (workspace_bytes < l.total) return fail_arg("workspace too small");
+    void* const word_at = device_view_of_host(word_host);
+    if (word_at == nullptr) return fail_arg("type_index: word_host must be pinned");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
+    uint32_t* const word = reinterpret_cast<uint32_t*>(ws + l.word);
+    uint64_t* const keys = reinterpret_cast<uint64_t*>(ws + l.keys);
+    const unsigned blocks = (unsigned)std::max<int64_t>(1, std::min<int64_t>((n_rows + TL_THREADS) / TL_THREADS, (int64_t)sm_count_cached() * 8));
+    DYNB_CUDA_OK(clear_ranges(s, {word, 4, 0}));
+    DYNB_CUDA_OK(launch_chained(tl_keys_kernel, blocks, TL_THREADS, 0, s, types_dev, n_rows, types, keys, reinterpret_cast<uint32_t*>(order_dev), word));
+    if (n_rows > 0) {
+        const int rc = dynb_radix_sort_pairs(keys, reinterpret_cast<uint32_t*>(order_dev), n_rows, 0, types <= 256 ? 8 : 16, ws + l.sort, l.total - l.sort, stream);
+        if (rc != DYNB_OK) return rc;
+    }
+    tl_start_kernel<<<blocks, TL_THREADS, 0, s>>>(keys, n_rows, types, start_dev, word, static_cast<int64_t*>(word_at));
+    DYNB_CUDA_OK(cudaGetLastError());
+    return DYNB_OK;
+}

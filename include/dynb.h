@@ -32,6 +32,8 @@ extern "C" {
 
 #define DYNB_F32 0
 #define DYNB_F64 1
+#define DYNB_F16 2
+#define DYNB_BF16 3
 
 /* Bits of dynb_rg_header.status (set by kernels, read by the host after the plan). */
 #define DYNB_RG_SRC_OVERFLOW 1u    /* more periodic images than src_capacity: re-plan with header.M */
@@ -426,6 +428,84 @@ int dynb_integrator_step(int kind, float* pos_dev, float* vel_dev, const float* 
                          const float* noise_dev, int64_t n_atoms, double dt, double gamma, double kT,
                          const float* drift_ref_dev, float* drift_prev_vel_dev, double drift_threshold,
                          uint32_t* drift_state_dev, int32_t* drift_flag_dev, void* stream);
+
+/* ------------------------------------------------------------------ message-passing layers
+ * The work of a model's layer between two halo exchanges.  No counterpart in the reference, whose model adapters leave it to
+ * their libraries' gathers, products and scatters along edge_index (dynamis_model/src/dynamis_model/nnp/mace.py:260-364).
+ *
+ * Lists of a graph.  An edge goes from src (a row of [owned | ghost]) to dst (an owned row); the edges of a target stand behind one
+ * another, as every graph call here returns them.
+ *   rows[n_targets]        targets in the order of their edges, then those without edges, ascending
+ *   row_start[n_targets+1] first edge of rows[r] (row_start[r+1]: behind its last); the edges keep their numbers
+ *   src32[n_edges]         sources
+ *   cols[n_sources]        sources in the order of their first edge, then those without edges, ascending
+ *   col_start[n_sources+1], in_edge[n_edges], in_dst[n_edges]
+ *                          edges that leave cols[c], in ascending order, and their targets
+ * Two phases: the plan writes rows, row_start, src32, cols and col_start, and two words to pinned host memory: word 0 has bit 0 set
+ * when an endpoint is out of range and bit 1 when the edges of a target are apart (nothing else is valid then), word 1 is the longest
+ * list of a source.  The caller waits for the stream and calls the fill with word 1 and the workspace of the plan. */
+int dynb_neighbor_index_workspace_bytes(int64_t n_edges, int64_t n_targets, int64_t n_sources, int64_t* bytes);
+int dynb_neighbor_index_plan(const int64_t* src_dev, const int64_t* dst_dev, int64_t n_edges, int64_t n_targets, int64_t n_sources,
+                             int32_t* rows_dev, int32_t* row_start_dev, int32_t* src32_dev, int32_t* cols_dev, int32_t* col_start_dev,
+                             int64_t* words_host, void* workspace_dev, int64_t workspace_bytes, void* stream);
+int dynb_neighbor_index_fill(const int64_t* dst_dev, int64_t n_edges, int64_t n_targets, int64_t n_sources, const int32_t* src32_dev,
+                             const int32_t* col_start_dev, int64_t longest, int32_t* in_edge_dev, int32_t* in_dst_dev, void* workspace_dev,
+                             int64_t workspace_bytes, void* stream);
+
+/* Attention of every target to its neighbours: per head, z_e = scale q[dst] . k[src] + bias[e], p = softmax of z over the edges of
+ * the target, out[dst] = sum p_e v[src].  Query head h reads key and value head h / (heads / kv_heads).  Edges with a bias of -inf take
+ * no part; a target without edges that do gives zeros.  Strides are in elements, a head's elements are consecutive; out is contiguous. */
+#define DYNB_ATTENTION_MAX_DIM 256
+typedef struct dynb_attention {
+    const void *q_dev, *k_dev, *v_dev;      /* [n_targets, heads, dim], [n_sources, kv_heads, dim] twice, of `dtype` */
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    const float* bias_dev;                  /* [n_edges, heads] or NULL */
+    const int32_t *rows_dev, *row_start_dev, *src_dev;
+    int64_t n_targets, n_sources, n_edges;
+    int32_t heads, kv_heads, dim, dtype;    /* DYNB_F32, DYNB_F16, DYNB_BF16 */
+    float scale;
+    int32_t reserved;
+} dynb_attention;
+/* out32_dev [n_targets, heads, dim] (the unrounded result; may be out_dev for DYNB_F32) and stats_dev [n_targets, 2, heads] are for
+ * the backward pass; NULL when there is none. */
+int dynb_neighbor_attention(const dynb_attention* args, void* out_dev, float* out32_dev, float* stats_dev, void* stream);
+/* Gradients, each NULL when it is not wanted; contiguous.  delta_dev [n_targets, heads] is scratch.  No atomics: the sums of a row
+ * are in the order of its list. */
+int dynb_neighbor_attention_backward(const dynb_attention* args, const void* d_out_dev, int64_t d_out_row, int64_t d_out_head,
+                                     const float* out32_dev, const float* stats_dev, const int32_t* cols_dev, const int32_t* col_start_dev,
+                                     const int32_t* in_edge_dev, const int32_t* in_dst_dev, float* delta_dev, void* dq_dev, void* dk_dev,
+                                     void* dv_dev, float* d_bias_dev, void* stream);
+
+/* Learned bias from distances: bias[e, h] = the cubic B-spline with the `buckets` values table[:, h] over [0, cutoff] at dist[e], plus
+ * (smooth) the logarithm of (1 - u)^3 (1 + 3 u + 6 u^2), u = dist / cutoff; -inf from the cutoff on.  The workspace is for d_table. */
+#define DYNB_DISTANCE_BIAS_MAX_BUCKETS 1024
+#define DYNB_DISTANCE_BIAS_MAX_HEADS 1024
+int dynb_distance_bias(const float* dist_dev, int64_t n, const float* table_dev, int buckets, int heads, double cutoff, int smooth,
+                       float* bias_dev, void* stream);
+int dynb_distance_bias_workspace_bytes(int64_t n, int buckets, int heads, int64_t* bytes);
+int dynb_distance_bias_backward(const float* dist_dev, int64_t n, const float* table_dev, int buckets, int heads, double cutoff, int smooth,
+                                const float* d_bias_dev, float* d_dist_dev, float* d_table_dev, void* workspace_dev, int64_t workspace_bytes,
+                                void* stream);
+
+/* Rows by type: order[n_rows] lists the rows of type 0, of type 1, ..., ascending inside a type; start[types + 1].  word_host (pinned):
+ * bit 0 when a type lies outside [0, types). */
+#define DYNB_TYPE_LINEAR_MAX_TYPES 4096
+#define DYNB_TYPE_LINEAR_MAX_WIDTH 16384
+int dynb_type_index_workspace_bytes(int64_t n_rows, int64_t* bytes);
+int dynb_type_index(const int64_t* types_dev, int64_t n_rows, int types, int32_t* order_dev, int32_t* start_dev, int64_t* word_host,
+                    void* workspace_dev, int64_t workspace_bytes, void* stream);
+/* Products with the matrix of a row's type: y[i] = x[i] weight[type_i] (+ bias[type_i]); weight [types, inner, outer], contiguous, as
+ * bias and the outputs are.  x and d_y have row strides in elements. */
+typedef struct dynb_type_linear_args {
+    const void* weight_dev;
+    const int32_t *order_dev, *start_dev;
+    int64_t n_rows;
+    int32_t types, inner, outer, dtype;     /* DYNB_F32, DYNB_F16, DYNB_BF16 */
+} dynb_type_linear_args;
+int dynb_type_linear(const dynb_type_linear_args* args, const void* x_dev, int64_t x_row, const void* bias_dev, void* y_dev, void* stream);
+int dynb_type_linear_workspace_bytes(const dynb_type_linear_args* args, int64_t* bytes);
+int dynb_type_linear_backward(const dynb_type_linear_args* args, const void* x_dev, int64_t x_row, const void* d_y_dev, int64_t d_y_row,
+                              void* d_x_dev, void* d_weight_dev, void* d_bias_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ partition without a workspace
  * No counterpart in the reference.  Same result as dynb_sfc_partition, for callers that must not
