@@ -94,6 +94,7 @@ class TypeLinear(ctypes.Structure):
         [(name, ctypes.c_void_p) for name in ("weight_dev", "order_dev", "start_dev")]
         + [("n_rows", ctypes.c_int64)]
         + [(name, ctypes.c_int32) for name in ("types", "inner", "outer", "dtype")]
+        + [("status_dev", ctypes.c_void_p)]
     )
 
 

@@ -4,65 +4,14 @@
 // rows as it loads them.  Products are summed in 32 bits and rounded once.  Sums over rows go in stretches of a fixed number of rows of a
 // type, joined in their order: no atomics.
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include <algorithm>
-
 #include "clear.cuh"
+#include "type_linear.cuh"
 
 namespace dynb {
 
 constexpr int TL_M = 64, TL_N = 64, TL_K = 16, TL_THREADS = 256;
-constexpr int TL_STRETCH = 4096;   // rows of a type whose products are summed by one block
 
-struct TlArgs {
-    const void *x, *w, *b, *dy;
-    void *y, *dx, *dw, *db;
-    float* partial;
-    const int32_t *order, *start;
-    int64_t n, x_row, dy_row;
-    int types, inner, outer;
-};
-
-__device__ __forceinline__ float tl_get(const float* p) { return *p; }
-__device__ __forceinline__ float tl_get(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ float tl_get(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void tl_put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void tl_put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void tl_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-struct TlTile { int type; int64_t begin, end; };   // places in `order`
-
-// The tile-th piece of `per` rows when every type's rows are cut into such pieces; type < 0 behind the last.  All lanes of a warp call it.
-__device__ __forceinline__ TlTile tl_tile(const TlArgs& a, int64_t tile, int per)
-{
-    const int lane = threadIdx.x & 31;
-    int64_t before = 0;
-    for (int t0 = 0; t0 < a.types; t0 += 32) {
-        const int t = t0 + lane;
-        const int64_t s0 = t < a.types ? max(a.start[t], 0) : 0, s1 = t < a.types ? min((int64_t)a.start[t + 1], a.n) : 0;
-        const int64_t rows = max(s1 - s0, (int64_t)0);
-        const int mine = (int)((rows + per - 1) / per);
-        int total;
-        const int excl = warp_excl_scan(mine, lane, &total);
-        const bool here = tile >= before + excl && tile < before + excl + mine;
-        const uint32_t found = __ballot_sync(0xffffffffu, here);
-        if (found != 0) {
-            const int from = __ffs(found) - 1;
-            const int64_t begin = s0 + (tile - before - excl) * per;
-            TlTile r;
-            r.type = t0 + from;
-            r.begin = __shfl_sync(0xffffffffu, begin, from);
-            r.end = min(r.begin + per, __shfl_sync(0xffffffffu, s1, from));
-            return r;
-        }
-        before += total;
-    }
-    return {-1, 0, 0};
-}
-
-// One tile of 64 gathered rows times 64 columns.  `back`: dx = dy W^T instead of y = x W + b.
+// One tile of 64 gathered rows times 64 columns, for matrices that do not fit into shared memory (type_linear_mma.cu).  `back`: dx = dy W^T instead of y = x W + b.
 template <typename T>
 __global__ void __launch_bounds__(TL_THREADS)
 tl_rows_kernel(const TlArgs a, int back)
@@ -130,62 +79,6 @@ tl_rows_kernel(const TlArgs a, int back)
     }
 }
 
-// Products x^T dy (and sums of dy) of one stretch of rows of a type, 64 x 64 elements of the matrix.
-template <typename T>
-__global__ void __launch_bounds__(TL_THREADS)
-tl_weights_kernel(const TlArgs a)
-{
-    __shared__ float sa[TL_K][TL_M + 4], sb[TL_K][TL_N + 4];
-    __shared__ int32_t rows[TL_K];
-    const TlTile tile = tl_tile(a, blockIdx.x, TL_STRETCH);
-    if (tile.type < 0) return;
-    const int row0 = blockIdx.y * TL_M, col0 = blockIdx.z * TL_N, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    float acc[4][4] = {}, sum = 0.0f;
-    for (int64_t k0 = tile.begin; k0 < tile.end; k0 += TL_K) {
-        if (threadIdx.x < TL_K) {
-            int32_t r = -1;
-            if (k0 + threadIdx.x < tile.end) {
-                r = a.order[k0 + threadIdx.x];
-                if ((uint32_t)r >= (uint64_t)a.n) r = -1;
-            }
-            rows[threadIdx.x] = r;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = threadIdx.x; i < TL_M * TL_K; i += TL_THREADS) {
-            const int k = i / TL_M, m = i % TL_M;
-            sa[k][m] = rows[k] >= 0 && row0 + m < a.inner ? tl_get(static_cast<const T*>(a.x) + rows[k] * a.x_row + row0 + m) : 0.0f;
-            sb[k][m] = rows[k] >= 0 && col0 + m < a.outer ? tl_get(static_cast<const T*>(a.dy) + rows[k] * a.dy_row + col0 + m) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < TL_K; k++) {
-            float fa[4], fb[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                fa[i] = sa[k][ty * 4 + i];
-                fb[i] = sb[k][tx * 4 + i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
-            if (threadIdx.x < TL_N) sum += sb[k][threadIdx.x];
-        }
-        __syncthreads();
-    }
-    const int64_t cells = (int64_t)a.inner * a.outer;
-    float* const mine = a.partial + blockIdx.x * (cells + a.outer);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int m = row0 + ty * 4 + i, n = col0 + tx * 4 + j;
-            if (m < a.inner && n < a.outer) mine[(int64_t)m * a.outer + n] = acc[i][j];
-        }
-    if (blockIdx.y == 0 && threadIdx.x < TL_N && col0 + threadIdx.x < a.outer) mine[cells + col0 + threadIdx.x] = sum;
-}
-
 // The stretches of a type joined: blockIdx.y is the type.
 template <typename T>
 __global__ void __launch_bounds__(TL_THREADS)
@@ -197,14 +90,14 @@ tl_join_kernel(const TlArgs a, int64_t stretches)
         int64_t first = 0;
         for (int t = threadIdx.x; t < type; t += 32) {
             const int64_t rows = min((int64_t)a.start[t + 1], a.n) - max(a.start[t], 0);
-            first += rows > 0 ? (rows + TL_STRETCH - 1) / TL_STRETCH : 0;
+            first += rows > 0 ? (rows + a.stretch - 1) / a.stretch : 0;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
         if (threadIdx.x == 0) {
             const int64_t rows = min((int64_t)a.start[type + 1], a.n) - max(a.start[type], 0);
             first_of = first;
-            count_of = rows > 0 ? (rows + TL_STRETCH - 1) / TL_STRETCH : 0;
+            count_of = rows > 0 ? (rows + a.stretch - 1) / a.stretch : 0;
         }
     }
     __syncthreads();
@@ -277,11 +170,13 @@ static int tl_args(const dynb_type_linear_args* in, TlArgs* a)
     a->types = in->types;
     a->inner = in->inner;
     a->outer = in->outer;
+    a->stretch = tl_stretch(in->n_rows, in->inner, in->outer, in->dtype);
+    a->status = in->status_dev;
     return DYNB_OK;
 }
 
 template <typename T>
-static cudaError_t tl_rows(const TlArgs& a, int back, cudaStream_t s)
+static cudaError_t tl_rows_plain(const TlArgs& a, int back, cudaStream_t s)
 {
     const int nn = back ? a.inner : a.outer;
     const dim3 grid((unsigned)((a.n + TL_M - 1) / TL_M + a.types), (nn + TL_N - 1) / TL_N);
@@ -289,16 +184,22 @@ static cudaError_t tl_rows(const TlArgs& a, int back, cudaStream_t s)
     return cudaGetLastError();
 }
 
-static int64_t tl_stretches(int64_t n, int types) { return (n + TL_STRETCH - 1) / TL_STRETCH + types; }
-
-template <typename T>
-static cudaError_t tl_weights(const TlArgs& a, cudaStream_t s)
+static cudaError_t tl_rows(const TlArgs& a, int back, int dtype, cudaStream_t s)
 {
-    const int64_t stretches = tl_stretches(a.n, a.types);
-    const dim3 grid((unsigned)stretches, (a.inner + TL_M - 1) / TL_M, (a.outer + TL_N - 1) / TL_N);
-    tl_weights_kernel<T><<<grid, TL_THREADS, 0, s>>>(a);
-    const int64_t all = (int64_t)a.inner * a.outer + a.outer;
-    tl_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((all + TL_THREADS - 1) / TL_THREADS, 1024), a.types), TL_THREADS, 0, s>>>(a, stretches);
+    cudaError_t rc;
+    if (tl_mma_rows(a, back, dtype, s, &rc)) return rc;
+    return dtype == DYNB_F32 ? tl_rows_plain<float>(a, back, s) : dtype == DYNB_F16 ? tl_rows_plain<__half>(a, back, s) : tl_rows_plain<__nv_bfloat16>(a, back, s);
+}
+
+static cudaError_t tl_weights(const TlArgs& a, int dtype, cudaStream_t s)
+{
+    const cudaError_t rc = tl_mma_weights(a, dtype, s);
+    if (rc != cudaSuccess) return rc;
+    const int64_t stretches = tl_stretches(a.n, a.types, a.stretch), all = (int64_t)a.inner * a.outer + a.outer;
+    const dim3 grid((unsigned)std::min<int64_t>((all + TL_THREADS - 1) / TL_THREADS, 1024), a.types);
+    if (dtype == DYNB_F32) tl_join_kernel<float><<<grid, TL_THREADS, 0, s>>>(a, stretches);
+    else if (dtype == DYNB_F16) tl_join_kernel<__half><<<grid, TL_THREADS, 0, s>>>(a, stretches);
+    else tl_join_kernel<__nv_bfloat16><<<grid, TL_THREADS, 0, s>>>(a, stretches);
     return cudaGetLastError();
 }
 
@@ -315,7 +216,7 @@ extern "C" int dynb_type_linear(const dynb_type_linear_args* args, const void* x
     if (!x_dev || !y_dev) return fail_arg("null pointer");
     a.x = x_dev; a.x_row = x_row; a.b = bias_dev; a.y = y_dev;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    DYNB_CUDA_OK(args->dtype == DYNB_F32 ? tl_rows<float>(a, 0, s) : args->dtype == DYNB_F16 ? tl_rows<__half>(a, 0, s) : tl_rows<__nv_bfloat16>(a, 0, s));
+    DYNB_CUDA_OK(tl_rows(a, 0, args->dtype, s));
     return DYNB_OK;
 }
 
@@ -325,7 +226,7 @@ extern "C" int dynb_type_linear_workspace_bytes(const dynb_type_linear_args* arg
     const int rc = tl_args(args, &a);
     if (rc != DYNB_OK) return rc;
     if (bytes == nullptr) return fail_arg("null pointer");
-    *bytes = tl_stretches(a.n, a.types) * ((int64_t)a.inner * a.outer + a.outer) * 4;
+    *bytes = tl_stretches(a.n, a.types, a.stretch) * ((int64_t)a.inner * a.outer + a.outer) * 4;
     return DYNB_OK;
 }
 
@@ -341,12 +242,12 @@ extern "C" int dynb_type_linear_backward(const dynb_type_linear_args* args, cons
     a.partial = static_cast<float*>(workspace_dev);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (d_x_dev != nullptr && a.n > 0)
-        DYNB_CUDA_OK(args->dtype == DYNB_F32 ? tl_rows<float>(a, 1, s) : args->dtype == DYNB_F16 ? tl_rows<__half>(a, 1, s) : tl_rows<__nv_bfloat16>(a, 1, s));
+        DYNB_CUDA_OK(tl_rows(a, 1, args->dtype, s));
     if (d_weight_dev != nullptr || d_bias_dev != nullptr) {
         int64_t need;
         (void)dynb_type_linear_workspace_bytes(args, &need);
         if (workspace_dev == nullptr || workspace_bytes < need) return fail_arg("workspace too small");
-        DYNB_CUDA_OK(args->dtype == DYNB_F32 ? tl_weights<float>(a, s) : args->dtype == DYNB_F16 ? tl_weights<__half>(a, s) : tl_weights<__nv_bfloat16>(a, s));
+        DYNB_CUDA_OK(tl_weights(a, args->dtype, s));
     }
     return DYNB_OK;
 }

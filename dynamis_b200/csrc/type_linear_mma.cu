@@ -1,0 +1,614 @@
+// The products by type on the tensor cores.
+//
+// y = x W + b and dx = dy W^T: a block keeps the whole matrix of a type for its columns in shared memory (laid out once per type) and takes
+// tiles of 128 rows one after the other: eight warps gather the rows into stages of 64 columns, one thread issues the products, four
+// warps take the sums out of tensor memory, which holds two of them, and store the rows.  What bounds it is the memory that the rows need.
+//
+// dW = sum x_i^T dy_i: a block takes a stretch of rows of one type, 128 x up to 256 elements of the matrix; both operands are the gathered
+// rows as they are, read along their columns.  db is a product too, with a tile of ones.
+//
+// fp32 operands are split into three bf16 parts (8 bits each, together all 24): v = p0 + p1 + p2.  Six of the nine products are formed,
+// those left out are below 2^-25 of the whole; the small ones are added first.  Sums are in fp32.
+
+#include <type_traits>
+
+#include "type_linear.cuh"
+#include "umma.cuh"
+
+namespace dynb {
+
+constexpr int TM_ROWS = 128;
+constexpr int TM_FEED = 8;                  // warps that gather
+constexpr int TM_THREADS = (4 + 1 + TM_FEED) * 32;
+constexpr int TM_FEED_THREADS = TM_FEED * 32;
+constexpr int TM_MAX_STAGES = 8;
+constexpr int TM_SMEM = 225 * 1024;
+constexpr int TW_ROWS = 32;                 // rows of a stage of the weights' gradient
+
+template <typename T> struct TmParts { static constexpr int N = 1; };
+template <> struct TmParts<float> { static constexpr int N = 3; };
+template <typename T> struct TmRaw { uint4 v[sizeof(T) == 4 ? 2 : 1]; };   // 8 elements as loaded
+
+// Eight elements `step` apart from p, the first `have` of them real, zeros behind.  `wide`: 16-byte boundaries, step 1 and have 0 or 8.
+template <typename T>
+__device__ __forceinline__ TmRaw<T> tm_load(const T* p, int64_t step, int have, bool wide)
+{
+    TmRaw<T> r;
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(r) / 16); i++) r.v[i] = have > 0 ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        return r;
+    }
+    using W = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+    union { TmRaw<T> r; W w[8]; } u;
+#pragma unroll
+    for (int i = 0; i < 8; i++) u.w[i] = i < have ? *reinterpret_cast<const W*>(p + i * step) : (W)0;
+    return u.r;
+}
+
+// The parts of eight elements, 16 bytes each, to `at`, `at + apart`, ...
+template <typename T>
+__device__ __forceinline__ void tm_store(const TmRaw<T>& r, unsigned char* at, int apart)
+{
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(at) = r.v[0];
+    } else {
+        const uint32_t* const bits = reinterpret_cast<const uint32_t*>(&r);
+        uint32_t part[3][4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float v[2] = {__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1])};
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(&b);
+                part[p][i] = w;
+                v[0] -= __uint_as_float(w << 16);          // exact
+                v[1] -= __uint_as_float(w & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) *reinterpret_cast<uint4*>(at + p * apart) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+    }
+}
+
+// The pairs of parts whose products are formed, the small ones first.
+template <int PARTS, typename F>
+__device__ __forceinline__ void tm_pairs(F f)
+{
+    if constexpr (PARTS == 1) {
+        f(0, 0);
+    } else {
+        f(2, 0); f(0, 2); f(1, 1); f(1, 0); f(0, 1); f(0, 0);
+    }
+}
+
+// Walks the pieces [first, first + count) of TM_ROWS rows.
+struct TmCursor {
+    TlTile tile;
+    int64_t end_of_type;
+    int64_t left;
+
+    __device__ __forceinline__ void start(const TlArgs& a, int64_t first, int64_t count)   // all lanes of a warp
+    {
+        left = count;
+        tile = {-1, 0, 0};
+        if (count <= 0) return;
+        tile = tl_tile(a, first, TM_ROWS);
+        if (tile.type < 0) { left = 0; return; }
+        int64_t s0;
+        tl_rows_of(a, tile.type, &s0, &end_of_type);
+    }
+    __device__ __forceinline__ void next(const TlArgs& a)
+    {
+        if (--left <= 0) { tile.type = -1; return; }
+        tile.begin += TM_ROWS;
+        if (tile.begin >= end_of_type) {
+            do {
+                if (++tile.type >= a.types) { tile.type = -1; left = 0; return; }
+                tl_rows_of(a, tile.type, &tile.begin, &end_of_type);
+            } while (tile.begin >= end_of_type);
+        }
+        tile.end = min(tile.begin + TM_ROWS, end_of_type);
+    }
+};
+
+struct TmPlan {
+    int back, columns, column_stride, chunks, stages, tensor_columns, panel_bytes, wide_in, wide_w, store;   // store: bytes a store may have
+};
+
+struct TmBars { uint64_t full[TM_MAX_STAGES], empty[TM_MAX_STAGES], panel_full, panel_free, sums_full[2], sums_free[2]; uint32_t tensor; };
+
+__device__ __forceinline__ void tm_ran_out(const TlArgs& a)
+{
+    if (a.status != nullptr) {
+        *reinterpret_cast<volatile uint32_t*>(a.status) = 1u;
+        __threadfence_system();
+    }
+}
+
+// `n` results of a row from column c on, in stores of `width` bytes (32, 16 or one element).
+template <typename T, int N>
+__device__ __forceinline__ void tm_put_row(T* at, const float (&v)[N], int n, int width)
+{
+    if (width >= 16 && n >= N) {
+        constexpr int WORDS = N * (int)sizeof(T) / 4;
+        uint32_t w[WORDS];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = __float_as_uint(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) {
+                if constexpr (std::is_same<T, __half>::value) {
+                    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+        }
+        if (width >= 32) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(reinterpret_cast<char*>(at) + 4 * i), "r"(w[i]), "r"(w[i + 1]),
+                             "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                             : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<char*>(at) + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (i < n) tl_put(at + i, v[i]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(TM_THREADS, 1)
+tm_rows_kernel(const TlArgs a, const TmPlan plan)
+{
+    constexpr int PARTS = TmParts<T>::N, STAGE = PARTS * TM_ROWS * 128;
+    extern __shared__ unsigned char raw_smem[];
+    __shared__ TmBars bars;
+    unsigned char* const panel = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+    unsigned char* const stage0 = panel + plan.panel_bytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const T* const in = static_cast<const T*>(plan.back ? a.dy : a.x);
+    T* const out = static_cast<T*>(plan.back ? a.dx : a.y);
+    const int64_t in_row = plan.back ? a.dy_row : a.x_row;
+    const int kk = plan.back ? a.outer : a.inner, nn = plan.back ? a.inner : a.outer;
+    const int col0 = blockIdx.y * plan.columns;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < plan.stages; s++) {
+            bar_init(&bars.full[s], TM_FEED);
+            bar_init(&bars.empty[s], 1);
+        }
+        bar_init(&bars.panel_full, TM_FEED);
+        bar_init(&bars.panel_free, 1);
+        for (int b = 0; b < 2; b++) {
+            bar_init(&bars.sums_full[b], 1);
+            bar_init(&bars.sums_free[b], 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tensor_alloc(&bars.tensor, plan.tensor_columns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = bars.tensor;
+
+    int64_t pieces = 0;
+    (void)tl_tile(a, INT64_MAX, TM_ROWS, &pieces);
+    const int64_t per = (pieces + gridDim.x - 1) / gridDim.x, first = blockIdx.x * per;
+    TmCursor cursor;
+    cursor.start(a, first, min(per, pieces - first));
+
+    if (warp < 4) {
+        // sums to the rows
+        const bool with_offset = !plan.back && a.b != nullptr;
+        int buffer = 0;
+        uint32_t phase = 0;
+        for (; cursor.tile.type >= 0; cursor.next(a)) {
+            const int64_t place = cursor.tile.begin + threadIdx.x;
+            int32_t r = place < cursor.tile.end ? a.order[place] : -1;
+            if ((uint32_t)r >= (uint64_t)a.n) r = -1;
+            if (!bar_wait(&bars.sums_full[buffer], phase)) { tm_ran_out(a); break; }
+            tensor_fence_after();
+            const T* const offset = static_cast<const T*>(a.b) + (int64_t)cursor.tile.type * a.outer + col0;
+            const int have = min(plan.columns, nn - col0);
+            for (int c = 0; c < have; c += 32) {
+                uint32_t bits[32];
+                __syncwarp();
+                tensor_load_32(tensor + ((uint32_t)(warp * 32) << 16) + buffer * plan.column_stride + c, bits);
+                tensor_wait_loads();
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(bits[i]);
+                if (with_offset) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (c + i < have) v[i] += tl_get(offset + c + i);
+                }
+                if (r >= 0) tm_put_row(out + (int64_t)r * nn + col0 + c, v, have - c, plan.store);
+            }
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars.sums_free[buffer]);
+            buffer ^= 1;
+            if (buffer == 0) phase ^= 1;
+        }
+    } else if (warp == 4) {
+        // products
+        const bool bf16 = !std::is_same<T, __half>::value;
+        const uint32_t what = mma_what(bf16, plan.columns, false, false);
+        const uint32_t panel_at = smem_addr(panel), stage_at = smem_addr(stage0);
+        const int part_bytes = plan.columns * 128;
+        int stage = 0, buffer = 0, panel_type = -1;
+        uint32_t phase = 0, panel_phase = 0, sums_phase = 1;
+        bool ok = true;
+        while (ok && cursor.tile.type >= 0) {
+            if (cursor.tile.type != panel_type) {
+                if (!bar_wait(&bars.panel_full, panel_phase)) { ok = false; break; }
+                panel_phase ^= 1;
+                panel_type = cursor.tile.type;
+            }
+            if (!bar_wait(&bars.sums_free[buffer], sums_phase)) { ok = false; break; }
+            tensor_fence_after();
+            const uint32_t sums = tensor + buffer * plan.column_stride;
+            for (int chunk = 0; chunk < plan.chunks; chunk++) {
+                if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+                tensor_fence_after();
+                if (lane == 0) {
+                    const int steps = min(4, (kk - chunk * 64 + 15) / 16);
+                    const uint32_t at_a = stage_at + stage * STAGE, at_b = panel_at + chunk * PARTS * part_bytes;
+                    bool add = chunk > 0;
+                    tm_pairs<PARTS>([&](int pa, int pb) {
+                        for (int k = 0; k < steps; k++) {
+                            tensor_mma(sums, tile_descriptor(at_a + pa * (TM_ROWS * 128) + k * 32, 16, 1024),
+                                       tile_descriptor(at_b + pb * part_bytes + k * 32, 16, 1024), what, add);
+                            add = true;
+                        }
+                    });
+                    tensor_commit(&bars.empty[stage]);
+                    if (chunk == plan.chunks - 1) tensor_commit(&bars.sums_full[buffer]);
+                }
+                __syncwarp();
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            cursor.next(a);
+            if (cursor.tile.type >= 0 && cursor.tile.type != panel_type && lane == 0) tensor_commit(&bars.panel_free);
+            __syncwarp();
+            buffer ^= 1;
+            if (buffer == 0) sums_phase ^= 1;
+        }
+        if (!ok) tm_ran_out(a);
+    } else {
+        // rows and matrices to shared memory
+        const int tid = threadIdx.x - 5 * 32, piece = tid & 7;
+        int panel_type = -1, stage = 0, chunk = 0;
+        uint32_t phase = 1, free_phase = 0;
+        TlTile now = cursor.tile;
+        int32_t rows[4], rows_next[4];
+        auto rows_of = [&](const TlTile& t, int32_t (&r)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t place = t.begin + (tid >> 3) + 32 * i;
+                r[i] = t.type >= 0 && place < t.end ? a.order[place] : -1;
+                if ((uint32_t)r[i] >= (uint64_t)a.n) r[i] = -1;
+            }
+        };
+        auto fetch = [&](const int32_t (&r)[4], int ch, TmRaw<T> (&v)[4]) {
+            const int k = ch * 64 + piece * 8, have = min(8, kk - k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = tm_load(in + (r[i] >= 0 ? r[i] * in_row + k : 0), 1, r[i] >= 0 ? have : 0, plan.wide_in != 0);
+        };
+        TmRaw<T> v[4], v_next[4];
+        rows_of(now, rows);
+        if (now.type >= 0) {
+            fetch(rows, 0, v);
+            cursor.next(a);
+            rows_of(cursor.tile, rows_next);
+        }
+        while (now.type >= 0) {
+            const bool last = chunk + 1 == plan.chunks;
+            if (!last) fetch(rows, chunk + 1, v_next);
+            else if (cursor.tile.type >= 0) fetch(rows_next, 0, v_next);
+            if (now.type != panel_type) {
+                if (panel_type >= 0) {
+                    if (!bar_wait(&bars.panel_free, free_phase)) { tm_ran_out(a); break; }
+                    free_phase ^= 1;
+                }
+                panel_type = now.type;
+                const T* const w = static_cast<const T*>(a.w) + (int64_t)now.type * a.inner * a.outer;
+                const int units = plan.chunks * 8 * plan.columns;
+                for (int u = tid; u < units; u += TM_FEED_THREADS) {
+                    const int n = u % plan.columns, k8 = u / plan.columns, k = k8 * 8;
+                    const int have = col0 + n < nn ? min(8, kk - k) : 0;
+                    const T* const p = have <= 0 ? w : plan.back ? w + (int64_t)(col0 + n) * a.outer + k : w + (int64_t)k * a.outer + col0 + n;
+                    const TmRaw<T> m = tm_load(p, plan.back ? 1 : a.outer, have, plan.back && plan.wide_w != 0);
+                    tm_store(m, panel + (int64_t)(k8 / 8) * PARTS * plan.columns * 128 + tile_piece(n, k8 & 7), plan.columns * 128);
+                }
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.panel_full);
+            }
+            if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+#pragma unroll
+            for (int i = 0; i < 4; i++) tm_store(v[i], stage0 + stage * STAGE + tile_piece((tid >> 3) + 32 * i, piece), TM_ROWS * 128);
+            fence_to_tensor();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars.full[stage]);
+            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = v_next[i];
+            chunk++;
+            if (last) {
+                chunk = 0;
+                now = cursor.tile;
+#pragma unroll
+                for (int i = 0; i < 4; i++) rows[i] = rows_next[i];
+                if (now.type >= 0) {
+                    cursor.next(a);
+                    rows_of(cursor.tile, rows_next);
+                }
+            }
+        }
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (warp == 0) tensor_free(tensor, plan.tensor_columns);
+}
+
+struct TwPlan { int columns, column_stride, x_blocks, y_blocks, stages, tensor_columns, wide_x, wide_y, vec; };
+
+template <typename T>
+__global__ void __launch_bounds__(TM_THREADS, 1)
+tm_weights_kernel(const TlArgs a, const TwPlan plan)
+{
+    constexpr int PARTS = TmParts<T>::N, BLOCK = TW_ROWS * 128;
+    constexpr int UNITS = PARTS == 1 ? 6 : 4;   // pieces of 8 elements a thread and stage: 32 rows x (128 + 256 or 128) elements
+    extern __shared__ unsigned char raw_smem[];
+    __shared__ TmBars bars;
+    unsigned char* const ones = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+    unsigned char* const stage0 = ones + TM_ROWS * 128;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row0 = blockIdx.y * TM_ROWS, col0 = blockIdx.z * plan.columns;
+    const int blocks = plan.x_blocks + plan.y_blocks, stage_bytes = blocks * PARTS * BLOCK;
+    const TlTile tile = tl_tile(a, blockIdx.x, a.stretch);
+    if (tile.type < 0) return;   // the whole block
+    const int steps = (int)((tile.end - tile.begin + TW_ROWS - 1) / TW_ROWS);
+    const bool sums_wanted = blockIdx.y == 0 && a.db != nullptr;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < plan.stages; s++) {
+            bar_init(&bars.full[s], TM_FEED);
+            bar_init(&bars.empty[s], 1);
+        }
+        bar_init(&bars.sums_full[0], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const uint32_t one = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+    for (int i = threadIdx.x; i < TM_ROWS * 8; i += TM_THREADS) reinterpret_cast<uint4*>(ones)[i] = make_uint4(one, one, one, one);
+    fence_to_tensor();
+    if (warp == 0) tensor_alloc(&bars.tensor, plan.tensor_columns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = bars.tensor;
+
+    if (warp < 4) {
+        if (!bar_wait(&bars.sums_full[0], 0)) {
+            tm_ran_out(a);
+        } else {
+            tensor_fence_after();
+            const int64_t cells = (int64_t)a.inner * a.outer;
+            float* const mine = a.partial + blockIdx.x * (cells + a.outer);
+            const int m = row0 + threadIdx.x, have = min(plan.columns, a.outer - col0);
+            for (int which = 0; which < (sums_wanted ? 2 : 1); which++) {
+                float* const at = which == 0 ? mine + (int64_t)m * a.outer + col0 : mine + cells + col0;
+                const bool write = which == 0 ? m < a.inner : threadIdx.x == 0;
+                for (int c = 0; c < have; c += 32) {
+                    uint32_t bits[32];
+                    __syncwarp();
+                    tensor_load_32(tensor + ((uint32_t)(warp * 32) << 16) + which * plan.column_stride + c, bits);
+                    tensor_wait_loads();
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(bits[i]);
+                    if (write) tm_put_row(at + c, v, have - c, plan.vec);
+                }
+            }
+        }
+    } else if (warp == 4) {
+        const bool bf16 = !std::is_same<T, __half>::value;
+        const uint32_t what = mma_what(bf16, plan.columns, true, true), what_sum = mma_what(bf16, plan.columns, false, true);
+        const uint32_t stage_at = smem_addr(stage0), ones_at = smem_addr(ones);
+        const uint32_t lead = PARTS * BLOCK, lead_x = plan.x_blocks > 1 ? lead : 0;   // one block: the upper 64 rows repeat the lower
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int step = 0; step < steps; step++) {
+            if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+            tensor_fence_after();
+            if (lane == 0) {
+                const uint32_t at_x = stage_at + stage * stage_bytes, at_y = at_x + plan.x_blocks * PARTS * BLOCK;
+                bool add = step > 0;
+                tm_pairs<PARTS>([&](int pa, int pb) {
+#pragma unroll
+                    for (int k = 0; k < TW_ROWS / 16; k++) {
+                        tensor_mma(tensor, tile_descriptor(at_x + pa * BLOCK + k * 2048, lead_x, 1024), tile_descriptor(at_y + pb * BLOCK + k * 2048, lead, 1024),
+                                   what, add);
+                        add = true;
+                    }
+                });
+                if (sums_wanted) {
+                    add = step > 0;
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+                        for (int k = 0; k < TW_ROWS / 16; k++) {
+                            tensor_mma(tensor + plan.column_stride, tile_descriptor(ones_at, 16, 1024), tile_descriptor(at_y + p * BLOCK + k * 2048, lead, 1024),
+                                       what_sum, add);
+                            add = true;
+                        }
+                }
+                tensor_commit(&bars.empty[stage]);
+                if (step == steps - 1) tensor_commit(&bars.sums_full[0]);
+            }
+            __syncwarp();
+            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) tm_ran_out(a);
+    } else {
+        const int tid = threadIdx.x - 5 * 32;
+        const int per_row = blocks * 8, units = TW_ROWS * per_row;
+        // this thread's pieces are the same ones in every stage: row, place in the stage, operand, column
+        int row[UNITS], at[UNITS], col[UNITS];
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) {
+            const int u = tid + i * TM_FEED_THREADS, r = u / per_row, piece = u % per_row;
+            const int block = piece >> 3;
+            const bool of_y = block >= plan.x_blocks;
+            row[i] = u < units ? r : -1;
+            at[i] = block * PARTS * BLOCK + (int)tile_piece(r, piece & 7);
+            const int c = (of_y ? col0 + (block - plan.x_blocks) * 64 : row0 + block * 64) + (piece & 7) * 8;
+            const int limit = of_y ? min(a.outer, col0 + plan.columns) : a.inner;
+            col[i] = c < limit ? (of_y ? c | (1 << 30) : c) : -1;
+        }
+        auto rows_of = [&](int step, int32_t (&r)[UNITS]) {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const int64_t place = tile.begin + (int64_t)step * TW_ROWS + row[i];
+                r[i] = row[i] >= 0 && col[i] >= 0 && place < tile.end ? a.order[place] : -1;
+                if ((uint32_t)r[i] >= (uint64_t)a.n) r[i] = -1;
+            }
+        };
+        auto fetch = [&](const int32_t (&r)[UNITS], TmRaw<T> (&v)[UNITS]) {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const bool of_y = (col[i] >> 30) & 1;
+                const int c = col[i] & ((1 << 30) - 1);
+                const T* const p = of_y ? static_cast<const T*>(a.dy) + r[i] * a.dy_row + c : static_cast<const T*>(a.x) + r[i] * a.x_row + c;
+                v[i] = tm_load(r[i] >= 0 ? p : static_cast<const T*>(a.x), 1, r[i] >= 0 ? min(8, (of_y ? a.outer : a.inner) - c) : 0,
+                               of_y ? plan.wide_y != 0 : plan.wide_x != 0);
+            }
+        };
+        // numbers of rows two stages ahead, rows one
+        int32_t ids[UNITS];
+        TmRaw<T> v[UNITS], v_next[UNITS];
+        rows_of(0, ids);
+        fetch(ids, v);
+        rows_of(1, ids);
+        int stage = 0;
+        uint32_t phase = 1;
+        for (int step = 0; step < steps; step++) {
+            fetch(ids, v_next);   // behind the stretch: zeros
+            rows_of(step + 2, ids);
+            if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                if (row[i] >= 0) tm_store(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                v[i] = v_next[i];
+            }
+            fence_to_tensor();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars.full[stage]);
+            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+        }
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (warp == 0) tensor_free(tensor, plan.tensor_columns);
+}
+
+static int tm_round(int v, int to) { return (v + to - 1) / to * to; }
+static int tm_tensor_columns(int need)
+{
+    int c = 32;
+    while (c < need) c *= 2;
+    return c;
+}
+static bool tm_on(const void* p, int64_t row, int size, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 && row * size % bytes == 0; }
+
+template <typename T>
+static bool tm_rows(const TlArgs& a, int back, cudaStream_t s, cudaError_t* rc)
+{
+    constexpr int PARTS = TmParts<T>::N, STAGE = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(T);
+    const int kk = back ? a.outer : a.inner, nn = back ? a.inner : a.outer;
+    TmPlan p = {};
+    p.back = back;
+    p.chunks = (kk + 63) / 64;
+    // as few column tiles as leave room for the matrix beside two stages (the rows are read once for each)
+    int tiles = 1;
+    for (;; tiles++) {
+        p.columns = tm_round((nn + tiles - 1) / tiles, 16);
+        p.panel_bytes = p.chunks * PARTS * p.columns * 128;
+        if (p.columns <= 256 && p.panel_bytes + 2 * STAGE + 1024 <= TM_SMEM) break;
+        if (p.columns == 16) return false;
+    }
+    tiles = (nn + p.columns - 1) / p.columns;
+    p.panel_bytes = tm_round(p.panel_bytes, 1024);
+    p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - p.panel_bytes) / STAGE);
+    p.column_stride = tm_round(p.columns, 32);
+    p.tensor_columns = tm_tensor_columns(2 * p.column_stride);
+    const void* const in = back ? a.dy : a.x;
+    const void* const out = back ? a.dx : a.y;
+    p.wide_in = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0;
+    p.wide_w = tm_on(a.w, a.outer, SIZE, 16) && kk % 8 == 0;
+    p.store = tm_on(out, nn, SIZE, 32) && p.columns * SIZE % 32 == 0 ? 32 : tm_on(out, nn, SIZE, 16) && p.columns * SIZE % 16 == 0 ? 16 : SIZE;
+    const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
+    const int smem = 1024 + p.panel_bytes + p.stages * STAGE;
+    *rc = cudaFuncSetAttribute(tm_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (*rc != cudaSuccess) return true;
+    tm_rows_kernel<T><<<grid, TM_THREADS, smem, s>>>(a, p);
+    *rc = cudaGetLastError();
+    return true;
+}
+
+bool tl_mma_rows(const TlArgs& a, int back, int dtype, cudaStream_t s, cudaError_t* rc)
+{
+    if (dtype == DYNB_F32) return tm_rows<float>(a, back, s, rc);
+    if (dtype == DYNB_F16) return tm_rows<__half>(a, back, s, rc);
+    return tm_rows<__nv_bfloat16>(a, back, s, rc);
+}
+
+template <typename T>
+static cudaError_t tm_weights(const TlArgs& a, cudaStream_t s)
+{
+    constexpr int PARTS = TmParts<T>::N, BLOCK = TW_ROWS * 128, SIZE = (int)sizeof(T);
+    TwPlan p = {};
+    const int most = PARTS == 1 ? 256 : 128, tiles = (a.outer + most - 1) / most;
+    p.columns = tm_round((a.outer + tiles - 1) / tiles, 16);
+    p.column_stride = tm_round(p.columns, 32);
+    p.x_blocks = a.inner > 64 ? 2 : 1;
+    p.y_blocks = (p.columns + 63) / 64;
+    const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
+    p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - TM_ROWS * 128) / stage);
+    p.tensor_columns = tm_tensor_columns(2 * p.column_stride);
+    p.wide_x = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0;
+    p.wide_y = tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
+    p.vec = a.outer % 4 == 0 ? 16 : 4;
+    const dim3 grid((unsigned)tl_stretches(a.n, a.types, a.stretch), (a.inner + TM_ROWS - 1) / TM_ROWS, (a.outer + p.columns - 1) / p.columns);
+    const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;
+    const cudaError_t rc = cudaFuncSetAttribute(tm_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc != cudaSuccess) return rc;
+    tm_weights_kernel<T><<<grid, TM_THREADS, smem, s>>>(a, p);
+    return cudaGetLastError();
+}
+
+cudaError_t tl_mma_weights(const TlArgs& a, int dtype, cudaStream_t s)
+{
+    if (dtype == DYNB_F32) return tm_weights<float>(a, s);
+    if (dtype == DYNB_F16) return tm_weights<__half>(a, s);
+    return tm_weights<__nv_bfloat16>(a, s);
+}
+
+}  // namespace dynb

@@ -368,8 +368,28 @@ def type_index(types: torch.Tensor, num_types: int) -> TypeIndex:
     return TypeIndex(order, start)
 
 
+_STATUS: dict = {}   # device -> (host word, device address): set by a kernel whose bounded wait ran out
+
+
+def _status_word(dev) -> int:
+    """Device address of the device's status word (0: none yet).  Raises when an earlier call's kernel gave up waiting."""
+    found = _STATUS.get(dev.index)
+    if found is None:
+        if torch.cuda.is_current_stream_capturing():   # memory cannot be had now
+            return 0
+        hp, dp = ctypes.c_void_p(), ctypes.c_void_p()
+        _lib.check(_lib.lib().dynb_host_alloc_mapped(8, ctypes.byref(hp), ctypes.byref(dp)), "host_alloc_mapped")
+        found = _STATUS[dev.index] = (ctypes.c_uint32.from_address(hp.value), dp.value)
+        found[0].value = 0
+    if found[0].value:
+        found[0].value = 0
+        raise RuntimeError("type_linear: a wait inside a kernel of an earlier call ran out; its results are not valid")
+    return found[1]
+
+
 def _linear_args(x, weight, index: TypeIndex) -> "_lib.TypeLinear":
     a = _lib.TypeLinear()
+    a.status_dev = _status_word(x.device) or None
     a.weight_dev, a.order_dev, a.start_dev = weight.data_ptr(), index.order.data_ptr(), index.start.data_ptr()
     a.n_rows, a.types, a.inner, a.outer, a.dtype = x.size(0), weight.size(0), weight.size(1), weight.size(2), _DTYPES[x.dtype]
     return a

@@ -501,6 +501,7 @@ typedef struct dynb_type_linear_args {
     const int32_t *order_dev, *start_dev;
     int64_t n_rows;
     int32_t types, inner, outer, dtype;     /* DYNB_F32, DYNB_F16, DYNB_BF16 */
+    uint32_t* status_dev;                   /* one word, or NULL: 1 when a bounded wait inside a kernel ran out (the results are not valid) */
 } dynb_type_linear_args;
 int dynb_type_linear(const dynb_type_linear_args* args, const void* x_dev, int64_t x_row, const void* bias_dev, void* y_dev, void* stream);
 int dynb_type_linear_workspace_bytes(const dynb_type_linear_args* args, int64_t* bytes);
