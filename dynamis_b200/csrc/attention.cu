@@ -14,6 +14,8 @@ static int attn_args(const dynb_attention* in, AttnArgs* a)
     if (in->dim < 1 || in->dim > DYNB_ATTENTION_MAX_DIM) return fail_arg("neighbor_attention: dim must lie in [1, 256]");
     if (in->n_targets > 0 && (!in->rows_dev || !in->row_start_dev || !in->q_dev)) return fail_arg("null pointer");
     if (in->n_edges > 0 && (!in->src_dev || !in->k_dev || !in->v_dev)) return fail_arg("null pointer");
+    for (const int64_t row : {in->q_row, in->k_row, in->v_row})
+        if (row < 0 || row >= DYNB_ATTENTION_MAX_ROW) return fail_arg("neighbor_attention: row strides must lie in [0, 2^30)");
     *a = AttnArgs{};
     a->q = {in->q_dev, in->q_row, in->q_head};
     a->k = {in->k_dev, in->k_row, in->k_head};
@@ -67,6 +69,7 @@ extern "C" int dynb_neighbor_attention_backward(const dynb_attention* args, cons
     AttnArgs a;
     const int rc = attn_args(args, &a);
     if (rc != DYNB_OK) return rc;
+    if (d_out_row < 0 || d_out_row >= DYNB_ATTENTION_MAX_ROW) return fail_arg("neighbor_attention: row strides must lie in [0, 2^30)");
     const int size = args->dtype == DYNB_F32 ? 4 : 2;
     a.d_out = {d_out_dev, d_out_row, d_out_head};
     a.out32 = out32_dev;

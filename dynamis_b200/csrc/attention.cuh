@@ -8,95 +8,133 @@
 
 namespace dynb {
 
-// A warp works on `heads` heads of one row at a time: G lanes a head hold the head's elements in pieces of 16 bytes (NV pieces a
-// lane, piece p of lane l at element (p * G + l) * VEC), and where G * heads < 32 the rest of the warp takes further edges ("slots").
+// A warp works on `warp_heads` heads of one row at a time.  G lanes a head hold eight of its elements each, and where G * warp_heads < 32 the
+// rest of the warp takes further edges ("slots"): eight elements a lane leave few instructions for addresses, sums over lanes and exponentials
+// per edge, which is what bounds these kernels (113 warp instructions an edge and 1.48 ms with four elements a lane, 64-bit indices and checks at
+// every load, forward, 10.5 M edges of 8 x 16 fp32).
 constexpr float LOG2E = 1.4426950408889634f;
 
-template <typename T> struct Piece;
-template <> struct Piece<float> {
-    static constexpr int VEC = 4;
-    static __device__ __forceinline__ void unpack(const uint4 u, float (&f)[4])
-    {
-        f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-    }
-    static __device__ __forceinline__ uint4 pack(const float (&f)[4])
-    {
-        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-    }
-    static __device__ __forceinline__ float one(float v) { return v; }
-    static __device__ __forceinline__ float round(float v) { return v; }
-};
-template <> struct Piece<__nv_bfloat16> {
-    static constexpr int VEC = 8;
-    static __device__ __forceinline__ void unpack(const uint4 u, float (&f)[8])
-    {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const float2 c)
+{
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)),
+          "l"(*reinterpret_cast<const unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(const float2 a, const float2 b)
+{
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+// 2^x to 2 ulp; results below the smallest normal number are zero.
+__device__ __forceinline__ float pow2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Eight elements of a head as they are loaded.
+template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };
+
+template <typename T> __device__ __forceinline__ float attn_get(T v);
+template <> __device__ __forceinline__ float attn_get<float>(float v) { return v; }
+template <> __device__ __forceinline__ float attn_get<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float attn_get<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T attn_put(float v);
+template <> __device__ __forceinline__ float attn_put<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half attn_put<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 attn_put<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ void attn_pairs(const Raw<float>& r, float2 (&f)[4])
+{
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+    for (int p = 0; p < 2; p++) {
+        f[2 * p] = make_float2(__uint_as_float(r.v[p].x), __uint_as_float(r.v[p].y));
+        f[2 * p + 1] = make_float2(__uint_as_float(r.v[p].z), __uint_as_float(r.v[p].w));
     }
-    static __device__ __forceinline__ uint4 pack(const float (&f)[8])
-    {
-        uint32_t w[4];
+}
+__device__ __forceinline__ void attn_pairs(const Raw<__nv_bfloat16>& r, float2 (&f)[4])
+{
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    static __device__ __forceinline__ float one(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
-};
-template <> struct Piece<__half> {
-    static constexpr int VEC = 8;
-    static __device__ __forceinline__ void unpack(const uint4 u, float (&f)[8])
-    {
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int i = 0; i < 4; i++) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void attn_pairs(const Raw<__half>& r, float2 (&f)[4])
+{
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = v.x;
-            f[2 * i + 1] = v.y;
-        }
-    }
-    static __device__ __forceinline__ uint4 pack(const float (&f)[8])
+    for (int i = 0; i < 4; i++) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+
+// Where a lane's elements stand in their head.  Two pieces of 16 bytes in fp32, of which every second run of lanes takes the second one first:
+// eight lanes then meet eight different pieces of 128 bytes, whatever G is.  One piece in 16 bits.
+template <typename T, int G>
+struct Place {
+    static constexpr int PIECES = (int)sizeof(T) / 2, VEC = 16 / (int)sizeof(T);
+    int at[PIECES];
+    __device__ __forceinline__ Place(int part, int head)
     {
-        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const __half2 b = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
+        for (int p = 0; p < PIECES; p++) at[p] = PIECES == 1 ? part * VEC : ((p ^ ((head * G >> 2) & 1)) * G + part) * VEC;
     }
-    static __device__ __forceinline__ float one(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
 };
 
-// Elements [at, at + VEC) of a head of `dim` elements; zeros behind its end.  `wide`: every piece starts on 16 bytes and dim is a
-// multiple of VEC (the same for all lanes of a launch).
-template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T* head, int at, int dim, bool wide)
+// FULL: heads of 8 G elements whose pieces start on 16 bytes.  Otherwise `wide` says whether pieces do (and end with the head).
+template <typename T, int G, bool FULL>
+__device__ __forceinline__ Raw<T> attn_load(const T* head, const Place<T, G>& place, int dim, bool wide)
 {
-    if (wide) return at < dim ? __ldg(reinterpret_cast<const uint4*>(head + at)) : make_uint4(0, 0, 0, 0);
-    float f[Piece<T>::VEC];
+    Raw<T> r;
+    constexpr int VEC = Place<T, G>::VEC;
 #pragma unroll
-    for (int i = 0; i < Piece<T>::VEC; i++) f[i] = at + i < dim ? Piece<T>::one(head[at + i]) : 0.0f;
-    return Piece<T>::pack(f);   // exact: the values are of the type
+    for (int p = 0; p < Place<T, G>::PIECES; p++) {
+        const int at = place.at[p];
+        if (FULL) {
+            r.v[p] = __ldg(reinterpret_cast<const uint4*>(head + at));
+        } else if (wide) {
+            r.v[p] = at < dim ? __ldg(reinterpret_cast<const uint4*>(head + at)) : make_uint4(0, 0, 0, 0);
+        } else {
+            __align__(16) T e[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; i++) e[i] = at + i < dim ? head[at + i] : attn_put<T>(0.0f);
+            r.v[p] = *reinterpret_cast<const uint4*>(e);
+        }
+    }
+    return r;
 }
 template <typename T>
-__device__ __forceinline__ void store_piece(T* head, int at, int dim, bool wide, const float (&f)[Piece<T>::VEC])
+__device__ __forceinline__ Raw<T> attn_nothing()
 {
-    if (wide) {
-        if (at < dim) *reinterpret_cast<uint4*>(head + at) = Piece<T>::pack(f);
-        return;
-    }
+    Raw<T> r;
 #pragma unroll
-    for (int i = 0; i < Piece<T>::VEC; i++)
-        if (at + i < dim) head[at + i] = Piece<T>::round(f[i]);
+    for (int p = 0; p < (int)(sizeof(T) / 2); p++) r.v[p] = make_uint4(0, 0, 0, 0);
+    return r;
+}
+// f holds the pieces in the lane's order: pairs 0, 1 of piece 0, then of piece 1 (fp32), or the four pairs of the one piece.
+template <typename T, int G, bool FULL>
+__device__ __forceinline__ void attn_store(T* head, const Place<T, G>& place, int dim, bool wide, const float2 (&f)[4])
+{
+    constexpr int VEC = Place<T, G>::VEC;
+#pragma unroll
+    for (int p = 0; p < Place<T, G>::PIECES; p++) {
+        const int at = place.at[p];
+        __align__(16) T e[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            e[i] = attn_put<T>(f[(p * VEC + i) / 2].x);
+            e[i + 1] = attn_put<T>(f[(p * VEC + i) / 2].y);
+        }
+        if (FULL || wide) {
+            if (FULL || at < dim) *reinterpret_cast<uint4*>(head + at) = *reinterpret_cast<const uint4*>(e);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i++)
+                if (at + i < dim) head[at + i] = e[i];
+        }
+    }
 }
 
 template <int G>
@@ -106,6 +144,30 @@ __device__ __forceinline__ float head_sum(float v)
     for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+__device__ __forceinline__ float dot8(const float2 (&a)[4], const float2 (&b)[4])
+{
+    float2 s = mul2(a[0], b[0]);
+#pragma unroll
+    for (int i = 1; i < 4; i++) s = fma2(a[i], b[i], s);
+    return s.x + s.y;
+}
+
+// Sources and biases of the edges [e, e + BATCH) of a slot, asked for a batch before the rows they name.
+template <int BATCH>
+struct AttnEdges {
+    int32_t s[BATCH];
+    float z[BATCH];
+    __device__ __forceinline__ void fetch(const int32_t* src, const float* bias, int e, int n, int heads)
+    {
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            s[u] = e + u < n ? __ldg(src + e + u) : -1;
+            z[u] = 0.0f;
+            if (bias != nullptr && e + u < n) z[u] = __ldg(bias + (int64_t)(e + u) * heads);
+        }
+    }
+    __device__ __forceinline__ bool live(int u, uint32_t sources) const { return (uint32_t)s[u] < sources && z[u] != -INFINITY; }
+};
 
 struct AttnRows { const void* at; int64_t row, head; };   // strides in elements, the elements of a head are consecutive
 
@@ -128,27 +190,32 @@ cudaError_t attn_forward(const AttnArgs& a, int dtype, cudaStream_t s);
 cudaError_t attn_backward_rows(const AttnArgs& a, int dtype, cudaStream_t s);
 cudaError_t attn_backward_cols(const AttnArgs& a, int dtype, cudaStream_t s);
 
-// Lanes a head and pieces a lane for a head of `dim` elements of type T.
-static inline int attn_lanes(int dim, int vec)
+// Lanes a head.
+static inline int attn_lanes(int dim)
 {
     int g = 1;
-    while (g < 32 && g * vec < dim) g *= 2;
+    while (g * 8 < dim) g *= 2;
     return g;
 }
 
-template <typename T, template <typename, int, int> class Launch>
+template <typename T, template <typename, int, bool> class Launch, int G>
+static inline cudaError_t attn_by_full(const AttnArgs& a, cudaStream_t s)
+{
+    return a.wide && a.dim == 8 * G ? Launch<T, G, true>::go(a, s) : Launch<T, G, false>::go(a, s);
+}
+template <typename T, template <typename, int, bool> class Launch>
 static inline cudaError_t attn_by_dim(const AttnArgs& a, cudaStream_t s)
 {
-    switch (attn_lanes(a.dim, Piece<T>::VEC)) {
-    case 1: return Launch<T, 1, 1>::go(a, s);
-    case 2: return Launch<T, 2, 1>::go(a, s);
-    case 4: return Launch<T, 4, 1>::go(a, s);
-    case 8: return Launch<T, 8, 1>::go(a, s);
-    case 16: return Launch<T, 16, 1>::go(a, s);
-    default: return a.dim <= 32 * Piece<T>::VEC ? Launch<T, 32, 1>::go(a, s) : Launch<T, 32, 2>::go(a, s);
+    switch (attn_lanes(a.dim)) {
+    case 1: return attn_by_full<T, Launch, 1>(a, s);
+    case 2: return attn_by_full<T, Launch, 2>(a, s);
+    case 4: return attn_by_full<T, Launch, 4>(a, s);
+    case 8: return attn_by_full<T, Launch, 8>(a, s);
+    case 16: return attn_by_full<T, Launch, 16>(a, s);
+    default: return attn_by_full<T, Launch, 32>(a, s);
     }
 }
-template <template <typename, int, int> class Launch>
+template <template <typename, int, bool> class Launch>
 static inline cudaError_t attn_by_type(const AttnArgs& a, int dtype, cudaStream_t s)
 {
     if (dtype == DYNB_F32) return attn_by_dim<float, Launch>(a, s);
@@ -163,5 +230,8 @@ static inline int attn_warp_heads(int heads, int g)
     while (h < heads && h * g < 32) h *= 2;
     return h;
 }
+
+// Whether four warps share a row: where there are too few rows for the SMs (148 x 16 warps), or the lists are long.
+static inline bool attn_split(int64_t warps, int64_t edges) { return warps < 148 * 16 || edges > warps * 512; }
 
 }  // namespace dynb

@@ -4,143 +4,181 @@
 // One pass over the edges with the running maximum and sum of the softmax.  Sums, maxima and probabilities are in 32 bits; the
 // result is rounded once.
 
+#include <algorithm>
+
 #include "attention.cuh"
 
 namespace dynb {
 
-constexpr int AF_WARPS = 4;
+constexpr int AF_WARPS = 8;
 constexpr int AF_BATCH = 4;   // edges of a slot in flight
 
-template <typename T, int G, int NV>
+// WPR warps take turns at the batches of a row and join through shared memory.
+template <typename T, int G, bool FULL, int WPR>
 __global__ void __launch_bounds__(AF_WARPS * 32)
 attn_forward_kernel(const AttnArgs a)
 {
-    constexpr int VEC = Piece<T>::VEC;
-    const int lane = threadIdx.x & 31;
-    const int64_t r = (int64_t)blockIdx.x * AF_WARPS + (threadIdx.x >> 5);
-    if (r >= a.n_targets) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = lane % G, slots = 32 / (G * a.warp_heads), slot = lane / (G * a.warp_heads);
     const int head = blockIdx.y * a.warp_heads + (lane / G) % a.warp_heads;
-    const bool live = head < a.heads;
-    const int h = live ? head : 0, kv = h / a.shared;
-    const int32_t t = a.rows[r];
-    if ((uint32_t)t >= (uint64_t)a.n_targets) return;
-    const int64_t begin = max(a.row_start[r], 0), end = min((int64_t)a.row_start[r + 1], a.n_edges);
-    const bool wide = a.wide != 0;
+    const bool mine = head < a.heads, wide = a.wide != 0;
+    const int h = mine ? head : 0, kv = h / a.shared;
+    const Place<T, G> place(part, h);
+    const uint32_t sources = (uint32_t)a.n_sources;
+    const uint32_t k_step = (uint32_t)(a.k.row * (int)sizeof(T)), v_step = (uint32_t)(a.v.row * (int)sizeof(T));
+    const char* const kb = reinterpret_cast<const char*>(static_cast<const T*>(a.k.at) + kv * a.k.head);
+    const char* const vb = reinterpret_cast<const char*>(static_cast<const T*>(a.v.at) + kv * a.v.head);
+    constexpr int ROWS = AF_WARPS / WPR;
+    const int turn = warp % WPR, step = AF_BATCH * slots;
 
-    float q[NV][VEC], acc[NV][VEC];
-#pragma unroll
-    for (int p = 0; p < NV; p++) {
-        Piece<T>::unpack(load_piece(static_cast<const T*>(a.q.at) + t * a.q.row + h * a.q.head, (p * G + part) * VEC, a.dim, wide), q[p]);
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            q[p][i] *= a.scale;
-            acc[p][i] = 0.0f;
+    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n_targets; r0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t r = r0 + warp / WPR;
+        int32_t t = r < a.n_targets ? a.rows[r] : -1;
+        if ((uint32_t)t >= (uint32_t)a.n_targets) t = -1;
+        if (WPR == 1 && t < 0) continue;
+        int64_t begin = 0, end = 0;
+        if (t >= 0) {
+            begin = max(a.row_start[r], 0);
+            end = min((int64_t)a.row_start[r + 1], a.n_edges);
         }
-    }
-    float top = -INFINITY, sum = 0.0f;
-    const T* const kb = static_cast<const T*>(a.k.at) + kv * a.k.head;
-    const T* const vb = static_cast<const T*>(a.v.at) + kv * a.v.head;
-    for (int64_t base = begin; base < end; base += AF_BATCH * slots) {
-        uint4 ku[AF_BATCH][NV], vu[AF_BATCH][NV];
-        float z[AF_BATCH];
+        const int n = (int)max(end - begin, (int64_t)0);
+        const int32_t* const src = a.src + begin;
+        const float* const bias = a.bias != nullptr ? a.bias + begin * a.heads + h : nullptr;
+
+        float2 q[4], acc[4];
+        if (t >= 0) attn_pairs(attn_load<T, G, FULL>(static_cast<const T*>(a.q.at) + t * a.q.row + h * a.q.head, place, a.dim, wide), q);
+        else attn_pairs(attn_nothing<T>(), q);
 #pragma unroll
-        for (int u = 0; u < AF_BATCH; u++) {
-            const int64_t e = base + u * slots + slot;
-            const int32_t s = e < end ? a.src[e] : -1;
-            const bool ok = (uint32_t)s < (uint64_t)a.n_sources;
-            z[u] = !ok ? -INFINITY : a.bias != nullptr ? a.bias[e * a.heads + h] : 0.0f;
-            const int64_t at = ok ? s : 0;
+        for (int i = 0; i < 4; i++) {
+            q[i] = mul2(q[i], make_float2(a.scale, a.scale));
+            acc[i] = make_float2(0.0f, 0.0f);
+        }
+        float top = -INFINITY, sum = 0.0f;
+        int e = turn * step + slot * AF_BATCH;
+        AttnEdges<AF_BATCH> now;
+        now.fetch(src, bias, e, n, a.heads);
+        for (int base = turn * step; base < n; base += WPR * step) {
+            Raw<T> ku[AF_BATCH], vu[AF_BATCH];
+            float z[AF_BATCH];
 #pragma unroll
-            for (int p = 0; p < NV; p++) {
-                ku[u][p] = ok ? load_piece(kb + at * a.k.row, (p * G + part) * VEC, a.dim, wide) : make_uint4(0, 0, 0, 0);
-                vu[u][p] = ok ? load_piece(vb + at * a.v.row, (p * G + part) * VEC, a.dim, wide) : make_uint4(0, 0, 0, 0);
+            for (int u = 0; u < AF_BATCH; u++) {
+                const bool ok = now.live(u, sources);
+                ku[u] = attn_nothing<T>();
+                vu[u] = attn_nothing<T>();   // masked: not even a product with what its rows hold
+                if (ok) {
+                    ku[u] = attn_load<T, G, FULL>(reinterpret_cast<const T*>(kb + (uint64_t)(uint32_t)now.s[u] * k_step), place, a.dim, wide);
+                    vu[u] = attn_load<T, G, FULL>(reinterpret_cast<const T*>(vb + (uint64_t)(uint32_t)now.s[u] * v_step), place, a.dim, wide);
+                }
+                z[u] = ok ? now.z[u] : -INFINITY;
             }
-        }
-        float most = top;
+            e += WPR * step;
+            now.fetch(src, bias, e, n, a.heads);
+            float most = top;
 #pragma unroll
-        for (int u = 0; u < AF_BATCH; u++) {
-            float dot = 0.0f;
-#pragma unroll
-            for (int p = 0; p < NV; p++) {
-                float f[VEC];
-                Piece<T>::unpack(ku[u][p], f);
-#pragma unroll
-                for (int i = 0; i < VEC; i++) dot = fmaf(q[p][i], f[i], dot);
+            for (int u = 0; u < AF_BATCH; u++) {
+                float2 f[4];
+                attn_pairs(ku[u], f);
+                z[u] += head_sum<G>(dot8(q, f));
+                most = fmaxf(most, z[u]);
             }
-            dot = head_sum<G>(dot);
-            if (z[u] != -INFINITY) z[u] += dot;
-            most = fmaxf(most, z[u]);
-        }
-        // NaN logits must not vanish in the maximum: they reach the sums through their own exponentials
-        if (most != -INFINITY) {
-            const float turn = exp2f((top - most) * LOG2E);
+            // NaN logits are not in the maximum: they reach the sums through their own exponentials
+            const float from = most == -INFINITY ? 0.0f : most, back = pow2((top - from) * LOG2E);
             top = most;
-            sum *= turn;
+            sum *= back;
 #pragma unroll
-            for (int p = 0; p < NV; p++)
+            for (int i = 0; i < 4; i++) acc[i] = mul2(acc[i], make_float2(back, back));
 #pragma unroll
-                for (int i = 0; i < VEC; i++) acc[p][i] *= turn;
-        }
+            for (int u = 0; u < AF_BATCH; u++) {
+                const float w = pow2((z[u] - from) * LOG2E);
+                sum += w;
+                float2 f[4];
+                attn_pairs(vu[u], f);
 #pragma unroll
-        for (int u = 0; u < AF_BATCH; u++) {
-            if (z[u] == -INFINITY) continue;   // masked: not even a product with what its rows hold
-            const float w = exp2f((z[u] - top) * LOG2E);
-            sum += w;
-#pragma unroll
-            for (int p = 0; p < NV; p++) {
-                float f[VEC];
-                Piece<T>::unpack(vu[u][p], f);
-#pragma unroll
-                for (int i = 0; i < VEC; i++) acc[p][i] = fmaf(w, f[i], acc[p][i]);
+                for (int i = 0; i < 4; i++) acc[i] = fma2(make_float2(w, w), f[i], acc[i]);
             }
         }
-    }
-    // the slots of the warp join
-    for (int o = G * a.warp_heads; o < 32; o <<= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, top, o);
-        const float most = fmaxf(top, other);
-        const float turn = most == -INFINITY ? 1.0f : exp2f((top - most) * LOG2E);
-        top = most;
-        sum *= turn;
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        // the slots of the warp join
+        for (int o = G * a.warp_heads; o < 32; o <<= 1) {
+            const float most = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float back = most == -INFINITY ? 1.0f : pow2((top - most) * LOG2E);
+            top = most;
+            sum *= back;
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
-        for (int p = 0; p < NV; p++)
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                acc[p][i] *= turn;
-                acc[p][i] += __shfl_xor_sync(0xffffffffu, acc[p][i], o);
+            for (int i = 0; i < 4; i++) {
+                acc[i].x *= back;
+                acc[i].y *= back;
+                acc[i].x += __shfl_xor_sync(0xffffffffu, acc[i].x, o);
+                acc[i].y += __shfl_xor_sync(0xffffffffu, acc[i].y, o);
             }
-    }
-    if (!live || slot != 0) return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t at = ((int64_t)t * a.heads + head) * a.dim;
-#pragma unroll
-    for (int p = 0; p < NV; p++) {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) acc[p][i] *= inv;
-        const int d = (p * G + part) * VEC;
-        store_piece(static_cast<T*>(a.out) + at, d, a.dim, wide, acc[p]);
-        if (a.out32_w != nullptr) {
-#pragma unroll
-            for (int i = 0; i < VEC; i++)
-                if (d + i < a.dim) a.out32_w[at + d + i] = acc[p][i];
         }
-    }
-    if (a.stats_w != nullptr && part == 0) {
-        a.stats_w[(int64_t)t * 2 * a.heads + head] = top;
-        a.stats_w[(int64_t)t * 2 * a.heads + a.heads + head] = inv;
+        if (WPR > 1) {   // the warps of the row join in their order
+            __shared__ float joint[AF_WARPS][10][32];
+            __syncthreads();
+            joint[warp][8][lane] = top;
+            joint[warp][9][lane] = sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                joint[warp][2 * i][lane] = acc[i].x;
+                joint[warp][2 * i + 1][lane] = acc[i].y;
+            }
+            __syncthreads();
+            if (turn != 0) continue;
+            float most = top;
+#pragma unroll
+            for (int w = 1; w < WPR; w++) most = fmaxf(most, joint[warp + w][8][lane]);
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < WPR; w++) {
+                const float back = most == -INFINITY ? 1.0f : pow2((joint[warp + w][8][lane] - most) * LOG2E);
+                sum = fmaf(joint[warp + w][9][lane], back, sum);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    acc[i].x = fmaf(joint[warp + w][2 * i][lane], back, acc[i].x);
+                    acc[i].y = fmaf(joint[warp + w][2 * i + 1][lane], back, acc[i].y);
+                }
+            }
+            top = most;
+        }
+        if (!mine || slot != 0 || t < 0) continue;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t at = ((int64_t)t * a.heads + head) * a.dim;
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = mul2(acc[i], make_float2(inv, inv));
+        attn_store<T, G, FULL>(static_cast<T*>(a.out) + at, place, a.dim, wide, acc);
+        if (sizeof(T) != 4 && a.out32_w != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d = place.at[0] + 2 * i;
+                if (FULL) {
+                    *reinterpret_cast<float2*>(a.out32_w + at + d) = acc[i];
+                } else {
+                    if (d < a.dim) a.out32_w[at + d] = acc[i].x;
+                    if (d + 1 < a.dim) a.out32_w[at + d + 1] = acc[i].y;
+                }
+            }
+        }
+        if (a.stats_w != nullptr && part == 0) {
+            a.stats_w[(int64_t)t * 2 * a.heads + head] = top;
+            a.stats_w[(int64_t)t * 2 * a.heads + a.heads + head] = inv;
+        }
     }
 }
 
-template <typename T, int G, int NV>
+template <typename T, int G, bool FULL>
 struct AttnForward {
     static cudaError_t go(const AttnArgs& args, cudaStream_t s)
     {
         AttnArgs a = args;
         a.warp_heads = attn_warp_heads(a.heads, G);
-        const dim3 grid((unsigned)((a.n_targets + AF_WARPS - 1) / AF_WARPS), (a.heads + a.warp_heads - 1) / a.warp_heads);
-        attn_forward_kernel<T, G, NV><<<grid, AF_WARPS * 32, 0, s>>>(a);
+        const int blocks = (a.heads + a.warp_heads - 1) / a.warp_heads;
+        const bool split = attn_split(a.n_targets * blocks, a.n_edges * blocks);
+        const int rows = split ? AF_WARPS / 4 : AF_WARPS;
+        const dim3 grid((unsigned)((a.n_targets + rows - 1) / rows), blocks);
+        if (split) attn_forward_kernel<T, G, FULL, 4><<<grid, AF_WARPS * 32, 0, s>>>(a);
+        else attn_forward_kernel<T, G, FULL, 1><<<grid, AF_WARPS * 32, 0, s>>>(a);
         return cudaGetLastError();
     }
 };

@@ -32,6 +32,7 @@ from .partition import scratch
 
 _DTYPES = {torch.float32: _lib.DYNB_F32, torch.float16: _lib.DYNB_F16, torch.bfloat16: _lib.DYNB_BF16}
 MAX_DIM = 256            # DYNB_ATTENTION_MAX_DIM
+MAX_ROW = 1 << 30        # DYNB_ATTENTION_MAX_ROW
 MAX_BUCKETS = 1024       # DYNB_DISTANCE_BIAS_MAX_BUCKETS
 MAX_BIAS_HEADS = 1024    # DYNB_DISTANCE_BIAS_MAX_HEADS
 MAX_TYPES = 4096         # DYNB_TYPE_LINEAR_MAX_TYPES
@@ -165,8 +166,8 @@ def neighbor_index(edge_index: torch.Tensor, num_targets: int, num_sources: int)
 
 
 def _heads_last(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as the kernels read it: any strides of rows and heads, the elements of a head consecutive."""
-    return t if t.stride(2) == 1 or t.size(2) == 1 else t.contiguous()
+    """``t`` as the kernels read it: any strides of rows (below 2^30 elements) and heads, the elements of a head consecutive."""
+    return t if (t.stride(2) == 1 or t.size(2) == 1) and t.stride(0) < MAX_ROW else t.contiguous()
 
 
 def _pointer(t: Optional[torch.Tensor]):

@@ -456,6 +456,7 @@ int dynb_neighbor_index_fill(const int64_t* dst_dev, int64_t n_edges, int64_t n_
  * the target, out[dst] = sum p_e v[src].  Query head h reads key and value head h / (heads / kv_heads).  Edges with a bias of -inf take
  * no part; a target without edges that do gives zeros.  Strides are in elements, a head's elements are consecutive; out is contiguous. */
 #define DYNB_ATTENTION_MAX_DIM 256
+#define DYNB_ATTENTION_MAX_ROW (1ll << 30)   /* strides of rows, in elements */
 typedef struct dynb_attention {
     const void *q_dev, *k_dev, *v_dev;      /* [n_targets, heads, dim], [n_sources, kv_heads, dim] twice, of `dtype` */
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
