@@ -1,5 +1,7 @@
 // C entry points of neighbour attention: checks of the arguments, then the kernels of attention_forward.cu and attention_backward.cu.
 
+#include <initializer_list>
+
 #include "attention.cuh"
 
 namespace dynb {
@@ -9,7 +11,7 @@ static int attn_args(const dynb_attention* in, AttnArgs* a)
     if (in == nullptr) return fail_arg("null pointer");
     if (in->dtype != DYNB_F32 && in->dtype != DYNB_F16 && in->dtype != DYNB_BF16) return fail_arg("neighbor_attention: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
     if (in->n_targets < 0 || in->n_sources < 0 || in->n_edges < 0) return fail_arg("neighbor_attention: sizes must be non-negative");
-    if (in->n_targets >= INT32_MAX || in->n_sources >= INT32_MAX || in->n_edges >= INT32_MAX) return fail_arg("neighbor_attention: sizes must be below 2^31 - 1");
+    if (in->n_targets >= INT32_MAX || in->n_sources >= INT32_MAX || in->n_edges >= DYNB_MAX_EDGES) return fail_arg("neighbor_attention: sizes must be below 2^31 - 1, edges below 2^31 - 2^16");
     if (in->heads < 1 || in->kv_heads < 1 || in->heads % in->kv_heads != 0 || in->heads > 65535) return fail_arg("neighbor_attention: heads must be a multiple of kv_heads");
     if (in->dim < 1 || in->dim > DYNB_ATTENTION_MAX_DIM) return fail_arg("neighbor_attention: dim must lie in [1, 256]");
     if (in->n_targets > 0 && (!in->rows_dev || !in->row_start_dev || !in->q_dev)) return fail_arg("null pointer");
@@ -35,10 +37,16 @@ static int attn_args(const dynb_attention* in, AttnArgs* a)
     return DYNB_OK;
 }
 
-// Whether every piece of 16 bytes of a head starts on 16 bytes.
-static bool attn_wide(const AttnRows& r, int size)
+// Whether the rows of a tensor lie in 64 GB.
+static bool attn_narrow(const AttnRows& r, int64_t rows, int heads, int size) { return (rows * r.row + heads * r.head) * size / 16 < (1ll << 32); }
+
+// Bytes on which the heads of all these tensors start and end.
+static int attn_wide(int dim, int size, std::initializer_list<AttnRows> all, std::initializer_list<const void*> outputs)
 {
-    return reinterpret_cast<uintptr_t>(r.at) % 16 == 0 && r.row * size % 16 == 0 && r.head * size % 16 == 0;
+    uint64_t bits = (uint64_t)dim * size;
+    for (const AttnRows& r : all) bits |= reinterpret_cast<uintptr_t>(r.at) | (uint64_t)r.row * size | (uint64_t)r.head * size;
+    for (const void* p : outputs) bits |= reinterpret_cast<uintptr_t>(p);
+    return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : size;
 }
 
 }  // namespace dynb
@@ -56,7 +64,8 @@ extern "C" int dynb_neighbor_attention(const dynb_attention* args, void* out_dev
     a.out = out_dev;
     a.out32_w = out32_dev;
     a.stats_w = stats_dev;
-    a.wide = a.dim * size % 16 == 0 && attn_wide(a.q, size) && attn_wide(a.k, size) && attn_wide(a.v, size) && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0;
+    a.wide = attn_wide(a.dim, size, {a.q, a.k, a.v}, {out_dev});
+    a.narrow = attn_narrow(a.k, a.n_sources, a.kv_heads, size) && attn_narrow(a.v, a.n_sources, a.kv_heads, size);
     DYNB_CUDA_OK(attn_forward(a, args->dtype, static_cast<cudaStream_t>(stream)));
     return DYNB_OK;
 }
@@ -74,7 +83,7 @@ extern "C" int dynb_neighbor_attention_backward(const dynb_attention* args, cons
     a.d_out = {d_out_dev, d_out_row, d_out_head};
     a.out32 = out32_dev;
     a.stats = stats_dev;
-    a.delta = delta_dev;
+    a.delta = static_cast<float4*>(static_cast<void*>(delta_dev));
     a.cols = cols_dev;
     a.col_start = col_start_dev;
     a.in_edge = in_edge_dev;
@@ -84,8 +93,9 @@ extern "C" int dynb_neighbor_attention_backward(const dynb_attention* args, cons
     a.dv = dv_dev;
     a.d_bias = d_bias_dev;
     if (d_bias_dev != nullptr && a.bias == nullptr) return fail_arg("neighbor_attention_backward: a gradient of a bias that is not there");
-    a.wide = a.dim * size % 16 == 0 && attn_wide(a.q, size) && attn_wide(a.k, size) && attn_wide(a.v, size) && attn_wide(a.d_out, size);
-    for (const void* p : {(const void*)dq_dev, (const void*)dk_dev, (const void*)dv_dev}) a.wide = a.wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    a.wide = attn_wide(a.dim, size, {a.q, a.k, a.v, a.d_out}, {dq_dev, dk_dev, dv_dev});
+    a.narrow = attn_narrow(a.k, a.n_sources, a.kv_heads, size) && attn_narrow(a.v, a.n_sources, a.kv_heads, size) &&
+               attn_narrow(a.q, a.n_targets, a.heads, size) && attn_narrow(a.d_out, a.n_targets, a.heads, size);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool cols = (dk_dev != nullptr || dv_dev != nullptr) && a.n_sources > 0;
     if (a.n_targets > 0) {   // also for the sources' gradients, which read delta

@@ -8,10 +8,9 @@
 
 namespace dynb {
 
-// A warp works on `warp_heads` heads of one row at a time.  G lanes a head hold eight of its elements each, and where G * warp_heads < 32 the
-// rest of the warp takes further edges ("slots"): eight elements a lane leave few instructions for addresses, sums over lanes and exponentials
-// per edge, which is what bounds these kernels (113 warp instructions an edge and 1.48 ms with four elements a lane, 64-bit indices and checks at
-// every load, forward, 10.5 M edges of 8 x 16 fp32).
+// A warp works on `warp_heads` heads of one row at a time.  G lanes a head hold 32 bytes of it each, and where G * warp_heads < 32 the rest of the
+// warp takes further edges ("slots"): 32 bytes a lane leave few instructions an edge for addresses, sums over lanes and exponentials (113 warp
+// instructions an edge and 1.48 ms with 16 bytes a lane, 64-bit indices and checks at every load; forward, 10.5 M edges of 8 x 16 fp32).
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const float2 c)
@@ -37,65 +36,65 @@ __device__ __forceinline__ float pow2(float x)
     return y;
 }
 
-// Eight elements of a head as they are loaded.
-template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };
+struct AttnRows { const void* at; int64_t row, head; };   // strides in elements, the elements of a head are consecutive
 
-template <typename T> __device__ __forceinline__ float attn_get(T v);
-template <> __device__ __forceinline__ float attn_get<float>(float v) { return v; }
-template <> __device__ __forceinline__ float attn_get<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float attn_get<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+// EL elements of a head (8 or 16) as they are loaded: pieces of 16 bytes.
+template <typename T, int EL> struct Raw { uint4 v[EL * (int)sizeof(T) / 16]; };
+
 template <typename T> __device__ __forceinline__ T attn_put(float v);
 template <> __device__ __forceinline__ float attn_put<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half attn_put<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 attn_put<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ void attn_pairs(const Raw<float>& r, float2 (&f)[4])
+__device__ __forceinline__ float2 attn_pair(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 attn_pair(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T, int EL>
+__device__ __forceinline__ void attn_pairs(const Raw<T, EL>& r, float2 (&f)[EL / 2])
 {
 #pragma unroll
-    for (int p = 0; p < 2; p++) {
-        f[2 * p] = make_float2(__uint_as_float(r.v[p].x), __uint_as_float(r.v[p].y));
-        f[2 * p + 1] = make_float2(__uint_as_float(r.v[p].z), __uint_as_float(r.v[p].w));
+    for (int p = 0; p < EL * (int)sizeof(T) / 16; p++) {
+        const uint32_t w[4] = {r.v[p].x, r.v[p].y, r.v[p].z, r.v[p].w};
+        if constexpr (sizeof(T) == 4) {
+            f[2 * p] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+            f[2 * p + 1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) f[4 * p + i] = attn_pair(w[i], T());
+        }
     }
 }
-__device__ __forceinline__ void attn_pairs(const Raw<__nv_bfloat16>& r, float2 (&f)[4])
-{
-    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-}
-__device__ __forceinline__ void attn_pairs(const Raw<__half>& r, float2 (&f)[4])
-{
-    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-}
 
-// Where a lane's elements stand in their head.  Two pieces of 16 bytes in fp32, of which every second run of lanes takes the second one first:
-// eight lanes then meet eight different pieces of 128 bytes, whatever G is.  One piece in 16 bits.
-template <typename T, int G>
+// Where a lane's pieces stand in their head: piece p of the lane is number (p ^ turn) G + part of the head.  The turn depends on the
+// head so that eight lanes, which are served at once, meet eight different pieces of 128 bytes.
+template <typename T, int G, int EL>
 struct Place {
-    static constexpr int PIECES = (int)sizeof(T) / 2, VEC = 16 / (int)sizeof(T);
+    static constexpr int PIECES = EL * (int)sizeof(T) / 16, VEC = 16 / (int)sizeof(T);
     int at[PIECES];
     __device__ __forceinline__ Place(int part, int head)
     {
+        const int turn = (G * PIECES < 8 ? head * (G * PIECES) >> 3 : head) & (PIECES - 1);
 #pragma unroll
-        for (int p = 0; p < PIECES; p++) at[p] = PIECES == 1 ? part * VEC : ((p ^ ((head * G >> 2) & 1)) * G + part) * VEC;
+        for (int p = 0; p < PIECES; p++) at[p] = ((p ^ turn) * G + part) * VEC;
     }
 };
 
-// FULL: heads of 8 G elements whose pieces start on 16 bytes.  Otherwise `wide` says whether pieces do (and end with the head).
-template <typename T, int G, bool FULL>
-__device__ __forceinline__ Raw<T> attn_load(const T* head, const Place<T, G>& place, int dim, bool wide)
+// FULL: heads of EL G elements whose pieces start on 16 bytes.  Otherwise `wide` says on how many bytes (16, 8 or fewer) heads start and end.
+template <typename T, int G, int EL, bool FULL>
+__device__ __forceinline__ Raw<T, EL> attn_load(const T* head, const Place<T, G, EL>& place, int dim, int wide)
 {
-    Raw<T> r;
-    constexpr int VEC = Place<T, G>::VEC;
+    Raw<T, EL> r;
+    constexpr int VEC = Place<T, G, EL>::VEC;
 #pragma unroll
-    for (int p = 0; p < Place<T, G>::PIECES; p++) {
+    for (int p = 0; p < Place<T, G, EL>::PIECES; p++) {
         const int at = place.at[p];
         if (FULL) {
             r.v[p] = __ldg(reinterpret_cast<const uint4*>(head + at));
-        } else if (wide) {
+        } else if (wide == 16) {
             r.v[p] = at < dim ? __ldg(reinterpret_cast<const uint4*>(head + at)) : make_uint4(0, 0, 0, 0);
+        } else if (wide == 8) {
+            const uint2 lo = at < dim ? __ldg(reinterpret_cast<const uint2*>(head + at)) : make_uint2(0, 0);
+            const uint2 hi = at + VEC / 2 < dim ? __ldg(reinterpret_cast<const uint2*>(head + at + VEC / 2)) : make_uint2(0, 0);
+            r.v[p] = make_uint4(lo.x, lo.y, hi.x, hi.y);
         } else {
             __align__(16) T e[VEC];
 #pragma unroll
@@ -105,21 +104,83 @@ __device__ __forceinline__ Raw<T> attn_load(const T* head, const Place<T, G>& pl
     }
     return r;
 }
-template <typename T>
-__device__ __forceinline__ Raw<T> attn_nothing()
-{
-    Raw<T> r;
+// Rows of full heads: a lane's pieces in units of 16 bytes from the tensor's start, in 32 bits (64 GB): one addition a piece, where a 64-bit
+// pointer per piece took two and a zero row for masked edges four more selections.
+template <typename T, int G, int EL>
+struct Lane {
+    static constexpr int PIECES = Place<T, G, EL>::PIECES;
+    const uint4* base;
+    uint32_t step, at[PIECES];
+    __device__ __forceinline__ Lane(const AttnRows& rows, int head, const Place<T, G, EL>& place)
+    {
+        base = static_cast<const uint4*>(rows.at);
+        step = (uint32_t)(rows.row * (int)sizeof(T) / 16);
 #pragma unroll
-    for (int p = 0; p < (int)(sizeof(T) / 2); p++) r.v[p] = make_uint4(0, 0, 0, 0);
-    return r;
+        for (int p = 0; p < PIECES; p++) at[p] = (uint32_t)((rows.head * head + place.at[p]) * (int)sizeof(T) / 16);
+    }
+    __device__ __forceinline__ Raw<T, EL> load(uint32_t row) const
+    {
+        Raw<T, EL> r;
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) r.v[p] = __ldg(base + (row * step + at[p]));
+        return r;
+    }
+};
+template <typename T, int EL>
+__device__ __forceinline__ void attn_clear(Raw<T, EL>& r, bool keep)
+{
+#pragma unroll
+    for (int p = 0; p < EL * (int)sizeof(T) / 16; p++) {
+        r.v[p].x = keep ? r.v[p].x : 0u;
+        r.v[p].y = keep ? r.v[p].y : 0u;
+        r.v[p].z = keep ? r.v[p].z : 0u;
+        r.v[p].w = keep ? r.v[p].w : 0u;
+    }
 }
-// f holds the pieces in the lane's order: pairs 0, 1 of piece 0, then of piece 1 (fp32), or the four pairs of the one piece.
-template <typename T, int G, bool FULL>
-__device__ __forceinline__ void attn_store(T* head, const Place<T, G>& place, int dim, bool wide, const float2 (&f)[4])
-{
-    constexpr int VEC = Place<T, G>::VEC;
+// A batch of edges on its way: what they read from two tensors, their biases, and whether they take part.  (The loads of those that do not go to
+// row 0, which is there: an edge has both ends.)
+template <typename T, int EL, int BATCH>
+struct AttnStep {
+    Raw<T, EL> x[BATCH], y[BATCH];
+    float z[BATCH];
+    bool ok[BATCH];
+
+    template <int G, bool FULL>
+    __device__ __forceinline__ void load(const Lane<T, G, EL>& a, const Lane<T, G, EL>& b, const Place<T, G, EL>& place, const AttnRows& ar, const AttnRows& br,
+                                         int head_a, int head_b, const uint32_t (&row)[BATCH], int dim, int wide)
+    {
 #pragma unroll
-    for (int p = 0; p < Place<T, G>::PIECES; p++) {
+        for (int u = 0; u < BATCH; u++) {
+            if constexpr (FULL) {
+                x[u] = a.load(row[u]);
+                y[u] = b.load(row[u]);
+            } else if (ok[u]) {
+                x[u] = attn_load<T, G, EL, false>(static_cast<const T*>(ar.at) + (row[u] * ar.row + head_a * ar.head), place, dim, wide);
+                y[u] = attn_load<T, G, EL, false>(static_cast<const T*>(br.at) + (row[u] * br.row + head_b * br.head), place, dim, wide);
+            }
+        }
+    }
+    // Zeros in place of what masked edges read: not even a product is formed with it.  All lanes of a warp call it.
+    __device__ __forceinline__ void clear()
+    {
+        bool all = true;
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) all = all && ok[u];
+        if (__all_sync(0xffffffffu, all)) return;
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            attn_clear(x[u], ok[u]);
+            attn_clear(y[u], ok[u]);
+        }
+    }
+};
+// f holds the elements in the lane's order of pieces.
+template <typename T, int G, int EL, bool FULL>
+__device__ __forceinline__ void attn_store(T* head, const Place<T, G, EL>& place, int dim, int wide, const float2 (&f)[EL / 2])
+{
+    constexpr int VEC = Place<T, G, EL>::VEC;
+#pragma unroll
+    for (int p = 0; p < Place<T, G, EL>::PIECES; p++) {
         const int at = place.at[p];
         __align__(16) T e[VEC];
 #pragma unroll
@@ -127,8 +188,11 @@ __device__ __forceinline__ void attn_store(T* head, const Place<T, G>& place, in
             e[i] = attn_put<T>(f[(p * VEC + i) / 2].x);
             e[i + 1] = attn_put<T>(f[(p * VEC + i) / 2].y);
         }
-        if (FULL || wide) {
+        if (FULL || wide == 16) {
             if (FULL || at < dim) *reinterpret_cast<uint4*>(head + at) = *reinterpret_cast<const uint4*>(e);
+        } else if (wide == 8) {
+            if (at < dim) *reinterpret_cast<uint2*>(head + at) = *reinterpret_cast<const uint2*>(e);
+            if (at + VEC / 2 < dim) *reinterpret_cast<uint2*>(head + at + VEC / 2) = *reinterpret_cast<const uint2*>(e + VEC / 2);
         } else {
 #pragma unroll
             for (int i = 0; i < VEC; i++)
@@ -136,6 +200,8 @@ __device__ __forceinline__ void attn_store(T* head, const Place<T, G>& place, in
         }
     }
 }
+// What an edge that takes no part reads in place of its rows.
+static __device__ __align__(16) unsigned char attn_zeros[DYNB_ATTENTION_MAX_DIM * 4];
 
 template <int G>
 __device__ __forceinline__ float head_sum(float v)
@@ -144,11 +210,12 @@ __device__ __forceinline__ float head_sum(float v)
     for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ float dot8(const float2 (&a)[4], const float2 (&b)[4])
+template <int N>
+__device__ __forceinline__ float inner(const float2 (&a)[N], const float2 (&b)[N])
 {
     float2 s = mul2(a[0], b[0]);
 #pragma unroll
-    for (int i = 1; i < 4; i++) s = fma2(a[i], b[i], s);
+    for (int i = 1; i < N; i++) s = fma2(a[i], b[i], s);
     return s.x + s.y;
 }
 
@@ -159,17 +226,32 @@ struct AttnEdges {
     float z[BATCH];
     __device__ __forceinline__ void fetch(const int32_t* src, const float* bias, int e, int n, int heads)
     {
+        src += e;
+        bias += (int64_t)e * heads;
+        if (e + BATCH <= n) {
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            s[u] = e + u < n ? __ldg(src + e + u) : -1;
-            z[u] = 0.0f;
-            if (bias != nullptr && e + u < n) z[u] = __ldg(bias + (int64_t)(e + u) * heads);
+            for (int u = 0; u < BATCH; u++) s[u] = __ldg(src + u);
+#pragma unroll
+            for (int u = 0; u < BATCH; u++, bias += heads) z[u] = heads > 0 ? __ldg(bias) : 0.0f;
+        } else {
+#pragma unroll
+            for (int u = 0; u < BATCH; u++, bias += heads) {
+                s[u] = e + u < n ? __ldg(src + u) : -1;
+                z[u] = heads > 0 && e + u < n ? __ldg(bias) : 0.0f;
+            }
         }
     }
-    __device__ __forceinline__ bool live(int u, uint32_t sources) const { return (uint32_t)s[u] < sources && z[u] != -INFINITY; }
+    // Rows to read and whether the edges take part.
+    __device__ __forceinline__ void rows(uint32_t sources, uint32_t (&row)[BATCH], bool (&ok)[BATCH]) const
+    {
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            const bool in = (uint32_t)s[u] < sources;
+            row[u] = in ? (uint32_t)s[u] : 0u;
+            ok[u] = in && z[u] != -INFINITY;
+        }
+    }
 };
-
-struct AttnRows { const void* at; int64_t row, head; };   // strides in elements, the elements of a head are consecutive
 
 struct AttnArgs {
     AttnRows q, k, v, d_out;
@@ -177,12 +259,15 @@ struct AttnArgs {
     const float* out32;         // [targets, heads, dim]: the result, unrounded
     const float* stats;         // [targets, 2, heads]: largest logit and 1 / sum of exponentials (a logarithm of the sum beside a
                                 // largest logit of -3e38, as masks of the type's lowest value give, would be lost)
-    float* delta;               // [targets, heads]: d_out . out
+    float4* delta;              // [targets, heads]: largest logit, 1 / sum, d_out . out, 0 (one load an edge for the pass by source)
     void *out, *dq, *dk, *dv;   // contiguous
     float *out32_w, *stats_w, *d_bias;
     const int32_t *rows, *row_start, *src, *cols, *col_start, *in_edge, *in_dst;
     int64_t n_targets, n_sources, n_edges;
-    int heads, kv_heads, shared, dim, warp_heads, wide;
+    int heads, kv_heads, shared, dim, warp_heads;
+    int wide;                   // bytes on which all heads start and end: 16, 8 or fewer
+    int narrow;                 // offsets in units of 16 bytes fit 32 bits
+    int block_rows;             // rows of a block, a multiple of those that it takes at once
     float scale;
 };
 
@@ -190,30 +275,26 @@ cudaError_t attn_forward(const AttnArgs& a, int dtype, cudaStream_t s);
 cudaError_t attn_backward_rows(const AttnArgs& a, int dtype, cudaStream_t s);
 cudaError_t attn_backward_cols(const AttnArgs& a, int dtype, cudaStream_t s);
 
-// Lanes a head.
-static inline int attn_lanes(int dim)
-{
-    int g = 1;
-    while (g * 8 < dim) g *= 2;
-    return g;
-}
+// Elements a lane: 32 bytes.
+template <typename T> struct LaneElements { static constexpr int N = 32 / (int)sizeof(T); };
 
 template <typename T, template <typename, int, bool> class Launch, int G>
 static inline cudaError_t attn_by_full(const AttnArgs& a, cudaStream_t s)
 {
-    return a.wide && a.dim == 8 * G ? Launch<T, G, true>::go(a, s) : Launch<T, G, false>::go(a, s);
+    return a.wide == 16 && a.narrow && a.dim == LaneElements<T>::N * G ? Launch<T, G, true>::go(a, s) : Launch<T, G, false>::go(a, s);
 }
 template <typename T, template <typename, int, bool> class Launch>
 static inline cudaError_t attn_by_dim(const AttnArgs& a, cudaStream_t s)
 {
-    switch (attn_lanes(a.dim)) {
-    case 1: return attn_by_full<T, Launch, 1>(a, s);
-    case 2: return attn_by_full<T, Launch, 2>(a, s);
-    case 4: return attn_by_full<T, Launch, 4>(a, s);
-    case 8: return attn_by_full<T, Launch, 8>(a, s);
-    case 16: return attn_by_full<T, Launch, 16>(a, s);
-    default: return attn_by_full<T, Launch, 32>(a, s);
+    const int lanes = (a.dim + LaneElements<T>::N - 1) / LaneElements<T>::N;
+    if (lanes <= 1) return attn_by_full<T, Launch, 1>(a, s);
+    if (lanes <= 2) return attn_by_full<T, Launch, 2>(a, s);
+    if (lanes <= 4) return attn_by_full<T, Launch, 4>(a, s);
+    if (lanes <= 8) return attn_by_full<T, Launch, 8>(a, s);
+    if constexpr (sizeof(T) == 4) {
+        if (lanes > 16) return attn_by_full<T, Launch, 32>(a, s);
     }
+    return attn_by_full<T, Launch, 16>(a, s);
 }
 template <template <typename, int, bool> class Launch>
 static inline cudaError_t attn_by_type(const AttnArgs& a, int dtype, cudaStream_t s)
@@ -231,6 +312,15 @@ static inline int attn_warp_heads(int heads, int g)
     return h;
 }
 
+// Rows of a block that takes `at_once` at once: neighbouring rows read the same rows of the other side, so a block goes on with the next ones
+// while L1 holds these, as long as there are eight blocks for every place on the SMs.
+constexpr int ATTN_TURNS = 8;
+static inline int attn_block_rows(int64_t rows, int at_once)
+{
+    int turns = ATTN_TURNS;
+    while (turns > 1 && rows < (int64_t)at_once * turns * 148 * 4 * 8) turns /= 2;
+    return at_once * turns;
+}
 // Whether four warps share a row: where there are too few rows for the SMs (148 x 16 warps), or the lists are long.
 static inline bool attn_split(int64_t warps, int64_t edges) { return warps < 148 * 16 || edges > warps * 512; }
 

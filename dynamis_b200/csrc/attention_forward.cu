@@ -10,30 +10,33 @@
 
 namespace dynb {
 
-constexpr int AF_WARPS = 8;
-constexpr int AF_BATCH = 4;   // edges of a slot in flight
+constexpr int AF_WARPS = 4;
+// Edges of a slot in a batch; heads of odd sizes need the registers for their loads.
+template <bool FULL> constexpr int AF_BATCH = FULL ? 4 : 2;
 
 // WPR warps take turns at the batches of a row and join through shared memory.
 template <typename T, int G, bool FULL, int WPR>
-__global__ void __launch_bounds__(AF_WARPS * 32)
+__global__ void __launch_bounds__(AF_WARPS * 32, 4)
 attn_forward_kernel(const AttnArgs a)
 {
+    constexpr int EL = LaneElements<T>::N, BATCH = AF_BATCH<FULL>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = lane % G, slots = 32 / (G * a.warp_heads), slot = lane / (G * a.warp_heads);
     const int head = blockIdx.y * a.warp_heads + (lane / G) % a.warp_heads;
-    const bool mine = head < a.heads, wide = a.wide != 0;
+    const bool mine = head < a.heads;
+    const int wide = a.wide;
     const int h = mine ? head : 0, kv = h / a.shared;
-    const Place<T, G> place(part, h);
+    const Place<T, G, EL> place(part, h);
     const uint32_t sources = (uint32_t)a.n_sources;
-    const uint32_t k_step = (uint32_t)(a.k.row * (int)sizeof(T)), v_step = (uint32_t)(a.v.row * (int)sizeof(T));
-    const char* const kb = reinterpret_cast<const char*>(static_cast<const T*>(a.k.at) + kv * a.k.head);
-    const char* const vb = reinterpret_cast<const char*>(static_cast<const T*>(a.v.at) + kv * a.v.head);
+    const Lane<T, G, EL> k_lane(a.k, kv, place), v_lane(a.v, kv, place);
     constexpr int ROWS = AF_WARPS / WPR;
-    const int turn = warp % WPR, step = AF_BATCH * slots;
+    const int turn = warp % WPR, step = BATCH * slots, bias_step = a.bias != nullptr ? a.heads : 0;
+    const char* const zeros = reinterpret_cast<const char*>(attn_zeros);
 
-    for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.n_targets; r0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t last = min(((int64_t)blockIdx.x + 1) * a.block_rows, a.n_targets);
+    for (int64_t r0 = (int64_t)blockIdx.x * a.block_rows; r0 < last; r0 += ROWS) {
         const int64_t r = r0 + warp / WPR;
-        int32_t t = r < a.n_targets ? a.rows[r] : -1;
+        int32_t t = r < last ? a.rows[r] : -1;
         if ((uint32_t)t >= (uint32_t)a.n_targets) t = -1;
         if (WPR == 1 && t < 0) continue;
         int64_t begin = 0, end = 0;
@@ -43,59 +46,59 @@ attn_forward_kernel(const AttnArgs a)
         }
         const int n = (int)max(end - begin, (int64_t)0);
         const int32_t* const src = a.src + begin;
-        const float* const bias = a.bias != nullptr ? a.bias + begin * a.heads + h : nullptr;
+        const float* const bias = a.bias + (begin * bias_step + h);   // not read where there is none
 
-        float2 q[4], acc[4];
-        if (t >= 0) attn_pairs(attn_load<T, G, FULL>(static_cast<const T*>(a.q.at) + t * a.q.row + h * a.q.head, place, a.dim, wide), q);
-        else attn_pairs(attn_nothing<T>(), q);
+        float2 q[EL / 2], acc[EL / 2];
+        attn_pairs(attn_load<T, G, EL, FULL>(t >= 0 ? static_cast<const T*>(a.q.at) + t * a.q.row + h * a.q.head : reinterpret_cast<const T*>(zeros), place, a.dim, wide), q);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < EL / 2; i++) {
             q[i] = mul2(q[i], make_float2(a.scale, a.scale));
             acc[i] = make_float2(0.0f, 0.0f);
         }
         float top = -INFINITY, sum = 0.0f;
-        int e = turn * step + slot * AF_BATCH;
-        AttnEdges<AF_BATCH> now;
-        now.fetch(src, bias, e, n, a.heads);
-        for (int base = turn * step; base < n; base += WPR * step) {
-            Raw<T> ku[AF_BATCH], vu[AF_BATCH];
-            float z[AF_BATCH];
+        int e = turn * step + slot * BATCH;
+        AttnEdges<BATCH> ahead;
+        ahead.fetch(src, bias, e, n, bias_step);
+        auto load = [&](AttnStep<T, EL, BATCH>& s) {
+            uint32_t row[BATCH];
+            ahead.rows(sources, row, s.ok);
+            s.template load<G, FULL>(k_lane, v_lane, place, a.k, a.v, kv, kv, row, a.dim, wide);
 #pragma unroll
-            for (int u = 0; u < AF_BATCH; u++) {
-                const bool ok = now.live(u, sources);
-                ku[u] = attn_nothing<T>();
-                vu[u] = attn_nothing<T>();   // masked: not even a product with what its rows hold
-                if (ok) {
-                    ku[u] = attn_load<T, G, FULL>(reinterpret_cast<const T*>(kb + (uint64_t)(uint32_t)now.s[u] * k_step), place, a.dim, wide);
-                    vu[u] = attn_load<T, G, FULL>(reinterpret_cast<const T*>(vb + (uint64_t)(uint32_t)now.s[u] * v_step), place, a.dim, wide);
-                }
-                z[u] = ok ? now.z[u] : -INFINITY;
-            }
+            for (int u = 0; u < BATCH; u++) s.z[u] = ahead.z[u];
             e += WPR * step;
-            now.fetch(src, bias, e, n, a.heads);
+            ahead.fetch(src, bias, e, n, bias_step);
+        };
+        auto work = [&](AttnStep<T, EL, BATCH>& s) {
+            s.clear();
             float most = top;
 #pragma unroll
-            for (int u = 0; u < AF_BATCH; u++) {
-                float2 f[4];
-                attn_pairs(ku[u], f);
-                z[u] += head_sum<G>(dot8(q, f));
-                most = fmaxf(most, z[u]);
+            for (int u = 0; u < BATCH; u++) {
+                float2 f[EL / 2];
+                attn_pairs(s.x[u], f);
+                const float product = head_sum<G>(inner(q, f));
+                s.z[u] = s.ok[u] ? s.z[u] + product : -INFINITY;
+                most = fmaxf(most, s.z[u]);
             }
             // NaN logits are not in the maximum: they reach the sums through their own exponentials
             const float from = most == -INFINITY ? 0.0f : most, back = pow2((top - from) * LOG2E);
             top = most;
             sum *= back;
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = mul2(acc[i], make_float2(back, back));
+            for (int i = 0; i < EL / 2; i++) acc[i] = mul2(acc[i], make_float2(back, back));
 #pragma unroll
-            for (int u = 0; u < AF_BATCH; u++) {
-                const float w = pow2((z[u] - from) * LOG2E);
+            for (int u = 0; u < BATCH; u++) {
+                const float w = pow2((s.z[u] - from) * LOG2E);
                 sum += w;
-                float2 f[4];
-                attn_pairs(vu[u], f);
+                float2 f[EL / 2];
+                attn_pairs(s.y[u], f);
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[i] = fma2(make_float2(w, w), f[i], acc[i]);
+                for (int i = 0; i < EL / 2; i++) acc[i] = fma2(make_float2(w, w), f[i], acc[i]);
             }
+        };
+        for (int base = turn * step; base < n; base += WPR * step) {   // the same for all lanes
+            AttnStep<T, EL, BATCH> s;
+            load(s);
+            work(s);
         }
         // the slots of the warp join
         for (int o = G * a.warp_heads; o < 32; o <<= 1) {
@@ -105,7 +108,7 @@ attn_forward_kernel(const AttnArgs a)
             sum *= back;
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < EL / 2; i++) {
                 acc[i].x *= back;
                 acc[i].y *= back;
                 acc[i].x += __shfl_xor_sync(0xffffffffu, acc[i].x, o);
@@ -113,12 +116,12 @@ attn_forward_kernel(const AttnArgs a)
             }
         }
         if (WPR > 1) {   // the warps of the row join in their order
-            __shared__ float joint[AF_WARPS][10][32];
+            __shared__ float joint[AF_WARPS][EL + 2][32];
             __syncthreads();
-            joint[warp][8][lane] = top;
-            joint[warp][9][lane] = sum;
+            joint[warp][EL][lane] = top;
+            joint[warp][EL + 1][lane] = sum;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < EL / 2; i++) {
                 joint[warp][2 * i][lane] = acc[i].x;
                 joint[warp][2 * i + 1][lane] = acc[i].y;
             }
@@ -126,16 +129,16 @@ attn_forward_kernel(const AttnArgs a)
             if (turn != 0) continue;
             float most = top;
 #pragma unroll
-            for (int w = 1; w < WPR; w++) most = fmaxf(most, joint[warp + w][8][lane]);
+            for (int w = 1; w < WPR; w++) most = fmaxf(most, joint[warp + w][EL][lane]);
             sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = make_float2(0.0f, 0.0f);
+            for (int i = 0; i < EL / 2; i++) acc[i] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < WPR; w++) {
-                const float back = most == -INFINITY ? 1.0f : pow2((joint[warp + w][8][lane] - most) * LOG2E);
-                sum = fmaf(joint[warp + w][9][lane], back, sum);
+                const float back = most == -INFINITY ? 1.0f : pow2((joint[warp + w][EL][lane] - most) * LOG2E);
+                sum = fmaf(joint[warp + w][EL + 1][lane], back, sum);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < EL / 2; i++) {
                     acc[i].x = fmaf(joint[warp + w][2 * i][lane], back, acc[i].x);
                     acc[i].y = fmaf(joint[warp + w][2 * i + 1][lane], back, acc[i].y);
                 }
@@ -146,12 +149,13 @@ attn_forward_kernel(const AttnArgs a)
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t at = ((int64_t)t * a.heads + head) * a.dim;
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = mul2(acc[i], make_float2(inv, inv));
-        attn_store<T, G, FULL>(static_cast<T*>(a.out) + at, place, a.dim, wide, acc);
+        for (int i = 0; i < EL / 2; i++) acc[i] = mul2(acc[i], make_float2(inv, inv));
+        attn_store<T, G, EL, FULL>(static_cast<T*>(a.out) + at, place, a.dim, wide, acc);
         if (sizeof(T) != 4 && a.out32_w != nullptr) {
+            constexpr int VEC = Place<T, G, EL>::VEC;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int d = place.at[0] + 2 * i;
+            for (int i = 0; i < EL / 2; i++) {
+                const int d = place.at[2 * i / VEC] + 2 * i % VEC;
                 if (FULL) {
                     *reinterpret_cast<float2*>(a.out32_w + at + d) = acc[i];
                 } else {
@@ -176,7 +180,8 @@ struct AttnForward {
         const int blocks = (a.heads + a.warp_heads - 1) / a.warp_heads;
         const bool split = attn_split(a.n_targets * blocks, a.n_edges * blocks);
         const int rows = split ? AF_WARPS / 4 : AF_WARPS;
-        const dim3 grid((unsigned)((a.n_targets + rows - 1) / rows), blocks);
+        a.block_rows = attn_block_rows(a.n_targets * blocks, rows);
+        const dim3 grid((unsigned)((a.n_targets + a.block_rows - 1) / a.block_rows), blocks);
         if (split) attn_forward_kernel<T, G, FULL, 4><<<grid, AF_WARPS * 32, 0, s>>>(a);
         else attn_forward_kernel<T, G, FULL, 1><<<grid, AF_WARPS * 32, 0, s>>>(a);
         return cudaGetLastError();

@@ -251,7 +251,7 @@ using namespace dynb;
 static int ni_check(int64_t E, int64_t nt, int64_t ns)
 {
     if (E < 0 || nt < 0 || ns < 0) return fail_arg("neighbor_index: sizes must be non-negative");
-    if (E >= INT32_MAX || nt >= INT32_MAX || ns >= INT32_MAX) return fail_arg("neighbor_index: sizes must be below 2^31 - 1");
+    if (E >= DYNB_MAX_EDGES || nt >= INT32_MAX || ns >= INT32_MAX) return fail_arg("neighbor_index: sizes must be below 2^31 - 1, edges below 2^31 - 2^16");
     return DYNB_OK;
 }
 

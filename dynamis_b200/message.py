@@ -38,6 +38,7 @@ MAX_BIAS_HEADS = 1024    # DYNB_DISTANCE_BIAS_MAX_HEADS
 MAX_TYPES = 4096         # DYNB_TYPE_LINEAR_MAX_TYPES
 MAX_WIDTH = 16384        # DYNB_TYPE_LINEAR_MAX_WIDTH
 INT32_MAX = 2 ** 31 - 1
+MAX_EDGES = 2 ** 31 - 2 ** 16   # DYNB_MAX_EDGES
 
 
 def _lists(what: str, **lists) -> None:
@@ -131,8 +132,8 @@ def neighbor_index(edge_index: torch.Tensor, num_targets: int, num_sources: int)
     T, S, E = int(num_targets), int(num_sources), edge_index.size(1)
     if not (0 <= T < INT32_MAX and 0 <= S < INT32_MAX):
         raise RuntimeError(f"num_targets and num_sources must lie in [0, 2^31 - 1), got {T} and {S}")
-    if E >= INT32_MAX:
-        raise RuntimeError(f"edge_index must have fewer than 2^31 - 1 edges, got {E}")
+    if E >= MAX_EDGES:
+        raise RuntimeError(f"edge_index must have fewer than {MAX_EDGES} edges, got {E}")
     if E > 0 and edge_index.stride(1) != 1:
         edge_index = edge_index.contiguous()
     dev = edge_index.device
@@ -219,7 +220,7 @@ class _NeighborAttention(torch.autograd.Function):
             dk = torch.empty(k.shape, dtype=k.dtype, device=dev) if want_k else None
             dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if want_v else None
             d_bias = torch.empty(bias.shape, dtype=torch.float32, device=dev) if want_bias else None
-            delta = torch.empty((q.size(0), q.size(1)), dtype=torch.float32, device=dev)
+            delta = torch.empty((q.size(0), q.size(1), 4), dtype=torch.float32, device=dev)
             args = _attention_args(q, k, v, bias, index, ctx.scale)
             _lib.check(_lib.lib().dynb_neighbor_attention_backward(
                 ctypes.byref(args), d_out.data_ptr(), d_out.stride(0), d_out.stride(1), out32.data_ptr(), stats.data_ptr(), index.cols.data_ptr(),

@@ -444,6 +444,7 @@ int dynb_integrator_step(int kind, float* pos_dev, float* vel_dev, const float* 
  * Two phases: the plan writes rows, row_start, src32, cols and col_start, and two words to pinned host memory: word 0 has bit 0 set
  * when an endpoint is out of range and bit 1 when the edges of a target are apart (nothing else is valid then), word 1 is the longest
  * list of a source.  The caller waits for the stream and calls the fill with word 1 and the workspace of the plan. */
+#define DYNB_MAX_EDGES ((1ll << 31) - (1ll << 16))
 int dynb_neighbor_index_workspace_bytes(int64_t n_edges, int64_t n_targets, int64_t n_sources, int64_t* bytes);
 int dynb_neighbor_index_plan(const int64_t* src_dev, const int64_t* dst_dev, int64_t n_edges, int64_t n_targets, int64_t n_sources,
                              int32_t* rows_dev, int32_t* row_start_dev, int32_t* src32_dev, int32_t* cols_dev, int32_t* col_start_dev,
@@ -470,7 +471,7 @@ typedef struct dynb_attention {
 /* out32_dev [n_targets, heads, dim] (the unrounded result; may be out_dev for DYNB_F32) and stats_dev [n_targets, 2, heads] are for
  * the backward pass; NULL when there is none. */
 int dynb_neighbor_attention(const dynb_attention* args, void* out_dev, float* out32_dev, float* stats_dev, void* stream);
-/* Gradients, each NULL when it is not wanted; contiguous.  delta_dev [n_targets, heads] is scratch.  No atomics: the sums of a row
+/* Gradients, each NULL when it is not wanted; contiguous.  delta_dev [n_targets, heads, 4] (on 16 bytes) is scratch.  No atomics: the sums of a row
  * are in the order of its list. */
 int dynb_neighbor_attention_backward(const dynb_attention* args, const void* d_out_dev, int64_t d_out_row, int64_t d_out_head,
                                      const float* out32_dev, const float* stats_dev, const int32_t* cols_dev, const int32_t* col_start_dev,
