@@ -14,6 +14,7 @@
 namespace dynb {
 
 constexpr int DB_THREADS = 256;
+constexpr int DB_TABLE_BYTES = 24 << 10;   // tables that blocks copy to shared memory: eight blocks an SM hold one each
 
 struct DbArgs {
     const float *dist, *table, *d_bias;
@@ -59,21 +60,144 @@ __device__ __forceinline__ void db_slopes(float t, float (&w)[4])
     w[3] = 0.5f * t * t;
 }
 
+// log f(u): one logarithm of the product, which is at least 2^-72.
+__device__ __forceinline__ float db_switch(const DbPlace& p)
+{
+    return logf(p.rest * p.rest * p.rest * fmaf(p.u, fmaf(p.u, 6.0f, 3.0f), 1.0f));
+}
+
+// A thread takes VEC heads of an edge (eight of them leave half sectors to write: 159 us for 10.5 M edges of 8 heads, four 111); the table is in shared memory (IN_SMEM) where it fits.
+template <int VEC, bool IN_SMEM>
 __global__ void __launch_bounds__(DB_THREADS)
 db_forward_kernel(const DbArgs a)
 {
-    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < a.n; e += (int64_t)gridDim.x * blockDim.x) {
-        const DbPlace p = db_place(a.dist[e], a);
-        float w[4];
+    extern __shared__ __align__(16) float copies[];
+    const float* table = a.table;
+    if (IN_SMEM) {
+        for (int i = threadIdx.x; i < a.buckets * a.heads; i += DB_THREADS) copies[i] = a.table[i];
+        __syncthreads();
+        table = copies;
+    }
+    const uint32_t per = (uint32_t)(a.heads / VEC);
+    const int64_t total = a.n * per;
+    for (int64_t i = (int64_t)blockIdx.x * DB_THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * DB_THREADS) {
+        const int64_t e = per == 2 ? i >> 1 : per == 1 ? i : i / per;
+        const int h = (int)(i - e * per) * VEC;
+        const DbPlace p = db_place(__ldg(a.dist + e), a);
+        float w[4], v[VEC];
         db_weights(p.t, w);
-        float add = 0.0f;
-        if (a.smooth) add = 3.0f * logf(p.rest) + logf(fmaf(p.u, fmaf(p.u, 6.0f, 3.0f), 1.0f));
-        for (int h = 0; h < a.heads; h++) {
-            float v = add;
+        const float add = a.smooth ? db_switch(p) : 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) v = fmaf(w[j], a.table[(p.at + j) * a.heads + h], v);
-            a.bias[e * a.heads + h] = p.inside ? v : -INFINITY;
+        for (int k = 0; k < VEC; k++) v[k] = add;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float* const row = table + (p.at + j) * a.heads + h;
+            if constexpr (VEC == 1) {
+                v[0] = fmaf(w[j], row[0], v[0]);
+            } else {
+                const float4 t = *reinterpret_cast<const float4*>(row);
+                v[0] = fmaf(w[j], t.x, v[0]);
+                v[1] = fmaf(w[j], t.y, v[1]);
+                v[2] = fmaf(w[j], t.z, v[2]);
+                v[3] = fmaf(w[j], t.w, v[3]);
+            }
         }
+#pragma unroll
+        for (int k = 0; k < VEC; k++) v[k] = p.inside ? v[k] : -INFINITY;
+        float* const out = a.bias + e * a.heads + h;
+        if constexpr (VEC == 1) out[0] = v[0];
+        else *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// Both gradients from one reading of the bias's gradient, for up to 32 heads.  A warp takes 32 edges at a time: every lane works out the
+// place, the weights and the slopes of one of them, then WIDE rounds follow in which the lanes are 32 / WIDE edges times WIDE heads.  A lane has
+// a column of its own in the warp's copy of the table's gradient, [buckets][32]: no atomics, no two lanes in one bank, and the order of
+// its sums is that of the edges.  Blocks write their sums; db_table_join_kernel adds these in 64 bits.
+// What bounds it is shared memory: 16 reads and writes a round (10.5 M edges, 64 x 8: 0.29 ms, 1.4 TB/s; 16 warps 0.33).  The two gradients in
+// kernels of their own, without rounds: 0.30 and 1.10 ms.
+constexpr int DB_SCRATCH = 32 * 12;   // floats of a warp: weights, slopes, {place, pull} of 32 edges, 16 + 16 + 16 bytes each
+template <int WIDE>
+__global__ void __launch_bounds__(704, 1)
+db_backward_kernel(const DbArgs a)
+{
+    extern __shared__ __align__(16) float copies[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    constexpr int SLOTS = 32 / WIDE;
+    const int h = lane % WIDE, slot = lane / WIDE, words = a.buckets * 32;
+    float* const table = copies;                                   // [buckets][32], the columns of a slot each
+    float* const mine = copies + words + warp * (words + DB_SCRATCH);
+    float4* const weights = reinterpret_cast<float4*>(mine + words);
+    float4* const slopes = weights + 32;
+    float2* const places = reinterpret_cast<float2*>(slopes + 32);
+    for (int i = threadIdx.x; i < words; i += blockDim.x) {
+        const int hh = i % WIDE;
+        table[i] = a.d_dist != nullptr && hh < a.heads ? a.table[i / 32 * a.heads + hh] : 0.0f;
+    }
+    for (int i = lane; i < words; i += 32) mine[i] = 0.0f;
+    __syncthreads();
+    const bool live = h < a.heads;
+    const float pieces = (float)(a.buckets - 3);
+    const int64_t step = (int64_t)gridDim.x * warps * 32;
+    int64_t base = ((int64_t)blockIdx.x * warps + warp) * 32;
+    auto distance = [&](int64_t at) { return at + lane < a.n ? __ldg(a.dist + at + lane) : INFINITY; };
+    float r = distance(base);
+    for (; base < a.n; base += step) {
+        float g[WIDE];
+#pragma unroll
+        for (int k = 0; k < WIDE; k++) {
+            const int64_t e = base + k * SLOTS + slot;
+            g[k] = live && e < a.n ? __ldg(a.d_bias + e * a.heads + h) : 0.0f;
+        }
+        const float r_next = distance(base + step);
+        const DbPlace p = db_place(r, a);
+        float w[4], s[4];
+        db_weights(p.t, w);
+        db_slopes(p.t, s);
+        // 1 / cutoff is taken at the end; pull: slope of the switch times the cutoff
+        const float pull = a.smooth && p.inside ? -30.0f * p.u * p.u / (p.rest * fmaf(p.u, fmaf(p.u, 6.0f, 3.0f), 1.0f)) : 0.0f;
+        __syncwarp();
+        const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        weights[lane] = p.inside ? make_float4(w[0], w[1], w[2], w[3]) : none;
+        slopes[lane] = p.inside ? make_float4(s[0] * pieces, s[1] * pieces, s[2] * pieces, s[3] * pieces) : none;
+        places[lane] = make_float2(__int_as_float(p.inside ? p.at : -1), pull);
+        __syncwarp();
+        float total = 0.0f;   // of edge base + lane, once its round has come
+#pragma unroll
+        for (int k = 0; k < WIDE; k++) {
+            const int at_edge = k * SLOTS + slot;
+            const float2 where = places[at_edge];
+            const int at = max(__float_as_int(where.x), 0);
+            const float gk = __float_as_int(where.x) < 0 ? 0.0f : g[k];   // beyond the cutoff: whatever the gradient holds
+            const float4 wk = weights[at_edge];
+            float* const column = mine + at * 32 + lane;
+            column[0] = fmaf(wk.x, gk, column[0]);
+            column[32] = fmaf(wk.y, gk, column[32]);
+            column[64] = fmaf(wk.z, gk, column[64]);
+            column[96] = fmaf(wk.w, gk, column[96]);
+            if (a.d_dist != nullptr) {
+                const float4 sk = slopes[at_edge];
+                const float* const t = table + at * 32 + lane;
+                float v = fmaf(sk.x, t[0], fmaf(sk.y, t[32], fmaf(sk.z, t[64], fmaf(sk.w, t[96], where.y)))) * gk;
+#pragma unroll
+                for (int o = WIDE / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                // the sum of edge k SLOTS + s is with the lanes of slot s
+                const float mine_now = __shfl_sync(0xffffffffu, v, (lane % SLOTS) * WIDE);
+                if (lane / SLOTS == k) total = mine_now;
+            }
+        }
+        if (a.d_dist != nullptr && base + lane < a.n) a.d_dist[base + lane] = r < 0.0f ? 0.0f : total / a.cutoff;
+        r = r_next;
+    }
+    if (a.partial == nullptr) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.buckets * WIDE; i += blockDim.x) {
+        const int hh = i % WIDE, k = i / WIDE;
+        if (hh >= a.heads) continue;
+        float sum = 0.0f;
+        for (int c = 0; c < warps; c++)
+            for (int s = 0; s < SLOTS; s++) sum += copies[words + c * (words + DB_SCRATCH) + k * 32 + s * WIDE + hh];
+        a.partial[((int64_t)blockIdx.x * a.buckets + k) * a.heads + hh] = sum;
     }
 }
 
@@ -98,7 +222,7 @@ db_dist_kernel(const DbArgs a)
     }
 }
 
-// Gradient of the table.  A warp's lanes are `slots` edges times `wide` heads; every slot has a copy of the table in shared memory that
+// Gradient of the table for more heads or buckets than the kernel above has room for.  A warp's lanes are `slots` edges times `wide` heads; every slot has a copy of the table in shared memory that
 // no other slot touches, so the sums need no atomics and their order is that of the edges.  Blocks take fixed stretches of the
 // edges and write their sums; db_table_join_kernel adds these in 64 bits.
 __global__ void
@@ -134,20 +258,45 @@ db_table_kernel(const DbArgs a, int wide)
     }
 }
 
+// 32 cells a block, eight runs of blocks each.
 __global__ void __launch_bounds__(DB_THREADS)
 db_table_join_kernel(const DbArgs a, int blocks)
 {
-    const int64_t cells = (int64_t)a.buckets * a.heads;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < cells; i += (int64_t)gridDim.x * blockDim.x) {
-        double sum = 0.0;
-        for (int b = 0; b < blocks; b++) sum += (double)a.partial[b * cells + i];
-        a.d_table[i] = (float)sum;
-    }
+    __shared__ double part[8][32];
+    const int64_t cells = (int64_t)a.buckets * a.heads, i = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
+    const int run = threadIdx.x / 32;
+    double sum = 0.0;
+    if (i < cells)
+        for (int b = run; b < blocks; b += 8) sum += (double)a.partial[b * cells + i];
+    part[run][threadIdx.x % 32] = sum;
+    __syncthreads();
+    if (run != 0 || i >= cells) return;
+#pragma unroll
+    for (int k = 1; k < 8; k++) sum += part[k][threadIdx.x];
+    a.d_table[i] = (float)sum;
 }
 
 static int db_table_blocks(int64_t n)
 {
     return (int)std::max<int64_t>(1, std::min<int64_t>((n + 1023) / 1024, 148));
+}
+
+// The kernel for both gradients: warps of a block, 0 where the heads or the buckets are too many for it.
+static int db_backward_warps(int buckets, int heads)
+{
+    if (heads > 32) return 0;
+    const int words = buckets * 32, room = (224 << 10) / 4 - words;
+    return std::min(22, room / (words + DB_SCRATCH));
+}
+
+template <int WIDE>
+static cudaError_t db_backward(const DbArgs& a, int blocks, int warps, cudaStream_t s)
+{
+    const int words = a.buckets * 32, smem = 4 * (words + warps * (words + DB_SCRATCH));
+    const cudaError_t rc = cudaFuncSetAttribute(db_backward_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc != cudaSuccess) return rc;
+    db_backward_kernel<WIDE><<<blocks, warps * 32, smem, s>>>(a);
+    return cudaGetLastError();
 }
 
 static int db_check(int64_t n, int heads, int buckets, double cutoff)
@@ -178,7 +327,18 @@ extern "C" int dynb_distance_bias(const float* dist_dev, int64_t n, const float*
     DbArgs a = {};
     a.dist = dist_dev; a.table = table_dev; a.bias = bias_dev;
     a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff;
-    db_forward_kernel<<<db_blocks(n), DB_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    const bool aligned = reinterpret_cast<uintptr_t>(bias_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(table_dev) % 16 == 0;
+    const int vec = aligned && heads % 4 == 0 ? 4 : 1;
+    const int bytes = buckets * heads * 4, smem = bytes <= DB_TABLE_BYTES ? bytes : 0;
+    const unsigned blocks = db_blocks(n * (heads / vec));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (smem > 0) {
+        if (vec == 4) db_forward_kernel<4, true><<<blocks, DB_THREADS, smem, s>>>(a);
+        else db_forward_kernel<1, true><<<blocks, DB_THREADS, smem, s>>>(a);
+    } else {
+        if (vec == 4) db_forward_kernel<4, false><<<blocks, DB_THREADS, 0, s>>>(a);
+        else db_forward_kernel<1, false><<<blocks, DB_THREADS, 0, s>>>(a);
+    }
     DYNB_CUDA_OK(cudaGetLastError());
     return DYNB_OK;
 }
@@ -203,24 +363,37 @@ extern "C" int dynb_distance_bias_backward(const float* dist_dev, int64_t n, con
     a.dist = dist_dev; a.table = table_dev; a.d_bias = d_bias_dev; a.d_dist = d_dist_dev; a.d_table = d_table_dev;
     a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (d_dist_dev != nullptr && n > 0) {
-        db_dist_kernel<<<db_blocks(n), DB_THREADS, 0, s>>>(a);
-        DYNB_CUDA_OK(cudaGetLastError());
-    }
+    const int blocks = db_table_blocks(n);
     if (d_table_dev != nullptr) {
-        const int blocks = db_table_blocks(n);
         if (workspace_dev == nullptr || workspace_bytes < (int64_t)blocks * buckets * heads * 4) return fail_arg("workspace too small");
         a.partial = static_cast<float*>(workspace_dev);
-        int wide = 1;
-        while (wide < heads && wide < 32) wide *= 2;
-        // as many warps as have their copies in 128 KB, and no more than 16
-        const int warps = std::max(1, std::min(16, (128 << 10) / (buckets * 128)));
-        const int smem = warps * buckets * 128;
-        DYNB_CUDA_OK(cudaFuncSetAttribute(db_table_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        db_table_kernel<<<dim3(blocks, (heads + wide - 1) / wide), warps * 32, smem, s>>>(a, wide);
-        DYNB_CUDA_OK(cudaGetLastError());
-        const unsigned join = (unsigned)std::min<int64_t>(((int64_t)buckets * heads + DB_THREADS - 1) / DB_THREADS, 1024);
-        db_table_join_kernel<<<join, DB_THREADS, 0, s>>>(a, blocks);
+    }
+    const int warps = db_backward_warps(buckets, heads);
+    if (warps > 0) {
+        if (d_table_dev != nullptr || (d_dist_dev != nullptr && n > 0)) {
+            const cudaError_t e = heads <= 1 ? db_backward<1>(a, blocks, warps, s) : heads <= 2 ? db_backward<2>(a, blocks, warps, s)
+                                : heads <= 4 ? db_backward<4>(a, blocks, warps, s) : heads <= 8 ? db_backward<8>(a, blocks, warps, s)
+                                : heads <= 16 ? db_backward<16>(a, blocks, warps, s) : db_backward<32>(a, blocks, warps, s);
+            DYNB_CUDA_OK(e);
+        }
+    } else {
+        if (d_dist_dev != nullptr && n > 0) {
+            db_dist_kernel<<<db_blocks(n), DB_THREADS, 0, s>>>(a);
+            DYNB_CUDA_OK(cudaGetLastError());
+        }
+        if (d_table_dev != nullptr) {
+            int wide = 1;
+            while (wide < heads && wide < 32) wide *= 2;
+            // as many warps as have their copies in 128 KB, and no more than 16
+            const int table_warps = std::max(1, std::min(16, (128 << 10) / (buckets * 128)));
+            const int smem = table_warps * buckets * 128;
+            DYNB_CUDA_OK(cudaFuncSetAttribute(db_table_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            db_table_kernel<<<dim3(blocks, (heads + wide - 1) / wide), table_warps * 32, smem, s>>>(a, wide);
+            DYNB_CUDA_OK(cudaGetLastError());
+        }
+    }
+    if (d_table_dev != nullptr) {
+        db_table_join_kernel<<<(unsigned)(((int64_t)buckets * heads + 31) / 32), DB_THREADS, 0, s>>>(a, blocks);
         DYNB_CUDA_OK(cudaGetLastError());
     }
     return DYNB_OK;
