@@ -2,7 +2,7 @@
 //
 // y = x W + b and dx = dy W^T: a block keeps the whole matrix of a type for its columns in shared memory (laid out once per type) and takes
 // tiles of 128 rows one after the other: eight warps gather the rows into stages of 64 columns, one thread issues the products, four
-// warps take the sums out of tensor memory, which holds two of them, and store the rows.  What bounds it is the memory that the rows need.
+// warps take the sums out of tensor memory, which holds two of them, turn them in shared memory and store the rows by whole lines.  What bounds it is the memory that the rows need.
 //
 // dW = sum x_i^T dy_i: a block takes a stretch of rows of one type, 128 x up to 256 elements of the matrix; both operands are the gathered
 // rows as they are, read along their columns.  db is a product too, with a tile of ones.
@@ -22,21 +22,27 @@ constexpr int TM_FEED = 8;                  // warps that gather
 constexpr int TM_THREADS = (4 + 1 + TM_FEED) * 32;
 constexpr int TM_FEED_THREADS = TM_FEED * 32;
 constexpr int TM_MAX_STAGES = 8;
-constexpr int TM_SMEM = 225 * 1024;
+// Stages whose rows are on their way in registers: what keeps memory busy is bytes under way, 32 KB a stage of fp32, 16 KB of 16 bits.
+template <typename T> constexpr int TM_AHEAD = sizeof(T) == 4 ? 2 : 3;
+constexpr int TM_SMEM = 202 * 1024;        // beside 23 KB of offsets, results under way and barriers
 constexpr int TW_ROWS = 32;                 // rows of a stage of the weights' gradient
 
 template <typename T> struct TmParts { static constexpr int N = 1; };
 template <> struct TmParts<float> { static constexpr int N = 3; };
 template <typename T> struct TmRaw { uint4 v[sizeof(T) == 4 ? 2 : 1]; };   // 8 elements as loaded
 
-// Eight elements `step` apart from p, the first `have` of them real, zeros behind.  `wide`: 16-byte boundaries, step 1 and have 0 or 8.
-template <typename T>
-__device__ __forceinline__ TmRaw<T> tm_load(const T* p, int64_t step, int have, bool wide)
+// Eight elements `step` apart from p, the first `have` of them real, zeros behind.  WIDE: 16-byte boundaries, step 1 and have 0 or 8.  (Chosen
+// at run time, the two ways meet in copies of what was loaded, and each load is waited for before the next.)
+template <bool WIDE, typename T>
+__device__ __forceinline__ TmRaw<T> tm_load(const T* p, int64_t step, int have)
 {
     TmRaw<T> r;
-    if (wide) {
+    if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(r) / 16); i++) r.v[i] = have > 0 ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < (int)(sizeof(r) / 16); i++) {
+            r.v[i] = make_uint4(0, 0, 0, 0);
+            if (have > 0) r.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        }
         return r;
     }
     using W = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
@@ -59,27 +65,34 @@ __device__ __forceinline__ void tm_store(const TmRaw<T>& r, unsigned char* at, i
         for (int i = 0; i < 4; i++) {
             float v[2] = {__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1])};
 #pragma unroll
-            for (int p = 0; p < 3; p++) {
+            for (int p = 0; p < 2; p++) {
                 const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
                 const uint32_t w = *reinterpret_cast<const uint32_t*>(&b);
                 part[p][i] = w;
                 v[0] -= __uint_as_float(w << 16);          // exact
                 v[1] -= __uint_as_float(w & 0xffff0000u);
             }
+            part[2][i] = __byte_perm(__float_as_uint(v[0]), __float_as_uint(v[1]), 0x7632);   // eight bits at most are left
         }
 #pragma unroll
         for (int p = 0; p < 3; p++) *reinterpret_cast<uint4*>(at + p * apart) = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
     }
 }
 
-// The pairs of parts whose products are formed, the small ones first.
-template <int PARTS, typename F>
-__device__ __forceinline__ void tm_pairs(F f)
+// Adds the products of one step of 16 summed elements to d: the parts of `a` are `a_part` apart, those of `b` `b_part` (units of 16 bytes).  The
+// small products come first; a part of `a` stays at the multipliers for its products.
+template <int PARTS>
+__device__ __forceinline__ void tm_step(uint32_t d, uint64_t a, int a_part, uint64_t b, int b_part, uint32_t what, bool add)
 {
     if constexpr (PARTS == 1) {
-        f(0, 0);
+        tensor_mma(d, a, b, what, add);
     } else {
-        f(2, 0); f(0, 2); f(1, 1); f(1, 0); f(0, 1); f(0, 0);
+        tensor_mma(d, a + 2 * a_part, b, what, add);
+        tensor_mma_keep<1>(d, a + a_part, b + b_part, what, true);
+        tensor_mma_keep<3>(d, a + a_part, b, what, true);
+        tensor_mma_keep<1>(d, a, b + 2 * b_part, what, true);
+        tensor_mma_keep<2>(d, a, b + b_part, what, true);
+        tensor_mma_keep<3>(d, a, b, what, true);
     }
 }
 
@@ -114,7 +127,7 @@ struct TmCursor {
 };
 
 struct TmPlan {
-    int back, columns, column_stride, chunks, stages, tensor_columns, panel_bytes, wide_in, wide_w, store;   // store: bytes a store may have
+    int back, columns, column_stride, chunks, stages, tensor_columns, panel_bytes, b_chunk, b_part, b_step, wide_w, store;   // store: bytes of a store of results, 16 or one element
 };
 
 struct TmBars { uint64_t full[TM_MAX_STAGES], empty[TM_MAX_STAGES], panel_full, panel_free, sums_full[2], sums_free[2]; uint32_t tensor; };
@@ -127,52 +140,67 @@ __device__ __forceinline__ void tm_ran_out(const TlArgs& a)
     }
 }
 
-// `n` results of a row from column c on, in stores of `width` bytes (32, 16 or one element).
-template <typename T, int N>
-__device__ __forceinline__ void tm_put_row(T* at, const float (&v)[N], int n, int width)
+// Four results as words of the type.
+template <typename T>
+__device__ __forceinline__ void tm_words(const float (&v)[4], uint32_t* w)
 {
-    if (width >= 16 && n >= N) {
-        constexpr int WORDS = N * (int)sizeof(T) / 4;
-        uint32_t w[WORDS];
-        if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < N; i++) w[i] = __float_as_uint(v[i]);
-        } else {
+        for (int i = 0; i < 4; i++) w[i] = __float_as_uint(v[i]);
+    } else {
 #pragma unroll
-            for (int i = 0; i < WORDS; i++) {
-                if constexpr (std::is_same<T, __half>::value) {
-                    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-                } else {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&h);
-                }
+        for (int i = 0; i < 2; i++) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
             }
         }
-        if (width >= 32) {
+    }
+}
+
+// `n` sums of a row, in stores of 16 bytes or of one element.
+__device__ __forceinline__ void tm_put_row(float* at, const uint32_t (&v)[32], int n, bool wide)
+{
+    if (wide && n >= 32) {
 #pragma unroll
-            for (int i = 0; i < WORDS; i += 8)
-                asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(reinterpret_cast<char*>(at) + 4 * i), "r"(w[i]), "r"(w[i + 1]),
-                             "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
-                             : "memory");
-        } else {
-#pragma unroll
-            for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(reinterpret_cast<char*>(at) + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        }
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(at + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < N; i++)
-        if (i < n) tl_put(at + i, v[i]);
+    for (int i = 0; i < 32; i++)
+        if (i < n) at[i] = __uint_as_float(v[i]);
 }
 
-template <typename T>
+// The matrix of a type, its rows as they are.  y = x W reads them along columns: blocks of 64 columns by all summed rows.  dx = dy W^T reads them along
+// rows: blocks of 64 summed columns by all rows.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void tm_panel(const TmPlan& plan, const T* w, unsigned char* panel, int tid, int kk, int nn, int col0, int outer)
+{
+    const int across = plan.back ? plan.chunks * 8 : (plan.columns + 63) / 64 * 8, down = plan.back ? plan.columns : plan.chunks * 64;
+    const int row0 = plan.back ? col0 : 0, piece0 = plan.back ? 0 : col0;
+    const int rows = plan.back ? min(nn - col0, plan.columns) : kk, columns = plan.back ? kk : min(nn, col0 + plan.columns);
+    const int block = plan.back ? TmParts<T>::N * down * 128 : down * 128, apart = plan.b_part * 16;
+#pragma unroll 2
+    for (int u = tid; u < across * down; u += TM_FEED_THREADS) {
+        const int piece = u % across, r = u / across, c = piece0 + piece * 8;
+        const int have = r < rows ? min(8, columns - c) : 0;
+        const TmRaw<T> m = tm_load<WIDE>(have > 0 ? w + (int64_t)(row0 + r) * outer + c : w, 1, have);
+        tm_store(m, panel + (piece / 8) * block + tile_piece(r, piece & 7), apart);
+    }
+}
+
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(TM_THREADS, 1)
 tm_rows_kernel(const TlArgs a, const TmPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, STAGE = PARTS * TM_ROWS * 128;
+    constexpr int PARTS = TmParts<T>::N, STAGE = PARTS * TM_ROWS * 128, COLUMNS = 128 / (int)sizeof(T);
     extern __shared__ unsigned char raw_smem[];
     __shared__ TmBars bars;
+    __shared__ __align__(16) float offsets[4][256];
+    __shared__ __align__(16) unsigned char turned[4][32 * 144];
     unsigned char* const panel = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
     unsigned char* const stage0 = panel + plan.panel_bytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -210,30 +238,65 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
     if (warp < 4) {
         // sums to the rows
         const bool with_offset = !plan.back && a.b != nullptr;
-        int buffer = 0;
+        float* const offset = offsets[warp];
+        int buffer = 0, offset_type = -1;
         uint32_t phase = 0;
         for (; cursor.tile.type >= 0; cursor.next(a)) {
             const int64_t place = cursor.tile.begin + threadIdx.x;
-            int32_t r = place < cursor.tile.end ? a.order[place] : -1;
-            if ((uint32_t)r >= (uint64_t)a.n) r = -1;
+            int32_t r = place < cursor.tile.end ? __ldg(a.order + place) : -1;
+            const int have = min(plan.columns, nn - col0);
+            if (with_offset && cursor.tile.type != offset_type) {
+                offset_type = cursor.tile.type;
+                __syncwarp();
+                for (int c = lane; c < have; c += 32) offset[c] = tl_get(static_cast<const T*>(a.b) + (int64_t)offset_type * a.outer + col0 + c);
+                __syncwarp();
+            }
             if (!bar_wait(&bars.sums_full[buffer], phase)) { tm_ran_out(a); break; }
             tensor_fence_after();
-            const T* const offset = static_cast<const T*>(a.b) + (int64_t)cursor.tile.type * a.outer + col0;
-            const int have = min(plan.columns, nn - col0);
-            for (int c = 0; c < have; c += 32) {
-                uint32_t bits[32];
-                __syncwarp();
-                tensor_load_32(tensor + ((uint32_t)(warp * 32) << 16) + buffer * plan.column_stride + c, bits);
-                tensor_wait_loads();
-                float v[32];
+            if ((uint32_t)r >= (uint64_t)a.n) r = -1;
+            // 32 words of every row at a time: out of tensor memory by rows, through shared memory, to memory by pieces of 16 bytes of whole lines
+            const uint32_t from = tensor + ((uint32_t)(warp * 32) << 16) + buffer * plan.column_stride;
+            for (int c = 0; c < have; c += COLUMNS) {
+                uint32_t words[32];
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(bits[i]);
-                if (with_offset) {
+                for (int half = 0; half < COLUMNS / 32; half++) {
+                    uint32_t bits[32];
+                    __syncwarp();
+                    tensor_load_32(from + min(c + 32 * half, plan.column_stride - 32), bits);
+                    tensor_wait_loads();
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (c + i < have) v[i] += tl_get(offset + c + i);
+                    for (int i = 0; i < 32; i += 4) {
+                        float v[4] = {__uint_as_float(bits[i]), __uint_as_float(bits[i + 1]), __uint_as_float(bits[i + 2]), __uint_as_float(bits[i + 3])};
+                        if (with_offset) {   // behind `have`: not stored
+                            const float4 o = *reinterpret_cast<const float4*>(offset + min(c + 32 * half, 224) + i);
+                            v[0] += o.x; v[1] += o.y; v[2] += o.z; v[3] += o.w;
+                        }
+                        tm_words<T>(v, words + (COLUMNS / 32 == 1 ? i : 16 * half + i / 2));
+                    }
                 }
-                if (r >= 0) tm_put_row(out + (int64_t)r * nn + col0 + c, v, have - c, plan.store);
+                unsigned char* const mine = turned[warp];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; i++) *reinterpret_cast<uint4*>(mine + lane * 144 + 16 * i) = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+                __syncwarp();
+                constexpr int PER = 16 / (int)sizeof(T);
+                const int at = c + (lane & 7) * PER;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int row = 4 * j + (lane >> 3);
+                    const int32_t to = __shfl_sync(0xffffffffu, r, row);
+                    const uint4 piece = *reinterpret_cast<const uint4*>(mine + row * 144 + 16 * (lane & 7));
+                    if (to < 0 || at >= have) continue;
+                    T* const p = out + (int64_t)to * nn + col0 + at;
+                    if (plan.store == 16) {
+                        *reinterpret_cast<uint4*>(p) = piece;
+                    } else {
+                        const T* const e = reinterpret_cast<const T*>(&piece);
+#pragma unroll
+                        for (int i = 0; i < PER; i++)
+                            if (at + i < have) p[i] = e[i];
+                    }
+                }
             }
             tensor_fence_before();
             __syncwarp();
@@ -244,9 +307,9 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
     } else if (warp == 4) {
         // products
         const bool bf16 = !std::is_same<T, __half>::value;
-        const uint32_t what = mma_what(bf16, plan.columns, false, false);
-        const uint32_t panel_at = smem_addr(panel), stage_at = smem_addr(stage0);
-        const int part_bytes = plan.columns * 128;
+        const uint32_t what = mma_what(bf16, plan.columns, false, !plan.back);
+        const uint32_t stage_at = smem_addr(stage0);
+        const uint64_t panel_from = tile_descriptor(smem_addr(panel), plan.back ? 16 : plan.chunks * 8192, 1024);
         int stage = 0, buffer = 0, panel_type = -1;
         uint32_t phase = 0, panel_phase = 0, sums_phase = 1;
         bool ok = true;
@@ -264,15 +327,11 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
                 tensor_fence_after();
                 if (lane == 0) {
                     const int steps = min(4, (kk - chunk * 64 + 15) / 16);
-                    const uint32_t at_a = stage_at + stage * STAGE, at_b = panel_at + chunk * PARTS * part_bytes;
-                    bool add = chunk > 0;
-                    tm_pairs<PARTS>([&](int pa, int pb) {
-                        for (int k = 0; k < steps; k++) {
-                            tensor_mma(sums, tile_descriptor(at_a + pa * (TM_ROWS * 128) + k * 32, 16, 1024),
-                                       tile_descriptor(at_b + pb * part_bytes + k * 32, 16, 1024), what, add);
-                            add = true;
-                        }
-                    });
+                    // descriptors are in units of 16 bytes: steps and parts are additions
+                    const uint64_t at_a = tile_descriptor(stage_at + stage * STAGE, 16, 1024), at_b = panel_from + (uint32_t)(chunk * plan.b_chunk);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (k < steps) tm_step<PARTS>(sums, at_a + 2 * k, TM_ROWS * 128 / 16, at_b + (uint32_t)(k * plan.b_step), plan.b_part, what, chunk > 0 || k > 0);
                     tensor_commit(&bars.empty[stage]);
                     if (chunk == plan.chunks - 1) tensor_commit(&bars.sums_full[buffer]);
                 }
@@ -288,74 +347,74 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
         }
         if (!ok) tm_ran_out(a);
     } else {
-        // rows and matrices to shared memory
+        // rows and matrices to shared memory: stages are asked for AHEAD of their turn
+        constexpr int AHEAD = TM_AHEAD<T>, UNITS = TM_ROWS * 8 / TM_FEED_THREADS;
         const int tid = threadIdx.x - 5 * 32, piece = tid & 7;
         int panel_type = -1, stage = 0, chunk = 0;
         uint32_t phase = 1, free_phase = 0;
-        TlTile now = cursor.tile;
-        int32_t rows[4], rows_next[4];
-        auto rows_of = [&](const TlTile& t, int32_t (&r)[4]) {
+        TlTile next = cursor.tile;                  // of the next stage to ask for
+        int32_t rows[UNITS], rows_next[UNITS];      // of that tile and the one behind it
+        auto rows_of = [&](const TlTile& t, int32_t (&r)[UNITS]) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t place = t.begin + (tid >> 3) + 32 * i;
-                r[i] = t.type >= 0 && place < t.end ? a.order[place] : -1;
-                if ((uint32_t)r[i] >= (uint64_t)a.n) r[i] = -1;
+            for (int i = 0; i < UNITS; i++) {
+                const int64_t place = t.begin + (tid >> 3) + (TM_FEED_THREADS / 8) * i;
+                r[i] = t.type >= 0 && place < t.end ? __ldg(a.order + place) : -1;   // looked at a tile later
             }
         };
-        auto fetch = [&](const int32_t (&r)[4], int ch, TmRaw<T> (&v)[4]) {
-            const int k = ch * 64 + piece * 8, have = min(8, kk - k);
+        TmRaw<T> v[AHEAD][UNITS];
+        int type_of[AHEAD];
+        auto ask = [&](TmRaw<T> (&to)[UNITS], int& type) {
+            type = next.type;
+            if (next.type < 0) return;
+            const int k = chunk * 64 + piece * 8, have = min(8, kk - k);
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = tm_load(in + (r[i] >= 0 ? r[i] * in_row + k : 0), 1, r[i] >= 0 ? have : 0, plan.wide_in != 0);
-        };
-        TmRaw<T> v[4], v_next[4];
-        rows_of(now, rows);
-        if (now.type >= 0) {
-            fetch(rows, 0, v);
-            cursor.next(a);
-            rows_of(cursor.tile, rows_next);
-        }
-        while (now.type >= 0) {
-            const bool last = chunk + 1 == plan.chunks;
-            if (!last) fetch(rows, chunk + 1, v_next);
-            else if (cursor.tile.type >= 0) fetch(rows_next, 0, v_next);
-            if (now.type != panel_type) {
-                if (panel_type >= 0) {
-                    if (!bar_wait(&bars.panel_free, free_phase)) { tm_ran_out(a); break; }
-                    free_phase ^= 1;
-                }
-                panel_type = now.type;
-                const T* const w = static_cast<const T*>(a.w) + (int64_t)now.type * a.inner * a.outer;
-                const int units = plan.chunks * 8 * plan.columns;
-                for (int u = tid; u < units; u += TM_FEED_THREADS) {
-                    const int n = u % plan.columns, k8 = u / plan.columns, k = k8 * 8;
-                    const int have = col0 + n < nn ? min(8, kk - k) : 0;
-                    const T* const p = have <= 0 ? w : plan.back ? w + (int64_t)(col0 + n) * a.outer + k : w + (int64_t)k * a.outer + col0 + n;
-                    const TmRaw<T> m = tm_load(p, plan.back ? 1 : a.outer, have, plan.back && plan.wide_w != 0);
-                    tm_store(m, panel + (int64_t)(k8 / 8) * PARTS * plan.columns * 128 + tile_piece(n, k8 & 7), plan.columns * 128);
-                }
-                fence_to_tensor();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.panel_full);
+            for (int i = 0; i < UNITS; i++) {
+                const bool ok = (uint32_t)rows[i] < (uint64_t)a.n;
+                to[i] = tm_load<WIDE>(in + (ok ? rows[i] * in_row + k : 0), 1, ok ? have : 0);
             }
-            if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
-#pragma unroll
-            for (int i = 0; i < 4; i++) tm_store(v[i], stage0 + stage * STAGE + tile_piece((tid >> 3) + 32 * i, piece), TM_ROWS * 128);
-            fence_to_tensor();
-            __syncwarp();
-            if (lane == 0) bar_arrive(&bars.full[stage]);
-            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = v_next[i];
-            chunk++;
-            if (last) {
+            if (++chunk == plan.chunks) {
                 chunk = 0;
-                now = cursor.tile;
+                next = cursor.tile;
 #pragma unroll
-                for (int i = 0; i < 4; i++) rows[i] = rows_next[i];
-                if (now.type >= 0) {
+                for (int i = 0; i < UNITS; i++) rows[i] = rows_next[i];
+                if (next.type >= 0) {
                     cursor.next(a);
                     rows_of(cursor.tile, rows_next);
                 }
+            }
+        };
+        rows_of(next, rows);
+        if (next.type >= 0) cursor.next(a);
+        rows_of(cursor.tile, rows_next);
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) ask(v[s], type_of[s]);
+        bool more = true;
+        while (more) {
+#pragma unroll
+            for (int s = 0; s < AHEAD; s++) {
+                if (type_of[s] < 0) { more = false; break; }
+                if (type_of[s] != panel_type) {
+                    if (panel_type >= 0) {
+                        if (!bar_wait(&bars.panel_free, free_phase)) { tm_ran_out(a); more = false; break; }
+                        free_phase ^= 1;
+                    }
+                    panel_type = type_of[s];
+                    const T* const w = static_cast<const T*>(a.w) + (int64_t)panel_type * a.inner * a.outer;
+                    if (plan.wide_w) tm_panel<T, true>(plan, w, panel, tid, kk, nn, col0, a.outer);
+                    else tm_panel<T, false>(plan, w, panel, tid, kk, nn, col0, a.outer);
+                    fence_to_tensor();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&bars.panel_full);
+                }
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
+#pragma unroll
+                for (int i = 0; i < UNITS; i++)
+                    tm_store(v[s][i], stage0 + stage * STAGE + tile_piece((tid >> 3) + (TM_FEED_THREADS / 8) * i, piece), TM_ROWS * 128);
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[stage]);
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                ask(v[s], type_of[s]);
             }
         }
     }
@@ -365,14 +424,15 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
     if (warp == 0) tensor_free(tensor, plan.tensor_columns);
 }
 
-struct TwPlan { int columns, column_stride, x_blocks, y_blocks, stages, tensor_columns, wide_x, wide_y, vec; };
+struct TwPlan { int columns, column_stride, x_blocks, y_blocks, stages, tensor_columns, vec; };
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(TM_THREADS, 1)
 tm_weights_kernel(const TlArgs a, const TwPlan plan)
 {
     constexpr int PARTS = TmParts<T>::N, BLOCK = TW_ROWS * 128;
     constexpr int UNITS = PARTS == 1 ? 6 : 4;   // pieces of 8 elements a thread and stage: 32 rows x (128 + 256 or 128) elements
+    constexpr int AHEAD = TM_AHEAD<T>;
     extern __shared__ unsigned char raw_smem[];
     __shared__ TmBars bars;
     unsigned char* const ones = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
@@ -418,17 +478,15 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
                     __syncwarp();
                     tensor_load_32(tensor + ((uint32_t)(warp * 32) << 16) + which * plan.column_stride + c, bits);
                     tensor_wait_loads();
-                    float v[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(bits[i]);
-                    if (write) tm_put_row(at + c, v, have - c, plan.vec);
+                    if (write) tm_put_row(at + c, bits, have - c, plan.vec != 0);
                 }
             }
         }
     } else if (warp == 4) {
         const bool bf16 = !std::is_same<T, __half>::value;
         const uint32_t what = mma_what(bf16, plan.columns, true, true), what_sum = mma_what(bf16, plan.columns, false, true);
-        const uint32_t stage_at = smem_addr(stage0), ones_at = smem_addr(ones);
+        const uint32_t stage_at = smem_addr(stage0);
+        const uint64_t ones_desc = tile_descriptor(smem_addr(ones), 16, 1024);
         const uint32_t lead = PARTS * BLOCK, lead_x = plan.x_blocks > 1 ? lead : 0;   // one block: the upper 64 rows repeat the lower
         int stage = 0;
         uint32_t phase = 0;
@@ -437,26 +495,19 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
             if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
             tensor_fence_after();
             if (lane == 0) {
-                const uint32_t at_x = stage_at + stage * stage_bytes, at_y = at_x + plan.x_blocks * PARTS * BLOCK;
-                bool add = step > 0;
-                tm_pairs<PARTS>([&](int pa, int pb) {
+                const uint32_t at = stage_at + stage * stage_bytes;
+                const uint64_t at_x = tile_descriptor(at, lead_x, 1024), at_y = tile_descriptor(at + plan.x_blocks * PARTS * BLOCK, lead, 1024);
 #pragma unroll
-                    for (int k = 0; k < TW_ROWS / 16; k++) {
-                        tensor_mma(tensor, tile_descriptor(at_x + pa * BLOCK + k * 2048, lead_x, 1024), tile_descriptor(at_y + pb * BLOCK + k * 2048, lead, 1024),
-                                   what, add);
+                for (int k = 0; k < TW_ROWS / 16; k++) tm_step<PARTS>(tensor, at_x + k * 128, BLOCK / 16, at_y + k * 128, BLOCK / 16, what, step > 0 || k > 0);
+                if (sums_wanted) {
+                    bool add = step > 0;
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; p--) {
+#pragma unroll
+                        for (int k = 0; k < TW_ROWS / 16; k++)
+                            tensor_mma(tensor + plan.column_stride, ones_desc, at_y + (p * BLOCK + k * 2048) / 16, what_sum, add || k > 0);
                         add = true;
                     }
-                });
-                if (sums_wanted) {
-                    add = step > 0;
-#pragma unroll
-                    for (int p = PARTS - 1; p >= 0; p--)
-#pragma unroll
-                        for (int k = 0; k < TW_ROWS / 16; k++) {
-                            tensor_mma(tensor + plan.column_stride, tile_descriptor(ones_at, 16, 1024), tile_descriptor(at_y + p * BLOCK + k * 2048, lead, 1024),
-                                       what_sum, add);
-                            add = true;
-                        }
                 }
                 tensor_commit(&bars.empty[stage]);
                 if (step == steps - 1) tensor_commit(&bars.sums_full[0]);
@@ -485,8 +536,7 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
 #pragma unroll
             for (int i = 0; i < UNITS; i++) {
                 const int64_t place = tile.begin + (int64_t)step * TW_ROWS + row[i];
-                r[i] = row[i] >= 0 && col[i] >= 0 && place < tile.end ? a.order[place] : -1;
-                if ((uint32_t)r[i] >= (uint64_t)a.n) r[i] = -1;
+                r[i] = row[i] >= 0 && col[i] >= 0 && place < tile.end ? __ldg(a.order + place) : -1;   // looked at a stage later
             }
         };
         auto fetch = [&](const int32_t (&r)[UNITS], TmRaw<T> (&v)[UNITS]) {
@@ -495,31 +545,38 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
                 const bool of_y = (col[i] >> 30) & 1;
                 const int c = col[i] & ((1 << 30) - 1);
                 const T* const p = of_y ? static_cast<const T*>(a.dy) + r[i] * a.dy_row + c : static_cast<const T*>(a.x) + r[i] * a.x_row + c;
-                v[i] = tm_load(r[i] >= 0 ? p : static_cast<const T*>(a.x), 1, r[i] >= 0 ? min(8, (of_y ? a.outer : a.inner) - c) : 0,
-                               of_y ? plan.wide_y != 0 : plan.wide_x != 0);
+                const bool ok = (uint32_t)r[i] < (uint64_t)a.n;
+                v[i] = tm_load<WIDE>(ok ? p : static_cast<const T*>(a.x), 1, ok ? min(8, (of_y ? a.outer : a.inner) - c) : 0);
             }
         };
-        // numbers of rows two stages ahead, rows one
+        // rows AHEAD stages ahead, their numbers one more
         int32_t ids[UNITS];
-        TmRaw<T> v[UNITS], v_next[UNITS];
+        TmRaw<T> v[AHEAD][UNITS];
         rows_of(0, ids);
-        fetch(ids, v);
-        rows_of(1, ids);
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) {
+            fetch(ids, v[s]);            // behind the stretch: zeros
+            rows_of(s + 1, ids);
+        }
         int stage = 0;
         uint32_t phase = 1;
-        for (int step = 0; step < steps; step++) {
-            fetch(ids, v_next);   // behind the stretch: zeros
-            rows_of(step + 2, ids);
-            if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+        bool more = true;
+        for (int step = 0; more && step < steps;) {
 #pragma unroll
-            for (int i = 0; i < UNITS; i++) {
-                if (row[i] >= 0) tm_store(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
-                v[i] = v_next[i];
+            for (int s = 0; s < AHEAD; s++) {
+                if (step >= steps) break;
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
+#pragma unroll
+                for (int i = 0; i < UNITS; i++)
+                    if (row[i] >= 0) tm_store(v[s][i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[stage]);
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                step++;
+                fetch(ids, v[s]);
+                rows_of(step + AHEAD, ids);
             }
-            fence_to_tensor();
-            __syncwarp();
-            if (lane == 0) bar_arrive(&bars.full[stage]);
-            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
         }
     }
     tensor_fence_before();
@@ -549,26 +606,29 @@ static bool tm_rows(const TlArgs& a, int back, cudaStream_t s, cudaError_t* rc)
     int tiles = 1;
     for (;; tiles++) {
         p.columns = tm_round((nn + tiles - 1) / tiles, 16);
-        p.panel_bytes = p.chunks * PARTS * p.columns * 128;
+        p.panel_bytes = back ? p.chunks * PARTS * p.columns * 128 : PARTS * ((p.columns + 63) / 64) * p.chunks * 8192;
         if (p.columns <= 256 && p.panel_bytes + 2 * STAGE + 1024 <= TM_SMEM) break;
         if (p.columns == 16) return false;
     }
     tiles = (nn + p.columns - 1) / p.columns;
-    p.panel_bytes = tm_round(p.panel_bytes, 1024);
+    p.b_part = (back ? p.columns * 128 : p.panel_bytes / PARTS) / 16;
+    p.b_chunk = (back ? PARTS * p.columns * 128 : 8192) / 16;
+    p.b_step = (back ? 32 : 2048) / 16;
     p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - p.panel_bytes) / STAGE);
     p.column_stride = tm_round(p.columns, 32);
     p.tensor_columns = tm_tensor_columns(2 * p.column_stride);
     const void* const in = back ? a.dy : a.x;
     const void* const out = back ? a.dx : a.y;
-    p.wide_in = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0;
-    p.wide_w = tm_on(a.w, a.outer, SIZE, 16) && kk % 8 == 0;
-    p.store = tm_on(out, nn, SIZE, 32) && p.columns * SIZE % 32 == 0 ? 32 : tm_on(out, nn, SIZE, 16) && p.columns * SIZE % 16 == 0 ? 16 : SIZE;
+    const bool wide = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0;
+    p.wide_w = tm_on(a.w, a.outer, SIZE, 16) && a.outer % 8 == 0;
+    p.store = tm_on(out, nn, SIZE, 16) && nn * SIZE % 16 == 0 ? 16 : SIZE;
     const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
     const int smem = 1024 + p.panel_bytes + p.stages * STAGE;
-    *rc = cudaFuncSetAttribute(tm_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    void (*const kernel)(TlArgs, TmPlan) = wide ? tm_rows_kernel<T, true> : tm_rows_kernel<T, false>;
+    *rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (*rc != cudaSuccess) return true;
-    tm_rows_kernel<T><<<grid, TM_THREADS, smem, s>>>(a, p);
+    kernel<<<grid, TM_THREADS, smem, s>>>(a, p);
     *rc = cudaGetLastError();
     return true;
 }
@@ -593,14 +653,14 @@ static cudaError_t tm_weights(const TlArgs& a, cudaStream_t s)
     const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
     p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - TM_ROWS * 128) / stage);
     p.tensor_columns = tm_tensor_columns(2 * p.column_stride);
-    p.wide_x = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0;
-    p.wide_y = tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
-    p.vec = a.outer % 4 == 0 ? 16 : 4;
+    const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
+    p.vec = a.outer % 4 == 0;
     const dim3 grid((unsigned)tl_stretches(a.n, a.types, a.stretch), (a.inner + TM_ROWS - 1) / TM_ROWS, (a.outer + p.columns - 1) / p.columns);
     const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;
-    const cudaError_t rc = cudaFuncSetAttribute(tm_weights_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    void (*const kernel)(TlArgs, TwPlan) = wide ? tm_weights_kernel<T, true> : tm_weights_kernel<T, false>;
+    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    tm_weights_kernel<T><<<grid, TM_THREADS, smem, s>>>(a, p);
+    kernel<<<grid, TM_THREADS, smem, s>>>(a, p);
     return cudaGetLastError();
 }
 

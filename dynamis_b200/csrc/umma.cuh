@@ -87,6 +87,24 @@ __device__ __forceinline__ void tensor_mma(uint32_t d, uint64_t a, uint64_t b, u
         "r"(what), "r"((uint32_t)add)
         : "memory");
 }
+// The same, keeping the tile of `a` at the multipliers for the next product with it (KEEP 1: from shared memory, 2: kept before, 3: kept before
+// and not after).
+template <int KEEP>
+__device__ __forceinline__ void tensor_mma_keep(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add)
+{
+    if constexpr (KEEP == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                     "l"(b), "r"(what), "r"((uint32_t)add)
+                     : "memory");
+    else if constexpr (KEEP == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16.collector::a::use [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                     "l"(b), "r"(what), "r"((uint32_t)add)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                     "l"(b), "r"(what), "r"((uint32_t)add)
+                     : "memory");
+}
 // The barrier gets one arrival when all products issued so far by this thread are done.
 __device__ __forceinline__ void tensor_commit(uint64_t* bar)
 {
