@@ -163,8 +163,8 @@ SIGNATURES = {
     "dynb_kdtree_workspace_bytes": (_i32, [_i64, _i64, ctypes.POINTER(_i64)]),
     "dynb_kdtree_partition": (_i32, [_p, _i64, _p, _i64, _p, _i32, _p, _i64, _p]),
     "dynb_integrator_step": (_i32, [_i32, _p, _p, _p, _p, _p, _i64, _f64, _f64, _f64, _p, _p, _f64, _p, _p, _p]),
-    "dynb_neighbor_index_workspace_bytes": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
-    "dynb_neighbor_index_plan": (_i32, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dynb_neighbor_index_workspace_bytes": (_i32, [_i64, _i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "dynb_neighbor_index_plan": (_i32, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "dynb_neighbor_index_fill": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p]),
     "dynb_neighbor_attention": (_i32, [_p, _p, _p, _p, _p]),
     "dynb_neighbor_attention_backward": (_i32, [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),

@@ -37,6 +37,7 @@ MAX_BUCKETS = 1024       # DYNB_DISTANCE_BIAS_MAX_BUCKETS
 MAX_BIAS_HEADS = 1024    # DYNB_DISTANCE_BIAS_MAX_HEADS
 MAX_TYPES = 4096         # DYNB_TYPE_LINEAR_MAX_TYPES
 MAX_WIDTH = 16384        # DYNB_TYPE_LINEAR_MAX_WIDTH
+LONGEST_LIST = 256       # NI_LONGEST (csrc/neighbors.cu): longer lists take a larger workspace
 INT32_MAX = 2 ** 31 - 1
 MAX_EDGES = 2 ** 31 - 2 ** 16   # DYNB_MAX_EDGES
 
@@ -145,22 +146,28 @@ def neighbor_index(edge_index: torch.Tensor, num_targets: int, num_sources: int)
         rows, row_start, src, cols, col_start, in_edge, in_dst = (
             torch.empty(n, dtype=torch.int32, device=dev) for n in (T, T + 1, E, S, S + 1, E, E))
         nbytes = ctypes.c_int64()
-        _lib.check(L.dynb_neighbor_index_workspace_bytes(E, T, S, ctypes.byref(nbytes)), "neighbor_index_workspace_bytes")
+        _lib.check(L.dynb_neighbor_index_workspace_bytes(E, T, S, 0, ctypes.byref(nbytes)), "neighbor_index_workspace_bytes")
         ws = scratch(dev, "neighbor_index", nbytes.value)
         words = take_host_words(2)
         try:
             _lib.check(L.dynb_neighbor_index_plan(src64, dst64, E, T, S, rows.data_ptr(), row_start.data_ptr(), src.data_ptr(), cols.data_ptr(),
-                                                  col_start.data_ptr(), words.data_ptr(), ws.data_ptr(), ws.numel(), stream), "neighbor_index_plan")
+                                                  col_start.data_ptr(), in_edge.data_ptr(), words.data_ptr(), ws.data_ptr(), ws.numel(), stream), "neighbor_index_plan")
             torch.cuda.current_stream(dev).synchronize()
         except BaseException:
             lose_host_words(words, dev)
             raise
-        status, longest = int(words[0]), int(words[1])
+        word = int(words[0])
+        status, longest = word & 0xFFFFFFFF, (word >> 32) & 0xFFFFFFFF
         give_host_words(words)
         if status & 1:
             raise RuntimeError(f"neighbor_index: an edge has a target outside [0, {T}) or a source outside [0, {S})")
         if status & 2:
             raise RuntimeError("neighbor_index: the edges of a target must stand behind one another")
+        if longest > LONGEST_LIST:
+            planned, ws = ws[:nbytes.value], None
+            _lib.check(L.dynb_neighbor_index_workspace_bytes(E, T, S, longest, ctypes.byref(nbytes)), "neighbor_index_workspace_bytes")
+            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+            _lib.check(L.dynb_copy_async(ws.data_ptr(), planned.data_ptr(), planned.numel(), stream), "copy_async")
         _lib.check(L.dynb_neighbor_index_fill(dst64, E, T, S, src.data_ptr(), col_start.data_ptr(), longest, in_edge.data_ptr(), in_dst.data_ptr(),
                                               ws.data_ptr(), ws.numel(), stream), "neighbor_index_fill")
     return NeighborIndex(rows, row_start, src, cols, col_start, in_edge, in_dst)

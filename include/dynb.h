@@ -441,14 +441,16 @@ int dynb_integrator_step(int kind, float* pos_dev, float* vel_dev, const float* 
  *   cols[n_sources]        sources in the order of their first edge, then those without edges, ascending
  *   col_start[n_sources+1], in_edge[n_edges], in_dst[n_edges]
  *                          edges that leave cols[c], in ascending order, and their targets
- * Two phases: the plan writes rows, row_start, src32, cols and col_start, and two words to pinned host memory: word 0 has bit 0 set
- * when an endpoint is out of range and bit 1 when the edges of a target are apart (nothing else is valid then), word 1 is the longest
- * list of a source.  The caller waits for the stream and calls the fill with word 1 and the workspace of the plan. */
+ * Two phases: the plan writes rows, row_start, src32, cols and col_start (in_edge: scratch that the fill reads), and 16 bytes to pinned host
+ * memory, four 32-bit words: word 0 has bit 0 set when an endpoint is out of range and bit 1 when the edges of a target are apart
+ * (nothing else is valid then), word 1 is the longest list of a source.  The caller waits for the stream and calls the fill with word 1 and
+ * the workspace of the plan.  The workspace for a longest list of 0 does for the plan and for lists of up to 256 edges; for longer ones the fill
+ * takes a larger one, which begins with the bytes of the plan's. */
 #define DYNB_MAX_EDGES ((1ll << 31) - (1ll << 16))
-int dynb_neighbor_index_workspace_bytes(int64_t n_edges, int64_t n_targets, int64_t n_sources, int64_t* bytes);
+int dynb_neighbor_index_workspace_bytes(int64_t n_edges, int64_t n_targets, int64_t n_sources, int64_t longest, int64_t* bytes);
 int dynb_neighbor_index_plan(const int64_t* src_dev, const int64_t* dst_dev, int64_t n_edges, int64_t n_targets, int64_t n_sources,
                              int32_t* rows_dev, int32_t* row_start_dev, int32_t* src32_dev, int32_t* cols_dev, int32_t* col_start_dev,
-                             int64_t* words_host, void* workspace_dev, int64_t workspace_bytes, void* stream);
+                             int32_t* in_edge_dev, int64_t* words_host, void* workspace_dev, int64_t workspace_bytes, void* stream);
 int dynb_neighbor_index_fill(const int64_t* dst_dev, int64_t n_edges, int64_t n_targets, int64_t n_sources, const int32_t* src32_dev,
                              const int32_t* col_start_dev, int64_t longest, int32_t* in_edge_dev, int32_t* in_dst_dev, void* workspace_dev,
                              int64_t workspace_bytes, void* stream);

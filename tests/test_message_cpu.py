@@ -58,10 +58,10 @@ def test_empty_calls_launch_nothing():
 
 def test_other_entries_refuse():
     L, n = _lib.lib(), ctypes.c_int64()
-    assert L.dynb_neighbor_index_workspace_bytes(-1, 2, 2, ctypes.byref(n)) == -1
-    assert L.dynb_neighbor_index_workspace_bytes(2 ** 31, 2, 2, ctypes.byref(n)) == -1
-    assert L.dynb_neighbor_index_workspace_bytes(1000, 20, 20, ctypes.byref(n)) == 0 and n.value >= 8000
-    assert L.dynb_neighbor_index_plan(None, None, 5, 2, 2, None, None, None, None, None, None, None, 0, None) == -1
+    assert L.dynb_neighbor_index_workspace_bytes(-1, 2, 2, 0, ctypes.byref(n)) == -1
+    assert L.dynb_neighbor_index_workspace_bytes(2 ** 31, 2, 2, 0, ctypes.byref(n)) == -1
+    assert L.dynb_neighbor_index_workspace_bytes(1000, 20, 20, 0, ctypes.byref(n)) == 0 and n.value >= 8000
+    assert L.dynb_neighbor_index_plan(None, None, 5, 2, 2, None, None, None, None, None, None, None, None, 0, None) == -1
     assert L.dynb_neighbor_index_fill(None, 5, 2, 2, None, None, 3, None, None, None, 0, None) == -1
     for buckets, heads, cutoff in ((3, 4, 5.0), (1025, 4, 5.0), (8, 0, 5.0), (8, 1025, 5.0), (8, 4, 0.0), (8, 4, math.nan), (8, 4, math.inf)):
         assert L.dynb_distance_bias(None, 3, None, buckets, heads, cutoff, 1, None, None) == -1
