@@ -1,7 +1,7 @@
 // The products by type on the tensor cores.
 //
 // y = x W + b and dx = dy W^T: a block keeps the whole matrix of a type for its columns in shared memory (laid out once per type) and takes
-// tiles of 128 rows one after the other: eight warps gather the rows into stages of 64 columns, one thread issues the products, four
+// tiles of 128 rows one after the other: eight or sixteen warps gather the rows into stages of 64 columns, one thread issues the products, four
 // warps take the sums out of tensor memory, which holds two of them, turn them in shared memory and store the rows by whole lines.  What bounds it is the memory that the rows need.
 //
 // dW = sum x_i^T dy_i: a block takes a stretch of rows of one type, 128 x up to 256 elements of the matrix; both operands are the gathered
@@ -18,12 +18,13 @@
 namespace dynb {
 
 constexpr int TM_ROWS = 128;
-constexpr int TM_FEED = 8;                  // warps that gather
-constexpr int TM_THREADS = (4 + 1 + TM_FEED) * 32;
-constexpr int TM_FEED_THREADS = TM_FEED * 32;
+// Warps that gather, and stages whose rows are on their way in their registers beside the one that is being stored.  Sixteen warps are ahead of one
+// another; rows in fp32 need the registers of eight (1 M rows 128 x 128, both passes: 519 us, sixteen 543; the weights' gradient 308 and 284).
+template <typename T> constexpr int TM_FEED = sizeof(T) == 4 ? 8 : 16;
+template <typename T> constexpr int TM_AHEAD = sizeof(T) == 4 ? 2 : 1;
+constexpr int TW_FEED = 16;
+__host__ __device__ constexpr int tm_threads(int feed) { return (4 + 1 + feed) * 32; }
 constexpr int TM_MAX_STAGES = 8;
-// Stages whose rows are on their way in registers: what keeps memory busy is bytes under way, 32 KB a stage of fp32, 16 KB of 16 bits.
-template <typename T> constexpr int TM_AHEAD = sizeof(T) == 4 ? 2 : 3;
 constexpr int TM_SMEM = 202 * 1024;        // beside 23 KB of offsets, results under way and barriers
 constexpr int TW_ROWS = 32;                 // rows of a stage of the weights' gradient
 
@@ -183,8 +184,9 @@ __device__ __forceinline__ void tm_panel(const TmPlan& plan, const T* w, unsigne
     const int row0 = plan.back ? col0 : 0, piece0 = plan.back ? 0 : col0;
     const int rows = plan.back ? min(nn - col0, plan.columns) : kk, columns = plan.back ? kk : min(nn, col0 + plan.columns);
     const int block = plan.back ? TmParts<T>::N * down * 128 : down * 128, apart = plan.b_part * 16;
-#pragma unroll 2
-    for (int u = tid; u < across * down; u += TM_FEED_THREADS) {
+    constexpr int threads = TM_FEED<T> * 32;
+#pragma unroll (sizeof(T) == 4 ? 1 : 8)
+    for (int u = tid; u < across * down; u += threads) {
         const int piece = u % across, r = u / across, c = piece0 + piece * 8;
         const int have = r < rows ? min(8, columns - c) : 0;
         const TmRaw<T> m = tm_load<WIDE>(have > 0 ? w + (int64_t)(row0 + r) * outer + c : w, 1, have);
@@ -193,10 +195,10 @@ __device__ __forceinline__ void tm_panel(const TmPlan& plan, const T* w, unsigne
 }
 
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(TM_THREADS, 1)
+__global__ void __launch_bounds__(tm_threads(TM_FEED<T>), 1)
 tm_rows_kernel(const TlArgs a, const TmPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, STAGE = PARTS * TM_ROWS * 128, COLUMNS = 128 / (int)sizeof(T);
+    constexpr int FEED = TM_FEED<T>, FEED_THREADS = FEED * 32, PARTS = TmParts<T>::N, STAGE = PARTS * TM_ROWS * 128, COLUMNS = 128 / (int)sizeof(T);
     extern __shared__ unsigned char raw_smem[];
     __shared__ TmBars bars;
     __shared__ __align__(16) float offsets[4][256];
@@ -212,10 +214,10 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], TM_FEED);
+            bar_init(&bars.full[s], FEED);
             bar_init(&bars.empty[s], 1);
         }
-        bar_init(&bars.panel_full, TM_FEED);
+        bar_init(&bars.panel_full, FEED);
         bar_init(&bars.panel_free, 1);
         for (int b = 0; b < 2; b++) {
             bar_init(&bars.sums_full[b], 1);
@@ -348,7 +350,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
         if (!ok) tm_ran_out(a);
     } else {
         // rows and matrices to shared memory: stages are asked for AHEAD of their turn
-        constexpr int AHEAD = TM_AHEAD<T>, UNITS = TM_ROWS * 8 / TM_FEED_THREADS;
+        constexpr int AHEAD = TM_AHEAD<T>, UNITS = TM_ROWS * 8 / FEED_THREADS;
         const int tid = threadIdx.x - 5 * 32, piece = tid & 7;
         int panel_type = -1, stage = 0, chunk = 0;
         uint32_t phase = 1, free_phase = 0;
@@ -357,7 +359,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
         auto rows_of = [&](const TlTile& t, int32_t (&r)[UNITS]) {
 #pragma unroll
             for (int i = 0; i < UNITS; i++) {
-                const int64_t place = t.begin + (tid >> 3) + (TM_FEED_THREADS / 8) * i;
+                const int64_t place = t.begin + (tid >> 3) + (FEED_THREADS / 8) * i;
                 r[i] = t.type >= 0 && place < t.end ? __ldg(a.order + place) : -1;   // looked at a tile later
             }
         };
@@ -409,7 +411,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
 #pragma unroll
                 for (int i = 0; i < UNITS; i++)
-                    tm_store(v[s][i], stage0 + stage * STAGE + tile_piece((tid >> 3) + (TM_FEED_THREADS / 8) * i, piece), TM_ROWS * 128);
+                    tm_store(v[s][i], stage0 + stage * STAGE + tile_piece((tid >> 3) + (FEED_THREADS / 8) * i, piece), TM_ROWS * 128);
                 fence_to_tensor();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bars.full[stage]);
@@ -427,12 +429,11 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
 struct TwPlan { int columns, column_stride, x_blocks, y_blocks, stages, tensor_columns, vec; };
 
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(TM_THREADS, 1)
+__global__ void __launch_bounds__(tm_threads(TW_FEED), 1)
 tm_weights_kernel(const TlArgs a, const TwPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, BLOCK = TW_ROWS * 128;
-    constexpr int UNITS = PARTS == 1 ? 6 : 4;   // pieces of 8 elements a thread and stage: 32 rows x (128 + 256 or 128) elements
-    constexpr int AHEAD = TM_AHEAD<T>;
+    constexpr int FEED = TW_FEED, FEED_THREADS = FEED * 32, PARTS = TmParts<T>::N, BLOCK = TW_ROWS * 128;
+    constexpr int UNITS = PARTS == 1 ? 3 : 2;   // pieces of 8 elements a thread and stage: 32 rows x (128 + 256 or 128) elements
     extern __shared__ unsigned char raw_smem[];
     __shared__ TmBars bars;
     unsigned char* const ones = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
@@ -447,14 +448,14 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], TM_FEED);
+            bar_init(&bars.full[s], FEED);
             bar_init(&bars.empty[s], 1);
         }
         bar_init(&bars.sums_full[0], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     const uint32_t one = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
-    for (int i = threadIdx.x; i < TM_ROWS * 8; i += TM_THREADS) reinterpret_cast<uint4*>(ones)[i] = make_uint4(one, one, one, one);
+    for (int i = threadIdx.x; i < TM_ROWS * 8; i += tm_threads(FEED)) reinterpret_cast<uint4*>(ones)[i] = make_uint4(one, one, one, one);
     fence_to_tensor();
     if (warp == 0) tensor_alloc(&bars.tensor, plan.tensor_columns);
     tensor_fence_before();
@@ -523,7 +524,7 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
         int row[UNITS], at[UNITS], col[UNITS];
 #pragma unroll
         for (int i = 0; i < UNITS; i++) {
-            const int u = tid + i * TM_FEED_THREADS, r = u / per_row, piece = u % per_row;
+            const int u = tid + i * FEED_THREADS, r = u / per_row, piece = u % per_row;
             const int block = piece >> 3;
             const bool of_y = block >= plan.x_blocks;
             row[i] = u < units ? r : -1;
@@ -549,34 +550,25 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
                 v[i] = tm_load<WIDE>(ok ? p : static_cast<const T*>(a.x), 1, ok ? min(8, (of_y ? a.outer : a.inner) - c) : 0);
             }
         };
-        // rows AHEAD stages ahead, their numbers one more
+        // the rows of the next stage are asked for behind this one, their numbers a stage earlier
         int32_t ids[UNITS];
-        TmRaw<T> v[AHEAD][UNITS];
+        TmRaw<T> v[UNITS];
         rows_of(0, ids);
-#pragma unroll
-        for (int s = 0; s < AHEAD; s++) {
-            fetch(ids, v[s]);            // behind the stretch: zeros
-            rows_of(s + 1, ids);
-        }
+        fetch(ids, v);
+        rows_of(1, ids);
         int stage = 0;
         uint32_t phase = 1;
-        bool more = true;
-        for (int step = 0; more && step < steps;) {
+        for (int step = 0; step < steps; step++) {
+            if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
 #pragma unroll
-            for (int s = 0; s < AHEAD; s++) {
-                if (step >= steps) break;
-                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
-#pragma unroll
-                for (int i = 0; i < UNITS; i++)
-                    if (row[i] >= 0) tm_store(v[s][i], stage0 + stage * stage_bytes + at[i], BLOCK);
-                fence_to_tensor();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.full[stage]);
-                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                step++;
-                fetch(ids, v[s]);
-                rows_of(step + AHEAD, ids);
-            }
+            for (int i = 0; i < UNITS; i++)
+                if (row[i] >= 0) tm_store(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+            fence_to_tensor();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars.full[stage]);
+            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+            fetch(ids, v);   // behind the stretch: zeros
+            rows_of(step + 2, ids);
         }
     }
     tensor_fence_before();
@@ -628,7 +620,7 @@ static bool tm_rows(const TlArgs& a, int back, cudaStream_t s, cudaError_t* rc)
     void (*const kernel)(TlArgs, TmPlan) = wide ? tm_rows_kernel<T, true> : tm_rows_kernel<T, false>;
     *rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (*rc != cudaSuccess) return true;
-    kernel<<<grid, TM_THREADS, smem, s>>>(a, p);
+    kernel<<<grid, tm_threads(TM_FEED<T>), smem, s>>>(a, p);
     *rc = cudaGetLastError();
     return true;
 }
@@ -660,7 +652,7 @@ static cudaError_t tm_weights(const TlArgs& a, cudaStream_t s)
     void (*const kernel)(TlArgs, TwPlan) = wide ? tm_weights_kernel<T, true> : tm_weights_kernel<T, false>;
     const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    kernel<<<grid, TM_THREADS, smem, s>>>(a, p);
+    kernel<<<grid, tm_threads(TW_FEED), smem, s>>>(a, p);
     return cudaGetLastError();
 }
 
