@@ -103,8 +103,10 @@ tl_join_kernel(const TlArgs a, int64_t stretches)
     __syncthreads();
     const int64_t cells = (int64_t)a.inner * a.outer, all = cells + a.outer, first = first_of, count = min(count_of, stretches - first_of);
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
-        float sum = 0.0f;
-        for (int64_t c = 0; c < count; c++) sum += a.partial[(first + c) * all + i];
+        double exact = 0.0;   // as many as a thousand stretches
+#pragma unroll 8
+        for (int64_t c = 0; c < count; c++) exact += (double)a.partial[(first + c) * all + i];
+        const float sum = (float)exact;
         if (i < cells) {
             if (a.dw != nullptr) tl_put(static_cast<T*>(a.dw) + type * cells + i, sum);
         } else if (a.db != nullptr) {

@@ -67,13 +67,13 @@ __device__ __forceinline__ TlTile tl_tile(const TlArgs& a, int64_t tile, int per
     return {-1, 0, 0};
 }
 
-// Rows of a stretch: four blocks an SM where there are as many rows, no more than 2048 (a sum in tensor memory is one chain of additions) and
+// Rows of a stretch: four blocks an SM where there are as many rows, no more than 1024 (a sum in tensor memory is one chain of additions that are cut off) and
 // no fewer than 256.
 static inline int tl_stretch(int64_t n, int inner, int outer, int dtype)
 {
     const int64_t tiles = (int64_t)((inner + 127) / 128) * ((outer + (dtype == DYNB_F32 ? 127 : 255)) / (dtype == DYNB_F32 ? 128 : 256));
     const int64_t rows = n * tiles / (148 * 4) + 1;
-    return (int)((std::min<int64_t>(2048, std::max<int64_t>(256, rows)) + 31) / 32 * 32);
+    return (int)((std::min<int64_t>(1024, std::max<int64_t>(256, rows)) + 31) / 32 * 32);
 }
 static inline int64_t tl_stretches(int64_t n, int types, int stretch) { return (n + stretch - 1) / stretch + types; }
 

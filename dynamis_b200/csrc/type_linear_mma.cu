@@ -80,20 +80,22 @@ __device__ __forceinline__ void tm_store(const TmRaw<T>& r, unsigned char* at, i
     }
 }
 
-// Adds the products of one step of 16 summed elements to d: the parts of `a` are `a_part` apart, those of `b` `b_part` (units of 16 bytes).  The
-// small products come first; a part of `a` stays at the multipliers for its products.
+// Adds the products of one step of 16 summed elements: the parts of `a` are `a_part` apart, those of `b` `b_part` (units of 16 bytes).  A part of `a`
+// stays at the multipliers for its products.  The products of the leading parts go to d, the small ones to `small`, which may be d: they then come
+// first.  The tensor cores cut sums off where they do not fit 24 bits, towards zero, every step: six additions a step to one sum over 2000 rows cost
+// 1.2e-5 of the weights' gradient, one a step to a sum of its own and 1024 rows a tenth of that.
 template <int PARTS>
-__device__ __forceinline__ void tm_step(uint32_t d, uint64_t a, int a_part, uint64_t b, int b_part, uint32_t what, bool add)
+__device__ __forceinline__ void tm_step(uint32_t d, uint32_t small, uint64_t a, int a_part, uint64_t b, int b_part, uint32_t what, bool add)
 {
     if constexpr (PARTS == 1) {
         tensor_mma(d, a, b, what, add);
     } else {
-        tensor_mma(d, a + 2 * a_part, b, what, add);
-        tensor_mma_keep<1>(d, a + a_part, b + b_part, what, true);
-        tensor_mma_keep<3>(d, a + a_part, b, what, true);
-        tensor_mma_keep<1>(d, a, b + 2 * b_part, what, true);
-        tensor_mma_keep<2>(d, a, b + b_part, what, true);
-        tensor_mma_keep<3>(d, a, b, what, true);
+        tensor_mma(small, a + 2 * a_part, b, what, add);
+        tensor_mma_keep<1>(small, a + a_part, b + b_part, what, true);
+        tensor_mma_keep<3>(small, a + a_part, b, what, true);
+        tensor_mma_keep<1>(small, a, b + 2 * b_part, what, true);
+        tensor_mma_keep<2>(small, a, b + b_part, what, true);
+        tensor_mma_keep<3>(d, a, b, what, add || d == small);
     }
 }
 
@@ -333,7 +335,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
                     const uint64_t at_a = tile_descriptor(stage_at + stage * STAGE, 16, 1024), at_b = panel_from + (uint32_t)(chunk * plan.b_chunk);
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        if (k < steps) tm_step<PARTS>(sums, at_a + 2 * k, TM_ROWS * 128 / 16, at_b + (uint32_t)(k * plan.b_step), plan.b_part, what, chunk > 0 || k > 0);
+                        if (k < steps) tm_step<PARTS>(sums, sums, at_a + 2 * k, TM_ROWS * 128 / 16, at_b + (uint32_t)(k * plan.b_step), plan.b_part, what, chunk > 0 || k > 0);
                     tensor_commit(&bars.empty[stage]);
                     if (chunk == plan.chunks - 1) tensor_commit(&bars.sums_full[buffer]);
                 }
@@ -432,6 +434,7 @@ template <typename T, bool WIDE>
 __global__ void __launch_bounds__(tm_threads(TW_FEED), 1)
 tm_weights_kernel(const TlArgs a, const TwPlan plan)
 {
+    constexpr int FIRST = TmParts<T>::N == 1 ? 1 : 2;   // sums of the matrix: leading parts, small ones; those of the rows behind them
     constexpr int FEED = TW_FEED, FEED_THREADS = FEED * 32, PARTS = TmParts<T>::N, BLOCK = TW_ROWS * 128;
     constexpr int UNITS = PARTS == 1 ? 3 : 2;   // pieces of 8 elements a thread and stage: 32 rows x (128 + 256 or 128) elements
     extern __shared__ unsigned char raw_smem[];
@@ -474,11 +477,19 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
             for (int which = 0; which < (sums_wanted ? 2 : 1); which++) {
                 float* const at = which == 0 ? mine + (int64_t)m * a.outer + col0 : mine + cells + col0;
                 const bool write = which == 0 ? m < a.inner : threadIdx.x == 0;
+                const uint32_t from = tensor + ((uint32_t)(warp * 32) << 16) + which * FIRST * plan.column_stride;
                 for (int c = 0; c < have; c += 32) {
                     uint32_t bits[32];
                     __syncwarp();
-                    tensor_load_32(tensor + ((uint32_t)(warp * 32) << 16) + which * plan.column_stride + c, bits);
+                    tensor_load_32(from + c, bits);
                     tensor_wait_loads();
+                    if constexpr (PARTS > 1) {
+                        uint32_t small[32];
+                        tensor_load_32(from + plan.column_stride + c, small);
+                        tensor_wait_loads();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
+                    }
                     if (write) tm_put_row(at + c, bits, have - c, plan.vec != 0);
                 }
             }
@@ -499,16 +510,14 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
                 const uint32_t at = stage_at + stage * stage_bytes;
                 const uint64_t at_x = tile_descriptor(at, lead_x, 1024), at_y = tile_descriptor(at + plan.x_blocks * PARTS * BLOCK, lead, 1024);
 #pragma unroll
-                for (int k = 0; k < TW_ROWS / 16; k++) tm_step<PARTS>(tensor, at_x + k * 128, BLOCK / 16, at_y + k * 128, BLOCK / 16, what, step > 0 || k > 0);
+                for (int k = 0; k < TW_ROWS / 16; k++) tm_step<PARTS>(tensor, tensor + plan.column_stride, at_x + k * 128, BLOCK / 16, at_y + k * 128, BLOCK / 16, what, step > 0 || k > 0);
                 if (sums_wanted) {
-                    bool add = step > 0;
 #pragma unroll
-                    for (int p = PARTS - 1; p >= 0; p--) {
+                    for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
                         for (int k = 0; k < TW_ROWS / 16; k++)
-                            tensor_mma(tensor + plan.column_stride, ones_desc, at_y + (p * BLOCK + k * 2048) / 16, what_sum, add || k > 0);
-                        add = true;
-                    }
+                            tensor_mma(tensor + (p == 0 ? FIRST : FIRST + 1) * plan.column_stride, ones_desc, at_y + (p * BLOCK + k * 2048) / 16, what_sum,
+                                       step > 0 || k > 0 || (p > 0 && p < PARTS - 1));
                 }
                 tensor_commit(&bars.empty[stage]);
                 if (step == steps - 1) tensor_commit(&bars.sums_full[0]);
@@ -644,7 +653,7 @@ static cudaError_t tm_weights(const TlArgs& a, cudaStream_t s)
     p.y_blocks = (p.columns + 63) / 64;
     const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
     p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - TM_ROWS * 128) / stage);
-    p.tensor_columns = tm_tensor_columns(2 * p.column_stride);
+    p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
     p.vec = a.outer % 4 == 0;
     const dim3 grid((unsigned)tl_stretches(a.n, a.types, a.stretch), (a.inner + TM_ROWS - 1) / TM_ROWS, (a.outer + p.columns - 1) / p.columns);
