@@ -67,15 +67,16 @@ __device__ __forceinline__ TlTile tl_tile(const TlArgs& a, int64_t tile, int per
     return {-1, 0, 0};
 }
 
-// Rows of a stretch: four blocks an SM where there are as many rows, no more than 1024 (a sum in tensor memory is one chain of additions that are cut off) and
-// no fewer than 256.
+// Rows of a stretch: four blocks an SM where there are as many rows, no fewer than 256, and no more than 1024 (a sum in tensor memory is one chain of
+// additions that are cut off), unless the stretches' sums would take more than twice the room of the rows.
 static inline int tl_stretch(int64_t n, int inner, int outer, int dtype)
 {
     const int64_t tiles = (int64_t)((inner + 127) / 128) * ((outer + (dtype == DYNB_F32 ? 127 : 255)) / (dtype == DYNB_F32 ? 128 : 256));
-    const int64_t rows = n * tiles / (148 * 4) + 1;
-    return (int)((std::min<int64_t>(1024, std::max<int64_t>(256, rows)) + 31) / 32 * 32);
+    const int64_t rows = n * tiles / (148 * 4) + 1, most = std::max<int64_t>(1024, (int64_t)inner * outer / (2 * ((int64_t)inner + outer)));
+    return (int)((std::min<int64_t>(most, std::max<int64_t>(256, rows)) + 31) / 32 * 32);
 }
-static inline int64_t tl_stretches(int64_t n, int types, int stretch) { return (n + stretch - 1) / stretch + types; }
+// An upper bound: every type with rows has one stretch that is not full.
+static inline int64_t tl_stretches(int64_t n, int types, int stretch) { return n / stretch + std::min<int64_t>(n, types) + 1; }
 
 // type_linear_mma.cu: the products on the tensor cores.  False: the widths are too large for it (nothing was launched).
 bool tl_mma_rows(const TlArgs& a, int back, int dtype, cudaStream_t s, cudaError_t* rc);

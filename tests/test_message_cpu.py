@@ -116,3 +116,20 @@ def test_walk_of_the_lists():
     lists = M.index_lists(src, dst, 5, 4)
     assert lists == {"rows": [3, 1, 0, 2, 4], "row_start": [0, 2, 3, 4, 4, 4], "src": [2, 0, 2, 2], "cols": [2, 0, 1, 3], "col_start": [0, 3, 4, 4, 4],
                      "in_edge": [0, 2, 3, 1], "in_dst": [3, 1, 0, 3]}
+
+
+def test_workspace_of_the_weights_gradient_follows_the_rows():
+    """Sums of stretches for the types that can have rows, and no more than about twice the room of wide rows (no memory is touched here)."""
+    L, n = _lib.lib(), ctypes.c_int64()
+
+    def room(rows, types, inner, outer):
+        a = _lib.TypeLinear()
+        a.weight_dev = a.order_dev = a.start_dev = 4096
+        a.n_rows, a.types, a.inner, a.outer, a.dtype = rows, types, inner, outer, _lib.DYNB_F32
+        assert L.dynb_type_linear_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == 0
+        return n.value
+
+    assert room(100, 4096, 128, 128) <= 102 * 4 * (128 * 128 + 128)
+    assert room(0, 4096, 128, 128) <= 2 * 4 * (128 * 128 + 128)
+    rows, wide = 1_000_000, 16384
+    assert room(rows, 1, wide, wide) <= 2.1 * rows * 2 * wide * 4

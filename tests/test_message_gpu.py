@@ -408,7 +408,7 @@ def _compare_linear(x, weight, offset, kinds, g):
 @pytest.mark.parametrize("rows,types,inner,outer,offset", [(1, 1, 1, 1, True), (1, 3, 16, 8, True), (63, 2, 7, 5, True), (64, 1, 64, 64, False), (65, 1, 64, 64, True),
                                                            (1000, 5, 128, 128, True), (1003, 5, 128, 64, True), (129, 89, 64, 256, True), (5000, 3, 130, 70, True),
                                                            (9001, 2, 33, 129, False), (4097, 1, 256, 16, True), (300, 7, 1, 300, True), (300, 7, 300, 1, True),
-                                                           (20000, 12, 96, 192, True), (777, 4, 512, 384, True), (256, 2, 8, 1024, True)])
+                                                           (20000, 12, 96, 192, True), (777, 4, 512, 384, True), (256, 2, 8, 1024, True), (70, 2, 1200, 40, True), (70, 3, 24, 1300, True)])
 def test_type_linear_and_gradients(cuda, dtype, rows, types, inner, outer, offset):
     gen, dtype = _gen(rows + inner), M.TYPES[dtype]
     kinds = _kinds(rows, types, rows + outer).to(cuda)
@@ -425,6 +425,24 @@ def test_type_linear_strides_and_missing_types(cuda, dtype):
         g = _normal(gen, 900, 2 * 48, dtype=dtype)[:, 48:]
         y, (dx, dw, db) = _compare_linear(x, _normal(gen, 7, 64, 48, dtype=dtype), _normal(gen, 7, 48, dtype=dtype), kinds, g)
         assert not dw[0::2].any() and not db[0::2].any()
+
+
+def test_type_linear_long_sums_of_one_sign(cuda):
+    """Operands of one sign, where sums that are cut off towards zero lose the most.  A step of 16 products cuts at most 2^-23 of the sum so far off, and a
+    leading sum has at most 1024 / 16 = 64 of them (y, dx: 128 / 16 = 8 steps of six); parts of 24 bits and the rest of the rounding stay
+    within 2^-21."""
+    gen = _gen(31)
+    n = 150_001
+    kinds = _kinds(n, 2, 3).to(cuda)
+    x, w, g = (torch.rand(*s, generator=gen, device="cuda") for s in ((n, 128), (2, 128, 128), (n, 128)))
+    leaves = [t.requires_grad_() for t in (x, w)]
+    y = D.type_linear(x, w, D.type_index(kinds, 2))
+    dx, dw = torch.autograd.grad(y, leaves, g)
+    for t in range(2):
+        m = torch.nonzero(kinds == t)[:, 0]
+        for got, ref, steps in ((y[m], x[m].double() @ w[t].double(), 48), (dx[m], g[m].double() @ w[t].double().T, 48),
+                                (dw[t], x[m].double().T @ g[m].double(), 64)):
+            assert float(((got.double() - ref) / ref).abs().max()) <= steps * 2.0 ** -23 + 2.0 ** -21
 
 
 def test_type_linear_of_no_rows(cuda):
