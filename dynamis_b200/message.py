@@ -42,16 +42,20 @@ INT32_MAX = 2 ** 31 - 1
 MAX_EDGES = 2 ** 31 - 2 ** 16   # DYNB_MAX_EDGES
 
 
-def _lists(what: str, **lists) -> None:
-    device = None
-    for name, t in lists.items():
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _lists(what: str, names, lists) -> None:
+    on = -1
+    for name, t in zip(names, lists):
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
             raise RuntimeError(f"{what}: {name} must be a CUDA tensor")
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous():
             raise RuntimeError(f"{what}: {name} must be a contiguous 1-D int32 tensor, got {t.dtype} {list(t.shape)}")
-        if device is not None and t.device != device:
+        at = t.get_device()
+        if on >= 0 and at != on:
             raise RuntimeError(f"{what}: all lists must be on the same device")
-        device = t.device
+        on = at
+
+
+_NEIGHBOR_LISTS = ("rows", "row_start", "src", "cols", "col_start", "in_edge", "in_dst")
 
 
 @dataclass(frozen=True)
@@ -74,8 +78,7 @@ class NeighborIndex:
     in_dst: torch.Tensor
 
     def __post_init__(self):
-        _lists("NeighborIndex", rows=self.rows, row_start=self.row_start, src=self.src, cols=self.cols, col_start=self.col_start,
-               in_edge=self.in_edge, in_dst=self.in_dst)
+        _lists("NeighborIndex", _NEIGHBOR_LISTS, (self.rows, self.row_start, self.src, self.cols, self.col_start, self.in_edge, self.in_dst))
         E = self.src.numel()
         if self.row_start.numel() != self.rows.numel() + 1 or self.col_start.numel() != self.cols.numel() + 1:
             raise RuntimeError("NeighborIndex: row_start and col_start must have one entry more than rows and cols")
@@ -104,7 +107,7 @@ class TypeIndex:
     start: torch.Tensor
 
     def __post_init__(self):
-        _lists("TypeIndex", order=self.order, start=self.start)
+        _lists("TypeIndex", ("order", "start"), (self.order, self.start))
         if self.start.numel() < 2 or self.start.numel() > MAX_TYPES + 1:
             raise RuntimeError(f"TypeIndex: the number of types must lie in [1, {MAX_TYPES}], got {self.start.numel() - 1}")
 
@@ -228,7 +231,7 @@ class _NeighborAttention(torch.autograd.Function):
             dv = torch.empty(v.shape, dtype=v.dtype, device=dev) if want_v else None
             d_bias = torch.empty(bias.shape, dtype=torch.float32, device=dev) if want_bias else None
             delta = torch.empty((q.size(0), q.size(1), 4), dtype=torch.float32, device=dev)
-            args = _attention_args(q, k, v, bias, index, ctx.scale)
+            args = _attention_args(q, k, v, bias, index, ctx.scale)   # anew: hooks may have moved what was saved
             _lib.check(_lib.lib().dynb_neighbor_attention_backward(
                 ctypes.byref(args), d_out.data_ptr(), d_out.stride(0), d_out.stride(1), out32.data_ptr(), stats.data_ptr(), index.cols.data_ptr(),
                 index.col_start.data_ptr(), index.in_edge.data_ptr(), index.in_dst.data_ptr(), delta.data_ptr(), _pointer(dq), _pointer(dk),
@@ -255,27 +258,29 @@ def neighbor_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
             raise RuntimeError(f"{name} must be a CUDA tensor")
         if t.dim() != 3:
             raise RuntimeError(f"{name} must have shape [rows, heads, dim], got {list(t.shape)}")
-        if t.dtype != q.dtype or t.dtype not in _DTYPES:
-            raise RuntimeError(f"q, k and v must all be float32, float16 or bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
-        if t.device != q.device:
-            raise RuntimeError("q, k and v must be on the same device")
+    if q.dtype not in _DTYPES or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        raise RuntimeError(f"q, k and v must all be float32, float16 or bfloat16, got {q.dtype}, {k.dtype} and {v.dtype}")
+    on = q.get_device()
+    if k.get_device() != on or v.get_device() != on:
+        raise RuntimeError("q, k and v must be on the same device")
+    (targets, heads, dim), (sources, kv_heads, kv_dim) = q.shape, k.shape
     if k.shape != v.shape:
         raise RuntimeError(f"k and v must have the same shape, got {list(k.shape)} and {list(v.shape)}")
-    if q.size(2) != k.size(2) or not 1 <= q.size(2) <= MAX_DIM:
-        raise RuntimeError(f"q, k and v must have the same dim in [1, {MAX_DIM}], got {q.size(2)} and {k.size(2)}")
-    if k.size(1) < 1 or q.size(1) < 1 or q.size(1) % k.size(1) != 0 or q.size(1) > 65535:
-        raise RuntimeError(f"the heads of q must be a multiple of those of k and v, got {q.size(1)} and {k.size(1)}")
-    if q.size(0) != index.num_targets or k.size(0) != index.num_sources:
-        raise RuntimeError(f"the index is of {index.num_targets} targets and {index.num_sources} sources, got {q.size(0)} and {k.size(0)} rows")
-    if index.src.device != q.device:
+    if dim != kv_dim or not 1 <= dim <= MAX_DIM:
+        raise RuntimeError(f"q, k and v must have the same dim in [1, {MAX_DIM}], got {dim} and {kv_dim}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads != 0 or heads > 65535:
+        raise RuntimeError(f"the heads of q must be a multiple of those of k and v, got {heads} and {kv_heads}")
+    if targets != index.num_targets or sources != index.num_sources:
+        raise RuntimeError(f"the index is of {index.num_targets} targets and {index.num_sources} sources, got {targets} and {sources} rows")
+    if index.src.get_device() != on:
         raise RuntimeError("index and q must be on the same device")
     if bias is not None:
-        if not isinstance(bias, torch.Tensor) or bias.device != q.device or bias.dtype != torch.float32:
+        if not isinstance(bias, torch.Tensor) or bias.get_device() != on or bias.dtype is not torch.float32:
             raise RuntimeError("bias must be a float32 tensor on the device of q")
-        if bias.shape != (index.num_edges, q.size(1)):
-            raise RuntimeError(f"bias must have shape [{index.num_edges}, {q.size(1)}], got {list(bias.shape)}")
+        if bias.shape != (index.num_edges, heads):
+            raise RuntimeError(f"bias must have shape [{index.num_edges}, {heads}], got {list(bias.shape)}")
         bias = bias.contiguous()
-    scale = 1.0 / math.sqrt(q.size(2)) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise RuntimeError(f"scale must be finite, got {scale}")
     return _NeighborAttention.apply(q, k, v, bias, index, scale)
@@ -430,7 +435,7 @@ class _TypeLinear(torch.autograd.Function):
         dev, d_y = x.device, _row_last(d_y)
         L = _lib.lib()
         with _lib.on_device(dev):
-            args = _linear_args(x, weight, ctx.index)
+            args = _linear_args(x, weight, ctx.index)   # anew: hooks may have moved what was saved
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
             dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[1] else None
             db = torch.empty((weight.size(0), weight.size(2)), dtype=x.dtype, device=dev) if ctx.needs_input_grad[2] else None

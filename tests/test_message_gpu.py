@@ -677,3 +677,28 @@ def test_captured_layer_replays_on_new_inputs(cuda):
         with torch.cuda.graph(graph):
             D.neighbor_index(ei, 300, 350)
     assert D.neighbor_index(ei, 300, 350).num_edges == 9000
+
+
+def test_gradients_of_tensors_that_hooks_moved(cuda):
+    """Saved tensors that went to the host and came back elsewhere, dense: the backward passes read them where they are then."""
+    ei, src, dst, q, k, v, b, g = _attention_case(RAGGED, 60, 4, 2, 16, torch.float32, True, 12)
+    index = D.neighbor_index(ei, q.size(0), k.size(0))
+    wide = torch.cat([k, v], dim=2)
+    k, v = wide[..., :16], wide[..., 16:]
+    kinds = _kinds(60, 3, 1).to(cuda)
+    tall, w = D.type_index(kinds, 3), torch.randn(3, 32, 16, device=cuda, requires_grad=True)
+    r, table = torch.rand(ei.size(1), device=cuda).mul_(5).requires_grad_(), torch.randn(12, 4, device=cuda, requires_grad=True)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    x = torch.randn(60, 64, device=cuda)[:, ::2].requires_grad_()
+
+    def grads(moved):
+        if moved:
+            with torch.autograd.graph.save_on_cpu():
+                out, y = D.neighbor_attention(*leaves, index, D.distance_bias(r, table, 5.0)), D.type_linear(x, w, tall)
+            junk = [torch.full((1 << 16,), float("nan"), device=cuda) for _ in range(20)]   # where the tensors were
+            del junk
+        else:
+            out, y = D.neighbor_attention(*leaves, index, D.distance_bias(r, table, 5.0)), D.type_linear(x, w, tall)
+        return torch.autograd.grad([out, y], [*leaves, r, table, x, w], [g, torch.ones_like(y)])
+
+    assert all(torch.equal(a, c) for a, c in zip(grads(False), grads(True)))
