@@ -207,7 +207,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
     __shared__ __align__(16) unsigned char turned[4][32 * 144];
     unsigned char* const panel = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
     unsigned char* const stage0 = panel + plan.panel_bytes;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_number(), lane = threadIdx.x & 31;
     const T* const in = static_cast<const T*>(plan.back ? a.dy : a.x);
     T* const out = static_cast<T*>(plan.back ? a.dx : a.y);
     const int64_t in_row = plan.back ? a.dy_row : a.x_row;
@@ -329,7 +329,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
             for (int chunk = 0; chunk < plan.chunks; chunk++) {
                 if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
                 tensor_fence_after();
-                if (lane == 0) {
+                if (elected()) {
                     const int steps = min(4, (kk - chunk * 64 + 15) / 16);
                     // descriptors are in units of 16 bytes: steps and parts are additions
                     const uint64_t at_a = tile_descriptor(stage_at + stage * STAGE, 16, 1024), at_b = panel_from + (uint32_t)(chunk * plan.b_chunk);
@@ -344,7 +344,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
             }
             if (!ok) break;
             cursor.next(a);
-            if (cursor.tile.type >= 0 && cursor.tile.type != panel_type && lane == 0) tensor_commit(&bars.panel_free);
+            if (cursor.tile.type >= 0 && cursor.tile.type != panel_type && elected()) tensor_commit(&bars.panel_free);
             __syncwarp();
             buffer ^= 1;
             if (buffer == 0) sums_phase ^= 1;
@@ -441,7 +441,7 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
     __shared__ TmBars bars;
     unsigned char* const ones = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
     unsigned char* const stage0 = ones + TM_ROWS * 128;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_number(), lane = threadIdx.x & 31;
     const int row0 = blockIdx.y * TM_ROWS, col0 = blockIdx.z * plan.columns;
     const int blocks = plan.x_blocks + plan.y_blocks, stage_bytes = blocks * PARTS * BLOCK;
     const TlTile tile = tl_tile(a, blockIdx.x, a.stretch);
@@ -506,7 +506,7 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
         for (int step = 0; step < steps; step++) {
             if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
             tensor_fence_after();
-            if (lane == 0) {
+            if (elected()) {
                 const uint32_t at = stage_at + stage * stage_bytes;
                 const uint64_t at_x = tile_descriptor(at, lead_x, 1024), at_y = tile_descriptor(at + plan.x_blocks * PARTS * BLOCK, lead, 1024);
 #pragma unroll

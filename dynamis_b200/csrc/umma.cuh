@@ -37,16 +37,27 @@ __device__ __forceinline__ uint64_t timer_ns()
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-// Waits at most two seconds for the phase; false when they have passed.
+// Waits at most two seconds for the phase; false when they have passed.  All lanes of a warp call it and get the same answer, which the compiler can
+// see from the vote: what follows stays uniform, and with it the operands of the products.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity)
 {
-    if (bar_try(bar, parity)) return true;
-    const uint64_t from = timer_ns();
-    for (uint32_t i = 1; i < (1u << 30); i++) {
-        if (bar_try(bar, parity)) return true;
-        if ((i & 63u) == 0 && timer_ns() - from > 2000000000ull) return false;
+    uint64_t from = 0;
+    for (uint32_t i = 0; i < (1u << 30); i++) {
+        if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+        if ((i & 1023u) != 1023u) continue;
+        const uint64_t now = timer_ns();
+        if (from == 0) from = now;
+        if (__any_sync(0xffffffffu, now - from > 2000000000ull)) return false;
     }
     return false;
+}
+// The number of this warp, and one of its lanes, in ways that the compiler knows to be uniform.
+__device__ __forceinline__ int warp_number() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+__device__ __forceinline__ bool elected()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 
 // What this thread wrote to shared memory becomes visible to the tensor cores.
