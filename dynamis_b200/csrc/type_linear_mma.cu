@@ -2,14 +2,14 @@
 //
 // y = x W + b and dx = dy W^T: a block keeps the whole matrix of a type for its columns in shared memory (laid out once per type) and takes
 // tiles of 128 rows one after the other: eight or sixteen warps gather the rows into stages of 64 columns, one thread issues the products, four
-// warps take the sums out of tensor memory, which holds two of them, turn them in shared memory and store the rows by whole lines.  What bounds it is the chain of a stage from memory to
-// the multipliers, and shared memory, which rows, matrix and results share.
+// warps take the sums out of tensor memory, which holds two of them, turn them in shared memory and store the rows by whole lines.  What bounds
+// it is the chain of a stage from memory to the multipliers, and shared memory, which rows, matrix and results share.
 //
 // dW = sum x_i^T dy_i: a block takes a stretch of rows of one type, 128 x up to 256 elements of the matrix; both operands are the gathered
 // rows as they are, read along their columns.  db is a product too, with a tile of ones.
 //
-// 1 M rows, 128 x 128 fp32, 5 types: y and dx 262 us each (3.9 TB/s; the products alone some 130), the weights' gradient 321 us; 400 k rows, 256 x 256 bf16,
-// 89 types: 140 us (3.0 TB/s).  A kernel of fused multiply-adds on 64 x 64 tiles took 1.6, 1.6 and 3.4 ms, and 3.3 ms.
+// 1 M rows, 128 x 128 fp32, 5 types: y and dx 262 us each (3.9 TB/s), the weights' gradient 321 us; 400 k rows, 256 x 256 bf16,
+// 89 types: 140 us (3.0 TB/s).  Kernels of fused multiply-adds on 64 x 64 tiles took 6.6 ms for the three, and 3.3 ms.
 //
 // fp32 operands are split into three bf16 parts (8 bits each, together all 24): v = p0 + p1 + p2.  Six of the nine products are formed,
 // those left out are below 2^-25 of the whole; the small ones are added first.  Sums are in fp32.

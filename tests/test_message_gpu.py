@@ -702,3 +702,17 @@ def test_gradients_of_tensors_that_hooks_moved(cuda):
         return torch.autograd.grad([out, y], [*leaves, r, table, x, w], [g, torch.ones_like(y)])
 
     assert all(torch.equal(a, c) for a, c in zip(grads(False), grads(True)))
+
+
+def test_a_wait_that_ran_out_is_told_at_the_next_call(cuda):
+    """The word that a kernel sets when one of its bounded waits runs out (set from the host here): the next call raises, the one behind it works."""
+    from dynamis_b200 import message
+
+    index = D.type_index(torch.tensor([0, 1, 1], device=cuda), 2)
+    x, w = torch.randn(3, 8, device=cuda), torch.randn(2, 8, 4, device=cuda)
+    y = D.type_linear(x, w, index)
+    torch.cuda.synchronize()
+    message._STATUS[x.device.index][0].value = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        D.type_linear(x, w, index)
+    assert torch.equal(D.type_linear(x, w, index), y)
