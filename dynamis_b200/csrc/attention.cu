@@ -37,8 +37,8 @@ static int attn_args(const dynb_attention* in, AttnArgs* a)
     return DYNB_OK;
 }
 
-// Whether the rows of a tensor lie in 64 GB.
-static bool attn_narrow(const AttnRows& r, int64_t rows, int heads, int size) { return (rows * r.row + heads * r.head) * size / 16 < (1ll << 32); }
+// Whether the rows of a tensor lie in 128 GB.
+static bool attn_narrow(const AttnRows& r, int64_t rows, int heads, int size) { return (rows * r.row + heads * r.head) * size / 32 < (1ll << 32); }
 
 // Bytes on which the heads of all these tensors start and end.
 static int attn_wide(int dim, int size, std::initializer_list<AttnRows> all, std::initializer_list<const void*> outputs)
@@ -46,7 +46,7 @@ static int attn_wide(int dim, int size, std::initializer_list<AttnRows> all, std
     uint64_t bits = (uint64_t)dim * size;
     for (const AttnRows& r : all) bits |= reinterpret_cast<uintptr_t>(r.at) | (uint64_t)r.row * size | (uint64_t)r.head * size;
     for (const void* p : outputs) bits |= reinterpret_cast<uintptr_t>(p);
-    return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : size;
+    return bits % 32 == 0 ? 32 : bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : size;
 }
 
 }  // namespace dynb

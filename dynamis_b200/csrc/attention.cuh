@@ -64,21 +64,19 @@ __device__ __forceinline__ void attn_pairs(const Raw<T, EL>& r, float2 (&f)[EL /
     }
 }
 
-// Where a lane's pieces stand in their head: piece p of the lane is number (p ^ turn) G + part of the head.  The turn depends on the
-// head so that eight lanes, which are served at once, meet eight different pieces of 128 bytes.
+// Where a lane's pieces stand in their head: 32 bytes in a row.
 template <typename T, int G, int EL>
 struct Place {
     static constexpr int PIECES = EL * (int)sizeof(T) / 16, VEC = 16 / (int)sizeof(T);
     int at[PIECES];
-    __device__ __forceinline__ Place(int part, int head)
+    __device__ __forceinline__ explicit Place(int part)
     {
-        const int turn = (G * PIECES < 8 ? head * (G * PIECES) >> 3 : head) & (PIECES - 1);
 #pragma unroll
-        for (int p = 0; p < PIECES; p++) at[p] = ((p ^ turn) * G + part) * VEC;
+        for (int p = 0; p < PIECES; p++) at[p] = (part * PIECES + p) * VEC;
     }
 };
 
-// FULL: heads of EL G elements whose pieces start on 16 bytes.  Otherwise `wide` says on how many bytes (16, 8 or fewer) heads start and end.
+// FULL: heads of EL G elements that start on 32 bytes.  Otherwise `wide` says on how many bytes (16, 8 or fewer) heads start and end.
 template <typename T, int G, int EL, bool FULL>
 __device__ __forceinline__ Raw<T, EL> attn_load(const T* head, const Place<T, G, EL>& place, int dim, int wide)
 {
@@ -89,7 +87,7 @@ __device__ __forceinline__ Raw<T, EL> attn_load(const T* head, const Place<T, G,
         const int at = place.at[p];
         if (FULL) {
             r.v[p] = __ldg(reinterpret_cast<const uint4*>(head + at));
-        } else if (wide == 16) {
+        } else if (wide >= 16) {
             r.v[p] = at < dim ? __ldg(reinterpret_cast<const uint4*>(head + at)) : make_uint4(0, 0, 0, 0);
         } else if (wide == 8) {
             const uint2 lo = at < dim ? __ldg(reinterpret_cast<const uint2*>(head + at)) : make_uint2(0, 0);
@@ -104,25 +102,25 @@ __device__ __forceinline__ Raw<T, EL> attn_load(const T* head, const Place<T, G,
     }
     return r;
 }
-// Rows of full heads: a lane's pieces in units of 16 bytes from the tensor's start, in 32 bits (64 GB): one addition a piece, where a 64-bit
-// pointer per piece took two and a zero row for masked edges four more selections.
+// Rows of full heads: a lane's 32 bytes by one load, in units of 32 bytes from the tensor's start, in 32 bits (128 GB): a pointer and two loads of 16 bytes
+// took five more instructions an edge.
 template <typename T, int G, int EL>
 struct Lane {
-    static constexpr int PIECES = Place<T, G, EL>::PIECES;
-    const uint4* base;
-    uint32_t step, at[PIECES];
+    const char* base;
+    uint32_t step, at;
     __device__ __forceinline__ Lane(const AttnRows& rows, int head, const Place<T, G, EL>& place)
     {
-        base = static_cast<const uint4*>(rows.at);
-        step = (uint32_t)(rows.row * (int)sizeof(T) / 16);
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) at[p] = (uint32_t)((rows.head * head + place.at[p]) * (int)sizeof(T) / 16);
+        base = static_cast<const char*>(rows.at);
+        step = (uint32_t)(rows.row * (int)sizeof(T) / 32);
+        at = (uint32_t)((rows.head * head + place.at[0]) * (int)sizeof(T) / 32);
     }
     __device__ __forceinline__ Raw<T, EL> load(uint32_t row) const
     {
         Raw<T, EL> r;
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) r.v[p] = __ldg(base + (row * step + at[p]));
+        static_assert(sizeof(r) == 32, "a lane holds 32 bytes");
+        asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=r"(r.v[0].x), "=r"(r.v[0].y), "=r"(r.v[0].z), "=r"(r.v[0].w), "=r"(r.v[1].x), "=r"(r.v[1].y), "=r"(r.v[1].z), "=r"(r.v[1].w)
+            : "l"(base + (uint64_t)(row * step + at) * 32));
         return r;
     }
 };
@@ -188,7 +186,7 @@ __device__ __forceinline__ void attn_store(T* head, const Place<T, G, EL>& place
             e[i] = attn_put<T>(f[(p * VEC + i) / 2].x);
             e[i + 1] = attn_put<T>(f[(p * VEC + i) / 2].y);
         }
-        if (FULL || wide == 16) {
+        if (FULL || wide >= 16) {
             if (FULL || at < dim) *reinterpret_cast<uint4*>(head + at) = *reinterpret_cast<const uint4*>(e);
         } else if (wide == 8) {
             if (at < dim) *reinterpret_cast<uint2*>(head + at) = *reinterpret_cast<const uint2*>(e);
@@ -265,8 +263,8 @@ struct AttnArgs {
     const int32_t *rows, *row_start, *src, *cols, *col_start, *in_edge, *in_dst;
     int64_t n_targets, n_sources, n_edges;
     int heads, kv_heads, shared, dim, warp_heads;
-    int wide;                   // bytes on which all heads start and end: 16, 8 or fewer
-    int narrow;                 // offsets in units of 16 bytes fit 32 bits
+    int wide;                   // bytes on which all heads start and end: 32, 16, 8 or fewer
+    int narrow;                 // offsets in units of 32 bytes fit 32 bits
     int block_rows;             // rows of a block, a multiple of those that it takes at once
     float scale;
 };
@@ -281,7 +279,7 @@ template <typename T> struct LaneElements { static constexpr int N = 32 / (int)s
 template <typename T, template <typename, int, bool> class Launch, int G>
 static inline cudaError_t attn_by_full(const AttnArgs& a, cudaStream_t s)
 {
-    return a.wide == 16 && a.narrow && a.dim == LaneElements<T>::N * G ? Launch<T, G, true>::go(a, s) : Launch<T, G, false>::go(a, s);
+    return a.wide == 32 && a.narrow && a.dim == LaneElements<T>::N * G ? Launch<T, G, true>::go(a, s) : Launch<T, G, false>::go(a, s);
 }
 template <typename T, template <typename, int, bool> class Launch>
 static inline cudaError_t attn_by_dim(const AttnArgs& a, cudaStream_t s)
@@ -313,8 +311,9 @@ static inline int attn_warp_heads(int heads, int g)
 }
 
 // Rows of a block that takes `at_once` at once: neighbouring rows read the same rows of the other side, so a block goes on with the next ones
-// while L1 holds these, as long as there are eight blocks for every place on the SMs.
-constexpr int ATTN_TURNS = 8;
+// while L1 holds these, as long as there are eight blocks for every place on the SMs (200 k targets, 8 x 16 fp32, forward and gradients: a turn 2793 us, two
+// 2664, four 2632, eight 2647).
+constexpr int ATTN_TURNS = 4;
 static inline int attn_block_rows(int64_t rows, int at_once)
 {
     int turns = ATTN_TURNS;

@@ -14,9 +14,11 @@
 namespace dynb {
 
 constexpr int AB_WARPS = 4;
-constexpr int AC_BATCH = 2;    // edges of a slot in a batch, by source
-// By target: 128 registers hold a batch of four pairs of rows in fp32, of two in 16 bits, which are unpacked (bf16, 4 x 64: four 491 us, two 377).
-template <typename T, bool FULL> constexpr int AB_BATCH = sizeof(T) == 4 && FULL ? 4 : 2;
+// Edges of a slot in a batch, by target and by source, and blocks an SM by target.  200 k targets, 8 x 16 fp32: by target two edges and 20 warps 894 us, four
+// edges and 16 warps 1010; by source three edges 1043, two 1192.  bf16, 4 x 64, by source: two edges 464, three 591 (its rows are unpacked).
+constexpr int AB_BATCH = 2;
+template <typename T> constexpr int AC_BATCH = sizeof(T) == 4 ? 3 : 2;
+template <typename T> constexpr int AB_BLOCKS = sizeof(T) == 4 ? 5 : 4;
 
 // Sums of the warps of a row, in their order, with the first of them (turn 0).  All warps of the block call it.
 template <int N, int WPR>
@@ -38,17 +40,17 @@ __device__ __forceinline__ void attn_join(float2 (&acc)[N], int warp, int lane)
 }
 
 template <typename T, int G, bool FULL, int WPR>
-__global__ void __launch_bounds__(AB_WARPS * 32, 4)
+__global__ void __launch_bounds__(AB_WARPS * 32, AB_BLOCKS<T>)
 attn_backward_rows_kernel(const AttnArgs a)
 {
-    constexpr int EL = LaneElements<T>::N, BATCH = AB_BATCH<T, FULL>;
+    constexpr int EL = LaneElements<T>::N, BATCH = AB_BATCH;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = lane % G, slots = 32 / (G * a.warp_heads), slot = lane / (G * a.warp_heads);
     const int head = blockIdx.y * a.warp_heads + (lane / G) % a.warp_heads;
     const bool mine = head < a.heads;
     const int wide = a.wide;
     const int h = mine ? head : 0, kv = h / a.shared;
-    const Place<T, G, EL> place(part, h);
+    const Place<T, G, EL> place(part);
     const uint32_t sources = (uint32_t)a.n_sources;
     const Lane<T, G, EL> k_lane(a.k, kv, place), v_lane(a.v, kv, place);
     constexpr int ROWS = AB_WARPS / WPR;
@@ -144,17 +146,17 @@ template <typename T, int G, bool FULL, int WPR>
 __global__ void __launch_bounds__(AB_WARPS * 32, 4)
 attn_backward_cols_kernel(const AttnArgs a)
 {
-    constexpr int EL = LaneElements<T>::N;
+    constexpr int EL = LaneElements<T>::N, BATCH = AC_BATCH<T>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = lane % G, slots = 32 / (G * a.warp_heads), slot = lane / (G * a.warp_heads);
     const int head = blockIdx.y * a.warp_heads + (lane / G) % a.warp_heads;
     const bool mine = head < a.kv_heads;
     const int wide = a.wide;
     const int kv = mine ? head : 0;
-    const Place<T, G, EL> place(part, kv);
+    const Place<T, G, EL> place(part);
     const uint32_t targets = (uint32_t)a.n_targets, edges = (uint32_t)a.n_edges, bias_bytes = 4u * a.heads;
     constexpr int ROWS = AB_WARPS / WPR;
-    const int turn = warp % WPR, step = AC_BATCH * slots;
+    const int turn = warp % WPR, step = BATCH * slots;
     const char* const zeros = reinterpret_cast<const char*>(attn_zeros);
 
     const int64_t last = min(((int64_t)blockIdx.x + 1) * a.block_rows, a.n_sources);
@@ -181,23 +183,23 @@ attn_backward_cols_kernel(const AttnArgs a)
             acc[i] = acc[EL / 2 + i] = make_float2(0.0f, 0.0f);
         }
         // A step is a batch of edges and one of the heads that share keys and values.
-        int32_t t_ahead[AC_BATCH], e_ahead[AC_BATCH];
+        int32_t t_ahead[BATCH], e_ahead[BATCH];
         auto fetch = [&](int i) {
 #pragma unroll
-            for (int u = 0; u < AC_BATCH; u++) {
+            for (int u = 0; u < BATCH; u++) {
                 t_ahead[u] = i + u < n ? __ldg(in_dst + i + u) : -1;
                 e_ahead[u] = i + u < n && a.bias != nullptr ? __ldg(in_edge + i + u) : 0;
             }
         };
-        struct ColStep : AttnStep<T, EL, AC_BATCH> { float4 stats[AC_BATCH]; };
-        int i = turn * step + slot * AC_BATCH, shared_head = 0;
+        struct ColStep : AttnStep<T, EL, BATCH> { float4 stats[BATCH]; };
+        int i = turn * step + slot * BATCH, shared_head = 0;
         fetch(i);
         auto load = [&](ColStep& s) {
             const int h = kv * a.shared + shared_head;
             const Lane<T, G, EL> q_lane(a.q, h, place), g_lane(a.d_out, h, place);
-            uint32_t t[AC_BATCH];
+            uint32_t t[BATCH];
 #pragma unroll
-            for (int u = 0; u < AC_BATCH; u++) {
+            for (int u = 0; u < BATCH; u++) {
                 const bool in = (uint32_t)t_ahead[u] < targets && (uint32_t)e_ahead[u] < edges;
                 t[u] = in ? (uint32_t)t_ahead[u] : 0u;
                 const uint32_t e = in ? (uint32_t)e_ahead[u] : 0u;
@@ -214,10 +216,10 @@ attn_backward_cols_kernel(const AttnArgs a)
         };
         auto work = [&](ColStep& s) {
 #pragma unroll
-            for (int u = 0; u < AC_BATCH; u++) s.ok[u] = s.ok[u] && s.z[u] != -INFINITY;
+            for (int u = 0; u < BATCH; u++) s.ok[u] = s.ok[u] && s.z[u] != -INFINITY;
             s.clear();
 #pragma unroll
-            for (int u = 0; u < AC_BATCH; u++) {
+            for (int u = 0; u < BATCH; u++) {
                 float2 q[EL / 2], g[EL / 2];
                 attn_pairs(s.x[u], q);
                 attn_pairs(s.y[u], g);

@@ -16,22 +16,22 @@
 namespace dynb {
 
 constexpr int AF_WARPS = 4;
-// Edges of a slot in a batch; heads of odd sizes need the registers for their loads.
-template <bool FULL> constexpr int AF_BATCH = FULL ? 4 : 2;
+// Edges of a slot in a batch: what 128 registers hold.  Rows of 16 bits are unpacked; heads of odd sizes need registers for their loads.
+template <typename T, bool FULL> constexpr int AF_BATCH = !FULL ? 2 : sizeof(T) == 4 ? 4 : 3;
 
 // WPR warps take turns at the batches of a row and join through shared memory.
 template <typename T, int G, bool FULL, int WPR>
 __global__ void __launch_bounds__(AF_WARPS * 32, 4)
 attn_forward_kernel(const AttnArgs a)
 {
-    constexpr int EL = LaneElements<T>::N, BATCH = AF_BATCH<FULL>;
+    constexpr int EL = LaneElements<T>::N, BATCH = AF_BATCH<T, FULL>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = lane % G, slots = 32 / (G * a.warp_heads), slot = lane / (G * a.warp_heads);
     const int head = blockIdx.y * a.warp_heads + (lane / G) % a.warp_heads;
     const bool mine = head < a.heads;
     const int wide = a.wide;
     const int h = mine ? head : 0, kv = h / a.shared;
-    const Place<T, G, EL> place(part, h);
+    const Place<T, G, EL> place(part);
     const uint32_t sources = (uint32_t)a.n_sources;
     const Lane<T, G, EL> k_lane(a.k, kv, place), v_lane(a.v, kv, place);
     constexpr int ROWS = AF_WARPS / WPR;

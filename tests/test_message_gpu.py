@@ -151,6 +151,8 @@ def test_attention_strides(cuda):
     g = _normal(gen, T, H, 2 * dim)[..., :dim]
     _compare_attention((ei, src, dst, q, k, v, None, g), index=index)
     odd = _normal(gen, S, H, dim + 1)[..., 1:]                # heads off the 16-byte boundaries
+    half = _normal(gen, S, H, dim + 4)[..., 4:]               # on 16 bytes, not on 32
+    _compare_attention((ei, src, dst, q, half, v, None, g), index=index)
     last = _normal(gen, S, dim, H).transpose(1, 2)            # the elements of a head apart
     _compare_attention((ei, src, dst, q, odd, last, None, g), index=index)
     leaves = [t.detach().requires_grad_() for t in (q, k, v)]
