@@ -5,9 +5,9 @@
 // result is rounded once.
 //
 // A warp takes a row and keeps its queries and sums in registers; what it reads an edge is a row of keys and one of values, gathered, mostly from L2
-// and L1.  What bounds it is latency and issue: 39 warp instructions an edge, 16 warps an SM.  200 k targets, 10.5 M edges, 8 x 16 fp32: 753 us
-// (8.2 TB/s from L2, 0.25 ms at memory's rate for what is read once); 150 k targets, bf16, 8 heads on 2 of 32: 733 us.  Blocks of
-// four warps: with eight of twice the rows 773 us.
+// and L1.  What bounds it is latency and issue with 16 warps an SM (with neighbouring rows in all of them half the bytes come from L2, and it is no
+// faster).  200 k targets, 10.5 M edges, 8 x 16 fp32: 713 us (the bytes that have to be read once take 0.11 ms of memory's time); 150 k targets, bf16, 8 heads
+// on 2 of 32: 691 us.
 
 #include <algorithm>
 
