@@ -6,7 +6,7 @@
 //
 // A warp takes a row and keeps its queries and sums in registers; what it reads an edge is a row of keys and one of values, gathered, mostly from L2
 // and L1.  What bounds it is latency and issue with 16 warps an SM (with neighbouring rows in all of them half the bytes come from L2, and it is no
-// faster).  200 k targets, 10.5 M edges, 8 x 16 fp32: 713 us (the bytes that have to be read once take 0.11 ms of memory's time); 150 k targets, bf16, 8 heads
+// faster).  200 k targets, 10.5 M edges, 8 x 16 fp32: 713 us (the bytes that have to be read once take 0.12 ms of memory's time); 150 k targets, bf16, 8 heads
 // on 2 of 32: 691 us.
 
 #include <algorithm>

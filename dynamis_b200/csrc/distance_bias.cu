@@ -14,6 +14,7 @@
 namespace dynb {
 
 constexpr int DB_THREADS = 256;
+constexpr int DB_COPIES_BYTES = 40 << 10;  // eight copies of a table
 constexpr int DB_TABLE_BYTES = 24 << 10;   // tables that blocks copy to shared memory: eight blocks an SM hold one each
 
 struct DbArgs {
@@ -66,17 +67,26 @@ __device__ __forceinline__ float db_switch(const DbPlace& p)
     return logf(p.rest * p.rest * p.rest * fmaf(p.u, fmaf(p.u, 6.0f, 3.0f), 1.0f));
 }
 
-// A thread takes VEC heads of an edge (eight of them leave half sectors to write: 159 us for 10.5 M edges of 8 heads, four 111); the table is in shared memory (IN_SMEM) where it fits.
+// A thread takes VEC heads of an edge.  Eight of them where the table fits into shared memory eight times: four heads of a bucket are 16 bytes, which stand
+// there in eight copies beside one another, one for each of the eight lanes that are served at once, so that no two of them meet in a bank
+// whatever their distances are.  Otherwise the table is in shared memory once (IN_SMEM) or stays where it is.  10.5 M edges, 64 x 8: four heads a
+// thread and one copy 112 us, eight heads and one copy 156.
 template <int VEC, bool IN_SMEM>
 __global__ void __launch_bounds__(DB_THREADS)
 db_forward_kernel(const DbArgs a)
 {
     extern __shared__ __align__(16) float copies[];
-    const float* table = a.table;
+    const float* const table = IN_SMEM ? copies + (VEC == 8 ? threadIdx.x % 8 * 4 : 0) : a.table;
     if (IN_SMEM) {
-        for (int i = threadIdx.x; i < a.buckets * a.heads; i += DB_THREADS) copies[i] = a.table[i];
+        if (VEC == 8) {
+            for (int i = threadIdx.x; i < a.buckets * a.heads * 8; i += DB_THREADS) {
+                const int line = i >> 5, four = line / a.buckets;   // lines of 32 floats: buckets of heads 0 to 3, of heads 4 to 7, ...
+                copies[i] = a.table[(line - four * a.buckets) * a.heads + 4 * four + (i & 3)];
+            }
+        } else {
+            for (int i = threadIdx.x; i < a.buckets * a.heads; i += DB_THREADS) copies[i] = a.table[i];
+        }
         __syncthreads();
-        table = copies;
     }
     const uint32_t per = (uint32_t)(a.heads / VEC);
     const int64_t total = a.n * per;
@@ -91,22 +101,32 @@ db_forward_kernel(const DbArgs a)
         for (int k = 0; k < VEC; k++) v[k] = add;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float* const row = table + (p.at + j) * a.heads + h;
+            const float* const row = VEC == 8 ? table + (h / 4 * a.buckets + p.at + j) * 32 : table + (p.at + j) * a.heads + h;
             if constexpr (VEC == 1) {
                 v[0] = fmaf(w[j], row[0], v[0]);
             } else {
-                const float4 t = *reinterpret_cast<const float4*>(row);
-                v[0] = fmaf(w[j], t.x, v[0]);
-                v[1] = fmaf(w[j], t.y, v[1]);
-                v[2] = fmaf(w[j], t.z, v[2]);
-                v[3] = fmaf(w[j], t.w, v[3]);
+#pragma unroll
+                for (int k = 0; k < VEC; k += 4) {
+                    const float4 t = *reinterpret_cast<const float4*>(row + (k == 0 ? 0 : a.buckets * 32));
+                    v[k] = fmaf(w[j], t.x, v[k]);
+                    v[k + 1] = fmaf(w[j], t.y, v[k + 1]);
+                    v[k + 2] = fmaf(w[j], t.z, v[k + 2]);
+                    v[k + 3] = fmaf(w[j], t.w, v[k + 3]);
+                }
             }
         }
 #pragma unroll
         for (int k = 0; k < VEC; k++) v[k] = p.inside ? v[k] : -INFINITY;
         float* const out = a.bias + e * a.heads + h;
-        if constexpr (VEC == 1) out[0] = v[0];
-        else *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+        if constexpr (VEC == 1) {
+            out[0] = v[0];
+        } else if constexpr (VEC == 4) {
+            *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+                         "f"(v[6]), "f"(v[7])
+                         : "memory");
+        }
     }
 }
 
@@ -328,17 +348,16 @@ extern "C" int dynb_distance_bias(const float* dist_dev, int64_t n, const float*
     a.dist = dist_dev; a.table = table_dev; a.bias = bias_dev;
     a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff;
     const bool aligned = reinterpret_cast<uintptr_t>(bias_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(table_dev) % 16 == 0;
-    const int vec = aligned && heads % 4 == 0 ? 4 : 1;
-    const int bytes = buckets * heads * 4, smem = bytes <= DB_TABLE_BYTES ? bytes : 0;
+    const bool eight = aligned && heads % 8 == 0 && reinterpret_cast<uintptr_t>(bias_dev) % 32 == 0 && buckets * heads * 32 <= DB_COPIES_BYTES;
+    const int vec = eight ? 8 : aligned && heads % 4 == 0 ? 4 : 1;
+    const bool held = buckets * heads * 4 <= DB_TABLE_BYTES;
     const unsigned blocks = db_blocks(n * (heads / vec));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (smem > 0) {
-        if (vec == 4) db_forward_kernel<4, true><<<blocks, DB_THREADS, smem, s>>>(a);
-        else db_forward_kernel<1, true><<<blocks, DB_THREADS, smem, s>>>(a);
-    } else {
-        if (vec == 4) db_forward_kernel<4, false><<<blocks, DB_THREADS, 0, s>>>(a);
-        else db_forward_kernel<1, false><<<blocks, DB_THREADS, 0, s>>>(a);
-    }
+    if (eight) db_forward_kernel<8, true><<<blocks, DB_THREADS, buckets * heads * 32, s>>>(a);
+    else if (vec == 4 && held) db_forward_kernel<4, true><<<blocks, DB_THREADS, buckets * heads * 4, s>>>(a);
+    else if (vec == 4) db_forward_kernel<4, false><<<blocks, DB_THREADS, 0, s>>>(a);
+    else if (held) db_forward_kernel<1, true><<<blocks, DB_THREADS, buckets * heads * 4, s>>>(a);
+    else db_forward_kernel<1, false><<<blocks, DB_THREADS, 0, s>>>(a);
     DYNB_CUDA_OK(cudaGetLastError());
     return DYNB_OK;
 }
