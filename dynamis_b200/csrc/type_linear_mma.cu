@@ -85,9 +85,9 @@ __device__ __forceinline__ void tm_store(const TmRaw<T>& r, unsigned char* at, i
 }
 
 // Adds the products of one step of 16 summed elements: the parts of `a` are `a_part` apart, those of `b` `b_part` (units of 16 bytes).  A part of `a`
-// stays at the multipliers for its products.  The products of the leading parts go to d, the small ones to `small`, which may be d: they then come
-// first.  The tensor cores cut sums off where they do not fit 24 bits, towards zero, every step: six additions a step to one sum over 2000 rows cost
-// 1.2e-5 of the weights' gradient, one a step to a sum of its own and 1024 rows a tenth of that.
+// stays at the multipliers for its products.  The products of the leading parts go to d, the small ones to `small`.  The tensor cores cut sums off
+// where they do not fit 24 bits, towards zero, every step: with six additions a step to one sum, 2000 rows cost 1.2e-5 of the weights' gradient
+// and 400 columns 2e-6 of y; one addition a step to a sum of its own, and 1024 rows, a tenth of that.
 template <int PARTS>
 __device__ __forceinline__ void tm_step(uint32_t d, uint32_t small, uint64_t a, int a_part, uint64_t b, int b_part, uint32_t what, bool add)
 {
@@ -99,7 +99,7 @@ __device__ __forceinline__ void tm_step(uint32_t d, uint32_t small, uint64_t a, 
         tensor_mma_keep<3>(small, a + a_part, b, what, true);
         tensor_mma_keep<1>(small, a, b + 2 * b_part, what, true);
         tensor_mma_keep<2>(small, a, b + b_part, what, true);
-        tensor_mma_keep<3>(d, a, b, what, add || d == small);
+        tensor_mma_keep<3>(d, a, b, what, add);
     }
 }
 
@@ -272,6 +272,13 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
                     __syncwarp();
                     tensor_load_32(from + min(c + 32 * half, plan.column_stride - 32), bits);
                     tensor_wait_loads();
+                    if constexpr (PARTS > 1) {   // the small products' sums
+                        uint32_t small[32];
+                        tensor_load_32(from + 2 * plan.column_stride + min(c + 32 * half, plan.column_stride - 32), small);
+                        tensor_wait_loads();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
+                    }
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         float v[4] = {__uint_as_float(bits[i]), __uint_as_float(bits[i + 1]), __uint_as_float(bits[i + 2]), __uint_as_float(bits[i + 3])};
@@ -339,7 +346,7 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
                     const uint64_t at_a = tile_descriptor(stage_at + stage * STAGE, 16, 1024), at_b = panel_from + (uint32_t)(chunk * plan.b_chunk);
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        if (k < steps) tm_step<PARTS>(sums, sums, at_a + 2 * k, TM_ROWS * 128 / 16, at_b + (uint32_t)(k * plan.b_step), plan.b_part, what, chunk > 0 || k > 0);
+                        if (k < steps) tm_step<PARTS>(sums, sums + 2 * plan.column_stride, at_a + 2 * k, TM_ROWS * 128 / 16, at_b + (uint32_t)(k * plan.b_step), plan.b_part, what, chunk > 0 || k > 0);
                     tensor_commit(&bars.empty[stage]);
                     if (chunk == plan.chunks - 1) tensor_commit(&bars.sums_full[buffer]);
                 }
@@ -612,7 +619,7 @@ static bool tm_rows(const TlArgs& a, int back, cudaStream_t s, cudaError_t* rc)
     for (;; tiles++) {
         p.columns = tm_round((nn + tiles - 1) / tiles, 16);
         p.panel_bytes = back ? p.chunks * PARTS * p.columns * 128 : PARTS * ((p.columns + 63) / 64) * p.chunks * 8192;
-        if (p.columns <= 256 && p.panel_bytes + 2 * STAGE + 1024 <= TM_SMEM) break;
+        if (p.columns <= (PARTS == 1 ? 256 : 128) && p.panel_bytes + 2 * STAGE + 1024 <= TM_SMEM) break;
         if (p.columns == 16) return false;
     }
     tiles = (nn + p.columns - 1) / p.columns;
@@ -621,7 +628,7 @@ static bool tm_rows(const TlArgs& a, int back, cudaStream_t s, cudaError_t* rc)
     p.b_step = (back ? 32 : 2048) / 16;
     p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - p.panel_bytes) / STAGE);
     p.column_stride = tm_round(p.columns, 32);
-    p.tensor_columns = tm_tensor_columns(2 * p.column_stride);
+    p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     const void* const in = back ? a.dy : a.x;
     const void* const out = back ? a.dx : a.y;
     const bool wide = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0;

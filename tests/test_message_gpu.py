@@ -429,20 +429,20 @@ def test_type_linear_strides_and_missing_types(cuda, dtype):
         assert not dw[0::2].any() and not db[0::2].any()
 
 
-def test_type_linear_long_sums_of_one_sign(cuda):
+@pytest.mark.parametrize("inner,outer", [(128, 128), (384, 250)])
+def test_type_linear_long_sums_of_one_sign(cuda, inner, outer):
     """Operands of one sign, where sums that are cut off towards zero lose the most.  A step of 16 products cuts at most 2^-23 of the sum so far off, and a
-    leading sum has at most 1024 / 16 = 64 of them (y, dx: 128 / 16 = 8 steps of six); parts of 24 bits and the rest of the rounding stay
-    within 2^-21."""
+    leading sum has at most 1024 / 16 = 64 of them (y, dx: one for every 16 columns); parts of 24 bits and the rest of the rounding stay within 2^-21."""
     gen = _gen(31)
     n = 150_001
     kinds = _kinds(n, 2, 3).to(cuda)
-    x, w, g = (torch.rand(*s, generator=gen, device="cuda") for s in ((n, 128), (2, 128, 128), (n, 128)))
+    x, w, g = (torch.rand(*s, generator=gen, device="cuda") for s in ((n, inner), (2, inner, outer), (n, outer)))
     leaves = [t.requires_grad_() for t in (x, w)]
     y = D.type_linear(x, w, D.type_index(kinds, 2))
     dx, dw = torch.autograd.grad(y, leaves, g)
     for t in range(2):
         m = torch.nonzero(kinds == t)[:, 0]
-        for got, ref, steps in ((y[m], x[m].double() @ w[t].double(), 48), (dx[m], g[m].double() @ w[t].double().T, 48),
+        for got, ref, steps in ((y[m], x[m].double() @ w[t].double(), inner // 16), (dx[m], g[m].double() @ w[t].double().T, -(-outer // 16)),
                                 (dw[t], x[m].double().T @ g[m].double(), 64)):
             assert float(((got.double() - ref) / ref).abs().max()) <= steps * 2.0 ** -23 + 2.0 ** -21
 
