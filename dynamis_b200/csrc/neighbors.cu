@@ -423,7 +423,7 @@ extern "C" int dynb_neighbor_index_plan(const int64_t* src_dev, const int64_t* d
     const bool publish = scan_publishes(n_sources + 1);
     DYNB_CUDA_OK(exclusive_scan(sorted_count, reinterpret_cast<uint32_t*>(col_start_dev), nullptr, n_sources + 1, reinterpret_cast<uint32_t*>(ws + l.scan),
                                 reinterpret_cast<uint32_t*>(words) + 2, s,
-                                publish ? ScanPublish{reinterpret_cast<const uint4*>(words), static_cast<uint4*>(words_at)} : ScanPublish{}));
+                                publish ? ScanPublish{reinterpret_cast<const uint4*>(words), static_cast<uint4*>(words_at), true} : ScanPublish{}));
     if (!publish)
         DYNB_CUDA_OK(launch_chained(ni_words_kernel, 1, 1, 0, s, reinterpret_cast<const uint4*>(words), static_cast<uint4*>(words_at)));
     return DYNB_OK;

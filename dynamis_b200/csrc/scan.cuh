@@ -198,9 +198,9 @@ scan_apply_pair_kernel(const TIn* in0, TOut* out0, const TIn* in1, TOut* out1, c
                                blockIdx.y ? copy1 : copy0);
 }
 
-// 64 bytes that the thread which writes the grand total copies behind it (dst == nullptr: none): a header that holds the total,
-// to host memory.
-struct ScanPublish { const uint4* src; uint4* dst; };
+// 64 bytes, or the first 16 of them (`first`), that the thread which writes the grand total copies behind it (dst == nullptr: none): a header that
+// holds the total, to host memory.
+struct ScanPublish { const uint4* src; uint4* dst; bool first = false; };
 __device__ __forceinline__ void publish_64_bytes(const uint4* src, uint4* dst)
 {
     uint4 v[4];
@@ -232,7 +232,8 @@ __device__ __forceinline__ TOut scan_prefix_of_sums(const TOut* __restrict__ sum
             *total_out = t + sums[mine];
             if (publish.dst != nullptr) {
                 __threadfence();
-                publish_64_bytes(publish.src, publish.dst);
+                if (publish.first) publish.dst[0] = __ldcg(publish.src);
+                else publish_64_bytes(publish.src, publish.dst);
             }
         }
     }

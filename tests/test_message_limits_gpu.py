@@ -1,0 +1,37 @@
+"""Message-passing operators at the borders of what they promise: bytes behind a result, large and small values, calls without gradients, captures.
+The bounds are derived beside the tests."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import dynamis_b200 as D
+from dynamis_b200 import _lib
+from tests import _message as M
+
+pytestmark = pytest.mark.gpu
+U = M.U
+
+
+# ------------------------------------------------------------------------------------------------ lists
+@pytest.mark.parametrize("sources", [3000, 17_000_000])
+def test_plan_writes_sixteen_bytes_to_the_host(cuda, sources):
+    """The words of the plan are four of 32 bits: what stands behind them in the caller's pinned memory stays.  (Both ways to the host: from the
+    scan's last block, and by a kernel of its own where the scan has many tiles.)"""
+    L, n = _lib.lib(), ctypes.c_int64()
+    degrees = [3, 0, 5, 1]
+    ei, src, dst = M.ragged_graph(degrees, 3000, 1, cuda)
+    E, T = ei.size(1), len(degrees)
+    words = torch.full((64,), -7, dtype=torch.int64).pin_memory()
+    rows, row_start, src32, cols, col_start, in_edge = (torch.empty(m, dtype=torch.int32, device=cuda) for m in (T, T + 1, E, sources, sources + 1, E))
+    _lib.check(L.dynb_neighbor_index_workspace_bytes(E, T, sources, 0, ctypes.byref(n)), "workspace_bytes")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=cuda)
+    _lib.check(L.dynb_neighbor_index_plan(ei[0].data_ptr(), ei[1].data_ptr(), E, T, sources, rows.data_ptr(), row_start.data_ptr(), src32.data_ptr(),
+                                          cols.data_ptr(), col_start.data_ptr(), in_edge.data_ptr(), words.data_ptr(), ws.data_ptr(), ws.numel(),
+                                          _lib.stream_of(cuda)), "plan")
+    torch.cuda.synchronize()
+    assert int(words[0]) & 0xFFFFFFFF == 0 and int(words[0]) >> 32 == int(torch.bincount(src).max())
+    assert (words[2:] == -7).all()
+    assert src32.tolist() == src.tolist() and row_start.tolist() == [0] + torch.cumsum(torch.bincount(dst, minlength=T)[rows.long()], 0).tolist()
