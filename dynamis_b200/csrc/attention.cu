@@ -61,6 +61,7 @@ extern "C" int dynb_neighbor_attention(const dynb_attention* args, void* out_dev
     if (a.n_targets == 0) return DYNB_OK;
     if (out_dev == nullptr) return fail_arg("null pointer");
     const int size = args->dtype == DYNB_F32 ? 4 : 2;
+    if (size == 2 && !starts_on(out32_dev, 8)) return fail_arg("neighbor_attention: out32 must start on an 8-byte boundary");
     a.out = out_dev;
     a.out32_w = out32_dev;
     a.stats_w = stats_dev;
@@ -100,6 +101,7 @@ extern "C" int dynb_neighbor_attention_backward(const dynb_attention* args, cons
     const bool cols = (dk_dev != nullptr || dv_dev != nullptr) && a.n_sources > 0;
     if (a.n_targets > 0) {   // also for the sources' gradients, which read delta
         if (!d_out_dev || !out32_dev || !stats_dev || !delta_dev) return fail_arg("null pointer");
+        if (!starts_on(delta_dev, 16)) return fail_arg("neighbor_attention_backward: delta must start on a 16-byte boundary");
         DYNB_CUDA_OK(attn_backward_rows(a, args->dtype, s));
     }
     if (cols) {

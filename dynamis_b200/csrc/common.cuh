@@ -111,6 +111,7 @@ static inline void* device_view_of_host(void* host)
     return at.type == cudaMemoryTypeHost ? at.devicePointer : nullptr;
 }
 
+static inline bool starts_on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 static inline int64_t align_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 static inline int sm_count_cached()
 {

@@ -393,10 +393,11 @@ extern "C" int dynb_neighbor_index_plan(const int64_t* src_dev, const int64_t* d
     if (row_start_dev == nullptr || col_start_dev == nullptr || workspace_dev == nullptr || words_host == nullptr) return fail_arg("null pointer");
     if ((n_edges > 0 && (!src_dev || !dst_dev || !src32_dev || !in_edge_dev)) || (n_targets > 0 && !rows_dev) || (n_sources > 0 && !cols_dev))
         return fail_arg("null pointer");
+    if (!starts_on(workspace_dev, 16)) return fail_arg("neighbor_index: the workspace must start on a 16-byte boundary");
     const NiLayout l = ni_layout(n_edges, n_targets, n_sources);
     if (workspace_bytes < l.total) return fail_arg("workspace too small");
     void* const words_at = device_view_of_host(words_host);
-    if (words_at == nullptr) return fail_arg("neighbor_index: words_host must be pinned");
+    if (words_at == nullptr) return fail_arg("neighbor_index: words_host must be pinned, on a 16-byte boundary");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
     uint32_t* const run_of = reinterpret_cast<uint32_t*>(ws + l.run_of);
@@ -437,6 +438,7 @@ extern "C" int dynb_neighbor_index_fill(const int64_t* dst_dev, int64_t n_edges,
     if (rc != DYNB_OK) return rc;
     if (n_edges == 0) return DYNB_OK;
     if (!dst_dev || !src32_dev || !col_start_dev || !in_edge_dev || !in_dst_dev || !workspace_dev) return fail_arg("null pointer");
+    if (!starts_on(workspace_dev, 16)) return fail_arg("neighbor_index: the workspace must start on a 16-byte boundary");
     const NiLayout l = ni_layout(n_edges, n_targets, n_sources);
     int64_t sort;
     (void)dynb_radix_sort_workspace_bytes(n_edges, &sort);

@@ -267,10 +267,11 @@ extern "C" int dynb_type_index(const int64_t* types_dev, int64_t n_rows, int typ
     if (n_rows < 0 || n_rows >= INT32_MAX) return fail_arg("type_index: rows must lie in [0, 2^31 - 1)");
     if (types < 1 || types > DYNB_TYPE_LINEAR_MAX_TYPES) return fail_arg("type_index: types must lie in [1, 4096]");
     if (!start_dev || !workspace_dev || !word_host || (n_rows > 0 && (!types_dev || !order_dev))) return fail_arg("null pointer");
+    if (!starts_on(workspace_dev, 16)) return fail_arg("type_index: the workspace must start on a 16-byte boundary");
     const TiLayout l = ti_layout(n_rows);
     if (workspace_bytes < l.total) return fail_arg("workspace too small");
     void* const word_at = device_view_of_host(word_host);
-    if (word_at == nullptr) return fail_arg("type_index: word_host must be pinned");
+    if (word_at == nullptr) return fail_arg("type_index: word_host must be pinned, on a 16-byte boundary");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
     uint32_t* const word = reinterpret_cast<uint32_t*>(ws + l.word);

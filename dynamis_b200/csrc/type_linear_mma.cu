@@ -666,7 +666,7 @@ static cudaError_t tm_weights(const TlArgs& a, cudaStream_t s)
     p.stages = std::min(TM_MAX_STAGES, (TM_SMEM - 1024 - TM_ROWS * 128) / stage);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
-    p.vec = a.outer % 4 == 0;
+    p.vec = a.outer % 4 == 0 && tm_on(a.partial, 0, 4, 16);
     const dim3 grid((unsigned)tl_stretches(a.n, a.types, a.stretch), (a.inner + TM_ROWS - 1) / TM_ROWS, (a.outer + p.columns - 1) / p.columns);
     const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;
     void (*const kernel)(TlArgs, TwPlan) = wide ? tm_weights_kernel<T, true> : tm_weights_kernel<T, false>;

@@ -35,3 +35,22 @@ def test_plan_writes_sixteen_bytes_to_the_host(cuda, sources):
     assert int(words[0]) & 0xFFFFFFFF == 0 and int(words[0]) >> 32 == int(torch.bincount(src).max())
     assert (words[2:] == -7).all()
     assert src32.tolist() == src.tolist() and row_start.tolist() == [0] + torch.cumsum(torch.bincount(dst, minlength=T)[rows.long()], 0).tolist()
+
+
+def test_weights_gradient_with_a_workspace_off_sixteen_bytes(cuda):
+    """The sums of stretches go to a workspace on any 4-byte boundary, by whole pieces where it allows."""
+    L, n = _lib.lib(), ctypes.c_int64()
+    x, w, g = (torch.randn(*s, device=cuda) for s in ((300, 64), (2, 64, 32), (300, 32)))
+    index = D.type_index((torch.arange(300, device=cuda) % 2), 2)
+    a = _lib.TypeLinear()
+    a.weight_dev, a.order_dev, a.start_dev = w.data_ptr(), index.order.data_ptr(), index.start.data_ptr()
+    a.n_rows, a.types, a.inner, a.outer, a.dtype = 300, 2, 64, 32, _lib.DYNB_F32
+    _lib.check(L.dynb_type_linear_workspace_bytes(ctypes.byref(a), ctypes.byref(n)), "workspace_bytes")
+    got = []
+    for off in (0, 4):
+        ws, dw, db = torch.empty(n.value + 16, dtype=torch.uint8, device=cuda), torch.empty_like(w), torch.empty(2, 32, device=cuda)
+        _lib.check(L.dynb_type_linear_backward(ctypes.byref(a), x.data_ptr(), 64, g.data_ptr(), 32, None, dw.data_ptr(), db.data_ptr(),
+                                               ws.data_ptr() + off, n.value, _lib.stream_of(cuda)), "backward")
+        torch.cuda.synchronize()
+        got.append((dw, db))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
