@@ -22,7 +22,7 @@ struct DbArgs {
     float *bias, *d_dist, *partial, *d_table;
     int64_t n;
     int heads, buckets, smooth;
-    float cutoff;
+    float cutoff, per;   // per: (buckets - 3) / cutoff
 };
 
 struct DbPlace {
@@ -38,9 +38,12 @@ __device__ __forceinline__ DbPlace db_place(float r, const DbArgs& a)
     p.inside = !(pos >= a.cutoff);
     p.u = pos / a.cutoff;
     p.rest = (a.cutoff - pos) / a.cutoff;
-    const float x = p.u * (float)(a.buckets - 3);
+    // What rounding took from the quotient and from the product comes back behind the subtraction, which is exact: t is off by 2^-24 whatever the number
+    // of buckets is (without it by 2^-24 of x; both products that it takes are exact).  A t that falls beside [0, 1] by it stays with its bucket: the neighbour's
+    // cubic differs by the third power of that.
+    const float pieces = (float)(a.buckets - 3), x = p.u * pieces;
     p.at = min(max((int)x, 0), a.buckets - 4);
-    p.t = x - (float)p.at;
+    p.t = (x - (float)p.at) + fmaf(fmaf(-p.u, a.cutoff, pos), a.per, fmaf(p.u, pieces, -x));
     return p;
 }
 
@@ -328,6 +331,9 @@ static int db_check(int64_t n, int heads, int buckets, double cutoff)
     return DYNB_OK;
 }
 
+// Of cutoffs so small that the remainder of a quotient by them has no room, 0.
+static float db_per(int buckets, float cutoff) { return cutoff > 1e-30f ? (float)(buckets - 3) / cutoff : 0.0f; }
+
 static unsigned db_blocks(int64_t n)
 {
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + DB_THREADS - 1) / DB_THREADS, (int64_t)sm_count_cached() * 8));
@@ -346,7 +352,7 @@ extern "C" int dynb_distance_bias(const float* dist_dev, int64_t n, const float*
     if (!dist_dev || !table_dev || !bias_dev) return fail_arg("null pointer");
     DbArgs a = {};
     a.dist = dist_dev; a.table = table_dev; a.bias = bias_dev;
-    a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff;
+    a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff; a.per = db_per(buckets, a.cutoff);
     const bool aligned = reinterpret_cast<uintptr_t>(bias_dev) % 16 == 0 && reinterpret_cast<uintptr_t>(table_dev) % 16 == 0;
     const bool eight = aligned && heads % 8 == 0 && reinterpret_cast<uintptr_t>(bias_dev) % 32 == 0 && buckets * heads * 32 <= DB_COPIES_BYTES;
     const int vec = eight ? 8 : aligned && heads % 4 == 0 ? 4 : 1;
@@ -380,7 +386,7 @@ extern "C" int dynb_distance_bias_backward(const float* dist_dev, int64_t n, con
     if (n > 0 && (!dist_dev || !table_dev || !d_bias_dev)) return fail_arg("null pointer");
     DbArgs a = {};
     a.dist = dist_dev; a.table = table_dev; a.d_bias = d_bias_dev; a.d_dist = d_dist_dev; a.d_table = d_table_dev;
-    a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff;
+    a.n = n; a.heads = heads; a.buckets = buckets; a.smooth = smooth; a.cutoff = (float)cutoff; a.per = db_per(buckets, a.cutoff);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int blocks = db_table_blocks(n);
     if (d_table_dev != nullptr) {

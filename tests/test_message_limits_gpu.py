@@ -54,3 +54,49 @@ def test_weights_gradient_with_a_workspace_off_sixteen_bytes(cuda):
         torch.cuda.synchronize()
         got.append((dw, db))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+# ------------------------------------------------------------------------------------------------ distance bias
+@pytest.mark.parametrize("buckets,heads,smooth", [(64, 8, False), (300, 8, False), (300, 8, True), (1024, 8, False), (1024, 3, True), (1000, 40, False)])
+def test_distance_bias_keeps_its_place_among_many_buckets(cuda, buckets, heads, smooth):
+    """The place between two buckets is off by 2 u (the sum of its exact leading part and a small one, and that small one's own roundings) however many
+    buckets stand below it: no bound here grows with the place.  Bias: the spline's slope is at most 2 of the largest value nearby (reach), its products and
+    weights are off by 12 u of their magnitudes, the logarithms as in test_message_gpu.py.  d_dist: the second derivative is at most 4 reach a bucket,
+    the weights' derivatives are off by 8 u twice over, sums of heads.  d_table: the weights' slopes are at most 0.75."""
+    gen, cutoff, edges = torch.Generator(device="cuda").manual_seed(buckets + heads), 5.0, 20011
+    r = 5.0 * torch.rand(edges, generator=gen, device="cuda")
+    r[:3] = torch.stack([torch.nextafter(torch.tensor(cutoff), torch.tensor(0.0)), torch.tensor(0.0), torch.tensor(cutoff / (buckets - 3))])
+    table = torch.randn(buckets, heads, generator=gen, device="cuda")
+    g = torch.randn(edges, heads, generator=gen, device="cuda")
+    leaves = [r.requires_grad_(), table.requires_grad_()]
+    bias = D.distance_bias(*leaves, cutoff, smooth)
+    d_dist, d_table = torch.autograd.grad(bias, leaves, g)
+    rd, td = r.detach().double(), table.detach().double()
+    x = rd / cutoff * (buckets - 3)
+    at = x.long().clamp(0, buckets - 4)
+    t = x - at
+    near = torch.stack([td[at + j] for j in range(4)])
+    w = torch.stack([(1 - t) ** 3, 3 * t ** 3 - 6 * t ** 2 + 4, -3 * t ** 3 + 3 * t ** 2 + 3 * t + 1, t ** 3]) / 6
+    dw = torch.stack([-(1 - t) ** 2, 3 * t ** 2 - 4 * t, -3 * t ** 2 + 2 * t + 1, t ** 2]) / 2
+    reach = near.abs().amax(0)
+    value = (w[..., None] * near).sum(0)
+    slack = 12 * U * (w[..., None] * near.abs()).sum(0) + 2 * reach * 2 * U
+    slope = (dw[..., None] * near).sum(0) * (buckets - 3)
+    pull = torch.zeros_like(rd)[:, None]
+    if smooth:
+        u = rd / cutoff
+        logs = (3 * torch.log1p(-u).abs() + torch.log1p(3 * u + 6 * u * u))[:, None]
+        value = value + (3 * torch.log1p(-u) + torch.log1p(3 * u + 6 * u * u))[:, None]
+        slack = slack + 8 * U * logs + 14 * U
+        pull = (30 * u * u / ((1 - u) * (1 + 3 * u + 6 * u * u)))[:, None]
+    M.check(bias.detach(), value, slack + 4 * U * value.abs(), "bias")
+    G, gd = g.double().abs(), g.double()
+    size = (buckets - 3) * 2 * reach + pull
+    off = (buckets - 3) * reach * (4 * 2 + 16) * U + 12 * U * pull
+    M.check(d_dist, (gd * (slope - pull)).sum(1) / cutoff, (G * (off + (heads + 4) * U * size)).sum(1) / cutoff, "d_dist")
+    want, w_off = torch.zeros_like(td), torch.zeros_like(td)
+    per = (edges + 147) // 148 + 40
+    for j in range(4):
+        want.index_add_(0, at + j, w[j][:, None] * gd)
+        w_off.index_add_(0, at + j, G * (0.75 * 2 + 8 + per) * U)
+    M.check(d_table, want, w_off, "d_table")
