@@ -136,7 +136,8 @@ db_forward_kernel(const DbArgs a)
 // Both gradients from one reading of the bias's gradient, for up to 32 heads.  A warp takes 32 edges at a time: every lane works out the
 // place, the weights and the slopes of one of them, then WIDE rounds follow in which the lanes are 32 / WIDE edges times WIDE heads.  A lane has
 // a column of its own in the warp's copy of the table's gradient, [buckets][32]: no atomics, no two lanes in one bank, and the order of
-// its sums is that of the edges.  Blocks write their sums; db_table_join_kernel adds these in 64 bits.
+// its sums is that of the edges.  Sums of a column and of a block are in 32 bits: short ones (10.5 M edges, 64 x 8: a column of fifty terms, 88
+// columns a block) whose roundings are independent; db_table_join_kernel adds those of the blocks in 64.
 // What bounds it is shared memory: 16 reads and writes a round (10.5 M edges, 64 x 8: 0.29 ms, 1.4 TB/s; 16 warps 0.33).  The two gradients in
 // kernels of their own, without rounds: 0.30 and 1.10 ms.
 constexpr int DB_SCRATCH = 32 * 12;   // floats of a warp: weights, slopes, {place, pull} of 32 edges, 16 + 16 + 16 bytes each
