@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 from dataclasses import dataclass
 from typing import Optional
 
@@ -110,6 +111,16 @@ class TypeIndex:
         _lists("TypeIndex", ("order", "start"), (self.order, self.start))
         if self.start.numel() < 2 or self.start.numel() > MAX_TYPES + 1:
             raise RuntimeError(f"TypeIndex: the number of types must lie in [1, {MAX_TYPES}], got {self.start.numel() - 1}")
+        if self.order.get_device() not in _STATUS:
+            _make_status_word(self.order.device)
+
+    def check_status(self) -> None:
+        """Synchronises and raises if a wait inside a kernel of a ``type_linear`` on this device ran out, whose results are not valid then.  ``type_linear``
+        looks, without waiting, before it launches; behind the last call, or where a graph replays the calls, look here."""
+        dev = self.order.device
+        torch.cuda.synchronize(dev)
+        with _lib.on_device(dev):
+            _status_word(dev)
 
     @property
     def num_types(self) -> int:
@@ -382,19 +393,36 @@ def type_index(types: torch.Tensor, num_types: int) -> TypeIndex:
     return TypeIndex(order, start)
 
 
-_STATUS: dict = {}   # device -> (host word, device address): set by a kernel whose bounded wait ran out
+_STATUS: dict = {}   # device -> (host word, device address): set by a kernel whose bounded wait ran out; kept as long as the process, graphs hold the address
+_STATUS_LOCK = threading.Lock()
+
+
+def _new_status_word():
+    hp, dp = ctypes.c_void_p(), ctypes.c_void_p()
+    _lib.check(_lib.lib().dynb_host_alloc_mapped(8, ctypes.byref(hp), ctypes.byref(dp)), "host_alloc_mapped")
+    word = ctypes.c_uint32.from_address(hp.value)
+    word.value = 0
+    return word, dp.value
+
+
+def _make_status_word(dev) -> None:
+    """The device's status word, once, whichever thread comes first; none while the current stream is being captured, when memory cannot be had."""
+    with _lib.on_device(dev):
+        if torch.cuda.is_current_stream_capturing():
+            return
+        with _STATUS_LOCK:
+            if dev.index not in _STATUS:
+                _STATUS[dev.index] = _new_status_word()
 
 
 def _status_word(dev) -> int:
-    """Device address of the device's status word (0: none yet).  Raises when an earlier call's kernel gave up waiting."""
+    """Device address of the device's status word.  Raises when an earlier call's kernel gave up waiting."""
     found = _STATUS.get(dev.index)
     if found is None:
-        if torch.cuda.is_current_stream_capturing():   # memory cannot be had now
-            return 0
-        hp, dp = ctypes.c_void_p(), ctypes.c_void_p()
-        _lib.check(_lib.lib().dynb_host_alloc_mapped(8, ctypes.byref(hp), ctypes.byref(dp)), "host_alloc_mapped")
-        found = _STATUS[dev.index] = (ctypes.c_uint32.from_address(hp.value), dp.value)
-        found[0].value = 0
+        _make_status_word(dev)
+        found = _STATUS.get(dev.index)
+        if found is None:
+            raise RuntimeError("type_linear: the first index of a device must be made before a capture, so that a wait that runs out can be told")
     if found[0].value:
         found[0].value = 0
         raise RuntimeError("type_linear: a wait inside a kernel of an earlier call ran out; its results are not valid")
@@ -403,7 +431,7 @@ def _status_word(dev) -> int:
 
 def _linear_args(x, weight, index: TypeIndex) -> "_lib.TypeLinear":
     a = _lib.TypeLinear()
-    a.status_dev = _status_word(x.device) or None
+    a.status_dev = _status_word(x.device)
     a.weight_dev, a.order_dev, a.start_dev = weight.data_ptr(), index.order.data_ptr(), index.start.data_ptr()
     a.n_rows, a.types, a.inner, a.outer, a.dtype = x.size(0), weight.size(0), weight.size(1), weight.size(2), _DTYPES[x.dtype]
     return a

@@ -100,3 +100,30 @@ def test_distance_bias_keeps_its_place_among_many_buckets(cuda, buckets, heads, 
         want.index_add_(0, at + j, w[j][:, None] * gd)
         w_off.index_add_(0, at + j, G * (0.75 * 2 + 8 + per) * U)
     M.check(d_table, want, w_off, "d_table")
+
+
+# ------------------------------------------------------------------------------------------------ products by type
+def test_a_wait_that_ran_out_in_a_replay_is_told(cuda, monkeypatch):
+    """Making the index makes the word, so that the first product may be a captured one; behind a replay the index tells (the word is set from the host here)."""
+    from dynamis_b200 import message
+
+    monkeypatch.setattr(message, "_STATUS", {})
+    index = D.type_index(torch.tensor([0, 1, 1], device=cuda), 2)
+    x, w = torch.randn(3, 8, device=cuda), torch.randn(2, 8, 4, device=cuda)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = D.type_linear(x, w, index)
+    graph.replay()
+    index.check_status()
+    M.check(y, torch.stack([x[0].double() @ w[0].double(), *(x[1:].double() @ w[1].double())]), 25 * U * torch.full((3, 4), 8.0, device=cuda) * x.abs().max() * w.abs().max(), "y")
+    message._STATUS[x.device.index][0].value = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        index.check_status()
+    index.check_status()
+    # lists made by hand under a capture, on a device without a word: refused, and the next call answers
+    monkeypatch.setattr(message, "_STATUS", {})
+    with pytest.raises(RuntimeError, match="before a capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            D.type_linear(x, w, D.TypeIndex(index.order, index.start))
+    assert torch.equal(D.type_linear(x, w, D.TypeIndex(index.order, index.start)), y)
