@@ -56,6 +56,29 @@ def _lists(what: str, names, lists) -> None:
         on = at
 
 
+def _lists_refused(what: str, checks) -> None:
+    """``checks``: pairs of a text and a function that says whether it holds, taken in turn (a later one may rely on the earlier ones)."""
+    _not_capturing(what)
+    for text, holds in checks:
+        if not holds():
+            raise RuntimeError(f"{what}: {text}")
+
+
+def _each_once(t: torch.Tensor) -> bool:
+    """Whether ``t`` [n] names every number below n once."""
+    n = t.numel()
+    return n == 0 or bool(((t >= 0) & (t < n)).all()) and bool((torch.bincount(t, minlength=n) == 1).all())
+
+
+def _runs(start: torch.Tensor, n: int) -> bool:
+    return int(start[0]) == 0 and int(start[-1]) == n and bool((start[1:] >= start[:-1]).all())
+
+
+def _spread(t: torch.Tensor, start: torch.Tensor) -> torch.Tensor:
+    """The entry of ``t`` that every place of its run belongs to."""
+    return torch.repeat_interleave(t, (start[1:] - start[:-1]).long())
+
+
 _NEIGHBOR_LISTS = ("rows", "row_start", "src", "cols", "col_start", "in_edge", "in_dst")
 
 
@@ -68,6 +91,9 @@ class NeighborIndex:
     src [E]                       sources of the edges
     cols [S], col_start [S + 1]   sources in the order of their first edge, those without edges behind them (ascending)
     in_edge [E], in_dst [E]       edges that leave ``cols[c]``, ascending, at ``col_start[c]`` and on, and their targets
+
+    ``neighbor_index`` makes them.  Lists made by hand have to be as described: entries out of range are passed over, but results of rows that ``rows`` or ``cols``
+    leave out or name twice, and of edges that no run holds, are not defined (memory may show that was not written).  ``check_lists`` looks.
     """
 
     rows: torch.Tensor
@@ -86,6 +112,19 @@ class NeighborIndex:
         if self.in_edge.numel() != E or self.in_dst.numel() != E:
             raise RuntimeError("NeighborIndex: src, in_edge and in_dst must have one entry per edge")
 
+    def check_lists(self) -> None:
+        """Waits and raises if the lists are not those of one graph: for lists that ``neighbor_index`` did not make."""
+        E, S = self.num_edges, self.num_sources
+        _lists_refused("NeighborIndex", (
+            ("rows must name every target once", lambda: _each_once(self.rows)),
+            ("cols must name every source once", lambda: _each_once(self.cols)),
+            ("in_edge must name every edge once", lambda: _each_once(self.in_edge)),
+            (f"row_start must rise from 0 to {E}", lambda: _runs(self.row_start, E)),
+            (f"col_start must rise from 0 to {E}", lambda: _runs(self.col_start, E)),
+            (f"src must lie in [0, {S})", lambda: bool(((self.src >= 0) & (self.src < S)).all())),
+            ("in_edge must list the edges of cols", lambda: torch.equal(self.src[self.in_edge.long()], _spread(self.cols, self.col_start))),
+            ("in_dst must hold the targets of in_edge", lambda: torch.equal(_spread(self.rows, self.row_start)[self.in_edge.long()], self.in_dst))))
+
     @property
     def num_targets(self) -> int:
         return self.rows.numel()
@@ -102,7 +141,10 @@ class NeighborIndex:
 @dataclass(frozen=True)
 class TypeIndex:
     """Rows by type (int32): ``order`` [N] lists the rows of type 0, of type 1, ..., ascending inside a type, every row once;
-    ``start`` [types + 1] is where every type begins."""
+    ``start`` [types + 1] is where every type begins, and N behind the last.
+
+    ``type_index`` makes them.  Lists made by hand have to be as described: entries out of range are passed over, but results of rows that are left out or
+    named twice are not defined (memory may show that was not written).  ``check_lists`` looks."""
 
     order: torch.Tensor
     start: torch.Tensor
@@ -113,6 +155,12 @@ class TypeIndex:
             raise RuntimeError(f"TypeIndex: the number of types must lie in [1, {MAX_TYPES}], got {self.start.numel() - 1}")
         if self.order.get_device() not in _STATUS:
             _make_status_word(self.order.device)
+
+    def check_lists(self) -> None:
+        """Waits and raises if the lists do not give every row one type: for lists that ``type_index`` did not make."""
+        N = self.order.numel()
+        _lists_refused("TypeIndex", (("order must name every row once", lambda: _each_once(self.order)),
+                                     (f"start must rise from 0 to {N}", lambda: _runs(self.start, N))))
 
     def check_status(self) -> None:
         """Synchronises and raises if a wait inside a kernel of a ``type_linear`` on this device ran out, whose results are not valid then.  ``type_linear``

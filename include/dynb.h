@@ -445,7 +445,8 @@ int dynb_integrator_step(int kind, float* pos_dev, float* vel_dev, const float* 
  * memory, four 32-bit words: word 0 has bit 0 set when an endpoint is out of range and bit 1 when the edges of a target are apart
  * (nothing else is valid then), word 1 is the longest list of a source.  The caller waits for the stream and calls the fill with word 1 and
  * the workspace of the plan.  The workspace for a longest list of 0 does for the plan and for lists of up to 256 edges; for longer ones the fill
- * takes a larger one, which begins with the bytes of the plan's.  words_host and the workspaces start on 16-byte boundaries. */
+ * takes a larger one, which begins with the bytes of the plan's.  Lists made otherwise have to be as described: the calls below pass over entries out of
+ * range, but do not write results of rows that rows or cols leave out, nor of edges that no run holds.  words_host and the workspaces start on 16-byte boundaries. */
 #define DYNB_MAX_EDGES ((1ll << 31) - (1ll << 16))
 int dynb_neighbor_index_workspace_bytes(int64_t n_edges, int64_t n_targets, int64_t n_sources, int64_t longest, int64_t* bytes);
 int dynb_neighbor_index_plan(const int64_t* src_dev, const int64_t* dst_dev, int64_t n_edges, int64_t n_targets, int64_t n_sources,
@@ -492,7 +493,7 @@ int dynb_distance_bias_backward(const float* dist_dev, int64_t n, const float* t
                                 void* stream);
 
 /* Rows by type: order[n_rows] lists the rows of type 0, of type 1, ..., ascending inside a type; start[types + 1].  word_host (pinned):
- * bit 0 when a type lies outside [0, types).  word_host and the workspace start on 16-byte boundaries. */
+ * bit 0 when a type lies outside [0, types).  The products do not write the results of rows that an order made otherwise leaves out.  word_host and the workspace start on 16-byte boundaries. */
 #define DYNB_TYPE_LINEAR_MAX_TYPES 4096
 #define DYNB_TYPE_LINEAR_MAX_WIDTH 16384
 int dynb_type_index_workspace_bytes(int64_t n_rows, int64_t* bytes);

@@ -127,3 +127,41 @@ def test_a_wait_that_ran_out_in_a_replay_is_told(cuda, monkeypatch):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             D.type_linear(x, w, D.TypeIndex(index.order, index.start))
     assert torch.equal(D.type_linear(x, w, D.TypeIndex(index.order, index.start)), y)
+
+
+# ------------------------------------------------------------------------------------------------ lists made by hand
+def test_lists_made_by_hand_are_looked_at(cuda):
+    ei, src, dst = M.ragged_graph([3, 0, 4, 2], 6, 3, cuda)
+    good = D.neighbor_index(ei, 4, 6)
+    good.check_lists()
+    names = ("rows", "row_start", "src", "cols", "col_start", "in_edge", "in_dst")
+
+    def changed(match, name, at, to):
+        lists = {n: getattr(good, n).clone() for n in names}
+        lists[name][at] = to
+        with pytest.raises(RuntimeError, match=match):
+            D.NeighborIndex(**lists).check_lists()
+
+    changed("rows must name", "rows", 0, int(good.rows[1]))
+    changed("rows must name", "rows", 0, 4)
+    changed("cols must name", "cols", 2, -1)
+    changed("in_edge must name", "in_edge", 3, int(good.in_edge[4]))
+    changed("row_start must rise", "row_start", 0, 1)
+    changed("row_start must rise", "row_start", 4, 8)
+    changed("row_start must rise", "row_start", 1, 1 + int(good.row_start[2]))
+    changed("col_start must rise", "col_start", 6, 10)
+    changed("src must lie", "src", 5, 6)
+    other = (int(good.src[0]) + 1) % 6
+    changed("in_edge must list", "src", 0, other)
+    changed("in_dst must hold", "in_dst", 0, (int(good.in_dst[0]) + 1) % 4)
+    for T, S in ((0, 0), (0, 5), (4, 0)):
+        D.neighbor_index(torch.empty((2, 0), dtype=torch.int64, device=cuda), T, S).check_lists()
+
+    types = D.type_index(torch.tensor([2, 0, 2, 0], device=cuda), 4)
+    types.check_lists()
+    D.type_index(torch.empty(0, dtype=torch.int64, device=cuda), 3).check_lists()
+    for order, start, match in (([1, 3, 0, 0], [0, 2, 2, 4, 4], "order must name"), ([1, 3, 0, 4], [0, 2, 2, 4, 4], "order must name"),
+                                ([1, 3, 0, 2], [0, 2, 2, 3, 3], "start must rise"), ([1, 3, 0, 2], [1, 2, 2, 4, 4], "start must rise"),
+                                ([1, 3, 0, 2], [0, 3, 2, 4, 4], "start must rise")):
+        with pytest.raises(RuntimeError, match=match):
+            D.TypeIndex(*(torch.tensor(t, dtype=torch.int32, device=cuda) for t in (order, start))).check_lists()
