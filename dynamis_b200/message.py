@@ -237,7 +237,9 @@ def neighbor_index(edge_index: torch.Tensor, num_targets: int, num_sources: int)
 
 def _heads_last(t: torch.Tensor) -> torch.Tensor:
     """``t`` as the kernels read it: any strides of rows (below 2^30 elements) and heads, the elements of a head consecutive."""
-    return t if (t.stride(2) == 1 or t.size(2) == 1) and t.stride(0) < MAX_ROW else t.contiguous()
+    if (t.stride(2) == 1 or t.size(2) == 1) and t.stride(0) < MAX_ROW:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)   # contiguous() would keep the stride of a single row, whatever it is
 
 
 def _pointer(t: Optional[torch.Tensor]):

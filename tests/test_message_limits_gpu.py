@@ -165,3 +165,18 @@ def test_lists_made_by_hand_are_looked_at(cuda):
                                 ([1, 3, 0, 2], [0, 3, 2, 4, 4], "start must rise")):
         with pytest.raises(RuntimeError, match=match):
             D.TypeIndex(*(torch.tensor(t, dtype=torch.int32, device=cuda) for t in (order, start))).check_lists()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def test_attention_of_a_single_row_with_any_stride(cuda):
+    """A dimension of one element may carry any stride: a row stride beyond what the kernels take is of no meaning here."""
+    index = D.neighbor_index(torch.zeros((2, 1), dtype=torch.int64, device=cuda), 1, 1)
+    base = torch.randn(3, 2, 8, device=cuda)
+    q, k, v = (torch.as_strided(base, (1, 2, 8), (1 << 30, 8, 1), 16 * i) for i in range(3))
+    assert q.stride(0) == 1 << 30
+    assert torch.equal(D.neighbor_attention(q, k, v, index), base[2:])   # one edge: its values
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    g = torch.as_strided(torch.randn(16, device=cuda), (1, 2, 8), (1 << 30, 8, 1))
+    dq, dk, dv = torch.autograd.grad(D.neighbor_attention(*leaves, index), leaves, g)
+    # p = 1 and delta = dp: ds is the difference of two sums of eight products of the same numbers
+    assert torch.equal(dv, g) and float(dq.abs().max()) <= 16 * U * float((g * v).abs().sum() * k.abs().max()) and dk.shape == k.shape
