@@ -262,13 +262,13 @@ def _attention_args(q, k, v, bias, index: NeighborIndex, scale: float) -> "_lib.
 
 class _NeighborAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, index, scale):
+    def forward(ctx, q, k, v, bias, index, scale, keep):
         dev = q.device
         q, k, v = _heads_last(q), _heads_last(k), _heads_last(v)
         with _lib.on_device(dev):
             out = torch.empty(q.shape, dtype=q.dtype, device=dev)
             out32 = stats = None
-            if any(ctx.needs_input_grad):
+            if keep:
                 out32 = out if q.dtype == torch.float32 else torch.empty(q.shape, dtype=torch.float32, device=dev)
                 stats = torch.empty((q.size(0), 2, q.size(1)), dtype=torch.float32, device=dev)
             args = _attention_args(q, k, v, bias, index, scale)
@@ -297,7 +297,7 @@ class _NeighborAttention(torch.autograd.Function):
                 ctypes.byref(args), d_out.data_ptr(), d_out.stride(0), d_out.stride(1), out32.data_ptr(), stats.data_ptr(), index.cols.data_ptr(),
                 index.col_start.data_ptr(), index.in_edge.data_ptr(), index.in_dst.data_ptr(), delta.data_ptr(), _pointer(dq), _pointer(dk),
                 _pointer(dv), _pointer(d_bias), _lib.stream_of(dev)), "neighbor_attention_backward")
-        return dq, dk, dv, d_bias, None, None
+        return dq, dk, dv, d_bias, None, None, None
 
 
 def neighbor_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index: NeighborIndex, bias: Optional[torch.Tensor] = None,
@@ -344,7 +344,9 @@ def neighbor_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise RuntimeError(f"scale must be finite, got {scale}")
-    return _NeighborAttention.apply(q, k, v, bias, index, scale)
+    # what the backward pass reads is kept where there can be one (needs_input_grad says yes under no_grad, too)
+    keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))
+    return _NeighborAttention.apply(q, k, v, bias, index, scale, keep)
 
 
 class _DistanceBias(torch.autograd.Function):
