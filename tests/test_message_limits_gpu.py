@@ -177,9 +177,12 @@ def test_attention_of_a_single_row_with_any_stride(cuda):
     assert torch.equal(D.neighbor_attention(q, k, v, index), base[2:])   # one edge: its values
     leaves = [t.detach().requires_grad_() for t in (q, k, v)]
     g = torch.as_strided(torch.randn(16, device=cuda), (1, 2, 8), (1 << 30, 8, 1))
-    dq, dk, dv = torch.autograd.grad(D.neighbor_attention(*leaves, index), leaves, g)
-    # p = 1 and delta = dp: ds is the difference of two sums of eight products of the same numbers
-    assert torch.equal(dv, g) and float(dq.abs().max()) <= 16 * U * float((g * v).abs().sum() * k.abs().max()) and dk.shape == k.shape
+    grads = torch.autograd.grad(D.neighbor_attention(*leaves, index), leaves, g)
+    # bounds beside the plain form: by source the logit is rounded in another order than the largest logit was, so that p is not exactly 1 there
+    zero = torch.zeros(1, dtype=torch.int64, device=cuda)
+    ref = M.attention(q, k, v, zero, zero, None, 8 ** -0.5, g)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        M.check(got, *ref[name], name)
 
 
 def test_attention_without_gradients_keeps_nothing_for_them(cuda):
