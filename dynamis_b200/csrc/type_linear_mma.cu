@@ -57,8 +57,49 @@ __device__ __forceinline__ TmRaw<T> tm_load(const T* p, int64_t step, int have)
     return u.r;
 }
 
-// The parts of eight elements, 16 bytes each, to `at`, `at + apart`, ...
-template <typename T>
+// Two elements one of which may not split by rounding, part by part: an infinity becomes (1, 0, itself), whose products with finite elements and
+// with another infinity are what they should be; where rounding to 8 bits gives an infinity, the largest number of 8 bits leads; a NaN leads itself.
+__device__ __forceinline__ void tm_split_odd(uint32_t lo, uint32_t hi, uint32_t (&part)[3])
+{
+    uint32_t p[2][3];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t bits = k == 0 ? lo : hi, size = bits & 0x7fffffffu, sign = bits & 0x80000000u;
+        if (size >= 0x7f800000u) {
+            p[k][0] = size == 0x7f800000u ? sign | 0x3f800000u : 0x7fc00000u;
+            p[k][1] = 0;
+            p[k][2] = size == 0x7f800000u ? bits : 0;
+        } else {
+            const float v = __uint_as_float(bits);
+            p[k][0] = size >= 0x7f7f8000u ? sign | 0x7f7f0000u : (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)) << 16;
+            const float rest = v - __uint_as_float(p[k][0]);
+            p[k][1] = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(rest)) << 16;
+            p[k][2] = __float_as_uint(rest - __uint_as_float(p[k][1]));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 3; i++) part[i] = __byte_perm(p[0][i], p[1][i], 0x7632);
+}
+
+// Whether one of these elements is among them (of a NaN this says nothing: it comes through by rounding, too).  Asked once for all pieces of a stage, which costs 8
+// of the 1028 us of all passes over 1 M rows of 128 x 128; a branch at every piece cost 17.
+template <typename T, int N>
+__device__ __forceinline__ bool tm_odd(const TmRaw<T> (&r)[N])
+{
+    if constexpr (sizeof(T) == 2) {
+        return false;
+    } else {
+        float most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(__uint_as_float(reinterpret_cast<const uint32_t*>(&r[k])[i])));
+        return most >= __uint_as_float(0x7f7f8000u);
+    }
+}
+
+// The parts of eight elements, 16 bytes each, to `at`, `at + apart`, ...  ODD: see above.
+template <bool ODD, typename T>
 __device__ __forceinline__ void tm_store(const TmRaw<T>& r, unsigned char* at, int apart)
 {
     if constexpr (sizeof(T) == 2) {
@@ -66,6 +107,16 @@ __device__ __forceinline__ void tm_store(const TmRaw<T>& r, unsigned char* at, i
     } else {
         const uint32_t* const bits = reinterpret_cast<const uint32_t*>(&r);
         uint32_t part[3][4];
+        if constexpr (ODD) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t p[3];
+                tm_split_odd(bits[2 * i], bits[2 * i + 1], p);
+#pragma unroll
+                for (int k = 0; k < 3; k++) *reinterpret_cast<uint32_t*>(at + k * apart + 4 * i) = p[k];
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float v[2] = {__uint_as_float(bits[2 * i]), __uint_as_float(bits[2 * i + 1])};
@@ -196,7 +247,10 @@ __device__ __forceinline__ void tm_panel(const TmPlan& plan, const T* w, unsigne
         const int piece = u % across, r = u / across, c = piece0 + piece * 8;
         const int have = r < rows ? min(8, columns - c) : 0;
         const TmRaw<T> m = tm_load<WIDE>(have > 0 ? w + (int64_t)(row0 + r) * outer + c : w, 1, have);
-        tm_store(m, panel + (piece / 8) * block + tile_piece(r, piece & 7), apart);
+        const TmRaw<T> one[1] = {m};
+        unsigned char* const to = panel + (piece / 8) * block + tile_piece(r, piece & 7);
+        if (tm_odd(one)) tm_store<true>(m, to, apart);
+        else tm_store<false>(m, to, apart);
     }
 }
 
@@ -422,9 +476,14 @@ tm_rows_kernel(const TlArgs a, const TmPlan plan)
                     if (lane == 0) bar_arrive(&bars.panel_full);
                 }
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
+                unsigned char* const to = stage0 + stage * STAGE + tile_piece(tid >> 3, piece);   // FEED_THREADS / 8 rows on: the same place among eight
+                if (tm_odd(v[s])) {
 #pragma unroll
-                for (int i = 0; i < UNITS; i++)
-                    tm_store(v[s][i], stage0 + stage * STAGE + tile_piece((tid >> 3) + (FEED_THREADS / 8) * i, piece), TM_ROWS * 128);
+                    for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * FEED_THREADS * 16, TM_ROWS * 128);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * FEED_THREADS * 16, TM_ROWS * 128);
+                }
                 fence_to_tensor();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bars.full[stage]);
@@ -580,9 +639,15 @@ tm_weights_kernel(const TlArgs a, const TwPlan plan)
         uint32_t phase = 1;
         for (int step = 0; step < steps; step++) {
             if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+            if (tm_odd(v)) {
 #pragma unroll
-            for (int i = 0; i < UNITS; i++)
-                if (row[i] >= 0) tm_store(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                for (int i = 0; i < UNITS; i++)
+                    if (row[i] >= 0) tm_store<true>(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+            } else {
+#pragma unroll
+                for (int i = 0; i < UNITS; i++)
+                    if (row[i] >= 0) tm_store<false>(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+            }
             fence_to_tensor();
             __syncwarp();
             if (lane == 0) bar_arrive(&bars.full[stage]);

@@ -228,3 +228,45 @@ def test_type_linear_cuts_a_sum_off_once_a_step(cuda):
     for name, values in lost.items():
         n = 64 if name == "dw" else 16
         assert all(-2.0 ** -24 <= v <= (n + 1) / 4 * 2.0 ** -23 + 2.0 ** -24 for v in values), (name, values)
+
+
+def _same_kinds(got, want, off, what):
+    """NaN where the 64-bit form has NaN, infinities of its sign where it has them, and the rest within the bounds."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf].double(), want[inf]), what
+    ok = torch.isfinite(want)
+    M.check(torch.where(ok, got, 0.0), torch.where(ok, want, 0.0), torch.where(ok, off, 0.0), what)
+
+
+@pytest.mark.parametrize("inner,outer", [(64, 48), (33, 130), (300, 40), (40, 1200)])
+def test_type_linear_infinities_and_the_largest_numbers(cuda, inner, outer):
+    """float32 operands with infinities, NaN and numbers that round to an infinity in 8 bits, in rows, matrices and gradients: what 64 bits give, whatever the width (the
+    last two are beyond the tensor cores forward and back).  Bounds as in test_message_gpu.py: the parts of the largest numbers leave out 2^-25."""
+    gen, top = torch.Generator(device="cuda").manual_seed(inner), torch.finfo(torch.float32).max
+    kinds = torch.arange(500, device="cuda") % 3
+
+    def away(*shape):      # no zeros: infinity times zero would be a NaN on both sides, and is tested by hand below
+        t = torch.rand(*shape, generator=gen, device="cuda") * 0.1 + 0.05
+        return torch.where(torch.rand(*shape, generator=gen, device="cuda") < 0.5, -t, t)
+
+    for what in ("x", "w", "g"):
+        x, w, g = away(500, inner), away(3, inner, outer), away(500, outer)
+        odd = {"x": x, "w": w.view(-1, outer), "g": g}[what]
+        odd[4, 3], odd[7, 5], odd[9, 2], odd[9, 6], odd[13, 1], odd[16, 0] = math.inf, -math.inf, math.inf, -math.inf, top, -top
+        odd[19, 4], odd[22, 7], odd[25, 9] = math.nan, 3.395e38, 3.3895e38
+        odd[28, 2:10] = torch.tensor([1.0, -1.0, 2.0, -2.0, 0.5, -0.5, 0.25, -0.25], device="cuda") * 2.0 ** 127 * 0.1
+        leaves = [x.requires_grad_(), w.requires_grad_()]
+        y = D.type_linear(x, w, D.type_index(kinds, 3))
+        dx, dw = torch.autograd.grad(y, leaves, g)
+        xd, wd, gd = x.detach().double(), w.detach().double(), g.double()
+        for t in range(3):
+            m = torch.nonzero(kinds == t)[:, 0]
+            for got, a, b, name in ((y.detach()[m], xd[m], wd[t], "y"), (dx[m], gd[m], wd[t].T, "dx"), (dw[t], xd[m].T, gd[m], "dw")):
+                ref = (a[:, :, None] * b[None]).sum(1) if a.size(0) * a.size(1) * b.size(1) < 40_000_000 else a @ b
+                _same_kinds(got, ref, (a.size(1) + 17) * U * (a.abs() @ b.abs()), f"{name} with odd {what}")
+    # an infinity times zero is a NaN, two infinities meet in one
+    x, w = torch.zeros(2, 32, device="cuda"), torch.ones(1, 32, 16, device="cuda")
+    x[0, 3], w[0, 3, 1], w[0, 3, 2] = math.inf, 0.0, -math.inf
+    y = D.type_linear(x, w, D.type_index(torch.zeros(2, dtype=torch.int64, device="cuda"), 1))
+    assert y[0, 0] == math.inf and torch.isnan(y[0, 1]) and y[0, 2] == -math.inf and torch.isnan(y[1, 2]) and y[1, 0] == 0
