@@ -270,3 +270,18 @@ def test_type_linear_infinities_and_the_largest_numbers(cuda, inner, outer):
     x[0, 3], w[0, 3, 1], w[0, 3, 2] = math.inf, 0.0, -math.inf
     y = D.type_linear(x, w, D.type_index(torch.zeros(2, dtype=torch.int64, device="cuda"), 1))
     assert y[0, 0] == math.inf and torch.isnan(y[0, 1]) and y[0, 2] == -math.inf and torch.isnan(y[1, 2]) and y[1, 0] == 0
+
+
+@pytest.mark.parametrize("inner,outer", [(64, 48), (256, 64)])
+def test_type_linear_of_the_smallest_numbers(cuda, inner, outer):
+    """float32 operands below 2^-109 have parts below the smallest steps of bfloat16, 2^-133, and are taken to within that; above, whole.  Beside bounds as in
+    test_message_gpu.py every product may be off by 2^-133 of its other operand."""
+    gen = torch.Generator(device="cuda").manual_seed(outer)
+    kinds = torch.arange(300, device="cuda") % 2
+    for power in (-100, -108, -116, -124, -130):
+        x = (torch.randn(300, inner, generator=gen, device="cuda").double() * 2.0 ** power).float()
+        w = torch.randn(2, inner, outer, generator=gen, device="cuda") * 2.0 ** 100
+        y = D.type_linear(x, w, D.type_index(kinds, 2))
+        for t in range(2):
+            m = torch.nonzero(kinds == t)[:, 0]
+            M.check(y[m], x[m].double() @ w[t].double(), (inner + 17) * U * (x[m].double().abs() @ w[t].double().abs()) + 2.0 ** -133 * w[t].double().abs().sum(0), f"y at 2^{power}")
