@@ -29,7 +29,6 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .graph import give_host_words, lose_host_words, take_host_words
-from .partition import scratch
 
 _DTYPES = {torch.float32: _lib.DYNB_F32, torch.float16: _lib.DYNB_F16, torch.bfloat16: _lib.DYNB_BF16}
 MAX_DIM = 256            # DYNB_ATTENTION_MAX_DIM
@@ -209,7 +208,7 @@ def neighbor_index(edge_index: torch.Tensor, num_targets: int, num_sources: int)
             torch.empty(n, dtype=torch.int32, device=dev) for n in (T, T + 1, E, S, S + 1, E, E))
         nbytes = ctypes.c_int64()
         _lib.check(L.dynb_neighbor_index_workspace_bytes(E, T, S, 0, ctypes.byref(nbytes)), "neighbor_index_workspace_bytes")
-        ws = scratch(dev, "neighbor_index", nbytes.value)
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)   # this call's own: behind its wait another thread may use the stream before the fill
         words = take_host_words(2)
         try:
             _lib.check(L.dynb_neighbor_index_plan(src64, dst64, E, T, S, rows.data_ptr(), row_start.data_ptr(), src.data_ptr(), cols.data_ptr(),
@@ -226,7 +225,7 @@ def neighbor_index(edge_index: torch.Tensor, num_targets: int, num_sources: int)
         if status & 2:
             raise RuntimeError("neighbor_index: the edges of a target must stand behind one another")
         if longest > LONGEST_LIST:
-            planned, ws = ws[:nbytes.value], None
+            planned = ws
             _lib.check(L.dynb_neighbor_index_workspace_bytes(E, T, S, longest, ctypes.byref(nbytes)), "neighbor_index_workspace_bytes")
             ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
             _lib.check(L.dynb_copy_async(ws.data_ptr(), planned.data_ptr(), planned.numel(), stream), "copy_async")
@@ -429,7 +428,7 @@ def type_index(types: torch.Tensor, num_types: int) -> TypeIndex:
         start = torch.empty(T + 1, dtype=torch.int32, device=dev)
         nbytes = ctypes.c_int64()
         _lib.check(L.dynb_type_index_workspace_bytes(N, ctypes.byref(nbytes)), "type_index_workspace_bytes")
-        ws = scratch(dev, "type_index", nbytes.value)
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
         words = take_host_words(1)
         try:
             _lib.check(L.dynb_type_index(types.data_ptr(), N, T, order.data_ptr(), start.data_ptr(), words.data_ptr(), ws.data_ptr(), ws.numel(),

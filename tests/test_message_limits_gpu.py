@@ -3,6 +3,7 @@ The bounds are derived beside the tests."""
 
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -285,3 +286,36 @@ def test_type_linear_of_the_smallest_numbers(cuda, inner, outer):
         for t in range(2):
             m = torch.nonzero(kinds == t)[:, 0]
             M.check(y[m], x[m].double() @ w[t].double(), (inner + 17) * U * (x[m].double().abs() @ w[t].double().abs()) + 2.0 ** -133 * w[t].double().abs().sum(0), f"y at 2^{power}")
+
+
+# ------------------------------------------------------------------------------------------------ threads
+class _Wait:
+    """A stream behind whose first wait another thread makes a call on the same stream, before the waiting one goes on."""
+
+    def __init__(self, stream, pending):
+        self.stream, self.pending = stream, pending
+
+    def __getattr__(self, name):
+        return getattr(self.stream, name)
+
+    def synchronize(self):
+        self.stream.synchronize()
+        if self.pending:
+            t = threading.Thread(target=self.pending.pop())
+            t.start()
+            t.join()
+
+
+@pytest.mark.parametrize("hub", [False, True])
+def test_neighbor_index_beside_another_thread(cuda, monkeypatch, hub):
+    """Between the two phases of the lists another thread makes lists of another graph on the same stream: each gets its own."""
+    mine = M.ragged_graph([5, 0, 700 if hub else 40, 3] * 3, 1 if hub else 90, 1, cuda)
+    other = M.ragged_graph([9] * 50, 30, 2, cuda)
+    got, pending, me, real = [], [], threading.get_ident(), torch.cuda.current_stream
+    pending.append(lambda: got.append(D.neighbor_index(other[0], 50, 30)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev=None: _Wait(real(dev), pending) if threading.get_ident() == me else real(dev))
+    index = D.neighbor_index(mine[0], 12, 1 if hub else 90)
+    assert not pending
+    for lists, (_, src, dst), T, S in ((index, mine, 12, 1 if hub else 90), (got[0], other, 50, 30)):
+        for name, want in M.index_lists(src, dst, T, S).items():
+            assert getattr(lists, name).tolist() == want, name
