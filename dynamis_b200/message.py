@@ -341,8 +341,8 @@ def neighbor_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
             raise RuntimeError(f"bias must have shape [{index.num_edges}, {heads}], got {list(bias.shape)}")
         bias = bias.contiguous()
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise RuntimeError(f"scale must be finite, got {scale}")
+    if not math.isfinite(ctypes.c_float(scale).value):
+        raise RuntimeError(f"scale must be finite in single precision, got {scale}")
     # what the backward pass reads is kept where there can be one (needs_input_grad says yes under no_grad, too)
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))
     return _NeighborAttention.apply(q, k, v, bias, index, scale, keep)

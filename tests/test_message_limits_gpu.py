@@ -186,6 +186,15 @@ def test_attention_of_a_single_row_with_any_stride(cuda):
         M.check(got, *ref[name], name)
 
 
+def test_attention_refuses_a_scale_beyond_single_precision(cuda):
+    index = D.neighbor_index(torch.zeros((2, 1), dtype=torch.int64, device=cuda), 1, 1)
+    q = torch.ones(1, 1, 4, device=cuda)
+    for scale in (1e39, -1e300, math.inf, math.nan):
+        with pytest.raises(RuntimeError, match="scale must be finite"):
+            D.neighbor_attention(q, q, q, index, None, scale)
+    assert torch.equal(D.neighbor_attention(q, q, q, index, None, 1e30), q)
+
+
 def test_attention_without_gradients_keeps_nothing_for_them(cuda):
     """Under no_grad the operands of a trained model still ask for gradients: no unrounded result and no statistics are written then (three times the
     memory of a result in 16 bits)."""
