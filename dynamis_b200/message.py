@@ -39,6 +39,7 @@ MAX_TYPES = 4096         # DYNB_TYPE_LINEAR_MAX_TYPES
 MAX_WIDTH = 16384        # DYNB_TYPE_LINEAR_MAX_WIDTH
 LONGEST_LIST = 256       # NI_LONGEST (csrc/neighbors.cu): longer lists take a larger workspace
 INT32_MAX = 2 ** 31 - 1
+FLOAT_MAX = 3.4028234663852886e38
 MAX_EDGES = 2 ** 31 - 2 ** 16   # DYNB_MAX_EDGES
 
 
@@ -341,7 +342,7 @@ def neighbor_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, index:
             raise RuntimeError(f"bias must have shape [{index.num_edges}, {heads}], got {list(bias.shape)}")
         bias = bias.contiguous()
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(ctypes.c_float(scale).value):
+    if not -FLOAT_MAX <= scale <= FLOAT_MAX:
         raise RuntimeError(f"scale must be finite in single precision, got {scale}")
     # what the backward pass reads is kept where there can be one (needs_input_grad says yes under no_grad, too)
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad))
