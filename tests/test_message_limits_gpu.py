@@ -103,6 +103,18 @@ def test_distance_bias_keeps_its_place_among_many_buckets(cuda, buckets, heads, 
     M.check(d_table, want, w_off, "d_table")
 
 
+@pytest.mark.parametrize("edges,buckets,heads", [(1000, 64, 8), (5000, 64, 1), (777, 17, 33), (30, 1024, 3), (4000, 700, 8)])
+def test_distance_bias_wants_some_gradients_only(cuda, edges, buckets, heads):
+    gen = torch.Generator(device="cuda").manual_seed(edges)
+    r, table = 5.2 * torch.rand(edges, generator=gen, device="cuda"), torch.randn(buckets, heads, generator=gen, device="cuda")
+    g = torch.randn(edges, heads, generator=gen, device="cuda")
+    both = [t.detach().requires_grad_() for t in (r, table)]
+    every = torch.autograd.grad(D.distance_bias(*both, 5.0), both, g)
+    for i in range(2):
+        some = [t if j == i else t.detach() for j, t in enumerate(both)]
+        assert torch.equal(torch.autograd.grad(D.distance_bias(*some, 5.0), [both[i]], g)[0], every[i])
+
+
 # ------------------------------------------------------------------------------------------------ products by type
 def test_a_wait_that_ran_out_in_a_replay_is_told(cuda, monkeypatch):
     """Making the index makes the word, so that the first product may be a captured one; behind a replay the index tells (the word is set from the host here)."""
@@ -184,6 +196,23 @@ def test_attention_of_a_single_row_with_any_stride(cuda):
     ref = M.attention(q, k, v, zero, zero, None, 8 ** -0.5, g)
     for name, got in zip(("dq", "dk", "dv"), grads):
         M.check(got, *ref[name], name)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_broadcast_operands(cuda, dtype):
+    """One row of keys for all sources, one head of values for all heads, one row of the result's gradient for all targets, read where they are: the bits of the
+    dense tensors."""
+    gen, T, S = torch.Generator(device="cuda").manual_seed(2), 14, 60
+    ei, _, _ = M.ragged_graph([0, 1, 2, 3, 31, 32, 33, 0, 64, 129, 5, 70, 0, 7], S, 4, cuda)
+    index = D.neighbor_index(ei, T, S)
+    q, k, v, g = (torch.randn(*s, generator=gen, device="cuda").to(M.TYPES[dtype]) for s in ((T, 4, 16), (1, 2, 16), (S, 1, 16), (1, 4, 16)))
+    wide = [q, k.expand(S, 2, 16), v.expand(S, 2, 16), g.expand(T, 4, 16)]
+    results = []
+    for q, k, v, g in (wide, [t.contiguous() for t in wide]):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = D.neighbor_attention(*leaves, index)
+        results.append((out, *torch.autograd.grad(out, leaves, g)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
 def test_attention_refuses_a_scale_beyond_single_precision(cuda):
