@@ -1,4 +1,4 @@
-// What the kernels of neighbour attention share: rows in pieces of 16 bytes a lane, and how a warp's lanes divide heads and edges.
+// What the kernels of neighbour attention share: rows as 32 bytes a lane, and how a warp's lanes divide heads and edges.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -9,8 +9,9 @@
 namespace dynb {
 
 // A warp works on `warp_heads` heads of one row at a time.  G lanes a head hold 32 bytes of it each, and where G * warp_heads < 32 the rest of the
-// warp takes further edges ("slots"): 32 bytes a lane leave few instructions an edge for addresses, sums over lanes and exponentials (113 warp
-// instructions an edge and 1.48 ms with 16 bytes a lane, 64-bit indices and checks at every load; forward, 10.5 M edges of 8 x 16 fp32).
+// warp takes further edges ("slots"): 32 bytes a lane leave few instructions an edge for addresses, sums over lanes and exponentials
+// (forward, 8 x 16 fp32: 34 warp instructions an edge; with 16 bytes a lane, 64-bit indices and checks at every load 113, and 1.48 ms in place of 0.70 for
+// 10.5 M edges).
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float2 fma2(const float2 a, const float2 b, const float2 c)
@@ -198,7 +199,7 @@ __device__ __forceinline__ void attn_store(T* head, const Place<T, G, EL>& place
         }
     }
 }
-// What an edge that takes no part reads in place of its rows.
+// What stands for the operands of a row that is not there (a block's last rows, numbers out of range), read 16 bytes at a time.
 static __device__ __align__(16) unsigned char attn_zeros[DYNB_ATTENTION_MAX_DIM * 4];
 
 template <int G>

@@ -4,8 +4,10 @@
 // Two passes, one over the lists by target and one over the lists by source, each of which adds up a row in registers in the order of
 // its list: no atomics, results do not change from run to run, and nothing of the size of the edges is kept but the bias's gradient.
 //
-// Latency and issue bound both, as forward.  200 k targets, 10.5 M edges, 8 x 16 fp32: by target 898 us, by source 1021 us (there an edge also gathers its
-// target's statistics and its own bias); 60 k targets, bf16, 4 x 64, a quarter of the edges masked: 340 and 464 us.
+// Latency and issue bound both, as forward.  200 k targets, 10.5 M edges, 8 x 16 fp32: by target 851 us, by source 1049 us (there an edge also gathers its
+// target's statistics and its own bias); 42 k targets of 60 k rows, bf16, 4 x 64, a quarter of the edges masked: 336 and 473 us.  Not all of it fits the
+// registers: by source full rows of 16 bits spill 72 bytes a thread (92 where a lane has a whole head), heads that do not fill their lanes 92 to 200, by target, too,
+// in every type (92 to 176).
 
 #include <algorithm>
 

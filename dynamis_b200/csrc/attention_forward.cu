@@ -6,8 +6,8 @@
 //
 // A warp takes a row and keeps its queries and sums in registers; what it reads an edge is a row of keys and one of values, gathered, mostly from L2
 // and L1.  What bounds it is latency and issue with 16 warps an SM (with neighbouring rows in all of them half the bytes come from L2, and it is no
-// faster).  200 k targets, 10.5 M edges, 8 x 16 fp32: 713 us (the bytes that have to be read once take 0.12 ms of memory's time); 150 k targets, bf16, 8 heads
-// on 2 of 32: 691 us.
+// faster).  200 k targets, 10.5 M edges, 8 x 16 fp32: 699 us (the bytes that have to be read once take 0.12 ms of memory's time); 150 k targets, bf16, 8 heads
+// on 2 of 32: 686 us.
 
 #include <algorithm>
 
@@ -16,7 +16,7 @@
 namespace dynb {
 
 constexpr int AF_WARPS = 4;
-// Edges of a slot in a batch: what 128 registers hold.  Rows of 16 bits are unpacked; heads of odd sizes need registers for their loads.
+// Edges of a slot in a batch: what 128 registers hold (4 bytes at most spill).  Rows of 16 bits are unpacked; heads of odd sizes need registers for their loads.
 template <typename T, bool FULL> constexpr int AF_BATCH = !FULL ? 2 : sizeof(T) == 4 ? 4 : 3;
 
 // WPR warps take turns at the batches of a row and join through shared memory.

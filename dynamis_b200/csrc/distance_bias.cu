@@ -138,8 +138,10 @@ db_forward_kernel(const DbArgs a)
 // a column of its own in the warp's copy of the table's gradient, [buckets][32]: no atomics, no two lanes in one bank, and the order of
 // its sums is that of the edges.  Sums of a column and of a block are in 32 bits: short ones (10.5 M edges, 64 x 8: a column of fifty terms, 88
 // columns a block) whose roundings are independent; db_table_join_kernel adds those of the blocks in 64.
-// What bounds it is shared memory: 16 reads and writes a round (10.5 M edges, 64 x 8: 0.29 ms, 1.4 TB/s; 16 warps 0.33).  The two gradients in
-// kernels of their own, without rounds: 0.30 and 1.10 ms.
+// What bounds it are the 16 reads and writes of shared memory a round, at 77 % of the pipe's peak, and the chain of read, sum and write of a column (10.5 M edges,
+// 64 x 8: 0.30 ms, 1.3 TB/s; 16 warps 0.33).  The two gradients in kernels of their own, without rounds: 0.30 and 1.10 ms.  The table's sums are made
+// also when nobody wants them (d_dist alone: 0.29 ms).  A warp's copy takes 128 bytes a bucket, so the warps go down with the buckets: 0.30 ms up to 64, 0.46 with
+// 128, 0.93 with 256, 2.2 with 512, 4.5 with 700.
 constexpr int DB_SCRATCH = 32 * 12;   // floats of a warp: weights, slopes, {place, pull} of 32 edges, 16 + 16 + 16 bytes each
 template <int WIDE>
 __global__ void __launch_bounds__(704, 1)
@@ -246,7 +248,8 @@ db_dist_kernel(const DbArgs a)
     }
 }
 
-// Gradient of the table for more heads or buckets than the kernel above has room for.  A warp's lanes are `slots` edges times `wide` heads; every slot has a copy of the table in shared memory that
+// Gradient of the table for more heads or buckets than the kernel above has room for (33 heads, 891 buckets).  10.5 M edges, 1024 x 8: 11.5 ms, with one warp
+// an SM; 2 M edges, 64 x 64: 1.0 ms.  A warp's lanes are `slots` edges times `wide` heads; every slot has a copy of the table in shared memory that
 // no other slot touches, so the sums need no atomics and their order is that of the edges.  Blocks take fixed stretches of the
 // edges and write their sums; db_table_join_kernel adds these in 64 bits.
 __global__ void

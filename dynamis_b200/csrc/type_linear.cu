@@ -11,7 +11,9 @@ namespace dynb {
 
 constexpr int TL_M = 64, TL_N = 64, TL_K = 16, TL_THREADS = 256;
 
-// One tile of 64 gathered rows times 64 columns, for matrices that do not fit into shared memory (type_linear_mma.cu).  `back`: dx = dy W^T instead of y = x W + b.
+// One tile of 64 gathered rows times 64 columns, for matrices that do not fit into shared memory (type_linear_mma.cu):
+// bound by its multiply-adds, 200 k rows of 400 x 400 in fp32 4.2 ms (a loop over the types with library products: 1.9), 512 x 128 1.5 ms (0.85).
+// `back`: dx = dy W^T instead of y = x W + b.
 template <typename T>
 __global__ void __launch_bounds__(TL_THREADS)
 tl_rows_kernel(const TlArgs a, int back)

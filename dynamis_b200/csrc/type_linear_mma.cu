@@ -8,8 +8,12 @@
 // dW = sum x_i^T dy_i: a block takes a stretch of rows of one type, 128 x up to 256 elements of the matrix; both operands are the gathered
 // rows as they are, read along their columns.  db is a product too, with a tile of ones.
 //
-// 1 M rows, 128 x 128 fp32, 5 types: y and dx 262 us each (3.9 TB/s), the weights' gradient 321 us; 400 k rows, 256 x 256 bf16,
-// 89 types: 140 us (3.0 TB/s).  Kernels of fused multiply-adds on 64 x 64 tiles took 6.6 ms for the three, and 3.3 ms.
+// 1 M rows, 128 x 128 fp32, 5 types: y 268 us, dx 271 (3.8 TB/s), the weights' gradient 384 us; bf16: 148, 150 and 325.  400 k rows, 256 x 256 bf16,
+// 89 types: 142 us (2.9 TB/s).  Kernels of fused multiply-adds on 64 x 64 tiles took 6.6 ms for the three in fp32, and 3.3 ms.
+//
+// The whole summed dimension of a matrix has to stand in shared memory beside two stages of rows.  So y sums at most 256 columns in fp32 and 1344 in 16 bits, dx
+// 1088 and 5376; wider ones go to tl_rows_kernel.  Columns that do not fit beside one another are tiles, each of which reads all rows (fp32, 129 to 256 summed
+// columns: tiles of 64).  200 k rows in fp32: 256 x 128 151 us, 257 x 128 778 us; the weights' gradient has no such limit.
 //
 // fp32 operands are split into three bf16 parts (8 bits each, together all 24): v = p0 + p1 + p2 (below
 // 2^-109 the last parts meet the smallest steps of bf16 and v is kept to within 2^-133).  Six of the nine products are formed,
