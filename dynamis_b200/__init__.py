@@ -1,7 +1,7 @@
 """dynamis_b200 — B200 (sm_100a) implementation of the Dynamis per-step data-parallel hot path.
 
 Radius graph, space-filling-curve partition, halo maps and halo exchange behind the reference's
-own Python-facing names, and the work of a message-passing layer between two exchanges.  The compute lives in ``libdynb.so`` (hand-written CUDA, C ABI in
+own Python-facing names, and the work of message-passing, attention and expert layers between two exchanges.  The compute lives in ``libdynb.so`` (hand-written CUDA, C ABI in
 ``include/dynb.h``); there is no CPU or PyTorch fallback.
 """
 
@@ -26,6 +26,7 @@ from .exchange import (  # noqa: F401
     push_buffer_create,
     supports_fabric_handles,
 )
+from .experts import Routing, expert_combine, expert_linear, route_experts  # noqa: F401
 from .halo import extract_halo_info, filter_edges_to_radius  # noqa: F401
 from .message import (  # noqa: F401
     NeighborIndex,
@@ -46,6 +47,7 @@ from .partition import (  # noqa: F401
     sfc_keys,
     sfc_partition_labels,
 )
+from .rotary import rotary_heads  # noqa: F401
 from .sim_state import DRIFT_BREACH, DRIFT_TRIP, SimState, scatter_rows  # noqa: F401
 from .state import (  # noqa: F401
     DistEnvironment,

@@ -98,6 +98,37 @@ class TypeLinear(ctypes.Structure):
     )
 
 
+class Rotary(ctypes.Structure):
+    """dynb_rotary"""
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("q_dev", "k_dev")]
+        + [(name, ctypes.c_int64) for name in ("q_row", "q_head", "k_row", "k_head")]
+        + [(name, ctypes.c_void_p) for name in ("pos_dev", "wave_dev", "q_weight_dev", "k_weight_dev")]
+        + [(name, ctypes.c_int64) for name in ("n_q", "n_k")]
+        + [(name, ctypes.c_int32) for name in ("heads", "kv_heads", "dim", "axes", "dtype", "pos_dtype", "interleaved", "norm")]
+        + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+    )
+
+
+class RoutingArgs(ctypes.Structure):
+    """dynb_routing"""
+    _fields_ = (
+        [("logits_dev", ctypes.c_void_p), ("logits_row", ctypes.c_int64), ("bias_dev", ctypes.c_void_p), ("n_rows", ctypes.c_int64)]
+        + [(name, ctypes.c_int32) for name in ("experts", "choices", "dtype", "score", "groups", "kept_groups", "renormalize")]
+        + [("scale", ctypes.c_float)]
+    )
+
+
+class ExpertLinear(ctypes.Structure):
+    """dynb_expert_linear_args"""
+    _fields_ = (
+        [(name, ctypes.c_void_p) for name in ("weight_dev", "order_dev", "start_dev")]
+        + [("n_rows", ctypes.c_int64)]
+        + [(name, ctypes.c_int32) for name in ("choices", "experts", "inner", "outer", "dtype", "paired", "activation", "reserved")]
+        + [("status_dev", ctypes.c_void_p)]
+    )
+
+
 # name -> (restype, argtypes); every symbol include/dynb.h declares must be listed here
 SIGNATURES = {
     "dynb_last_error": (ctypes.c_char_p, []),
@@ -176,6 +207,17 @@ SIGNATURES = {
     "dynb_type_linear": (_i32, [_p, _p, _i64, _p, _p, _p]),
     "dynb_type_linear_workspace_bytes": (_i32, [_p, ctypes.POINTER(_i64)]),
     "dynb_type_linear_backward": (_i32, [_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p]),
+    "dynb_rotary_heads": (_i32, [_p, _p, _p, _p]),
+    "dynb_rotary_heads_workspace_bytes": (_i32, [_p, ctypes.POINTER(_i64)]),
+    "dynb_rotary_heads_backward": (_i32, [_p, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dynb_route_experts_workspace_bytes": (_i32, [_p, ctypes.POINTER(_i64)]),
+    "dynb_route_experts": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dynb_route_experts_backward": (_i32, [_p, _p, _p, _p, _p, _p]),
+    "dynb_expert_linear": (_i32, [_p, _p, _i64, _p, _p, _p, _p]),
+    "dynb_expert_linear_workspace_bytes": (_i32, [_p, _i32, _i32, ctypes.POINTER(_i64)]),
+    "dynb_expert_linear_backward": (_i32, [_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
+    "dynb_expert_combine": (_i32, [_p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _p, _p]),
+    "dynb_expert_combine_backward": (_i32, [_p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _p, _p, _p]),
     "dynb_sfc_static_max_atoms": (_i64, []),
     "dynb_sfc_partition_static": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p]),
 }

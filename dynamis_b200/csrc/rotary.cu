@@ -1,0 +1,403 @@
+// Queries and keys of every row normalised per head and turned by the row's position (no counterpart in the reference, whose models leave
+// it to their libraries):  r = 1 / sqrt(mean x^2 + eps),  n = x r g,  the pair (a, b) number p of n becomes (a c - b s, a s + b c) with c, s = cos, sin
+// of 2 pi wave_p . pos_i.  Pairs are (p, p + dim / 2), or (2 p, 2 p + 1).
+//     back:  dn = the gradient turned back;  dg = sum dn x r;  dx = r (g dn - x r^2 mean(g dn x));  dpos_i = 2 pi sum over pairs of wave_p
+//     times the sum over the heads of q and k of (dn_b n_a - dn_a n_b).
+// A warp takes whole rows: a head's pairs lie over 1 to 32 lanes, so its sums are a few exchanges, and what a row's heads share (cosines, sines and the
+// gradient of the position) stays in the warp.  Turns are in 64 bits, whole ones are dropped, and what is left goes to 32 bits.
+
+#include <algorithm>
+
+#include "type_linear.cuh"
+
+namespace dynb {
+
+constexpr int RH_WARPS = 8, RH_MAX_HALF = 128, RH_MAX_AXES = 3;
+
+struct RhSide {
+    const void *x, *dy;          // [n, heads, dim]; the gradient of the result
+    void* out;                   // result, or gradient of x
+    const float* weight;
+    int64_t n, row, head, dy_row, dy_head;
+    int heads;
+};
+struct RhArgs {
+    RhSide side[2];              // queries, keys
+    const void* pos;
+    const float* wave;
+    void* d_pos;
+    float* partial;              // [blocks][2][dim]: sums for the weights
+    int64_t rows;
+    int half, axes, pos64, norm, per_head;   // per_head: lanes of a head
+    float eps;
+};
+
+template <typename T, int N> struct __align__(sizeof(T) * N) RhPack { T v[N]; };
+
+// VP pairs from pair p0 on of the head at `at`.
+template <typename T, int VP, bool MIXED>
+__device__ __forceinline__ void rh_load(const T* at, int p0, int half, float (&a)[VP], float (&b)[VP])
+{
+    if constexpr (MIXED) {
+        constexpr int N = VP == 1 ? 1 : 2 * VP * sizeof(T) > 16 ? VP : 2 * VP;   // one pair may stand on any element
+        RhPack<T, N> v[2 * VP / N];
+#pragma unroll
+        for (int i = 0; i < 2 * VP / N; i++) v[i] = *reinterpret_cast<const RhPack<T, N>*>(at + 2 * p0 + i * N);
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            a[i] = tl_get(&v[2 * i / N].v[2 * i % N]);
+            b[i] = tl_get(&v[(2 * i + 1) / N].v[(2 * i + 1) % N]);
+        }
+    } else {
+        const RhPack<T, VP> u = *reinterpret_cast<const RhPack<T, VP>*>(at + p0), w = *reinterpret_cast<const RhPack<T, VP>*>(at + half + p0);
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            a[i] = tl_get(&u.v[i]);
+            b[i] = tl_get(&w.v[i]);
+        }
+    }
+}
+template <typename T, int VP, bool MIXED>
+__device__ __forceinline__ void rh_store(T* at, int p0, int half, const float (&a)[VP], const float (&b)[VP])
+{
+    if constexpr (MIXED) {
+        constexpr int N = VP == 1 ? 1 : 2 * VP * sizeof(T) > 16 ? VP : 2 * VP;   // one pair may stand on any element
+        RhPack<T, N> v[2 * VP / N];
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            tl_put(&v[2 * i / N].v[2 * i % N], a[i]);
+            tl_put(&v[(2 * i + 1) / N].v[(2 * i + 1) % N], b[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * VP / N; i++) *reinterpret_cast<RhPack<T, N>*>(at + 2 * p0 + i * N) = v[i];
+    } else {
+        RhPack<T, VP> u, w;
+#pragma unroll
+        for (int i = 0; i < VP; i++) {
+            tl_put(&u.v[i], a[i]);
+            tl_put(&w.v[i], b[i]);
+        }
+        *reinterpret_cast<RhPack<T, VP>*>(at + p0) = u;
+        *reinterpret_cast<RhPack<T, VP>*>(at + half + p0) = w;
+    }
+}
+
+__device__ __forceinline__ float rh_sum(float v, int lanes)
+{
+    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Cosine and sine of pair p of row i.
+__device__ __forceinline__ float2 rh_turn(const RhArgs& a, int64_t i, int p)
+{
+    double turns = 0.0;
+    for (int x = 0; x < a.axes; x++) {
+        const double at = a.pos64 ? static_cast<const double*>(a.pos)[i * a.axes + x] : (double)static_cast<const float*>(a.pos)[i * a.axes + x];
+        turns = fma(at, (double)__ldg(a.wave + p * a.axes + x), turns);
+    }
+    const float rest = (float)(turns - rint(turns));
+    float2 cs;
+    sincospif(2.0f * rest, &cs.y, &cs.x);
+    return cs;
+}
+
+template <typename T, int VP, int PIECES, bool MIXED, bool BACK>
+__global__ void __launch_bounds__(RH_WARPS * 32)
+rh_kernel(const RhArgs a)
+{
+    __shared__ float2 turn_of[RH_WARPS][RH_MAX_HALF];
+    __shared__ float wave[RH_MAX_HALF * RH_MAX_AXES];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = a.half, dim = 2 * half;
+    if constexpr (BACK) {
+        for (int i = threadIdx.x; i < half * a.axes; i += RH_WARPS * 32) wave[i] = a.wave[i];
+        __syncthreads();
+    }
+    float2* const turns = turn_of[warp];
+    const int in_head = lane & (a.per_head - 1), group = lane / a.per_head, groups = 32 / a.per_head;
+    const int batch = half <= 32 ? 32 / half : 1;         // rows whose cosines a warp computes at a time
+    float ga[2][PIECES][VP], gb[2][PIECES][VP];           // the norms' weights, and sums for their gradients
+    float sa[2][PIECES][VP], sb[2][PIECES][VP];
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int c = 0; c < PIECES; c++)
+#pragma unroll
+            for (int i = 0; i < VP; i++) {
+                const int p = (c * a.per_head + in_head) * VP + i;
+                const float* const w = a.side[s].weight;
+                ga[s][c][i] = w != nullptr && p < half ? w[MIXED ? 2 * p : p] : 1.0f;
+                gb[s][c][i] = w != nullptr && p < half ? w[MIXED ? 2 * p + 1 : half + p] : 1.0f;
+                sa[s][c][i] = sb[s][c][i] = 0.0f;
+            }
+    const int units = a.side[0].heads + a.side[1].heads;
+    const int64_t warps = (int64_t)gridDim.x * RH_WARPS;
+    for (int64_t r0 = ((int64_t)blockIdx.x * RH_WARPS + warp) * batch; r0 < a.rows; r0 += warps * batch) {
+        const int here = (int)min((int64_t)batch, a.rows - r0);
+        __syncwarp();
+        for (int i = lane; i < here * half; i += 32) turns[i] = rh_turn(a, r0 + i / half, i % half);
+        __syncwarp();
+        for (int b = 0; b < here; b++) {
+            const int64_t row = r0 + b;
+            const int from = row < a.side[0].n ? 0 : a.side[0].heads;
+            float dtheta[PIECES][VP] = {};
+            for (int u0 = from; u0 < units; u0 += groups) {
+                const int u = u0 + group, s = u >= a.side[0].heads, h = s ? u - a.side[0].heads : u;
+                const RhSide& side = a.side[s];
+                const bool live = u < units && row < side.n;
+                const T* const x = static_cast<const T*>(side.x) + (live ? row * side.row + h * side.head : 0);
+                float xa[PIECES][VP], xb[PIECES][VP], ya[PIECES][VP], yb[PIECES][VP];
+                float squares = 0.0f, dot = 0.0f;
+#pragma unroll
+                for (int c = 0; c < PIECES; c++) {
+                    const int p = (c * a.per_head + in_head) * VP;
+                    const bool ok = live && p < half;
+#pragma unroll
+                    for (int i = 0; i < VP; i++) xa[c][i] = xb[c][i] = ya[c][i] = yb[c][i] = 0.0f;
+                    if (ok) rh_load<T, VP, MIXED>(x, p, half, xa[c], xb[c]);
+                    if constexpr (BACK) {
+                        if (ok) rh_load<T, VP, MIXED>(static_cast<const T*>(side.dy) + row * side.dy_row + h * side.dy_head, p, half, ya[c], yb[c]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VP; i++) {
+                        squares = fmaf(xa[c][i], xa[c][i], fmaf(xb[c][i], xb[c][i], squares));
+                        if constexpr (BACK) {
+                            const float2 cs = ok ? turns[b * half + p + i] : make_float2(1.0f, 0.0f);
+                            const float da = ya[c][i] * cs.x + yb[c][i] * cs.y, db = yb[c][i] * cs.x - ya[c][i] * cs.y;
+                            ya[c][i] = da;
+                            yb[c][i] = db;
+                            dot += (s ? ga[1][c][i] : ga[0][c][i]) * da * xa[c][i] + (s ? gb[1][c][i] : gb[0][c][i]) * db * xb[c][i];
+                        }
+                    }
+                }
+                float r = 1.0f, back = 0.0f;
+                if (a.norm) {
+                    r = 1.0f / sqrtf(rh_sum(squares, a.per_head) / (float)dim + a.eps);
+                    if constexpr (BACK) back = r * r * (rh_sum(dot, a.per_head) / (float)dim);
+                }
+                T* const out = static_cast<T*>(side.out);
+#pragma unroll
+                for (int c = 0; c < PIECES; c++) {
+                    const int p = (c * a.per_head + in_head) * VP;
+                    if (!live || p >= half) continue;
+                    float oa[VP], ob[VP];
+#pragma unroll
+                    for (int i = 0; i < VP; i++) {
+                        const float wa = s ? ga[1][c][i] : ga[0][c][i], wb = s ? gb[1][c][i] : gb[0][c][i];
+                        const float ua = xa[c][i] * r, ub = xb[c][i] * r;
+                        if constexpr (BACK) {
+                            dtheta[c][i] += yb[c][i] * (ua * wa) - ya[c][i] * (ub * wb);
+                            if (s) {
+                                sa[1][c][i] = fmaf(ya[c][i], ua, sa[1][c][i]);
+                                sb[1][c][i] = fmaf(yb[c][i], ub, sb[1][c][i]);
+                            } else {
+                                sa[0][c][i] = fmaf(ya[c][i], ua, sa[0][c][i]);
+                                sb[0][c][i] = fmaf(yb[c][i], ub, sb[0][c][i]);
+                            }
+                            oa[i] = r * (wa * ya[c][i] - xa[c][i] * back);
+                            ob[i] = r * (wb * yb[c][i] - xb[c][i] * back);
+                        } else {
+                            const float2 cs = turns[b * half + p + i];
+                            oa[i] = ua * wa * cs.x - ub * wb * cs.y;
+                            ob[i] = ua * wa * cs.y + ub * wb * cs.x;
+                        }
+                    }
+                    if (out != nullptr) rh_store<T, VP, MIXED>(out + (row * side.heads + h) * dim, p, half, oa, ob);
+                }
+            }
+            if constexpr (BACK) {
+                if (a.d_pos != nullptr) {
+                    for (int x = 0; x < a.axes; x++) {
+                        float d = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < PIECES; c++)
+#pragma unroll
+                            for (int i = 0; i < VP; i++) {
+                                const int p = (c * a.per_head + in_head) * VP + i;
+                                if (p < half) d = fmaf(dtheta[c][i], wave[p * a.axes + x], d);
+                            }
+                        d = 6.2831853071795865f * rh_sum(d, 32);
+                        if (lane == 0) {
+                            if (a.pos64) static_cast<double*>(a.d_pos)[row * a.axes + x] = d;
+                            else static_cast<float*>(a.d_pos)[row * a.axes + x] = d;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (BACK) {
+        if (a.partial == nullptr) return;
+        // the groups of a warp, then the warps of the block, in their order
+        __shared__ float sums[RH_WARPS][2][2 * RH_MAX_HALF];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int c = 0; c < PIECES; c++)
+#pragma unroll
+                for (int i = 0; i < VP; i++) {
+                    float va = sa[s][c][i], vb = sb[s][c][i];
+                    for (int o = a.per_head; o < 32; o <<= 1) {
+                        va += __shfl_xor_sync(0xffffffffu, va, o);
+                        vb += __shfl_xor_sync(0xffffffffu, vb, o);
+                    }
+                    const int p = (c * a.per_head + in_head) * VP + i;
+                    if (group == 0 && p < half) {
+                        sums[warp][s][MIXED ? 2 * p : p] = va;
+                        sums[warp][s][MIXED ? 2 * p + 1 : half + p] = vb;
+                    }
+                }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * dim; i += RH_WARPS * 32) {
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < RH_WARPS; w++) v += sums[w][i / dim][i % dim];
+            a.partial[(int64_t)blockIdx.x * 2 * dim + i] = v;
+        }
+    }
+}
+
+// The blocks' sums for the weights joined, in 64 bits: blockIdx.x is an element of [2][dim].
+__global__ void __launch_bounds__(128)
+rh_join_kernel(const float* partial, int blocks, int dim, float* d_q_weight, float* d_k_weight)
+{
+    __shared__ double sums[4];
+    const int at = blockIdx.x;
+    double v = 0.0;
+    for (int b = threadIdx.x; b < blocks; b += 128) v += (double)partial[(int64_t)b * 2 * dim + at];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = v;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    float* const to = at < dim ? d_q_weight : d_k_weight;
+    if (to != nullptr) to[at % dim] = (float)(sums[0] + sums[1] + sums[2] + sums[3]);
+}
+
+static int rh_blocks(int64_t rows, int half)
+{
+    const int batch = half <= 32 ? 32 / half : 1;
+    const int64_t need = (rows + (int64_t)batch * RH_WARPS - 1) / ((int64_t)batch * RH_WARPS);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)sm_count_cached() * 8));
+}
+
+static int rh_args(const dynb_rotary* in, RhArgs* a)
+{
+    if (in == nullptr) return fail_arg("null pointer");
+    if (in->dtype != DYNB_F32 && in->dtype != DYNB_F16 && in->dtype != DYNB_BF16) return fail_arg("rotary_heads: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
+    if (in->pos_dtype != DYNB_F32 && in->pos_dtype != DYNB_F64) return fail_arg("rotary_heads: pos_dtype must be DYNB_F32 or DYNB_F64");
+    if (in->n_q < 0 || in->n_k < 0 || in->n_q >= INT32_MAX || in->n_k >= INT32_MAX) return fail_arg("rotary_heads: rows must lie in [0, 2^31 - 1)");
+    if (in->heads < 1 || in->kv_heads < 1 || in->heads > 65535 || in->kv_heads > 65535) return fail_arg("rotary_heads: heads must lie in [1, 65535]");
+    if (in->dim < 2 || in->dim > DYNB_ROTARY_MAX_DIM || in->dim % 2 != 0) return fail_arg("rotary_heads: dim must be even and lie in [2, 256]");
+    if (in->axes < 1 || in->axes > DYNB_ROTARY_MAX_AXES) return fail_arg("rotary_heads: axes must lie in [1, 3]");
+    if (in->norm && !(in->eps >= 0.0f && in->eps <= 3.0e38f)) return fail_arg("rotary_heads: eps must be finite and not negative");
+    const int64_t rows = std::max(in->n_q, in->n_k);
+    if (rows > 0 && (!in->pos_dev || !in->wave_dev)) return fail_arg("null pointer");
+    if ((in->n_q > 0 && !in->q_dev) || (in->n_k > 0 && !in->k_dev)) return fail_arg("null pointer");
+    *a = RhArgs{};
+    a->side[0].x = in->q_dev; a->side[0].row = in->q_row; a->side[0].head = in->q_head; a->side[0].n = in->n_q; a->side[0].heads = in->heads;
+    a->side[1].x = in->k_dev; a->side[1].row = in->k_row; a->side[1].head = in->k_head; a->side[1].n = in->n_k; a->side[1].heads = in->kv_heads;
+    a->side[0].weight = in->norm ? in->q_weight_dev : nullptr;
+    a->side[1].weight = in->norm ? in->k_weight_dev : nullptr;
+    a->pos = in->pos_dev; a->wave = in->wave_dev;
+    a->rows = rows;
+    a->half = in->dim / 2; a->axes = in->axes; a->pos64 = in->pos_dtype == DYNB_F64; a->norm = in->norm != 0; a->eps = in->eps;
+    return DYNB_OK;
+}
+
+template <typename T, int VP, int PIECES, bool BACK>
+static void rh_start(RhArgs& a, bool mixed, int blocks, cudaStream_t s)
+{
+    const int lanes = (a.half + VP - 1) / VP;
+    a.per_head = 1;
+    while (a.per_head < lanes && a.per_head < 32) a.per_head *= 2;
+    if (mixed) rh_kernel<T, VP, PIECES, true, BACK><<<blocks, RH_WARPS * 32, 0, s>>>(a);
+    else rh_kernel<T, VP, PIECES, false, BACK><<<blocks, RH_WARPS * 32, 0, s>>>(a);
+}
+
+template <typename T, bool BACK>
+static cudaError_t rh_launch(RhArgs& a, bool mixed, int blocks, cudaStream_t s)
+{
+    // the widest pieces that all addresses allow: a piece is VP elements of one half of a head, or 2 VP of pairs side by side
+    constexpr int MOST = 16 / (int)sizeof(T);
+    int vp = MOST;
+    for (; vp > 1; vp /= 2) {
+        const int64_t bytes = std::min(16, (int)sizeof(T) * vp * (mixed ? 2 : 1));
+        bool ok = a.half % vp == 0;
+        for (const RhSide& d : a.side) {
+            if (d.n == 0) continue;
+            const uint64_t all = reinterpret_cast<uint64_t>(d.x) | reinterpret_cast<uint64_t>(d.dy) | reinterpret_cast<uint64_t>(d.out) |
+                                 (uint64_t)(sizeof(T) * d.row) | (uint64_t)(sizeof(T) * d.head) | (uint64_t)(sizeof(T) * d.dy_row) | (uint64_t)(sizeof(T) * d.dy_head);
+            ok = ok && all % bytes == 0;
+        }
+        if (ok) break;
+    }
+    if constexpr (MOST == 8) {
+        if (vp == 8) rh_start<T, 8, 1, BACK>(a, mixed, blocks, s);
+    }
+    if (vp == 4) rh_start<T, 4, 1, BACK>(a, mixed, blocks, s);
+    else if (vp == 2) rh_start<T, 2, 2, BACK>(a, mixed, blocks, s);
+    else if (vp == 1) rh_start<T, 1, 4, BACK>(a, mixed, blocks, s);
+    return cudaGetLastError();
+}
+
+template <bool BACK>
+static cudaError_t rh_run(RhArgs& a, int dtype, bool mixed, int blocks, cudaStream_t s)
+{
+    if (dtype == DYNB_F32) return rh_launch<float, BACK>(a, mixed, blocks, s);
+    if (dtype == DYNB_F16) return rh_launch<__half, BACK>(a, mixed, blocks, s);
+    return rh_launch<__nv_bfloat16, BACK>(a, mixed, blocks, s);
+}
+
+}  // namespace dynb
+
+using namespace dynb;
+
+extern "C" int dynb_rotary_heads(const dynb_rotary* args, void* q_out_dev, void* k_out_dev, void* stream)
+{
+    RhArgs a;
+    const int rc = rh_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (a.rows == 0) return DYNB_OK;
+    if ((args->n_q > 0 && !q_out_dev) || (args->n_k > 0 && !k_out_dev)) return fail_arg("null pointer");
+    a.side[0].out = q_out_dev;
+    a.side[1].out = k_out_dev;
+    DYNB_CUDA_OK(rh_run<false>(a, args->dtype, args->interleaved != 0, rh_blocks(a.rows, a.half), static_cast<cudaStream_t>(stream)));
+    return DYNB_OK;
+}
+
+extern "C" int dynb_rotary_heads_workspace_bytes(const dynb_rotary* args, int64_t* bytes)
+{
+    RhArgs a;
+    const int rc = rh_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (bytes == nullptr) return fail_arg("null pointer");
+    *bytes = (int64_t)rh_blocks(a.rows, a.half) * 4 * a.half * 4;
+    return DYNB_OK;
+}
+
+extern "C" int dynb_rotary_heads_backward(const dynb_rotary* args, const void* d_q_out_dev, int64_t d_q_row, int64_t d_q_head, const void* d_k_out_dev,
+                                          int64_t d_k_row, int64_t d_k_head, void* d_q_dev, void* d_k_dev, void* d_pos_dev, float* d_q_weight_dev,
+                                          float* d_k_weight_dev, void* workspace_dev, int64_t workspace_bytes, void* stream)
+{
+    RhArgs a;
+    const int rc = rh_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if ((args->n_q > 0 && !d_q_out_dev) || (args->n_k > 0 && !d_k_out_dev)) return fail_arg("null pointer");
+    const bool weights = d_q_weight_dev != nullptr || d_k_weight_dev != nullptr;
+    const int blocks = rh_blocks(a.rows, a.half);
+    if (weights && (workspace_dev == nullptr || !starts_on(workspace_dev, 4) || workspace_bytes < (int64_t)blocks * 4 * a.half * 4))
+        return fail_arg("workspace too small");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    a.side[0].dy = d_q_out_dev; a.side[0].dy_row = d_q_row; a.side[0].dy_head = d_q_head; a.side[0].out = d_q_dev;
+    a.side[1].dy = d_k_out_dev; a.side[1].dy_row = d_k_row; a.side[1].dy_head = d_k_head; a.side[1].out = d_k_dev;
+    a.d_pos = d_pos_dev;
+    a.partial = weights ? static_cast<float*>(workspace_dev) : nullptr;
+    if (a.rows == 0 && !weights) return DYNB_OK;
+    DYNB_CUDA_OK(rh_run<true>(a, args->dtype, args->interleaved != 0, blocks, s));
+    if (weights) {
+        rh_join_kernel<<<4 * a.half, 128, 0, s>>>(a.partial, blocks, 2 * a.half, d_q_weight_dev, d_k_weight_dev);
+        DYNB_CUDA_OK(cudaGetLastError());
+    }
+    return DYNB_OK;
+}

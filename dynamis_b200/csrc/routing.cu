@@ -1,0 +1,449 @@
+// Experts for rows (no counterpart in the reference, whose models leave it to their libraries).  From a row's logits l:
+//     s = softmax(l), or sigmoid(l);   key = s + bias;   a group's key is the sum of its two largest keys; the largest `kept` groups stay, and of their
+//     experts the `choices` largest keys are chosen, in falling order, the lowest number first among equal ones;   w = scale s, or scale s / (sum of the chosen s).
+// Logits or biases of -inf close an expert.  A place that no expert is left for gets number -1 and weight 0.
+// Keys are compared in 64 bits, and where nothing but the logits decides, by the logits themselves: which expert is chosen does not depend on how a
+// 32-bit exponential rounds.
+//
+// The (row, choice) pairs by expert, ascending inside one: every block counts its rows' choices, the counts are summed over the blocks, and every block
+// puts its pairs where its counts say.  No atomics on memory, no wait of the host: the same order each time, and the calls can be captured.
+
+#include <algorithm>
+
+#include "type_linear.cuh"
+
+namespace dynb {
+
+constexpr int RE_WARPS = 8;
+
+struct ReArgs {
+    const void* logits;
+    const float* bias;
+    int32_t *experts, *order, *start, *counts, *sums;   // counts [experts + 1][blocks], sums [experts + 1]
+    float* weights;
+    int64_t n, row;          // row: stride of the logits
+    int64_t chunk;           // rows of a block
+    int count, choices, groups, kept, sigmoid, renormalize;
+    float scale;
+};
+
+__device__ __forceinline__ uint64_t re_max(uint64_t v)   // of a warp
+{
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return (uint64_t)hi << 32 | lo;
+}
+// A key as a whole number in the same order: 0 for what is closed, NaN above all.
+__device__ __forceinline__ uint64_t re_order(double key)
+{
+    if (isnan(key)) return ~0ull;
+    return key == -INFINITY ? 0ull : ordered_u64(key);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(RE_WARPS * 32)
+re_choose_kernel(const ReArgs a)
+{
+    extern __shared__ unsigned char raw_smem[];
+    int32_t* const counts = reinterpret_cast<int32_t*>(raw_smem);                              // [experts + 1]
+    double* const scratch = reinterpret_cast<double*>(raw_smem + ((a.count + 1) * 4 + 15) / 16 * 16) + (threadIdx.x / 32) * (a.count + a.groups);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int i = threadIdx.x; i <= a.count; i += RE_WARPS * 32) counts[i] = 0;
+    __syncthreads();
+    const bool plain = a.bias == nullptr && a.groups == 1;   // the logits decide
+    const int per = a.count / a.groups;
+    const int64_t first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.n);
+    for (int64_t row = first + warp; row < last; row += RE_WARPS) {
+        const T* const l = static_cast<const T*>(a.logits) + row * a.row;
+        float logit[V];
+        uint64_t key[V];
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int e = lane + 32 * i;
+            logit[i] = e < a.count ? tl_get(l + e) : -INFINITY;
+            top = fmaxf(top, logit[i]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (plain) {
+#pragma unroll
+            for (int i = 0; i < V; i++) key[i] = re_order((double)logit[i]);
+        } else {
+            double s[V], sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                if (a.sigmoid) {
+                    s[i] = 1.0 / (1.0 + exp(-(double)logit[i]));
+                } else {
+                    s[i] = logit[i] == -INFINITY ? 0.0 : exp((double)logit[i] - (double)top);
+                    sum += s[i];
+                }
+            }
+            if (!a.sigmoid) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int e = lane + 32 * i;
+                const double v = (a.sigmoid ? s[i] : s[i] / sum) + (a.bias != nullptr && e < a.count ? (double)a.bias[e] : 0.0);
+                key[i] = logit[i] == -INFINITY ? 0ull : re_order(v);
+            }
+            if (a.groups > 1) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (lane + 32 * i < a.count) scratch[lane + 32 * i] = __longlong_as_double((long long)key[i]);
+                __syncwarp();
+                uint64_t* const of_group = reinterpret_cast<uint64_t*>(scratch + a.count);
+                for (int g = lane; g < a.groups; g += 32) {
+                    uint64_t one = 0, two = 0;
+                    for (int j = 0; j < per; j++) {
+                        const uint64_t k = (uint64_t)__double_as_longlong(scratch[g * per + j]);
+                        two = max(two, min(one, k));
+                        one = max(one, k);
+                    }
+                    uint64_t both = one;
+                    if (one == ~0ull || two == ~0ull) both = ~0ull;
+                    else if (two != 0) both = re_order(unordered_f64(one) + unordered_f64(two));
+                    if (one != 0 && both == 0) both = 1;   // open, however low
+                    of_group[g] = both;
+                }
+                __syncwarp();
+                // a group stays when fewer than `kept` come before it
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const int e = lane + 32 * i;
+                    if (e >= a.count) continue;
+                    const int g = e / per;
+                    const uint64_t mine = of_group[g];
+                    int before = 0;
+                    for (int h = 0; h < a.groups; h++) before += of_group[h] > mine || (of_group[h] == mine && h < g);
+                    if (before >= a.kept) key[i] = 0;
+                }
+            }
+        }
+        // the choices, one after the other; lane j keeps choice j
+        int32_t mine = -1;
+        float mine_logit = -INFINITY;
+        for (int j = 0; j < a.choices; j++) {
+            uint64_t best = key[0];
+#pragma unroll
+            for (int i = 1; i < V; i++) best = max(best, key[i]);
+            best = re_max(best);
+            if (best == 0) break;
+            uint32_t at = 0xffffffffu;
+            float with = 0.0f;
+#pragma unroll
+            for (int i = V - 1; i >= 0; i--)
+                if (key[i] == best) { at = lane + 32 * i; with = logit[i]; }
+            const uint32_t chosen = __reduce_min_sync(0xffffffffu, at);
+            with = __shfl_sync(0xffffffffu, with, chosen & 31);
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (chosen == lane + 32 * i) key[i] = 0;
+            if (lane == j) { mine = (int32_t)chosen; mine_logit = with; }
+        }
+        float w = 0.0f;
+        if (a.sigmoid && !a.renormalize) {
+            w = 1.0f / (1.0f + expf(-mine_logit));
+        } else {
+            // log s up to what all share; sums of exponentials below the largest
+            const float z = a.sigmoid ? fminf(mine_logit, 0.0f) - log1pf(expf(-fabsf(mine_logit))) : mine_logit;
+            const float zz = mine < 0 ? -INFINITY : isnan(mine_logit) ? mine_logit : z;
+            float most = zz;
+            if (a.renormalize) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            } else {
+                most = top;
+            }
+            w = mine < 0 ? 0.0f : expf(zz - most);
+            float sum = 0.0f;
+            if (a.renormalize) {
+                sum = w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) sum += logit[i] == -INFINITY ? 0.0f : expf(logit[i] - top);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (mine >= 0) w /= sum;
+            if (!a.sigmoid) {   // a NaN or +inf anywhere leaves no score of the row a number
+                bool odd = top == INFINITY;
+#pragma unroll
+                for (int i = 0; i < V; i++) odd = odd || isnan(logit[i]);
+                if (__any_sync(0xffffffffu, odd)) w = NAN;
+            }
+        }
+        if (lane < a.choices) {
+            a.experts[row * a.choices + lane] = mine;
+            a.weights[row * a.choices + lane] = mine < 0 ? 0.0f : a.scale * w;
+            atomicAdd(counts + (mine < 0 ? a.count : mine), 1);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= a.count; i += RE_WARPS * 32) a.counts[(int64_t)i * gridDim.x + blockIdx.x] = counts[i];
+}
+
+// Counts of an expert (blockIdx.x) over the blocks become the pairs of it before each block; their sum.
+__global__ void __launch_bounds__(256)
+re_sums_kernel(int32_t* counts, int32_t* sums, int blocks)
+{
+    __shared__ int warp_sums[8];
+    chain_begin();
+    int32_t* const mine = counts + (int64_t)blockIdx.x * blocks;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    int before = 0;
+    for (int b0 = 0; b0 < blocks; b0 += 256) {
+        const int b = b0 + threadIdx.x, v = b < blocks ? mine[b] : 0;
+        int total;
+        int at = warp_excl_scan(v, lane, &total);
+        if (lane == 0) warp_sums[warp] = total;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < 8; w++) {
+            if (w < warp) at += warp_sums[w];
+            all += warp_sums[w];
+        }
+        if (b < blocks) mine[b] = before + at;
+        before += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) sums[blockIdx.x] = before;
+}
+
+// Pairs of a block's rows to their places: a warp takes a run of them, 32 at a time.
+__global__ void __launch_bounds__(RE_WARPS * 32)
+re_place_kernel(const ReArgs a)
+{
+    extern __shared__ unsigned char raw_smem[];
+    int32_t* const start = reinterpret_cast<int32_t*>(raw_smem);          // [experts + 1]; then [warps][experts + 1]
+    int32_t* const next = start + a.count + 1;
+    __shared__ int warp_sums[RE_WARPS];
+    chain_begin();
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, all = a.count + 1;
+    for (int i = threadIdx.x; i < RE_WARPS * all; i += RE_WARPS * 32) next[i] = 0;
+    int before = 0;
+    for (int e0 = 0; e0 < all; e0 += RE_WARPS * 32) {
+        const int e = e0 + threadIdx.x, v = e < all ? a.sums[e] : 0;
+        int total;
+        int at = warp_excl_scan(v, lane, &total);
+        if (lane == 0) warp_sums[warp] = total;
+        __syncthreads();
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < RE_WARPS; w++) {
+            if (w < warp) at += warp_sums[w];
+            sum += warp_sums[w];
+        }
+        if (e < all) {
+            start[e] = before + at;
+            if (blockIdx.x == 0) a.start[e] = before + at;
+        }
+        before += sum;
+        __syncthreads();
+    }
+    const int64_t first = blockIdx.x * a.chunk * a.choices, last = min(blockIdx.x * a.chunk + a.chunk, a.n) * a.choices;
+    const int64_t run = ((last - first + RE_WARPS - 1) / RE_WARPS + 31) / 32 * 32, from = min(first + warp * run, last), to = min(from + run, last);
+    for (int64_t p = from + lane; p < to; p += 32) {
+        const int e = a.experts[p];
+        atomicAdd(next + warp * all + (e < 0 ? a.count : e), 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < all; e += RE_WARPS * 32) {
+        int at = start[e] + a.counts[(int64_t)e * gridDim.x + blockIdx.x];
+        for (int w = 0; w < RE_WARPS; w++) {
+            const int v = next[w * all + e];
+            next[w * all + e] = at;
+            at += v;
+        }
+    }
+    __syncthreads();
+    for (int64_t p0 = from; p0 < to; p0 += 32) {
+        const int64_t p = p0 + lane;
+        const bool live = p < to;
+        const int e = live ? a.experts[p] : -2, slot = e < 0 ? a.count : e;
+        const uint32_t same = __match_any_sync(0xffffffffu, live ? slot : -2);
+        const int at = live ? next[warp * all + slot] : 0, rank = __popc(same & lanemask_lt());
+        __syncwarp();
+        if (live) {
+            a.order[at + rank] = (int32_t)p;
+            if (rank == 0) next[warp * all + slot] = at + __popc(same);
+        }
+        __syncwarp();
+    }
+}
+
+// The gradient of the logits.  p: the weights without the scale, g: their gradient times the scale.
+//     renormalised: d = p (g - sum p g), for sigmoids times 1 - s;   sigmoid: g s (1 - s);   softmax: s_e (g_e - sum s g) for every expert e.
+template <typename T, int V>
+__global__ void __launch_bounds__(RE_WARPS * 32)
+re_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits)
+{
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    for (int64_t row = (int64_t)blockIdx.x * RE_WARPS + warp; row < a.n; row += (int64_t)gridDim.x * RE_WARPS) {
+        const T* const l = static_cast<const T*>(a.logits) + row * a.row;
+        int32_t e = -1;
+        float w = 0.0f, g = 0.0f;
+        if (lane < a.choices) {
+            e = a.experts[row * a.choices + lane];
+            if ((uint32_t)e >= (uint32_t)a.count) e = -1;
+            w = a.weights[row * a.choices + lane] / a.scale;
+            g = d_weights[row * a.choices + lane] * a.scale;
+        }
+        const bool live = e >= 0;
+        const float s = live && a.sigmoid ? 1.0f / (1.0f + expf(-tl_get(l + e))) : 0.0f;
+        float dot = live ? w * g : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        float d = 0.0f;
+        if (live) {
+            if (a.renormalize) d = w * (g - dot) * (a.sigmoid ? 1.0f - s : 1.0f);
+            else d = a.sigmoid ? g * s * (1.0f - s) : g;
+        }
+        float out[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) out[i] = 0.0f;
+        for (int j = 0; j < a.choices; j++) {
+            const int at = __shfl_sync(0xffffffffu, e, j);
+            const float v = __shfl_sync(0xffffffffu, d, j);
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (at == lane + 32 * i) out[i] = v;
+        }
+        if (!a.sigmoid && !a.renormalize) {
+            float logit[V], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                logit[i] = lane + 32 * i < a.count ? tl_get(l + lane + 32 * i) : -INFINITY;
+                top = fmaxf(top, logit[i]);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                logit[i] = logit[i] == -INFINITY ? 0.0f : expf(logit[i] - top);
+                sum += logit[i];
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+#pragma unroll
+            for (int i = 0; i < V; i++) out[i] = sum == 0.0f ? 0.0f : logit[i] / sum * (out[i] - dot);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (lane + 32 * i < a.count) tl_put(d_logits + row * a.count + lane + 32 * i, out[i]);
+    }
+}
+
+struct ReLayout { int64_t chunk, blocks, counts, sums, total; };
+static ReLayout re_layout(int64_t n, int count)
+{
+    ReLayout l;
+    const int64_t most = (int64_t)sm_count_cached() * 4;
+    l.chunk = std::max<int64_t>(RE_WARPS, (n + most - 1) / most);
+    l.blocks = std::max<int64_t>(1, (n + l.chunk - 1) / l.chunk);
+    l.counts = 0;
+    l.sums = align_up(4 * l.blocks * (count + 1), 256);
+    l.total = l.sums + align_up(4 * (count + 1), 256);
+    return l;
+}
+
+static int re_args(const dynb_routing* in, ReArgs* a)
+{
+    if (in == nullptr) return fail_arg("null pointer");
+    if (in->dtype != DYNB_F32 && in->dtype != DYNB_F16 && in->dtype != DYNB_BF16) return fail_arg("route_experts: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
+    if (in->experts < 1 || in->experts > DYNB_ROUTING_MAX_EXPERTS) return fail_arg("route_experts: experts must lie in [1, 1024]");
+    if (in->choices < 1 || in->choices > DYNB_ROUTING_MAX_CHOICES || in->choices > in->experts)
+        return fail_arg("route_experts: choices must lie in [1, 32] and be no more than the experts");
+    if (in->n_rows < 0 || in->n_rows * in->choices >= INT32_MAX) return fail_arg("route_experts: rows times choices must lie in [0, 2^31 - 1)");
+    if (in->groups < 1 || in->experts % in->groups != 0 || in->kept_groups < 1 || in->kept_groups > in->groups)
+        return fail_arg("route_experts: groups must divide the experts, and kept_groups lie in [1, groups]");
+    if (in->score != DYNB_SCORE_SOFTMAX && in->score != DYNB_SCORE_SIGMOID) return fail_arg("route_experts: score must be DYNB_SCORE_SOFTMAX or DYNB_SCORE_SIGMOID");
+    if (!(in->scale > 0.0f && in->scale <= 3.0e38f)) return fail_arg("route_experts: scale must be positive and finite");
+    *a = ReArgs{};
+    a->logits = in->logits_dev; a->row = in->logits_row; a->bias = in->bias_dev; a->n = in->n_rows;
+    a->count = in->experts; a->choices = in->choices; a->groups = in->groups; a->kept = in->kept_groups;
+    a->sigmoid = in->score == DYNB_SCORE_SIGMOID; a->renormalize = in->renormalize != 0; a->scale = in->scale;
+    return DYNB_OK;
+}
+
+template <typename T>
+static cudaError_t re_choose(const ReArgs& a, unsigned blocks, cudaStream_t s)
+{
+    const int smem = ((a.count + 1) * 4 + 15) / 16 * 16 + (a.groups > 1 ? RE_WARPS * (a.count + a.groups) * 8 : 0);
+    void (*kernel)(ReArgs) = a.count <= 32 ? re_choose_kernel<T, 1> : a.count <= 64 ? re_choose_kernel<T, 2> : a.count <= 128 ? re_choose_kernel<T, 4> :
+                             a.count <= 256 ? re_choose_kernel<T, 8> : a.count <= 512 ? re_choose_kernel<T, 16> : re_choose_kernel<T, 32>;
+    const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+    if (rc != cudaSuccess) return rc;
+    kernel<<<blocks, RE_WARPS * 32, smem, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t re_backward(const ReArgs& a, const float* d_weights, void* d_logits, cudaStream_t s)
+{
+    void (*kernel)(ReArgs, const float*, T*) = a.count <= 32 ? re_backward_kernel<T, 1> : a.count <= 64 ? re_backward_kernel<T, 2> : a.count <= 128 ? re_backward_kernel<T, 4> :
+                                               a.count <= 256 ? re_backward_kernel<T, 8> : a.count <= 512 ? re_backward_kernel<T, 16> : re_backward_kernel<T, 32>;
+    const unsigned blocks = (unsigned)std::min<int64_t>((a.n + RE_WARPS - 1) / RE_WARPS, (int64_t)sm_count_cached() * 8);
+    kernel<<<blocks, RE_WARPS * 32, 0, s>>>(a, d_weights, static_cast<T*>(d_logits));
+    return cudaGetLastError();
+}
+
+}  // namespace dynb
+
+using namespace dynb;
+
+extern "C" int dynb_route_experts_workspace_bytes(const dynb_routing* args, int64_t* bytes)
+{
+    ReArgs a;
+    const int rc = re_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (bytes == nullptr) return fail_arg("null pointer");
+    *bytes = re_layout(a.n, a.count).total;
+    return DYNB_OK;
+}
+
+extern "C" int dynb_route_experts(const dynb_routing* args, int32_t* experts_dev, float* weights_dev, int32_t* order_dev, int32_t* start_dev,
+                                  void* workspace_dev, int64_t workspace_bytes, void* stream)
+{
+    ReArgs a;
+    const int rc = re_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (!start_dev || !workspace_dev || (a.n > 0 && (!a.logits || !experts_dev || !weights_dev || !order_dev))) return fail_arg("null pointer");
+    if (!starts_on(workspace_dev, 4)) return fail_arg("route_experts: the workspace must start on a 4-byte boundary");
+    const ReLayout l = re_layout(a.n, a.count);
+    if (workspace_bytes < l.total) return fail_arg("workspace too small");
+    unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
+    a.experts = experts_dev; a.weights = weights_dev; a.order = order_dev; a.start = start_dev; a.chunk = l.chunk;
+    a.counts = reinterpret_cast<int32_t*>(ws + l.counts);
+    a.sums = reinterpret_cast<int32_t*>(ws + l.sums);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const unsigned blocks = (unsigned)l.blocks;
+    if (args->dtype == DYNB_F32) DYNB_CUDA_OK(re_choose<float>(a, blocks, s));
+    else if (args->dtype == DYNB_F16) DYNB_CUDA_OK(re_choose<__half>(a, blocks, s));
+    else DYNB_CUDA_OK(re_choose<__nv_bfloat16>(a, blocks, s));
+    DYNB_CUDA_OK(launch_chained(re_sums_kernel, a.count + 1, 256, 0, s, a.counts, a.sums, (int)blocks));
+    DYNB_CUDA_OK(launch_chained(re_place_kernel, blocks, RE_WARPS * 32, (size_t)(a.count + 1) * 4 * (RE_WARPS + 1), s, a));
+    return DYNB_OK;
+}
+
+extern "C" int dynb_route_experts_backward(const dynb_routing* args, const int32_t* experts_dev, const float* weights_dev, const float* d_weights_dev,
+                                           void* d_logits_dev, void* stream)
+{
+    ReArgs a;
+    const int rc = re_args(args, &a);
+    if (rc != DYNB_OK) return rc;
+    if (a.n == 0) return DYNB_OK;
+    if (!a.logits || !experts_dev || !weights_dev || !d_weights_dev || !d_logits_dev) return fail_arg("null pointer");
+    a.experts = const_cast<int32_t*>(experts_dev);
+    a.weights = const_cast<float*>(weights_dev);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (args->dtype == DYNB_F32) DYNB_CUDA_OK(re_backward<float>(a, d_weights_dev, d_logits_dev, s));
+    else if (args->dtype == DYNB_F16) DYNB_CUDA_OK(re_backward<__half>(a, d_weights_dev, d_logits_dev, s));
+    else DYNB_CUDA_OK(re_backward<__nv_bfloat16>(a, d_weights_dev, d_logits_dev, s));
+    return DYNB_OK;
+}

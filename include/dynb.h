@@ -513,6 +513,84 @@ int dynb_type_linear_workspace_bytes(const dynb_type_linear_args* args, int64_t*
 int dynb_type_linear_backward(const dynb_type_linear_args* args, const void* x_dev, int64_t x_row, const void* d_y_dev, int64_t d_y_row,
                               void* d_x_dev, void* d_weight_dev, void* d_bias_dev, void* workspace_dev, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ attention and expert layers
+ * Beside neighbor_attention and type_linear: queries and keys normalised and turned by positions, and rows that choose their matrices themselves.  No
+ * counterpart in the reference (its model adapters leave it to their libraries, dynamis_model/src/dynamis_model/nnp/uma.py).
+ *
+ * Queries [n_q, heads, dim] and keys [n_k, kv_heads, dim], row i of both at pos[i] (axes coordinates; as many rows as the longer of the two): with `norm`
+ * every head x becomes x / sqrt(mean x^2 + eps) times its weight (NULL: ones), then pair p of it, elements (p, p + dim / 2) or (2 p, 2 p + 1)
+ * (`interleaved`), turns by the angle 2 pi wave[p] . pos[i], wave [dim / 2, axes].  Strides are in elements, a head's elements are consecutive; results
+ * are contiguous. */
+#define DYNB_ROTARY_MAX_DIM 256
+#define DYNB_ROTARY_MAX_AXES 3
+typedef struct dynb_rotary {
+    const void *q_dev, *k_dev;              /* of `dtype`: DYNB_F32, DYNB_F16, DYNB_BF16 */
+    int64_t q_row, q_head, k_row, k_head;
+    const void* pos_dev;                    /* [max(n_q, n_k), axes] of `pos_dtype`: DYNB_F32, DYNB_F64 */
+    const float *wave_dev, *q_weight_dev, *k_weight_dev;
+    int64_t n_q, n_k;
+    int32_t heads, kv_heads, dim, axes, dtype, pos_dtype, interleaved, norm;
+    float eps;
+    int32_t reserved;
+} dynb_rotary;
+int dynb_rotary_heads(const dynb_rotary* args, void* q_out_dev, void* k_out_dev, void* stream);
+/* Gradients, each NULL when it is not wanted; contiguous.  The workspace is for the weights' gradients.  Computed in 32 bits; d_pos has the type of pos. */
+int dynb_rotary_heads_workspace_bytes(const dynb_rotary* args, int64_t* bytes);
+int dynb_rotary_heads_backward(const dynb_rotary* args, const void* d_q_out_dev, int64_t d_q_row, int64_t d_q_head, const void* d_k_out_dev, int64_t d_k_row,
+                               int64_t d_k_head, void* d_q_dev, void* d_k_dev, void* d_pos_dev, float* d_q_weight_dev, float* d_k_weight_dev,
+                               void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* Experts of rows from logits [n_rows, experts]: scores s = softmax or sigmoid, keys s + bias, groups of experts / groups neighbours of which the kept_groups with
+ * the largest sums of two keys stay, of these the `choices` largest keys in falling order (the lowest number first among equal ones); weights scale s, or
+ * scale s / (sum of the chosen s).  -inf as a logit or a bias closes an expert; a place without an expert has number -1 and weight 0.
+ *   experts[n_rows, choices], weights[n_rows, choices]
+ *   order[n_rows choices], start[experts + 1]   pairs (row choices + choice) of expert 0, of expert 1, ..., ascending inside one; those without an expert behind
+ * No host wait.  The workspace starts on a 4-byte boundary. */
+#define DYNB_ROUTING_MAX_EXPERTS 1024
+#define DYNB_ROUTING_MAX_CHOICES 32
+#define DYNB_SCORE_SOFTMAX 0
+#define DYNB_SCORE_SIGMOID 1
+typedef struct dynb_routing {
+    const void* logits_dev;                 /* of `dtype` */
+    int64_t logits_row;
+    const float* bias_dev;                  /* [experts] or NULL */
+    int64_t n_rows;
+    int32_t experts, choices, dtype, score, groups, kept_groups, renormalize;
+    float scale;
+} dynb_routing;
+int dynb_route_experts_workspace_bytes(const dynb_routing* args, int64_t* bytes);
+int dynb_route_experts(const dynb_routing* args, int32_t* experts_dev, float* weights_dev, int32_t* order_dev, int32_t* start_dev, void* workspace_dev,
+                       int64_t workspace_bytes, void* stream);
+/* experts and weights as the call above gave them; d_logits [n_rows, experts], contiguous. */
+int dynb_route_experts_backward(const dynb_routing* args, const int32_t* experts_dev, const float* weights_dev, const float* d_weights_dev, void* d_logits_dev,
+                                void* stream);
+
+/* Products with the matrices of a row's experts: z[i, j] = act(x[i] weight[e_ij] (+ bias[e_ij])), or x[i, j] where x is `paired`; weight
+ * [experts, inner, outer], contiguous, as bias, z and the gradients are.  x and d_z have strides in elements from row to row (from pair to pair).  Places
+ * without an expert give zeros.  slope_dev (NULL when there is no backward pass, or no activation): what the backward pass needs of the activation,
+ * [n_rows choices, outer] of 4 bytes for DYNB_F32 and 2 otherwise. */
+#define DYNB_ACTIVATION_NONE 0
+#define DYNB_ACTIVATION_SILU 1
+#define DYNB_ACTIVATION_GELU 2
+typedef struct dynb_expert_linear_args {
+    const void* weight_dev;
+    const int32_t *order_dev, *start_dev;
+    int64_t n_rows;
+    int32_t choices, experts, inner, outer, dtype, paired, activation, reserved;
+    uint32_t* status_dev;                   /* as in dynb_type_linear_args */
+} dynb_expert_linear_args;
+int dynb_expert_linear(const dynb_expert_linear_args* args, const void* x_dev, int64_t x_row, const void* bias_dev, void* z_dev, void* slope_dev, void* stream);
+int dynb_expert_linear_workspace_bytes(const dynb_expert_linear_args* args, int want_x, int want_weights, int64_t* bytes);
+int dynb_expert_linear_backward(const dynb_expert_linear_args* args, const void* x_dev, int64_t x_row, const void* d_z_dev, int64_t d_z_row, const void* slope_dev,
+                                const int32_t* experts_dev, void* d_x_dev, void* d_weight_dev, void* d_bias_dev, void* workspace_dev, int64_t workspace_bytes,
+                                void* stream);
+/* y[i] = residual[i] + sum_j weights[i, j] z[i, j] over the places with an expert; z [n_rows, choices, width], contiguous, as y and the gradients are.
+ * The residual's gradient is d_y. */
+int dynb_expert_combine(const void* z_dev, const float* weights_dev, const int32_t* experts_dev, const void* residual_dev, int64_t residual_row, int64_t n_rows,
+                        int choices, int width, int dtype, void* y_dev, void* stream);
+int dynb_expert_combine_backward(const void* z_dev, const float* weights_dev, const int32_t* experts_dev, const void* d_y_dev, int64_t d_y_row, int64_t n_rows,
+                                 int choices, int width, int dtype, void* d_z_dev, float* d_weights_dev, void* stream);
+
 /* ------------------------------------------------------------------ partition without a workspace
  * No counterpart in the reference.  Same result as dynb_sfc_partition, for callers that must not
  * allocate device memory while they run (an engine that gave its whole memory budget to its own
