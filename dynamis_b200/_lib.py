@@ -213,8 +213,8 @@ SIGNATURES = {
     "dynb_route_experts_workspace_bytes": (_i32, [_p, ctypes.POINTER(_i64)]),
     "dynb_route_experts": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p]),
     "dynb_route_experts_backward": (_i32, [_p, _p, _p, _p, _p, _p]),
-    "dynb_expert_linear": (_i32, [_p, _p, _i64, _p, _p, _p, _p]),
-    "dynb_expert_linear_workspace_bytes": (_i32, [_p, _i32, _i32, ctypes.POINTER(_i64)]),
+    "dynb_expert_linear": (_i32, [_p, _p, _i64, _p, _p, _p, _p, _i64, _p]),
+    "dynb_expert_linear_workspace_bytes": (_i32, [_p, _i32, _i32, _i32, ctypes.POINTER(_i64)]),
     "dynb_expert_linear_backward": (_i32, [_p, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _p]),
     "dynb_expert_combine": (_i32, [_p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _p, _p]),
     "dynb_expert_combine_backward": (_i32, [_p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _p, _p, _p]),

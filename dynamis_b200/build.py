@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libdynb.so")
 SOURCES = ["lib.cu", "radius_graph.cu", "sfc.cu", "halo.cu", "exchange.cu", "state_ops.cu", "integrators.cu", "kdtree.cu",
            "neighbors.cu", "attention.cu", "attention_forward.cu", "attention_backward.cu", "distance_bias.cu", "type_linear.cu",
-           "type_linear_mma.cu", "rotary.cu", "routing.cu", "experts.cu"]
+           "type_linear_mma.cu", "rotary.cu", "routing.cu", "experts.cu",
+           "experts_mma.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,0 +1,855 @@
+// The products by expert on the tensor cores.
+//
+// z = act(x W + b) and dx = du W^T, du = dz act'(u): tiles of 128 pairs of one expert by up to 256 columns (fp32: 128).  Eight warps gather the rows of x (or of dz, times
+// the slope) into stages of 64 summed columns, one warp brings the matrix, one issues the products, eight take the sums out of tensor memory, which holds two tiles, and
+// apply offset and activation.  The matrices are laid out once per call as the multipliers read them (ex_pack_kernel: both products read them along the summed
+// index, fp32 in its three parts), so that a piece of 64 summed columns is one copy of a run of bytes.  A matrix that fits beside three stages of rows stays for
+// all tiles of its expert; a larger one comes anew with every stage, from L2.
+//
+// dW = sum x^T du: a block takes a stretch of an expert's pairs, 128 x up to 256 elements of the matrix; both operands are the gathered rows as they
+// are, read along their columns.  db is a product too, with a tile of ones.
+//
+// fp32 operands are three bf16 parts, six of nine products (mma_parts.cuh).
+
+#include "experts.cuh"
+#include "mma_parts.cuh"
+
+namespace dynb {
+
+constexpr int EM_FEED = 8, EM_OUT = 8;                               // warps that gather, and that store results
+constexpr int EM_THREADS = (EM_OUT + 2 + EM_FEED) * 32;
+constexpr int EM_MAX_STAGES = 8;
+constexpr int EM_SMEM = 204 * 1024;                                  // beside 20 KB of results under way and offsets
+constexpr int EM_DEPTH = 3;                                          // stages whose copies a gathering warp leaves under way
+
+enum EmPath { EM_ASYNC, EM_REGISTERS, EM_SLOPE };
+
+struct EmPlan {
+    int back, columns, column_stride, chunks, stages, depth, tensor_columns, resident, b_bytes, stage_bytes, store, slope_store;   // b_bytes: matrix of one stage
+    const unsigned char* packed;
+};
+
+struct EmBars { uint64_t full[EM_MAX_STAGES], empty[EM_MAX_STAGES], b_full[EM_MAX_STAGES], panel_full, panel_free, sums_full[2], sums_free[2]; uint32_t tensor; };
+
+__device__ __forceinline__ void bulk_expect(uint64_t* bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_copy(void* to, const void* from, uint32_t bytes, uint64_t* bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(to)), "l"(from), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+// 16 bytes, zeros where `live` is false (nothing is read then).
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool live)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last `left` groups of this thread have arrived.
+__device__ __forceinline__ void copies_wait(int left)
+{
+    if (left >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Matrices in the order of the multipliers: [expert][tile of columns][64 summed columns][part][column][128 bytes, 16-byte pieces swizzled], zeros beyond the matrix.
+template <typename T>
+__global__ void __launch_bounds__(256)
+ex_pack_kernel(const T* w, int64_t experts, int inner, int outer, int back, int columns, int tiles, int chunks, unsigned char* packed)
+{
+    constexpr int PARTS = TmParts<T>::N;
+    const int64_t all = experts * tiles * chunks * columns * 8;
+    const int kk = back ? outer : inner, nn = back ? inner : outer;
+    for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < all; u += (int64_t)gridDim.x * blockDim.x) {
+        // what lies side by side in memory goes to neighbouring threads: columns forward, pieces of the summed index backward
+        int64_t rest = u;
+        const int inside = (int)(rest % (columns * 8));
+        rest /= columns * 8;
+        const int n = back ? inside / 8 : inside % columns, piece = back ? inside % 8 : inside / columns;
+        const int chunk = (int)(rest % chunks);
+        rest /= chunks;
+        const int tile = (int)(rest % tiles);
+        const int64_t e = rest / tiles;
+        const int k = chunk * 64 + piece * 8, col = tile * columns + n;
+        const int have = col < nn ? min(8, kk - k) : 0;
+        const T* const from = w + e * inner * outer + (back ? (int64_t)col * outer + k : (int64_t)k * outer + col);
+        const TmRaw<T> v = tm_load<false>(have > 0 ? from : w, back ? 1 : outer, have);
+        const TmRaw<T> one[1] = {v};
+        unsigned char* const to = packed + ((e * tiles + tile) * chunks + chunk) * ((int64_t)PARTS * columns * 128) + tile_piece(n, piece);
+        if (tm_odd(one)) tm_store<true>(v, to, columns * 128);
+        else tm_store<false>(v, to, columns * 128);
+    }
+}
+
+// Eight elements times their slopes.
+template <typename T>
+__device__ __forceinline__ void em_times(TmRaw<T>& v, const TmRaw<T>& slope)
+{
+    if constexpr (sizeof(T) == 4) {
+        uint32_t* const a = reinterpret_cast<uint32_t*>(&v);
+        const uint32_t* const s = reinterpret_cast<const uint32_t*>(&slope);
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] = __float_as_uint(__uint_as_float(a[i]) * __uint_as_float(s[i]));
+    } else {
+        uint32_t* const a = reinterpret_cast<uint32_t*>(&v);
+        const uint32_t* const s = reinterpret_cast<const uint32_t*>(&slope);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float lo = ex_slope_of(s[i] & 0xffffu), hi = ex_slope_of(s[i] >> 16);
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(a + i));
+                const __half2 h = __floats2half2_rn(f.x * lo, f.y * hi);
+                a[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a[i] << 16) * lo, __uint_as_float(a[i] & 0xffff0000u) * hi);
+                a[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+    }
+}
+
+// 64 bytes of each of a warp's 32 rows, lane l's from row l, to memory by pieces of 16 bytes (or elements of `size`) that lie side by side.  `mine`: 2 KB of
+// the warp, its pieces swizzled.  `row`: number of the lane's row, or -1; `bytes`: how many of the 64 there are.
+__device__ __forceinline__ void em_put(unsigned char* mine, const uint32_t* words, int lane, int32_t row, unsigned char* out, int64_t row_bytes, int bytes, int store, int size)
+{
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        *reinterpret_cast<uint4*>(mine + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
+    __syncwarp();
+    const int at = (lane & 3) * 16;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int r = 8 * j + (lane >> 2);
+        const int32_t to = __shfl_sync(0xffffffffu, row, r);
+        const uint4 piece = *reinterpret_cast<const uint4*>(mine + r * 64 + (((lane & 3) ^ (r >> 1)) & 3) * 16);
+        if (to < 0 || at >= bytes) continue;
+        unsigned char* const p = out + to * row_bytes + at;
+        if (store == 16) {
+            *reinterpret_cast<uint4*>(p) = piece;
+        } else if (size == 4) {
+            const uint32_t* const e = reinterpret_cast<const uint32_t*>(&piece);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (at + 4 * i < bytes) reinterpret_cast<uint32_t*>(p)[i] = e[i];
+        } else {
+            const uint16_t* const e = reinterpret_cast<const uint16_t*>(&piece);
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (at + 2 * i < bytes) reinterpret_cast<uint16_t*>(p)[i] = e[i];
+        }
+    }
+}
+
+// O: type of the results (fp32 for gradients that are summed over the choices before they are rounded).
+template <typename T, typename O, EmPath PATH, bool WIDE>
+__global__ void __launch_bounds__(EM_THREADS, 1)
+em_rows_kernel(const ExArgs e, const EmPlan plan)
+{
+    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O);
+    const TlArgs& a = e.t;
+    extern __shared__ unsigned char raw_smem[];
+    __shared__ EmBars bars;
+    __shared__ __align__(16) float offsets[EM_OUT][128];
+    __shared__ __align__(16) unsigned char turned[EM_OUT][2048];
+    unsigned char* const panel = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+    unsigned char* const stage0 = panel + (plan.resident ? plan.chunks * plan.b_bytes : 0);
+    const int warp = warp_number(), lane = threadIdx.x & 31;
+    const int kk = plan.back ? a.outer : a.inner, nn = plan.back ? a.inner : a.outer;
+    const int col0 = blockIdx.y * plan.columns;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < plan.stages; s++) {
+            bar_init(&bars.full[s], EM_FEED);
+            bar_init(&bars.empty[s], 1);
+            bar_init(&bars.b_full[s], 1);
+        }
+        bar_init(&bars.panel_full, 1);
+        bar_init(&bars.panel_free, 1);
+        for (int b = 0; b < 2; b++) {
+            bar_init(&bars.sums_full[b], 1);
+            bar_init(&bars.sums_free[b], EM_OUT);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) tensor_alloc(&bars.tensor, plan.tensor_columns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = bars.tensor;
+
+    int64_t pieces = 0;
+    (void)tl_tile(a, INT64_MAX, TM_ROWS, &pieces);
+    const int64_t per = (pieces + gridDim.x - 1) / gridDim.x, first = blockIdx.x * per;
+    TmCursor cursor;
+    cursor.start(a, first, min(per, pieces - first));
+
+    if (warp < EM_OUT) {
+        // sums to results: warps w and w + 4 share the rows 32 (w % 4) on, and take the groups of 32 columns in turn
+        unsigned char* const out = static_cast<unsigned char*>(plan.back ? a.dx : a.y);
+        const int have = min(plan.columns, nn - col0), half = warp >> 2;
+        const bool with_offset = !plan.back && a.b != nullptr;
+        const int activation = plan.back ? DYNB_ACTIVATION_NONE : e.activation;
+        const bool with_slope = activation != DYNB_ACTIVATION_NONE && e.slope != nullptr;
+        if (blockIdx.y == 0) ex_clear_absent(a, out, (int64_t)nn * SIZE, threadIdx.x, EM_OUT * 32);
+        float* const offset = offsets[warp];
+        int buffer = 0, offset_type = -1;
+        uint32_t phase = 0;
+        for (; cursor.tile.type >= 0; cursor.next(a)) {
+            const int64_t place = cursor.tile.begin + (warp & 3) * 32 + lane;
+            int32_t r = place < cursor.tile.end ? __ldg(a.order + place) : -1;
+            if (with_offset && cursor.tile.type != offset_type) {
+                offset_type = cursor.tile.type;
+                __syncwarp();
+                for (int c = half * 32; c < have; c += 64)
+                    offset[c / 64 * 32 + lane] = c + lane < have ? tl_get(static_cast<const T*>(a.b) + (int64_t)offset_type * a.outer + col0 + c + lane) : 0.0f;
+                __syncwarp();
+            }
+            if (!bar_wait(&bars.sums_full[buffer], phase)) { tm_ran_out(a); break; }
+            tensor_fence_after();
+            if ((uint32_t)r >= (uint64_t)a.n) r = -1;
+            const uint32_t from = tensor + ((uint32_t)((warp & 3) * 32) << 16) + buffer * plan.column_stride;
+            for (int c = half * 32; c < have; c += 64) {
+                uint32_t bits[32];
+                __syncwarp();
+                tensor_load_32(from + c, bits);
+                if constexpr (PARTS > 1) {   // the small products' sums
+                    uint32_t small[32];
+                    tensor_load_32(from + 2 * plan.column_stride + c, small);
+                    tensor_wait_loads();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
+                } else {
+                    tensor_wait_loads();
+                }
+                if (with_offset) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 o = *reinterpret_cast<const float4*>(offset + c / 64 * 32 + i);
+                        bits[i] = __float_as_uint(__uint_as_float(bits[i]) + o.x);
+                        bits[i + 1] = __float_as_uint(__uint_as_float(bits[i + 1]) + o.y);
+                        bits[i + 2] = __float_as_uint(__uint_as_float(bits[i + 2]) + o.z);
+                        bits[i + 3] = __float_as_uint(__uint_as_float(bits[i + 3]) + o.w);
+                    }
+                }
+                uint32_t slopes[sizeof(T) == 4 ? 32 : 16];
+                if (activation != DYNB_ACTIVATION_NONE) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float s0, s1;
+                        const float v0 = ex_activate(__uint_as_float(bits[i]), activation, &s0), v1 = ex_activate(__uint_as_float(bits[i + 1]), activation, &s1);
+                        bits[i] = __float_as_uint(v0);
+                        bits[i + 1] = __float_as_uint(v1);
+                        if constexpr (sizeof(T) == 4) {
+                            slopes[i] = __float_as_uint(s0);
+                            slopes[i + 1] = __float_as_uint(s1);
+                        } else {
+                            slopes[i / 2] = __byte_perm(ex_slope_bits(s0), ex_slope_bits(s1), 0x5410);
+                        }
+                    }
+                }
+                unsigned char* const mine = turned[warp];
+                const int64_t row_bytes = (int64_t)nn * SIZE;
+                unsigned char* const at = out + (int64_t)(col0 + c) * SIZE;
+                const int bytes = (have - c) * SIZE;
+                if constexpr (SIZE == 4) {
+                    em_put(mine, bits, lane, r, at, row_bytes, bytes, plan.store, 4);
+                    if (bytes > 64) em_put(mine, bits + 16, lane, r, at + 64, row_bytes, bytes - 64, plan.store, 4);
+                } else {
+                    uint32_t words[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float v[4] = {__uint_as_float(bits[i]), __uint_as_float(bits[i + 1]), __uint_as_float(bits[i + 2]), __uint_as_float(bits[i + 3])};
+                        tm_words<O>(v, words + i / 2);
+                    }
+                    em_put(mine, words, lane, r, at, row_bytes, bytes, plan.store, 2);
+                }
+                if (with_slope) {
+                    constexpr int S = sizeof(T) == 4 ? 4 : 2;
+                    unsigned char* const to = static_cast<unsigned char*>(e.slope) + (int64_t)(col0 + c) * S;
+                    em_put(mine, slopes, lane, r, to, (int64_t)nn * S, (have - c) * S, plan.slope_store, S);
+                    if constexpr (S == 4) {
+                        if (have - c > 16) em_put(mine, slopes + 16, lane, r, to + 64, (int64_t)nn * S, (have - c - 16) * S, plan.slope_store, S);
+                    }
+                }
+            }
+            tensor_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(&bars.sums_free[buffer]);
+            buffer ^= 1;
+            if (buffer == 0) phase ^= 1;
+        }
+    } else if (warp == EM_OUT) {
+        // products
+        const bool bf16 = !std::is_same<T, __half>::value;
+        const uint32_t what = mma_what(bf16, plan.columns, false, false);
+        const int b_part = plan.columns * 128 / 16;
+        int stage = 0, buffer = 0, panel_type = -1;
+        uint32_t phase = 0, panel_phase = 0, sums_phase = 1;
+        bool ok = true;
+        while (ok && cursor.tile.type >= 0) {
+            if (plan.resident && cursor.tile.type != panel_type) {
+                if (!bar_wait(&bars.panel_full, panel_phase)) { ok = false; break; }
+                panel_phase ^= 1;
+                panel_type = cursor.tile.type;
+            }
+            if (!bar_wait(&bars.sums_free[buffer], sums_phase)) { ok = false; break; }
+            tensor_fence_after();
+            const uint32_t sums = tensor + buffer * plan.column_stride;
+            for (int chunk = 0; chunk < plan.chunks; chunk++) {
+                if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+                if (!plan.resident && !bar_wait(&bars.b_full[stage], phase)) { ok = false; break; }
+                tensor_fence_after();
+                if (elected()) {
+                    const int steps = min(4, (kk - chunk * 64 + 15) / 16);
+                    unsigned char* const at = stage0 + stage * plan.stage_bytes;
+                    const uint64_t at_a = tile_descriptor(smem_addr(at), 16, 1024);
+                    const uint64_t at_b = tile_descriptor(smem_addr(plan.resident ? panel + chunk * plan.b_bytes : at + A_BYTES), 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (k < steps) tm_step<PARTS>(sums, sums + 2 * plan.column_stride, at_a + 2 * k, TM_ROWS * 128 / 16, at_b + 2 * k, b_part, what, chunk > 0 || k > 0);
+                    tensor_commit(&bars.empty[stage]);
+                    if (chunk == plan.chunks - 1) tensor_commit(&bars.sums_full[buffer]);
+                }
+                __syncwarp();
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+            }
+            if (!ok) break;
+            cursor.next(a);
+            if (plan.resident && cursor.tile.type >= 0 && cursor.tile.type != panel_type && elected()) tensor_commit(&bars.panel_free);
+            __syncwarp();
+            buffer ^= 1;
+            if (buffer == 0) sums_phase ^= 1;
+        }
+        if (!ok) tm_ran_out(a);
+    } else if (warp == EM_OUT + 1) {
+        // matrices
+        const int64_t tiles = gridDim.y;
+        if (plan.resident) {
+            int panel_type = -1;
+            uint32_t free_phase = 0, asked = 0;
+            for (; cursor.tile.type >= 0; cursor.next(a)) {
+                if (cursor.tile.type == panel_type) continue;
+                if (panel_type >= 0) {
+                    if (!bar_wait(&bars.panel_free, free_phase)) { tm_ran_out(a); break; }
+                    free_phase ^= 1;
+                }
+                panel_type = cursor.tile.type;
+                if (elected()) {
+                    const unsigned char* const from = plan.packed + ((int64_t)panel_type * tiles + blockIdx.y) * plan.chunks * plan.b_bytes;
+                    bulk_expect(&bars.panel_full, plan.chunks * plan.b_bytes);
+                    for (int chunk = 0; chunk < plan.chunks; chunk++) bulk_copy(panel + chunk * plan.b_bytes, from + (int64_t)chunk * plan.b_bytes, plan.b_bytes, &bars.panel_full);
+                }
+                __syncwarp();
+                asked++;
+            }
+            if (asked > 0) (void)bar_wait(&bars.panel_full, (asked - 1) & 1);   // a block does not end before its copies
+        } else {
+            int stage = 0;
+            uint32_t phase = 1;
+            int64_t asked = 0;
+            bool ok = true;
+            for (; ok && cursor.tile.type >= 0; cursor.next(a)) {
+                const unsigned char* from = plan.packed + ((int64_t)cursor.tile.type * tiles + blockIdx.y) * plan.chunks * plan.b_bytes;
+                for (int chunk = 0; chunk < plan.chunks; chunk++, from += plan.b_bytes) {
+                    if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); ok = false; break; }
+                    if (elected()) {
+                        bulk_expect(&bars.b_full[stage], plan.b_bytes);
+                        bulk_copy(stage0 + stage * plan.stage_bytes + A_BYTES, from, plan.b_bytes, &bars.b_full[stage]);
+                    }
+                    __syncwarp();
+                    asked++;
+                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                }
+            }
+            // the last copy of every stage: number c of stage c % stages
+            for (int64_t c = max(asked - plan.stages, (int64_t)0); c < asked; c++) (void)bar_wait(&bars.b_full[c % plan.stages], (uint32_t)(c / plan.stages) & 1);
+        }
+    } else {
+        // rows to shared memory
+        const T* const in = static_cast<const T*>(plan.back ? a.dy : a.x);
+        const int64_t in_row = plan.back ? a.dy_row : a.x_row;
+        const int fan = plan.back ? 1 : e.fan;
+        const uint32_t rows_in = (uint32_t)(plan.back ? a.n : e.n_in);
+        constexpr int UNITS = TM_ROWS * 8 / (EM_FEED * 32);
+        const int tid = threadIdx.x - (EM_OUT + 2) * 32, piece = tid & 7;
+        int32_t rows[UNITS], rows_next[UNITS];      // of the next tile to ask for, and the one behind it
+        auto rows_of = [&](const TlTile& t, int32_t (&r)[UNITS]) {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const int64_t place = t.begin + (tid >> 3) + (EM_FEED * 4) * i;
+                r[i] = t.type >= 0 && place < t.end ? __ldg(a.order + place) : -1;   // looked at a tile later
+            }
+        };
+        // the pair's row, or a number that is no row
+        auto row_in = [&](int32_t p) { return (uint32_t)p >= (uint64_t)a.n ? 0xffffffffu : fan == 1 ? (uint32_t)p : (uint32_t)p / (uint32_t)fan; };
+        int stage = 0;
+        uint32_t phase = 1;
+        if constexpr (PATH == EM_ASYNC) {
+            int arrived = 0;                        // stage of the next arrival
+            int64_t asked = 0;
+            rows_of(cursor.tile, rows);
+            bool ok = true;
+            auto arrive = [&] {
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[arrived]);
+                if (++arrived == plan.stages) arrived = 0;
+            };
+            while (ok && cursor.tile.type >= 0) {
+                uint32_t at[UNITS];
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) at[i] = row_in(rows[i]);
+                cursor.next(a);
+                rows_of(cursor.tile, rows);
+                for (int chunk = 0; chunk < plan.chunks; chunk++) {
+                    if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); ok = false; break; }
+                    const uint32_t to = smem_addr(stage0) + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);   // EM_FEED * 4 rows on: the same place among eight
+                    const int k = chunk * 64 + piece * 8;
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) {
+                        const bool live = at[i] < rows_in && k < kk;
+                        copy_16(to + i * EM_FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
+                    }
+                    copies_commit();
+                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                    if (++asked > plan.depth) {
+                        copies_wait(plan.depth);
+                        arrive();
+                    }
+                }
+            }
+            for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
+                copies_wait(left - 1);
+                arrive();
+            }
+            copies_wait(0);
+        } else {
+            constexpr int AHEAD = sizeof(T) == 4 && PATH == EM_SLOPE ? 1 : 2;
+            constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
+            TlTile next = cursor.tile;
+            int chunk = 0;
+            TmRaw<T> v[AHEAD][UNITS], slope[AHEAD][SLOPES];
+            bool live[AHEAD];
+            auto ask = [&](TmRaw<T> (&to)[UNITS], TmRaw<T> (&to_slope)[SLOPES], bool& any) {
+                any = next.type >= 0;
+                if (!any) return;
+                const int k = chunk * 64 + piece * 8, have = min(8, kk - k);
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) {
+                    const uint32_t at = row_in(rows[i]);
+                    const bool ok = at < rows_in;
+                    to[i] = tm_load<WIDE>(in + (ok ? at * in_row + k : 0), 1, ok ? have : 0);
+                    if constexpr (PATH == EM_SLOPE) to_slope[i] = tm_load<WIDE>(static_cast<const T*>(e.slope) + (ok ? (int64_t)at * kk + k : 0), 1, ok ? have : 0);
+                }
+                if (++chunk == plan.chunks) {
+                    chunk = 0;
+                    next = cursor.tile;
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) rows[i] = rows_next[i];
+                    if (next.type >= 0) {
+                        cursor.next(a);
+                        rows_of(cursor.tile, rows_next);
+                    }
+                }
+            };
+            rows_of(next, rows);
+            if (next.type >= 0) cursor.next(a);
+            rows_of(cursor.tile, rows_next);
+#pragma unroll
+            for (int s = 0; s < AHEAD; s++) ask(v[s], slope[s], live[s]);
+            bool more = true;
+            while (more) {
+#pragma unroll
+                for (int s = 0; s < AHEAD; s++) {
+                    if (!live[s]) { more = false; break; }
+                    if constexpr (PATH == EM_SLOPE) {
+#pragma unroll
+                        for (int i = 0; i < UNITS; i++) em_times(v[s][i], slope[s][i]);
+                    }
+                    if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
+                    unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
+                    if (tm_odd(v[s])) {
+#pragma unroll
+                        for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * EM_FEED * 512, TM_ROWS * 128);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * EM_FEED * 512, TM_ROWS * 128);
+                    }
+                    fence_to_tensor();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&bars.full[stage]);
+                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                    ask(v[s], slope[s], live[s]);
+                }
+            }
+        }
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (warp == 0) tensor_free(tensor, plan.tensor_columns);
+}
+
+// ------------------------------------------------------------------------------------------------ gradients of the matrices
+constexpr int EW_FEED = 16, EW_THREADS = (4 + 1 + EW_FEED) * 32, EW_ROWS = 32, EW_MAX_STAGES = 8;
+constexpr int EW_SMEM = 222 * 1024;
+
+struct EwPlan { int columns, column_stride, x_blocks, y_blocks, row_tiles, column_tiles, stages, depth, tensor_columns, vec; };
+struct EwBars { uint64_t full[EW_MAX_STAGES], empty[EW_MAX_STAGES], sums_full; uint32_t tensor; };
+
+__device__ __forceinline__ void ew_put_row(float* at, const uint32_t (&v)[32], int n, bool wide)
+{
+    if (wide && n >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(at + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; i++)
+        if (i < n) at[i] = __uint_as_float(v[i]);
+}
+
+template <typename T, EmPath PATH, bool WIDE>
+__global__ void __launch_bounds__(EW_THREADS, 1)
+em_weights_kernel(const ExArgs e, const EwPlan plan)
+{
+    constexpr int PARTS = TmParts<T>::N, FIRST = PARTS == 1 ? 1 : 2;   // sums of the matrix: leading parts, small ones; those of the rows behind them
+    constexpr int FEED_THREADS = EW_FEED * 32, BLOCK = EW_ROWS * 128;
+    constexpr int UNITS = PARTS == 1 ? 3 : 2;   // pieces of 8 elements a thread and stage: 32 pairs x (128 + 256 or 128) elements
+    const TlArgs& a = e.t;
+    extern __shared__ unsigned char raw_smem[];
+    __shared__ EwBars bars;
+    unsigned char* const ones = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
+    unsigned char* const stage0 = ones + TM_ROWS * 128;
+    const int warp = warp_number(), lane = threadIdx.x & 31;
+    // the tiles of a stretch are neighbours: what they share comes from L2
+    const int tiles = plan.row_tiles * plan.column_tiles, of_tile = blockIdx.x % tiles;
+    const int64_t stretch = blockIdx.x / tiles;
+    const int row0 = of_tile / plan.column_tiles * TM_ROWS, col0 = of_tile % plan.column_tiles * plan.columns;
+    const int blocks = plan.x_blocks + plan.y_blocks, stage_bytes = blocks * PARTS * BLOCK;
+    const TlTile tile = tl_tile(a, stretch, a.stretch);
+    if (tile.type < 0) return;   // the whole block
+    const int steps = (int)((tile.end - tile.begin + EW_ROWS - 1) / EW_ROWS);
+    const bool sums_wanted = row0 == 0 && a.db != nullptr;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < plan.stages; s++) {
+            bar_init(&bars.full[s], EW_FEED);
+            bar_init(&bars.empty[s], 1);
+        }
+        bar_init(&bars.sums_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    const uint32_t one = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+    for (int i = threadIdx.x; i < TM_ROWS * 8; i += EW_THREADS) reinterpret_cast<uint4*>(ones)[i] = make_uint4(one, one, one, one);
+    fence_to_tensor();
+    if (warp == 0) tensor_alloc(&bars.tensor, plan.tensor_columns);
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    const uint32_t tensor = bars.tensor;
+
+    if (warp < 4) {
+        if (!bar_wait(&bars.sums_full, 0)) {
+            tm_ran_out(a);
+        } else {
+            tensor_fence_after();
+            const int64_t cells = (int64_t)a.inner * a.outer;
+            float* const mine = a.partial + stretch * (cells + a.outer);
+            const int m = row0 + threadIdx.x, have = min(plan.columns, a.outer - col0);
+            for (int which = 0; which < (sums_wanted ? 2 : 1); which++) {
+                float* const at = which == 0 ? mine + (int64_t)m * a.outer + col0 : mine + cells + col0;
+                const bool write = which == 0 ? m < a.inner : threadIdx.x == 0;
+                const uint32_t from = tensor + ((uint32_t)(warp * 32) << 16) + which * FIRST * plan.column_stride;
+                for (int c = 0; c < have; c += 32) {
+                    uint32_t bits[32];
+                    __syncwarp();
+                    tensor_load_32(from + c, bits);
+                    tensor_wait_loads();
+                    if constexpr (PARTS > 1) {
+                        uint32_t small[32];
+                        tensor_load_32(from + plan.column_stride + c, small);
+                        tensor_wait_loads();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
+                    }
+                    if (write) ew_put_row(at + c, bits, have - c, plan.vec != 0);
+                }
+            }
+        }
+    } else if (warp == 4) {
+        const bool bf16 = !std::is_same<T, __half>::value;
+        const uint32_t what = mma_what(bf16, plan.columns, true, true), what_sum = mma_what(bf16, plan.columns, false, true);
+        const uint32_t stage_at = smem_addr(stage0);
+        const uint64_t ones_desc = tile_descriptor(smem_addr(ones), 16, 1024);
+        const uint32_t lead = PARTS * BLOCK, lead_x = plan.x_blocks > 1 ? lead : 0;   // one block: the upper 64 rows repeat the lower
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int step = 0; step < steps; step++) {
+            if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+            tensor_fence_after();
+            if (elected()) {
+                const uint32_t at = stage_at + stage * stage_bytes;
+                const uint64_t at_x = tile_descriptor(at, lead_x, 1024), at_y = tile_descriptor(at + plan.x_blocks * PARTS * BLOCK, lead, 1024);
+#pragma unroll
+                for (int k = 0; k < EW_ROWS / 16; k++) tm_step<PARTS>(tensor, tensor + plan.column_stride, at_x + k * 128, BLOCK / 16, at_y + k * 128, BLOCK / 16, what, step > 0 || k > 0);
+                if (sums_wanted) {
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+                        for (int k = 0; k < EW_ROWS / 16; k++)
+                            tensor_mma(tensor + (p == 0 ? FIRST : FIRST + 1) * plan.column_stride, ones_desc, at_y + (p * BLOCK + k * 2048) / 16, what_sum,
+                                       step > 0 || k > 0 || (p > 0 && p < PARTS - 1));
+                }
+                tensor_commit(&bars.empty[stage]);
+                if (step == steps - 1) tensor_commit(&bars.sums_full);
+            }
+            __syncwarp();
+            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) tm_ran_out(a);
+    } else {
+        const int tid = threadIdx.x - 5 * 32;
+        const int per_row = blocks * 8, units = EW_ROWS * per_row;
+        // this thread's pieces are the same ones in every stage: row, place in the stage, operand, column
+        int row[UNITS], at[UNITS], col[UNITS];
+#pragma unroll
+        for (int i = 0; i < UNITS; i++) {
+            const int u = tid + i * FEED_THREADS, r = u / per_row, piece = u % per_row;
+            const int block = piece >> 3;
+            const bool of_y = block >= plan.x_blocks;
+            row[i] = u < units ? r : -1;
+            at[i] = block * PARTS * BLOCK + (int)tile_piece(r, piece & 7);
+            const int c = (of_y ? col0 + (block - plan.x_blocks) * 64 : row0 + block * 64) + (piece & 7) * 8;
+            const int limit = of_y ? min(a.outer, col0 + plan.columns) : a.inner;
+            col[i] = c < limit ? (of_y ? c | (1 << 30) : c) : -1;
+        }
+        auto rows_of = [&](int step, int32_t (&r)[UNITS]) {
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const int64_t place = tile.begin + (int64_t)step * EW_ROWS + row[i];
+                r[i] = row[i] >= 0 && col[i] >= 0 && place < tile.end ? __ldg(a.order + place) : -1;   // looked at a stage later
+            }
+        };
+        const uint32_t fan = e.fan;
+        auto address = [&](int i, int32_t p) {
+            const int c = col[i] & ((1 << 30) - 1);
+            if ((col[i] >> 30) & 1) return static_cast<const T*>(a.dy) + p * a.dy_row + c;
+            return static_cast<const T*>(a.x) + (int64_t)(fan == 1 ? (uint32_t)p : (uint32_t)p / fan) * a.x_row + c;
+        };
+        int32_t ids[UNITS];
+        int stage = 0;
+        uint32_t phase = 1;
+        if constexpr (PATH == EM_ASYNC) {
+            int arrived = 0;
+            auto arrive = [&] {
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[arrived]);
+                if (++arrived == plan.stages) arrived = 0;
+            };
+            rows_of(0, ids);
+            int asked = 0;
+            for (int step = 0; step < steps; step++) {
+                int32_t next[UNITS];
+                rows_of(step + 1, next);
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+                const uint32_t to = smem_addr(stage0) + stage * stage_bytes;
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) {
+                    const bool live = (uint32_t)ids[i] < (uint64_t)a.n;
+                    if (row[i] >= 0) copy_16(to + at[i], live ? address(i, ids[i]) : static_cast<const T*>(a.x), live);
+                    ids[i] = next[i];
+                }
+                copies_commit();
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                if (++asked > plan.depth) {
+                    copies_wait(plan.depth);
+                    arrive();
+                }
+            }
+            for (int left = min(asked, plan.depth); left > 0; left--) {
+                copies_wait(left - 1);
+                arrive();
+            }
+            copies_wait(0);
+        } else {
+            constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
+            TmRaw<T> v[UNITS], slope[SLOPES];
+            auto fetch = [&](const int32_t (&r)[UNITS]) {
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) {
+                    const bool of_y = (col[i] >> 30) & 1, ok = (uint32_t)r[i] < (uint64_t)a.n;
+                    const int c = col[i] & ((1 << 30) - 1), have = ok ? min(8, (of_y ? a.outer : a.inner) - c) : 0;
+                    v[i] = tm_load<WIDE>(ok ? address(i, r[i]) : static_cast<const T*>(a.x), 1, have);
+                    if constexpr (PATH == EM_SLOPE) {
+                        const bool with = ok && of_y;
+                        slope[i] = tm_load<WIDE>(static_cast<const T*>(e.slope) + (with ? (int64_t)r[i] * a.outer + c : 0), 1, with ? have : 0);
+                    }
+                }
+            };
+            // the rows of the next stage are asked for behind this one, their numbers a stage earlier
+            rows_of(0, ids);
+            fetch(ids);
+            rows_of(1, ids);
+            for (int step = 0; step < steps; step++) {
+                if constexpr (PATH == EM_SLOPE) {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++)
+                        if ((col[i] >> 30) & 1) em_times(v[i], slope[i]);
+                }
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+                if (tm_odd(v)) {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++)
+                        if (row[i] >= 0) tm_store<true>(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++)
+                        if (row[i] >= 0) tm_store<false>(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                }
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[stage]);
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                fetch(ids);   // behind the stretch: zeros
+                rows_of(step + 2, ids);
+            }
+        }
+    }
+    tensor_fence_before();
+    __syncthreads();
+    tensor_fence_after();
+    if (warp == 0) tensor_free(tensor, plan.tensor_columns);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+template <typename T>
+static EmPlan em_plan(const ExArgs& e, int back, int* tiles)
+{
+    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, MOST = PARTS == 1 ? 256 : 128;
+    const int kk = back ? e.t.outer : e.t.inner, nn = back ? e.t.inner : e.t.outer;
+    EmPlan p = {};
+    p.back = back;
+    p.chunks = (kk + 63) / 64;
+    *tiles = (nn + MOST - 1) / MOST;
+    p.columns = tm_round((nn + *tiles - 1) / *tiles, 16);
+    *tiles = (nn + p.columns - 1) / p.columns;
+    p.column_stride = tm_round(p.columns, 32);
+    p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
+    p.b_bytes = PARTS * p.columns * 128;
+    p.resident = (int64_t)p.chunks * p.b_bytes + (PARTS == 1 ? 4 : 2) * A_BYTES + 1024 <= EM_SMEM;
+    p.stage_bytes = A_BYTES + (p.resident ? 0 : p.b_bytes);
+    p.stages = std::min(EM_MAX_STAGES, (EM_SMEM - 1024 - (p.resident ? p.chunks * p.b_bytes : 0)) / p.stage_bytes);
+    p.depth = std::min(EM_DEPTH, p.stages - 1);
+    return p;
+}
+
+template <typename T>
+static int64_t em_packed(const ExArgs& e, int back)
+{
+    int tiles;
+    const EmPlan p = em_plan<T>(e, back, &tiles);
+    return (int64_t)e.t.types * tiles * p.chunks * p.b_bytes;
+}
+
+int64_t ex_packed_bytes(const ExArgs& e, int back, int dtype) { return dtype == DYNB_F32 ? em_packed<float>(e, back) : em_packed<__nv_bfloat16>(e, back); }
+
+template <typename T, typename O>
+static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t s)
+{
+    constexpr int SIZE = (int)sizeof(T);
+    const TlArgs& a = e.t;
+    int tiles;
+    EmPlan p = em_plan<T>(e, back, &tiles);
+    p.packed = static_cast<const unsigned char*>(packed);
+    const int kk = back ? a.outer : a.inner, nn = back ? a.inner : a.outer;
+    const void* const in = back ? a.dy : a.x;
+    const void* const out = back ? a.dx : a.y;
+    const bool slope = back && e.activation != DYNB_ACTIVATION_NONE;
+    const bool wide = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0 && (!slope || tm_on(e.slope, kk, SIZE, 16));
+    p.store = tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
+    p.slope_store = e.slope != nullptr && tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
+    const int64_t units = (int64_t)a.types * tiles * p.chunks * p.columns * 8;
+    ex_pack_kernel<T><<<(unsigned)std::min<int64_t>((units + 255) / 256, (int64_t)sm_count_cached() * 8), 256, 0, s>>>(
+        static_cast<const T*>(a.w), a.types, a.inner, a.outer, back, p.columns, tiles, p.chunks, static_cast<unsigned char*>(packed));
+    cudaError_t rc = cudaGetLastError();
+    if (rc != cudaSuccess) return rc;
+    void (*kernel)(ExArgs, EmPlan);
+    if (slope) kernel = wide ? em_rows_kernel<T, O, EM_SLOPE, true> : em_rows_kernel<T, O, EM_SLOPE, false>;
+    else if (!wide) kernel = em_rows_kernel<T, O, EM_REGISTERS, false>;
+    else if constexpr (SIZE == 4) kernel = em_rows_kernel<T, O, EM_REGISTERS, true>;
+    else kernel = em_rows_kernel<T, O, EM_ASYNC, true>;
+    const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
+    const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
+    const int smem = 1024 + (p.resident ? p.chunks * p.b_bytes : 0) + p.stages * p.stage_bytes;
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc != cudaSuccess) return rc;
+    kernel<<<grid, EM_THREADS, smem, s>>>(e, p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t em_rows_of(const ExArgs& e, int back, void* packed, cudaStream_t s)
+{
+    if constexpr (sizeof(T) == 2) {
+        if (back && e.fan > 1) return em_rows<T, float>(e, back, packed, s);
+    }
+    return em_rows<T, T>(e, back, packed, s);
+}
+
+cudaError_t ex_mma_rows(const ExArgs& e, int back, int dtype, void* packed, cudaStream_t s)
+{
+    if (dtype == DYNB_F32) return em_rows_of<float>(e, back, packed, s);
+    if (dtype == DYNB_F16) return em_rows_of<__half>(e, back, packed, s);
+    return em_rows_of<__nv_bfloat16>(e, back, packed, s);
+}
+
+int64_t ex_stretches(const ExArgs& e) { return tl_stretches(e.t.n, e.t.types, e.t.stretch); }
+
+template <typename T>
+static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
+{
+    constexpr int PARTS = TmParts<T>::N, BLOCK = EW_ROWS * 128, SIZE = (int)sizeof(T);
+    const TlArgs& a = e.t;
+    EwPlan p = {};
+    const int most = PARTS == 1 ? 256 : 128, tiles = (a.outer + most - 1) / most;
+    p.columns = tm_round((a.outer + tiles - 1) / tiles, 16);
+    p.column_stride = tm_round(p.columns, 32);
+    p.x_blocks = a.inner > 64 ? 2 : 1;
+    p.y_blocks = (p.columns + 63) / 64;
+    p.row_tiles = (a.inner + TM_ROWS - 1) / TM_ROWS;
+    p.column_tiles = (a.outer + p.columns - 1) / p.columns;
+    const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
+    p.stages = std::min(EW_MAX_STAGES, (EW_SMEM - 1024 - TM_ROWS * 128) / stage);
+    p.depth = std::min(EM_DEPTH, p.stages - 1);
+    p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
+    const bool slope = e.activation != DYNB_ACTIVATION_NONE;
+    const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0 && (!slope || tm_on(e.slope, 0, SIZE, 16));
+    p.vec = a.outer % 4 == 0 && tm_on(a.partial, 0, 4, 16);
+    void (*kernel)(ExArgs, EwPlan);
+    if (slope) kernel = wide ? em_weights_kernel<T, EM_SLOPE, true> : em_weights_kernel<T, EM_SLOPE, false>;
+    else if (!wide) kernel = em_weights_kernel<T, EM_REGISTERS, false>;
+    else if constexpr (SIZE == 4) kernel = em_weights_kernel<T, EM_REGISTERS, true>;
+    else kernel = em_weights_kernel<T, EM_ASYNC, true>;
+    const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;
+    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc != cudaSuccess) return rc;
+    const int64_t grid = ex_stretches(e) * p.row_tiles * p.column_tiles;
+    kernel<<<(unsigned)grid, EW_THREADS, smem, s>>>(e, p);
+    return cudaGetLastError();
+}
+
+cudaError_t ex_mma_weights(const ExArgs& e, int dtype, cudaStream_t s)
+{
+    if (dtype == DYNB_F32) return em_weights<float>(e, s);
+    if (dtype == DYNB_F16) return em_weights<__half>(e, s);
+    return em_weights<__nv_bfloat16>(e, s);
+}
+
+}  // namespace dynb

@@ -196,6 +196,12 @@ def _linear_args(weight, routing: Routing, paired: bool, activation: int, dtype)
     return a
 
 
+def _linear_workspace(args, backward: int, want_x: int, want_weights: int, dev) -> torch.Tensor:
+    nbytes = ctypes.c_int64()
+    _lib.check(_lib.lib().dynb_expert_linear_workspace_bytes(ctypes.byref(args), backward, want_x, want_weights, ctypes.byref(nbytes)), "expert_linear_workspace_bytes")
+    return torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+
+
 def _pairs(t: torch.Tensor) -> torch.Tensor:
     """[rows, choices, width] as [pairs, width] with one stride from pair to pair and consecutive elements."""
     rows, choices, width = t.shape
@@ -221,8 +227,9 @@ class _ExpertLinear(torch.autograd.Function):
             if keep and activation:
                 slope = torch.empty(z.shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16, device=dev)
             args = _linear_args(weight, routing, paired, activation, x.dtype)
+            ws = _linear_workspace(args, 0, 0, 0, dev)
             _lib.check(_lib.lib().dynb_expert_linear(ctypes.byref(args), flat.data_ptr(), flat.stride(0), _pointer(bias), z.data_ptr(), _pointer(slope),
-                                                     _lib.stream_of(dev)), "expert_linear")
+                                                     ws.data_ptr(), ws.numel(), _lib.stream_of(dev)), "expert_linear")
         if keep:
             ctx.save_for_backward(flat, weight, slope)
             ctx.routing, ctx.activation, ctx.shape = routing, activation, x.shape
@@ -234,17 +241,13 @@ class _ExpertLinear(torch.autograd.Function):
         x, weight, slope = ctx.saved_tensors
         dev, d_z, routing, paired = x.device, _pairs(d_z), ctx.routing, len(ctx.shape) == 3
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        L = _lib.lib()
         with _lib.on_device(dev):
             args = _linear_args(weight, routing, paired, ctx.activation, x.dtype)   # anew: hooks may have moved what was saved
             dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if want_x else None
             dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if want_w else None
             db = torch.empty((weight.size(0), weight.size(2)), dtype=x.dtype, device=dev) if want_b else None
-            nbytes = ctypes.c_int64()
-            _lib.check(L.dynb_expert_linear_workspace_bytes(ctypes.byref(args), int(want_x), int(want_w or want_b), ctypes.byref(nbytes)),
-                       "expert_linear_workspace_bytes")
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-            _lib.check(L.dynb_expert_linear_backward(ctypes.byref(args), x.data_ptr(), x.stride(0), d_z.data_ptr(), d_z.stride(0), _pointer(slope),
+            ws = _linear_workspace(args, 1, int(want_x), int(want_w or want_b), dev)
+            _lib.check(_lib.lib().dynb_expert_linear_backward(ctypes.byref(args), x.data_ptr(), x.stride(0), d_z.data_ptr(), d_z.stride(0), _pointer(slope),
                                                      routing.experts.data_ptr(), _pointer(dx), _pointer(dw), _pointer(db), ws.data_ptr(), ws.numel(),
                                                      _lib.stream_of(dev)), "expert_linear_backward")
         return dx, dw, db, None, None, None

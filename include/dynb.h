@@ -568,7 +568,7 @@ int dynb_route_experts_backward(const dynb_routing* args, const int32_t* experts
 /* Products with the matrices of a row's experts: z[i, j] = act(x[i] weight[e_ij] (+ bias[e_ij])), or x[i, j] where x is `paired`; weight
  * [experts, inner, outer], contiguous, as bias, z and the gradients are.  x and d_z have strides in elements from row to row (from pair to pair).  Places
  * without an expert give zeros.  slope_dev (NULL when there is no backward pass, or no activation): what the backward pass needs of the activation,
- * [n_rows choices, outer] of 4 bytes for DYNB_F32 and 2 otherwise. */
+ * [n_rows choices, outer] of 4 bytes for DYNB_F32 and 2 otherwise.  Workspaces start on 16-byte boundaries. */
 #define DYNB_ACTIVATION_NONE 0
 #define DYNB_ACTIVATION_SILU 1
 #define DYNB_ACTIVATION_GELU 2
@@ -579,8 +579,9 @@ typedef struct dynb_expert_linear_args {
     int32_t choices, experts, inner, outer, dtype, paired, activation, reserved;
     uint32_t* status_dev;                   /* as in dynb_type_linear_args */
 } dynb_expert_linear_args;
-int dynb_expert_linear(const dynb_expert_linear_args* args, const void* x_dev, int64_t x_row, const void* bias_dev, void* z_dev, void* slope_dev, void* stream);
-int dynb_expert_linear_workspace_bytes(const dynb_expert_linear_args* args, int want_x, int want_weights, int64_t* bytes);
+int dynb_expert_linear_workspace_bytes(const dynb_expert_linear_args* args, int backward, int want_x, int want_weights, int64_t* bytes);
+int dynb_expert_linear(const dynb_expert_linear_args* args, const void* x_dev, int64_t x_row, const void* bias_dev, void* z_dev, void* slope_dev,
+                       void* workspace_dev, int64_t workspace_bytes, void* stream);
 int dynb_expert_linear_backward(const dynb_expert_linear_args* args, const void* x_dev, int64_t x_row, const void* d_z_dev, int64_t d_z_row, const void* slope_dev,
                                 const int32_t* experts_dev, void* d_x_dev, void* d_weight_dev, void* d_bias_dev, void* workspace_dev, int64_t workspace_bytes,
                                 void* stream);

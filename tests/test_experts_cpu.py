@@ -87,16 +87,19 @@ def _linear(**change):
 def test_linear_entry_refuses(change):
     """The last case: null pointers."""
     L, a, n = _lib.lib(), _linear(**change), ctypes.c_int64()
-    assert L.dynb_expert_linear(ctypes.byref(a), None, 8, None, None, None, None) == -1
+    assert L.dynb_expert_linear(ctypes.byref(a), None, 8, None, None, None, None, 0, None) == -1
     assert L.dynb_expert_linear_backward(ctypes.byref(a), None, 8, None, 4, None, None, None, None, None, None, 0, None) == -1
-    assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), 1, 1, ctypes.byref(n)) == -1
-    assert L.dynb_expert_linear(None, None, 8, None, None, None, None) == -1
+    assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), 1, 1, 1, ctypes.byref(n)) == -1
+    assert L.dynb_expert_linear(None, None, 8, None, None, None, None, 0, None) == -1
 
 
 def test_linear_entry_checks_its_workspace():
     L, at, n = _lib.lib(), 4096, ctypes.c_int64()
     a = _linear(weight_dev=at, order_dev=at, start_dev=at, activation=1)
-    assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), 1, 1, ctypes.byref(n)) == 0 and n.value > 0
+    assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), 0, 0, 0, ctypes.byref(n)) == 0 and n.value > 0
+    for ws, size in ((None, 0), (at, n.value - 1), (at + 8, n.value)):
+        assert L.dynb_expert_linear(ctypes.byref(a), at, 8, None, at, None, ws, size, None) == -1 and b"workspace" in L.dynb_last_error()
+    assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), 1, 1, 1, ctypes.byref(n)) == 0 and n.value > 0
     args = (ctypes.byref(a), at, 8, at, 4, at, at, at, at, at)
     assert L.dynb_expert_linear_backward(*args, None, 0, None) == -1
     assert L.dynb_expert_linear_backward(*args, at, n.value - 1, None) == -1 and b"workspace" in L.dynb_last_error()
@@ -119,7 +122,7 @@ def test_empty_calls_launch_nothing():
     assert L.dynb_rotary_heads_backward(ctypes.byref(a), None, 0, 0, None, 0, 0, None, None, None, None, None, None, 0, None) == 0
     assert L.dynb_route_experts_backward(ctypes.byref(_routing(n_rows=0)), None, None, None, None, None) == 0
     b = _linear(n_rows=0, weight_dev=4096, start_dev=4096)
-    assert L.dynb_expert_linear(ctypes.byref(b), None, 8, None, None, None, None) == 0
+    assert L.dynb_expert_linear(ctypes.byref(b), None, 8, None, None, None, None, 0, None) == 0
     assert L.dynb_expert_linear_backward(ctypes.byref(b), None, 8, None, 4, None, None, 4096, None, None, None, 0, None) == 0
     assert L.dynb_expert_combine(None, None, None, None, 0, 0, 2, 8, 0, None, None) == 0
 
