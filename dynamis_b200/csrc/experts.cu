@@ -12,47 +12,120 @@ namespace dynb {
 
 constexpr int EX_THREADS = 256;
 
-// y_i = r_i + sum_j w_ij z_ij (w null: ones).  Z: type of z.
-template <typename Z, typename T>
+template <typename T, int N> struct __align__(sizeof(T) * N) ExPack { T v[N]; };
+
+// y_i = r_i + sum_j w_ij z_ij (w null: ones).  Z: type of z.  `lanes` threads (a power of two) a row, N elements each, four choices under way.
+template <typename Z, typename T, int N>
 __global__ void __launch_bounds__(EX_THREADS)
-ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide)
+ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide, int lanes)
 {
-    const int64_t all = n * wide;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / wide, c = i % wide;
-        float v = residual != nullptr ? tl_get(residual + row * residual_row + c) : 0.0f;
-        for (int j = 0; j < choices; j++) {
-            const int64_t p = row * choices + j;
-            if (experts[p] >= 0) v = fmaf(weights != nullptr ? weights[p] : 1.0f, tl_get(z + p * wide + c), v);
+    const int in_row = threadIdx.x & (lanes - 1), rows = EX_THREADS / lanes;
+    for (int64_t row = (int64_t)blockIdx.x * rows + threadIdx.x / lanes; row < n; row += (int64_t)gridDim.x * rows) {
+        const int32_t* const es = experts + row * choices;
+        for (int c = in_row * N; c < wide; c += lanes * N) {
+            float sum[N];
+            if (residual != nullptr) {
+                const ExPack<T, N> r = *reinterpret_cast<const ExPack<T, N>*>(residual + row * residual_row + c);
+#pragma unroll
+                for (int i = 0; i < N; i++) sum[i] = tl_get(&r.v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) sum[i] = 0.0f;
+            }
+            const Z* at = z + row * choices * wide + c;
+            for (int j0 = 0; j0 < choices; j0 += 4, at += 4 * wide) {
+                ExPack<Z, N> v[4];
+                float w[4];
+                bool live[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    live[j] = j0 + j < choices && es[j0 + j] >= 0;
+                    w[j] = live[j] && weights != nullptr ? weights[row * choices + j0 + j] : 1.0f;
+                    if (live[j]) v[j] = *reinterpret_cast<const ExPack<Z, N>*>(at + j * wide);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (live[j]) {
+#pragma unroll
+                        for (int i = 0; i < N; i++) sum[i] = fmaf(w[j], tl_get(&v[j].v[i]), sum[i]);
+                    }
+            }
+            ExPack<T, N> out;
+#pragma unroll
+            for (int i = 0; i < N; i++) tl_put(&out.v[i], sum[i]);
+            *reinterpret_cast<ExPack<T, N>*>(y + row * wide + c) = out;
         }
-        tl_put(y + i, v);
     }
 }
 
-// A warp a row: dz_ij = w_ij dy_i, dw_ij = dy_i . z_ij.
-template <typename T>
+// dz_ij = w_ij dy_i, dw_ij = dy_i . z_ij: `lanes` lanes of a warp (a power of two) a row, N elements each, four choices at a time.
+template <typename T, int N>
 __global__ void __launch_bounds__(EX_THREADS)
 ex_combine_backward_kernel(const T* z, const float* weights, const int32_t* experts, const T* d_y, int64_t d_y_row, T* d_z, float* d_weights, int64_t n,
-                           int choices, int wide)
+                           int choices, int wide, int lanes)
 {
-    const int lane = threadIdx.x % 32;
-    for (int64_t row = (int64_t)blockIdx.x * (EX_THREADS / 32) + threadIdx.x / 32; row < n; row += (int64_t)gridDim.x * (EX_THREADS / 32)) {
-        for (int j = 0; j < choices; j++) {
-            const int64_t p = row * choices + j;
-            const bool live = experts[p] >= 0;
-            const float w = weights[p];
-            float dot = 0.0f;
-            for (int c = lane; c < wide; c += 32) {
-                const float g = tl_get(d_y + row * d_y_row + c);
-                if (live && d_weights != nullptr) dot = fmaf(g, tl_get(z + p * wide + c), dot);
-                if (d_z != nullptr) tl_put(d_z + p * wide + c, live ? w * g : 0.0f);
+    const int in_row = threadIdx.x & (lanes - 1), rows = EX_THREADS / lanes;
+    const int64_t step = (int64_t)gridDim.x * rows, rounds = (n + step - 1) / step;
+    int64_t row = (int64_t)blockIdx.x * rows + threadIdx.x / lanes;
+    for (int64_t round = 0; round < rounds; round++, row += step) {   // all lanes of a warp go as often
+        const bool here = row < n;
+        for (int j0 = 0; j0 < choices; j0 += 4) {
+            float w[4], dot[4] = {};
+            bool real[4], live[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                real[j] = here && j0 + j < choices;
+                live[j] = real[j] && experts[row * choices + j0 + j] >= 0;
+                w[j] = live[j] ? weights[row * choices + j0 + j] : 0.0f;
+            }
+            if (here) {
+                const int64_t from = (row * choices + j0) * wide;
+                for (int c = in_row * N; c < wide; c += lanes * N) {
+                    const ExPack<T, N> g = *reinterpret_cast<const ExPack<T, N>*>(d_y + row * d_y_row + c);
+                    ExPack<T, N> v[4];
+                    if (d_weights != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (live[j]) v[j] = *reinterpret_cast<const ExPack<T, N>*>(z + from + (int64_t)j * wide + c);
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (live[j]) {
+#pragma unroll
+                                for (int i = 0; i < N; i++) dot[j] = fmaf(tl_get(&g.v[i]), tl_get(&v[j].v[i]), dot[j]);
+                            }
+                    }
+                    if (d_z != nullptr) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (real[j]) {
+                                ExPack<T, N> out;
+#pragma unroll
+                                for (int i = 0; i < N; i++) tl_put(&out.v[i], live[j] ? w[j] * tl_get(&g.v[i]) : 0.0f);
+                                *reinterpret_cast<ExPack<T, N>*>(d_z + from + (int64_t)j * wide + c) = out;
+                            }
+                    }
+                }
             }
             if (d_weights == nullptr) continue;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            if (lane == 0) d_weights[p] = dot;
+            for (int j = 0; j < 4; j++) {
+                for (int o = 1; o < lanes; o <<= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+                if (in_row == 0 && real[j]) d_weights[row * choices + j0 + j] = live[j] ? dot[j] : 0.0f;
+            }
         }
     }
+}
+
+// du = dz times the slope, for a gradient of the matrices alone (otherwise the pass of dx leaves it).
+template <typename T>
+__global__ void __launch_bounds__(EX_THREADS)
+ex_slope_kernel(const T* dz, int64_t dz_row, const void* slope, T* du, int64_t n, int wide)
+{
+    for (int64_t p = blockIdx.x; p < n; p += gridDim.x)
+        for (int c = threadIdx.x; c < wide; c += EX_THREADS) {
+            const float s = sizeof(T) == 4 ? static_cast<const float*>(slope)[p * wide + c] : ex_slope_of(static_cast<const uint16_t*>(slope)[p * wide + c]);
+            tl_put(du + p * wide + c, tl_get(dz + p * dz_row + c) * s);
+        }
 }
 
 // The stretches of an expert joined: blockIdx.y is the expert.
@@ -81,7 +154,7 @@ ex_join_kernel(const TlArgs a, int64_t stretches)
     __syncthreads();
     const int64_t cells = (int64_t)a.inner * a.outer, all = cells + a.outer, first = first_of;
     const int64_t count = min(count_of, max(stretches - first, (int64_t)0));
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {   // a few elements a thread: the start of a block is long
         double exact = 0.0;
 #pragma unroll 8
         for (int64_t c = 0; c < count; c++) exact += (double)a.partial[(first + c) * all + i];
@@ -116,7 +189,7 @@ static int ex_args(const dynb_expert_linear_args* in, ExArgs* e)
     a.types = in->experts;
     a.inner = in->inner;
     a.outer = in->outer;
-    a.stretch = tl_stretch(a.n, in->inner, in->outer, in->dtype);
+    a.stretch = ex_stretch(a.n, in->inner, in->outer, in->dtype);
     a.status = in->status_dev;
     e->n_in = in->paired ? a.n : in->n_rows;
     e->fan = in->paired ? 1 : in->choices;
@@ -124,12 +197,36 @@ static int ex_args(const dynb_expert_linear_args* in, ExArgs* e)
     return DYNB_OK;
 }
 
-// Workspace of the backward pass: the matrices as the kernel reads them, the gradients of x by pairs, the sums of stretches.
-struct ExLayout { int64_t by_pair, partial, total; };
+// Pieces of `bytes` may be read and written at p and everywhere `row` elements on.
+static bool ex_on(const void* p, int64_t row, int size, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 && row * size % bytes == 0; }
+// Threads of a row whose pieces are `pieces`, at most `most`.
+static int ex_lanes(int pieces, int most)
+{
+    int lanes = 1;
+    while (lanes < pieces && lanes < most) lanes *= 2;
+    return lanes;
+}
+
+template <typename Z, typename T>
+static cudaError_t ex_combine(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide, cudaStream_t s)
+{
+    constexpr int N = 16 / (int)sizeof(Z);
+    const bool pieces = wide % N == 0 && ex_on(z, 0, 1, 16) && ex_on(y, 0, 1, sizeof(T) * N) && (residual == nullptr || ex_on(residual, residual_row, sizeof(T), sizeof(T) * N));
+    const int lanes = ex_lanes(pieces ? wide / N : wide, EX_THREADS);
+    const unsigned grid = ex_grid(n * lanes);
+    if (pieces) ex_combine_kernel<Z, T, N><<<grid, EX_THREADS, 0, s>>>(z, weights, experts, residual, residual_row, y, n, choices, wide, lanes);
+    else ex_combine_kernel<Z, T, 1><<<grid, EX_THREADS, 0, s>>>(z, weights, experts, residual, residual_row, y, n, choices, wide, lanes);
+    return cudaGetLastError();
+}
+
+// Workspace of the backward pass: the matrices as the kernel reads them, du, the gradients of x by pairs, the sums of stretches.
+struct ExLayout { int64_t du, by_pair, partial, total; };
 static ExLayout ex_layout(const ExArgs& e, int dtype, bool dx, bool weights)
 {
+    const int size = dtype == DYNB_F32 ? 4 : 2;
     ExLayout l;
-    l.by_pair = align_up(dx ? ex_packed_bytes(e, 1, dtype) : 0, 256);
+    l.du = align_up(dx ? ex_packed_bytes(e, 1, dtype) : 0, 256);
+    l.by_pair = l.du + align_up(weights && e.activation != DYNB_ACTIVATION_NONE ? e.t.n * e.t.outer * size : 0, 256);
     l.partial = l.by_pair + align_up(dx && e.fan > 1 ? e.t.n * e.t.inner * 4 : 0, 256);
     l.total = l.partial + align_up(weights ? ex_stretches(e) * ((int64_t)e.t.inner * e.t.outer + e.t.outer) * 4 : 0, 256);
     return l;
@@ -139,19 +236,21 @@ template <typename T>
 static int ex_backward(ExArgs& e, int dtype, const int32_t* experts, void* d_x, unsigned char* ws, const ExLayout& l, cudaStream_t s)
 {
     TlArgs& a = e.t;
+    const bool weights = a.dw != nullptr || a.db != nullptr;
+    if (weights && e.activation != DYNB_ACTIVATION_NONE) e.du = ws + l.du;
     if (d_x != nullptr && a.n > 0) {
         a.dx = e.fan > 1 ? ws + l.by_pair : static_cast<unsigned char*>(d_x);
         DYNB_CUDA_OK(ex_mma_rows(e, 1, dtype, ws, s));
-        if (e.fan > 1) {
-            ex_combine_kernel<float, T><<<ex_grid(e.n_in * a.inner), EX_THREADS, 0, s>>>(reinterpret_cast<const float*>(ws + l.by_pair), nullptr, experts, static_cast<const T*>(nullptr), 0,
-                                                                                     static_cast<T*>(d_x), e.n_in, e.fan, a.inner);
-            DYNB_CUDA_OK(cudaGetLastError());
-        }
+        if (e.fan > 1) DYNB_CUDA_OK((ex_combine<float, T>(reinterpret_cast<const float*>(ws + l.by_pair), nullptr, experts, nullptr, 0, static_cast<T*>(d_x), e.n_in, e.fan, a.inner, s)));
+    } else if (e.du != nullptr && a.n > 0) {
+        ex_slope_kernel<T><<<(unsigned)std::min<int64_t>(a.n, (int64_t)sm_count_cached() * 8), EX_THREADS, 0, s>>>(static_cast<const T*>(a.dy), a.dy_row, e.slope, static_cast<T*>(e.du), a.n, a.outer);
+        DYNB_CUDA_OK(cudaGetLastError());
     }
-    if (a.dw != nullptr || a.db != nullptr) {
+    if (weights) {
+        if (e.du != nullptr) { a.dy = e.du; a.dy_row = a.outer; }
         DYNB_CUDA_OK(ex_mma_weights(e, dtype, s));
         const int64_t all = (int64_t)a.inner * a.outer + a.outer;
-        ex_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((all + EX_THREADS - 1) / EX_THREADS, 1024), a.types), EX_THREADS, 0, s>>>(a, ex_stretches(e));
+        ex_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((all + 4 * EX_THREADS - 1) / (4 * EX_THREADS), 1024), a.types), EX_THREADS, 0, s>>>(a, ex_stretches(e));
         DYNB_CUDA_OK(cudaGetLastError());
     }
     return DYNB_OK;
@@ -170,16 +269,22 @@ template <typename T>
 static cudaError_t ec_forward(const void* z, const float* weights, const int32_t* experts, const void* residual, int64_t residual_row, void* y, int64_t n, int choices,
                               int wide, cudaStream_t s)
 {
-    ex_combine_kernel<T, T><<<ex_grid(n * wide), EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(residual), residual_row, static_cast<T*>(y), n,
-                                                                  choices, wide);
-    return cudaGetLastError();
+    return ex_combine<T, T>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(residual), residual_row, static_cast<T*>(y), n, choices, wide, s);
 }
 template <typename T>
 static cudaError_t ec_backward(const void* z, const float* weights, const int32_t* experts, const void* d_y, int64_t d_y_row, void* d_z, float* d_weights, int64_t n,
                                int choices, int wide, cudaStream_t s)
 {
-    ex_combine_backward_kernel<T><<<ex_grid(n * 32), EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(d_y), d_y_row, static_cast<T*>(d_z), d_weights,
-                                                                       n, choices, wide);
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool pieces = wide % N == 0 && ex_on(z, 0, 1, 16) && ex_on(d_z, 0, 1, 16) && ex_on(d_y, d_y_row, sizeof(T), 16);
+    const int lanes = ex_lanes(pieces ? wide / N : wide, 32);
+    const unsigned grid = ex_grid(n * lanes);
+    if (pieces)
+        ex_combine_backward_kernel<T, N><<<grid, EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(d_y), d_y_row, static_cast<T*>(d_z), d_weights, n,
+                                                                    choices, wide, lanes);
+    else
+        ex_combine_backward_kernel<T, 1><<<grid, EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(d_y), d_y_row, static_cast<T*>(d_z), d_weights, n,
+                                                                    choices, wide, lanes);
     return cudaGetLastError();
 }
 

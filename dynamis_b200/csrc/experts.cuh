@@ -9,6 +9,7 @@ namespace dynb {
 struct ExArgs {
     TlArgs t;                  // x, w, b, dy, order, start; n: pairs; y: result, dx: gradient of x by pairs
     void* slope;               // the activation's slope, [pairs, outer], or null
+    void* du;                  // room for dz times the slope, [pairs, outer], or null
     int64_t n_in;              // rows of x
     int fan, activation;
 };
@@ -40,22 +41,38 @@ __device__ __forceinline__ float ex_activate(float u, int activation, float* slo
     return u;
 }
 
-// Rows of places without an expert are set to zero, `wide` bytes a row, by `threads` threads of every block of row `blockIdx.y` 0.
-__device__ __forceinline__ void ex_clear_absent(const TlArgs& a, void* out, int64_t wide, int thread, int threads)
+// Rows of places without an expert are set to zero, `wide` bytes a row (16: whole pieces of 16 bytes), by warp `warp` of `warps`: it looks at 32 places at a time.
+__device__ __forceinline__ void ex_clear_absent(const TlArgs& a, void* out, int64_t wide, int piece, int64_t warp, int64_t warps)
 {
-    const int64_t from = min(max((int64_t)a.start[a.types], (int64_t)0), a.n);
-    for (int64_t at = from + blockIdx.x; at < a.n; at += gridDim.x) {
-        const int32_t p = a.order[at];
-        if ((uint32_t)p >= (uint64_t)a.n) continue;
-        uint16_t* const row = reinterpret_cast<uint16_t*>(static_cast<unsigned char*>(out) + p * wide);
-        for (int64_t i = thread; i < wide / 2; i += threads) row[i] = 0;
+    const int lane = threadIdx.x & 31;
+    for (int64_t at = min(max((int64_t)a.start[a.types], (int64_t)0), a.n) + 32 * warp; at < a.n; at += 32 * warps) {
+        const int32_t mine = at + lane < a.n ? a.order[at + lane] : -1;
+        for (int i = 0; i < 32; i++) {
+            const int32_t p = __shfl_sync(0xffffffffu, mine, i);
+            if ((uint32_t)p >= (uint64_t)a.n) continue;
+            unsigned char* const row = static_cast<unsigned char*>(out) + p * wide;
+            if (piece == 16) {
+                for (int64_t c = 16 * lane; c < wide; c += 512) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+            } else {
+                for (int64_t c = 2 * lane; c < wide; c += 64) *reinterpret_cast<uint16_t*>(row + c) = 0;
+            }
+        }
     }
 }
 
 // experts_mma.cu: the products on the tensor cores.  `packed`: room for the matrices as the kernel reads them, on 16 bytes.
 int64_t ex_packed_bytes(const ExArgs& e, int back, int dtype);
-cudaError_t ex_mma_rows(const ExArgs& e, int back, int dtype, void* packed, cudaStream_t s);
+cudaError_t ex_mma_rows(const ExArgs& e, int back, int dtype, void* packed, cudaStream_t s);   // back: du goes to e.du as well, where it is not null
 cudaError_t ex_mma_weights(const ExArgs& e, int dtype, cudaStream_t s);
 int64_t ex_stretches(const ExArgs& e);
+
+// Pairs of an expert whose products one block sums: four blocks an SM where there are as many pairs, no fewer than 256.  In fp32 as in tl_stretch (a sum in tensor
+// memory is one chain of additions that are cut off); results of 16 bits do not see that, and longer stretches leave fewer sums to write and join.
+static inline int ex_stretch(int64_t n, int inner, int outer, int dtype)
+{
+    if (dtype == DYNB_F32) return tl_stretch(n, inner, outer, dtype);
+    const int64_t tiles = (int64_t)((inner + 127) / 128) * ((outer + 255) / 256);
+    return (int)((std::min<int64_t>(8192, std::max<int64_t>(256, n * tiles / (148 * 4) + 1)) + 31) / 32 * 32);
+}
 
 }  // namespace dynb

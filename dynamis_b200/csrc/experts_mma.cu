@@ -16,16 +16,19 @@
 
 namespace dynb {
 
-constexpr int EM_FEED = 8, EM_OUT = 8;                               // warps that gather, and that store results
-constexpr int EM_THREADS = (EM_OUT + 2 + EM_FEED) * 32;
+// Warps that gather, and that store results.  An SM's four schedulers have room for five warps of 96 registers each, or four of 128: rows in fp32 wait in the registers of
+// their threads and need the latter.
+constexpr int EM_FEED = 8;
+template <typename T> constexpr int EM_OUT = sizeof(T) == 4 ? 4 : 8;
+template <typename T> constexpr int EM_THREADS = (EM_OUT<T> + 2 + EM_FEED) * 32;
 constexpr int EM_MAX_STAGES = 8;
 constexpr int EM_SMEM = 204 * 1024;                                  // beside 20 KB of results under way and offsets
 constexpr int EM_DEPTH = 3;                                          // stages whose copies a gathering warp leaves under way
 
-enum EmPath { EM_ASYNC, EM_REGISTERS, EM_SLOPE };
+enum EmPath { EM_ASYNC, EM_REGISTERS, EM_SLOPE, EM_ASYNC_SLOPE };
 
 struct EmPlan {
-    int back, columns, column_stride, chunks, stages, depth, tensor_columns, resident, b_bytes, stage_bytes, store, slope_store;   // b_bytes: matrix of one stage
+    int back, columns, column_stride, chunks, stages, depth, tensor_columns, resident, b_bytes, stage_bytes, slope_at, store, slope_store;   // b_bytes: matrix of one stage; slope_at: slopes behind its rows
     const unsigned char* packed;
 };
 
@@ -111,6 +114,21 @@ __device__ __forceinline__ void em_times(TmRaw<T>& v, const TmRaw<T>& slope)
     }
 }
 
+// Eight elements, the first `have` of them real, back to memory.
+template <bool WIDE, typename T>
+__device__ __forceinline__ void em_keep(const TmRaw<T>& v, T* to, int have)
+{
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(v) / 16); i++) reinterpret_cast<uint4*>(to)[i] = v.v[i];
+    } else {
+        const T* const from = reinterpret_cast<const T*>(&v);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < have) to[i] = from[i];
+    }
+}
+
 // 64 bytes of each of a warp's 32 rows, lane l's from row l, to memory by pieces of 16 bytes (or elements of `size`) that lie side by side.  `mine`: 2 KB of
 // the warp, its pieces swizzled.  `row`: number of the lane's row, or -1; `bytes`: how many of the 64 there are.
 __device__ __forceinline__ void em_put(unsigned char* mine, const uint32_t* words, int lane, int32_t row, unsigned char* out, int64_t row_bytes, int bytes, int store, int size)
@@ -146,15 +164,16 @@ __device__ __forceinline__ void em_put(unsigned char* mine, const uint32_t* word
 
 // O: type of the results (fp32 for gradients that are summed over the choices before they are rounded).
 template <typename T, typename O, EmPath PATH, bool WIDE>
-__global__ void __launch_bounds__(EM_THREADS, 1)
+__global__ void __launch_bounds__(EM_THREADS<T>, 1)
 em_rows_kernel(const ExArgs e, const EmPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O);
+    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = 64 / SIZE;   // columns of 64 bytes of results
+    constexpr int OUT = EM_OUT<T>, SHARES = OUT / 4;
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EmBars bars;
-    __shared__ __align__(16) float offsets[EM_OUT][128];
-    __shared__ __align__(16) unsigned char turned[EM_OUT][2048];
+    __shared__ __align__(16) float offsets[OUT][256 / SHARES];
+    __shared__ __align__(16) unsigned char turned[OUT][2048];
     unsigned char* const panel = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
     unsigned char* const stage0 = panel + (plan.resident ? plan.chunks * plan.b_bytes : 0);
     const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -171,7 +190,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         bar_init(&bars.panel_free, 1);
         for (int b = 0; b < 2; b++) {
             bar_init(&bars.sums_full[b], 1);
-            bar_init(&bars.sums_free[b], EM_OUT);
+            bar_init(&bars.sums_free[b], OUT);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -187,14 +206,14 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
     TmCursor cursor;
     cursor.start(a, first, min(per, pieces - first));
 
-    if (warp < EM_OUT) {
-        // sums to results: warps w and w + 4 share the rows 32 (w % 4) on, and take the groups of 32 columns in turn
+    if (warp < OUT) {
+        // sums to results: the warps of the rows 32 (warp % 4) on take the groups of columns in turn
         unsigned char* const out = static_cast<unsigned char*>(plan.back ? a.dx : a.y);
-        const int have = min(plan.columns, nn - col0), half = warp >> 2;
+        const int have = min(plan.columns, nn - col0), share = warp >> 2;
         const bool with_offset = !plan.back && a.b != nullptr;
         const int activation = plan.back ? DYNB_ACTIVATION_NONE : e.activation;
         const bool with_slope = activation != DYNB_ACTIVATION_NONE && e.slope != nullptr;
-        if (blockIdx.y == 0) ex_clear_absent(a, out, (int64_t)nn * SIZE, threadIdx.x, EM_OUT * 32);
+        ex_clear_absent(a, out, (int64_t)nn * SIZE, plan.store, ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OUT + warp, (int64_t)gridDim.x * gridDim.y * OUT);
         float* const offset = offsets[warp];
         int buffer = 0, offset_type = -1;
         uint32_t phase = 0;
@@ -204,41 +223,43 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             if (with_offset && cursor.tile.type != offset_type) {
                 offset_type = cursor.tile.type;
                 __syncwarp();
-                for (int c = half * 32; c < have; c += 64)
-                    offset[c / 64 * 32 + lane] = c + lane < have ? tl_get(static_cast<const T*>(a.b) + (int64_t)offset_type * a.outer + col0 + c + lane) : 0.0f;
+                for (int i = lane; i < (have + SHARES * COLUMNS - 1) / (SHARES * COLUMNS) * COLUMNS; i += 32) {   // of this warp's columns, one group behind the other
+                    const int c = i / COLUMNS * SHARES * COLUMNS + share * COLUMNS + i % COLUMNS;
+                    offset[i] = c < have ? tl_get(static_cast<const T*>(a.b) + (int64_t)offset_type * a.outer + col0 + c) : 0.0f;
+                }
                 __syncwarp();
             }
             if (!bar_wait(&bars.sums_full[buffer], phase)) { tm_ran_out(a); break; }
             tensor_fence_after();
             if ((uint32_t)r >= (uint64_t)a.n) r = -1;
             const uint32_t from = tensor + ((uint32_t)((warp & 3) * 32) << 16) + buffer * plan.column_stride;
-            for (int c = half * 32; c < have; c += 64) {
-                uint32_t bits[32];
+            for (int c = share * COLUMNS; c < have; c += SHARES * COLUMNS) {
+                uint32_t bits[COLUMNS];
                 __syncwarp();
-                tensor_load_32(from + c, bits);
+                tensor_load(from + c, bits);
                 if constexpr (PARTS > 1) {   // the small products' sums
-                    uint32_t small[32];
-                    tensor_load_32(from + 2 * plan.column_stride + c, small);
+                    uint32_t small[COLUMNS];
+                    tensor_load(from + 2 * plan.column_stride + c, small);
                     tensor_wait_loads();
 #pragma unroll
-                    for (int i = 0; i < 32; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
+                    for (int i = 0; i < COLUMNS; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
                 } else {
                     tensor_wait_loads();
                 }
                 if (with_offset) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 o = *reinterpret_cast<const float4*>(offset + c / 64 * 32 + i);
+                    for (int i = 0; i < COLUMNS; i += 4) {
+                        const float4 o = *reinterpret_cast<const float4*>(offset + c / (SHARES * COLUMNS) * COLUMNS + i);
                         bits[i] = __float_as_uint(__uint_as_float(bits[i]) + o.x);
                         bits[i + 1] = __float_as_uint(__uint_as_float(bits[i + 1]) + o.y);
                         bits[i + 2] = __float_as_uint(__uint_as_float(bits[i + 2]) + o.z);
                         bits[i + 3] = __float_as_uint(__uint_as_float(bits[i + 3]) + o.w);
                     }
                 }
-                uint32_t slopes[sizeof(T) == 4 ? 32 : 16];
+                uint32_t words[16], slopes[16];
                 if (activation != DYNB_ACTIVATION_NONE) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
+                    for (int i = 0; i < COLUMNS; i += 2) {
                         float s0, s1;
                         const float v0 = ex_activate(__uint_as_float(bits[i]), activation, &s0), v1 = ex_activate(__uint_as_float(bits[i + 1]), activation, &s1);
                         bits[i] = __float_as_uint(v0);
@@ -246,35 +267,18 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                         if constexpr (sizeof(T) == 4) {
                             slopes[i] = __float_as_uint(s0);
                             slopes[i + 1] = __float_as_uint(s1);
-                        } else {
+                        } else if constexpr (COLUMNS == 32) {
                             slopes[i / 2] = __byte_perm(ex_slope_bits(s0), ex_slope_bits(s1), 0x5410);
                         }
                     }
                 }
-                unsigned char* const mine = turned[warp];
-                const int64_t row_bytes = (int64_t)nn * SIZE;
-                unsigned char* const at = out + (int64_t)(col0 + c) * SIZE;
-                const int bytes = (have - c) * SIZE;
-                if constexpr (SIZE == 4) {
-                    em_put(mine, bits, lane, r, at, row_bytes, bytes, plan.store, 4);
-                    if (bytes > 64) em_put(mine, bits + 16, lane, r, at + 64, row_bytes, bytes - 64, plan.store, 4);
-                } else {
-                    uint32_t words[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float v[4] = {__uint_as_float(bits[i]), __uint_as_float(bits[i + 1]), __uint_as_float(bits[i + 2]), __uint_as_float(bits[i + 3])};
-                        tm_words<O>(v, words + i / 2);
-                    }
-                    em_put(mine, words, lane, r, at, row_bytes, bytes, plan.store, 2);
+                for (int i = 0; i < COLUMNS; i += 4) {
+                    const float v[4] = {__uint_as_float(bits[i]), __uint_as_float(bits[i + 1]), __uint_as_float(bits[i + 2]), __uint_as_float(bits[i + 3])};
+                    tm_words<O>(v, words + i * SIZE / 4);
                 }
-                if (with_slope) {
-                    constexpr int S = sizeof(T) == 4 ? 4 : 2;
-                    unsigned char* const to = static_cast<unsigned char*>(e.slope) + (int64_t)(col0 + c) * S;
-                    em_put(mine, slopes, lane, r, to, (int64_t)nn * S, (have - c) * S, plan.slope_store, S);
-                    if constexpr (S == 4) {
-                        if (have - c > 16) em_put(mine, slopes + 16, lane, r, to + 64, (int64_t)nn * S, (have - c - 16) * S, plan.slope_store, S);
-                    }
-                }
+                em_put(turned[warp], words, lane, r, out + (int64_t)(col0 + c) * SIZE, (int64_t)nn * SIZE, (have - c) * SIZE, plan.store, SIZE);
+                if (with_slope) em_put(turned[warp], slopes, lane, r, static_cast<unsigned char*>(e.slope) + (int64_t)(col0 + c) * SIZE, (int64_t)nn * SIZE, (have - c) * SIZE, plan.slope_store, SIZE);
             }
             tensor_fence_before();
             __syncwarp();
@@ -282,7 +286,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             buffer ^= 1;
             if (buffer == 0) phase ^= 1;
         }
-    } else if (warp == EM_OUT) {
+    } else if (warp == OUT) {
         // products
         const bool bf16 = !std::is_same<T, __half>::value;
         const uint32_t what = mma_what(bf16, plan.columns, false, false);
@@ -325,7 +329,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             if (buffer == 0) sums_phase ^= 1;
         }
         if (!ok) tm_ran_out(a);
-    } else if (warp == EM_OUT + 1) {
+    } else if (warp == OUT + 1) {
         // matrices
         const int64_t tiles = gridDim.y;
         if (plan.resident) {
@@ -375,7 +379,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         const int fan = plan.back ? 1 : e.fan;
         const uint32_t rows_in = (uint32_t)(plan.back ? a.n : e.n_in);
         constexpr int UNITS = TM_ROWS * 8 / (EM_FEED * 32);
-        const int tid = threadIdx.x - (EM_OUT + 2) * 32, piece = tid & 7;
+        const int tid = threadIdx.x - (OUT + 2) * 32, piece = tid & 7;
         int32_t rows[UNITS], rows_next[UNITS];      // of the next tile to ask for, and the one behind it
         auto rows_of = [&](const TlTile& t, int32_t (&r)[UNITS]) {
 #pragma unroll
@@ -388,12 +392,36 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         auto row_in = [&](int32_t p) { return (uint32_t)p >= (uint64_t)a.n ? 0xffffffffu : fan == 1 ? (uint32_t)p : (uint32_t)p / (uint32_t)fan; };
         int stage = 0;
         uint32_t phase = 1;
-        if constexpr (PATH == EM_ASYNC) {
+        if constexpr (PATH == EM_ASYNC || PATH == EM_ASYNC_SLOPE) {
+            constexpr bool SLOPE = PATH == EM_ASYNC_SLOPE;
             int arrived = 0;                        // stage of the next arrival
             int64_t asked = 0;
             rows_of(cursor.tile, rows);
             bool ok = true;
+            const bool keep_du = SLOPE && e.du != nullptr && blockIdx.y == 0;
+            TmCursor behind = cursor;               // of the next arrival, for du
+            int behind_chunk = 0;
+            int32_t behind_rows[UNITS];
+            if (keep_du) rows_of(behind.tile, behind_rows);
             auto arrive = [&] {
+                if constexpr (SLOPE) {   // each thread multiplies what it has copied itself
+                    unsigned char* const at = stage0 + arrived * plan.stage_bytes + tile_piece(tid >> 3, piece);
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) {
+                        TmRaw<T> v, slope;
+                        v.v[0] = *reinterpret_cast<const uint4*>(at + i * EM_FEED * 512);
+                        slope.v[0] = *reinterpret_cast<const uint4*>(at + i * EM_FEED * 512 + plan.slope_at);
+                        em_times(v, slope);
+                        *reinterpret_cast<uint4*>(at + i * EM_FEED * 512) = v.v[0];
+                        const int k = behind_chunk * 64 + piece * 8;
+                        if (keep_du && (uint32_t)behind_rows[i] < rows_in && k < kk) *reinterpret_cast<uint4*>(static_cast<T*>(e.du) + (int64_t)behind_rows[i] * kk + k) = v.v[0];
+                    }
+                    if (keep_du && ++behind_chunk == plan.chunks) {
+                        behind_chunk = 0;
+                        behind.next(a);
+                        rows_of(behind.tile, behind_rows);
+                    }
+                }
                 fence_to_tensor();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bars.full[arrived]);
@@ -413,6 +441,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     for (int i = 0; i < UNITS; i++) {
                         const bool live = at[i] < rows_in && k < kk;
                         copy_16(to + i * EM_FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
+                        if constexpr (SLOPE) copy_16(to + i * EM_FEED * 512 + plan.slope_at, static_cast<const T*>(e.slope) + (live ? (int64_t)at[i] * kk + k : 0), live);
                     }
                     copies_commit();
                     if (++stage == plan.stages) { stage = 0; phase ^= 1; }
@@ -434,14 +463,19 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             int chunk = 0;
             TmRaw<T> v[AHEAD][UNITS], slope[AHEAD][SLOPES];
             bool live[AHEAD];
-            auto ask = [&](TmRaw<T> (&to)[UNITS], TmRaw<T> (&to_slope)[SLOPES], bool& any) {
+            uint32_t row_du[AHEAD][SLOPES];         // pair whose du is kept, or a number that is none; its first column
+            int k_du[AHEAD];
+            const bool keep_du = PATH == EM_SLOPE && e.du != nullptr && blockIdx.y == 0;
+            auto ask = [&](TmRaw<T> (&to)[UNITS], TmRaw<T> (&to_slope)[SLOPES], uint32_t (&to_du)[SLOPES], int& to_k, bool& any) {
                 any = next.type >= 0;
                 if (!any) return;
                 const int k = chunk * 64 + piece * 8, have = min(8, kk - k);
+                to_k = k;
 #pragma unroll
                 for (int i = 0; i < UNITS; i++) {
                     const uint32_t at = row_in(rows[i]);
                     const bool ok = at < rows_in;
+                    if constexpr (PATH == EM_SLOPE) to_du[i] = keep_du && have > 0 ? at : 0xffffffffu;
                     to[i] = tm_load<WIDE>(in + (ok ? at * in_row + k : 0), 1, ok ? have : 0);
                     if constexpr (PATH == EM_SLOPE) to_slope[i] = tm_load<WIDE>(static_cast<const T*>(e.slope) + (ok ? (int64_t)at * kk + k : 0), 1, ok ? have : 0);
                 }
@@ -460,7 +494,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             if (next.type >= 0) cursor.next(a);
             rows_of(cursor.tile, rows_next);
 #pragma unroll
-            for (int s = 0; s < AHEAD; s++) ask(v[s], slope[s], live[s]);
+            for (int s = 0; s < AHEAD; s++) ask(v[s], slope[s], row_du[s], k_du[s], live[s]);
             bool more = true;
             while (more) {
 #pragma unroll
@@ -468,7 +502,10 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     if (!live[s]) { more = false; break; }
                     if constexpr (PATH == EM_SLOPE) {
 #pragma unroll
-                        for (int i = 0; i < UNITS; i++) em_times(v[s][i], slope[s][i]);
+                        for (int i = 0; i < UNITS; i++) {
+                            em_times(v[s][i], slope[s][i]);
+                            if (row_du[s][i] < rows_in) em_keep<WIDE>(v[s][i], static_cast<T*>(e.du) + (int64_t)row_du[s][i] * kk + k_du[s], kk - k_du[s]);
+                        }
                     }
                     if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
                     unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
@@ -483,7 +520,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     __syncwarp();
                     if (lane == 0) bar_arrive(&bars.full[stage]);
                     if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                    ask(v[s], slope[s], live[s]);
+                    ask(v[s], slope[s], row_du[s], k_du[s], live[s]);
                 }
             }
         }
@@ -679,18 +716,13 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             }
             copies_wait(0);
         } else {
-            constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
-            TmRaw<T> v[UNITS], slope[SLOPES];
+            TmRaw<T> v[UNITS];
             auto fetch = [&](const int32_t (&r)[UNITS]) {
 #pragma unroll
                 for (int i = 0; i < UNITS; i++) {
                     const bool of_y = (col[i] >> 30) & 1, ok = (uint32_t)r[i] < (uint64_t)a.n;
                     const int c = col[i] & ((1 << 30) - 1), have = ok ? min(8, (of_y ? a.outer : a.inner) - c) : 0;
                     v[i] = tm_load<WIDE>(ok ? address(i, r[i]) : static_cast<const T*>(a.x), 1, have);
-                    if constexpr (PATH == EM_SLOPE) {
-                        const bool with = ok && of_y;
-                        slope[i] = tm_load<WIDE>(static_cast<const T*>(e.slope) + (with ? (int64_t)r[i] * a.outer + c : 0), 1, with ? have : 0);
-                    }
                 }
             };
             // the rows of the next stage are asked for behind this one, their numbers a stage earlier
@@ -698,11 +730,6 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             fetch(ids);
             rows_of(1, ids);
             for (int step = 0; step < steps; step++) {
-                if constexpr (PATH == EM_SLOPE) {
-#pragma unroll
-                    for (int i = 0; i < UNITS; i++)
-                        if ((col[i] >> 30) & 1) em_times(v[i], slope[i]);
-                }
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
                 if (tm_odd(v)) {
 #pragma unroll
@@ -730,7 +757,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
 
 // ------------------------------------------------------------------------------------------------ host
 template <typename T>
-static EmPlan em_plan(const ExArgs& e, int back, int* tiles)
+static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // slopes: they are copied beside the rows
 {
     constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, MOST = PARTS == 1 ? 256 : 128;
     const int kk = back ? e.t.outer : e.t.inner, nn = back ? e.t.inner : e.t.outer;
@@ -743,8 +770,10 @@ static EmPlan em_plan(const ExArgs& e, int back, int* tiles)
     p.column_stride = tm_round(p.columns, 32);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     p.b_bytes = PARTS * p.columns * 128;
-    p.resident = (int64_t)p.chunks * p.b_bytes + (PARTS == 1 ? 4 : 2) * A_BYTES + 1024 <= EM_SMEM;
-    p.stage_bytes = A_BYTES + (p.resident ? 0 : p.b_bytes);
+    const int rows_bytes = A_BYTES * (slopes ? 2 : 1);
+    p.resident = (int64_t)p.chunks * p.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * rows_bytes + 1024 <= EM_SMEM;
+    p.slope_at = A_BYTES + (p.resident ? 0 : p.b_bytes);
+    p.stage_bytes = rows_bytes + (p.resident ? 0 : p.b_bytes);
     p.stages = std::min(EM_MAX_STAGES, (EM_SMEM - 1024 - (p.resident ? p.chunks * p.b_bytes : 0)) / p.stage_bytes);
     p.depth = std::min(EM_DEPTH, p.stages - 1);
     return p;
@@ -754,7 +783,7 @@ template <typename T>
 static int64_t em_packed(const ExArgs& e, int back)
 {
     int tiles;
-    const EmPlan p = em_plan<T>(e, back, &tiles);
+    const EmPlan p = em_plan<T>(e, back, false, &tiles);
     return (int64_t)e.t.types * tiles * p.chunks * p.b_bytes;
 }
 
@@ -765,14 +794,14 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
 {
     constexpr int SIZE = (int)sizeof(T);
     const TlArgs& a = e.t;
-    int tiles;
-    EmPlan p = em_plan<T>(e, back, &tiles);
-    p.packed = static_cast<const unsigned char*>(packed);
     const int kk = back ? a.outer : a.inner, nn = back ? a.inner : a.outer;
     const void* const in = back ? a.dy : a.x;
     const void* const out = back ? a.dx : a.y;
     const bool slope = back && e.activation != DYNB_ACTIVATION_NONE;
-    const bool wide = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0 && (!slope || tm_on(e.slope, kk, SIZE, 16));
+    const bool wide = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0 && (!slope || (tm_on(e.slope, kk, SIZE, 16) && tm_on(e.du, kk, SIZE, 16)));
+    int tiles;
+    EmPlan p = em_plan<T>(e, back, SIZE == 2 && slope && wide, &tiles);
+    p.packed = static_cast<const unsigned char*>(packed);
     p.store = tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
     p.slope_store = e.slope != nullptr && tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
     const int64_t units = (int64_t)a.types * tiles * p.chunks * p.columns * 8;
@@ -781,7 +810,8 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     cudaError_t rc = cudaGetLastError();
     if (rc != cudaSuccess) return rc;
     void (*kernel)(ExArgs, EmPlan);
-    if (slope) kernel = wide ? em_rows_kernel<T, O, EM_SLOPE, true> : em_rows_kernel<T, O, EM_SLOPE, false>;
+    if (slope && !wide) kernel = em_rows_kernel<T, O, EM_SLOPE, false>;
+    else if (slope) kernel = em_rows_kernel<T, O, SIZE == 4 ? EM_SLOPE : EM_ASYNC_SLOPE, true>;
     else if (!wide) kernel = em_rows_kernel<T, O, EM_REGISTERS, false>;
     else if constexpr (SIZE == 4) kernel = em_rows_kernel<T, O, EM_REGISTERS, true>;
     else kernel = em_rows_kernel<T, O, EM_ASYNC, true>;
@@ -790,7 +820,7 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     const int smem = 1024 + (p.resident ? p.chunks * p.b_bytes : 0) + p.stages * p.stage_bytes;
     rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    kernel<<<grid, EM_THREADS, smem, s>>>(e, p);
+    kernel<<<grid, EM_THREADS<T>, smem, s>>>(e, p);
     return cudaGetLastError();
 }
 
@@ -829,12 +859,10 @@ static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
     p.stages = std::min(EW_MAX_STAGES, (EW_SMEM - 1024 - TM_ROWS * 128) / stage);
     p.depth = std::min(EM_DEPTH, p.stages - 1);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
-    const bool slope = e.activation != DYNB_ACTIVATION_NONE;
-    const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0 && (!slope || tm_on(e.slope, 0, SIZE, 16));
+    const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
     p.vec = a.outer % 4 == 0 && tm_on(a.partial, 0, 4, 16);
     void (*kernel)(ExArgs, EwPlan);
-    if (slope) kernel = wide ? em_weights_kernel<T, EM_SLOPE, true> : em_weights_kernel<T, EM_SLOPE, false>;
-    else if (!wide) kernel = em_weights_kernel<T, EM_REGISTERS, false>;
+    if (!wide) kernel = em_weights_kernel<T, EM_REGISTERS, false>;
     else if constexpr (SIZE == 4) kernel = em_weights_kernel<T, EM_REGISTERS, true>;
     else kernel = em_weights_kernel<T, EM_ASYNC, true>;
     const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;

@@ -88,6 +88,16 @@ __device__ __forceinline__ void tensor_load_32(uint32_t at, uint32_t (&v)[32])
           "=r"(v[31])
         : "r"(at));
 }
+// 16 columns.
+__device__ __forceinline__ void tensor_load_16(uint32_t at, uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+                   "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tensor_load(uint32_t at, uint32_t (&v)[32]) { tensor_load_32(at, v); }
+__device__ __forceinline__ void tensor_load(uint32_t at, uint32_t (&v)[16]) { tensor_load_16(at, v); }
 __device__ __forceinline__ void tensor_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // d (+)= a b: 128 rows, `n` columns from the descriptor of the instruction, 16 summed elements.  One thread issues it.

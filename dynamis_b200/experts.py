@@ -123,6 +123,7 @@ class _RouteExperts(torch.autograd.Function):
             _lib.check(L.dynb_route_experts(ctypes.byref(args), chosen.data_ptr(), weights.data_ptr(), order.data_ptr(), start.data_ptr(), ws.data_ptr(),
                                             ws.numel(), _lib.stream_of(dev)), "route_experts")
         ctx.mark_non_differentiable(chosen, order, start)
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, chosen, weights)
         ctx.fixed = fixed
         return chosen, weights, order, start
@@ -130,6 +131,8 @@ class _RouteExperts(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, _, d_weights, *__):
+        if d_weights is None:
+            return (None,) * 8
         logits, chosen, weights = ctx.saved_tensors
         dev = logits.device
         d_weights = d_weights.contiguous()
