@@ -128,7 +128,7 @@ ex_slope_kernel(const T* dz, int64_t dz_row, const void* slope, T* du, int64_t n
         }
 }
 
-// The stretches of an expert joined: blockIdx.y is the expert.
+// The sums of an expert joined (its pairs are cut at multiples of the stretch): blockIdx.y is the expert.
 template <typename T>
 __global__ void __launch_bounds__(EX_THREADS)
 ex_join_kernel(const TlArgs a, int64_t stretches)
@@ -140,7 +140,7 @@ ex_join_kernel(const TlArgs a, int64_t stretches)
         for (int t = threadIdx.x; t < type; t += 32) {
             int64_t s0, s1;
             tl_rows_of(a, t, &s0, &s1);
-            first += (s1 - s0 + a.stretch - 1) / a.stretch;
+            first += s1 > s0 ? (s1 + a.stretch - 1) / a.stretch - s0 / a.stretch : 0;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(0xffffffffu, first, o);
@@ -148,7 +148,7 @@ ex_join_kernel(const TlArgs a, int64_t stretches)
             int64_t s0, s1;
             tl_rows_of(a, type, &s0, &s1);
             first_of = first;
-            count_of = (s1 - s0 + a.stretch - 1) / a.stretch;
+            count_of = s1 > s0 ? (s1 + a.stretch - 1) / a.stretch - s0 / a.stretch : 0;
         }
     }
     __syncthreads();

@@ -1,6 +1,8 @@
 // What the kernels of the products by expert share.
 #pragma once
 
+#include <algorithm>
+
 #include "type_linear.cuh"
 
 namespace dynb {
@@ -20,25 +22,29 @@ struct ExArgs {
 __device__ __forceinline__ uint32_t ex_slope_bits(float v) { return __float_as_uint(fmaf(v, 16384.0f, 8388608.0f + 8192.0f)); }   // the lower 16
 __device__ __forceinline__ float ex_slope_of(uint32_t bits) { return bits == 0xffffu ? NAN : fmaf(__uint_as_float(0x4b000000u | bits), 1.0f / 16384.0f, -512.5f); }
 
+__device__ __forceinline__ float ex_inverse(float v)   // to within an unit in the last place; 0 of an infinity
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 // The activation and its slope.  Exponentials by the fast route: off by 2 + |u| units in the last place of 1 + e^-u.  The normal distribution function by formula
 // 7.1.26 of Abramowitz and Stegun, off by 7.5e-8, whose exponential the slope shares.
-__device__ __forceinline__ float ex_activate(float u, int activation, float* slope)
+template <int ACTIVATION>
+__device__ __forceinline__ float ex_activate(float u, float* slope)
 {
-    if (activation == DYNB_ACTIVATION_SILU) {
-        const float p = __fdividef(1.0f, 1.0f + __expf(-u));
+    if constexpr (ACTIVATION == DYNB_ACTIVATION_SILU) {
+        const float p = ex_inverse(1.0f + __expf(-u));
         const float z = u * p;
         *slope = fmaf(z, 1.0f - p, p);
         return z;
-    }
-    if (activation == DYNB_ACTIVATION_GELU) {
-        const float x = fabsf(u) * 0.70710678118654752f, t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f)), e = __expf(-x * x);
+    } else {
+        const float x = fabsf(u) * 0.70710678118654752f, t = ex_inverse(fmaf(0.3275911f, x, 1.0f)), e = __expf(-x * x);
         const float tail = 0.5f * e * t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
         const float p = u < 0.0f ? tail : 1.0f - tail;
         *slope = fmaf(u * 0.3989422804014327f, e, p);
         return u * p;
     }
-    *slope = 1.0f;
-    return u;
 }
 
 // Rows of places without an expert are set to zero, `wide` bytes a row (16: whole pieces of 16 bytes), by warp `warp` of `warps`: it looks at 32 places at a time.
@@ -66,13 +72,20 @@ cudaError_t ex_mma_rows(const ExArgs& e, int back, int dtype, void* packed, cuda
 cudaError_t ex_mma_weights(const ExArgs& e, int dtype, cudaStream_t s);
 int64_t ex_stretches(const ExArgs& e);
 
-// Pairs of an expert whose products one block sums: four blocks an SM where there are as many pairs, no fewer than 256.  In fp32 as in tl_stretch (a sum in tensor
-// memory is one chain of additions that are cut off); results of 16 bits do not see that, and longer stretches leave fewer sums to write and join.
+// The weights' gradient: slices of the pairs that run beside one another, as many as its tiles leave SMs for.
+static inline int ex_slices(int inner, int outer, int size)
+{
+    const int most = size == 4 ? 128 : 256;
+    return std::max(1, sm_count_cached() / std::max(1, ((inner + 127) / 128) * ((outer + most - 1) / most)));
+}
+// Pairs that one sum takes: a slice, or an equal part of it, of at most 1024 pairs in fp32 (a sum in tensor memory is one chain of additions that are cut off) and 8192 in
+// 16 bits, whose results do not see that, unless the sums would take more than twice the room of the rows.
 static inline int ex_stretch(int64_t n, int inner, int outer, int dtype)
 {
-    if (dtype == DYNB_F32) return tl_stretch(n, inner, outer, dtype);
-    const int64_t tiles = (int64_t)((inner + 127) / 128) * ((outer + 255) / 256);
-    return (int)((std::min<int64_t>(8192, std::max<int64_t>(256, n * tiles / (148 * 4) + 1)) + 31) / 32 * 32);
+    const int64_t most = std::max<int64_t>(dtype == DYNB_F32 ? 1024 : 8192, (int64_t)inner * outer / (2 * ((int64_t)inner + outer)));
+    const int slices = ex_slices(inner, outer, dtype == DYNB_F32 ? 4 : 2);
+    const int64_t slice = std::max<int64_t>(256, (n + slices - 1) / slices), parts = (slice + most - 1) / most;
+    return (int)(((slice + parts - 1) / parts + 31) / 32 * 32);
 }
 
 }  // namespace dynb

@@ -19,10 +19,11 @@ namespace dynb {
 // Warps that gather, and that store results.  An SM's four schedulers have room for five warps of 96 registers each, or four of 128: rows in fp32 wait in the registers of
 // their threads and need the latter.
 constexpr int EM_FEED = 8;
-template <typename T> constexpr int EM_OUT = sizeof(T) == 4 ? 4 : 8;
+template <typename T> constexpr int EM_OUT = sizeof(T) == 4 ? 4 : 16;
+template <typename T> constexpr int EM_COLUMNS = 16;
 template <typename T> constexpr int EM_THREADS = (EM_OUT<T> + 2 + EM_FEED) * 32;
 constexpr int EM_MAX_STAGES = 8;
-constexpr int EM_SMEM = 204 * 1024;                                  // beside 20 KB of results under way and offsets
+constexpr int EM_SMEM = 220 * 1024;                                  // beside 4 KB of offsets and barriers
 constexpr int EM_DEPTH = 3;                                          // stages whose copies a gathering warp leaves under way
 
 enum EmPath { EM_ASYNC, EM_REGISTERS, EM_SLOPE, EM_ASYNC_SLOPE };
@@ -129,35 +130,48 @@ __device__ __forceinline__ void em_keep(const TmRaw<T>& v, T* to, int have)
     }
 }
 
-// 64 bytes of each of a warp's 32 rows, lane l's from row l, to memory by pieces of 16 bytes (or elements of `size`) that lie side by side.  `mine`: 2 KB of
-// the warp, its pieces swizzled.  `row`: number of the lane's row, or -1; `bytes`: how many of the 64 there are.
-__device__ __forceinline__ void em_put(unsigned char* mine, const uint32_t* words, int lane, int32_t row, unsigned char* out, int64_t row_bytes, int bytes, int store, int size)
+// WORDS words of a row, the first `bytes` bytes of them real, in stores of 32 or 16 bytes or of elements of `size`.  Every lane stores its own row: a store of 32 bytes a lane fills
+// whole sectors, and what goes through shared memory to lie side by side costs more steps than that saves (300 k pairs 256 x 512 bf16 with slopes: 250 against 196 us).
+template <int WORDS>
+__device__ __forceinline__ void em_put(unsigned char* to, const uint32_t (&w)[WORDS], int bytes, int store, int size)
 {
-    __syncwarp();
+    if (store == 32) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        *reinterpret_cast<uint4*>(mine + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16) = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
-    __syncwarp();
-    const int at = (lane & 3) * 16;
+        for (int i = 0; i < WORDS; i += 8)
+            if (4 * i < bytes)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + 4 * i), "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                             "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                             : "memory");
+    } else if (store == 16) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int r = 8 * j + (lane >> 2);
-        const int32_t to = __shfl_sync(0xffffffffu, row, r);
-        const uint4 piece = *reinterpret_cast<const uint4*>(mine + r * 64 + (((lane & 3) ^ (r >> 1)) & 3) * 16);
-        if (to < 0 || at >= bytes) continue;
-        unsigned char* const p = out + to * row_bytes + at;
-        if (store == 16) {
-            *reinterpret_cast<uint4*>(p) = piece;
-        } else if (size == 4) {
-            const uint32_t* const e = reinterpret_cast<const uint32_t*>(&piece);
+        for (int i = 0; i < WORDS; i += 4)
+            if (4 * i < bytes) *reinterpret_cast<uint4*>(to + 4 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else if (size == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (at + 4 * i < bytes) reinterpret_cast<uint32_t*>(p)[i] = e[i];
+        for (int i = 0; i < WORDS; i++)
+            if (4 * i < bytes) reinterpret_cast<uint32_t*>(to)[i] = w[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2 * WORDS; i++)
+            if (2 * i < bytes) reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    }
+}
+
+// The activation of a row's sums, and their slopes.
+template <typename T, int ACTIVATION>
+__device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS<T>], uint32_t (&slopes)[EM_COLUMNS<T> * sizeof(T) / 4])
+{
+#pragma unroll
+    for (int i = 0; i < EM_COLUMNS<T>; i += 2) {
+        float s0, s1;
+        const float v0 = ex_activate<ACTIVATION>(__uint_as_float(bits[i]), &s0), v1 = ex_activate<ACTIVATION>(__uint_as_float(bits[i + 1]), &s1);
+        bits[i] = __float_as_uint(v0);
+        bits[i + 1] = __float_as_uint(v1);
+        if constexpr (sizeof(T) == 4) {
+            slopes[i] = __float_as_uint(s0);
+            slopes[i + 1] = __float_as_uint(s1);
         } else {
-            const uint16_t* const e = reinterpret_cast<const uint16_t*>(&piece);
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (at + 2 * i < bytes) reinterpret_cast<uint16_t*>(p)[i] = e[i];
+            slopes[i / 2] = __byte_perm(ex_slope_bits(s0), ex_slope_bits(s1), 0x5410);
         }
     }
 }
@@ -167,13 +181,12 @@ template <typename T, typename O, EmPath PATH, bool WIDE>
 __global__ void __launch_bounds__(EM_THREADS<T>, 1)
 em_rows_kernel(const ExArgs e, const EmPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = 64 / SIZE;   // columns of 64 bytes of results
+    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = EM_COLUMNS<T>, WORDS = COLUMNS * SIZE / 4;   // columns that a warp takes at a time
     constexpr int OUT = EM_OUT<T>, SHARES = OUT / 4;
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EmBars bars;
     __shared__ __align__(16) float offsets[OUT][256 / SHARES];
-    __shared__ __align__(16) unsigned char turned[OUT][2048];
     unsigned char* const panel = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
     unsigned char* const stage0 = panel + (plan.resident ? plan.chunks * plan.b_bytes : 0);
     const int warp = warp_number(), lane = threadIdx.x & 31;
@@ -213,7 +226,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         const bool with_offset = !plan.back && a.b != nullptr;
         const int activation = plan.back ? DYNB_ACTIVATION_NONE : e.activation;
         const bool with_slope = activation != DYNB_ACTIVATION_NONE && e.slope != nullptr;
-        ex_clear_absent(a, out, (int64_t)nn * SIZE, plan.store, ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OUT + warp, (int64_t)gridDim.x * gridDim.y * OUT);
+        ex_clear_absent(a, out, (int64_t)nn * SIZE, plan.store >= 16 ? 16 : 2, ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OUT + warp, (int64_t)gridDim.x * gridDim.y * OUT);
         float* const offset = offsets[warp];
         int buffer = 0, offset_type = -1;
         uint32_t phase = 0;
@@ -256,29 +269,19 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                         bits[i + 3] = __float_as_uint(__uint_as_float(bits[i + 3]) + o.w);
                     }
                 }
-                uint32_t words[16], slopes[16];
-                if (activation != DYNB_ACTIVATION_NONE) {
-#pragma unroll
-                    for (int i = 0; i < COLUMNS; i += 2) {
-                        float s0, s1;
-                        const float v0 = ex_activate(__uint_as_float(bits[i]), activation, &s0), v1 = ex_activate(__uint_as_float(bits[i + 1]), activation, &s1);
-                        bits[i] = __float_as_uint(v0);
-                        bits[i + 1] = __float_as_uint(v1);
-                        if constexpr (sizeof(T) == 4) {
-                            slopes[i] = __float_as_uint(s0);
-                            slopes[i + 1] = __float_as_uint(s1);
-                        } else if constexpr (COLUMNS == 32) {
-                            slopes[i / 2] = __byte_perm(ex_slope_bits(s0), ex_slope_bits(s1), 0x5410);
-                        }
-                    }
+                uint32_t words[WORDS], slopes[COLUMNS * sizeof(T) / 4];
+                if constexpr (std::is_same<T, O>::value) {   // one choice for all elements: with one at each, they wait for one another (381 us in place of 150)
+                    if (activation == DYNB_ACTIVATION_SILU) em_activate<T, DYNB_ACTIVATION_SILU>(bits, slopes);
+                    else if (activation == DYNB_ACTIVATION_GELU) em_activate<T, DYNB_ACTIVATION_GELU>(bits, slopes);
                 }
 #pragma unroll
                 for (int i = 0; i < COLUMNS; i += 4) {
                     const float v[4] = {__uint_as_float(bits[i]), __uint_as_float(bits[i + 1]), __uint_as_float(bits[i + 2]), __uint_as_float(bits[i + 3])};
                     tm_words<O>(v, words + i * SIZE / 4);
                 }
-                em_put(turned[warp], words, lane, r, out + (int64_t)(col0 + c) * SIZE, (int64_t)nn * SIZE, (have - c) * SIZE, plan.store, SIZE);
-                if (with_slope) em_put(turned[warp], slopes, lane, r, static_cast<unsigned char*>(e.slope) + (int64_t)(col0 + c) * SIZE, (int64_t)nn * SIZE, (have - c) * SIZE, plan.slope_store, SIZE);
+                if (r < 0) continue;
+                em_put(out + ((int64_t)r * nn + col0 + c) * SIZE, words, (have - c) * SIZE, plan.store, SIZE);
+                if (with_slope) em_put(static_cast<unsigned char*>(e.slope) + ((int64_t)r * nn + col0 + c) * SIZE, slopes, (have - c) * SIZE, plan.slope_store, SIZE);
             }
             tensor_fence_before();
             __syncwarp();
@@ -532,127 +535,206 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 }
 
 // ------------------------------------------------------------------------------------------------ gradients of the matrices
-constexpr int EW_FEED = 16, EW_THREADS = (4 + 1 + EW_FEED) * 32, EW_ROWS = 32, EW_MAX_STAGES = 8;
+// Warps that store sums, issue products, sum up the offsets' gradient, and gather.
+constexpr int EW_OUT = 4, EW_SUM = 4, EW_FEED = 16, EW_THREADS = (EW_OUT + 1 + EW_SUM + EW_FEED) * 32, EW_MAX_STAGES = 8;
+template <typename T> constexpr int EW_ROWS = sizeof(T) == 4 ? 32 : 64;   // pairs of a stage
 constexpr int EW_SMEM = 222 * 1024;
 
-struct EwPlan { int columns, column_stride, x_blocks, y_blocks, row_tiles, column_tiles, stages, depth, tensor_columns, vec; };
-struct EwBars { uint64_t full[EW_MAX_STAGES], empty[EW_MAX_STAGES], sums_full; uint32_t tensor; };
+struct EwPlan { int64_t most; int columns, column_stride, x_blocks, y_blocks, row_tiles, column_tiles, stages, depth, tensor_columns, store; };   // most: sums that there is room for
+struct EwBars { uint64_t full[EW_MAX_STAGES], empty[EW_MAX_STAGES], sums_full[2], sums_free[2]; uint32_t tensor; };
 
-__device__ __forceinline__ void ew_put_row(float* at, const uint32_t (&v)[32], int n, bool wide)
-{
-    if (wide && n >= 32) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(at + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        return;
+// The pairs in the order of their experts are cut at multiples of `stretch` and where experts begin; a block takes the pieces of its slice one after the other.
+struct EwCursor {
+    int type;                       // -1 behind the last
+    int64_t begin, end, end_of_type, end_of_slice, index;   // index: number of the piece among all
+
+    __device__ __forceinline__ void cut(int stretch) { end = min(min(end_of_type, end_of_slice), (begin / stretch + 1) * stretch); }
+    __device__ __forceinline__ void start(const TlArgs& a, int64_t first, int64_t last)   // all lanes of a warp
+    {
+        const int lane = threadIdx.x & 31;
+        type = -1;
+        end_of_slice = last;
+        index = 0;
+        begin = first;
+        if (first >= last) return;
+        for (int t0 = 0; t0 < a.types; t0 += 32) {
+            int64_t s0 = 0, s1 = 0;
+            if (t0 + lane < a.types) tl_rows_of(a, t0 + lane, &s0, &s1);
+            const int mine = s1 > s0 ? (int)((s1 + a.stretch - 1) / a.stretch - s0 / a.stretch) : 0;
+            int total;
+            const int before = warp_excl_scan(mine, lane, &total);
+            const uint32_t found = __ballot_sync(0xffffffffu, s0 <= first && first < s1);
+            if (found != 0) {
+                const int from = __ffs(found) - 1;
+                type = t0 + from;
+                end_of_type = __shfl_sync(0xffffffffu, s1, from);
+                index += __shfl_sync(0xffffffffu, before, from) + first / a.stretch - __shfl_sync(0xffffffffu, s0, from) / a.stretch;
+                cut(a.stretch);
+                return;
+            }
+            index += total;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 32; i++)
-        if (i < n) at[i] = __uint_as_float(v[i]);
-}
+    __device__ __forceinline__ void next(const TlArgs& a)
+    {
+        begin = end;
+        index++;
+        if (begin >= end_of_slice) { type = -1; return; }
+        while (begin >= end_of_type) {
+            if (++type >= a.types) { type = -1; return; }
+            int64_t s0;
+            tl_rows_of(a, type, &s0, &end_of_type);
+        }
+        cut(a.stretch);
+    }
+};
 
 template <typename T, EmPath PATH, bool WIDE>
 __global__ void __launch_bounds__(EW_THREADS, 1)
 em_weights_kernel(const ExArgs e, const EwPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, FIRST = PARTS == 1 ? 1 : 2;   // sums of the matrix: leading parts, small ones; those of the rows behind them
-    constexpr int FEED_THREADS = EW_FEED * 32, BLOCK = EW_ROWS * 128;
-    constexpr int UNITS = PARTS == 1 ? 3 : 2;   // pieces of 8 elements a thread and stage: 32 pairs x (128 + 256 or 128) elements
+    constexpr int PARTS = TmParts<T>::N, FEED_THREADS = EW_FEED * 32, ROWS = EW_ROWS<T>, BLOCK = ROWS * 128;
+    constexpr int SUMS = PARTS == 1 ? 1 : 2;    // sums of a buffer: leading parts, small ones
+    constexpr int UNITS = PARTS == 1 ? 6 : 2;   // pieces of 8 elements a thread and stage: 64 pairs x (128 + 256) elements, or 32 x (128 + 128)
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EwBars bars;
-    unsigned char* const ones = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
-    unsigned char* const stage0 = ones + TM_ROWS * 128;
+    unsigned char* const stage0 = raw_smem + ((1024 - (smem_addr(raw_smem) & 1023)) & 1023);
     const int warp = warp_number(), lane = threadIdx.x & 31;
-    // the tiles of a stretch are neighbours: what they share comes from L2
-    const int tiles = plan.row_tiles * plan.column_tiles, of_tile = blockIdx.x % tiles;
-    const int64_t stretch = blockIdx.x / tiles;
+    // the tiles of a slice are neighbours: what they share comes from L2
+    const int tiles = plan.row_tiles * plan.column_tiles, of_tile = blockIdx.x % tiles, slices = gridDim.x / tiles;
     const int row0 = of_tile / plan.column_tiles * TM_ROWS, col0 = of_tile % plan.column_tiles * plan.columns;
     const int blocks = plan.x_blocks + plan.y_blocks, stage_bytes = blocks * PARTS * BLOCK;
-    const TlTile tile = tl_tile(a, stretch, a.stretch);
-    if (tile.type < 0) return;   // the whole block
-    const int steps = (int)((tile.end - tile.begin + EW_ROWS - 1) / EW_ROWS);
     const bool sums_wanted = row0 == 0 && a.db != nullptr;
+    const int64_t cells = (int64_t)a.inner * a.outer;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
             bar_init(&bars.full[s], EW_FEED);
-            bar_init(&bars.empty[s], 1);
+            bar_init(&bars.empty[s], sums_wanted ? 1 + EW_SUM : 1);
         }
-        bar_init(&bars.sums_full, 1);
+        for (int b = 0; b < 2; b++) {
+            bar_init(&bars.sums_full[b], 1);
+            bar_init(&bars.sums_free[b], EW_OUT);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const uint32_t one = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
-    for (int i = threadIdx.x; i < TM_ROWS * 8; i += EW_THREADS) reinterpret_cast<uint4*>(ones)[i] = make_uint4(one, one, one, one);
-    fence_to_tensor();
     if (warp == 0) tensor_alloc(&bars.tensor, plan.tensor_columns);
     tensor_fence_before();
     __syncthreads();
     tensor_fence_after();
     const uint32_t tensor = bars.tensor;
+    const int64_t all = min(max((int64_t)a.start[a.types], (int64_t)0), a.n), pieces = (all + a.stretch - 1) / a.stretch;
+    const int64_t slice = ((pieces + slices - 1) / slices) * a.stretch, first = min((int64_t)(blockIdx.x / tiles) * slice, all);
+    EwCursor cursor;
+    cursor.start(a, first, min(first + slice, all));
 
-    if (warp < 4) {
-        if (!bar_wait(&bars.sums_full, 0)) {
-            tm_ran_out(a);
-        } else {
-            tensor_fence_after();
-            const int64_t cells = (int64_t)a.inner * a.outer;
-            float* const mine = a.partial + stretch * (cells + a.outer);
-            const int m = row0 + threadIdx.x, have = min(plan.columns, a.outer - col0);
-            for (int which = 0; which < (sums_wanted ? 2 : 1); which++) {
-                float* const at = which == 0 ? mine + (int64_t)m * a.outer + col0 : mine + cells + col0;
-                const bool write = which == 0 ? m < a.inner : threadIdx.x == 0;
-                const uint32_t from = tensor + ((uint32_t)(warp * 32) << 16) + which * FIRST * plan.column_stride;
-                for (int c = 0; c < have; c += 32) {
-                    uint32_t bits[32];
-                    __syncwarp();
-                    tensor_load_32(from + c, bits);
-                    tensor_wait_loads();
-                    if constexpr (PARTS > 1) {
-                        uint32_t small[32];
-                        tensor_load_32(from + plan.column_stride + c, small);
-                        tensor_wait_loads();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
-                    }
-                    if (write) ew_put_row(at + c, bits, have - c, plan.vec != 0);
-                }
-            }
-        }
-    } else if (warp == 4) {
-        const bool bf16 = !std::is_same<T, __half>::value;
-        const uint32_t what = mma_what(bf16, plan.columns, true, true), what_sum = mma_what(bf16, plan.columns, false, true);
-        const uint32_t stage_at = smem_addr(stage0);
-        const uint64_t ones_desc = tile_descriptor(smem_addr(ones), 16, 1024);
-        const uint32_t lead = PARTS * BLOCK, lead_x = plan.x_blocks > 1 ? lead : 0;   // one block: the upper 64 rows repeat the lower
-        int stage = 0;
+    if (warp < EW_OUT) {
+        int buffer = 0;
         uint32_t phase = 0;
-        bool ok = true;
-        for (int step = 0; step < steps; step++) {
-            if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+        const int m = row0 + threadIdx.x, have = min(plan.columns, a.outer - col0);
+        for (; cursor.type >= 0; cursor.next(a)) {
+            if (!bar_wait(&bars.sums_full[buffer], phase)) { tm_ran_out(a); break; }
             tensor_fence_after();
-            if (elected()) {
-                const uint32_t at = stage_at + stage * stage_bytes;
-                const uint64_t at_x = tile_descriptor(at, lead_x, 1024), at_y = tile_descriptor(at + plan.x_blocks * PARTS * BLOCK, lead, 1024);
+            unsigned char* const at = reinterpret_cast<unsigned char*>(a.partial + cursor.index * (cells + a.outer) + (int64_t)m * a.outer + col0);
+            const uint32_t from = tensor + ((uint32_t)(warp * 32) << 16) + buffer * SUMS * plan.column_stride;
+            for (int c = 0; c < have; c += 16) {
+                uint32_t bits[16];
+                __syncwarp();
+                tensor_load(from + c, bits);
+                if constexpr (PARTS > 1) {
+                    uint32_t small[16];
+                    tensor_load(from + plan.column_stride + c, small);
+                    tensor_wait_loads();
 #pragma unroll
-                for (int k = 0; k < EW_ROWS / 16; k++) tm_step<PARTS>(tensor, tensor + plan.column_stride, at_x + k * 128, BLOCK / 16, at_y + k * 128, BLOCK / 16, what, step > 0 || k > 0);
-                if (sums_wanted) {
-#pragma unroll
-                    for (int p = PARTS - 1; p >= 0; p--)
-#pragma unroll
-                        for (int k = 0; k < EW_ROWS / 16; k++)
-                            tensor_mma(tensor + (p == 0 ? FIRST : FIRST + 1) * plan.column_stride, ones_desc, at_y + (p * BLOCK + k * 2048) / 16, what_sum,
-                                       step > 0 || k > 0 || (p > 0 && p < PARTS - 1));
+                    for (int i = 0; i < 16; i++) bits[i] = __float_as_uint(__uint_as_float(bits[i]) + __uint_as_float(small[i]));
+                } else {
+                    tensor_wait_loads();
                 }
-                tensor_commit(&bars.empty[stage]);
-                if (step == steps - 1) tensor_commit(&bars.sums_full);
+                if (m < a.inner && cursor.index < plan.most) em_put(at + 4 * c, bits, 4 * (have - c), plan.store, 4);
             }
+            tensor_fence_before();
             __syncwarp();
-            if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+            if (lane == 0) bar_arrive(&bars.sums_free[buffer]);
+            buffer ^= 1;
+            if (buffer == 0) phase ^= 1;
+        }
+    } else if (warp == EW_OUT) {
+        const bool bf16 = !std::is_same<T, __half>::value;
+        const uint32_t what = mma_what(bf16, plan.columns, true, true);
+        const uint32_t stage_at = smem_addr(stage0);
+        const uint32_t lead = PARTS * BLOCK, lead_x = plan.x_blocks > 1 ? lead : 0;   // one block: the upper 64 rows repeat the lower
+        int stage = 0, buffer = 0;
+        uint32_t phase = 0, sums_phase = 1;
+        bool ok = true;
+        for (; ok && cursor.type >= 0; cursor.next(a)) {
+            const int steps = (int)((cursor.end - cursor.begin + ROWS - 1) / ROWS);
+            if (!bar_wait(&bars.sums_free[buffer], sums_phase)) { ok = false; break; }
+            tensor_fence_after();
+            const uint32_t sums = tensor + buffer * SUMS * plan.column_stride;
+            for (int step = 0; step < steps; step++) {
+                if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+                tensor_fence_after();
+                if (elected()) {
+                    const uint32_t at = stage_at + stage * stage_bytes;
+                    const uint64_t at_x = tile_descriptor(at, lead_x, 1024), at_y = tile_descriptor(at + plan.x_blocks * PARTS * BLOCK, lead, 1024);
+#pragma unroll
+                    for (int k = 0; k < ROWS / 16; k++) tm_step<PARTS>(sums, sums + plan.column_stride, at_x + k * 128, BLOCK / 16, at_y + k * 128, BLOCK / 16, what, step > 0 || k > 0);
+                    tensor_commit(&bars.empty[stage]);
+                    if (step == steps - 1) tensor_commit(&bars.sums_full[buffer]);
+                }
+                __syncwarp();
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+            }
+            buffer ^= 1;
+            if (buffer == 0) sums_phase ^= 1;
         }
         if (!ok) tm_ran_out(a);
+    } else if (warp < EW_OUT + 1 + EW_SUM) {
+        // the offsets' gradient: a thread sums two columns of the stages as they stand in shared memory, all parts
+        if (sums_wanted) {
+            const int c = (threadIdx.x - (EW_OUT + 1) * 32) * 2, have = min(plan.columns, a.outer - col0);
+            const uint32_t at = smem_addr(stage0) + (plan.x_blocks + c / 64) * PARTS * BLOCK + (c & 7) * 2;
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (; ok && cursor.type >= 0; cursor.next(a)) {
+                const int steps = (int)((cursor.end - cursor.begin + ROWS - 1) / ROWS);
+                float lo = 0.0f, hi = 0.0f;
+                for (int step = 0; step < steps; step++) {
+                    if (!bar_wait(&bars.full[stage], phase)) { tm_ran_out(a); ok = false; break; }
+                    if (c < plan.columns) {
+                        float l = 0.0f, h = 0.0f;
+#pragma unroll
+                        for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll 16
+                            for (int r = 0; r < ROWS; r++) {
+                                uint32_t v;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at + stage * stage_bytes + p * BLOCK + tile_piece(r, (c >> 3) & 7)));
+                                if constexpr (std::is_same<T, __half>::value) {
+                                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                                    l += f.x;
+                                    h += f.y;
+                                } else {
+                                    l += __uint_as_float(v << 16);
+                                    h += __uint_as_float(v & 0xffff0000u);
+                                }
+                            }
+                        lo += l;
+                        hi += h;
+                    }
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&bars.empty[stage]);
+                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                }
+                float* const to = a.partial + cursor.index * (cells + a.outer) + cells + col0 + c;
+                if (ok && c < have && cursor.index < plan.most) to[0] = lo;
+                if (ok && c + 1 < have && cursor.index < plan.most) to[1] = hi;
+            }
+        }
     } else {
-        const int tid = threadIdx.x - 5 * 32;
-        const int per_row = blocks * 8, units = EW_ROWS * per_row;
+        const int tid = threadIdx.x - (EW_OUT + 1 + EW_SUM) * 32;
+        const int per_row = blocks * 8, units = ROWS * per_row;
         // this thread's pieces are the same ones in every stage: row, place in the stage, operand, column
         int row[UNITS], at[UNITS], col[UNITS];
 #pragma unroll
@@ -666,12 +748,19 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             const int limit = of_y ? min(a.outer, col0 + plan.columns) : a.inner;
             col[i] = c < limit ? (of_y ? c | (1 << 30) : c) : -1;
         }
-        auto rows_of = [&](int step, int32_t (&r)[UNITS]) {
+        // the pairs of the next stage
+        int64_t place = cursor.begin;
+        auto rows_of = [&](int32_t (&r)[UNITS]) {
 #pragma unroll
-            for (int i = 0; i < UNITS; i++) {
-                const int64_t place = tile.begin + (int64_t)step * EW_ROWS + row[i];
-                r[i] = row[i] >= 0 && col[i] >= 0 && place < tile.end ? __ldg(a.order + place) : -1;   // looked at a stage later
+            for (int i = 0; i < UNITS; i++)
+                r[i] = cursor.type >= 0 && row[i] >= 0 && col[i] >= 0 && place + row[i] < cursor.end ? __ldg(a.order + place + row[i]) : -1;   // looked at a stage later
+            if (cursor.type < 0) return false;
+            place += ROWS;
+            if (place >= cursor.end) {
+                cursor.next(a);
+                place = cursor.begin;
             }
+            return true;
         };
         const uint32_t fan = e.fan;
         auto address = [&](int i, int32_t p) {
@@ -682,6 +771,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
         int32_t ids[UNITS];
         int stage = 0;
         uint32_t phase = 1;
+        bool more = rows_of(ids);
         if constexpr (PATH == EM_ASYNC) {
             int arrived = 0;
             auto arrive = [&] {
@@ -690,18 +780,14 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                 if (lane == 0) bar_arrive(&bars.full[arrived]);
                 if (++arrived == plan.stages) arrived = 0;
             };
-            rows_of(0, ids);
-            int asked = 0;
-            for (int step = 0; step < steps; step++) {
-                int32_t next[UNITS];
-                rows_of(step + 1, next);
-                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+            int64_t asked = 0;
+            auto ask = [&](const int32_t (&r)[UNITS]) {
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); return false; }
                 const uint32_t to = smem_addr(stage0) + stage * stage_bytes;
 #pragma unroll
                 for (int i = 0; i < UNITS; i++) {
-                    const bool live = (uint32_t)ids[i] < (uint64_t)a.n;
-                    if (row[i] >= 0) copy_16(to + at[i], live ? address(i, ids[i]) : static_cast<const T*>(a.x), live);
-                    ids[i] = next[i];
+                    const bool live = (uint32_t)r[i] < (uint64_t)a.n;
+                    if (row[i] >= 0) copy_16(to + at[i], live ? address(i, r[i]) : static_cast<const T*>(a.x), live);
                 }
                 copies_commit();
                 if (++stage == plan.stages) { stage = 0; phase ^= 1; }
@@ -709,8 +795,18 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                     copies_wait(plan.depth);
                     arrive();
                 }
+                return true;
+            };
+            // numbers of two stages by turns, each asked for two stages ahead (copied from one place to another they would be waited for at once)
+            int32_t others[UNITS];
+            bool other = rows_of(others);
+            while (more) {
+                if (!ask(ids)) break;
+                more = rows_of(ids);
+                if (!other || !ask(others)) break;
+                other = rows_of(others);
             }
-            for (int left = min(asked, plan.depth); left > 0; left--) {
+            for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
                 copies_wait(left - 1);
                 arrive();
             }
@@ -726,10 +822,9 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                 }
             };
             // the rows of the next stage are asked for behind this one, their numbers a stage earlier
-            rows_of(0, ids);
             fetch(ids);
-            rows_of(1, ids);
-            for (int step = 0; step < steps; step++) {
+            bool behind = rows_of(ids);
+            while (more) {
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
                 if (tm_odd(v)) {
 #pragma unroll
@@ -744,8 +839,9 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bars.full[stage]);
                 if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                fetch(ids);   // behind the stretch: zeros
-                rows_of(step + 2, ids);
+                fetch(ids);   // behind the last stage: zeros
+                more = behind;
+                behind = rows_of(ids);
             }
         }
     }
@@ -802,8 +898,8 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     int tiles;
     EmPlan p = em_plan<T>(e, back, SIZE == 2 && slope && wide, &tiles);
     p.packed = static_cast<const unsigned char*>(packed);
-    p.store = tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
-    p.slope_store = e.slope != nullptr && tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
+    p.store = tm_on(out, nn, sizeof(O), 32) ? 32 : tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
+    p.slope_store = tm_on(e.slope, nn, SIZE, 32) ? 32 : tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
     const int64_t units = (int64_t)a.types * tiles * p.chunks * p.columns * 8;
     ex_pack_kernel<T><<<(unsigned)std::min<int64_t>((units + 255) / 256, (int64_t)sm_count_cached() * 8), 256, 0, s>>>(
         static_cast<const T*>(a.w), a.types, a.inner, a.outer, back, p.columns, tiles, p.chunks, static_cast<unsigned char*>(packed));
@@ -840,14 +936,15 @@ cudaError_t ex_mma_rows(const ExArgs& e, int back, int dtype, void* packed, cuda
     return em_rows_of<__nv_bfloat16>(e, back, packed, s);
 }
 
-int64_t ex_stretches(const ExArgs& e) { return tl_stretches(e.t.n, e.t.types, e.t.stretch); }
+int64_t ex_stretches(const ExArgs& e) { return e.t.n / e.t.stretch + 1 + std::min<int64_t>(e.t.n, e.t.types); }   // cuts at multiples, and where experts begin
 
 template <typename T>
 static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
 {
-    constexpr int PARTS = TmParts<T>::N, BLOCK = EW_ROWS * 128, SIZE = (int)sizeof(T);
+    constexpr int PARTS = TmParts<T>::N, BLOCK = EW_ROWS<T> * 128, SIZE = (int)sizeof(T);
     const TlArgs& a = e.t;
     EwPlan p = {};
+    p.most = ex_stretches(e);
     const int most = PARTS == 1 ? 256 : 128, tiles = (a.outer + most - 1) / most;
     p.columns = tm_round((a.outer + tiles - 1) / tiles, 16);
     p.column_stride = tm_round(p.columns, 32);
@@ -856,20 +953,19 @@ static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
     p.row_tiles = (a.inner + TM_ROWS - 1) / TM_ROWS;
     p.column_tiles = (a.outer + p.columns - 1) / p.columns;
     const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
-    p.stages = std::min(EW_MAX_STAGES, (EW_SMEM - 1024 - TM_ROWS * 128) / stage);
+    p.stages = std::min(EW_MAX_STAGES, (EW_SMEM - 1024) / stage);
     p.depth = std::min(EM_DEPTH, p.stages - 1);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
-    p.vec = a.outer % 4 == 0 && tm_on(a.partial, 0, 4, 16);
+    p.store = tm_on(a.partial, a.outer, 4, 32) && (int64_t)a.inner * a.outer % 8 == 0 ? 32 : tm_on(a.partial, a.outer, 4, 16) ? 16 : 4;
     void (*kernel)(ExArgs, EwPlan);
     if (!wide) kernel = em_weights_kernel<T, EM_REGISTERS, false>;
     else if constexpr (SIZE == 4) kernel = em_weights_kernel<T, EM_REGISTERS, true>;
     else kernel = em_weights_kernel<T, EM_ASYNC, true>;
-    const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;
+    const int smem = 1024 + p.stages * stage, tiles_of = p.row_tiles * p.column_tiles;
     const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    const int64_t grid = ex_stretches(e) * p.row_tiles * p.column_tiles;
-    kernel<<<(unsigned)grid, EW_THREADS, smem, s>>>(e, p);
+    kernel<<<(unsigned)(std::max(1, ex_slices(a.inner, a.outer, sizeof(T))) * tiles_of), EW_THREADS, smem, s>>>(e, p);
     return cudaGetLastError();
 }
 
