@@ -733,27 +733,14 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             }
         }
     } else {
-        const int tid = threadIdx.x - (EW_OUT + 1 + EW_SUM) * 32;
-        const int per_row = blocks * 8, units = ROWS * per_row;
-        // this thread's pieces are the same ones in every stage: row, place in the stage, operand, column
-        int row[UNITS], at[UNITS], col[UNITS];
-#pragma unroll
-        for (int i = 0; i < UNITS; i++) {
-            const int u = tid + i * FEED_THREADS, r = u / per_row, piece = u % per_row;
-            const int block = piece >> 3;
-            const bool of_y = block >= plan.x_blocks;
-            row[i] = u < units ? r : -1;
-            at[i] = block * PARTS * BLOCK + (int)tile_piece(r, piece & 7);
-            const int c = (of_y ? col0 + (block - plan.x_blocks) * 64 : row0 + block * 64) + (piece & 7) * 8;
-            const int limit = of_y ? min(a.outer, col0 + plan.columns) : a.inner;
-            col[i] = c < limit ? (of_y ? c | (1 << 30) : c) : -1;
-        }
-        // the pairs of the next stage
+        // a thread takes pieces of one pair's rows, piece `piece` of every block (of every other one): number, division and addresses of the pair are its own, once a stage
+        constexpr int GROUPS = FEED_THREADS / (ROWS * 8);
+        const int tid = threadIdx.x - (EW_OUT + 1 + EW_SUM) * 32, piece = tid & 7, group = (tid >> 3) % GROUPS, r = tid / (8 * GROUPS);
+        const int at0 = group * PARTS * BLOCK + (int)tile_piece(r, piece), y_limit = min(a.outer, col0 + plan.columns);
+        // the pair of the next stage
         int64_t place = cursor.begin;
-        auto rows_of = [&](int32_t (&r)[UNITS]) {
-#pragma unroll
-            for (int i = 0; i < UNITS; i++)
-                r[i] = cursor.type >= 0 && row[i] >= 0 && col[i] >= 0 && place + row[i] < cursor.end ? __ldg(a.order + place + row[i]) : -1;   // looked at a stage later
+        auto row_of = [&](int32_t& p) {
+            p = cursor.type >= 0 && place + r < cursor.end ? __ldg(a.order + place + r) : -1;   // looked at a stage later
             if (cursor.type < 0) return false;
             place += ROWS;
             if (place >= cursor.end) {
@@ -762,16 +749,24 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             }
             return true;
         };
-        const uint32_t fan = e.fan;
-        auto address = [&](int i, int32_t p) {
-            const int c = col[i] & ((1 << 30) - 1);
-            if ((col[i] >> 30) & 1) return static_cast<const T*>(a.dy) + p * a.dy_row + c;
-            return static_cast<const T*>(a.x) + (int64_t)(fan == 1 ? (uint32_t)p : (uint32_t)p / fan) * a.x_row + c;
+        // f(unit, address, elements there are) for every unit of pair p
+        auto units_of = [&](int32_t p, auto&& f) {
+            const bool live = (uint32_t)p < (uint64_t)a.n;
+            const T* const x = static_cast<const T*>(a.x) + (live ? (int64_t)(e.fan == 1 ? (uint32_t)p : (uint32_t)p / (uint32_t)e.fan) * a.x_row : 0);
+            const T* const y = static_cast<const T*>(a.dy) + (live ? p * a.dy_row : 0);
+#pragma unroll
+            for (int i = 0; i < UNITS; i++) {
+                const int block = i * GROUPS + group;
+                if (block >= blocks) continue;
+                const bool of_y = block >= plan.x_blocks;
+                const int c = (of_y ? col0 + (block - plan.x_blocks) * 64 : row0 + block * 64) + piece * 8, have = live ? min(8, (of_y ? y_limit : a.inner) - c) : 0;
+                f(i, (of_y ? y : x) + (have > 0 ? c : 0), have);
+            }
         };
-        int32_t ids[UNITS];
+        int32_t id;
         int stage = 0;
         uint32_t phase = 1;
-        bool more = rows_of(ids);
+        bool more = row_of(id);
         if constexpr (PATH == EM_ASYNC) {
             int arrived = 0;
             auto arrive = [&] {
@@ -781,14 +776,10 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                 if (++arrived == plan.stages) arrived = 0;
             };
             int64_t asked = 0;
-            auto ask = [&](const int32_t (&r)[UNITS]) {
+            auto ask = [&](int32_t p) {
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); return false; }
-                const uint32_t to = smem_addr(stage0) + stage * stage_bytes;
-#pragma unroll
-                for (int i = 0; i < UNITS; i++) {
-                    const bool live = (uint32_t)r[i] < (uint64_t)a.n;
-                    if (row[i] >= 0) copy_16(to + at[i], live ? address(i, r[i]) : static_cast<const T*>(a.x), live);
-                }
+                const uint32_t to = smem_addr(stage0) + stage * stage_bytes + at0;
+                units_of(p, [&](int i, const T* from, int have) { copy_16(to + i * GROUPS * BLOCK, from, have > 0); });
                 copies_commit();
                 if (++stage == plan.stages) { stage = 0; phase ^= 1; }
                 if (++asked > plan.depth) {
@@ -798,13 +789,13 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                 return true;
             };
             // numbers of two stages by turns, each asked for two stages ahead (copied from one place to another they would be waited for at once)
-            int32_t others[UNITS];
-            bool other = rows_of(others);
+            int32_t other_id;
+            bool other = row_of(other_id);
             while (more) {
-                if (!ask(ids)) break;
-                more = rows_of(ids);
-                if (!other || !ask(others)) break;
-                other = rows_of(others);
+                if (!ask(id)) break;
+                more = row_of(id);
+                if (!other || !ask(other_id)) break;
+                other = row_of(other_id);
             }
             for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
                 copies_wait(left - 1);
@@ -812,36 +803,30 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             }
             copies_wait(0);
         } else {
-            TmRaw<T> v[UNITS];
-            auto fetch = [&](const int32_t (&r)[UNITS]) {
-#pragma unroll
-                for (int i = 0; i < UNITS; i++) {
-                    const bool of_y = (col[i] >> 30) & 1, ok = (uint32_t)r[i] < (uint64_t)a.n;
-                    const int c = col[i] & ((1 << 30) - 1), have = ok ? min(8, (of_y ? a.outer : a.inner) - c) : 0;
-                    v[i] = tm_load<WIDE>(ok ? address(i, r[i]) : static_cast<const T*>(a.x), 1, have);
-                }
-            };
+            TmRaw<T> v[UNITS] = {};
+            auto fetch = [&](int32_t p) { units_of(p, [&](int i, const T* from, int have) { v[i] = tm_load<WIDE>(from, 1, have); }); };
             // the rows of the next stage are asked for behind this one, their numbers a stage earlier
-            fetch(ids);
-            bool behind = rows_of(ids);
+            fetch(id);
+            bool behind = row_of(id);
             while (more) {
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+                unsigned char* const to = stage0 + stage * stage_bytes + at0;
                 if (tm_odd(v)) {
 #pragma unroll
                     for (int i = 0; i < UNITS; i++)
-                        if (row[i] >= 0) tm_store<true>(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                        if (i * GROUPS + group < blocks) tm_store<true>(v[i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
                 } else {
 #pragma unroll
                     for (int i = 0; i < UNITS; i++)
-                        if (row[i] >= 0) tm_store<false>(v[i], stage0 + stage * stage_bytes + at[i], BLOCK);
+                        if (i * GROUPS + group < blocks) tm_store<false>(v[i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
                 }
                 fence_to_tensor();
                 __syncwarp();
                 if (lane == 0) bar_arrive(&bars.full[stage]);
                 if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                fetch(ids);   // behind the last stage: zeros
+                fetch(id);   // behind the last stage: zeros
                 more = behind;
-                behind = rows_of(ids);
+                behind = row_of(id);
             }
         }
     }
