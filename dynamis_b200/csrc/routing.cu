@@ -37,7 +37,7 @@ __device__ __forceinline__ uint64_t re_max(uint64_t v)   // of a warp
 __device__ __forceinline__ uint64_t re_order(double key)
 {
     if (isnan(key)) return ~0ull;
-    return key == -INFINITY ? 0ull : ordered_u64(key);
+    return key == -INFINITY ? 0ull : ordered_u64(key + 0.0);   // -0 and 0 are equal
 }
 
 template <typename T, int V>
@@ -185,6 +185,242 @@ re_choose_kernel(const ReArgs a)
     }
     __syncthreads();
     for (int i = threadIdx.x; i <= a.count; i += RE_WARPS * 32) a.counts[(int64_t)i * gridDim.x + blockIdx.x] = counts[i];
+}
+
+// ------------------------------------------------------------------------------------------------ a thread a row
+// Up to 128 experts, 8 choices and 16 groups: a warp brings 32 rows to shared memory and every lane goes along one.  (A warp a row spends its time on exchanges between
+// lanes: 1 M rows of 32 bf16 logits, two choices, 350 us; gradient 292 us.)  Where more than the logits decide, keys are formed in 32 bits first; rows in which two that
+// matter lie nearer to one another than these may be off are looked at again in 64 bits.
+constexpr int RT_WARPS = 4, RT_MAX_EXPERTS = 128, RT_MAX_CHOICES = 8, RT_MAX_GROUPS = 16;
+
+__device__ __forceinline__ uint32_t rt_order(float key)   // as re_order
+{
+    if (isnan(key)) return 0xffffffffu;
+    return key == -INFINITY ? 0u : ordered_u32(key + 0.0f);
+}
+__device__ __forceinline__ uint64_t rt_order(double key) { return re_order(key); }
+__device__ __forceinline__ float rt_value(uint32_t order) { return order == 0xffffffffu ? NAN : unordered_f32(order); }
+__device__ __forceinline__ double rt_value(uint64_t order) { return order == ~0ull ? NAN : unordered_f64(order); }
+template <typename K> struct RtOrder { using type = uint32_t; };
+template <> struct RtOrder<double> { using type = uint64_t; };
+
+__device__ __forceinline__ float rt_exp(float v) { return expf(v); }
+__device__ __forceinline__ double rt_exp(double v) { return exp(v); }
+
+// 32 rows from `row0` on to `tile` (`pitch` floats a row), rows behind the last as zeros.
+template <typename T>
+__device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* tile, int pitch, int wide)
+{
+    const int lane = threadIdx.x & 31;
+    const T* const l = static_cast<const T*>(a.logits);
+    constexpr int N = 16 / (int)sizeof(T);
+    if (wide) {
+        const int per = a.count / N;
+        for (int u = lane; u < 32 * per; u += 32) {
+            const int r = u / per, c = (u % per) * N;
+            if (row0 + r >= a.n) break;
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(l + (row0 + r) * a.row + c));
+            const T* const e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int i = 0; i < N; i++) tile[r * pitch + c + i] = tl_get(e + i);
+        }
+    } else {
+        for (int u = lane; u < 32 * a.count; u += 32) {
+            const int r = u / a.count, c = u % a.count;
+            if (row0 + r >= a.n) break;
+            tile[r * pitch + c] = tl_get(l + (row0 + r) * a.row + c);
+        }
+    }
+}
+
+// The experts of a lane's row by keys of type K; MOST: choices and two more, the first that are left out.  False: rounding of the keys may have decided.
+template <typename K, int MOST>
+__device__ __forceinline__ bool rt_choose(const ReArgs& a, const float* l, const float* bias, float top, K sum, K near, int (&chosen)[MOST], typename RtOrder<K>::type (&order)[MOST])
+{
+    using O = typename RtOrder<K>::type;
+    auto key_of = [&](int e) -> O {
+        const float v = l[e];
+        if (v == -INFINITY) return 0;
+        const K s = a.sigmoid ? (K)1 / ((K)1 + rt_exp(-(K)v)) : rt_exp((K)v - (K)top) / sum;
+        return rt_order(s + (K)bias[e]);
+    };
+    bool sure = true;
+    uint32_t kept = 0xffffffffu;
+    const int per = a.count / a.groups;
+    if (a.groups > 1) {
+        O of_group[RT_MAX_GROUPS];
+#pragma unroll
+        for (int g = 0; g < RT_MAX_GROUPS; g++) {
+            of_group[g] = 0;
+            if (g >= a.groups) continue;
+            O one = 0, two = 0;
+            for (int i = 0; i < per; i++) {
+                const O k = key_of(g * per + i);
+                two = max(two, min(one, k));
+                one = max(one, k);
+            }
+            O both = one;
+            if (one == (O)~(O)0 || two == (O)~(O)0) both = ~(O)0;
+            else if (two != 0) both = rt_order(rt_value(one) + rt_value(two));
+            if (one != 0 && both == 0) both = 1;   // open, however low
+            of_group[g] = both;
+        }
+        kept = 0;
+        O lowest = ~(O)0, highest = 0;   // of those that stay, and of the others
+#pragma unroll
+        for (int g = 0; g < RT_MAX_GROUPS; g++) {
+            if (g >= a.groups) continue;
+            int before = 0;
+#pragma unroll
+            for (int h = 0; h < RT_MAX_GROUPS; h++) before += h < a.groups && (of_group[h] > of_group[g] || (of_group[h] == of_group[g] && h < g));
+            if (before < a.kept) {
+                kept |= 1u << g;
+                lowest = min(lowest, of_group[g]);
+            } else {
+                highest = max(highest, of_group[g]);
+            }
+        }
+        if (highest != 0) sure = rt_value(lowest) - rt_value(highest) > (K)6 * near;
+    }
+#pragma unroll
+    for (int j = 0; j < MOST; j++) {
+        order[j] = 0;
+        chosen[j] = -1;
+    }
+    for (int g = 0; g < a.groups; g++) {
+        if (!(kept >> (g & 31) & 1)) continue;
+        for (int i = 0; i < per; i++) {
+            const O k = key_of(g * per + i);
+            if (k <= order[MOST - 1]) continue;
+#pragma unroll
+            for (int j = MOST - 1; j >= 0; j--) {
+                if (k <= order[j]) continue;
+                if (j + 1 < MOST) {
+                    order[j + 1] = order[j];
+                    chosen[j + 1] = chosen[j];
+                }
+                order[j] = k;
+                chosen[j] = g * per + i;
+            }
+        }
+    }
+    bool tie = false;   // the last choice and the first that is left out have the same key, whatever its type
+#pragma unroll
+    for (int j = 0; j + 1 < MOST; j++) {
+        if (order[j + 1] == 0 || j > a.choices || (j == a.choices && !tie)) continue;
+        if (rt_value(order[j]) - rt_value(order[j + 1]) > (K)2 * near) continue;
+        const int p = chosen[j], q = chosen[j + 1];
+        tie = j == a.choices - 1;
+        if (j == a.choices || !(l[p] == l[q] && bias[p] == bias[q])) sure = false;
+    }
+    return sure;
+}
+
+template <typename T, int MOST>
+__global__ void __launch_bounds__(RT_WARPS * 32)
+rt_choose_kernel(const ReArgs a, int pitch, int wide)
+{
+    extern __shared__ unsigned char raw_smem[];
+    int32_t* const counts = reinterpret_cast<int32_t*>(raw_smem);   // [experts + 1], then the biases [experts], then the rows of every warp
+    float* const bias = reinterpret_cast<float*>(counts + a.count + 1);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    float* const tile = bias + a.count + warp * 32 * pitch;
+    const float* const l = tile + lane * pitch;
+    const bool plain = a.bias == nullptr && a.groups == 1;   // the logits decide
+    float far = 0.0f;
+    for (int i = threadIdx.x; i <= a.count; i += RT_WARPS * 32) counts[i] = 0;
+    for (int i = threadIdx.x; i < a.count; i += RT_WARPS * 32) bias[i] = a.bias != nullptr ? a.bias[i] : 0.0f;
+    __syncthreads();
+    if (!plain)
+        for (int i = lane; i < a.count; i += 32) far = fmaxf(far, isinf(bias[i]) ? 0.0f : fabsf(bias[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) far = fmaxf(far, __shfl_xor_sync(0xffffffffu, far, o));
+    // how far a key in 32 bits may be off: a score by (experts + 16) 2^-24 (sigmoids 16), the sum with the bias by half a step
+    const float near = ((a.sigmoid ? 16.0f : a.count + 16.0f) + 2.0f * far) * 0x1p-24f;
+    const int64_t first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.n);
+    for (int64_t row0 = first + warp * 32; row0 < last; row0 += RT_WARPS * 32) {
+        const int64_t row = row0 + lane;
+        const bool live = row < last;
+        __syncwarp();
+        rt_bring<T>(a, row0, tile, pitch, wide);
+        __syncwarp();
+        int chosen[MOST];
+        float top = -INFINITY, sum = 0.0f;
+        bool odd = false;
+        if (live) {
+            for (int e = 0; e < a.count; e++) {
+                top = fmaxf(top, l[e]);
+                odd = odd || isnan(l[e]);
+            }
+            odd = odd || top == INFINITY;
+            if (!a.sigmoid && (!a.renormalize || !plain))
+                for (int e = 0; e < a.count; e++) sum += l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
+        }
+        if (plain) {
+            uint32_t order[MOST];
+#pragma unroll
+            for (int j = 0; j < MOST; j++) {
+                order[j] = 0;
+                chosen[j] = -1;
+            }
+            if (live)
+                for (int e = 0; e < a.count; e++) {
+                    const uint32_t k = rt_order(l[e]);
+                    if (k <= order[MOST - 1]) continue;
+#pragma unroll
+                    for (int j = MOST - 1; j >= 0; j--) {
+                        if (k <= order[j]) continue;
+                        if (j + 1 < MOST) {
+                            order[j + 1] = order[j];
+                            chosen[j + 1] = chosen[j];
+                        }
+                        order[j] = k;
+                        chosen[j] = e;
+                    }
+                }
+        } else {
+            uint32_t order[MOST];
+            if (live && !rt_choose<float, MOST>(a, l, bias, top, sum, near, chosen, order)) {
+                double exact = 0.0;
+                if (!a.sigmoid)
+                    for (int e = 0; e < a.count; e++) exact += l[e] == -INFINITY ? 0.0 : exp((double)l[e] - (double)top);
+                uint64_t order64[MOST];
+                (void)rt_choose<double, MOST>(a, l, bias, top, exact, 0.0, chosen, order64);
+            }
+        }
+        if (live) {
+            float w[MOST], most = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int j = 0; j < MOST; j++) {
+                const bool have = j < a.choices && chosen[j] >= 0;
+                const float v = have ? l[chosen[j]] : 0.0f;
+                // log s up to what all share; sums of exponentials below the largest
+                w[j] = !a.sigmoid || !a.renormalize ? v : isnan(v) ? v : fminf(v, 0.0f) - log1pf(expf(-fabsf(v)));
+                if (have) most = fmaxf(most, w[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < MOST; j++) {
+                if (j >= a.choices || chosen[j] < 0) continue;
+                if (a.renormalize) {
+                    w[j] = expf(w[j] - most);
+                    total += w[j];
+                } else {
+                    w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-w[j])) : expf(w[j] - top) / sum;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < MOST; j++) {
+                if (j >= a.choices) continue;
+                float v = chosen[j] < 0 ? 0.0f : a.renormalize ? w[j] / total : w[j];
+                if (!a.sigmoid && odd && chosen[j] >= 0) v = NAN;   // a NaN or +inf anywhere leaves no score of the row a number
+                a.experts[row * a.choices + j] = chosen[j];
+                a.weights[row * a.choices + j] = chosen[j] < 0 ? 0.0f : a.scale * v;
+                atomicAdd(counts + (chosen[j] < 0 ? a.count : chosen[j]), 1);
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= a.count; i += RT_WARPS * 32) a.counts[(int64_t)i * gridDim.x + blockIdx.x] = counts[i];
 }
 
 // Counts of an expert (blockIdx.x) over the blocks become the pairs of it before each block; their sum.
@@ -339,12 +575,87 @@ re_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits)
     }
 }
 
+// The same, a thread a row (see rt_choose_kernel): the gradients of 32 rows are put together in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(RT_WARPS * 32)
+rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitch, int wide, int wide_out)
+{
+    extern __shared__ unsigned char raw_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+    float* const tile = reinterpret_cast<float*>(raw_smem) + warp * 32 * pitch;
+    float* const l = tile + lane * pitch;
+    const bool dense = !a.sigmoid && !a.renormalize;   // every logit has a gradient
+    for (int64_t row0 = ((int64_t)blockIdx.x * RT_WARPS + warp) * 32; row0 < a.n; row0 += (int64_t)gridDim.x * RT_WARPS * 32) {
+        const int64_t row = row0 + lane;
+        __syncwarp();
+        if (dense) rt_bring<T>(a, row0, tile, pitch, wide);
+        else
+            for (int i = lane; i < 32 * pitch; i += 32) tile[i] = 0.0f;
+        __syncwarp();
+        if (row < a.n) {
+            const int32_t* const es = a.experts + row * a.choices;
+            const float *const ws = a.weights + row * a.choices, *const gs = d_weights + row * a.choices;
+            float dot = 0.0f;
+            for (int j = 0; j < a.choices; j++)
+                if ((uint32_t)es[j] < (uint32_t)a.count) dot = fmaf(ws[j] / a.scale, gs[j] * a.scale, dot);
+            if (dense) {
+                float top = -INFINITY, sum = 0.0f;
+                for (int e = 0; e < a.count; e++) top = fmaxf(top, l[e]);
+                for (int e = 0; e < a.count; e++) {
+                    l[e] = l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
+                    sum += l[e];
+                }
+                const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
+                float add[RT_MAX_CHOICES];
+#pragma unroll
+                for (int j = 0; j < RT_MAX_CHOICES; j++) add[j] = j < a.choices && (uint32_t)es[j] < (uint32_t)a.count ? l[es[j]] * over * (gs[j] * a.scale - dot) : 0.0f;
+                for (int e = 0; e < a.count; e++) l[e] = l[e] * over * -dot;
+#pragma unroll
+                for (int j = 0; j < RT_MAX_CHOICES; j++)
+                    if (j < a.choices && (uint32_t)es[j] < (uint32_t)a.count) l[es[j]] = add[j];
+            } else {
+                for (int j = 0; j < a.choices; j++) {
+                    const int e = es[j];
+                    if ((uint32_t)e >= (uint32_t)a.count) continue;
+                    const float w = ws[j] / a.scale, g = gs[j] * a.scale;
+                    const float s = a.sigmoid ? 1.0f / (1.0f + expf(-tl_get(static_cast<const T*>(a.logits) + row * a.row + e))) : 0.0f;
+                    l[e] = a.renormalize ? w * (g - dot) * (1.0f - s) : g * s * (1.0f - s);
+                }
+            }
+        }
+        __syncwarp();
+        constexpr int N = 16 / (int)sizeof(T);
+        if (wide_out) {
+            const int per = a.count / N;
+            for (int u = lane; u < 32 * per; u += 32) {
+                const int r = u / per, c = (u % per) * N;
+                if (row0 + r >= a.n) break;
+                uint4 v;
+                T* const e = reinterpret_cast<T*>(&v);
+#pragma unroll
+                for (int i = 0; i < N; i++) tl_put(e + i, tile[r * pitch + c + i]);
+                *reinterpret_cast<uint4*>(d_logits + (row0 + r) * a.count + c) = v;
+            }
+        } else {
+            for (int u = lane; u < 32 * a.count; u += 32) {
+                const int r = u / a.count, c = u % a.count;
+                if (row0 + r >= a.n) break;
+                tl_put(d_logits + (row0 + r) * a.count + c, tile[r * pitch + c]);
+            }
+        }
+    }
+}
+
 struct ReLayout { int64_t chunk, blocks, counts, sums, total; };
-static ReLayout re_layout(int64_t n, int count)
+// Whether a thread takes a row.
+static bool rt_takes(const ReArgs& a) { return a.count <= RT_MAX_EXPERTS && a.choices <= RT_MAX_CHOICES && a.groups <= RT_MAX_GROUPS; }
+static ReLayout re_layout(const ReArgs& a)
 {
     ReLayout l;
-    const int64_t most = (int64_t)sm_count_cached() * 4;
-    l.chunk = std::max<int64_t>(RE_WARPS, (n + most - 1) / most);
+    const int64_t n = a.n;
+    const int count = a.count;
+    const int64_t most = (int64_t)sm_count_cached() * 4, least = rt_takes(a) ? RT_WARPS * 32 : RE_WARPS;
+    l.chunk = std::max<int64_t>(least, ((n + most - 1) / most + least - 1) / least * least);
     l.blocks = std::max<int64_t>(1, (n + l.chunk - 1) / l.chunk);
     l.counts = 0;
     l.sums = align_up(4 * l.blocks * (count + 1), 256);
@@ -371,9 +682,20 @@ static int re_args(const dynb_routing* in, ReArgs* a)
     return DYNB_OK;
 }
 
+// Rows of `row` elements may be read, or written, by pieces of 16 bytes.
+static bool re_wide(const void* p, int64_t row, int count, int size) { return starts_on(p, 16) && row * size % 16 == 0 && count * size % 16 == 0; }
+
 template <typename T>
 static cudaError_t re_choose(const ReArgs& a, unsigned blocks, cudaStream_t s)
 {
+    if (rt_takes(a)) {
+        const int pitch = a.count | 1, smem = (2 * a.count + 1 + RT_WARPS * 32 * pitch) * 4;
+        void (*const kernel)(ReArgs, int, int) = a.choices <= 2 ? rt_choose_kernel<T, 4> : a.choices <= 4 ? rt_choose_kernel<T, 6> : rt_choose_kernel<T, 10>;
+        const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+        if (rc != cudaSuccess) return rc;
+        kernel<<<blocks, RT_WARPS * 32, smem, s>>>(a, pitch, re_wide(a.logits, a.row, a.count, sizeof(T)));
+        return cudaGetLastError();
+    }
     const int smem = ((a.count + 1) * 4 + 15) / 16 * 16 + (a.groups > 1 ? RE_WARPS * (a.count + a.groups) * 8 : 0);
     void (*kernel)(ReArgs) = a.count <= 32 ? re_choose_kernel<T, 1> : a.count <= 64 ? re_choose_kernel<T, 2> : a.count <= 128 ? re_choose_kernel<T, 4> :
                              a.count <= 256 ? re_choose_kernel<T, 8> : a.count <= 512 ? re_choose_kernel<T, 16> : re_choose_kernel<T, 32>;
@@ -386,6 +708,15 @@ static cudaError_t re_choose(const ReArgs& a, unsigned blocks, cudaStream_t s)
 template <typename T>
 static cudaError_t re_backward(const ReArgs& a, const float* d_weights, void* d_logits, cudaStream_t s)
 {
+    if (rt_takes(a)) {
+        const int pitch = a.count | 1, smem = RT_WARPS * 32 * pitch * 4;
+        const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(rt_backward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+        if (rc != cudaSuccess) return rc;
+        const unsigned blocks = (unsigned)std::min<int64_t>((a.n + RT_WARPS * 32 - 1) / (RT_WARPS * 32), (int64_t)sm_count_cached() * 16);
+        rt_backward_kernel<T><<<blocks, RT_WARPS * 32, smem, s>>>(a, d_weights, static_cast<T*>(d_logits), pitch, re_wide(a.logits, a.row, a.count, sizeof(T)),
+                                                                  re_wide(d_logits, a.count, a.count, sizeof(T)));
+        return cudaGetLastError();
+    }
     void (*kernel)(ReArgs, const float*, T*) = a.count <= 32 ? re_backward_kernel<T, 1> : a.count <= 64 ? re_backward_kernel<T, 2> : a.count <= 128 ? re_backward_kernel<T, 4> :
                                                a.count <= 256 ? re_backward_kernel<T, 8> : a.count <= 512 ? re_backward_kernel<T, 16> : re_backward_kernel<T, 32>;
     const unsigned blocks = (unsigned)std::min<int64_t>((a.n + RE_WARPS - 1) / RE_WARPS, (int64_t)sm_count_cached() * 8);
@@ -403,7 +734,7 @@ extern "C" int dynb_route_experts_workspace_bytes(const dynb_routing* args, int6
     const int rc = re_args(args, &a);
     if (rc != DYNB_OK) return rc;
     if (bytes == nullptr) return fail_arg("null pointer");
-    *bytes = re_layout(a.n, a.count).total;
+    *bytes = re_layout(a).total;
     return DYNB_OK;
 }
 
@@ -415,7 +746,7 @@ extern "C" int dynb_route_experts(const dynb_routing* args, int32_t* experts_dev
     if (rc != DYNB_OK) return rc;
     if (!start_dev || !workspace_dev || (a.n > 0 && (!a.logits || !experts_dev || !weights_dev || !order_dev))) return fail_arg("null pointer");
     if (!starts_on(workspace_dev, 4)) return fail_arg("route_experts: the workspace must start on a 4-byte boundary");
-    const ReLayout l = re_layout(a.n, a.count);
+    const ReLayout l = re_layout(a);
     if (workspace_bytes < l.total) return fail_arg("workspace too small");
     unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
     a.experts = experts_dev; a.weights = weights_dev; a.order = order_dev; a.start = start_dev; a.chunk = l.chunk;

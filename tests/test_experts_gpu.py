@@ -225,6 +225,20 @@ def test_route_extremes(cuda):
     assert torch.equal(D.route_experts(row, 3).experts, D.route_experts(row.contiguous(), 3).experts)
 
 
+@pytest.mark.parametrize("experts", [8, 64, 200])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_route_close_and_equal_keys(cuda, experts, groups):
+    """Keys that 32 bits cannot tell apart, equal ones, and zeros of both signs: chosen as 64 bits choose, the lowest number first among equal ones."""
+    gen = _gen(experts)
+    logits = torch.randint(-2, 3, (600, experts), generator=gen, device="cuda").float() * 2.0 ** -20      # sigmoids 2^-22 apart, many of them equal
+    logits[::3] = 0.0
+    logits[::3][torch.rand(200, experts, generator=gen, device="cuda") < 0.5] *= -1.0
+    bias = torch.randint(-3, 4, (experts,), generator=gen, device="cuda").float() * 2.0 ** -23
+    for score in ("softmax", "sigmoid"):
+        for b in (None, bias, 1000 * bias + 0.5):
+            _compare_route(logits, 5, score=score, groups=groups, kept_groups=(groups + 1) // 2, bias=b)
+
+
 def test_route_numbers_that_are_none(cuda):
     """A NaN comes first, its row's weights are NaN (sigmoids without sums: its own alone), other rows are as they were; every number stays in range."""
     logits = _normal(_gen(8), 9, 8)
