@@ -204,9 +204,6 @@ __device__ __forceinline__ double rt_value(uint64_t order) { return order == ~0u
 template <typename K> struct RtOrder { using type = uint32_t; };
 template <> struct RtOrder<double> { using type = uint64_t; };
 
-__device__ __forceinline__ float rt_exp(float v) { return expf(v); }
-__device__ __forceinline__ double rt_exp(double v) { return exp(v); }
-
 // 32 rows from `row0` on to `tile` (`pitch` floats a row), rows behind the last as zeros.
 template <typename T>
 __device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* tile, int pitch, int wide)
@@ -233,17 +230,29 @@ __device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* t
     }
 }
 
-// The experts of a lane's row by keys of type K; MOST: choices and two more, the first that are left out.  False: rounding of the keys may have decided.
-template <typename K, int MOST>
-__device__ __forceinline__ bool rt_choose(const ReArgs& a, const float* l, const float* bias, float top, K sum, K near, int (&chosen)[MOST], typename RtOrder<K>::type (&order)[MOST])
+// Puts key k of expert e where it belongs among the largest: behind those that are equal.
+template <typename O, int MOST>
+__device__ __forceinline__ void rt_insert(O k, int e, int (&chosen)[MOST], O (&order)[MOST])
+{
+    if (k <= order[MOST - 1]) return;
+#pragma unroll
+    for (int j = MOST - 1; j >= 0; j--) {
+        if (k <= order[j]) continue;
+        if (j + 1 < MOST) {
+            order[j + 1] = order[j];
+            chosen[j + 1] = chosen[j];
+        }
+        order[j] = k;
+        chosen[j] = e;
+    }
+}
+
+// The experts of a lane's row.  key_of(e): keys of type K in their order, as often as asked; MOST: choices and two more, the first that are left out.  False: keys
+// that are off by up to `near` may have decided.  same(p, q): two experts have the same logit and bias, and so the same key, whatever its type.
+template <typename K, int MOST, typename Key, typename Same>
+__device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)[MOST], Key&& key_of, Same&& same)
 {
     using O = typename RtOrder<K>::type;
-    auto key_of = [&](int e) -> O {
-        const float v = l[e];
-        if (v == -INFINITY) return 0;
-        const K s = a.sigmoid ? (K)1 / ((K)1 + rt_exp(-(K)v)) : rt_exp((K)v - (K)top) / sum;
-        return rt_order(s + (K)bias[e]);
-    };
     bool sure = true;
     uint32_t kept = 0xffffffffu;
     const int per = a.count / a.groups;
@@ -254,6 +263,7 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, const float* l, const
             of_group[g] = 0;
             if (g >= a.groups) continue;
             O one = 0, two = 0;
+#pragma unroll 4
             for (int i = 0; i < per; i++) {
                 const O k = key_of(g * per + i);
                 two = max(two, min(one, k));
@@ -282,6 +292,7 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, const float* l, const
         }
         if (highest != 0) sure = rt_value(lowest) - rt_value(highest) > (K)6 * near;
     }
+    O order[MOST];
 #pragma unroll
     for (int j = 0; j < MOST; j++) {
         order[j] = 0;
@@ -289,35 +300,43 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, const float* l, const
     }
     for (int g = 0; g < a.groups; g++) {
         if (!(kept >> (g & 31) & 1)) continue;
-        for (int i = 0; i < per; i++) {
-            const O k = key_of(g * per + i);
-            if (k <= order[MOST - 1]) continue;
-#pragma unroll
-            for (int j = MOST - 1; j >= 0; j--) {
-                if (k <= order[j]) continue;
-                if (j + 1 < MOST) {
-                    order[j + 1] = order[j];
-                    chosen[j + 1] = chosen[j];
-                }
-                order[j] = k;
-                chosen[j] = g * per + i;
-            }
-        }
+#pragma unroll 4
+        for (int i = 0; i < per; i++) rt_insert(key_of(g * per + i), g * per + i, chosen, order);
     }
-    bool tie = false;   // the last choice and the first that is left out have the same key, whatever its type
+    bool tie = false;   // the last choice and the first that is left out have the same key
 #pragma unroll
     for (int j = 0; j + 1 < MOST; j++) {
         if (order[j + 1] == 0 || j > a.choices || (j == a.choices && !tie)) continue;
         if (rt_value(order[j]) - rt_value(order[j + 1]) > (K)2 * near) continue;
-        const int p = chosen[j], q = chosen[j + 1];
         tie = j == a.choices - 1;
-        if (j == a.choices || !(l[p] == l[q] && bias[p] == bias[q])) sure = false;
+        if (j == a.choices || !same(chosen[j], chosen[j + 1])) sure = false;
     }
     return sure;
 }
 
+// A row once more in 64 bits.
 template <typename T, int MOST>
-__global__ void __launch_bounds__(RT_WARPS * 32)
+__device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, const float* bias, float top, int* out)
+{
+    const T* const l = static_cast<const T*>(a.logits) + row * a.row;
+    double sum = 0.0;
+    if (!a.sigmoid)
+        for (int e = 0; e < a.count; e++) sum += tl_get(l + e) == -INFINITY ? 0.0 : exp((double)tl_get(l + e) - (double)top);
+    int chosen[MOST];
+    (void)rt_choose<double, MOST>(
+        a, 0.0, chosen,
+        [&](int e) -> uint64_t {
+            const double v = (double)tl_get(l + e);
+            if (v == -INFINITY) return 0;
+            return re_order((a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / sum) + (double)bias[e]);
+        },
+        [](int, int) { return true; });
+    for (int j = 0; j < a.choices; j++) out[j] = chosen[j];
+}
+
+// PLAIN: the logits decide.
+template <typename T, int MOST, bool PLAIN>
+__global__ void __launch_bounds__(RT_WARPS * 32, PLAIN ? 12 : 8)
 rt_choose_kernel(const ReArgs a, int pitch, int wide)
 {
     extern __shared__ unsigned char raw_smem[];
@@ -325,13 +344,12 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
     float* const bias = reinterpret_cast<float*>(counts + a.count + 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     float* const tile = bias + a.count + warp * 32 * pitch;
-    const float* const l = tile + lane * pitch;
-    const bool plain = a.bias == nullptr && a.groups == 1;   // the logits decide
+    float* const l = tile + lane * pitch;
     float far = 0.0f;
     for (int i = threadIdx.x; i <= a.count; i += RT_WARPS * 32) counts[i] = 0;
     for (int i = threadIdx.x; i < a.count; i += RT_WARPS * 32) bias[i] = a.bias != nullptr ? a.bias[i] : 0.0f;
     __syncthreads();
-    if (!plain)
+    if constexpr (!PLAIN)
         for (int i = lane; i < a.count; i += 32) far = fmaxf(far, isinf(bias[i]) ? 0.0f : fabsf(bias[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) far = fmaxf(far, __shfl_xor_sync(0xffffffffu, far, o));
@@ -340,83 +358,93 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
     const int64_t first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.n);
     for (int64_t row0 = first + warp * 32; row0 < last; row0 += RT_WARPS * 32) {
         const int64_t row = row0 + lane;
-        const bool live = row < last;
         __syncwarp();
         rt_bring<T>(a, row0, tile, pitch, wide);
         __syncwarp();
+        if (row >= last) continue;
         int chosen[MOST];
         float top = -INFINITY, sum = 0.0f;
         bool odd = false;
-        if (live) {
-            for (int e = 0; e < a.count; e++) {
-                top = fmaxf(top, l[e]);
-                odd = odd || isnan(l[e]);
-            }
-            odd = odd || top == INFINITY;
-            if (!a.sigmoid && (!a.renormalize || !plain))
-                for (int e = 0; e < a.count; e++) sum += l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
-        }
-        if (plain) {
+        if constexpr (PLAIN) {
             uint32_t order[MOST];
 #pragma unroll
             for (int j = 0; j < MOST; j++) {
                 order[j] = 0;
                 chosen[j] = -1;
             }
-            if (live)
-                for (int e = 0; e < a.count; e++) {
-                    const uint32_t k = rt_order(l[e]);
-                    if (k <= order[MOST - 1]) continue;
-#pragma unroll
-                    for (int j = MOST - 1; j >= 0; j--) {
-                        if (k <= order[j]) continue;
-                        if (j + 1 < MOST) {
-                            order[j + 1] = order[j];
-                            chosen[j + 1] = chosen[j];
-                        }
-                        order[j] = k;
-                        chosen[j] = e;
-                    }
-                }
+#pragma unroll 4
+            for (int e = 0; e < a.count; e++) {
+                const float v = l[e];
+                top = fmaxf(top, v);
+                odd = odd || isnan(v);
+                rt_insert(rt_order(v), e, chosen, order);
+            }
+            if (!a.sigmoid && !a.renormalize) {
+#pragma unroll 4
+                for (int e = 0; e < a.count; e++) sum += l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
+            }
         } else {
-            uint32_t order[MOST];
-            if (live && !rt_choose<float, MOST>(a, l, bias, top, sum, near, chosen, order)) {
-                double exact = 0.0;
-                if (!a.sigmoid)
-                    for (int e = 0; e < a.count; e++) exact += l[e] == -INFINITY ? 0.0 : exp((double)l[e] - (double)top);
-                uint64_t order64[MOST];
-                (void)rt_choose<double, MOST>(a, l, bias, top, exact, 0.0, chosen, order64);
+            // logits give way to their keys
+            if (!a.sigmoid) {
+#pragma unroll 4
+                for (int e = 0; e < a.count; e++) {
+                    top = fmaxf(top, l[e]);
+                    odd = odd || isnan(l[e]);
+                }
+#pragma unroll 4
+                for (int e = 0; e < a.count; e++) {
+                    const float v = l[e] == -INFINITY ? -1.0f : expf(l[e] - top);
+                    sum += fmaxf(v, 0.0f) + (v - v);   // a NaN stays one
+                    l[e] = v;
+                }
+            }
+            const float over = 1.0f / sum;
+#pragma unroll 4
+            for (int e = 0; e < a.count; e++) {
+                const float v = l[e];
+                const float key = a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-v)) : v * over;
+                const bool closed = a.sigmoid ? v == -INFINITY : v < 0.0f;
+                l[e] = __uint_as_float(closed ? 0u : rt_order(key + bias[e]));
+            }
+            const T* const from = static_cast<const T*>(a.logits) + row * a.row;
+            if (!rt_choose<float, MOST>(
+                    a, near, chosen, [&](int e) { return __float_as_uint(l[e]); },
+                    [&](int p, int q) { return tl_get(from + p) == tl_get(from + q) && bias[p] == bias[q]; })) {
+                int again[MOST];   // on the way through memory, as `chosen` must not be
+                rt_again<T, MOST>(a, row, bias, top, again);
+#pragma unroll
+                for (int j = 0; j < MOST; j++) chosen[j] = j < a.choices ? again[j] : -1;
             }
         }
-        if (live) {
-            float w[MOST], most = -INFINITY, total = 0.0f;
+        odd = odd || top == INFINITY;
+        const T* const from = static_cast<const T*>(a.logits) + row * a.row;
+        float w[MOST], most = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int j = 0; j < MOST; j++) {
-                const bool have = j < a.choices && chosen[j] >= 0;
-                const float v = have ? l[chosen[j]] : 0.0f;
-                // log s up to what all share; sums of exponentials below the largest
-                w[j] = !a.sigmoid || !a.renormalize ? v : isnan(v) ? v : fminf(v, 0.0f) - log1pf(expf(-fabsf(v)));
-                if (have) most = fmaxf(most, w[j]);
-            }
+        for (int j = 0; j < MOST; j++) {
+            const bool have = j < a.choices && chosen[j] >= 0;
+            const float v = have ? (PLAIN ? l[chosen[j]] : tl_get(from + chosen[j])) : 0.0f;
+            // log s up to what all share; sums of exponentials below the largest
+            w[j] = !a.sigmoid || !a.renormalize ? v : isnan(v) ? v : fminf(v, 0.0f) - log1pf(expf(-fabsf(v)));
+            if (have) most = fmaxf(most, w[j]);
+        }
 #pragma unroll
-            for (int j = 0; j < MOST; j++) {
-                if (j >= a.choices || chosen[j] < 0) continue;
-                if (a.renormalize) {
-                    w[j] = expf(w[j] - most);
-                    total += w[j];
-                } else {
-                    w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-w[j])) : expf(w[j] - top) / sum;
-                }
+        for (int j = 0; j < MOST; j++) {
+            if (j >= a.choices || chosen[j] < 0) continue;
+            if (a.renormalize) {
+                w[j] = expf(w[j] - most);
+                total += w[j];
+            } else {
+                w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-w[j])) : expf(w[j] - top) / sum;
             }
+        }
 #pragma unroll
-            for (int j = 0; j < MOST; j++) {
-                if (j >= a.choices) continue;
-                float v = chosen[j] < 0 ? 0.0f : a.renormalize ? w[j] / total : w[j];
-                if (!a.sigmoid && odd && chosen[j] >= 0) v = NAN;   // a NaN or +inf anywhere leaves no score of the row a number
-                a.experts[row * a.choices + j] = chosen[j];
-                a.weights[row * a.choices + j] = chosen[j] < 0 ? 0.0f : a.scale * v;
-                atomicAdd(counts + (chosen[j] < 0 ? a.count : chosen[j]), 1);
-            }
+        for (int j = 0; j < MOST; j++) {
+            if (j >= a.choices) continue;
+            float v = chosen[j] < 0 ? 0.0f : a.renormalize ? w[j] / total : w[j];
+            if (!a.sigmoid && odd && chosen[j] >= 0) v = NAN;   // a NaN or +inf anywhere leaves no score of the row a number
+            a.experts[row * a.choices + j] = chosen[j];
+            a.weights[row * a.choices + j] = chosen[j] < 0 ? 0.0f : a.scale * v;
+            atomicAdd(counts + (chosen[j] < 0 ? a.count : chosen[j]), 1);
         }
     }
     __syncthreads();
@@ -600,7 +628,9 @@ rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitc
                 if ((uint32_t)es[j] < (uint32_t)a.count) dot = fmaf(ws[j] / a.scale, gs[j] * a.scale, dot);
             if (dense) {
                 float top = -INFINITY, sum = 0.0f;
+#pragma unroll 8
                 for (int e = 0; e < a.count; e++) top = fmaxf(top, l[e]);
+#pragma unroll 4
                 for (int e = 0; e < a.count; e++) {
                     l[e] = l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
                     sum += l[e];
@@ -609,6 +639,7 @@ rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitc
                 float add[RT_MAX_CHOICES];
 #pragma unroll
                 for (int j = 0; j < RT_MAX_CHOICES; j++) add[j] = j < a.choices && (uint32_t)es[j] < (uint32_t)a.count ? l[es[j]] * over * (gs[j] * a.scale - dot) : 0.0f;
+#pragma unroll 8
                 for (int e = 0; e < a.count; e++) l[e] = l[e] * over * -dot;
 #pragma unroll
                 for (int j = 0; j < RT_MAX_CHOICES; j++)
@@ -654,7 +685,7 @@ static ReLayout re_layout(const ReArgs& a)
     ReLayout l;
     const int64_t n = a.n;
     const int count = a.count;
-    const int64_t most = (int64_t)sm_count_cached() * 4, least = rt_takes(a) ? RT_WARPS * 32 : RE_WARPS;
+    const int64_t most = (int64_t)sm_count_cached() * (rt_takes(a) ? 16 : 4), least = rt_takes(a) ? RT_WARPS * 32 : RE_WARPS;   // blocks
     l.chunk = std::max<int64_t>(least, ((n + most - 1) / most + least - 1) / least * least);
     l.blocks = std::max<int64_t>(1, (n + l.chunk - 1) / l.chunk);
     l.counts = 0;
@@ -682,6 +713,14 @@ static int re_args(const dynb_routing* in, ReArgs* a)
     return DYNB_OK;
 }
 
+// As few places in the list as the choices need: a longer one is entered more often (six choices with ten places 182 us, eight 161).
+template <typename T, bool PLAIN>
+static void (*rt_kernel(int choices))(ReArgs, int, int)
+{
+    return choices <= 1 ? rt_choose_kernel<T, 3, PLAIN> : choices <= 2 ? rt_choose_kernel<T, 4, PLAIN> : choices <= 4 ? rt_choose_kernel<T, 6, PLAIN> :
+           choices <= 6 ? rt_choose_kernel<T, 8, PLAIN> : rt_choose_kernel<T, 10, PLAIN>;
+}
+
 // Rows of `row` elements may be read, or written, by pieces of 16 bytes.
 static bool re_wide(const void* p, int64_t row, int count, int size) { return starts_on(p, 16) && row * size % 16 == 0 && count * size % 16 == 0; }
 
@@ -690,7 +729,7 @@ static cudaError_t re_choose(const ReArgs& a, unsigned blocks, cudaStream_t s)
 {
     if (rt_takes(a)) {
         const int pitch = a.count | 1, smem = (2 * a.count + 1 + RT_WARPS * 32 * pitch) * 4;
-        void (*const kernel)(ReArgs, int, int) = a.choices <= 2 ? rt_choose_kernel<T, 4> : a.choices <= 4 ? rt_choose_kernel<T, 6> : rt_choose_kernel<T, 10>;
+        void (*const kernel)(ReArgs, int, int) = a.bias == nullptr && a.groups == 1 ? rt_kernel<T, true>(a.choices) : rt_kernel<T, false>(a.choices);
         const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
         if (rc != cudaSuccess) return rc;
         kernel<<<blocks, RT_WARPS * 32, smem, s>>>(a, pitch, re_wide(a.logits, a.row, a.count, sizeof(T)));
