@@ -3,8 +3,9 @@
 // of 2 pi wave_p . pos_i.  Pairs are (p, p + dim / 2), or (2 p, 2 p + 1).
 //     back:  dn = the gradient turned back;  dg = sum dn x r;  dx = r (g dn - x r^2 mean(g dn x));  dpos_i = 2 pi sum over pairs of wave_p
 //     times the sum over the heads of q and k of (dn_b n_a - dn_a n_b).
-// A warp takes whole rows: a head's pairs lie over 1 to 32 lanes, so its sums are a few exchanges, and what a row's heads share (cosines, sines and the
-// gradient of the position) stays in the warp.  Turns are in 64 bits, whole ones are dropped, and what is left goes to 32 bits.
+// A head's pairs lie over 1 to 32 lanes, and these lanes take the heads of a row one after the other: what the heads share (cosines, sines and the gradient of the
+// position) stays in their registers, every cosine is formed once, and the norms' sums are a few exchanges.  Where there are few rows, the heads of one are
+// shared out among several such groups.  Turns are in 64 bits, whole ones are dropped, and what is left goes to 32 bits.
 
 #include <algorithm>
 
@@ -28,7 +29,7 @@ struct RhArgs {
     void* d_pos;
     float* partial;              // [blocks][2][dim]: sums for the weights
     int64_t rows;
-    int half, axes, pos64, norm, per_head;   // per_head: lanes of a head
+    int half, axes, pos64, norm, per_head, shares;   // per_head: lanes of a head; shares: groups of them that share the heads of a row
     float eps;
 };
 
@@ -82,11 +83,13 @@ __device__ __forceinline__ void rh_store(T* at, int p0, int half, const float (&
     }
 }
 
-__device__ __forceinline__ float rh_sum(float v, int lanes)
+// Sum over neighbouring lanes, a power of two of them, all of which call it.
+__device__ __forceinline__ float rh_sum(float v, int lanes, uint32_t mask)
 {
-    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor_sync(mask, v, o);
     return v;
 }
+__device__ __forceinline__ uint32_t rh_mask(int lanes) { return lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << ((threadIdx.x & 31) & ~(lanes - 1)); }
 
 // Cosine and sine of pair p of row i.
 __device__ __forceinline__ float2 rh_turn(const RhArgs& a, int64_t i, int p)
@@ -106,121 +109,122 @@ template <typename T, int VP, int PIECES, bool MIXED, bool BACK>
 __global__ void __launch_bounds__(RH_WARPS * 32)
 rh_kernel(const RhArgs a)
 {
-    __shared__ float2 turn_of[RH_WARPS][RH_MAX_HALF];
-    __shared__ float wave[RH_MAX_HALF * RH_MAX_AXES];
+    __shared__ __align__(16) float weight[2][2][RH_MAX_HALF];   // of the first and of the second elements of the pairs
+    __shared__ float wave[BACK ? RH_MAX_HALF * RH_MAX_AXES : 1];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = a.half, dim = 2 * half;
-    if constexpr (BACK) {
-        for (int i = threadIdx.x; i < half * a.axes; i += RH_WARPS * 32) wave[i] = a.wave[i];
-        __syncthreads();
+    for (int i = threadIdx.x; i < 2 * dim; i += RH_WARPS * 32) {
+        const int s = i / dim, at = i % dim;
+        const float v = a.side[s].weight != nullptr ? a.side[s].weight[at] : 1.0f;
+        weight[s][MIXED ? at % 2 : at / half][MIXED ? at / 2 : at % half] = v;
     }
-    float2* const turns = turn_of[warp];
-    const int in_head = lane & (a.per_head - 1), group = lane / a.per_head, groups = 32 / a.per_head;
-    const int batch = half <= 32 ? 32 / half : 1;         // rows whose cosines a warp computes at a time
-    float ga[2][PIECES][VP], gb[2][PIECES][VP];           // the norms' weights, and sums for their gradients
-    float sa[2][PIECES][VP], sb[2][PIECES][VP];
+    if constexpr (BACK)
+        for (int i = threadIdx.x; i < half * a.axes; i += RH_WARPS * 32) wave[i] = a.wave[i];
+    __syncthreads();
+    const int per_row = a.per_head * a.shares, in_head = lane & (a.per_head - 1), share = (lane & (per_row - 1)) / a.per_head, rows_here = 32 / per_row;
+    const uint32_t head_mask = rh_mask(a.per_head), row_mask = rh_mask(per_row);
+    const float over_dim = 1.0f / (float)dim;
+    float sa[2][PIECES][VP], sb[2][PIECES][VP];                  // sums for the weights' gradients
+    if constexpr (BACK) {
 #pragma unroll
-    for (int s = 0; s < 2; s++)
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int c = 0; c < PIECES; c++)
+#pragma unroll
+                for (int i = 0; i < VP; i++) sa[s][c][i] = sb[s][c][i] = 0.0f;
+    }
+    for (int64_t row = ((int64_t)blockIdx.x * RH_WARPS + warp) * rows_here + lane / per_row; row < a.rows; row += (int64_t)gridDim.x * RH_WARPS * rows_here) {
+        float2 cs[PIECES][VP];
+        float dtheta[PIECES][VP];
 #pragma unroll
         for (int c = 0; c < PIECES; c++)
 #pragma unroll
             for (int i = 0; i < VP; i++) {
                 const int p = (c * a.per_head + in_head) * VP + i;
-                const float* const w = a.side[s].weight;
-                ga[s][c][i] = w != nullptr && p < half ? w[MIXED ? 2 * p : p] : 1.0f;
-                gb[s][c][i] = w != nullptr && p < half ? w[MIXED ? 2 * p + 1 : half + p] : 1.0f;
-                sa[s][c][i] = sb[s][c][i] = 0.0f;
+                cs[c][i] = p < half ? rh_turn(a, row, p) : make_float2(1.0f, 0.0f);
+                dtheta[c][i] = 0.0f;
             }
-    const int units = a.side[0].heads + a.side[1].heads;
-    const int64_t warps = (int64_t)gridDim.x * RH_WARPS;
-    for (int64_t r0 = ((int64_t)blockIdx.x * RH_WARPS + warp) * batch; r0 < a.rows; r0 += warps * batch) {
-        const int here = (int)min((int64_t)batch, a.rows - r0);
-        __syncwarp();
-        for (int i = lane; i < here * half; i += 32) turns[i] = rh_turn(a, r0 + i / half, i % half);
-        __syncwarp();
-        for (int b = 0; b < here; b++) {
-            const int64_t row = r0 + b;
-            const int from = row < a.side[0].n ? 0 : a.side[0].heads;
-            float dtheta[PIECES][VP] = {};
-            for (int u0 = from; u0 < units; u0 += groups) {
-                const int u = u0 + group, s = u >= a.side[0].heads, h = s ? u - a.side[0].heads : u;
-                const RhSide& side = a.side[s];
-                const bool live = u < units && row < side.n;
-                const T* const x = static_cast<const T*>(side.x) + (live ? row * side.row + h * side.head : 0);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const RhSide& side = a.side[s];
+            if (row >= side.n) continue;
+            const T* const x = static_cast<const T*>(side.x) + row * side.row;
+            const T* const dy = static_cast<const T*>(side.dy) + row * side.dy_row;
+            T* const out = static_cast<T*>(side.out) + row * side.heads * dim;
+#pragma unroll 2
+            for (int h = share; h < side.heads; h += a.shares) {
                 float xa[PIECES][VP], xb[PIECES][VP], ya[PIECES][VP], yb[PIECES][VP];
                 float squares = 0.0f, dot = 0.0f;
 #pragma unroll
                 for (int c = 0; c < PIECES; c++) {
                     const int p = (c * a.per_head + in_head) * VP;
-                    const bool ok = live && p < half;
+                    if (p < half) {
+                        rh_load<T, VP, MIXED>(x + h * side.head, p, half, xa[c], xb[c]);
+                        if constexpr (BACK) rh_load<T, VP, MIXED>(dy + h * side.dy_head, p, half, ya[c], yb[c]);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < VP; i++) xa[c][i] = xb[c][i] = ya[c][i] = yb[c][i] = 0.0f;
-                    if (ok) rh_load<T, VP, MIXED>(x, p, half, xa[c], xb[c]);
-                    if constexpr (BACK) {
-                        if (ok) rh_load<T, VP, MIXED>(static_cast<const T*>(side.dy) + row * side.dy_row + h * side.dy_head, p, half, ya[c], yb[c]);
+                        for (int i = 0; i < VP; i++) xa[c][i] = xb[c][i] = ya[c][i] = yb[c][i] = 0.0f;
                     }
+                }
+#pragma unroll
+                for (int c = 0; c < PIECES; c++) {
+                    const int p = min((c * a.per_head + in_head) * VP, half - VP);
 #pragma unroll
                     for (int i = 0; i < VP; i++) {
                         squares = fmaf(xa[c][i], xa[c][i], fmaf(xb[c][i], xb[c][i], squares));
                         if constexpr (BACK) {
-                            const float2 cs = ok ? turns[b * half + p + i] : make_float2(1.0f, 0.0f);
-                            const float da = ya[c][i] * cs.x + yb[c][i] * cs.y, db = yb[c][i] * cs.x - ya[c][i] * cs.y;
+                            const float da = ya[c][i] * cs[c][i].x + yb[c][i] * cs[c][i].y, db = yb[c][i] * cs[c][i].x - ya[c][i] * cs[c][i].y;
                             ya[c][i] = da;
                             yb[c][i] = db;
-                            dot += (s ? ga[1][c][i] : ga[0][c][i]) * da * xa[c][i] + (s ? gb[1][c][i] : gb[0][c][i]) * db * xb[c][i];
+                            dot = fmaf(weight[s][0][p + i] * da, xa[c][i], fmaf(weight[s][1][p + i] * db, xb[c][i], dot));
                         }
                     }
                 }
                 float r = 1.0f, back = 0.0f;
                 if (a.norm) {
-                    r = 1.0f / sqrtf(rh_sum(squares, a.per_head) / (float)dim + a.eps);
-                    if constexpr (BACK) back = r * r * (rh_sum(dot, a.per_head) / (float)dim);
+                    r = 1.0f / sqrtf(rh_sum(squares, a.per_head, head_mask) * over_dim + a.eps);
+                    if constexpr (BACK) back = r * r * (rh_sum(dot, a.per_head, head_mask) * over_dim);
                 }
-                T* const out = static_cast<T*>(side.out);
 #pragma unroll
                 for (int c = 0; c < PIECES; c++) {
                     const int p = (c * a.per_head + in_head) * VP;
-                    if (!live || p >= half) continue;
+                    if (p >= half) continue;
                     float oa[VP], ob[VP];
 #pragma unroll
                     for (int i = 0; i < VP; i++) {
-                        const float wa = s ? ga[1][c][i] : ga[0][c][i], wb = s ? gb[1][c][i] : gb[0][c][i];
+                        const float wa = weight[s][0][p + i], wb = weight[s][1][p + i];
                         const float ua = xa[c][i] * r, ub = xb[c][i] * r;
                         if constexpr (BACK) {
                             dtheta[c][i] += yb[c][i] * (ua * wa) - ya[c][i] * (ub * wb);
-                            if (s) {
-                                sa[1][c][i] = fmaf(ya[c][i], ua, sa[1][c][i]);
-                                sb[1][c][i] = fmaf(yb[c][i], ub, sb[1][c][i]);
-                            } else {
-                                sa[0][c][i] = fmaf(ya[c][i], ua, sa[0][c][i]);
-                                sb[0][c][i] = fmaf(yb[c][i], ub, sb[0][c][i]);
-                            }
+                            sa[s][c][i] = fmaf(ya[c][i], ua, sa[s][c][i]);
+                            sb[s][c][i] = fmaf(yb[c][i], ub, sb[s][c][i]);
                             oa[i] = r * (wa * ya[c][i] - xa[c][i] * back);
                             ob[i] = r * (wb * yb[c][i] - xb[c][i] * back);
                         } else {
-                            const float2 cs = turns[b * half + p + i];
-                            oa[i] = ua * wa * cs.x - ub * wb * cs.y;
-                            ob[i] = ua * wa * cs.y + ub * wb * cs.x;
+                            const float na = ua * wa, nb = ub * wb;
+                            oa[i] = na * cs[c][i].x - nb * cs[c][i].y;
+                            ob[i] = na * cs[c][i].y + nb * cs[c][i].x;
                         }
                     }
-                    if (out != nullptr) rh_store<T, VP, MIXED>(out + (row * side.heads + h) * dim, p, half, oa, ob);
+                    if (side.out != nullptr) rh_store<T, VP, MIXED>(out + h * dim, p, half, oa, ob);
                 }
             }
-            if constexpr (BACK) {
-                if (a.d_pos != nullptr) {
-                    for (int x = 0; x < a.axes; x++) {
-                        float d = 0.0f;
+        }
+        if constexpr (BACK) {
+            if (a.d_pos != nullptr) {
+                for (int x = 0; x < a.axes; x++) {
+                    float d = 0.0f;
 #pragma unroll
-                        for (int c = 0; c < PIECES; c++)
+                    for (int c = 0; c < PIECES; c++)
 #pragma unroll
-                            for (int i = 0; i < VP; i++) {
-                                const int p = (c * a.per_head + in_head) * VP + i;
-                                if (p < half) d = fmaf(dtheta[c][i], wave[p * a.axes + x], d);
-                            }
-                        d = 6.2831853071795865f * rh_sum(d, 32);
-                        if (lane == 0) {
-                            if (a.pos64) static_cast<double*>(a.d_pos)[row * a.axes + x] = d;
-                            else static_cast<float*>(a.d_pos)[row * a.axes + x] = d;
+                        for (int i = 0; i < VP; i++) {
+                            const int p = (c * a.per_head + in_head) * VP + i;
+                            if (p < half) d = fmaf(dtheta[c][i], wave[p * a.axes + x], d);
                         }
+                    __syncwarp(row_mask);
+                    d = 6.2831853071795865f * rh_sum(d, per_row, row_mask);
+                    if ((lane & (per_row - 1)) == 0) {
+                        if (a.pos64) static_cast<double*>(a.d_pos)[row * a.axes + x] = d;
+                        else static_cast<float*>(a.d_pos)[row * a.axes + x] = d;
                     }
                 }
             }
@@ -230,6 +234,7 @@ rh_kernel(const RhArgs a)
         if (a.partial == nullptr) return;
         // the groups of a warp, then the warps of the block, in their order
         __shared__ float sums[RH_WARPS][2][2 * RH_MAX_HALF];
+        __syncwarp();
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
@@ -242,7 +247,7 @@ rh_kernel(const RhArgs a)
                         vb += __shfl_xor_sync(0xffffffffu, vb, o);
                     }
                     const int p = (c * a.per_head + in_head) * VP + i;
-                    if (group == 0 && p < half) {
+                    if (lane < a.per_head && p < half) {
                         sums[warp][s][MIXED ? 2 * p : p] = va;
                         sums[warp][s][MIXED ? 2 * p + 1 : half + p] = vb;
                     }
@@ -274,11 +279,11 @@ rh_join_kernel(const float* partial, int blocks, int dim, float* d_q_weight, flo
     if (to != nullptr) to[at % dim] = (float)(sums[0] + sums[1] + sums[2] + sums[3]);
 }
 
-static int rh_blocks(int64_t rows, int half)
+// Blocks for rows of `lanes` lanes each: no more than stay on the SMs together, as they leave a sum each.
+static int rh_blocks(int64_t rows, int lanes)
 {
-    const int batch = half <= 32 ? 32 / half : 1;
-    const int64_t need = (rows + (int64_t)batch * RH_WARPS - 1) / ((int64_t)batch * RH_WARPS);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)sm_count_cached() * 8));
+    const int64_t need = (rows * lanes + 32 * RH_WARPS - 1) / (32 * RH_WARPS);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)sm_count_cached() * 4));
 }
 
 static int rh_args(const dynb_rotary* in, RhArgs* a)
@@ -306,17 +311,21 @@ static int rh_args(const dynb_rotary* in, RhArgs* a)
 }
 
 template <typename T, int VP, int PIECES, bool BACK>
-static void rh_start(RhArgs& a, bool mixed, int blocks, cudaStream_t s)
+static int rh_start(RhArgs& a, bool mixed, cudaStream_t s)
 {
-    const int lanes = (a.half + VP - 1) / VP;
+    const int lanes = (a.half + VP - 1) / VP, heads = std::max(a.side[0].heads, a.side[1].heads);
     a.per_head = 1;
     while (a.per_head < lanes && a.per_head < 32) a.per_head *= 2;
+    a.shares = 1;
+    while (a.per_head * a.shares < 32 && a.shares < heads && a.rows * a.per_head * a.shares < (int64_t)sm_count_cached() * 1024) a.shares *= 2;
+    const int blocks = rh_blocks(a.rows, a.per_head * a.shares);
     if (mixed) rh_kernel<T, VP, PIECES, true, BACK><<<blocks, RH_WARPS * 32, 0, s>>>(a);
     else rh_kernel<T, VP, PIECES, false, BACK><<<blocks, RH_WARPS * 32, 0, s>>>(a);
+    return blocks;
 }
 
 template <typename T, bool BACK>
-static cudaError_t rh_launch(RhArgs& a, bool mixed, int blocks, cudaStream_t s)
+static int rh_launch(RhArgs& a, bool mixed, cudaStream_t s)   // the number of blocks
 {
     // the widest pieces that all addresses allow: a piece is VP elements of one half of a head, or 2 VP of pairs side by side
     constexpr int MOST = 16 / (int)sizeof(T);
@@ -333,20 +342,19 @@ static cudaError_t rh_launch(RhArgs& a, bool mixed, int blocks, cudaStream_t s)
         if (ok) break;
     }
     if constexpr (MOST == 8) {
-        if (vp == 8) rh_start<T, 8, 1, BACK>(a, mixed, blocks, s);
+        if (vp == 8) return rh_start<T, 8, 1, BACK>(a, mixed, s);
     }
-    if (vp == 4) rh_start<T, 4, 1, BACK>(a, mixed, blocks, s);
-    else if (vp == 2) rh_start<T, 2, 2, BACK>(a, mixed, blocks, s);
-    else if (vp == 1) rh_start<T, 1, 4, BACK>(a, mixed, blocks, s);
-    return cudaGetLastError();
+    if (vp == 4) return rh_start<T, 4, 1, BACK>(a, mixed, s);
+    if (vp == 2) return rh_start<T, 2, 2, BACK>(a, mixed, s);
+    return rh_start<T, 1, 4, BACK>(a, mixed, s);
 }
 
 template <bool BACK>
-static cudaError_t rh_run(RhArgs& a, int dtype, bool mixed, int blocks, cudaStream_t s)
+static int rh_run(RhArgs& a, int dtype, bool mixed, cudaStream_t s)
 {
-    if (dtype == DYNB_F32) return rh_launch<float, BACK>(a, mixed, blocks, s);
-    if (dtype == DYNB_F16) return rh_launch<__half, BACK>(a, mixed, blocks, s);
-    return rh_launch<__nv_bfloat16, BACK>(a, mixed, blocks, s);
+    if (dtype == DYNB_F32) return rh_launch<float, BACK>(a, mixed, s);
+    if (dtype == DYNB_F16) return rh_launch<__half, BACK>(a, mixed, s);
+    return rh_launch<__nv_bfloat16, BACK>(a, mixed, s);
 }
 
 }  // namespace dynb
@@ -362,7 +370,8 @@ extern "C" int dynb_rotary_heads(const dynb_rotary* args, void* q_out_dev, void*
     if ((args->n_q > 0 && !q_out_dev) || (args->n_k > 0 && !k_out_dev)) return fail_arg("null pointer");
     a.side[0].out = q_out_dev;
     a.side[1].out = k_out_dev;
-    DYNB_CUDA_OK(rh_run<false>(a, args->dtype, args->interleaved != 0, rh_blocks(a.rows, a.half), static_cast<cudaStream_t>(stream)));
+    (void)rh_run<false>(a, args->dtype, args->interleaved != 0, static_cast<cudaStream_t>(stream));
+    DYNB_CUDA_OK(cudaGetLastError());
     return DYNB_OK;
 }
 
@@ -372,7 +381,7 @@ extern "C" int dynb_rotary_heads_workspace_bytes(const dynb_rotary* args, int64_
     const int rc = rh_args(args, &a);
     if (rc != DYNB_OK) return rc;
     if (bytes == nullptr) return fail_arg("null pointer");
-    *bytes = (int64_t)rh_blocks(a.rows, a.half) * 4 * a.half * 4;
+    *bytes = (int64_t)rh_blocks(a.rows, 32) * 4 * a.half * 4;
     return DYNB_OK;
 }
 
@@ -385,8 +394,7 @@ extern "C" int dynb_rotary_heads_backward(const dynb_rotary* args, const void* d
     if (rc != DYNB_OK) return rc;
     if ((args->n_q > 0 && !d_q_out_dev) || (args->n_k > 0 && !d_k_out_dev)) return fail_arg("null pointer");
     const bool weights = d_q_weight_dev != nullptr || d_k_weight_dev != nullptr;
-    const int blocks = rh_blocks(a.rows, a.half);
-    if (weights && (workspace_dev == nullptr || !starts_on(workspace_dev, 4) || workspace_bytes < (int64_t)blocks * 4 * a.half * 4))
+    if (weights && (workspace_dev == nullptr || !starts_on(workspace_dev, 4) || workspace_bytes < (int64_t)rh_blocks(a.rows, 32) * 4 * a.half * 4))
         return fail_arg("workspace too small");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     a.side[0].dy = d_q_out_dev; a.side[0].dy_row = d_q_row; a.side[0].dy_head = d_q_head; a.side[0].out = d_q_dev;
@@ -394,7 +402,8 @@ extern "C" int dynb_rotary_heads_backward(const dynb_rotary* args, const void* d
     a.d_pos = d_pos_dev;
     a.partial = weights ? static_cast<float*>(workspace_dev) : nullptr;
     if (a.rows == 0 && !weights) return DYNB_OK;
-    DYNB_CUDA_OK(rh_run<true>(a, args->dtype, args->interleaved != 0, blocks, s));
+    const int blocks = rh_run<true>(a, args->dtype, args->interleaved != 0, s);
+    DYNB_CUDA_OK(cudaGetLastError());
     if (weights) {
         rh_join_kernel<<<4 * a.half, 128, 0, s>>>(a.partial, blocks, 2 * a.half, d_q_weight_dev, d_k_weight_dev);
         DYNB_CUDA_OK(cudaGetLastError());
