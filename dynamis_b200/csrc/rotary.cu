@@ -106,7 +106,7 @@ __device__ __forceinline__ float2 rh_turn(const RhArgs& a, int64_t i, int p)
 }
 
 template <typename T, int VP, int PIECES, bool MIXED, bool BACK>
-__global__ void __launch_bounds__(RH_WARPS * 32)
+__global__ void __launch_bounds__(RH_WARPS * 32, BACK ? 2 : 4)
 rh_kernel(const RhArgs a)
 {
     __shared__ __align__(16) float weight[2][2][RH_MAX_HALF];   // of the first and of the second elements of the pairs
@@ -283,7 +283,7 @@ rh_join_kernel(const float* partial, int blocks, int dim, float* d_q_weight, flo
 static int rh_blocks(int64_t rows, int lanes)
 {
     const int64_t need = (rows * lanes + 32 * RH_WARPS - 1) / (32 * RH_WARPS);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)sm_count_cached() * 4));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(need, (int64_t)sm_count_cached() * 8));
 }
 
 static int rh_args(const dynb_rotary* in, RhArgs* a)
