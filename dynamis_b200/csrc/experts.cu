@@ -131,7 +131,7 @@ ex_slope_kernel(const T* dz, int64_t dz_row, const void* slope, T* du, int64_t n
 // The sums of an expert joined (its pairs are cut at multiples of the stretch): blockIdx.y is the expert.
 template <typename T>
 __global__ void __launch_bounds__(EX_THREADS)
-ex_join_kernel(const TlArgs a, int64_t stretches)
+ex_join_kernel(const TlArgs a, int64_t stretches, int quads)   // quads: sums are read by 16 bytes
 {
     const int type = blockIdx.y;
     __shared__ int64_t first_of, count_of;
@@ -154,16 +154,32 @@ ex_join_kernel(const TlArgs a, int64_t stretches)
     __syncthreads();
     const int64_t cells = (int64_t)a.inner * a.outer, all = cells + a.outer, first = first_of;
     const int64_t count = min(count_of, max(stretches - first, (int64_t)0));
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {   // a few elements a thread: the start of a block is long
-        double exact = 0.0;
-#pragma unroll 8
-        for (int64_t c = 0; c < count; c++) exact += (double)a.partial[(first + c) * all + i];
-        const float sum = (float)exact;
+    const auto put = [&](int64_t i, double v) {
         if (i < cells) {
-            if (a.dw != nullptr) tl_put(static_cast<T*>(a.dw) + type * cells + i, sum);
+            if (a.dw != nullptr) tl_put(static_cast<T*>(a.dw) + type * cells + i, (float)v);
         } else if (a.db != nullptr) {
-            tl_put(static_cast<T*>(a.db) + (int64_t)type * a.outer + (i - cells), sum);
+            tl_put(static_cast<T*>(a.db) + (int64_t)type * a.outer + (i - cells), (float)v);
         }
+    };
+    const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+    if (quads) {
+        for (int64_t i = 4 * at; i < all; i += 4 * step) {
+            double v[4] = {};
+#pragma unroll 4
+            for (int64_t c = 0; c < count; c++) {
+                const float4 f = *reinterpret_cast<const float4*>(a.partial + (first + c) * all + i);
+                v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) put(i + j, v[j]);
+        }
+        return;
+    }
+    for (int64_t i = at; i < all; i += step) {
+        double v = 0.0;
+#pragma unroll 8
+        for (int64_t c = 0; c < count; c++) v += (double)a.partial[(first + c) * all + i];
+        put(i, v);
     }
 }
 
@@ -250,7 +266,7 @@ static int ex_backward(ExArgs& e, int dtype, const int32_t* experts, void* d_x, 
         if (e.du != nullptr) { a.dy = e.du; a.dy_row = a.outer; }
         DYNB_CUDA_OK(ex_mma_weights(e, dtype, s));
         const int64_t all = (int64_t)a.inner * a.outer + a.outer;
-        ex_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((all + 4 * EX_THREADS - 1) / (4 * EX_THREADS), 1024), a.types), EX_THREADS, 0, s>>>(a, ex_stretches(e));
+        ex_join_kernel<T><<<dim3((unsigned)std::min<int64_t>((all + 4 * EX_THREADS - 1) / (4 * EX_THREADS), 1024), a.types), EX_THREADS, 0, s>>>(a, ex_stretches(e), all % 4 == 0);
         DYNB_CUDA_OK(cudaGetLastError());
     }
     return DYNB_OK;

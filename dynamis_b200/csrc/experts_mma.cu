@@ -19,9 +19,8 @@ namespace dynb {
 // Warps that gather, and that store results.  An SM's four schedulers have room for five warps of 96 registers each, or four of 128: rows in fp32 wait in the registers of
 // their threads and need the latter.
 constexpr int EM_FEED = 8;
-template <typename T> constexpr int EM_OUT = sizeof(T) == 4 ? 4 : 16;
-template <typename T> constexpr int EM_COLUMNS = 16;
-template <typename T> constexpr int EM_THREADS = (EM_OUT<T> + 2 + EM_FEED) * 32;
+constexpr int EM_COLUMNS = 16;                                       // columns that a warp takes out of tensor memory at a time
+__host__ __device__ constexpr int em_threads(int out) { return (out + 2 + EM_FEED) * 32; }
 constexpr int EM_MAX_STAGES = 8;
 constexpr int EM_SMEM = 220 * 1024;                                  // beside 4 KB of offsets and barriers
 constexpr int EM_DEPTH = 3;                                          // stages whose copies a gathering warp leaves under way
@@ -60,31 +59,47 @@ __device__ __forceinline__ void copies_wait(int left)
 }
 
 // Matrices in the order of the multipliers: [expert][tile of columns][64 summed columns][part][column][128 bytes, 16-byte pieces swizzled], zeros beyond the matrix.
-template <typename T>
+// WIDE: rows of the matrix are read by 16 bytes; forward a thread turns a piece of 8 rows by that many columns round.  What is written lies side by side for 8 threads.
+// (64 matrices of 512 x 256 bf16 by single elements: 12.7 us.)
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 ex_pack_kernel(const T* w, int64_t experts, int inner, int outer, int back, int columns, int tiles, int chunks, unsigned char* packed)
 {
-    constexpr int PARTS = TmParts<T>::N;
-    const int64_t all = experts * tiles * chunks * columns * 8;
-    const int kk = back ? outer : inner, nn = back ? inner : outer;
+    constexpr int PARTS = TmParts<T>::N, N = 16 / (int)sizeof(T);
+    const int kk = back ? outer : inner, nn = back ? inner : outer, group = WIDE && !back ? N : 1, groups = columns / group;
+    const int64_t all = experts * tiles * chunks * groups * 8;
     for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < all; u += (int64_t)gridDim.x * blockDim.x) {
-        // what lies side by side in memory goes to neighbouring threads: columns forward, pieces of the summed index backward
-        int64_t rest = u;
-        const int inside = (int)(rest % (columns * 8));
-        rest /= columns * 8;
-        const int n = back ? inside / 8 : inside % columns, piece = back ? inside % 8 : inside / columns;
-        const int chunk = (int)(rest % chunks);
-        rest /= chunks;
-        const int tile = (int)(rest % tiles);
-        const int64_t e = rest / tiles;
+        const int64_t block = u / (groups * 8);
+        const int inside = (int)(u - block * (groups * 8)), piece = inside % 8, n = inside / 8 * group;
+        const int64_t run = block / chunks, e = run / tiles;
+        const int chunk = (int)(block - run * chunks), tile = (int)(run - e * tiles);
         const int k = chunk * 64 + piece * 8, col = tile * columns + n;
         const int have = col < nn ? min(8, kk - k) : 0;
         const T* const from = w + e * inner * outer + (back ? (int64_t)col * outer + k : (int64_t)k * outer + col);
-        const TmRaw<T> v = tm_load<false>(have > 0 ? from : w, back ? 1 : outer, have);
-        const TmRaw<T> one[1] = {v};
-        unsigned char* const to = packed + ((e * tiles + tile) * chunks + chunk) * ((int64_t)PARTS * columns * 128) + tile_piece(n, piece);
-        if (tm_odd(one)) tm_store<true>(v, to, columns * 128);
-        else tm_store<false>(v, to, columns * 128);
+        unsigned char* const to = packed + block * ((int64_t)PARTS * columns * 128);
+        TmRaw<T> v[N];
+        if constexpr (WIDE) {
+            if (!back) {
+                uint4 row[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) row[j] = j < have ? __ldg(reinterpret_cast<const uint4*>(from + (int64_t)j * outer)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) reinterpret_cast<T*>(&v[i])[j] = reinterpret_cast<const T*>(&row[j])[i];
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const TmRaw<T> one[1] = {v[i]};
+                    if (tm_odd(one)) tm_store<true>(v[i], to + tile_piece(n + i, piece), columns * 128);
+                    else tm_store<false>(v[i], to + tile_piece(n + i, piece), columns * 128);
+                }
+                continue;
+            }
+        }
+        v[0] = back && WIDE ? tm_load<true>(have > 0 ? from : w, 1, have) : tm_load<false>(have > 0 ? from : w, back ? 1 : outer, have);
+        const TmRaw<T> one[1] = {v[0]};
+        if (tm_odd(one)) tm_store<true>(v[0], to + tile_piece(n, piece), columns * 128);
+        else tm_store<false>(v[0], to + tile_piece(n, piece), columns * 128);
     }
 }
 
@@ -159,10 +174,10 @@ __device__ __forceinline__ void em_put(unsigned char* to, const uint32_t (&w)[WO
 
 // The activation of a row's sums, and their slopes.
 template <typename T, int ACTIVATION>
-__device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS<T>], uint32_t (&slopes)[EM_COLUMNS<T> * sizeof(T) / 4])
+__device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS], uint32_t (&slopes)[EM_COLUMNS * sizeof(T) / 4])
 {
 #pragma unroll
-    for (int i = 0; i < EM_COLUMNS<T>; i += 2) {
+    for (int i = 0; i < EM_COLUMNS; i += 2) {
         float s0, s1;
         const float v0 = ex_activate<ACTIVATION>(__uint_as_float(bits[i]), &s0), v1 = ex_activate<ACTIVATION>(__uint_as_float(bits[i + 1]), &s1);
         bits[i] = __float_as_uint(v0);
@@ -177,12 +192,12 @@ __device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS<T>], uin
 }
 
 // O: type of the results (fp32 for gradients that are summed over the choices before they are rounded).
-template <typename T, typename O, EmPath PATH, bool WIDE>
-__global__ void __launch_bounds__(EM_THREADS<T>, 1)
+template <typename T, typename O, EmPath PATH, bool WIDE, int OUT>
+__global__ void __launch_bounds__(em_threads(OUT), 1)
 em_rows_kernel(const ExArgs e, const EmPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = EM_COLUMNS<T>, WORDS = COLUMNS * SIZE / 4;   // columns that a warp takes at a time
-    constexpr int OUT = EM_OUT<T>, SHARES = OUT / 4;
+    constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = EM_COLUMNS, WORDS = COLUMNS * SIZE / 4;   // columns that a warp takes at a time
+    constexpr int SHARES = OUT / 4;
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EmBars bars;
@@ -838,24 +853,34 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
 
 // ------------------------------------------------------------------------------------------------ host
 template <typename T>
-static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // slopes: they are copied beside the rows
+static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // slopes: they are brought beside the rows
 {
     constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, MOST = PARTS == 1 ? 256 : 128;
     const int kk = back ? e.t.outer : e.t.inner, nn = back ? e.t.inner : e.t.outer;
     EmPlan p = {};
     p.back = back;
     p.chunks = (kk + 63) / 64;
-    *tiles = (nn + MOST - 1) / MOST;
-    p.columns = tm_round((nn + *tiles - 1) / *tiles, 16);
-    *tiles = (nn + p.columns - 1) / p.columns;
+    const int rows_bytes = A_BYTES * (slopes ? 2 : 1), room = EM_SMEM - 1024;
+    // Every tile of columns reads the rows anew, and a matrix that does not stay comes anew with every tile of rows: as few bytes as possible for 128 pairs.
+    const int least = (nn + MOST - 1) / MOST;
+    int64_t best = INT64_MAX;
+    for (int t = least; t <= 4 * least; t++) {
+        EmPlan q = p;
+        q.columns = tm_round((nn + t - 1) / t, 16);
+        q.b_bytes = PARTS * q.columns * 128;
+        q.resident = (int64_t)q.chunks * q.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * rows_bytes <= room;
+        const int count = (nn + q.columns - 1) / q.columns;
+        const int64_t bytes = (int64_t)count * (TM_ROWS * 64 * (int)sizeof(T) * (slopes ? 2 : 1) + (q.resident ? 0 : q.b_bytes));
+        if (bytes >= best) continue;
+        best = bytes;
+        q.slope_at = A_BYTES + (q.resident ? 0 : q.b_bytes);
+        q.stage_bytes = rows_bytes + (q.resident ? 0 : q.b_bytes);
+        q.stages = std::min(EM_MAX_STAGES, (room - (q.resident ? q.chunks * q.b_bytes : 0)) / q.stage_bytes);
+        *tiles = count;
+        p = q;
+    }
     p.column_stride = tm_round(p.columns, 32);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
-    p.b_bytes = PARTS * p.columns * 128;
-    const int rows_bytes = A_BYTES * (slopes ? 2 : 1);
-    p.resident = (int64_t)p.chunks * p.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * rows_bytes + 1024 <= EM_SMEM;
-    p.slope_at = A_BYTES + (p.resident ? 0 : p.b_bytes);
-    p.stage_bytes = rows_bytes + (p.resident ? 0 : p.b_bytes);
-    p.stages = std::min(EM_MAX_STAGES, (EM_SMEM - 1024 - (p.resident ? p.chunks * p.b_bytes : 0)) / p.stage_bytes);
     p.depth = std::min(EM_DEPTH, p.stages - 1);
     return p;
 }
@@ -863,9 +888,13 @@ static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // s
 template <typename T>
 static int64_t em_packed(const ExArgs& e, int back)
 {
-    int tiles;
-    const EmPlan p = em_plan<T>(e, back, false, &tiles);
-    return (int64_t)e.t.types * tiles * p.chunks * p.b_bytes;
+    int64_t most = 0;
+    for (int slopes = 0; slopes < 2; slopes++) {   // which of them it is depends on addresses that are not known here
+        int tiles;
+        const EmPlan p = em_plan<T>(e, back, slopes != 0, &tiles);
+        most = std::max(most, (int64_t)e.t.types * tiles * p.chunks * p.b_bytes);
+    }
+    return most;
 }
 
 int64_t ex_packed_bytes(const ExArgs& e, int back, int dtype) { return dtype == DYNB_F32 ? em_packed<float>(e, back) : em_packed<__nv_bfloat16>(e, back); }
@@ -885,23 +914,26 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     p.packed = static_cast<const unsigned char*>(packed);
     p.store = tm_on(out, nn, sizeof(O), 32) ? 32 : tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
     p.slope_store = tm_on(e.slope, nn, SIZE, 32) ? 32 : tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
-    const int64_t units = (int64_t)a.types * tiles * p.chunks * p.columns * 8;
-    ex_pack_kernel<T><<<(unsigned)std::min<int64_t>((units + 255) / 256, (int64_t)sm_count_cached() * 8), 256, 0, s>>>(
+    const bool wide_w = tm_on(a.w, a.outer, SIZE, 16) && a.outer % 8 == 0;
+    const int64_t units = (int64_t)a.types * tiles * p.chunks * (p.columns / (wide_w && !back ? 16 / SIZE : 1)) * 8;
+    (wide_w ? ex_pack_kernel<T, true> : ex_pack_kernel<T, false>)<<<(unsigned)std::min<int64_t>((units + 255) / 256, (int64_t)sm_count_cached() * 8), 256, 0, s>>>(
         static_cast<const T*>(a.w), a.types, a.inner, a.outer, back, p.columns, tiles, p.chunks, static_cast<unsigned char*>(packed));
     cudaError_t rc = cudaGetLastError();
     if (rc != cudaSuccess) return rc;
-    void (*kernel)(ExArgs, EmPlan);
-    if (slope && !wide) kernel = em_rows_kernel<T, O, EM_SLOPE, false>;
-    else if (slope) kernel = em_rows_kernel<T, O, SIZE == 4 ? EM_SLOPE : EM_ASYNC_SLOPE, true>;
-    else if (!wide) kernel = em_rows_kernel<T, O, EM_REGISTERS, false>;
-    else if constexpr (SIZE == 4) kernel = em_rows_kernel<T, O, EM_REGISTERS, true>;
-    else kernel = em_rows_kernel<T, O, EM_ASYNC, true>;
+    // Warps that store results: activations in 16 bits keep sixteen busy (300 k pairs 256 x 512, SiLU: 178 us, with eight 210); without them eight leave the others more registers.
+    constexpr int FEW = SIZE == 4 ? 4 : 8, MANY = SIZE == 4 ? 4 : 16;
+    const bool many = MANY != FEW && std::is_same<T, O>::value && !back && e.activation != DYNB_ACTIVATION_NONE;
+    constexpr EmPath QUICK = SIZE == 4 ? EM_REGISTERS : EM_ASYNC, QUICK_SLOPE = SIZE == 4 ? EM_SLOPE : EM_ASYNC_SLOPE;
+    void (*kernel)(ExArgs, EmPlan) = slope ? (wide ? em_rows_kernel<T, O, QUICK_SLOPE, true, FEW> : em_rows_kernel<T, O, EM_SLOPE, false, FEW>)
+                                           : (wide ? em_rows_kernel<T, O, QUICK, true, FEW> : em_rows_kernel<T, O, EM_REGISTERS, false, FEW>);
+    if constexpr (std::is_same<T, O>::value)
+        if (many) kernel = wide ? em_rows_kernel<T, O, QUICK, true, MANY> : em_rows_kernel<T, O, EM_REGISTERS, false, MANY>;
     const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
     const int smem = 1024 + (p.resident ? p.chunks * p.b_bytes : 0) + p.stages * p.stage_bytes;
     rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    kernel<<<grid, EM_THREADS<T>, smem, s>>>(e, p);
+    kernel<<<grid, em_threads(many ? MANY : FEW), smem, s>>>(e, p);
     return cudaGetLastError();
 }
 
