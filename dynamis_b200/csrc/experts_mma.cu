@@ -23,7 +23,7 @@ constexpr int EM_COLUMNS = 16;                                       // columns 
 __host__ __device__ constexpr int em_threads(int out) { return (out + 2 + EM_FEED) * 32; }
 constexpr int EM_MAX_STAGES = 8;
 constexpr int EM_SMEM = 220 * 1024;                                  // beside 4 KB of offsets and barriers
-constexpr int EM_DEPTH = 3;                                          // stages whose copies a gathering warp leaves under way
+constexpr int EM_DEPTH = 2;                                          // stages whose copies a gathering warp leaves under way
 
 enum EmPath { EM_ASYNC, EM_REGISTERS, EM_SLOPE, EM_ASYNC_SLOPE };
 
@@ -48,12 +48,13 @@ __device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool live
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
+// The barrier gets this thread's arrival when all its copies so far are there.  What they wrote is made visible to the tensor cores by the thread that waits.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory"); }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All but the last `left` groups of this thread have arrived.
 __device__ __forceinline__ void copies_wait(int left)
 {
-    if (left >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    if (left >= 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
     else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -210,7 +211,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], EM_FEED);
+            bar_init(&bars.full[s], PATH == EM_ASYNC ? EM_FEED * 32 : EM_FEED);
             bar_init(&bars.empty[s], 1);
             bar_init(&bars.b_full[s], 1);
         }
@@ -323,6 +324,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             const uint32_t sums = tensor + buffer * plan.column_stride;
             for (int chunk = 0; chunk < plan.chunks; chunk++) {
                 if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+                if constexpr (PATH == EM_ASYNC) fence_to_tensor();
                 if (!plan.resident && !bar_wait(&bars.b_full[stage], phase)) { ok = false; break; }
                 tensor_fence_after();
                 if (elected()) {
@@ -461,18 +463,25 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                         copy_16(to + i * EM_FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
                         if constexpr (SLOPE) copy_16(to + i * EM_FEED * 512 + plan.slope_at, static_cast<const T*>(e.slope) + (live ? (int64_t)at[i] * kk + k : 0), live);
                     }
-                    copies_commit();
-                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                    if (++asked > plan.depth) {
-                        copies_wait(plan.depth);
-                        arrive();
+                    if constexpr (!SLOPE) {
+                        copies_arrive(&bars.full[stage]);
+                        if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                    } else {
+                        copies_commit();
+                        if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                        if (++asked > plan.depth) {
+                            copies_wait(plan.depth);
+                            arrive();
+                        }
                     }
                 }
             }
-            for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
-                copies_wait(left - 1);
-                arrive();
-            }
+            if constexpr (SLOPE)
+                for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
+                    copies_wait(left - 1);
+                    arrive();
+                }
+            copies_commit();
             copies_wait(0);
         } else {
             constexpr int AHEAD = sizeof(T) == 4 && PATH == EM_SLOPE ? 1 : 2;
@@ -555,7 +564,7 @@ constexpr int EW_OUT = 4, EW_SUM = 4, EW_FEED = 16, EW_THREADS = (EW_OUT + 1 + E
 template <typename T> constexpr int EW_ROWS = sizeof(T) == 4 ? 32 : 64;   // pairs of a stage
 constexpr int EW_SMEM = 222 * 1024;
 
-struct EwPlan { int64_t most; int columns, column_stride, x_blocks, y_blocks, row_tiles, column_tiles, stages, depth, tensor_columns, store; };   // most: sums that there is room for
+struct EwPlan { int64_t most; int columns, column_stride, x_blocks, y_blocks, row_tiles, column_tiles, stages, tensor_columns, store; };   // most: sums that there is room for
 struct EwBars { uint64_t full[EW_MAX_STAGES], empty[EW_MAX_STAGES], sums_full[2], sums_free[2]; uint32_t tensor; };
 
 // The pairs in the order of their experts are cut at multiples of `stretch` and where experts begin; a block takes the pieces of its slice one after the other.
@@ -625,7 +634,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], EW_FEED);
+            bar_init(&bars.full[s], PATH == EM_ASYNC ? EW_FEED * 32 : EW_FEED);
             bar_init(&bars.empty[s], sums_wanted ? 1 + EW_SUM : 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -689,6 +698,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             const uint32_t sums = tensor + buffer * SUMS * plan.column_stride;
             for (int step = 0; step < steps; step++) {
                 if (!bar_wait(&bars.full[stage], phase)) { ok = false; break; }
+                if constexpr (PATH == EM_ASYNC) fence_to_tensor();
                 tensor_fence_after();
                 if (elected()) {
                     const uint32_t at = stage_at + stage * stage_bytes;
@@ -783,24 +793,12 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
         uint32_t phase = 1;
         bool more = row_of(id);
         if constexpr (PATH == EM_ASYNC) {
-            int arrived = 0;
-            auto arrive = [&] {
-                fence_to_tensor();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.full[arrived]);
-                if (++arrived == plan.stages) arrived = 0;
-            };
-            int64_t asked = 0;
             auto ask = [&](int32_t p) {
                 if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); return false; }
                 const uint32_t to = smem_addr(stage0) + stage * stage_bytes + at0;
                 units_of(p, [&](int i, const T* from, int have) { copy_16(to + i * GROUPS * BLOCK, from, have > 0); });
-                copies_commit();
+                copies_arrive(&bars.full[stage]);
                 if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                if (++asked > plan.depth) {
-                    copies_wait(plan.depth);
-                    arrive();
-                }
                 return true;
             };
             // numbers of two stages by turns, each asked for two stages ahead (copied from one place to another they would be waited for at once)
@@ -812,10 +810,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                 if (!other || !ask(other_id)) break;
                 other = row_of(other_id);
             }
-            for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
-                copies_wait(left - 1);
-                arrive();
-            }
+            copies_commit();
             copies_wait(0);
         } else {
             TmRaw<T> v[UNITS] = {};
@@ -881,7 +876,7 @@ static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // s
     }
     p.column_stride = tm_round(p.columns, 32);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
-    p.depth = std::min(EM_DEPTH, p.stages - 1);
+    p.depth = std::max(1, std::min(EM_DEPTH, p.stages - 1));
     return p;
 }
 
@@ -971,7 +966,6 @@ static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
     p.column_tiles = (a.outer + p.columns - 1) / p.columns;
     const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
     p.stages = std::min(EW_MAX_STAGES, (EW_SMEM - 1024) / stage);
-    p.depth = std::min(EM_DEPTH, p.stages - 1);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
     p.store = tm_on(a.partial, a.outer, 4, 32) && (int64_t)a.inner * a.outer % 8 == 0 ? 32 : tm_on(a.partial, a.outer, 4, 16) ? 16 : 4;
