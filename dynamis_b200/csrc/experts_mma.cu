@@ -23,12 +23,12 @@ constexpr int EM_COLUMNS = 16;                                       // columns 
 __host__ __device__ constexpr int em_threads(int out) { return (out + 2 + EM_FEED) * 32; }
 constexpr int EM_MAX_STAGES = 8;
 constexpr int EM_SMEM = 220 * 1024;                                  // beside 4 KB of offsets and barriers
-constexpr int EM_DEPTH = 2;                                          // stages whose copies a gathering warp leaves under way
+constexpr int EM_RAW = 3;                                            // stages of rows and slopes on their way beside those of the products
 
 enum EmPath { EM_ASYNC, EM_REGISTERS, EM_SLOPE, EM_ASYNC_SLOPE };
 
 struct EmPlan {
-    int back, columns, column_stride, chunks, stages, depth, tensor_columns, resident, b_bytes, stage_bytes, slope_at, store, slope_store;   // b_bytes: matrix of one stage; slope_at: slopes behind its rows
+    int back, columns, column_stride, chunks, stages, tensor_columns, resident, b_bytes, stage_bytes, store, slope_store, smem;   // b_bytes: matrix of one stage
     const unsigned char* packed;
 };
 
@@ -50,6 +50,10 @@ __device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool live
 }
 // The barrier gets this thread's arrival when all its copies so far are there.  What they wrote is made visible to the tensor cores by the thread that waits.
 __device__ __forceinline__ void copies_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory"); }
+__device__ __forceinline__ void load_16(uint32_t from, uint4& v)
+{
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All but the last `left` groups of this thread have arrived.
 __device__ __forceinline__ void copies_wait(int left)
@@ -412,41 +416,9 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         auto row_in = [&](int32_t p) { return (uint32_t)p >= (uint64_t)a.n ? 0xffffffffu : fan == 1 ? (uint32_t)p : (uint32_t)p / (uint32_t)fan; };
         int stage = 0;
         uint32_t phase = 1;
-        if constexpr (PATH == EM_ASYNC || PATH == EM_ASYNC_SLOPE) {
-            constexpr bool SLOPE = PATH == EM_ASYNC_SLOPE;
-            int arrived = 0;                        // stage of the next arrival
-            int64_t asked = 0;
+        if constexpr (PATH == EM_ASYNC) {
             rows_of(cursor.tile, rows);
             bool ok = true;
-            const bool keep_du = SLOPE && e.du != nullptr && blockIdx.y == 0;
-            TmCursor behind = cursor;               // of the next arrival, for du
-            int behind_chunk = 0;
-            int32_t behind_rows[UNITS];
-            if (keep_du) rows_of(behind.tile, behind_rows);
-            auto arrive = [&] {
-                if constexpr (SLOPE) {   // each thread multiplies what it has copied itself
-                    unsigned char* const at = stage0 + arrived * plan.stage_bytes + tile_piece(tid >> 3, piece);
-#pragma unroll
-                    for (int i = 0; i < UNITS; i++) {
-                        TmRaw<T> v, slope;
-                        v.v[0] = *reinterpret_cast<const uint4*>(at + i * EM_FEED * 512);
-                        slope.v[0] = *reinterpret_cast<const uint4*>(at + i * EM_FEED * 512 + plan.slope_at);
-                        em_times(v, slope);
-                        *reinterpret_cast<uint4*>(at + i * EM_FEED * 512) = v.v[0];
-                        const int k = behind_chunk * 64 + piece * 8;
-                        if (keep_du && (uint32_t)behind_rows[i] < rows_in && k < kk) *reinterpret_cast<uint4*>(static_cast<T*>(e.du) + (int64_t)behind_rows[i] * kk + k) = v.v[0];
-                    }
-                    if (keep_du && ++behind_chunk == plan.chunks) {
-                        behind_chunk = 0;
-                        behind.next(a);
-                        rows_of(behind.tile, behind_rows);
-                    }
-                }
-                fence_to_tensor();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.full[arrived]);
-                if (++arrived == plan.stages) arrived = 0;
-            };
             while (ok && cursor.tile.type >= 0) {
                 uint32_t at[UNITS];
 #pragma unroll
@@ -461,27 +433,79 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     for (int i = 0; i < UNITS; i++) {
                         const bool live = at[i] < rows_in && k < kk;
                         copy_16(to + i * EM_FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
-                        if constexpr (SLOPE) copy_16(to + i * EM_FEED * 512 + plan.slope_at, static_cast<const T*>(e.slope) + (live ? (int64_t)at[i] * kk + k : 0), live);
                     }
-                    if constexpr (!SLOPE) {
-                        copies_arrive(&bars.full[stage]);
-                        if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                    } else {
-                        copies_commit();
-                        if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                        if (++asked > plan.depth) {
-                            copies_wait(plan.depth);
-                            arrive();
-                        }
-                    }
+                    copies_arrive(&bars.full[stage]);
+                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
                 }
             }
-            if constexpr (SLOPE)
-                for (int left = (int)min(asked, (int64_t)plan.depth); left > 0; left--) {
-                    copies_wait(left - 1);
-                    arrive();
-                }
             copies_commit();
+            copies_wait(0);
+        } else if constexpr (PATH == EM_ASYNC_SLOPE) {
+            // Rows and slopes come to places that are this thread's own, EM_RAW stages of them, and go from there, multiplied, to the stages of the products
+            const uint32_t raw = smem_addr(stage0) + plan.stages * plan.stage_bytes + tid * 16;
+            constexpr uint32_t UNIT = EM_FEED * 512, SLOT = 2 * UNITS * UNIT;
+            const bool keep_du = e.du != nullptr && blockIdx.y == 0;
+            TmCursor behind = cursor;               // of the stage that is multiplied, for du
+            int chunk = 0, behind_chunk = 0, slot = 0, behind_slot = 0;
+            int32_t behind_rows[UNITS];
+            if (keep_du) rows_of(behind.tile, behind_rows);
+            rows_of(cursor.tile, rows);
+            uint32_t at[UNITS];
+            int64_t left = 0;                       // stages asked for and not yet multiplied
+            auto ask = [&] {
+                if (chunk == 0 && cursor.tile.type >= 0) {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) at[i] = row_in(rows[i]);
+                }
+                if (cursor.tile.type >= 0) {
+                    const int k = chunk * 64 + piece * 8;
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) {
+                        const bool ok = at[i] < rows_in && k < kk;
+                        copy_16(raw + slot * SLOT + i * UNIT, in + (ok ? at[i] * in_row + k : 0), ok);
+                        copy_16(raw + slot * SLOT + (UNITS + i) * UNIT, static_cast<const T*>(e.slope) + (ok ? (int64_t)at[i] * kk + k : 0), ok);
+                    }
+                    left++;
+                    if (++slot == EM_RAW) slot = 0;
+                    if (++chunk == plan.chunks) {
+                        chunk = 0;
+                        cursor.next(a);
+                        rows_of(cursor.tile, rows);
+                    }
+                }
+                copies_commit();                    // an empty group behind the last stage: the number of those under way stays the same
+            };
+#pragma unroll
+            for (int i = 0; i < EM_RAW - 1; i++) ask();
+            while (left > 0) {
+                ask();
+                copies_wait(EM_RAW - 1);
+                TmRaw<T> v[UNITS];
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) {
+                    TmRaw<T> slope;
+                    load_16(raw + behind_slot * SLOT + i * UNIT, v[i].v[0]);
+                    load_16(raw + behind_slot * SLOT + (UNITS + i) * UNIT, slope.v[0]);
+                    em_times(v[i], slope);
+                    const int k = behind_chunk * 64 + piece * 8;
+                    if (keep_du && (uint32_t)behind_rows[i] < rows_in && k < kk) *reinterpret_cast<uint4*>(static_cast<T*>(e.du) + (int64_t)behind_rows[i] * kk + k) = v[i].v[0];
+                }
+                if (++behind_slot == EM_RAW) behind_slot = 0;
+                if (keep_du && ++behind_chunk == plan.chunks) {
+                    behind_chunk = 0;
+                    behind.next(a);
+                    rows_of(behind.tile, behind_rows);
+                }
+                left--;
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+                unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
+#pragma unroll
+                for (int i = 0; i < UNITS; i++) *reinterpret_cast<uint4*>(to + i * UNIT) = v[i].v[0];
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[stage]);
+                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+            }
             copies_wait(0);
         } else {
             constexpr int AHEAD = sizeof(T) == 4 && PATH == EM_SLOPE ? 1 : 2;
@@ -855,7 +879,7 @@ static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // s
     EmPlan p = {};
     p.back = back;
     p.chunks = (kk + 63) / 64;
-    const int rows_bytes = A_BYTES * (slopes ? 2 : 1), room = EM_SMEM - 1024;
+    const int raw = slopes ? EM_RAW * 2 * A_BYTES : 0, room = EM_SMEM - 1024 - raw;
     // Every tile of columns reads the rows anew, and a matrix that does not stay comes anew with every tile of rows: as few bytes as possible for 128 pairs.
     const int least = (nn + MOST - 1) / MOST;
     int64_t best = INT64_MAX;
@@ -863,20 +887,19 @@ static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // s
         EmPlan q = p;
         q.columns = tm_round((nn + t - 1) / t, 16);
         q.b_bytes = PARTS * q.columns * 128;
-        q.resident = (int64_t)q.chunks * q.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * rows_bytes <= room;
+        q.resident = (int64_t)q.chunks * q.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * A_BYTES <= room;
         const int count = (nn + q.columns - 1) / q.columns;
         const int64_t bytes = (int64_t)count * (TM_ROWS * 64 * (int)sizeof(T) * (slopes ? 2 : 1) + (q.resident ? 0 : q.b_bytes));
         if (bytes >= best) continue;
         best = bytes;
-        q.slope_at = A_BYTES + (q.resident ? 0 : q.b_bytes);
-        q.stage_bytes = rows_bytes + (q.resident ? 0 : q.b_bytes);
+        q.stage_bytes = A_BYTES + (q.resident ? 0 : q.b_bytes);
         q.stages = std::min(EM_MAX_STAGES, (room - (q.resident ? q.chunks * q.b_bytes : 0)) / q.stage_bytes);
         *tiles = count;
         p = q;
     }
     p.column_stride = tm_round(p.columns, 32);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
-    p.depth = std::max(1, std::min(EM_DEPTH, p.stages - 1));
+    p.smem = 1024 + (p.resident ? p.chunks * p.b_bytes : 0) + p.stages * p.stage_bytes + raw;
     return p;
 }
 
@@ -925,10 +948,9 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
         if (many) kernel = wide ? em_rows_kernel<T, O, QUICK, true, MANY> : em_rows_kernel<T, O, EM_REGISTERS, false, MANY>;
     const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
-    const int smem = 1024 + (p.resident ? p.chunks * p.b_bytes : 0) + p.stages * p.stage_bytes;
-    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
     if (rc != cudaSuccess) return rc;
-    kernel<<<grid, em_threads(many ? MANY : FEW), smem, s>>>(e, p);
+    kernel<<<grid, em_threads(many ? MANY : FEW), p.smem, s>>>(e, p);
     return cudaGetLastError();
 }
 
