@@ -193,14 +193,21 @@ re_choose_kernel(const ReArgs a)
 // matter lie nearer to one another than these may be off are looked at again in 64 bits.
 constexpr int RT_WARPS = 4, RT_MAX_EXPERTS = 128, RT_MAX_CHOICES = 8, RT_MAX_GROUPS = 16;
 
-__device__ __forceinline__ uint32_t rt_order(float key)   // as re_order
+// As re_order: 0 for -infinity, NaN above all (arithmetic gives the one NaN whose bits below the sign are all set); adding zero makes zeros of both signs equal.
+__device__ __forceinline__ uint32_t rt_order(float key)
 {
-    if (isnan(key)) return 0xffffffffu;
-    return key == -INFINITY ? 0u : ordered_u32(key + 0.0f);
+    const uint32_t bits = __float_as_uint(key + 0.0f);
+    return (bits ^ (uint32_t)((int32_t)bits >> 31 | (int32_t)0x80000000)) - 0x007fffffu;
 }
 __device__ __forceinline__ uint64_t rt_order(double key) { return re_order(key); }
-__device__ __forceinline__ float rt_value(uint32_t order) { return order == 0xffffffffu ? NAN : unordered_f32(order); }
+__device__ __forceinline__ float rt_value(uint32_t order)
+{
+    const uint32_t bits = order + 0x007fffffu;
+    return __uint_as_float(bits ^ (uint32_t)(~((int32_t)bits >> 31) | (int32_t)0x80000000));
+}
 __device__ __forceinline__ double rt_value(uint64_t order) { return order == ~0ull ? NAN : unordered_f64(order); }
+__device__ __forceinline__ bool rt_nan(uint32_t order) { return order == 0xff800000u; }
+__device__ __forceinline__ bool rt_nan(uint64_t order) { return order == ~0ull; }
 template <typename K> struct RtOrder { using type = uint32_t; };
 template <> struct RtOrder<double> { using type = uint64_t; };
 
@@ -213,13 +220,19 @@ __device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* t
     constexpr int N = 16 / (int)sizeof(T);
     if (wide) {
         const int per = a.count / N;
+        int r = lane / per, c = lane % per;
+        const int rows = 32 / per, rest = 32 % per;      // 32 pieces on
+#pragma unroll 4
         for (int u = lane; u < 32 * per; u += 32) {
-            const int r = u / per, c = (u % per) * N;
-            if (row0 + r >= a.n) break;
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(l + (row0 + r) * a.row + c));
-            const T* const e = reinterpret_cast<const T*>(&v);
+            if (row0 + r < a.n) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(l + (row0 + r) * a.row + c * N));
+                const T* const e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-            for (int i = 0; i < N; i++) tile[r * pitch + c + i] = tl_get(e + i);
+                for (int i = 0; i < N; i++) tile[r * pitch + c * N + i] = tl_get(e + i);
+            }
+            r += rows;
+            c += rest;
+            if (c >= per) { c -= per; r++; }
         }
     } else {
         for (int u = lane; u < 32 * a.count; u += 32) {
@@ -249,17 +262,17 @@ __device__ __forceinline__ void rt_insert(O k, int e, int (&chosen)[MOST], O (&o
 
 // The experts of a lane's row.  key_of(e): keys of type K in their order, as often as asked; MOST: choices and two more, the first that are left out.  False: keys
 // that are off by up to `near` may have decided.  same(p, q): two experts have the same logit and bias, and so the same key, whatever its type.
-template <typename K, int MOST, typename Key, typename Same>
+template <typename K, int MOST, int GROUPS, typename Key, typename Same>
 __device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)[MOST], Key&& key_of, Same&& same)
 {
     using O = typename RtOrder<K>::type;
     bool sure = true;
     uint32_t kept = 0xffffffffu;
     const int per = a.count / a.groups;
-    if (a.groups > 1) {
-        O of_group[RT_MAX_GROUPS];
+    if constexpr (GROUPS > 1) {
+        O of_group[GROUPS];
 #pragma unroll
-        for (int g = 0; g < RT_MAX_GROUPS; g++) {
+        for (int g = 0; g < GROUPS; g++) {
             of_group[g] = 0;
             if (g >= a.groups) continue;
             O one = 0, two = 0;
@@ -270,19 +283,18 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)
                 one = max(one, k);
             }
             O both = one;
-            if (one == (O)~(O)0 || two == (O)~(O)0) both = ~(O)0;
-            else if (two != 0) both = rt_order(rt_value(one) + rt_value(two));
+            if (two != 0) both = rt_nan(one) ? one : rt_order(rt_value(one) + rt_value(two));
             if (one != 0 && both == 0) both = 1;   // open, however low
             of_group[g] = both;
         }
         kept = 0;
         O lowest = ~(O)0, highest = 0;   // of those that stay, and of the others
 #pragma unroll
-        for (int g = 0; g < RT_MAX_GROUPS; g++) {
+        for (int g = 0; g < GROUPS; g++) {
             if (g >= a.groups) continue;
             int before = 0;
 #pragma unroll
-            for (int h = 0; h < RT_MAX_GROUPS; h++) before += h < a.groups && (of_group[h] > of_group[g] || (of_group[h] == of_group[g] && h < g));
+            for (int h = 0; h < GROUPS; h++) before += h < a.groups && (of_group[h] > of_group[g] || (of_group[h] == of_group[g] && h < g));
             if (before < a.kept) {
                 kept |= 1u << g;
                 lowest = min(lowest, of_group[g]);
@@ -315,7 +327,7 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)
 }
 
 // A row once more in 64 bits.
-template <typename T, int MOST>
+template <typename T, int MOST, int GROUPS>
 __device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, const float* bias, float top, int* out)
 {
     const T* const l = static_cast<const T*>(a.logits) + row * a.row;
@@ -323,7 +335,7 @@ __device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, const float*
     if (!a.sigmoid)
         for (int e = 0; e < a.count; e++) sum += tl_get(l + e) == -INFINITY ? 0.0 : exp((double)tl_get(l + e) - (double)top);
     int chosen[MOST];
-    (void)rt_choose<double, MOST>(
+    (void)rt_choose<double, MOST, GROUPS>(
         a, 0.0, chosen,
         [&](int e) -> uint64_t {
             const double v = (double)tl_get(l + e);
@@ -334,11 +346,12 @@ __device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, const float*
     for (int j = 0; j < a.choices; j++) out[j] = chosen[j];
 }
 
-// PLAIN: the logits decide.
-template <typename T, int MOST, bool PLAIN>
-__global__ void __launch_bounds__(RT_WARPS * 32, PLAIN ? 12 : 8)
+// GROUPS: 0 where the logits decide, 1 without groups, else their largest number.
+template <typename T, int MOST, int GROUPS>
+__global__ void __launch_bounds__(RT_WARPS * 32, GROUPS == 0 ? 12 : 8)
 rt_choose_kernel(const ReArgs a, int pitch, int wide)
 {
+    constexpr bool PLAIN = GROUPS == 0;
     extern __shared__ unsigned char raw_smem[];
     int32_t* const counts = reinterpret_cast<int32_t*>(raw_smem);   // [experts + 1], then the biases [experts], then the rows of every warp
     float* const bias = reinterpret_cast<float*>(counts + a.count + 1);
@@ -353,8 +366,8 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
         for (int i = lane; i < a.count; i += 32) far = fmaxf(far, isinf(bias[i]) ? 0.0f : fabsf(bias[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) far = fmaxf(far, __shfl_xor_sync(0xffffffffu, far, o));
-    // how far a key in 32 bits may be off: a score by (experts + 16) 2^-24 (sigmoids 16), the sum with the bias by half a step
-    const float near = ((a.sigmoid ? 16.0f : a.count + 16.0f) + 2.0f * far) * 0x1p-24f;
+    // how far a key in 32 bits may be off: a score by (experts + 16) 2^-24 (sigmoids 8: exponential and division (3 + |v|) s (1 - s) and 2), the sum with the bias by half a step
+    const float near = ((a.sigmoid ? 8.0f : a.count + 16.0f) + 2.0f * far) * 0x1p-24f;
     const int64_t first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.n);
     for (int64_t row0 = first + warp * 32; row0 < last; row0 += RT_WARPS * 32) {
         const int64_t row = row0 + lane;
@@ -403,15 +416,15 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
             for (int e = 0; e < a.count; e++) {
                 const float v = l[e];
                 const float key = a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-v)) : v * over;
-                const bool closed = a.sigmoid ? v == -INFINITY : v < 0.0f;
+                const bool closed = v < (a.sigmoid ? -3.402823466e38f : 0.0f);   // -infinity, or its mark
                 l[e] = __uint_as_float(closed ? 0u : rt_order(key + bias[e]));
             }
             const T* const from = static_cast<const T*>(a.logits) + row * a.row;
-            if (!rt_choose<float, MOST>(
+            if (!rt_choose<float, MOST, GROUPS>(
                     a, near, chosen, [&](int e) { return __float_as_uint(l[e]); },
                     [&](int p, int q) { return tl_get(from + p) == tl_get(from + q) && bias[p] == bias[q]; })) {
                 int again[MOST];   // on the way through memory, as `chosen` must not be
-                rt_again<T, MOST>(a, row, bias, top, again);
+                rt_again<T, MOST, GROUPS>(a, row, bias, top, again);
 #pragma unroll
                 for (int j = 0; j < MOST; j++) chosen[j] = j < a.choices ? again[j] : -1;
             }
@@ -714,11 +727,11 @@ static int re_args(const dynb_routing* in, ReArgs* a)
 }
 
 // As few places in the list as the choices need: a longer one is entered more often (six choices with ten places 182 us, eight 161).
-template <typename T, bool PLAIN>
+template <typename T, int GROUPS>
 static void (*rt_kernel(int choices))(ReArgs, int, int)
 {
-    return choices <= 1 ? rt_choose_kernel<T, 3, PLAIN> : choices <= 2 ? rt_choose_kernel<T, 4, PLAIN> : choices <= 4 ? rt_choose_kernel<T, 6, PLAIN> :
-           choices <= 6 ? rt_choose_kernel<T, 8, PLAIN> : rt_choose_kernel<T, 10, PLAIN>;
+    return choices <= 1 ? rt_choose_kernel<T, 3, GROUPS> : choices <= 2 ? rt_choose_kernel<T, 4, GROUPS> : choices <= 4 ? rt_choose_kernel<T, 6, GROUPS> :
+           choices <= 6 ? rt_choose_kernel<T, 8, GROUPS> : rt_choose_kernel<T, 10, GROUPS>;
 }
 
 // Rows of `row` elements may be read, or written, by pieces of 16 bytes.
@@ -729,7 +742,8 @@ static cudaError_t re_choose(const ReArgs& a, unsigned blocks, cudaStream_t s)
 {
     if (rt_takes(a)) {
         const int pitch = a.count | 1, smem = (2 * a.count + 1 + RT_WARPS * 32 * pitch) * 4;
-        void (*const kernel)(ReArgs, int, int) = a.bias == nullptr && a.groups == 1 ? rt_kernel<T, true>(a.choices) : rt_kernel<T, false>(a.choices);
+        void (*const kernel)(ReArgs, int, int) = a.groups > 8 ? rt_kernel<T, 16>(a.choices) : a.groups > 1 ? rt_kernel<T, 8>(a.choices) :
+                                                   a.bias != nullptr ? rt_kernel<T, 1>(a.choices) : rt_kernel<T, 0>(a.choices);
         const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
         if (rc != cudaSuccess) return rc;
         kernel<<<blocks, RT_WARPS * 32, smem, s>>>(a, pitch, re_wide(a.logits, a.row, a.count, sizeof(T)));
