@@ -40,6 +40,142 @@ __device__ __forceinline__ uint64_t re_order(double key)
     return key == -INFINITY ? 0ull : ordered_u64(key + 0.0);   // -0 and 0 are equal
 }
 
+// A row by a warp.  V: experts of a lane; scratch: room for the experts and the groups.
+template <typename T, int V>
+__device__ __forceinline__ void re_row(const ReArgs& a, int64_t row, double* scratch, int32_t* counts)
+{
+    const int lane = threadIdx.x & 31, per = a.count / a.groups;
+    const bool plain = a.bias == nullptr && a.groups == 1;   // the logits decide
+    const T* const l = static_cast<const T*>(a.logits) + row * a.row;
+    float logit[V];
+    uint64_t key[V];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int e = lane + 32 * i;
+        logit[i] = e < a.count ? tl_get(l + e) : -INFINITY;
+        top = fmaxf(top, logit[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (plain) {
+#pragma unroll
+        for (int i = 0; i < V; i++) key[i] = re_order((double)logit[i]);
+    } else {
+        double s[V], sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            if (a.sigmoid) {
+                s[i] = 1.0 / (1.0 + exp(-(double)logit[i]));
+            } else {
+                s[i] = logit[i] == -INFINITY ? 0.0 : exp((double)logit[i] - (double)top);
+                sum += s[i];
+            }
+        }
+        if (!a.sigmoid) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int e = lane + 32 * i;
+            const double v = (a.sigmoid ? s[i] : s[i] / sum) + (a.bias != nullptr && e < a.count ? (double)a.bias[e] : 0.0);
+            key[i] = logit[i] == -INFINITY ? 0ull : re_order(v);
+        }
+        if (a.groups > 1) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (lane + 32 * i < a.count) scratch[lane + 32 * i] = __longlong_as_double((long long)key[i]);
+            __syncwarp();
+            uint64_t* const of_group = reinterpret_cast<uint64_t*>(scratch + a.count);
+            for (int g = lane; g < a.groups; g += 32) {
+                uint64_t one = 0, two = 0;
+                for (int j = 0; j < per; j++) {
+                    const uint64_t k = (uint64_t)__double_as_longlong(scratch[g * per + j]);
+                    two = max(two, min(one, k));
+                    one = max(one, k);
+                }
+                uint64_t both = one;
+                if (one == ~0ull || two == ~0ull) both = ~0ull;
+                else if (two != 0) both = re_order(unordered_f64(one) + unordered_f64(two));
+                if (one != 0 && both == 0) both = 1;   // open, however low
+                of_group[g] = both;
+            }
+            __syncwarp();
+            // a group stays when fewer than `kept` come before it
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int e = lane + 32 * i;
+                if (e >= a.count) continue;
+                const int g = e / per;
+                const uint64_t mine = of_group[g];
+                int before = 0;
+                for (int h = 0; h < a.groups; h++) before += of_group[h] > mine || (of_group[h] == mine && h < g);
+                if (before >= a.kept) key[i] = 0;
+            }
+        }
+    }
+    // the choices, one after the other; lane j keeps choice j
+    int32_t mine = -1;
+    float mine_logit = -INFINITY;
+    for (int j = 0; j < a.choices; j++) {
+        uint64_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; i++) best = max(best, key[i]);
+        best = re_max(best);
+        if (best == 0) break;
+        uint32_t at = 0xffffffffu;
+        float with = 0.0f;
+#pragma unroll
+        for (int i = V - 1; i >= 0; i--)
+            if (key[i] == best) { at = lane + 32 * i; with = logit[i]; }
+        const uint32_t chosen = __reduce_min_sync(0xffffffffu, at);
+        with = __shfl_sync(0xffffffffu, with, chosen & 31);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (chosen == lane + 32 * i) key[i] = 0;
+        if (lane == j) { mine = (int32_t)chosen; mine_logit = with; }
+    }
+    float w = 0.0f;
+    if (a.sigmoid && !a.renormalize) {
+        w = 1.0f / (1.0f + expf(-mine_logit));
+    } else {
+        // log s up to what all share; sums of exponentials below the largest
+        const float z = a.sigmoid ? fminf(mine_logit, 0.0f) - log1pf(expf(-fabsf(mine_logit))) : mine_logit;
+        const float zz = mine < 0 ? -INFINITY : isnan(mine_logit) ? mine_logit : z;
+        float most = zz;
+        if (a.renormalize) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        } else {
+            most = top;
+        }
+        w = mine < 0 ? 0.0f : expf(zz - most);
+        float sum = 0.0f;
+        if (a.renormalize) {
+            sum = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) sum += logit[i] == -INFINITY ? 0.0f : expf(logit[i] - top);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (mine >= 0) w /= sum;
+        if (!a.sigmoid) {   // a NaN or +inf anywhere leaves no score of the row a number
+            bool odd = top == INFINITY;
+#pragma unroll
+            for (int i = 0; i < V; i++) odd = odd || isnan(logit[i]);
+            if (__any_sync(0xffffffffu, odd)) w = NAN;
+        }
+    }
+    if (lane < a.choices) {
+        a.experts[row * a.choices + lane] = mine;
+        a.weights[row * a.choices + lane] = mine < 0 ? 0.0f : a.scale * w;
+        atomicAdd(counts + (mine < 0 ? a.count : mine), 1);
+    }
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(RE_WARPS * 32)
 re_choose_kernel(const ReArgs a)
@@ -47,142 +183,10 @@ re_choose_kernel(const ReArgs a)
     extern __shared__ unsigned char raw_smem[];
     int32_t* const counts = reinterpret_cast<int32_t*>(raw_smem);                              // [experts + 1]
     double* const scratch = reinterpret_cast<double*>(raw_smem + ((a.count + 1) * 4 + 15) / 16 * 16) + (threadIdx.x / 32) * (a.count + a.groups);
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     for (int i = threadIdx.x; i <= a.count; i += RE_WARPS * 32) counts[i] = 0;
     __syncthreads();
-    const bool plain = a.bias == nullptr && a.groups == 1;   // the logits decide
-    const int per = a.count / a.groups;
     const int64_t first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.n);
-    for (int64_t row = first + warp; row < last; row += RE_WARPS) {
-        const T* const l = static_cast<const T*>(a.logits) + row * a.row;
-        float logit[V];
-        uint64_t key[V];
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int e = lane + 32 * i;
-            logit[i] = e < a.count ? tl_get(l + e) : -INFINITY;
-            top = fmaxf(top, logit[i]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (plain) {
-#pragma unroll
-            for (int i = 0; i < V; i++) key[i] = re_order((double)logit[i]);
-        } else {
-            double s[V], sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                if (a.sigmoid) {
-                    s[i] = 1.0 / (1.0 + exp(-(double)logit[i]));
-                } else {
-                    s[i] = logit[i] == -INFINITY ? 0.0 : exp((double)logit[i] - (double)top);
-                    sum += s[i];
-                }
-            }
-            if (!a.sigmoid) {
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            }
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int e = lane + 32 * i;
-                const double v = (a.sigmoid ? s[i] : s[i] / sum) + (a.bias != nullptr && e < a.count ? (double)a.bias[e] : 0.0);
-                key[i] = logit[i] == -INFINITY ? 0ull : re_order(v);
-            }
-            if (a.groups > 1) {
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < V; i++)
-                    if (lane + 32 * i < a.count) scratch[lane + 32 * i] = __longlong_as_double((long long)key[i]);
-                __syncwarp();
-                uint64_t* const of_group = reinterpret_cast<uint64_t*>(scratch + a.count);
-                for (int g = lane; g < a.groups; g += 32) {
-                    uint64_t one = 0, two = 0;
-                    for (int j = 0; j < per; j++) {
-                        const uint64_t k = (uint64_t)__double_as_longlong(scratch[g * per + j]);
-                        two = max(two, min(one, k));
-                        one = max(one, k);
-                    }
-                    uint64_t both = one;
-                    if (one == ~0ull || two == ~0ull) both = ~0ull;
-                    else if (two != 0) both = re_order(unordered_f64(one) + unordered_f64(two));
-                    if (one != 0 && both == 0) both = 1;   // open, however low
-                    of_group[g] = both;
-                }
-                __syncwarp();
-                // a group stays when fewer than `kept` come before it
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const int e = lane + 32 * i;
-                    if (e >= a.count) continue;
-                    const int g = e / per;
-                    const uint64_t mine = of_group[g];
-                    int before = 0;
-                    for (int h = 0; h < a.groups; h++) before += of_group[h] > mine || (of_group[h] == mine && h < g);
-                    if (before >= a.kept) key[i] = 0;
-                }
-            }
-        }
-        // the choices, one after the other; lane j keeps choice j
-        int32_t mine = -1;
-        float mine_logit = -INFINITY;
-        for (int j = 0; j < a.choices; j++) {
-            uint64_t best = key[0];
-#pragma unroll
-            for (int i = 1; i < V; i++) best = max(best, key[i]);
-            best = re_max(best);
-            if (best == 0) break;
-            uint32_t at = 0xffffffffu;
-            float with = 0.0f;
-#pragma unroll
-            for (int i = V - 1; i >= 0; i--)
-                if (key[i] == best) { at = lane + 32 * i; with = logit[i]; }
-            const uint32_t chosen = __reduce_min_sync(0xffffffffu, at);
-            with = __shfl_sync(0xffffffffu, with, chosen & 31);
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                if (chosen == lane + 32 * i) key[i] = 0;
-            if (lane == j) { mine = (int32_t)chosen; mine_logit = with; }
-        }
-        float w = 0.0f;
-        if (a.sigmoid && !a.renormalize) {
-            w = 1.0f / (1.0f + expf(-mine_logit));
-        } else {
-            // log s up to what all share; sums of exponentials below the largest
-            const float z = a.sigmoid ? fminf(mine_logit, 0.0f) - log1pf(expf(-fabsf(mine_logit))) : mine_logit;
-            const float zz = mine < 0 ? -INFINITY : isnan(mine_logit) ? mine_logit : z;
-            float most = zz;
-            if (a.renormalize) {
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            } else {
-                most = top;
-            }
-            w = mine < 0 ? 0.0f : expf(zz - most);
-            float sum = 0.0f;
-            if (a.renormalize) {
-                sum = w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) sum += logit[i] == -INFINITY ? 0.0f : expf(logit[i] - top);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (mine >= 0) w /= sum;
-            if (!a.sigmoid) {   // a NaN or +inf anywhere leaves no score of the row a number
-                bool odd = top == INFINITY;
-#pragma unroll
-                for (int i = 0; i < V; i++) odd = odd || isnan(logit[i]);
-                if (__any_sync(0xffffffffu, odd)) w = NAN;
-            }
-        }
-        if (lane < a.choices) {
-            a.experts[row * a.choices + lane] = mine;
-            a.weights[row * a.choices + lane] = mine < 0 ? 0.0f : a.scale * w;
-            atomicAdd(counts + (mine < 0 ? a.count : mine), 1);
-        }
-    }
+    for (int64_t row = first + threadIdx.x / 32; row < last; row += RE_WARPS) re_row<T, V>(a, row, scratch, counts);
     __syncthreads();
     for (int i = threadIdx.x; i <= a.count; i += RE_WARPS * 32) a.counts[(int64_t)i * gridDim.x + blockIdx.x] = counts[i];
 }
@@ -199,18 +203,12 @@ __device__ __forceinline__ uint32_t rt_order(float key)
     const uint32_t bits = __float_as_uint(key + 0.0f);
     return (bits ^ (uint32_t)((int32_t)bits >> 31 | (int32_t)0x80000000)) - 0x007fffffu;
 }
-__device__ __forceinline__ uint64_t rt_order(double key) { return re_order(key); }
 __device__ __forceinline__ float rt_value(uint32_t order)
 {
     const uint32_t bits = order + 0x007fffffu;
     return __uint_as_float(bits ^ (uint32_t)(~((int32_t)bits >> 31) | (int32_t)0x80000000));
 }
-__device__ __forceinline__ double rt_value(uint64_t order) { return order == ~0ull ? NAN : unordered_f64(order); }
 __device__ __forceinline__ bool rt_nan(uint32_t order) { return order == 0xff800000u; }
-__device__ __forceinline__ bool rt_nan(uint64_t order) { return order == ~0ull; }
-template <typename K> struct RtOrder { using type = uint32_t; };
-template <> struct RtOrder<double> { using type = uint64_t; };
-
 // 32 rows from `row0` on to `tile` (`pitch` floats a row), rows behind the last as zeros.
 template <typename T>
 __device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* tile, int pitch, int wide)
@@ -244,8 +242,8 @@ __device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* t
 }
 
 // Puts key k of expert e where it belongs among the largest: behind those that are equal.
-template <typename O, int MOST>
-__device__ __forceinline__ void rt_insert(O k, int e, int (&chosen)[MOST], O (&order)[MOST])
+template <int MOST>
+__device__ __forceinline__ void rt_insert(uint32_t k, int e, int (&chosen)[MOST], uint32_t (&order)[MOST])
 {
     if (k <= order[MOST - 1]) return;
 #pragma unroll
@@ -260,35 +258,34 @@ __device__ __forceinline__ void rt_insert(O k, int e, int (&chosen)[MOST], O (&o
     }
 }
 
-// The experts of a lane's row.  key_of(e): keys of type K in their order, as often as asked; MOST: choices and two more, the first that are left out.  False: keys
-// that are off by up to `near` may have decided.  same(p, q): two experts have the same logit and bias, and so the same key, whatever its type.
-template <typename K, int MOST, int GROUPS, typename Key, typename Same>
-__device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)[MOST], Key&& key_of, Same&& same)
+// The experts of a lane's row.  key_of(e): keys in their order, as often as asked; MOST: choices and two or more, the first that are left out.
+// False: keys that are off by up to `near` may have decided.  same(p, q): two experts have the same logit and bias, and so the same key, whatever its type.
+template <int MOST, int GROUPS, typename Key, typename Same>
+__device__ __forceinline__ bool rt_choose(const ReArgs& a, float near, int (&chosen)[MOST], Key&& key_of, Same&& same)
 {
-    using O = typename RtOrder<K>::type;
     bool sure = true;
     uint32_t kept = 0xffffffffu;
     const int per = a.count / a.groups;
     if constexpr (GROUPS > 1) {
-        O of_group[GROUPS];
+        uint32_t of_group[GROUPS];
 #pragma unroll
         for (int g = 0; g < GROUPS; g++) {
             of_group[g] = 0;
             if (g >= a.groups) continue;
-            O one = 0, two = 0;
+            uint32_t one = 0, two = 0;
 #pragma unroll 4
             for (int i = 0; i < per; i++) {
-                const O k = key_of(g * per + i);
+                const uint32_t k = key_of(g * per + i);
                 two = max(two, min(one, k));
                 one = max(one, k);
             }
-            O both = one;
+            uint32_t both = one;
             if (two != 0) both = rt_nan(one) ? one : rt_order(rt_value(one) + rt_value(two));
             if (one != 0 && both == 0) both = 1;   // open, however low
             of_group[g] = both;
         }
         kept = 0;
-        O lowest = ~(O)0, highest = 0;   // of those that stay, and of the others
+        uint32_t lowest = ~0u, highest = 0;   // of those that stay, and of the others
 #pragma unroll
         for (int g = 0; g < GROUPS; g++) {
             if (g >= a.groups) continue;
@@ -302,9 +299,9 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)
                 highest = max(highest, of_group[g]);
             }
         }
-        if (highest != 0) sure = rt_value(lowest) - rt_value(highest) > (K)6 * near;
+        if (highest != 0) sure = rt_value(lowest) - rt_value(highest) > 6.0f * near;
     }
-    O order[MOST];
+    uint32_t order[MOST];
 #pragma unroll
     for (int j = 0; j < MOST; j++) {
         order[j] = 0;
@@ -319,32 +316,52 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, K near, int (&chosen)
 #pragma unroll
     for (int j = 0; j + 1 < MOST; j++) {
         if (order[j + 1] == 0 || j > a.choices || (j == a.choices && !tie)) continue;
-        if (rt_value(order[j]) - rt_value(order[j + 1]) > (K)2 * near) continue;
+        if (rt_value(order[j]) - rt_value(order[j + 1]) > 2.0f * near) continue;
         tie = j == a.choices - 1;
         if (j == a.choices || !same(chosen[j], chosen[j + 1])) sure = false;
     }
     return sure;
 }
 
-// A row once more in 64 bits.
-template <typename T, int MOST, int GROUPS>
-__device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, const float* bias, float top, int* out)
+// The weights of a row's choices and its entries in the counts.  sum: of the row's exponentials below `top`, for softmax without renormalising; odd: a logit is NaN.
+template <typename T, int MOST>
+__device__ __forceinline__ void rt_weigh(const ReArgs& a, int64_t row, const int (&chosen)[MOST], float top, float sum, bool odd, int32_t* counts)
 {
-    const T* const l = static_cast<const T*>(a.logits) + row * a.row;
-    double sum = 0.0;
-    if (!a.sigmoid)
-        for (int e = 0; e < a.count; e++) sum += tl_get(l + e) == -INFINITY ? 0.0 : exp((double)tl_get(l + e) - (double)top);
-    int chosen[MOST];
-    (void)rt_choose<double, MOST, GROUPS>(
-        a, 0.0, chosen,
-        [&](int e) -> uint64_t {
-            const double v = (double)tl_get(l + e);
-            if (v == -INFINITY) return 0;
-            return re_order((a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - (double)top) / sum) + (double)bias[e]);
-        },
-        [](int, int) { return true; });
-    for (int j = 0; j < a.choices; j++) out[j] = chosen[j];
+    const T* const from = static_cast<const T*>(a.logits) + row * a.row;
+    odd = odd || top == INFINITY;
+    float w[MOST], most = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < MOST; j++) {
+        const bool have = j < a.choices && chosen[j] >= 0;
+        const float v = have ? tl_get(from + chosen[j]) : 0.0f;
+        // log s up to what all share; sums of exponentials below the largest
+        w[j] = !a.sigmoid || !a.renormalize ? v : isnan(v) ? v : fminf(v, 0.0f) - log1pf(expf(-fabsf(v)));
+        if (have) most = fmaxf(most, w[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < MOST; j++) {
+        if (j >= a.choices || chosen[j] < 0) continue;
+        if (a.renormalize) {
+            w[j] = expf(w[j] - most);
+            total += w[j];
+        } else {
+            w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-w[j])) : expf(w[j] - top) / sum;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MOST; j++) {
+        if (j >= a.choices) continue;
+        float v = chosen[j] < 0 ? 0.0f : a.renormalize ? w[j] / total : w[j];
+        if (!a.sigmoid && odd && chosen[j] >= 0) v = NAN;   // a NaN or +inf anywhere leaves no score of the row a number
+        a.experts[row * a.choices + j] = chosen[j];
+        a.weights[row * a.choices + j] = chosen[j] < 0 ? 0.0f : a.scale * v;
+        atomicAdd(counts + (chosen[j] < 0 ? a.count : chosen[j]), 1);
+    }
 }
+
+// A row from the start in 64 bits, by the whole warp (by one lane the others wait for: 131 in place of 100 us).
+template <typename T>
+__device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, double* scratch, int32_t* counts) { re_row<T, RT_MAX_EXPERTS / 32>(a, row, scratch, counts); }
 
 // GROUPS: 0 where the logits decide, 1 without groups, else their largest number.
 template <typename T, int MOST, int GROUPS>
@@ -374,7 +391,8 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
         __syncwarp();
         rt_bring<T>(a, row0, tile, pitch, wide);
         __syncwarp();
-        if (row >= last) continue;
+        bool again = false;
+        if (row < last) {
         int chosen[MOST];
         float top = -INFINITY, sum = 0.0f;
         bool odd = false;
@@ -420,44 +438,16 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
                 l[e] = __uint_as_float(closed ? 0u : rt_order(key + bias[e]));
             }
             const T* const from = static_cast<const T*>(a.logits) + row * a.row;
-            if (!rt_choose<float, MOST, GROUPS>(
-                    a, near, chosen, [&](int e) { return __float_as_uint(l[e]); },
-                    [&](int p, int q) { return tl_get(from + p) == tl_get(from + q) && bias[p] == bias[q]; })) {
-                int again[MOST];   // on the way through memory, as `chosen` must not be
-                rt_again<T, MOST, GROUPS>(a, row, bias, top, again);
-#pragma unroll
-                for (int j = 0; j < MOST; j++) chosen[j] = j < a.choices ? again[j] : -1;
-            }
+            // what is to be done once more waits until nothing else is in registers
+            again = !rt_choose<MOST, GROUPS>(
+                a, near, chosen, [&](int e) { return __float_as_uint(l[e]); },
+                [&](int p, int q) { return tl_get(from + p) == tl_get(from + q) && bias[p] == bias[q]; });
         }
-        odd = odd || top == INFINITY;
-        const T* const from = static_cast<const T*>(a.logits) + row * a.row;
-        float w[MOST], most = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int j = 0; j < MOST; j++) {
-            const bool have = j < a.choices && chosen[j] >= 0;
-            const float v = have ? (PLAIN ? l[chosen[j]] : tl_get(from + chosen[j])) : 0.0f;
-            // log s up to what all share; sums of exponentials below the largest
-            w[j] = !a.sigmoid || !a.renormalize ? v : isnan(v) ? v : fminf(v, 0.0f) - log1pf(expf(-fabsf(v)));
-            if (have) most = fmaxf(most, w[j]);
+        if (!again) rt_weigh<T, MOST>(a, row, chosen, top, sum, odd, counts);
         }
-#pragma unroll
-        for (int j = 0; j < MOST; j++) {
-            if (j >= a.choices || chosen[j] < 0) continue;
-            if (a.renormalize) {
-                w[j] = expf(w[j] - most);
-                total += w[j];
-            } else {
-                w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-w[j])) : expf(w[j] - top) / sum;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < MOST; j++) {
-            if (j >= a.choices) continue;
-            float v = chosen[j] < 0 ? 0.0f : a.renormalize ? w[j] / total : w[j];
-            if (!a.sigmoid && odd && chosen[j] >= 0) v = NAN;   // a NaN or +inf anywhere leaves no score of the row a number
-            a.experts[row * a.choices + j] = chosen[j];
-            a.weights[row * a.choices + j] = chosen[j] < 0 ? 0.0f : a.scale * v;
-            atomicAdd(counts + (chosen[j] < 0 ? a.count : chosen[j]), 1);
+        if constexpr (!PLAIN) {   // the rows' places serve as scratch meanwhile
+            double* const scratch = reinterpret_cast<double*>(tile + (reinterpret_cast<uintptr_t>(tile) % 8 != 0));
+            for (uint32_t todo = __ballot_sync(0xffffffffu, again); todo != 0; todo &= todo - 1) rt_again<T>(a, row0 + __ffs(todo) - 1, scratch, counts);
         }
     }
     __syncthreads();
