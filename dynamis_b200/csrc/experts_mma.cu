@@ -18,9 +18,9 @@ namespace dynb {
 
 // Warps that gather, and that store results.  An SM's four schedulers have room for five warps of 96 registers each, or four of 128: rows in fp32 wait in the registers of
 // their threads and need the latter.
-constexpr int EM_FEED = 8;
+template <typename T> constexpr int EM_FEED = sizeof(T) == 4 ? 16 : 8;
 constexpr int EM_COLUMNS = 16;                                       // columns that a warp takes out of tensor memory at a time
-__host__ __device__ constexpr int em_threads(int out) { return (out + 2 + EM_FEED) * 32; }
+template <typename T> __host__ __device__ constexpr int em_threads(int out) { return (out + 2 + EM_FEED<T>) * 32; }
 constexpr int EM_MAX_STAGES = 8;
 constexpr int EM_SMEM = 220 * 1024;                                  // beside 4 KB of offsets and barriers
 constexpr int EM_RAW = 3;                                            // stages of rows and slopes on their way beside those of the products
@@ -198,11 +198,11 @@ __device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS], uint32
 
 // O: type of the results (fp32 for gradients that are summed over the choices before they are rounded).
 template <typename T, typename O, EmPath PATH, bool WIDE, int OUT>
-__global__ void __launch_bounds__(em_threads(OUT), 1)
+__global__ void __launch_bounds__(em_threads<T>(OUT), 1)
 em_rows_kernel(const ExArgs e, const EmPlan plan)
 {
     constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = EM_COLUMNS, WORDS = COLUMNS * SIZE / 4;   // columns that a warp takes at a time
-    constexpr int SHARES = OUT / 4;
+    constexpr int SHARES = OUT / 4, FEED = EM_FEED<T>;
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EmBars bars;
@@ -215,7 +215,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], PATH == EM_ASYNC ? EM_FEED * 32 : EM_FEED);
+            bar_init(&bars.full[s], PATH == EM_ASYNC ? FEED * 32 : FEED);
             bar_init(&bars.empty[s], 1);
             bar_init(&bars.b_full[s], 1);
         }
@@ -402,13 +402,13 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         const int64_t in_row = plan.back ? a.dy_row : a.x_row;
         const int fan = plan.back ? 1 : e.fan;
         const uint32_t rows_in = (uint32_t)(plan.back ? a.n : e.n_in);
-        constexpr int UNITS = TM_ROWS * 8 / (EM_FEED * 32);
+        constexpr int UNITS = TM_ROWS * 8 / (FEED * 32);
         const int tid = threadIdx.x - (OUT + 2) * 32, piece = tid & 7;
         int32_t rows[UNITS], rows_next[UNITS];      // of the next tile to ask for, and the one behind it
         auto rows_of = [&](const TlTile& t, int32_t (&r)[UNITS]) {
 #pragma unroll
             for (int i = 0; i < UNITS; i++) {
-                const int64_t place = t.begin + (tid >> 3) + (EM_FEED * 4) * i;
+                const int64_t place = t.begin + (tid >> 3) + (FEED * 4) * i;
                 r[i] = t.type >= 0 && place < t.end ? __ldg(a.order + place) : -1;   // looked at a tile later
             }
         };
@@ -427,12 +427,12 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                 rows_of(cursor.tile, rows);
                 for (int chunk = 0; chunk < plan.chunks; chunk++) {
                     if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); ok = false; break; }
-                    const uint32_t to = smem_addr(stage0) + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);   // EM_FEED * 4 rows on: the same place among eight
+                    const uint32_t to = smem_addr(stage0) + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);   // FEED * 4 rows on: the same place among eight
                     const int k = chunk * 64 + piece * 8;
 #pragma unroll
                     for (int i = 0; i < UNITS; i++) {
                         const bool live = at[i] < rows_in && k < kk;
-                        copy_16(to + i * EM_FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
+                        copy_16(to + i * FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
                     }
                     copies_arrive(&bars.full[stage]);
                     if (++stage == plan.stages) { stage = 0; phase ^= 1; }
@@ -443,7 +443,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         } else if constexpr (PATH == EM_ASYNC_SLOPE) {
             // Rows and slopes come to places that are this thread's own, EM_RAW stages of them, and go from there, multiplied, to the stages of the products
             const uint32_t raw = smem_addr(stage0) + plan.stages * plan.stage_bytes + tid * 16;
-            constexpr uint32_t UNIT = EM_FEED * 512, SLOT = 2 * UNITS * UNIT;
+            constexpr uint32_t UNIT = FEED * 512, SLOT = 2 * UNITS * UNIT;
             const bool keep_du = e.du != nullptr && blockIdx.y == 0;
             TmCursor behind = cursor;               // of the stage that is multiplied, for du
             int chunk = 0, behind_chunk = 0, slot = 0, behind_slot = 0;
@@ -508,7 +508,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             }
             copies_wait(0);
         } else {
-            constexpr int AHEAD = sizeof(T) == 4 && PATH == EM_SLOPE ? 1 : 2;
+            constexpr int AHEAD = sizeof(T) == 2 ? 2 : PATH == EM_SLOPE ? 1 : 2;
             constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
             TlTile next = cursor.tile;
             int chunk = 0;
@@ -562,10 +562,10 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
                     if (tm_odd(v[s])) {
 #pragma unroll
-                        for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * EM_FEED * 512, TM_ROWS * 128);
+                        for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * FEED * 512, TM_ROWS * 128);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * EM_FEED * 512, TM_ROWS * 128);
+                        for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * FEED * 512, TM_ROWS * 128);
                     }
                     fence_to_tensor();
                     __syncwarp();
@@ -950,7 +950,7 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
     rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
     if (rc != cudaSuccess) return rc;
-    kernel<<<grid, em_threads(many ? MANY : FEW), p.smem, s>>>(e, p);
+    kernel<<<grid, em_threads<T>(many ? MANY : FEW), p.smem, s>>>(e, p);
     return cudaGetLastError();
 }
 
