@@ -584,7 +584,9 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 
 // ------------------------------------------------------------------------------------------------ gradients of the matrices
 // Warps that store sums, issue products, sum up the offsets' gradient, and gather.
-constexpr int EW_OUT = 4, EW_SUM = 4, EW_FEED = 16, EW_THREADS = (EW_OUT + 1 + EW_SUM + EW_FEED) * 32, EW_MAX_STAGES = 8;
+constexpr int EW_OUT = 4, EW_FEED = 16, EW_MAX_STAGES = 8;
+template <typename T> constexpr int EW_SUM = sizeof(T) == 4 ? 2 : 4;
+template <typename T> constexpr int EW_THREADS = (EW_OUT + 1 + EW_SUM<T> + EW_FEED) * 32;
 template <typename T> constexpr int EW_ROWS = sizeof(T) == 4 ? 32 : 64;   // pairs of a stage
 constexpr int EW_SMEM = 222 * 1024;
 
@@ -638,7 +640,7 @@ struct EwCursor {
 };
 
 template <typename T, EmPath PATH, bool WIDE>
-__global__ void __launch_bounds__(EW_THREADS, 1)
+__global__ void __launch_bounds__(EW_THREADS<T>, 1)
 em_weights_kernel(const ExArgs e, const EwPlan plan)
 {
     constexpr int PARTS = TmParts<T>::N, FEED_THREADS = EW_FEED * 32, ROWS = EW_ROWS<T>, BLOCK = ROWS * 128;
@@ -659,7 +661,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
             bar_init(&bars.full[s], PATH == EM_ASYNC ? EW_FEED * 32 : EW_FEED);
-            bar_init(&bars.empty[s], sums_wanted ? 1 + EW_SUM : 1);
+            bar_init(&bars.empty[s], sums_wanted ? 1 + EW_SUM<T> : 1);
         }
         for (int b = 0; b < 2; b++) {
             bar_init(&bars.sums_full[b], 1);
@@ -739,7 +741,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             if (buffer == 0) sums_phase ^= 1;
         }
         if (!ok) tm_ran_out(a);
-    } else if (warp < EW_OUT + 1 + EW_SUM) {
+    } else if (warp < EW_OUT + 1 + EW_SUM<T>) {
         // the offsets' gradient: a thread sums two columns of the stages as they stand in shared memory, all parts
         if (sums_wanted) {
             const int c = (threadIdx.x - (EW_OUT + 1) * 32) * 2, have = min(plan.columns, a.outer - col0);
@@ -784,7 +786,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
     } else {
         // a thread takes pieces of one pair's rows, piece `piece` of every block (of every other one): number, division and addresses of the pair are its own, once a stage
         constexpr int GROUPS = FEED_THREADS / (ROWS * 8);
-        const int tid = threadIdx.x - (EW_OUT + 1 + EW_SUM) * 32, piece = tid & 7, group = (tid >> 3) % GROUPS, r = tid / (8 * GROUPS);
+        const int tid = threadIdx.x - (EW_OUT + 1 + EW_SUM<T>) * 32, piece = tid & 7, group = (tid >> 3) % GROUPS, r = tid / (8 * GROUPS);
         const int at0 = group * PARTS * BLOCK + (int)tile_piece(r, piece), y_limit = min(a.outer, col0 + plan.columns);
         // the pair of the next stage
         int64_t place = cursor.begin;
@@ -837,30 +839,39 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             copies_commit();
             copies_wait(0);
         } else {
-            TmRaw<T> v[UNITS] = {};
-            auto fetch = [&](int32_t p) { units_of(p, [&](int i, const T* from, int have) { v[i] = tm_load<WIDE>(from, 1, have); }); };
-            // the rows of the next stage are asked for behind this one, their numbers a stage earlier
-            fetch(id);
-            bool behind = row_of(id);
-            while (more) {
-                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
-                unsigned char* const to = stage0 + stage * stage_bytes + at0;
-                if (tm_odd(v)) {
+            // two stages under way in registers, the number of the next pair a stage earlier
+            constexpr int AHEAD = 2;
+            TmRaw<T> v[AHEAD][UNITS] = {};
+            bool live[AHEAD];
+            auto fetch = [&](int s) {
+                units_of(id, [&](int i, const T* from, int have) { v[s][i] = tm_load<WIDE>(from, 1, have); });
+                live[s] = more;
+                more = row_of(id);
+            };
 #pragma unroll
-                    for (int i = 0; i < UNITS; i++)
-                        if (i * GROUPS + group < blocks) tm_store<true>(v[i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
-                } else {
+            for (int s = 0; s < AHEAD; s++) fetch(s);
+            bool ok = true;
+            while (ok) {
 #pragma unroll
-                    for (int i = 0; i < UNITS; i++)
-                        if (i * GROUPS + group < blocks) tm_store<false>(v[i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
+                for (int s = 0; s < AHEAD; s++) {
+                    if (!live[s]) { ok = false; break; }
+                    if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); ok = false; break; }
+                    unsigned char* const to = stage0 + stage * stage_bytes + at0;
+                    if (tm_odd(v[s])) {
+#pragma unroll
+                        for (int i = 0; i < UNITS; i++)
+                            if (i * GROUPS + group < blocks) tm_store<true>(v[s][i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < UNITS; i++)
+                            if (i * GROUPS + group < blocks) tm_store<false>(v[s][i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
+                    }
+                    fence_to_tensor();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(&bars.full[stage]);
+                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                    fetch(s);   // behind the last stage: zeros
                 }
-                fence_to_tensor();
-                __syncwarp();
-                if (lane == 0) bar_arrive(&bars.full[stage]);
-                if (++stage == plan.stages) { stage = 0; phase ^= 1; }
-                fetch(id);   // behind the last stage: zeros
-                more = behind;
-                behind = row_of(id);
             }
         }
     }
@@ -998,7 +1009,7 @@ static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
     const int smem = 1024 + p.stages * stage, tiles_of = p.row_tiles * p.column_tiles;
     const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    kernel<<<(unsigned)(std::max(1, ex_slices(a.inner, a.outer, sizeof(T))) * tiles_of), EW_THREADS, smem, s>>>(e, p);
+    kernel<<<(unsigned)(std::max(1, ex_slices(a.inner, a.outer, sizeof(T))) * tiles_of), EW_THREADS<T>, smem, s>>>(e, p);
     return cudaGetLastError();
 }
 
