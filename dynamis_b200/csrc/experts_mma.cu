@@ -108,6 +108,10 @@ ex_pack_kernel(const T* w, int64_t experts, int inner, int outer, int back, int 
     }
 }
 
+// The warps that gather by way of registers in fp32 are two teams, which take the stages by turns: what a warp does for a stage is one long chain (wait, conversion, stores,
+// fence, addresses of the next), and while one team is in it the other is, too (200 k pairs 512 x 128: one team with two stages ahead 174 us, rows' pass).
+template <typename T, EmPath PATH> constexpr int EM_TEAMS = sizeof(T) == 4 && PATH == EM_REGISTERS ? 2 : 1;
+
 // Eight elements times their slopes.
 template <typename T>
 __device__ __forceinline__ void em_times(TmRaw<T>& v, const TmRaw<T>& slope)
@@ -203,6 +207,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 {
     constexpr int PARTS = TmParts<T>::N, A_BYTES = PARTS * TM_ROWS * 128, SIZE = (int)sizeof(O), COLUMNS = EM_COLUMNS, WORDS = COLUMNS * SIZE / 4;   // columns that a warp takes at a time
     constexpr int SHARES = OUT / 4, FEED = EM_FEED<T>;
+    constexpr int TEAMS = EM_TEAMS<T, PATH>, TEAM = FEED / TEAMS;
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EmBars bars;
@@ -215,7 +220,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], PATH == EM_ASYNC ? FEED * 32 : FEED);
+            bar_init(&bars.full[s], PATH == EM_ASYNC ? FEED * 32 : TEAM);
             bar_init(&bars.empty[s], 1);
             bar_init(&bars.b_full[s], 1);
         }
@@ -402,13 +407,13 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         const int64_t in_row = plan.back ? a.dy_row : a.x_row;
         const int fan = plan.back ? 1 : e.fan;
         const uint32_t rows_in = (uint32_t)(plan.back ? a.n : e.n_in);
-        constexpr int UNITS = TM_ROWS * 8 / (FEED * 32);
-        const int tid = threadIdx.x - (OUT + 2) * 32, piece = tid & 7;
+        constexpr int UNITS = TM_ROWS * 8 / (TEAM * 32);
+        const int team = (warp - OUT - 2) / TEAM, tid = threadIdx.x - (OUT + 2 + team * TEAM) * 32, piece = tid & 7;
         int32_t rows[UNITS], rows_next[UNITS];      // of the next tile to ask for, and the one behind it
         auto rows_of = [&](const TlTile& t, int32_t (&r)[UNITS]) {
 #pragma unroll
             for (int i = 0; i < UNITS; i++) {
-                const int64_t place = t.begin + (tid >> 3) + (FEED * 4) * i;
+                const int64_t place = t.begin + (tid >> 3) + (TEAM * 4) * i;
                 r[i] = t.type >= 0 && place < t.end ? __ldg(a.order + place) : -1;   // looked at a tile later
             }
         };
@@ -427,12 +432,12 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                 rows_of(cursor.tile, rows);
                 for (int chunk = 0; chunk < plan.chunks; chunk++) {
                     if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); ok = false; break; }
-                    const uint32_t to = smem_addr(stage0) + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);   // FEED * 4 rows on: the same place among eight
+                    const uint32_t to = smem_addr(stage0) + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);   // TEAM * 4 rows on: the same place among eight
                     const int k = chunk * 64 + piece * 8;
 #pragma unroll
                     for (int i = 0; i < UNITS; i++) {
                         const bool live = at[i] < rows_in && k < kk;
-                        copy_16(to + i * FEED * 512, in + (live ? at[i] * in_row + k : 0), live);
+                        copy_16(to + i * TEAM * 512, in + (live ? at[i] * in_row + k : 0), live);
                     }
                     copies_arrive(&bars.full[stage]);
                     if (++stage == plan.stages) { stage = 0; phase ^= 1; }
@@ -443,7 +448,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         } else if constexpr (PATH == EM_ASYNC_SLOPE) {
             // Rows and slopes come to places that are this thread's own, EM_RAW stages of them, and go from there, multiplied, to the stages of the products
             const uint32_t raw = smem_addr(stage0) + plan.stages * plan.stage_bytes + tid * 16;
-            constexpr uint32_t UNIT = FEED * 512, SLOT = 2 * UNITS * UNIT;
+            constexpr uint32_t UNIT = TEAM * 512, SLOT = 2 * UNITS * UNIT;
             const bool keep_du = e.du != nullptr && blockIdx.y == 0;
             TmCursor behind = cursor;               // of the stage that is multiplied, for du
             int chunk = 0, behind_chunk = 0, slot = 0, behind_slot = 0;
@@ -508,7 +513,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             }
             copies_wait(0);
         } else {
-            constexpr int AHEAD = sizeof(T) == 2 ? 2 : PATH == EM_SLOPE ? 1 : 2;
+            constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
             constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
             TlTile next = cursor.tile;
             int chunk = 0;
@@ -517,6 +522,19 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             uint32_t row_du[AHEAD][SLOPES];         // pair whose du is kept, or a number that is none; its first column
             int k_du[AHEAD];
             const bool keep_du = PATH == EM_SLOPE && e.du != nullptr && blockIdx.y == 0;
+            auto step = [&](int stages) {           // on to a stage behind the next
+                for (int i = 0; i < stages && next.type >= 0; i++) {
+                    if (++chunk < plan.chunks) continue;
+                    chunk = 0;
+                    next = cursor.tile;
+#pragma unroll
+                    for (int j = 0; j < UNITS; j++) rows[j] = rows_next[j];
+                    if (next.type >= 0) {
+                        cursor.next(a);
+                        rows_of(cursor.tile, rows_next);
+                    }
+                }
+            };
             auto ask = [&](TmRaw<T> (&to)[UNITS], TmRaw<T> (&to_slope)[SLOPES], uint32_t (&to_du)[SLOPES], int& to_k, bool& any) {
                 any = next.type >= 0;
                 if (!any) return;
@@ -530,20 +548,13 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     to[i] = tm_load<WIDE>(in + (ok ? at * in_row + k : 0), 1, ok ? have : 0);
                     if constexpr (PATH == EM_SLOPE) to_slope[i] = tm_load<WIDE>(static_cast<const T*>(e.slope) + (ok ? (int64_t)at * kk + k : 0), 1, ok ? have : 0);
                 }
-                if (++chunk == plan.chunks) {
-                    chunk = 0;
-                    next = cursor.tile;
-#pragma unroll
-                    for (int i = 0; i < UNITS; i++) rows[i] = rows_next[i];
-                    if (next.type >= 0) {
-                        cursor.next(a);
-                        rows_of(cursor.tile, rows_next);
-                    }
-                }
+                step(TEAMS);
             };
             rows_of(next, rows);
             if (next.type >= 0) cursor.next(a);
             rows_of(cursor.tile, rows_next);
+            step(team);
+            stage = team;
 #pragma unroll
             for (int s = 0; s < AHEAD; s++) ask(v[s], slope[s], row_du[s], k_du[s], live[s]);
             bool more = true;
@@ -562,15 +573,16 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
                     if (tm_odd(v[s])) {
 #pragma unroll
-                        for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * FEED * 512, TM_ROWS * 128);
+                        for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * TEAM * 512, TM_ROWS * 128);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * FEED * 512, TM_ROWS * 128);
+                        for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * TEAM * 512, TM_ROWS * 128);
                     }
                     fence_to_tensor();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&bars.full[stage]);
-                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                    stage += TEAMS;
+                    if (stage >= plan.stages) { stage -= plan.stages; phase ^= 1; }
                     ask(v[s], slope[s], row_du[s], k_du[s], live[s]);
                 }
             }
@@ -643,9 +655,9 @@ template <typename T, EmPath PATH, bool WIDE>
 __global__ void __launch_bounds__(EW_THREADS<T>, 1)
 em_weights_kernel(const ExArgs e, const EwPlan plan)
 {
-    constexpr int PARTS = TmParts<T>::N, FEED_THREADS = EW_FEED * 32, ROWS = EW_ROWS<T>, BLOCK = ROWS * 128;
+    constexpr int PARTS = TmParts<T>::N, TEAMS = EM_TEAMS<T, PATH>, TEAM = EW_FEED / TEAMS, FEED_THREADS = TEAM * 32, ROWS = EW_ROWS<T>, BLOCK = ROWS * 128;
     constexpr int SUMS = PARTS == 1 ? 1 : 2;    // sums of a buffer: leading parts, small ones
-    constexpr int UNITS = PARTS == 1 ? 6 : 2;   // pieces of 8 elements a thread and stage: 64 pairs x (128 + 256) elements, or 32 x (128 + 128)
+    constexpr int UNITS = PARTS == 1 ? 6 : 2 * TEAMS;   // pieces of 8 elements a thread and stage: 64 pairs x (128 + 256) elements, or 32 x (128 + 128)
     const TlArgs& a = e.t;
     extern __shared__ unsigned char raw_smem[];
     __shared__ EwBars bars;
@@ -660,7 +672,7 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < plan.stages; s++) {
-            bar_init(&bars.full[s], PATH == EM_ASYNC ? EW_FEED * 32 : EW_FEED);
+            bar_init(&bars.full[s], PATH == EM_ASYNC ? EW_FEED * 32 : TEAM);
             bar_init(&bars.empty[s], sums_wanted ? 1 + EW_SUM<T> : 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -786,18 +798,22 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
     } else {
         // a thread takes pieces of one pair's rows, piece `piece` of every block (of every other one): number, division and addresses of the pair are its own, once a stage
         constexpr int GROUPS = FEED_THREADS / (ROWS * 8);
-        const int tid = threadIdx.x - (EW_OUT + 1 + EW_SUM<T>) * 32, piece = tid & 7, group = (tid >> 3) % GROUPS, r = tid / (8 * GROUPS);
+        const int team = (warp - EW_OUT - 1 - EW_SUM<T>) / TEAM, tid = threadIdx.x - (EW_OUT + 1 + EW_SUM<T> + team * TEAM) * 32, piece = tid & 7, group = (tid >> 3) % GROUPS, r = tid / (8 * GROUPS);
         const int at0 = group * PARTS * BLOCK + (int)tile_piece(r, piece), y_limit = min(a.outer, col0 + plan.columns);
         // the pair of the next stage
         int64_t place = cursor.begin;
-        auto row_of = [&](int32_t& p) {
-            p = cursor.type >= 0 && place + r < cursor.end ? __ldg(a.order + place + r) : -1;   // looked at a stage later
-            if (cursor.type < 0) return false;
-            place += ROWS;
-            if (place >= cursor.end) {
+        auto step = [&](int stages) {
+            for (int i = 0; i < stages && cursor.type >= 0; i++) {
+                place += ROWS;
+                if (place < cursor.end) continue;
                 cursor.next(a);
                 place = cursor.begin;
             }
+        };
+        auto row_of = [&](int32_t& p) {
+            p = cursor.type >= 0 && place + r < cursor.end ? __ldg(a.order + place + r) : -1;   // looked at a stage later
+            if (cursor.type < 0) return false;
+            step(TEAMS);
             return true;
         };
         // f(unit, address, elements there are) for every unit of pair p
@@ -815,8 +831,9 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             }
         };
         int32_t id;
-        int stage = 0;
+        int stage = team;
         uint32_t phase = 1;
+        step(team);
         bool more = row_of(id);
         if constexpr (PATH == EM_ASYNC) {
             auto ask = [&](int32_t p) {
@@ -839,8 +856,8 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             copies_commit();
             copies_wait(0);
         } else {
-            // two stages under way in registers, the number of the next pair a stage earlier
-            constexpr int AHEAD = 2;
+            // the rows of the next stage are under way in registers, the number of the pair behind it
+            constexpr int AHEAD = 1;
             TmRaw<T> v[AHEAD][UNITS] = {};
             bool live[AHEAD];
             auto fetch = [&](int s) {
@@ -869,7 +886,8 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
                     fence_to_tensor();
                     __syncwarp();
                     if (lane == 0) bar_arrive(&bars.full[stage]);
-                    if (++stage == plan.stages) { stage = 0; phase ^= 1; }
+                    stage += TEAMS;
+                    if (stage >= plan.stages) { stage -= plan.stages; phase ^= 1; }
                     fetch(s);   // behind the last stage: zeros
                 }
             }
