@@ -106,7 +106,7 @@ class Routing:
 
 class _RouteExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, choices, score, groups, kept_groups, renormalize, scale):
+    def forward(ctx, logits, bias, choices, score, groups, kept_groups, renormalize, scale):   # ctx None: without gradients nothing is kept for them
         dev, (rows, experts) = logits.device, logits.shape
         logits = _row_last(logits)
         L = _lib.lib()
@@ -122,10 +122,11 @@ class _RouteExperts(torch.autograd.Function):
             ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
             _lib.check(L.dynb_route_experts(ctypes.byref(args), chosen.data_ptr(), weights.data_ptr(), order.data_ptr(), start.data_ptr(), ws.data_ptr(),
                                             ws.numel(), _lib.stream_of(dev)), "route_experts")
-        ctx.mark_non_differentiable(chosen, order, start)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, chosen, weights)
-        ctx.fixed = fixed
+        if ctx is not None:
+            ctx.mark_non_differentiable(chosen, order, start)
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(logits, chosen, weights)
+            ctx.fixed = fixed
         return chosen, weights, order, start
 
     @staticmethod
@@ -187,7 +188,10 @@ def route_experts(logits: torch.Tensor, choices: int, score: str = "softmax", bi
         bias = bias.contiguous()
     if not 1e-30 <= scale <= 1e30:
         raise RuntimeError(f"scale must lie in [1e-30, 1e30], got {scale}")
-    return Routing(*_RouteExperts.apply(logits, bias, choices, _SCORES[score], groups, kept_groups, int(bool(renormalize)), scale))
+    args = (logits, bias, choices, _SCORES[score], groups, kept_groups, int(bool(renormalize)), scale)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return Routing(*_RouteExperts.apply(*args))
+    return Routing(*_RouteExperts.forward(None, *args))     # a third of a small call's time is autograd's
 
 
 def _linear_args(weight, routing: Routing, paired: bool, activation: int, dtype) -> "_lib.ExpertLinear":
@@ -220,20 +224,20 @@ def _pairs(t: torch.Tensor) -> torch.Tensor:
 
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, routing, activation, keep):
+    def forward(ctx, x, weight, bias, routing, activation):   # ctx None: without gradients nothing is kept for them
         dev, paired = x.device, x.dim() == 3
         flat, weight = _pairs(x) if paired else _row_last(x), weight.contiguous()
         bias = None if bias is None else bias.contiguous()
         with _lib.on_device(dev):
             z = torch.empty((routing.num_rows, routing.choices, weight.size(2)), dtype=x.dtype, device=dev)
             slope = None
-            if keep and activation:
+            if ctx is not None and activation:
                 slope = torch.empty(z.shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16, device=dev)
             args = _linear_args(weight, routing, paired, activation, x.dtype)
             ws = _linear_workspace(args, 0, 0, 0, dev)
             _lib.check(_lib.lib().dynb_expert_linear(ctypes.byref(args), flat.data_ptr(), flat.stride(0), _pointer(bias), z.data_ptr(), _pointer(slope),
                                                      ws.data_ptr(), ws.numel(), _lib.stream_of(dev)), "expert_linear")
-        if keep:
+        if ctx is not None:
             ctx.save_for_backward(flat, weight, slope)
             ctx.routing, ctx.activation, ctx.shape = routing, activation, x.shape
         return z
@@ -253,7 +257,7 @@ class _ExpertLinear(torch.autograd.Function):
             _lib.check(_lib.lib().dynb_expert_linear_backward(ctypes.byref(args), x.data_ptr(), x.stride(0), d_z.data_ptr(), d_z.stride(0), _pointer(slope),
                                                      routing.experts.data_ptr(), _pointer(dx), _pointer(dw), _pointer(db), ws.data_ptr(), ws.numel(),
                                                      _lib.stream_of(dev)), "expert_linear_backward")
-        return dx, dw, db, None, None, None
+        return dx, dw, db, None, None
 
 
 def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
@@ -286,13 +290,15 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias:
             raise RuntimeError(f"bias must have shape [{weight.size(0)}, {weight.size(2)}], got {list(bias.shape)}")
     if activation not in _ACTIVATIONS:
         raise RuntimeError(f"activation must be None, 'silu' or 'gelu', got {activation!r}")
-    keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
-    return _ExpertLinear.apply(x, weight, bias, routing, _ACTIVATIONS[activation], keep)
+    args = (x, weight, bias, routing, _ACTIVATIONS[activation])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _ExpertLinear.apply(*args)
+    return _ExpertLinear.forward(None, *args)
 
 
 class _ExpertCombine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, weights, residual, experts):
+    def forward(ctx, z, weights, residual, experts):   # ctx None: without gradients nothing is kept for them
         dev, (rows, choices, width) = z.device, z.shape
         z, weights = z.contiguous(), weights.contiguous()
         if residual is not None:
@@ -302,7 +308,8 @@ class _ExpertCombine(torch.autograd.Function):
             _lib.check(_lib.lib().dynb_expert_combine(z.data_ptr(), weights.data_ptr(), experts.data_ptr(), _pointer(residual),
                                                       0 if residual is None else residual.stride(0), rows, choices, width, _DTYPES[z.dtype], y.data_ptr(),
                                                       _lib.stream_of(dev)), "expert_combine")
-        ctx.save_for_backward(z, weights, experts)
+        if ctx is not None:
+            ctx.save_for_backward(z, weights, experts)
         return y
 
     @staticmethod
@@ -344,4 +351,7 @@ def expert_combine(z: torch.Tensor, routing: Routing, residual: Optional[torch.T
             raise RuntimeError("residual must be on the device and of the type of z")
         if residual.shape != (z.size(0), z.size(2)):
             raise RuntimeError(f"residual must have shape [{z.size(0)}, {z.size(2)}], got {list(residual.shape)}")
-    return _ExpertCombine.apply(z, routing.weights, residual, routing.experts)
+    args = (z, routing.weights, residual, routing.experts)
+    if torch.is_grad_enabled() and (z.requires_grad or routing.weights.requires_grad or (residual is not None and residual.requires_grad)):
+        return _ExpertCombine.apply(*args)
+    return _ExpertCombine.forward(None, *args)

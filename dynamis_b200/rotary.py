@@ -37,15 +37,16 @@ def _rotary_args(q, k, pos, wave, q_weight, k_weight, eps, interleaved) -> "_lib
 
 class _RotaryHeads(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, pos, wave, q_weight, k_weight, eps, interleaved):
+    def forward(ctx, q, k, pos, wave, q_weight, k_weight, eps, interleaved):   # ctx None: without gradients nothing is kept for them
         dev = q.device
         q, k = _heads_last(q), _heads_last(k)
         with _lib.on_device(dev):
             q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k))
             args = _rotary_args(q, k, pos, wave, q_weight, k_weight, eps, interleaved)
             _lib.check(_lib.lib().dynb_rotary_heads(ctypes.byref(args), q_out.data_ptr(), k_out.data_ptr(), _lib.stream_of(dev)), "rotary_heads")
-        ctx.save_for_backward(q, k, pos, wave, q_weight, k_weight)
-        ctx.eps, ctx.interleaved = eps, interleaved
+        if ctx is not None:
+            ctx.save_for_backward(q, k, pos, wave, q_weight, k_weight)
+            ctx.eps, ctx.interleaved = eps, interleaved
         return q_out, k_out
 
     @staticmethod
@@ -126,4 +127,7 @@ def rotary_heads(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, wave: torc
         if not 0.0 <= eps <= FLOAT_MAX or math.isinf(ctypes.c_float(eps).value) or eps > 3e38:
             raise RuntimeError(f"eps must be finite and not negative, got {eps}")
     weights = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    return _RotaryHeads.apply(q, k, pos.contiguous(), wave.contiguous(), *weights, eps, int(bool(interleaved)))
+    args = (q, k, pos.contiguous(), wave.contiguous(), *weights, eps, int(bool(interleaved)))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, pos, q_weight, k_weight)):
+        return _RotaryHeads.apply(*args)
+    return _RotaryHeads.forward(None, *args)     # a third of a small call's time is autograd's
