@@ -608,7 +608,7 @@ re_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits)
 
 // The same, a thread a row (see rt_choose_kernel): the gradients of 32 rows are put together in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(RT_WARPS * 32)
+__global__ void __launch_bounds__(RT_WARPS * 32, 10)
 rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitch, int wide, int wide_out)
 {
     extern __shared__ unsigned char raw_smem[];
@@ -624,51 +624,67 @@ rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitc
             for (int i = lane; i < 32 * pitch; i += 32) tile[i] = 0.0f;
         __syncwarp();
         if (row < a.n) {
-            const int32_t* const es = a.experts + row * a.choices;
-            const float *const ws = a.weights + row * a.choices, *const gs = d_weights + row * a.choices;
-            float dot = 0.0f;
-            for (int j = 0; j < a.choices; j++)
-                if ((uint32_t)es[j] < (uint32_t)a.count) dot = fmaf(ws[j] / a.scale, gs[j] * a.scale, dot);
+            // all of a row's choices at once: their loads do not wait for one another
+            int e[RT_MAX_CHOICES];
+            float w[RT_MAX_CHOICES], g[RT_MAX_CHOICES], dot = 0.0f;
+#pragma unroll
+            for (int j = 0; j < RT_MAX_CHOICES; j++) {
+                e[j] = j < a.choices ? a.experts[row * a.choices + j] : -1;
+                w[j] = j < a.choices ? a.weights[row * a.choices + j] / a.scale : 0.0f;
+                g[j] = j < a.choices ? d_weights[row * a.choices + j] * a.scale : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < RT_MAX_CHOICES; j++) {
+                if ((uint32_t)e[j] >= (uint32_t)a.count) e[j] = -1;
+                if (e[j] >= 0) dot = fmaf(w[j], g[j], dot);
+            }
             if (dense) {
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll 8
-                for (int e = 0; e < a.count; e++) top = fmaxf(top, l[e]);
-#pragma unroll 4
-                for (int e = 0; e < a.count; e++) {
-                    l[e] = l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
-                    sum += l[e];
+                for (int i = 0; i < a.count; i++) top = fmaxf(top, l[i]);
+#pragma unroll 8
+                for (int i = 0; i < a.count; i++) {
+                    l[i] = l[i] == -INFINITY ? 0.0f : expf(l[i] - top);
+                    sum += l[i];
                 }
                 const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
                 float add[RT_MAX_CHOICES];
 #pragma unroll
-                for (int j = 0; j < RT_MAX_CHOICES; j++) add[j] = j < a.choices && (uint32_t)es[j] < (uint32_t)a.count ? l[es[j]] * over * (gs[j] * a.scale - dot) : 0.0f;
+                for (int j = 0; j < RT_MAX_CHOICES; j++) add[j] = e[j] >= 0 ? l[e[j]] * over * (g[j] - dot) : 0.0f;
 #pragma unroll 8
-                for (int e = 0; e < a.count; e++) l[e] = l[e] * over * -dot;
+                for (int i = 0; i < a.count; i++) l[i] = l[i] * over * -dot;
 #pragma unroll
                 for (int j = 0; j < RT_MAX_CHOICES; j++)
-                    if (j < a.choices && (uint32_t)es[j] < (uint32_t)a.count) l[es[j]] = add[j];
+                    if (e[j] >= 0) l[e[j]] = add[j];
             } else {
-                for (int j = 0; j < a.choices; j++) {
-                    const int e = es[j];
-                    if ((uint32_t)e >= (uint32_t)a.count) continue;
-                    const float w = ws[j] / a.scale, g = gs[j] * a.scale;
-                    const float s = a.sigmoid ? 1.0f / (1.0f + expf(-tl_get(static_cast<const T*>(a.logits) + row * a.row + e))) : 0.0f;
-                    l[e] = a.renormalize ? w * (g - dot) * (1.0f - s) : g * s * (1.0f - s);
+                float s[RT_MAX_CHOICES];
+#pragma unroll
+                for (int j = 0; j < RT_MAX_CHOICES; j++) s[j] = a.sigmoid && e[j] >= 0 ? tl_get(static_cast<const T*>(a.logits) + row * a.row + e[j]) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < RT_MAX_CHOICES; j++) {
+                    if (e[j] < 0) continue;
+                    const float p = a.sigmoid ? 1.0f / (1.0f + expf(-s[j])) : 0.0f;
+                    l[e[j]] = a.renormalize ? w[j] * (g[j] - dot) * (1.0f - p) : g[j] * p * (1.0f - p);
                 }
             }
         }
         __syncwarp();
         constexpr int N = 16 / (int)sizeof(T);
         if (wide_out) {
-            const int per = a.count / N;
+            const int per = a.count / N, rows = 32 / per, rest = 32 % per;   // 32 pieces on
+            int r = lane / per, c = lane % per;
+#pragma unroll 4
             for (int u = lane; u < 32 * per; u += 32) {
-                const int r = u / per, c = (u % per) * N;
-                if (row0 + r >= a.n) break;
-                uint4 v;
-                T* const e = reinterpret_cast<T*>(&v);
+                if (row0 + r < a.n) {
+                    uint4 v;
+                    T* const out = reinterpret_cast<T*>(&v);
 #pragma unroll
-                for (int i = 0; i < N; i++) tl_put(e + i, tile[r * pitch + c + i]);
-                *reinterpret_cast<uint4*>(d_logits + (row0 + r) * a.count + c) = v;
+                    for (int i = 0; i < N; i++) tl_put(out + i, tile[r * pitch + c * N + i]);
+                    *reinterpret_cast<uint4*>(d_logits + (row0 + r) * a.count + c * N) = v;
+                }
+                r += rows;
+                c += rest;
+                if (c >= per) { c -= per; r++; }
             }
         } else {
             for (int u = lane; u < 32 * a.count; u += 32) {
