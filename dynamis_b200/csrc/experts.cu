@@ -16,7 +16,7 @@ template <typename T, int N> struct __align__(sizeof(T) * N) ExPack { T v[N]; };
 
 // y_i = r_i + sum_j w_ij z_ij (w null: ones).  Z: type of z.  `lanes` threads (a power of two) a row, N elements each, four choices under way.
 template <typename Z, typename T, int N>
-__global__ void __launch_bounds__(EX_THREADS)
+__global__ void __launch_bounds__(EX_THREADS, sizeof(Z) == 4 ? 6 : 4)   // blocks that their registers leave room for without spilling
 ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide, int lanes)
 {
     const int in_row = threadIdx.x & (lanes - 1), rows = EX_THREADS / lanes;
@@ -39,9 +39,10 @@ ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, cons
                 bool live[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    live[j] = j0 + j < choices && es[j0 + j] >= 0;
-                    w[j] = live[j] && weights != nullptr ? weights[row * choices + j0 + j] : 1.0f;
-                    if (live[j]) v[j] = *reinterpret_cast<const ExPack<Z, N>*>(at + j * wide);
+                    const bool here = j0 + j < choices;
+                    live[j] = here && es[j0 + j] >= 0;
+                    w[j] = here && weights != nullptr ? weights[row * choices + j0 + j] : 1.0f;
+                    if (here) v[j] = *reinterpret_cast<const ExPack<Z, N>*>(at + (int64_t)j * wide);   // also where there is no expert: it does not wait to be told
                 }
 #pragma unroll
                 for (int j = 0; j < 4; j++)
@@ -76,7 +77,7 @@ ex_combine_backward_kernel(const T* z, const float* weights, const int32_t* expe
             for (int j = 0; j < 4; j++) {
                 real[j] = here && j0 + j < choices;
                 live[j] = real[j] && experts[row * choices + j0 + j] >= 0;
-                w[j] = live[j] ? weights[row * choices + j0 + j] : 0.0f;
+                w[j] = real[j] ? weights[row * choices + j0 + j] : 0.0f;
             }
             if (here) {
                 const int64_t from = (row * choices + j0) * wide;
@@ -86,7 +87,7 @@ ex_combine_backward_kernel(const T* z, const float* weights, const int32_t* expe
                     if (d_weights != nullptr) {
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            if (live[j]) v[j] = *reinterpret_cast<const ExPack<T, N>*>(z + from + (int64_t)j * wide + c);
+                            if (real[j]) v[j] = *reinterpret_cast<const ExPack<T, N>*>(z + from + (int64_t)j * wide + c);
 #pragma unroll
                         for (int j = 0; j < 4; j++)
                             if (live[j]) {
