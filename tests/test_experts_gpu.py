@@ -348,7 +348,7 @@ def test_linear_strides(cuda, dtype):
     gen = _gen(4)
     wide, pairs = _normal(gen, 300, 200, dtype=dtype), _normal(gen, 300, 2, 200, dtype=dtype)
     slice_of_g = _normal(gen, 300, 2, 96, dtype=dtype)[..., 48:]
-    for t in (wide[:, 8:72], wide[:, 3:67], wide[:, ::3][:, :64], _normal(gen, 64, 300, dtype=dtype).t(), pairs[..., 8:72], pairs[..., 1:65], pairs.transpose(0, 1).contiguous().transpose(0, 1)[..., :64]):
+    for t in (wide[:, 8:72], wide[:, 4:68], wide[:, 3:67], wide[:, ::3][:, :64], _normal(gen, 64, 300, dtype=dtype).t(), pairs[..., 8:72], pairs[..., 1:65], pairs.transpose(0, 1).contiguous().transpose(0, 1)[..., :64]):
         _compare_linear(routing, t, w, b, slice_of_g, "silu")
     _compare_linear(routing, x, _normal(gen, 5, 48, 64, dtype=dtype).transpose(1, 2), b, g, "gelu")
     leaves = [t.detach().requires_grad_() for t in (x, w, b)]
@@ -365,13 +365,65 @@ def test_linear_strides(cuda, dtype):
 
 
 def test_linear_of_no_rows(cuda):
-    for rows in (0,):
-        routing = D.Routing(*X.routing_by_hand(rows, 3, 2, 0.0, 1, "cuda"))
-        x, w, b = (torch.randn(*s, device=cuda, requires_grad=True) for s in ((rows, 8), (3, 8, 4), (3, 4)))
-        z = D.expert_linear(x, w, routing, b, "silu")
-        assert z.shape == (0, 2, 4)
-        dx, dw, db = torch.autograd.grad(z.sum(), (x, w, b))
-        assert dx.shape == (0, 8) and not dw.any() and not db.any()
+    routing = D.Routing(*X.routing_by_hand(0, 3, 2, 0.0, 1, "cuda"))
+    x, w, b = (torch.randn(*s, device=cuda, requires_grad=True) for s in ((0, 8), (3, 8, 4), (3, 4)))
+    z = D.expert_linear(x, w, routing, b, "silu")
+    assert z.shape == (0, 2, 4)
+    dx, dw, db = torch.autograd.grad(z.sum(), (x, w, b))
+    assert dx.shape == (0, 8) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,experts,choices,inner,outer,paired", [(600, 3, 2, 1032, 520, False), (50, 1000, 2, 24, 40, False), (9000, 1, 1, 64, 64, True), (700, 5, 32, 16, 24, False),
+                                                                     (40, 2, 2, 2050, 1030, True)])
+def test_linear_wide_matrices_and_many_experts(cuda, dtype, rows, experts, choices, inner, outer, paired):
+    """Matrices that come in pieces, more experts than rows, one expert for all, and the same experts several times in a row."""
+    gen = _gen(rows)
+    of = torch.randint(0, experts, (rows, choices), generator=torch.Generator().manual_seed(inner)).to(torch.int32)
+    flat = of.reshape(-1).long()
+    start = torch.cat([flat.new_zeros(1), torch.bincount(flat, minlength=experts).cumsum(0)]).to(torch.int32)
+    routing = D.Routing(of.to(cuda), torch.rand(rows, choices, device=cuda), torch.sort(flat, stable=True).indices.to(torch.int32).to(cuda), start.to(cuda))
+    routing.check_lists()
+    dtype = M.TYPES[dtype]
+    x = _normal(gen, *((rows, choices) if paired else (rows,)), inner, dtype=dtype)
+    w = (_normal(gen, experts, inner, outer) * inner ** -0.5).to(dtype)
+    _compare_linear(routing, x, w, _normal(gen, experts, outer, dtype=dtype), _normal(gen, rows, choices, outer, dtype=dtype), "silu")
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 elements of pairs: the last rows have the bits that they have in a small call, and so have their gradients."""
+    rows, tail, wide = 2_200_000, 300, 512
+    gen = _gen(1)
+    x_tail, g_tail, z_tail = (_normal(gen, tail, *s, dtype=torch.bfloat16) for s in ((16,), (2, wide), (2, wide)))
+    w = _normal(gen, 3, 16, wide, dtype=torch.bfloat16)
+    logits = _normal(gen, rows, 3)
+    big, small = (D.route_experts(t, 2) for t in (logits, logits[-tail:]))
+    assert torch.equal(big.experts[-tail:], small.experts) and torch.equal(big.weights[-tail:], small.weights)
+    assert rows * 2 * wide > 2 ** 31
+    x = torch.zeros(rows, 16, device=cuda, dtype=torch.bfloat16)
+    x[-tail:] = x_tail
+    g = torch.zeros(rows, 2, wide, device=cuda, dtype=torch.bfloat16)
+    g[-tail:] = g_tail
+
+    def products(t, routing, grad):
+        t = t.detach().requires_grad_()
+        z = D.expert_linear(t, w, routing, None, "silu")
+        return z.detach()[-tail:], torch.autograd.grad(z, [t], grad)[0][-tail:]
+
+    for a, b in zip(products(x, big, g), products(x_tail, small, g_tail)):
+        assert torch.equal(a, b)
+    del x
+    g[-tail:] = z_tail
+
+    def sums(z, routing, grad):
+        z, weights = z.detach().requires_grad_(), routing.weights.detach().requires_grad_()
+        y = D.expert_combine(z, D.Routing(routing.experts, weights, routing.order, routing.start))
+        return [t[-tail:] for t in (y.detach(), *torch.autograd.grad(y, [z, weights], grad))]
+
+    d_y = torch.zeros(rows, wide, device=cuda, dtype=torch.bfloat16)
+    d_y[-tail:] = g_tail[:, 0]
+    for a, b in zip(sums(g, big, d_y), sums(z_tail, small, g_tail[:, 0])):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
