@@ -412,7 +412,7 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
             }
             if (!a.sigmoid && !a.renormalize) {
 #pragma unroll 4
-                for (int e = 0; e < a.count; e++) sum += l[e] == -INFINITY ? 0.0f : expf(l[e] - top);
+                for (int e = 0; e < a.count; e++) sum += l[e] == -INFINITY ? 0.0f : __expf(l[e] - top);   // off by 2 + |l - top| units in the last place, of what is small where that is large
             }
         } else {
             // logits give way to their keys
@@ -424,7 +424,7 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
                 }
 #pragma unroll 4
                 for (int e = 0; e < a.count; e++) {
-                    const float v = l[e] == -INFINITY ? -1.0f : expf(l[e] - top);
+                    const float v = l[e] == -INFINITY ? -1.0f : __expf(l[e] - top);
                     sum += fmaxf(v, 0.0f) + (v - v);   // a NaN stays one
                     l[e] = v;
                 }
@@ -644,7 +644,7 @@ rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitc
                 for (int i = 0; i < a.count; i++) top = fmaxf(top, l[i]);
 #pragma unroll 8
                 for (int i = 0; i < a.count; i++) {
-                    l[i] = l[i] == -INFINITY ? 0.0f : expf(l[i] - top);
+                    l[i] = l[i] == -INFINITY ? 0.0f : __expf(l[i] - top);
                     sum += l[i];
                 }
                 const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
