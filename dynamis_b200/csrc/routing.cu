@@ -403,7 +403,7 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
                 order[j] = 0;
                 chosen[j] = -1;
             }
-#pragma unroll 4
+#pragma unroll 8
             for (int e = 0; e < a.count; e++) {
                 const float v = l[e];
                 top = fmaxf(top, v);
@@ -411,7 +411,7 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
                 rt_insert(rt_order(v), e, chosen, order);
             }
             if (!a.sigmoid && !a.renormalize) {
-#pragma unroll 4
+#pragma unroll 8
                 for (int e = 0; e < a.count; e++) sum += l[e] == -INFINITY ? 0.0f : __expf(l[e] - top);   // off by 2 + |l - top| units in the last place, of what is small where that is large
             }
         } else {
@@ -736,6 +736,9 @@ static int re_args(const dynb_routing* in, ReArgs* a)
 template <typename T, int GROUPS>
 static void (*rt_kernel(int choices))(ReArgs, int, int)
 {
+    if constexpr (GROUPS == 0)   // logits decide for good: nothing is looked at beside the choices
+        return choices <= 1 ? rt_choose_kernel<T, 1, 0> : choices <= 2 ? rt_choose_kernel<T, 2, 0> : choices <= 4 ? rt_choose_kernel<T, 4, 0> :
+               choices <= 6 ? rt_choose_kernel<T, 6, 0> : rt_choose_kernel<T, 8, 0>;
     return choices <= 1 ? rt_choose_kernel<T, 3, GROUPS> : choices <= 2 ? rt_choose_kernel<T, 4, GROUPS> : choices <= 4 ? rt_choose_kernel<T, 6, GROUPS> :
            choices <= 6 ? rt_choose_kernel<T, 8, GROUPS> : rt_choose_kernel<T, 10, GROUPS>;
 }
