@@ -2,7 +2,9 @@
 // their libraries).  Row i has the experts e_i1 ... e_ic (route_experts); pairs (i, j) are numbered i c + j, and `order` lists them by expert:
 //     z_ij = act(x_i W[e_ij] + b[e_ij]),   y_i = r_i + sum_j w_ij z_ij.
 //     back:  du = dz act'(u);  dx_i = sum_j du_ij W^T;  dW[e] = sum x^T du;  db[e] = sum du;   dz_ij = w_ij dy_i;  dw_ij = dy_i . z_ij.
-// A place without an expert gives zeros and gets zero gradients.  Sums are in 32 bits, over pairs of an expert in stretches joined in their order: no atomics.
+// A place without an expert gives zeros and gets zero gradients.  Sums are in 32 bits, over pairs of an expert in pieces joined in their order: no atomics.
+//
+// The weighted sums are bound by memory: 300 k rows of 4 x 256 bf16 with a residual 179 us (5.2 TB/s), gradients 285 us (4.9 TB/s); with an element a thread 471 and 496.
 
 #include <algorithm>
 

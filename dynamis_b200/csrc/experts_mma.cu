@@ -10,6 +10,11 @@
 // are, read along their columns.  db is a product too, with a tile of ones.
 //
 // fp32 operands are three bf16 parts, six of nine products (mma_parts.cuh).
+//
+// 300 k pairs of 64 experts in bf16: 512 x 256 127 us (3.6 TB/s), 256 x 512 with SiLU and its slopes 174 us (4.0 TB/s), dx 248 us (5.0 TB/s, du for the weights' pass among it), dW 152 us.
+// 200 k pairs of 16 experts in fp32, 512 x 128: 163, 163 and 216 us (0.58, 0.58 and 0.44 of the six products' time).  In 16 bits the rows' passes are bound by the latency of gathered
+// rows and what they write, in fp32 by the chain of a stage from memory through the conversion to the multipliers.  Tiles of 64 x 64 with fused multiply-adds took
+// 4549 us for the first, 14 483 for the next three together and 5502 for the last three.
 
 #include <atomic>
 
@@ -67,7 +72,7 @@ __device__ __forceinline__ void copies_wait(int left)
 
 // Matrices in the order of the multipliers: [expert][tile of columns][64 summed columns][part][column][128 bytes, 16-byte pieces swizzled], zeros beyond the matrix.
 // WIDE: rows of the matrix are read by 16 bytes; forward a thread turns a piece of 8 rows by that many columns round.  What is written lies side by side for 8 threads.
-// (64 matrices of 512 x 256 bf16 by single elements: 12.7 us.)
+// (64 matrices of 512 x 256 bf16: 8.6 us, by single elements 12.7.)
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256)
 ex_pack_kernel(const T* w, int64_t experts, int inner, int outer, int back, int columns, int tiles, int chunks, unsigned char* packed)
@@ -111,7 +116,7 @@ ex_pack_kernel(const T* w, int64_t experts, int inner, int outer, int back, int 
 }
 
 // The warps that gather by way of registers in fp32 are two teams, which take the stages by turns: what a warp does for a stage is one long chain (wait, conversion, stores,
-// fence, addresses of the next), and while one team is in it the other is, too (200 k pairs 512 x 128: one team with two stages ahead 174 us, rows' pass).
+// fence, addresses of the next), and while one team is in it the other is, too (200 k pairs 512 x 128: one team with two stages ahead 174 us, two teams 166, rows' pass).
 template <typename T, EmPath PATH> constexpr int EM_TEAMS = sizeof(T) == 4 && PATH == EM_REGISTERS ? 2 : 1;
 
 // Eight elements times their slopes.
@@ -173,7 +178,7 @@ __device__ __forceinline__ void em_keep(const TmRaw<T>& v, T* to, int have)
 }
 
 // WORDS words of a row, the first `bytes` bytes of them real, in stores of 32 or 16 bytes or of elements of `size`.  Every lane stores its own row: a store of 32 bytes a lane fills
-// whole sectors, and what goes through shared memory to lie side by side costs more steps than that saves (300 k pairs 256 x 512 bf16 with slopes: 250 against 196 us).
+// whole sectors, and what goes through shared memory to lie side by side costs more steps than that saves (300 k pairs 256 x 512 bf16 with slopes: 250 against 227 us).
 template <int WORDS>
 __device__ __forceinline__ void em_put(unsigned char* to, const uint32_t (&w)[WORDS], int bytes, int store, int size)
 {
@@ -313,7 +318,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     }
                 }
                 uint32_t words[WORDS], slopes[COLUMNS * sizeof(T) / 4];
-                if constexpr (std::is_same<T, O>::value) {   // one choice for all elements: with one at each, they wait for one another (381 us in place of 150)
+                if constexpr (std::is_same<T, O>::value) {   // one choice for all elements: with one at each, they wait for one another (300 k pairs 256 x 512 with slopes: 421 in place of 250 us)
                     if (activation == DYNB_ACTIVATION_SILU) em_activate<T, DYNB_ACTIVATION_SILU>(bits, slopes);
                     else if (activation == DYNB_ACTIVATION_GELU) em_activate<T, DYNB_ACTIVATION_GELU>(bits, slopes);
                 }
@@ -998,7 +1003,7 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
         static_cast<const T*>(a.w), a.types, a.inner, a.outer, back, p.columns, tiles, p.chunks, static_cast<unsigned char*>(packed));
     cudaError_t rc = cudaGetLastError();
     if (rc != cudaSuccess) return rc;
-    // Warps that store results: activations in 16 bits keep sixteen busy (300 k pairs 256 x 512, SiLU: 178 us, with eight 210); without them eight leave the others more registers.
+    // Warps that store results: activations in 16 bits keep sixteen busy (300 k pairs 256 x 512 with slopes: 196 us, with eight 227); without them eight leave the others more registers.
     constexpr int FEW = SIZE == 4 ? 4 : 8, MANY = SIZE == 4 ? 4 : 16;
     const bool many = MANY != FEW && std::is_same<T, O>::value && !back && e.activation != DYNB_ACTIVATION_NONE;
     constexpr EmPath QUICK = SIZE == 4 ? EM_REGISTERS : EM_ASYNC, QUICK_SLOPE = SIZE == 4 ? EM_SLOPE : EM_ASYNC_SLOPE;

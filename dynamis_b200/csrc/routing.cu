@@ -7,6 +7,9 @@
 //
 // The (row, choice) pairs by expert, ascending inside one: every block counts its rows' choices, the counts are summed over the blocks, and every block
 // puts its pairs where its counts say.  No atomics on memory, no wait of the host: the same order each time, and the calls can be captured.
+//
+// 200 k rows of 64 experts, six choices of four of eight groups, bias: 112 us and 35 for the gradient; 1 M rows of 32 experts in bf16, two choices: 89 and 59 us.  Bound by the
+// instructions of a row (keys, lists), not by its bytes.
 
 #include <algorithm>
 
@@ -193,7 +196,7 @@ re_choose_kernel(const ReArgs a)
 
 // ------------------------------------------------------------------------------------------------ a thread a row
 // Up to 128 experts, 8 choices and 16 groups: a warp brings 32 rows to shared memory and every lane goes along one.  (A warp a row spends its time on exchanges between
-// lanes: 1 M rows of 32 bf16 logits, two choices, 350 us; gradient 292 us.)  Where more than the logits decide, keys are formed in 32 bits first; rows in which two that
+// lanes: 1 M rows of 32 bf16 logits, two choices, 350 us and now 65; gradient 292 and 59.)  Where more than the logits decide, keys are formed in 32 bits first; rows in which two that
 // matter lie nearer to one another than these may be off are looked at again in 64 bits.
 constexpr int RT_WARPS = 4, RT_MAX_EXPERTS = 128, RT_MAX_CHOICES = 8, RT_MAX_GROUPS = 16;
 
@@ -359,7 +362,7 @@ __device__ __forceinline__ void rt_weigh(const ReArgs& a, int64_t row, const int
     }
 }
 
-// A row from the start in 64 bits, by the whole warp (by one lane the others wait for: 131 in place of 100 us).
+// A row from the start in 64 bits, by the whole warp (by the lane alone, for which the others wait, 200 k rows of 64 experts in groups take 131 in place of 91 us).
 template <typename T>
 __device__ __noinline__ void rt_again(const ReArgs& a, int64_t row, double* scratch, int32_t* counts) { re_row<T, RT_MAX_EXPERTS / 32>(a, row, scratch, counts); }
 
@@ -732,7 +735,7 @@ static int re_args(const dynb_routing* in, ReArgs* a)
     return DYNB_OK;
 }
 
-// As few places in the list as the choices need: a longer one is entered more often (six choices with ten places 182 us, eight 161).
+// As few places in the list as the choices need: a longer one is entered more often (six choices of 64 experts, 200 k rows, with ten places 182 us, with eight 155).
 template <typename T, int GROUPS>
 static void (*rt_kernel(int choices))(ReArgs, int, int)
 {
