@@ -11,7 +11,7 @@
 //
 // fp32 operands are three bf16 parts, six of nine products (mma_parts.cuh).
 //
-// 300 k pairs of 64 experts in bf16: 512 x 256 127 us (3.6 TB/s), 256 x 512 with SiLU and its slopes 174 us (4.0 TB/s), dx 248 us (5.0 TB/s, du for the weights' pass among it), dW 152 us.
+// 300 k pairs of 64 experts in bf16: 512 x 256 101 us (4.6 TB/s), 256 x 512 with SiLU and its slopes 174 us (4.0 TB/s), dx 248 us (5.0 TB/s, du for the weights' pass among it), dW 152 us.
 // 200 k pairs of 16 experts in fp32, 512 x 128: 163, 163 and 216 us (0.58, 0.58 and 0.44 of the six products' time).  In 16 bits the rows' passes are bound by the latency of gathered
 // rows and what they write, in fp32 by the chain of a stage from memory through the conversion to the multipliers.  Tiles of 64 x 64 with fused multiply-adds took
 // 4549 us for the first, 14 483 for the next three together and 5502 for the last three.
@@ -945,23 +945,15 @@ static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // s
     p.back = back;
     p.chunks = (kk + 63) / 64;
     const int raw = slopes ? EM_RAW * 2 * A_BYTES : 0, room = EM_SMEM - 1024 - raw;
-    // Every tile of columns reads the rows anew, and a matrix that does not stay comes anew with every tile of rows: as few bytes as possible for 128 pairs.
-    const int least = (nn + MOST - 1) / MOST;
-    int64_t best = INT64_MAX;
-    for (int t = least; t <= 4 * least; t++) {
-        EmPlan q = p;
-        q.columns = tm_round((nn + t - 1) / t, 16);
-        q.b_bytes = PARTS * q.columns * 128;
-        q.resident = (int64_t)q.chunks * q.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * A_BYTES <= room;
-        const int count = (nn + q.columns - 1) / q.columns;
-        const int64_t bytes = (int64_t)count * (TM_ROWS * 64 * (int)sizeof(T) * (slopes ? 2 : 1) + (q.resident ? 0 : q.b_bytes));
-        if (bytes >= best) continue;
-        best = bytes;
-        q.stage_bytes = A_BYTES + (q.resident ? 0 : q.b_bytes);
-        q.stages = std::min(EM_MAX_STAGES, (room - (q.resident ? q.chunks * q.b_bytes : 0)) / q.stage_bytes);
-        *tiles = count;
-        p = q;
-    }
+    // As few tiles of columns as there is room for sums: every tile gathers the rows anew, which costs more than a matrix that comes from L2 with every tile of
+    // rows (300 k pairs 512 x 256 bf16 in one tile, from L2: 101 us; in two whose halves of the matrix stay: 131).
+    *tiles = (nn + MOST - 1) / MOST;
+    p.columns = tm_round((nn + *tiles - 1) / *tiles, 16);
+    *tiles = (nn + p.columns - 1) / p.columns;
+    p.b_bytes = PARTS * p.columns * 128;
+    p.resident = (int64_t)p.chunks * p.b_bytes + (PARTS == 1 && !slopes ? 4 : 2) * A_BYTES <= room;
+    p.stage_bytes = A_BYTES + (p.resident ? 0 : p.b_bytes);
+    p.stages = std::min(EM_MAX_STAGES, (room - (p.resident ? p.chunks * p.b_bytes : 0)) / p.stage_bytes);
     p.column_stride = tm_round(p.columns, 32);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
     p.smem = 1024 + (p.resident ? p.chunks * p.b_bytes : 0) + p.stages * p.stage_bytes + raw;
@@ -971,13 +963,9 @@ static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // s
 template <typename T>
 static int64_t em_packed(const ExArgs& e, int back)
 {
-    int64_t most = 0;
-    for (int slopes = 0; slopes < 2; slopes++) {   // which of them it is depends on addresses that are not known here
-        int tiles;
-        const EmPlan p = em_plan<T>(e, back, slopes != 0, &tiles);
-        most = std::max(most, (int64_t)e.t.types * tiles * p.chunks * p.b_bytes);
-    }
-    return most;
+    int tiles;
+    const EmPlan p = em_plan<T>(e, back, false, &tiles);
+    return (int64_t)e.t.types * tiles * p.chunks * p.b_bytes;
 }
 
 int64_t ex_packed_bytes(const ExArgs& e, int back, int dtype) { return dtype == DYNB_F32 ? em_packed<float>(e, back) : em_packed<__nv_bfloat16>(e, back); }
