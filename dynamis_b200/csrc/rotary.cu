@@ -95,14 +95,13 @@ __device__ __forceinline__ float rh_sum(float v, int lanes, uint32_t mask)
 }
 __device__ __forceinline__ uint32_t rh_mask(int lanes) { return lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << ((threadIdx.x & 31) & ~(lanes - 1)); }
 
-// Cosine and sine of pair p of row i.
-__device__ __forceinline__ float2 rh_turn(const RhArgs& a, int64_t i, int p)
+// Cosine and sine of a pair with the waves `wave` of a row at `at`.
+template <int AXES>
+__device__ __forceinline__ float2 rh_turn(const double (&at)[RH_MAX_AXES], const double* wave)
 {
     double turns = 0.0;
-    for (int x = 0; x < a.axes; x++) {
-        const double at = a.pos64 ? static_cast<const double*>(a.pos)[i * a.axes + x] : (double)static_cast<const float*>(a.pos)[i * a.axes + x];
-        turns = fma(at, (double)__ldg(a.wave + p * a.axes + x), turns);
-    }
+#pragma unroll
+    for (int x = 0; x < AXES; x++) turns = fma(at[x], wave[x], turns);
     const float rest = (float)(turns - rint(turns));
     float2 cs;
     sincospif(2.0f * rest, &cs.y, &cs.x);
@@ -114,15 +113,14 @@ __global__ void __launch_bounds__(RH_WARPS * 32, BACK ? 2 : 4)
 rh_kernel(const RhArgs a)
 {
     __shared__ __align__(16) float weight[2][2][RH_MAX_HALF];   // of the first and of the second elements of the pairs
-    __shared__ float wave[BACK ? RH_MAX_HALF * RH_MAX_AXES : 1];
+    __shared__ double wave[RH_MAX_HALF * RH_MAX_AXES];           // in 64 bits once for all rows: conversions cost a row more than the sums
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, half = a.half, dim = 2 * half;
     for (int i = threadIdx.x; i < 2 * dim; i += RH_WARPS * 32) {
         const int s = i / dim, at = i % dim;
         const float v = a.side[s].weight != nullptr ? a.side[s].weight[at] : 1.0f;
         weight[s][MIXED ? at % 2 : at / half][MIXED ? at / 2 : at % half] = v;
     }
-    if constexpr (BACK)
-        for (int i = threadIdx.x; i < half * a.axes; i += RH_WARPS * 32) wave[i] = a.wave[i];
+    for (int i = threadIdx.x; i < half * a.axes; i += RH_WARPS * 32) wave[i] = (double)a.wave[i];
     __syncthreads();
     const int per_row = a.per_head * a.shares, in_head = lane & (a.per_head - 1), share = (lane & (per_row - 1)) / a.per_head, rows_here = 32 / per_row;
     const uint32_t head_mask = rh_mask(a.per_head), row_mask = rh_mask(per_row);
@@ -139,12 +137,19 @@ rh_kernel(const RhArgs a)
     for (int64_t row = ((int64_t)blockIdx.x * RH_WARPS + warp) * rows_here + lane / per_row; row < a.rows; row += (int64_t)gridDim.x * RH_WARPS * rows_here) {
         float2 cs[PIECES][VP];
         float dtheta[PIECES][VP];
+        double at[RH_MAX_AXES];
+#pragma unroll
+        for (int x = 0; x < RH_MAX_AXES; x++)
+            if (x < a.axes) at[x] = a.pos64 ? static_cast<const double*>(a.pos)[row * a.axes + x] : (double)static_cast<const float*>(a.pos)[row * a.axes + x];
 #pragma unroll
         for (int c = 0; c < PIECES; c++)
 #pragma unroll
             for (int i = 0; i < VP; i++) {
                 const int p = (c * a.per_head + in_head) * VP + i;
-                cs[c][i] = p < half ? rh_turn(a, row, p) : make_float2(1.0f, 0.0f);
+                if (p >= half) cs[c][i] = make_float2(1.0f, 0.0f);
+                else if (a.axes == 3) cs[c][i] = rh_turn<3>(at, wave + 3 * p);
+                else if (a.axes == 2) cs[c][i] = rh_turn<2>(at, wave + 2 * p);
+                else cs[c][i] = rh_turn<1>(at, wave + p);
                 dtheta[c][i] = 0.0f;
             }
 #pragma unroll
@@ -247,7 +252,7 @@ rh_kernel(const RhArgs a)
 #pragma unroll
                         for (int i = 0; i < VP; i++) {
                             const int p = (c * a.per_head + in_head) * VP + i;
-                            if (p < half) d = fmaf(dtheta[c][i], wave[p * a.axes + x], d);
+                            if (p < half) d = fmaf(dtheta[c][i], (float)wave[p * a.axes + x], d);
                         }
                     __syncwarp(row_mask);
                     d = 6.2831853071795865f * rh_sum(d, per_row, row_mask);
