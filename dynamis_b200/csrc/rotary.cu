@@ -7,8 +7,8 @@
 // position) stays in their registers, every cosine is formed once, and the norms' sums are a few exchanges.  Where there are few rows, the heads of one are
 // shared out among several such groups.  Turns are in 64 bits, whole ones are dropped, and what is left goes to 32 bits.
 //
-// 1 M rows of 8 + 8 heads of 16 in fp32: 335 us (6.1 TB/s), gradients 600 us (5.1 TB/s); bound by memory and the warps that registers leave.  90 k rows, 63 k of them with 8 heads of
-// 64 queries, all with 2 of keys, bf16: 51 and 124 us, bound by instructions and latency.  With a warp a row and its heads side by side 394, 984, 103 and 368 us.
+// 1 M rows of 8 + 8 heads of 16 in fp32: 328 us (6.2 TB/s), gradients 605 us (5.1 TB/s); bound by memory and the warps that registers leave.  90 k rows, 63 k of them with 8 heads of
+// 64 queries, all with 2 of keys, bf16: 49 and 125 us, bound by instructions and latency.  With a warp a row and its heads side by side 394, 984, 103 and 368 us.
 
 #include <algorithm>
 

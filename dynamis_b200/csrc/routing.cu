@@ -267,7 +267,7 @@ template <int MOST, int GROUPS, typename Key, typename Same>
 __device__ __forceinline__ bool rt_choose(const ReArgs& a, float near, int (&chosen)[MOST], Key&& key_of, Same&& same)
 {
     bool sure = true;
-    uint32_t kept = 0xffffffffu;
+    uint32_t kept = 0;
     const int per = a.count / a.groups;
     if constexpr (GROUPS > 1) {
         uint32_t of_group[GROUPS];
@@ -287,7 +287,6 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, float near, int (&cho
             if (one != 0 && both == 0) both = 1;   // open, however low
             of_group[g] = both;
         }
-        kept = 0;
         uint32_t lowest = ~0u, highest = 0;   // of those that stay, and of the others
 #pragma unroll
         for (int g = 0; g < GROUPS; g++) {
@@ -310,10 +309,16 @@ __device__ __forceinline__ bool rt_choose(const ReArgs& a, float near, int (&cho
         order[j] = 0;
         chosen[j] = -1;
     }
-    for (int g = 0; g < a.groups; g++) {
-        if (!(kept >> (g & 31) & 1)) continue;
+    if constexpr (GROUPS > 1) {
+        // the groups that stay, ascending: each lane its own, so that none waits for those of the others
+        for (int i0 = 0; i0 < a.kept; i0++, kept &= kept - 1) {
+            const int first = (__ffs(kept) - 1) * per;
 #pragma unroll 4
-        for (int i = 0; i < per; i++) rt_insert(key_of(g * per + i), g * per + i, chosen, order);
+            for (int i = 0; i < per; i++) rt_insert(key_of(first + i), first + i, chosen, order);
+        }
+    } else {
+#pragma unroll 4
+        for (int e = 0; e < a.count; e++) rt_insert(key_of(e), e, chosen, order);
     }
     bool tie = false;   // the last choice and the first that is left out have the same key
 #pragma unroll
