@@ -16,27 +16,26 @@ constexpr int EX_THREADS = 256;
 
 template <typename T, int N> struct __align__(sizeof(T) * N) ExPack { T v[N]; };
 
-// y_i = r_i + sum_j w_ij z_ij (w null: ones).  Z: type of z.  `lanes` threads (a power of two) a row, N elements each, four choices under way.
-template <typename Z, typename T, int N>
+// y_i = r_i + sum_j w_ij z_ij (w null: ones).  Z: type of z.  `lanes` threads (a power of two) a row, K pieces of N elements each at a time, four choices under way.
+template <typename Z, typename T, int N, int K>
 __global__ void __launch_bounds__(EX_THREADS, sizeof(Z) == 4 ? 6 : 4)   // blocks that their registers leave room for without spilling
 ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide, int lanes)
 {
-    const int in_row = threadIdx.x & (lanes - 1), rows = EX_THREADS / lanes;
+    const int in_row = threadIdx.x & (lanes - 1), rows = EX_THREADS / lanes, apart = lanes * N;
     for (int64_t row = (int64_t)blockIdx.x * rows + threadIdx.x / lanes; row < n; row += (int64_t)gridDim.x * rows) {
         const int32_t* const es = experts + row * choices;
-        for (int c = in_row * N; c < wide; c += lanes * N) {
-            float sum[N];
-            if (residual != nullptr) {
-                const ExPack<T, N> r = *reinterpret_cast<const ExPack<T, N>*>(residual + row * residual_row + c);
+        for (int c = in_row * N; c < wide; c += K * apart) {
+            float sum[K][N];
 #pragma unroll
-                for (int i = 0; i < N; i++) sum[i] = tl_get(&r.v[i]);
-            } else {
+            for (int k = 0; k < K; k++) {
+                ExPack<T, N> r = {};
+                if (residual != nullptr && (K == 1 || c + k * apart < wide)) r = *reinterpret_cast<const ExPack<T, N>*>(residual + row * residual_row + c + k * apart);
 #pragma unroll
-                for (int i = 0; i < N; i++) sum[i] = 0.0f;
+                for (int i = 0; i < N; i++) sum[k][i] = residual != nullptr ? tl_get(&r.v[i]) : 0.0f;
             }
             const Z* at = z + row * choices * wide + c;
-            for (int j0 = 0; j0 < choices; j0 += 4, at += 4 * wide) {
-                ExPack<Z, N> v[4];
+            for (int j0 = 0; j0 < choices; j0 += 4, at += (int64_t)4 * wide) {
+                ExPack<Z, N> v[4][K];
                 float w[4];
                 bool live[4];
 #pragma unroll
@@ -44,19 +43,27 @@ ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, cons
                     const bool here = j0 + j < choices;
                     live[j] = here && es[j0 + j] >= 0;
                     w[j] = here && weights != nullptr ? weights[row * choices + j0 + j] : 1.0f;
-                    if (here) v[j] = *reinterpret_cast<const ExPack<Z, N>*>(at + (int64_t)j * wide);   // also where there is no expert: it does not wait to be told
+#pragma unroll
+                    for (int k = 0; k < K; k++)   // also where there is no expert: it does not wait to be told
+                        if (here && (K == 1 || c + k * apart < wide)) v[j][k] = *reinterpret_cast<const ExPack<Z, N>*>(at + (int64_t)j * wide + k * apart);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (live[j]) {
 #pragma unroll
-                        for (int i = 0; i < N; i++) sum[i] = fmaf(w[j], tl_get(&v[j].v[i]), sum[i]);
+                        for (int k = 0; k < K; k++)
+#pragma unroll
+                            for (int i = 0; i < N; i++) sum[k][i] = fmaf(w[j], tl_get(&v[j][k].v[i]), sum[k][i]);
                     }
             }
-            ExPack<T, N> out;
 #pragma unroll
-            for (int i = 0; i < N; i++) tl_put(&out.v[i], sum[i]);
-            *reinterpret_cast<ExPack<T, N>*>(y + row * wide + c) = out;
+            for (int k = 0; k < K; k++) {
+                if (K > 1 && c + k * apart >= wide) continue;
+                ExPack<T, N> out;
+#pragma unroll
+                for (int i = 0; i < N; i++) tl_put(&out.v[i], sum[k][i]);
+                *reinterpret_cast<ExPack<T, N>*>(y + row * wide + c + k * apart) = out;
+            }
         }
     }
 }
@@ -229,12 +236,19 @@ static int ex_lanes(int pieces, int most)
 template <typename Z, typename T>
 static cudaError_t ex_combine(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide, cudaStream_t s)
 {
-    constexpr int N = 16 / (int)sizeof(Z);
-    const bool pieces = wide % N == 0 && ex_on(z, 0, 1, 16) && ex_on(y, 0, 1, sizeof(T) * N) && (residual == nullptr || ex_on(residual, residual_row, sizeof(T), sizeof(T) * N));
-    const int lanes = ex_lanes(pieces ? wide / N : wide, EX_THREADS);
-    const unsigned grid = ex_grid(n * lanes);
-    if (pieces) ex_combine_kernel<Z, T, N><<<grid, EX_THREADS, 0, s>>>(z, weights, experts, residual, residual_row, y, n, choices, wide, lanes);
-    else ex_combine_kernel<Z, T, 1><<<grid, EX_THREADS, 0, s>>>(z, weights, experts, residual, residual_row, y, n, choices, wide, lanes);
+    // the widest pieces that all addresses allow; narrow ones several at a time (150 k rows of 4 x 100 fp16 by single elements 178 us, of 4 x 256 by whole pieces 75)
+    constexpr int MOST = 16 / (int)sizeof(Z);
+    int piece = MOST;
+    while (piece > 1 && !(wide % piece == 0 && ex_on(z, 0, 1, sizeof(Z) * piece) && ex_on(y, 0, 1, sizeof(T) * piece) && (residual == nullptr || ex_on(residual, residual_row, sizeof(T), sizeof(T) * piece))))
+        piece /= 2;
+    const auto start = [&](auto kernel, int at_once) {
+        const int lanes = ex_lanes((wide / piece + at_once - 1) / at_once, EX_THREADS);
+        kernel<<<ex_grid(n * lanes), EX_THREADS, 0, s>>>(z, weights, experts, residual, residual_row, y, n, choices, wide, lanes);
+    };
+    if (piece == MOST) start(ex_combine_kernel<Z, T, MOST, 1>, 1);
+    else if (piece == 4) start(ex_combine_kernel<Z, T, 4, 2>, 2);
+    else if (piece == 2) start(ex_combine_kernel<Z, T, 2, 4>, 4);
+    else start(ex_combine_kernel<Z, T, 1, 4>, 4);
     return cudaGetLastError();
 }
 
@@ -296,16 +310,14 @@ template <typename T>
 static cudaError_t ec_backward(const void* z, const float* weights, const int32_t* experts, const void* d_y, int64_t d_y_row, void* d_z, float* d_weights, int64_t n,
                                int choices, int wide, cudaStream_t s)
 {
-    constexpr int N = 16 / (int)sizeof(T);
-    const bool pieces = wide % N == 0 && ex_on(z, 0, 1, 16) && ex_on(d_z, 0, 1, 16) && ex_on(d_y, d_y_row, sizeof(T), 16);
-    const int lanes = ex_lanes(pieces ? wide / N : wide, 32);
+    constexpr int MOST = 16 / (int)sizeof(T);
+    int piece = MOST;
+    while (piece > 1 && !(wide % piece == 0 && ex_on(z, 0, sizeof(T), sizeof(T) * piece) && ex_on(d_z, 0, sizeof(T), sizeof(T) * piece) && ex_on(d_y, d_y_row, sizeof(T), sizeof(T) * piece))) piece /= 2;
+    const int lanes = ex_lanes(wide / piece, 32);
     const unsigned grid = ex_grid(n * lanes);
-    if (pieces)
-        ex_combine_backward_kernel<T, N><<<grid, EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(d_y), d_y_row, static_cast<T*>(d_z), d_weights, n,
-                                                                    choices, wide, lanes);
-    else
-        ex_combine_backward_kernel<T, 1><<<grid, EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(d_y), d_y_row, static_cast<T*>(d_z), d_weights, n,
-                                                                    choices, wide, lanes);
+    void (*const kernel)(const T*, const float*, const int32_t*, const T*, int64_t, T*, float*, int64_t, int, int, int) =
+        piece == MOST ? ex_combine_backward_kernel<T, MOST> : piece == 4 ? ex_combine_backward_kernel<T, 4> : piece == 2 ? ex_combine_backward_kernel<T, 2> : ex_combine_backward_kernel<T, 1>;
+    kernel<<<grid, EX_THREADS, 0, s>>>(static_cast<const T*>(z), weights, experts, static_cast<const T*>(d_y), d_y_row, static_cast<T*>(d_z), d_weights, n, choices, wide, lanes);
     return cudaGetLastError();
 }
 

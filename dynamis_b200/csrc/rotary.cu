@@ -379,8 +379,9 @@ static int rh_launch(RhArgs& a, bool mixed, cudaStream_t s)   // the number of b
         if (vp == 8) return rh_start<T, 8, 1, BACK>(a, mixed, s);
     }
     if (vp == 4) return rh_start<T, 4, 1, BACK>(a, mixed, s);
-    if (vp == 2) return rh_start<T, 2, 2, BACK>(a, mixed, s);
-    return rh_start<T, 1, 4, BACK>(a, mixed, s);
+    // pieces of a lane: as few as 32 lanes need (100 k rows of 8 + 8 heads of 10 in fp16 with four, three of them empty: 102 and 257 us)
+    if (vp == 2) return a.half <= 64 ? rh_start<T, 2, 1, BACK>(a, mixed, s) : rh_start<T, 2, 2, BACK>(a, mixed, s);
+    return a.half <= 32 ? rh_start<T, 1, 1, BACK>(a, mixed, s) : a.half <= 64 ? rh_start<T, 1, 2, BACK>(a, mixed, s) : rh_start<T, 1, 4, BACK>(a, mixed, s);
 }
 
 template <bool BACK>
