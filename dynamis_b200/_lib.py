@@ -124,7 +124,7 @@ class ExpertLinear(ctypes.Structure):
     _fields_ = (
         [(name, ctypes.c_void_p) for name in ("weight_dev", "order_dev", "start_dev")]
         + [("n_rows", ctypes.c_int64)]
-        + [(name, ctypes.c_int32) for name in ("choices", "experts", "inner", "outer", "dtype", "paired", "activation", "reserved")]
+        + [(name, ctypes.c_int32) for name in ("choices", "experts", "inner", "outer", "dtype", "paired", "activation", "unaligned")]
         + [("status_dev", ctypes.c_void_p)]
     )
 

@@ -126,15 +126,18 @@ ex_combine_backward_kernel(const T* z, const float* weights, const int32_t* expe
     }
 }
 
-// du = dz times the slope, for a gradient of the matrices alone (otherwise the pass of dx leaves it).
+// Rows (times their slopes, or as they are where there are none) to rows of `out_row` elements, zeros behind `wide`: a warp a row.  For gradients of the matrices alone, where no
+// pass of dx leaves du, and for rows that the products cannot read by whole pieces (120 k pairs of 129 x 131 bf16 read by single elements: 233 us for dx and 87 for dW, copied first 118 and 50, and 22 a copy).
 template <typename T>
 __global__ void __launch_bounds__(EX_THREADS)
-ex_slope_kernel(const T* dz, int64_t dz_row, const void* slope, T* du, int64_t n, int wide)
+ex_copy_kernel(const T* in, int64_t in_row, const void* slope, T* out, int64_t n, int wide, int out_row)
 {
-    for (int64_t p = blockIdx.x; p < n; p += gridDim.x)
-        for (int c = threadIdx.x; c < wide; c += EX_THREADS) {
-            const float s = sizeof(T) == 4 ? static_cast<const float*>(slope)[p * wide + c] : ex_slope_of(static_cast<const uint16_t*>(slope)[p * wide + c]);
-            tl_put(du + p * wide + c, tl_get(dz + p * dz_row + c) * s);
+    for (int64_t p = (int64_t)blockIdx.x * (EX_THREADS / 32) + threadIdx.x / 32; p < n; p += (int64_t)gridDim.x * (EX_THREADS / 32))
+#pragma unroll 4
+        for (int c = threadIdx.x % 32; c < out_row; c += 32) {
+            float v = c < wide ? tl_get(in + p * in_row + c) : 0.0f;
+            if (slope != nullptr && c < wide) v *= sizeof(T) == 4 ? static_cast<const float*>(slope)[p * wide + c] : ex_slope_of(static_cast<const uint16_t*>(slope)[p * wide + c]);
+            tl_put(out + p * out_row + c, v);
         }
 }
 
@@ -252,35 +255,73 @@ static cudaError_t ex_combine(const Z* z, const float* weights, const int32_t* e
     return cudaGetLastError();
 }
 
-// Workspace of the backward pass: the matrices as the kernel reads them, du, the gradients of x by pairs, the sums of stretches.
-struct ExLayout { int64_t du, by_pair, partial, total; };
-static ExLayout ex_layout(const ExArgs& e, int dtype, bool dx, bool weights)
+static int ex_whole(int wide) { return (wide + 7) / 8 * 8; }
+// Whether rows are copied before the products read them: they do so by pieces of 8 elements on 16 bytes.
+static bool ex_copies(const void* p, int64_t row, int wide, int size) { return wide % 8 != 0 || !ex_on(p, row, size, 16); }
+
+template <typename T>
+static cudaError_t ex_copy(const void* in, int64_t in_row, const void* slope, void* out, int64_t n, int wide, int out_row, cudaStream_t s)
+{
+    ex_copy_kernel<T><<<ex_grid(n * 32), EX_THREADS, 0, s>>>(static_cast<const T*>(in), in_row, slope, static_cast<T*>(out), n, wide, out_row);
+    return cudaGetLastError();
+}
+
+// Workspaces: the matrices as the kernel reads them, rows of x that were copied; backward also du, or copies of its rows, the gradients of x by pairs, the sums of pieces.
+struct ExLayout { int64_t x, du, by_pair, partial, total; };
+static ExLayout ex_layout(const ExArgs& e, int dtype, bool back, bool dx, bool weights, bool copy_x, bool copy_dy)
 {
     const int size = dtype == DYNB_F32 ? 4 : 2;
     ExLayout l;
-    l.du = align_up(dx ? ex_packed_bytes(e, 1, dtype) : 0, 256);
-    l.by_pair = l.du + align_up(weights && e.activation != DYNB_ACTIVATION_NONE ? e.t.n * e.t.outer * size : 0, 256);
-    l.partial = l.by_pair + align_up(dx && e.fan > 1 ? e.t.n * e.t.inner * 4 : 0, 256);
-    l.total = l.partial + align_up(weights ? ex_stretches(e) * ((int64_t)e.t.inner * e.t.outer + e.t.outer) * 4 : 0, 256);
+    l.x = align_up(!back || dx ? ex_packed_bytes(e, back, dtype) : 0, 256);
+    l.du = l.x + align_up(copy_x && (!back || weights) ? e.n_in * ex_whole(e.t.inner) * size : 0, 256);
+    l.by_pair = l.du + align_up(!back ? 0 : copy_dy ? e.t.n * ex_whole(e.t.outer) * size : weights && e.activation != DYNB_ACTIVATION_NONE ? e.t.n * e.t.outer * size : 0, 256);
+    l.partial = l.by_pair + align_up(back && dx && e.fan > 1 ? e.t.n * e.t.inner * 4 : 0, 256);
+    l.total = l.partial + align_up(back && weights ? ex_stretches(e) * ((int64_t)e.t.inner * e.t.outer + e.t.outer) * 4 : 0, 256);
     return l;
 }
 
 template <typename T>
-static int ex_backward(ExArgs& e, int dtype, const int32_t* experts, void* d_x, unsigned char* ws, const ExLayout& l, cudaStream_t s)
+static int ex_forward(ExArgs& e, int dtype, unsigned char* ws, const ExLayout& l, bool copy_x, cudaStream_t s)
 {
     TlArgs& a = e.t;
-    const bool weights = a.dw != nullptr || a.db != nullptr;
-    if (weights && e.activation != DYNB_ACTIVATION_NONE) e.du = ws + l.du;
-    if (d_x != nullptr && a.n > 0) {
-        a.dx = e.fan > 1 ? ws + l.by_pair : static_cast<unsigned char*>(d_x);
-        DYNB_CUDA_OK(ex_mma_rows(e, 1, dtype, ws, s));
-        if (e.fan > 1) DYNB_CUDA_OK((ex_combine<float, T>(reinterpret_cast<const float*>(ws + l.by_pair), nullptr, experts, nullptr, 0, static_cast<T*>(d_x), e.n_in, e.fan, a.inner, s)));
-    } else if (e.du != nullptr && a.n > 0) {
-        ex_slope_kernel<T><<<(unsigned)std::min<int64_t>(a.n, (int64_t)sm_count_cached() * 8), EX_THREADS, 0, s>>>(static_cast<const T*>(a.dy), a.dy_row, e.slope, static_cast<T*>(e.du), a.n, a.outer);
-        DYNB_CUDA_OK(cudaGetLastError());
+    if (copy_x) {
+        DYNB_CUDA_OK(ex_copy<T>(a.x, a.x_row, nullptr, ws + l.x, e.n_in, a.inner, ex_whole(a.inner), s));
+        a.x = ws + l.x;
+        a.x_row = ex_whole(a.inner);
+    }
+    DYNB_CUDA_OK(ex_mma_rows(e, 0, dtype, ws, s));
+    return DYNB_OK;
+}
+
+template <typename T>
+static int ex_backward(ExArgs& e, int dtype, const int32_t* experts, void* d_x, unsigned char* ws, const ExLayout& l, bool copy_x, bool copy_dy, cudaStream_t s)
+{
+    TlArgs& a = e.t;
+    const bool weights = a.dw != nullptr || a.db != nullptr, active = e.activation != DYNB_ACTIVATION_NONE;
+    if (a.n > 0) {
+        if (copy_dy) {   // times the slopes
+            DYNB_CUDA_OK(ex_copy<T>(a.dy, a.dy_row, active ? e.slope : nullptr, ws + l.du, a.n, a.outer, ex_whole(a.outer), s));
+            a.dy = ws + l.du;
+            a.dy_row = ex_whole(a.outer);
+            e.slope = nullptr;
+        } else if (weights && active) {
+            e.du = ws + l.du;
+        }
+        if (d_x != nullptr) {
+            a.dx = e.fan > 1 ? ws + l.by_pair : static_cast<unsigned char*>(d_x);
+            DYNB_CUDA_OK(ex_mma_rows(e, 1, dtype, ws, s));
+            if (e.fan > 1) DYNB_CUDA_OK((ex_combine<float, T>(reinterpret_cast<const float*>(ws + l.by_pair), nullptr, experts, nullptr, 0, static_cast<T*>(d_x), e.n_in, e.fan, a.inner, s)));
+        } else if (e.du != nullptr) {
+            DYNB_CUDA_OK(ex_copy<T>(a.dy, a.dy_row, e.slope, e.du, a.n, a.outer, a.outer, s));
+        }
     }
     if (weights) {
         if (e.du != nullptr) { a.dy = e.du; a.dy_row = a.outer; }
+        if (copy_x && a.n > 0) {
+            DYNB_CUDA_OK(ex_copy<T>(a.x, a.x_row, nullptr, ws + l.x, e.n_in, a.inner, ex_whole(a.inner), s));
+            a.x = ws + l.x;
+            a.x_row = ex_whole(a.inner);
+        }
         DYNB_CUDA_OK(ex_mma_weights(e, dtype, s));
         const int64_t all = (int64_t)a.inner * a.outer + a.outer;
         // enough blocks for all SMs, and no more: finding an expert's sums takes a block longer than adding a few (64 experts of 256 x 512: 129 blocks each 33 us, 37 blocks 22)
@@ -331,7 +372,7 @@ extern "C" int dynb_expert_linear_workspace_bytes(const dynb_expert_linear_args*
     const int rc = ex_args(args, &e);
     if (rc != DYNB_OK) return rc;
     if (bytes == nullptr) return fail_arg("null pointer");
-    *bytes = backward ? ex_layout(e, args->dtype, want_x != 0, want_weights != 0).total : ex_packed_bytes(e, 0, args->dtype);
+    *bytes = ex_layout(e, args->dtype, backward != 0, want_x != 0, want_weights != 0, args->inner % 8 != 0 || (args->unaligned & 1), args->outer % 8 != 0 || (args->unaligned & 2)).total;
     return DYNB_OK;
 }
 
@@ -343,11 +384,16 @@ extern "C" int dynb_expert_linear(const dynb_expert_linear_args* args, const voi
     if (rc != DYNB_OK) return rc;
     if (e.t.n == 0) return DYNB_OK;
     if (!x_dev || !z_dev) return fail_arg("null pointer");
-    if (workspace_dev == nullptr || !starts_on(workspace_dev, 16) || workspace_bytes < ex_packed_bytes(e, 0, args->dtype)) return fail_arg("workspace too small");
+    const bool copy_x = ex_copies(x_dev, x_row, args->inner, args->dtype == DYNB_F32 ? 4 : 2);
+    const ExLayout l = ex_layout(e, args->dtype, false, false, false, copy_x, false);
+    if (workspace_dev == nullptr || !starts_on(workspace_dev, 16) || workspace_bytes < l.total) return fail_arg("workspace too small");
     e.t.x = x_dev; e.t.x_row = x_row; e.t.b = bias_dev; e.t.y = z_dev;
     e.slope = e.activation != DYNB_ACTIVATION_NONE ? slope_dev : nullptr;
-    DYNB_CUDA_OK(ex_mma_rows(e, 0, args->dtype, workspace_dev, static_cast<cudaStream_t>(stream)));
-    return DYNB_OK;
+    unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (args->dtype == DYNB_F32) return ex_forward<float>(e, args->dtype, ws, l, copy_x, s);
+    if (args->dtype == DYNB_F16) return ex_forward<__half>(e, args->dtype, ws, l, copy_x, s);
+    return ex_forward<__nv_bfloat16>(e, args->dtype, ws, l, copy_x, s);
 }
 
 extern "C" int dynb_expert_linear_backward(const dynb_expert_linear_args* args, const void* x_dev, int64_t x_row, const void* d_z_dev, int64_t d_z_row,
@@ -361,16 +407,18 @@ extern "C" int dynb_expert_linear_backward(const dynb_expert_linear_args* args, 
     if (!weights && (d_x_dev == nullptr || e.t.n == 0)) return DYNB_OK;
     if (e.t.n > 0 && (!x_dev || !d_z_dev || !experts_dev)) return fail_arg("null pointer");
     if (e.t.n > 0 && e.activation != DYNB_ACTIVATION_NONE && !slope_dev) return fail_arg("null pointer");
-    const ExLayout l = ex_layout(e, args->dtype, d_x_dev != nullptr, weights);
+    const int size = args->dtype == DYNB_F32 ? 4 : 2;
+    const bool copy_x = ex_copies(x_dev, x_row, args->inner, size), copy_dy = ex_copies(d_z_dev, d_z_row, args->outer, size) || !ex_on(e.activation != DYNB_ACTIVATION_NONE ? slope_dev : nullptr, 0, size, 16);
+    const ExLayout l = ex_layout(e, args->dtype, true, d_x_dev != nullptr, weights, copy_x, copy_dy);
     if (l.total > 0 && (workspace_dev == nullptr || !starts_on(workspace_dev, 16) || workspace_bytes < l.total)) return fail_arg("workspace too small");
     unsigned char* const ws = static_cast<unsigned char*>(workspace_dev);
     e.t.x = x_dev; e.t.x_row = x_row; e.t.dy = d_z_dev; e.t.dy_row = d_z_row; e.t.dw = d_weight_dev; e.t.db = d_bias_dev;
     e.t.partial = reinterpret_cast<float*>(ws + l.partial);
     e.slope = const_cast<void*>(slope_dev);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (args->dtype == DYNB_F32) return ex_backward<float>(e, args->dtype, experts_dev, d_x_dev, ws, l, s);
-    if (args->dtype == DYNB_F16) return ex_backward<__half>(e, args->dtype, experts_dev, d_x_dev, ws, l, s);
-    return ex_backward<__nv_bfloat16>(e, args->dtype, experts_dev, d_x_dev, ws, l, s);
+    if (args->dtype == DYNB_F32) return ex_backward<float>(e, args->dtype, experts_dev, d_x_dev, ws, l, copy_x, copy_dy, s);
+    if (args->dtype == DYNB_F16) return ex_backward<__half>(e, args->dtype, experts_dev, d_x_dev, ws, l, copy_x, copy_dy, s);
+    return ex_backward<__nv_bfloat16>(e, args->dtype, experts_dev, d_x_dev, ws, l, copy_x, copy_dy, s);
 }
 
 extern "C" int dynb_expert_combine(const void* z_dev, const float* weights_dev, const int32_t* experts_dev, const void* residual_dev, int64_t residual_row,

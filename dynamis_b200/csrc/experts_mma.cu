@@ -3,7 +3,7 @@
 // z = act(x W + b) and dx = du W^T, du = dz act'(u): tiles of 128 pairs of one expert by up to 256 columns (fp32: 128).  Eight warps gather the rows of x (or of dz, times
 // the slope) into stages of 64 summed columns, one warp brings the matrix, one issues the products, eight take the sums out of tensor memory, which holds two tiles, and
 // apply offset and activation.  The matrices are laid out once per call as the multipliers read them (ex_pack_kernel: both products read them along the summed
-// index, fp32 in its three parts), so that a piece of 64 summed columns is one copy of a run of bytes.  A matrix that fits beside three stages of rows stays for
+// index, fp32 in its three parts), so that a piece of 64 summed columns is one copy of a run of bytes.  A matrix that fits beside four stages of rows (two in fp32 and with slopes) stays for
 // all tiles of its expert; a larger one comes anew with every stage, from L2.
 //
 // dW = sum x^T du: a block takes a stretch of an expert's pairs, 128 x up to 256 elements of the matrix; both operands are the gathered rows as they
@@ -146,7 +146,7 @@ __device__ __forceinline__ void em_times(TmRaw<T>& v, const TmRaw<T>& slope)
     }
 }
 
-// Eight elements from p, as tm_load; WIDE 2: fp32 on 32 bytes, by one load.
+// Eight elements from p, where there are any (behind them, zeros are in memory); WIDE 2: fp32 on 32 bytes, by one load.
 template <int WIDE, typename T>
 __device__ __forceinline__ TmRaw<T> em_load(const T* p, int64_t step, int have)
 {
@@ -158,22 +158,7 @@ __device__ __forceinline__ TmRaw<T> em_load(const T* p, int64_t step, int have)
                          : "l"(p));
         return r;
     } else {
-        return tm_load<WIDE != 0>(p, step, have);
-    }
-}
-
-// Eight elements, the first `have` of them real, back to memory.
-template <bool WIDE, typename T>
-__device__ __forceinline__ void em_keep(const TmRaw<T>& v, T* to, int have)
-{
-    if constexpr (WIDE) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(v) / 16); i++) reinterpret_cast<uint4*>(to)[i] = v.v[i];
-    } else {
-        const T* const from = reinterpret_cast<const T*>(&v);
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < have) to[i] = from[i];
+        return tm_load<true>(p, step, have);
     }
 }
 
@@ -223,7 +208,7 @@ __device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS], uint32
     }
 }
 
-// WIDE: elements are read by 32 bytes (2), 16 (1) or one by one (0).  O: type of the results (fp32 for gradients that are summed over the choices before they are rounded).
+// Rows are read by pieces of 8 elements on 16 bytes, with WIDE 2 in fp32 on 32.  O: type of the results (fp32 for gradients that are summed over the choices before they are rounded).
 template <typename T, typename O, EmPath PATH, int WIDE, int OUT>
 __global__ void __launch_bounds__(em_threads<T>(OUT), 1)
 em_rows_kernel(const ExArgs e, const EmPlan plan)
@@ -536,7 +521,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             }
             copies_wait(0);
         } else {
-            constexpr int AHEAD = sizeof(T) == 2 ? 2 : 1;
+            constexpr int AHEAD = 1;
             constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
             TlTile next = cursor.tile;
             int chunk = 0;
@@ -589,7 +574,11 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
 #pragma unroll
                         for (int i = 0; i < UNITS; i++) {
                             em_times(v[s][i], slope[s][i]);
-                            if (row_du[s][i] < rows_in) em_keep<WIDE != 0>(v[s][i], static_cast<T*>(e.du) + (int64_t)row_du[s][i] * kk + k_du[s], kk - k_du[s]);
+                            if (row_du[s][i] < rows_in) {
+                                uint4* const to = reinterpret_cast<uint4*>(static_cast<T*>(e.du) + (int64_t)row_du[s][i] * kk + k_du[s]);
+#pragma unroll
+                                for (int h = 0; h < (int)(sizeof(TmRaw<T>) / 16); h++) to[h] = v[s][i].v[h];
+                            }
                         }
                     }
                     if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
@@ -978,10 +967,9 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     const int kk = back ? a.outer : a.inner, nn = back ? a.inner : a.outer;
     const void* const in = back ? a.dy : a.x;
     const void* const out = back ? a.dx : a.y;
-    const bool slope = back && e.activation != DYNB_ACTIVATION_NONE;
-    const bool wide = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 16) && kk % 8 == 0 && (!slope || (tm_on(e.slope, kk, SIZE, 16) && tm_on(e.du, kk, SIZE, 16)));
+    const bool slope = back && e.activation != DYNB_ACTIVATION_NONE && e.slope != nullptr;   // rows that were copied have met theirs
     int tiles;
-    EmPlan p = em_plan<T>(e, back, SIZE == 2 && slope && wide, &tiles);
+    EmPlan p = em_plan<T>(e, back, SIZE == 2 && slope, &tiles);
     p.packed = static_cast<const unsigned char*>(packed);
     p.store = tm_on(out, nn, sizeof(O), 32) ? 32 : tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
     p.slope_store = tm_on(e.slope, nn, SIZE, 32) ? 32 : tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
@@ -994,16 +982,16 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     // Warps that store results: activations in 16 bits keep sixteen busy (300 k pairs 256 x 512 with slopes: 196 us, with eight 227); without them eight leave the others more registers.
     constexpr int FEW = SIZE == 4 ? 4 : 8, MANY = SIZE == 4 ? 4 : 16;
     const bool many = MANY != FEW && std::is_same<T, O>::value && !back && e.activation != DYNB_ACTIVATION_NONE;
-    constexpr EmPath QUICK = SIZE == 4 ? EM_REGISTERS : EM_ASYNC, QUICK_SLOPE = SIZE == 4 ? EM_SLOPE : EM_ASYNC_SLOPE;
-    void (*kernel)(ExArgs, EmPlan) = slope ? (wide ? em_rows_kernel<T, O, QUICK_SLOPE, 1, FEW> : em_rows_kernel<T, O, EM_SLOPE, 0, FEW>)
-                                           : (wide ? em_rows_kernel<T, O, QUICK, 1, FEW> : em_rows_kernel<T, O, EM_REGISTERS, 0, FEW>);
+    void (*kernel)(ExArgs, EmPlan);
     if constexpr (SIZE == 4) {   // by 32 bytes half as many steps to the same lines (200 k pairs 512 x 128: 166 -> 163 us, the weights' pass 224 -> 216)
-        const bool all = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 32) && kk % 8 == 0 && (!slope || tm_on(e.slope, kk, SIZE, 32));
-        if (all && slope) kernel = em_rows_kernel<T, O, EM_SLOPE, 2, FEW>;
-        else if (all) kernel = em_rows_kernel<T, O, EM_REGISTERS, 2, FEW>;
+        const bool all = tm_on(in, back ? a.dy_row : a.x_row, SIZE, 32) && (!slope || tm_on(e.slope, kk, SIZE, 32));
+        if (slope) kernel = all ? em_rows_kernel<T, O, EM_SLOPE, 2, FEW> : em_rows_kernel<T, O, EM_SLOPE, 1, FEW>;
+        else kernel = all ? em_rows_kernel<T, O, EM_REGISTERS, 2, FEW> : em_rows_kernel<T, O, EM_REGISTERS, 1, FEW>;
+    } else {
+        kernel = slope ? em_rows_kernel<T, O, EM_ASYNC_SLOPE, 1, FEW> : em_rows_kernel<T, O, EM_ASYNC, 1, FEW>;
+        if constexpr (std::is_same<T, O>::value)
+            if (many) kernel = em_rows_kernel<T, O, EM_ASYNC, 1, MANY>;
     }
-    if constexpr (std::is_same<T, O>::value)
-        if (many) kernel = wide ? em_rows_kernel<T, O, QUICK, 1, MANY> : em_rows_kernel<T, O, EM_REGISTERS, 0, MANY>;
     const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
     rc = em_allow(reinterpret_cast<const void*>(kernel), EM_SMEM);
@@ -1047,11 +1035,9 @@ static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
     const int stage = (p.x_blocks + p.y_blocks) * PARTS * BLOCK;
     p.stages = std::min(EW_MAX_STAGES, (EW_SMEM - 1024) / stage);
     p.tensor_columns = tm_tensor_columns((PARTS == 1 ? 2 : 4) * p.column_stride);
-    const bool wide = tm_on(a.x, a.x_row, SIZE, 16) && a.inner % 8 == 0 && tm_on(a.dy, a.dy_row, SIZE, 16) && a.outer % 8 == 0;
     p.store = tm_on(a.partial, a.outer, 4, 32) && (int64_t)a.inner * a.outer % 8 == 0 ? 32 : tm_on(a.partial, a.outer, 4, 16) ? 16 : 4;
     void (*kernel)(ExArgs, EwPlan);
-    if (!wide) kernel = em_weights_kernel<T, EM_REGISTERS, 0>;
-    else if constexpr (SIZE == 4) kernel = tm_on(a.x, a.x_row, SIZE, 32) && tm_on(a.dy, a.dy_row, SIZE, 32) ? em_weights_kernel<T, EM_REGISTERS, 2> : em_weights_kernel<T, EM_REGISTERS, 1>;
+    if constexpr (SIZE == 4) kernel = tm_on(a.x, a.x_row, SIZE, 32) && tm_on(a.dy, a.dy_row, SIZE, 32) ? em_weights_kernel<T, EM_REGISTERS, 2> : em_weights_kernel<T, EM_REGISTERS, 1>;
     else kernel = em_weights_kernel<T, EM_ASYNC, 1>;
     const int smem = 1024 + p.stages * stage, tiles_of = p.row_tiles * p.column_tiles;
     const cudaError_t rc = em_allow(reinterpret_cast<const void*>(kernel), EW_SMEM);

@@ -203,6 +203,11 @@ def _linear_args(weight, routing: Routing, paired: bool, activation: int, dtype)
     return a
 
 
+def _unaligned(t: torch.Tensor) -> bool:
+    """Whether rows of ``t`` start off 16-byte boundaries (they are copied then)."""
+    return t.data_ptr() % 16 != 0 or t.stride(0) * t.element_size() % 16 != 0
+
+
 def _linear_workspace(args, backward: int, want_x: int, want_weights: int, dev) -> torch.Tensor:
     nbytes = ctypes.c_int64()
     _lib.check(_lib.lib().dynb_expert_linear_workspace_bytes(ctypes.byref(args), backward, want_x, want_weights, ctypes.byref(nbytes)), "expert_linear_workspace_bytes")
@@ -234,6 +239,7 @@ class _ExpertLinear(torch.autograd.Function):
             if ctx is not None and activation:
                 slope = torch.empty(z.shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16, device=dev)
             args = _linear_args(weight, routing, paired, activation, x.dtype)
+            args.unaligned = int(_unaligned(flat))
             ws = _linear_workspace(args, 0, 0, 0, dev)
             _lib.check(_lib.lib().dynb_expert_linear(ctypes.byref(args), flat.data_ptr(), flat.stride(0), _pointer(bias), z.data_ptr(), _pointer(slope),
                                                      ws.data_ptr(), ws.numel(), _lib.stream_of(dev)), "expert_linear")
@@ -253,6 +259,7 @@ class _ExpertLinear(torch.autograd.Function):
             dx = torch.empty(ctx.shape, dtype=x.dtype, device=dev) if want_x else None
             dw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if want_w else None
             db = torch.empty((weight.size(0), weight.size(2)), dtype=x.dtype, device=dev) if want_b else None
+            args.unaligned = int(_unaligned(x)) + 2 * int(_unaligned(d_z) or (slope is not None and slope.data_ptr() % 16 != 0))
             ws = _linear_workspace(args, 1, int(want_x), int(want_w or want_b), dev)
             _lib.check(_lib.lib().dynb_expert_linear_backward(ctypes.byref(args), x.data_ptr(), x.stride(0), d_z.data_ptr(), d_z.stride(0), _pointer(slope),
                                                      routing.experts.data_ptr(), _pointer(dx), _pointer(dw), _pointer(db), ws.data_ptr(), ws.numel(),

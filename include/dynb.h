@@ -576,7 +576,8 @@ typedef struct dynb_expert_linear_args {
     const void* weight_dev;
     const int32_t *order_dev, *start_dev;
     int64_t n_rows;
-    int32_t choices, experts, inner, outer, dtype, paired, activation, reserved;
+    int32_t choices, experts, inner, outer, dtype, paired, activation;
+    int32_t unaligned;                      /* for the sizes of workspaces: bit 0 where rows of x do not start on 16 bytes, bit 1 where those of d_z or the slopes do not */
     uint32_t* status_dev;                   /* as in dynb_type_linear_args */
 } dynb_expert_linear_args;
 int dynb_expert_linear_workspace_bytes(const dynb_expert_linear_args* args, int backward, int want_x, int want_weights, int64_t* bytes);

@@ -107,6 +107,25 @@ def test_linear_entry_checks_its_workspace():
     assert L.dynb_expert_linear_backward(ctypes.byref(a), at, 8, at, 4, None, at, at, at, at, at, n.value, None) == -1   # an activation without its slopes
 
 
+def test_linear_entry_checks_the_workspace_of_rows_off_16_bytes():
+    L, at, n = _lib.lib(), 4096, ctypes.c_int64()
+    a = _linear(weight_dev=at, order_dev=at, start_dev=at, outer=16, activation=1)
+    sizes = {}
+    for back in (0, 1):
+        for flags in range(4):
+            a.unaligned = flags
+            assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), back, 1, 1, ctypes.byref(n)) == 0
+            sizes[back, flags] = n.value
+    assert sizes[0, 0] == sizes[0, 2] < sizes[0, 1] and sizes[1, 0] < sizes[1, 1]
+    for x, row in ((at + 4, 8), (at, 9)):
+        assert L.dynb_expert_linear(ctypes.byref(a), x, row, None, at, None, at, sizes[0, 0], None) == -1 and b"workspace" in L.dynb_last_error()
+        assert L.dynb_expert_linear_backward(ctypes.byref(a), x, row, at, 16, at, at, at, at, at, at, sizes[1, 0], None) == -1 and b"workspace" in L.dynb_last_error()
+    a.activation = 0                                   # without slopes no rows of d_z are kept, unless they are copied
+    a.unaligned = 0
+    assert L.dynb_expert_linear_workspace_bytes(ctypes.byref(a), 1, 1, 1, ctypes.byref(n)) == 0
+    assert L.dynb_expert_linear_backward(ctypes.byref(a), at, 8, at, 17, None, at, at, at, at, at, n.value, None) == -1 and b"workspace" in L.dynb_last_error()
+
+
 @pytest.mark.parametrize("n,choices,width,dtype", [(-1, 2, 8, 0), (3, 0, 8, 0), (3, 33, 8, 0), (2 ** 30, 2, 8, 0), (3, 2, 0, 0), (3, 2, 16385, 0), (3, 2, 8, 1), (3, 2, 8, 0)])
 def test_combine_entry_refuses(n, choices, width, dtype):
     """The last case: null pointers."""

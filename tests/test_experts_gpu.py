@@ -364,6 +364,31 @@ def test_linear_strides(cuda, dtype):
         grad.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_linear_rows_off_16_bytes_give_the_same_bits(cuda, dtype):
+    dtype = M.TYPES[dtype]
+    routing, x, w, b, g = _linear_case(700, 4, 3, 72, 136, dtype, False, True)
+
+    def off(t):
+        moved = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        return moved.copy_(t)
+
+    def run(x, g, want, activation):
+        leaves = [t.detach().requires_grad_(i in want) for i, t in enumerate((x, w, b))]
+        z = D.expert_linear(*leaves[:2], routing, leaves[2], activation)
+        return [z.detach(), *torch.autograd.grad(z, [leaves[i] for i in want], g)]
+
+    odd = torch.cat([x, x], 1)[:, :73]
+    odd = odd.contiguous()[:, :72]
+    for activation in (None, "silu"):
+        for want in ((0,), (1, 2), (0, 1, 2)):
+            one = run(x, g, want, activation)
+            for xx, gg in ((off(x), g), (odd, g), (x, off(g)), (off(x), off(g))):
+                assert all(torch.equal(a, c) for a, c in zip(one, run(xx, gg, want, activation)))
+            with torch.autograd.graph.saved_tensors_hooks(off, lambda t: t):   # slopes among them
+                assert all(torch.equal(a, c) for a, c in zip(one, run(x, g, want, activation)))
+
+
 def test_linear_of_no_rows(cuda):
     routing = D.Routing(*X.routing_by_hand(0, 3, 2, 0.0, 1, "cuda"))
     x, w, b = (torch.randn(*s, device=cuda, requires_grad=True) for s in ((0, 8), (3, 8, 4), (3, 4)))
