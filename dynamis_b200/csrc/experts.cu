@@ -126,17 +126,21 @@ ex_combine_backward_kernel(const T* z, const float* weights, const int32_t* expe
     }
 }
 
+__host__ __device__ constexpr int ex_whole(int wide) { return (wide + 7) / 8 * 8; }
+
 // Rows (times their slopes, or as they are where there are none) to rows of `out_row` elements, zeros behind `wide`: a warp a row.  For gradients of the matrices alone, where no
-// pass of dx leaves du, and for rows that the products cannot read by whole pieces (120 k pairs of 129 x 131 bf16 read by single elements: 233 us for dx and 87 for dW, copied first 118 and 50, and 22 a copy).
+// pass of dx leaves du, and for rows that the products cannot read or store by whole pieces (120 k pairs of 129 x 131 bf16 with SiLU, forward, dx and dW: 354, 298 and 87 us by single
+// elements; 48, 45 and 49 on copies, and 24 a copy).
 template <typename T>
 __global__ void __launch_bounds__(EX_THREADS)
 ex_copy_kernel(const T* in, int64_t in_row, const void* slope, T* out, int64_t n, int wide, int out_row)
 {
+    const int slope_row = ex_whole(wide);
     for (int64_t p = (int64_t)blockIdx.x * (EX_THREADS / 32) + threadIdx.x / 32; p < n; p += (int64_t)gridDim.x * (EX_THREADS / 32))
 #pragma unroll 4
         for (int c = threadIdx.x % 32; c < out_row; c += 32) {
             float v = c < wide ? tl_get(in + p * in_row + c) : 0.0f;
-            if (slope != nullptr && c < wide) v *= sizeof(T) == 4 ? static_cast<const float*>(slope)[p * wide + c] : ex_slope_of(static_cast<const uint16_t*>(slope)[p * wide + c]);
+            if (slope != nullptr && c < wide) v *= sizeof(T) == 4 ? static_cast<const float*>(slope)[p * slope_row + c] : ex_slope_of(static_cast<const uint16_t*>(slope)[p * slope_row + c]);
             tl_put(out + p * out_row + c, v);
         }
 }
@@ -255,7 +259,6 @@ static cudaError_t ex_combine(const Z* z, const float* weights, const int32_t* e
     return cudaGetLastError();
 }
 
-static int ex_whole(int wide) { return (wide + 7) / 8 * 8; }
 // Whether rows are copied before the products read them: they do so by pieces of 8 elements on 16 bytes.
 static bool ex_copies(const void* p, int64_t row, int wide, int size) { return wide % 8 != 0 || !ex_on(p, row, size, 16); }
 
@@ -266,16 +269,17 @@ static cudaError_t ex_copy(const void* in, int64_t in_row, const void* slope, vo
     return cudaGetLastError();
 }
 
-// Workspaces: the matrices as the kernel reads them, rows of x that were copied; backward also du, or copies of its rows, the gradients of x by pairs, the sums of pieces.
-struct ExLayout { int64_t x, du, by_pair, partial, total; };
+// Workspaces: the matrices as the kernel reads them, rows of x that were copied, and of results that will be; backward also du, or copies of its rows, the gradients of x by pairs, the sums of pieces.
+struct ExLayout { int64_t x, out, du, by_pair, partial, total; };
 static ExLayout ex_layout(const ExArgs& e, int dtype, bool back, bool dx, bool weights, bool copy_x, bool copy_dy)
 {
     const int size = dtype == DYNB_F32 ? 4 : 2;
     ExLayout l;
     l.x = align_up(!back || dx ? ex_packed_bytes(e, back, dtype) : 0, 256);
-    l.du = l.x + align_up(copy_x && (!back || weights) ? e.n_in * ex_whole(e.t.inner) * size : 0, 256);
+    l.out = l.x + align_up(copy_x && (!back || weights) ? e.n_in * ex_whole(e.t.inner) * size : 0, 256);
+    l.du = l.out + align_up(!back && e.t.outer % 8 != 0 ? e.t.n * ex_whole(e.t.outer) * size : back && dx && e.t.inner % 8 != 0 ? e.n_in * ex_whole(e.t.inner) * size : 0, 256);
     l.by_pair = l.du + align_up(!back ? 0 : copy_dy ? e.t.n * ex_whole(e.t.outer) * size : weights && e.activation != DYNB_ACTIVATION_NONE ? e.t.n * e.t.outer * size : 0, 256);
-    l.partial = l.by_pair + align_up(back && dx && e.fan > 1 ? e.t.n * e.t.inner * 4 : 0, 256);
+    l.partial = l.by_pair + align_up(back && dx && e.fan > 1 ? e.t.n * ex_whole(e.t.inner) * 4 : 0, 256);
     l.total = l.partial + align_up(back && weights ? ex_stretches(e) * ((int64_t)e.t.inner * e.t.outer + e.t.outer) * 4 : 0, 256);
     return l;
 }
@@ -289,7 +293,11 @@ static int ex_forward(ExArgs& e, int dtype, unsigned char* ws, const ExLayout& l
         a.x = ws + l.x;
         a.x_row = ex_whole(a.inner);
     }
+    void* const z = a.y;
+    e.out_row = ex_whole(a.outer);
+    if (a.outer % 8 != 0) a.y = ws + l.out;   // whole pieces are stored; single elements by the copy alone
     DYNB_CUDA_OK(ex_mma_rows(e, 0, dtype, ws, s));
+    if (a.outer % 8 != 0) DYNB_CUDA_OK(ex_copy<T>(a.y, e.out_row, nullptr, z, a.n, a.outer, a.outer, s));
     return DYNB_OK;
 }
 
@@ -308,9 +316,13 @@ static int ex_backward(ExArgs& e, int dtype, const int32_t* experts, void* d_x, 
             e.du = ws + l.du;
         }
         if (d_x != nullptr) {
-            a.dx = e.fan > 1 ? ws + l.by_pair : static_cast<unsigned char*>(d_x);
+            const bool copy = a.inner % 8 != 0;   // as forward
+            void* const sums = copy ? ws + l.out : d_x;
+            e.out_row = ex_whole(a.inner);
+            a.dx = e.fan > 1 ? ws + l.by_pair : static_cast<unsigned char*>(sums);
             DYNB_CUDA_OK(ex_mma_rows(e, 1, dtype, ws, s));
-            if (e.fan > 1) DYNB_CUDA_OK((ex_combine<float, T>(reinterpret_cast<const float*>(ws + l.by_pair), nullptr, experts, nullptr, 0, static_cast<T*>(d_x), e.n_in, e.fan, a.inner, s)));
+            if (e.fan > 1) DYNB_CUDA_OK((ex_combine<float, T>(static_cast<const float*>(a.dx), nullptr, experts, nullptr, 0, static_cast<T*>(sums), e.n_in, e.fan, ex_whole(a.inner), s)));
+            if (copy) DYNB_CUDA_OK(ex_copy<T>(sums, e.out_row, nullptr, d_x, e.n_in, a.inner, a.inner, s));
         } else if (e.du != nullptr) {
             DYNB_CUDA_OK(ex_copy<T>(a.dy, a.dy_row, e.slope, e.du, a.n, a.outer, a.outer, s));
         }

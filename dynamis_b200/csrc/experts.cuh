@@ -10,9 +10,10 @@ namespace dynb {
 // Pairs p = (row, choice), numbered row * choices + choice.  A pair reads row p / fan of x (fan = choices, or 1 where x is of pairs).
 struct ExArgs {
     TlArgs t;                  // x, w, b, dy, order, start; n: pairs; y: result, dx: gradient of x by pairs
-    void* slope;               // the activation's slope, [pairs, outer], or null
+    void* slope;               // the activation's slope, [pairs, outer rounded up to 8], or null
     void* du;                  // room for dz times the slope, [pairs, outer], or null
     int64_t n_in;              // rows of x
+    int64_t out_row;           // elements from row to row of the results of a rows' pass, and forward of the slopes
     int fan, activation;
 };
 

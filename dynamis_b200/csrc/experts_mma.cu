@@ -259,7 +259,7 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
         const bool with_offset = !plan.back && a.b != nullptr;
         const int activation = plan.back ? DYNB_ACTIVATION_NONE : e.activation;
         const bool with_slope = activation != DYNB_ACTIVATION_NONE && e.slope != nullptr;
-        ex_clear_absent(a, out, (int64_t)nn * SIZE, plan.store >= 16 ? 16 : 2, ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OUT + warp, (int64_t)gridDim.x * gridDim.y * OUT);
+        ex_clear_absent(a, out, e.out_row * SIZE, plan.store >= 16 ? 16 : 2, ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * OUT + warp, (int64_t)gridDim.x * gridDim.y * OUT);
         float* const offset = offsets[warp];
         int buffer = 0, offset_type = -1;
         uint32_t phase = 0;
@@ -313,8 +313,8 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     tm_words<O>(v, words + i * SIZE / 4);
                 }
                 if (r < 0) continue;
-                em_put(out + ((int64_t)r * nn + col0 + c) * SIZE, words, (have - c) * SIZE, plan.store, SIZE);
-                if (with_slope) em_put(static_cast<unsigned char*>(e.slope) + ((int64_t)r * nn + col0 + c) * SIZE, slopes, (have - c) * SIZE, plan.slope_store, SIZE);
+                em_put(out + (r * e.out_row + col0 + c) * SIZE, words, (have - c) * SIZE, plan.store, SIZE);
+                if (with_slope) em_put(static_cast<unsigned char*>(e.slope) + (r * e.out_row + col0 + c) * SIZE, slopes, (have - c) * SIZE, plan.slope_store, SIZE);
             }
             tensor_fence_before();
             __syncwarp();
@@ -964,15 +964,15 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
 {
     constexpr int SIZE = (int)sizeof(T);
     const TlArgs& a = e.t;
-    const int kk = back ? a.outer : a.inner, nn = back ? a.inner : a.outer;
+    const int kk = back ? a.outer : a.inner;
     const void* const in = back ? a.dy : a.x;
     const void* const out = back ? a.dx : a.y;
     const bool slope = back && e.activation != DYNB_ACTIVATION_NONE && e.slope != nullptr;   // rows that were copied have met theirs
     int tiles;
     EmPlan p = em_plan<T>(e, back, SIZE == 2 && slope, &tiles);
     p.packed = static_cast<const unsigned char*>(packed);
-    p.store = tm_on(out, nn, sizeof(O), 32) ? 32 : tm_on(out, nn, sizeof(O), 16) ? 16 : (int)sizeof(O);
-    p.slope_store = tm_on(e.slope, nn, SIZE, 32) ? 32 : tm_on(e.slope, nn, SIZE, 16) ? 16 : SIZE;
+    p.store = tm_on(out, e.out_row, sizeof(O), 32) ? 32 : tm_on(out, e.out_row, sizeof(O), 16) ? 16 : (int)sizeof(O);
+    p.slope_store = tm_on(e.slope, e.out_row, SIZE, 32) ? 32 : tm_on(e.slope, e.out_row, SIZE, 16) ? 16 : SIZE;
     const bool wide_w = tm_on(a.w, a.outer, SIZE, 16) && a.outer % 8 == 0;
     const int64_t units = (int64_t)a.types * tiles * p.chunks * (p.columns / (wide_w && !back ? 16 / SIZE : 1)) * 8;
     (wide_w ? ex_pack_kernel<T, true> : ex_pack_kernel<T, false>)<<<(unsigned)std::min<int64_t>((units + 255) / 256, (int64_t)sm_count_cached() * 8), 256, 0, s>>>(

@@ -237,7 +237,7 @@ class _ExpertLinear(torch.autograd.Function):
             z = torch.empty((routing.num_rows, routing.choices, weight.size(2)), dtype=x.dtype, device=dev)
             slope = None
             if ctx is not None and activation:
-                slope = torch.empty(z.shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.int16, device=dev)
+                slope = torch.empty((*z.shape[:2], -(-z.size(2) // 8) * 8), dtype=torch.float32 if x.dtype == torch.float32 else torch.int16, device=dev)
             args = _linear_args(weight, routing, paired, activation, x.dtype)
             args.unaligned = int(_unaligned(flat))
             ws = _linear_workspace(args, 0, 0, 0, dev)

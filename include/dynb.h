@@ -568,7 +568,7 @@ int dynb_route_experts_backward(const dynb_routing* args, const int32_t* experts
 /* Products with the matrices of a row's experts: z[i, j] = act(x[i] weight[e_ij] (+ bias[e_ij])), or x[i, j] where x is `paired`; weight
  * [experts, inner, outer], contiguous, as bias, z and the gradients are.  x and d_z have strides in elements from row to row (from pair to pair).  Places
  * without an expert give zeros.  slope_dev (NULL when there is no backward pass, or no activation): what the backward pass needs of the activation,
- * [n_rows choices, outer] of 4 bytes for DYNB_F32 and 2 otherwise.  Workspaces start on 16-byte boundaries. */
+ * [n_rows choices, outer rounded up to a multiple of 8] of 4 bytes for DYNB_F32 and 2 otherwise.  Workspaces start on 16-byte boundaries. */
 #define DYNB_ACTIVATION_NONE 0
 #define DYNB_ACTIVATION_SILU 1
 #define DYNB_ACTIVATION_GELU 2
