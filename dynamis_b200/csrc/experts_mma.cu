@@ -1,13 +1,13 @@
 // The products by expert on the tensor cores.
 //
 // z = act(x W + b) and dx = du W^T, du = dz act'(u): tiles of 128 pairs of one expert by up to 256 columns (fp32: 128).  Eight warps gather the rows of x (or of dz, times
-// the slope) into stages of 64 summed columns, one warp brings the matrix, one issues the products, eight take the sums out of tensor memory, which holds two tiles, and
+// the slope) into stages of 64 summed columns, one warp brings the matrix, one issues the products, four, eight or sixteen take the sums out of tensor memory, which holds two tiles, and
 // apply offset and activation.  The matrices are laid out once per call as the multipliers read them (ex_pack_kernel: both products read them along the summed
 // index, fp32 in its three parts), so that a piece of 64 summed columns is one copy of a run of bytes.  A matrix that fits beside four stages of rows (two in fp32 and with slopes) stays for
 // all tiles of its expert; a larger one comes anew with every stage, from L2.
 //
 // dW = sum x^T du: a block takes a stretch of an expert's pairs, 128 x up to 256 elements of the matrix; both operands are the gathered rows as they
-// are, read along their columns.  db is a product too, with a tile of ones.
+// are, read along their columns.  db is summed by threads from the stages as they stand in shared memory.
 //
 // fp32 operands are three bf16 parts, six of nine products (mma_parts.cuh).
 //
