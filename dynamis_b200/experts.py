@@ -11,7 +11,7 @@ A layer is ``expert_combine(expert_linear(expert_linear(x, w1, r, b1, "silu"), w
 No counterpart in the reference: its model adapters leave this to their libraries (dynamis_model/src/dynamis_model/nnp/uma.py).
 
 All work is enqueued on the current stream of the tensors' device; nothing waits for the host, and the calls can be captured into a graph.  Gradients are
-formed without atomics on floating-point numbers: the same inputs give the same bits.  They can be taken once; a gradient of a gradient raises.
+formed without atomics on floating-point numbers: the same inputs give the same bits.  They can be taken once; a gradient of a gradient raises, and so does a tangent of forward mode.
 """
 
 from __future__ import annotations
@@ -24,7 +24,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .message import _DTYPES, INT32_MAX, MAX_WIDTH, _STATUS, _each_once, _lists, _lists_refused, _make_status_word, _pointer, _row_last, _runs, _status_word
+from .message import _DTYPES, INT32_MAX, MAX_WIDTH, _STATUS, _differentiates, _each_once, _lists, _lists_refused, _make_status_word, _pointer, _row_last, _runs, _status_word
 
 MAX_EXPERTS = 1024   # DYNB_ROUTING_MAX_EXPERTS
 MAX_CHOICES = 32     # DYNB_ROUTING_MAX_CHOICES
@@ -189,7 +189,7 @@ def route_experts(logits: torch.Tensor, choices: int, score: str = "softmax", bi
     if not 1e-30 <= scale <= 1e30:
         raise RuntimeError(f"scale must lie in [1e-30, 1e30], got {scale}")
     args = (logits, bias, choices, _SCORES[score], groups, kept_groups, int(bool(renormalize)), scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _differentiates(logits):
         return Routing(*_RouteExperts.apply(*args))
     return Routing(*_RouteExperts.forward(None, *args))     # a third of a small call's time is autograd's
 
@@ -298,7 +298,7 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias:
     if activation not in _ACTIVATIONS:
         raise RuntimeError(f"activation must be None, 'silu' or 'gelu', got {activation!r}")
     args = (x, weight, bias, routing, _ACTIVATIONS[activation])
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if _differentiates(x, weight, bias):
         return _ExpertLinear.apply(*args)
     return _ExpertLinear.forward(None, *args)
 
@@ -359,6 +359,6 @@ def expert_combine(z: torch.Tensor, routing: Routing, residual: Optional[torch.T
         if residual.shape != (z.size(0), z.size(2)):
             raise RuntimeError(f"residual must have shape [{z.size(0)}, {z.size(2)}], got {list(residual.shape)}")
     args = (z, routing.weights, residual, routing.experts)
-    if torch.is_grad_enabled() and (z.requires_grad or routing.weights.requires_grad or (residual is not None and residual.requires_grad)):
+    if _differentiates(z, routing.weights, residual):
         return _ExpertCombine.apply(*args)
     return _ExpertCombine.forward(None, *args)

@@ -25,6 +25,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -487,6 +488,12 @@ def _linear_args(x, weight, index: TypeIndex) -> "_lib.TypeLinear":
     a.weight_dev, a.order_dev, a.start_dev = weight.data_ptr(), index.order.data_ptr(), index.start.data_ptr()
     a.n_rows, a.types, a.inner, a.outer, a.dtype = x.size(0), weight.size(0), weight.size(1), weight.size(2), _DTYPES[x.dtype]
     return a
+
+
+def _differentiates(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on these tensors has to go by way of autograd: a gradient is wanted of one of them, or a level of forward mode is open, in which one may
+    have a tangent (autograd refuses that, as there is no formula for it; past autograd the tangent would be lost without a word)."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _row_last(t: torch.Tensor) -> torch.Tensor:

@@ -4,7 +4,7 @@
 No counterpart in the reference: its model adapters leave this to their libraries (dynamis_model/src/dynamis_model/nnp/uma.py).
 
 All work is enqueued on the current stream of the tensors' device.  Gradients are formed without atomics: the same inputs give the same bits.
-They can be taken once; a gradient of a gradient raises.
+They can be taken once; a gradient of a gradient raises, and so does a tangent of forward mode.
 """
 
 from __future__ import annotations
@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .message import _DTYPES, FLOAT_MAX, INT32_MAX, _heads_last, _pointer
+from .message import _DTYPES, FLOAT_MAX, INT32_MAX, _differentiates, _heads_last, _pointer
 
 _POSITIONS = {torch.float32: _lib.DYNB_F32, torch.float64: _lib.DYNB_F64}
 MAX_DIM = 256        # DYNB_ROTARY_MAX_DIM
@@ -128,6 +128,6 @@ def rotary_heads(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, wave: torc
             raise RuntimeError(f"eps must be finite and not negative, got {eps}")
     weights = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
     args = (q, k, pos.contiguous(), wave.contiguous(), *weights, eps, int(bool(interleaved)))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, pos, q_weight, k_weight)):
+    if _differentiates(q, k, pos, q_weight, k_weight):
         return _RotaryHeads.apply(*args)
     return _RotaryHeads.forward(None, *args)     # a third of a small call's time is autograd's
