@@ -7,8 +7,10 @@ from torch.autograd import forward_ad
 
 import dynamis_b200 as D
 from tests import _experts as X
+from tests import _message as M
 
 pytestmark = pytest.mark.gpu
+U = M.U
 
 
 def _gen(seed):
@@ -45,3 +47,40 @@ def test_forward_mode_derivatives_are_refused(cuda):
                     with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="jvp"):
                         call(*args[:i], forward_ad.make_dual(t, torch.ones_like(t)), *args[i + 1:])
             assert torch.equal(call(*args), want)
+
+
+# ------------------------------------------------------------------------------------------------ routing
+def _sigmoid_gradient(logits, experts, g, renormalize, scale):
+    """(value, bound) of the gradient of sigmoid weights.  1 - s = 1 / (1 + e^l) as a whole: exponential 4 u, addition and division 2 u, relative, whatever is
+    left of it; products and the other factor (weights as in X.route) beside it.  1 - s below 2^-126 may be flushed before it meets g (e^l overflows from
+    l = 88.7 on, where 1 - s is 2.9e-39): off by 2^-126 |g|, in p (g - sum p g) by twice the largest |g|; and the product by 2^-126."""
+    l64, at = logits.detach().double(), experts.long()
+    chosen, g = l64.gather(1, at), g.double() * scale
+    s, rest = torch.sigmoid(chosen), torch.sigmoid(-chosen)
+    if renormalize:
+        logs = torch.nn.functional.logsigmoid(chosen)
+        p = torch.softmax(logs, 1)
+        r = (8 * logs.abs().max(1, keepdim=True).values + at.size(1) + 28) * U
+        dot, off_dot = (p * g).sum(1, keepdim=True), (p * g.abs() * (r + (at.size(1) + 8) * U)).sum(1, keepdim=True)
+        d = p * (g - dot) * rest
+        off = p * (r * (g - dot).abs() + off_dot + 4 * U * (g.abs() + dot.abs())) * rest + 10 * U * d.abs() + 2.0 ** -125 * g.abs().max(1, keepdim=True).values
+    else:
+        d = g * s * rest
+        off = 24 * U * d.abs() + 2.0 ** -126 * g.abs()
+    put = lambda t: torch.zeros_like(l64).scatter_(1, at, t)  # noqa: E731
+    return put(d), put(off) + 2.0 ** -126
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("experts,choices", [(16, 4), (200, 4), (64, 12)])
+def test_route_gradients_of_open_gates(cuda, dtype, renormalize, experts, choices):
+    """Sigmoids next to 1: what they leave of 1 keeps its digits, whichever kernel takes the rows."""
+    gen = _gen(experts)
+    logits = (10 + 20 * torch.rand(300, experts, generator=gen, device="cuda")).to(M.TYPES[dtype])
+    logits[:20] += 60.0
+    g = _normal(gen, 300, choices)
+    leaf = logits.detach().requires_grad_()
+    r = D.route_experts(leaf, choices, score="sigmoid", renormalize=renormalize, scale=1.5)
+    got, = torch.autograd.grad(r.weights, [leaf], g)
+    M.check(got, *_sigmoid_gradient(logits, r.experts, g, renormalize, 1.5), "d_logits")
