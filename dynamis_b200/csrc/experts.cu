@@ -140,7 +140,7 @@ ex_copy_kernel(const T* in, int64_t in_row, const void* slope, T* out, int64_t n
 #pragma unroll 4
         for (int c = threadIdx.x % 32; c < out_row; c += 32) {
             float v = c < wide ? tl_get(in + p * in_row + c) : 0.0f;
-            if (slope != nullptr && c < wide) v *= sizeof(T) == 4 ? static_cast<const float*>(slope)[p * slope_row + c] : ex_slope_of(static_cast<const uint16_t*>(slope)[p * slope_row + c]);
+            if (slope != nullptr && c < wide) v *= sizeof(T) == 4 ? static_cast<const float*>(slope)[p * slope_row + c] : ex_slopes_of(static_cast<const uint16_t*>(slope)[p * slope_row + c]).x;
             tl_put(out + p * out_row + c, v);
         }
 }

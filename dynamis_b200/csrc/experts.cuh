@@ -17,11 +17,26 @@ struct ExArgs {
     int fan, activation;
 };
 
-// The activation's slope beside 16-bit results: steps of 2^-14 from -0.5 on, as 16 bits (slopes lie in [-0.13, 1.13]); all bits set for NaN.  It is off by
-// 2^-15 at most, and 0 and 1 are kept as they are.  (As a 16-bit float it would be off by as much as the result's own rounding, and the gradient with it.)
-// The lowest bits of 2^23 + a whole number are that number; of a NaN that arithmetic makes they are all set.
-__device__ __forceinline__ uint32_t ex_slope_bits(float v) { return __float_as_uint(fmaf(v, 16384.0f, 8388608.0f + 8192.0f)); }   // the lower 16
-__device__ __forceinline__ float ex_slope_of(uint32_t bits) { return bits == 0xffffu ? NAN : fmaf(__uint_as_float(0x4b000000u | bits), 1.0f / 16384.0f, -512.5f); }
+// The activation's slope beside 16-bit results, in 16 bits (slopes lie in [-0.129, 1.13]).  From 1/8 on: steps of 2^-14, the numbers 0x3000 and on, off by 2^-15 at most (a 16-bit
+// float would be off by as much as the result's own rounding, and the gradient with it); 0 and 1 are kept as they are.  Below: an fp16 number, 31/32 of the slope, so that no negative one
+// reaches 1/8, where its steps would be twice as wide; off by 2^-11 of the slope, or 2^-25 where that is more.  (In steps of 2^-14 throughout, SiLU's slopes
+// from u = -13 on were zero, and 7 % off at -10.)  NaN stays one: arithmetic gives 0x7fff, behind the steps.
+constexpr float EX_SLOPE_SCALE = 31.0f / 32.0f;
+__device__ __forceinline__ uint32_t ex_slopes_bits(float v0, float v1)
+{
+    const __half2 h = __floats2half2_rn(v0 * EX_SLOPE_SCALE, v1 * EX_SLOPE_SCALE);
+    const uint32_t small = *reinterpret_cast<const uint32_t*>(&h);
+    // the lowest bits of 2^23 + a whole number are that number
+    const uint32_t s0 = __float_as_uint(fmaf(v0, 16384.0f, 8388608.0f + 12288.0f - 2048.0f)), s1 = __float_as_uint(fmaf(v1, 16384.0f, 8388608.0f + 12288.0f - 2048.0f));
+    return __byte_perm(v0 >= 0.125f ? s0 : small, v1 >= 0.125f ? s1 : small >> 16, 0x5410);
+}
+__device__ __forceinline__ float2 ex_slopes_of(uint32_t pair)
+{
+    const float2 small = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+    const uint32_t b0 = pair & 0xffffu, b1 = pair >> 16;
+    const float s0 = fmaf(__uint_as_float(0x4b000000u | b0), 1.0f / 16384.0f, -512.625f), s1 = fmaf(__uint_as_float(0x4b000000u | b1), 1.0f / 16384.0f, -512.625f);
+    return make_float2(b0 - 0x3000u < 0x4800u ? s0 : small.x * (1.0f / EX_SLOPE_SCALE), b1 - 0x3000u < 0x4800u ? s1 : small.y * (1.0f / EX_SLOPE_SCALE));
+}
 
 __device__ __forceinline__ float ex_inverse(float v)   // to within an unit in the last place; 0 of an infinity
 {

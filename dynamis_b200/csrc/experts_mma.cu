@@ -119,7 +119,8 @@ ex_pack_kernel(const T* w, int64_t experts, int inner, int outer, int back, int 
 // fence, addresses of the next), and while one team is in it the other is, too (200 k pairs 512 x 128: one team with two stages ahead 174 us, two teams 166, rows' pass).
 template <typename T, EmPath PATH> constexpr int EM_TEAMS = sizeof(T) == 4 && PATH == EM_REGISTERS ? 2 : 1;
 
-// Eight elements times their slopes.
+// Eight elements times their slopes.  In 16 bits the product is rounded to the type: it is an operand of the tensor cores, as a 16-bit gradient of a step by step
+// program would be (two operands, rounded and rest, would double the products of dx and dW).
 template <typename T>
 __device__ __forceinline__ void em_times(TmRaw<T>& v, const TmRaw<T>& slope)
 {
@@ -133,13 +134,13 @@ __device__ __forceinline__ void em_times(TmRaw<T>& v, const TmRaw<T>& slope)
         const uint32_t* const s = reinterpret_cast<const uint32_t*>(&slope);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float lo = ex_slope_of(s[i] & 0xffffu), hi = ex_slope_of(s[i] >> 16);
+            const float2 by = ex_slopes_of(s[i]);
             if constexpr (std::is_same<T, __half>::value) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(a + i));
-                const __half2 h = __floats2half2_rn(f.x * lo, f.y * hi);
+                const __half2 h = __floats2half2_rn(f.x * by.x, f.y * by.y);
                 a[i] = *reinterpret_cast<const uint32_t*>(&h);
             } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a[i] << 16) * lo, __uint_as_float(a[i] & 0xffff0000u) * hi);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a[i] << 16) * by.x, __uint_as_float(a[i] & 0xffff0000u) * by.y);
                 a[i] = *reinterpret_cast<const uint32_t*>(&h);
             }
         }
@@ -203,7 +204,7 @@ __device__ __forceinline__ void em_activate(uint32_t (&bits)[EM_COLUMNS], uint32
             slopes[i] = __float_as_uint(s0);
             slopes[i + 1] = __float_as_uint(s1);
         } else {
-            slopes[i / 2] = __byte_perm(ex_slope_bits(s0), ex_slope_bits(s1), 0x5410);
+            slopes[i / 2] = ex_slopes_bits(s0, s1);
         }
     }
 }

@@ -272,8 +272,9 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias:
     [experts, inner, outer], bias [experts, outer]; float32, float16 or bfloat16, all alike; widths at most 16384.  z [rows, choices, outer]; places without an
     expert give zeros and get zero gradients.  activation: None, "silu" or "gelu" (with the normal distribution function).
 
-    Products are summed in 32 bits and rounded once behind the activation; gradients for x, weight and bias.  For 16-bit types the gradient in front of the
-    activation is rounded to the type before it is multiplied.  float32 operands go to the tensor cores as three parts of 8 bits, which hold them whole."""
+    Products are summed in 32 bits and rounded once behind the activation; gradients for x, weight and bias.  For 16-bit types the backward pass takes the
+    activation's slope in 16 bits (to within 2^-15, below 1/8 within 2^-11 of itself or 2^-25), and the gradient in front of the activation is rounded to the
+    type before it is multiplied and summed.  float32 operands go to the tensor cores as three parts of 8 bits, which hold them whole."""
     if not isinstance(routing, Routing):
         raise RuntimeError("routing must be a Routing (see route_experts)")
     if not isinstance(x, torch.Tensor) or not x.is_cuda:

@@ -1,6 +1,8 @@
 """Expert layers and rotary heads on the GPU: calls and values at the limits of what they are for.  The bounds are derived beside the plain forms
 (tests/_experts.py) and here."""
 
+import math
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -84,3 +86,30 @@ def test_route_gradients_of_open_gates(cuda, dtype, renormalize, experts, choice
     r = D.route_experts(leaf, choices, score="sigmoid", renormalize=renormalize, scale=1.5)
     got, = torch.autograd.grad(r.weights, [leaf], g)
     M.check(got, *_sigmoid_gradient(logits, r.experts, g, renormalize, 1.5), "d_logits")
+
+
+# ------------------------------------------------------------------------------------------------ products
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("wide", [16, 17])
+def test_linear_small_slopes_keep_their_digits(cuda, dtype, activation, wide):
+    """Far on the negative side slopes are small, and so are the gradients, but for their own digits: d_x = d_z act'(x) through a matrix of ones on the diagonal.
+      slope in 32 bits: SiLU p (1 + u (1 - p)): exponential (2 + |u|) 2 u, addition and reciprocal 4 u, relative to p, twice in the product;
+        GELU: 7.1.26 of Abramowitz and Stegun, 7.5e-8 in all and below -3 at most 2e-4 of the slope (evaluated down to -10)
+      in memory: 2^-15 from 1/8 on, below 2^-11 of itself, or 2^-25 where that is more, on a scale of 31/32."""
+    dtype = M.TYPES[dtype]
+    x = torch.linspace(-16, 4, 40 * wide, device=cuda).to(dtype).view(40, wide)
+    g = _normal(_gen(wide), 40, 1, wide, dtype=dtype)
+    w = torch.eye(wide, device=cuda, dtype=dtype)[None]
+    leaf = x.detach().requires_grad_()
+    z = D.expert_linear(leaf, w, _routing(40, 1, 1), None, activation)
+    got, = torch.autograd.grad(z, [leaf], g)
+    u, gd = x.double(), g[:, 0].double()
+    if activation == "silu":
+        p = torch.sigmoid(u)
+        slope, off = p * (1 + u * (1 - p)), p * (1 + u.abs()) * (20 + 4 * u.abs()) * U
+    else:
+        slope = 0.5 * torch.erfc(-u * math.sqrt(0.5)) + u * torch.exp(-0.5 * u * u) / math.sqrt(2 * math.pi)
+        off = torch.where(u < -3, 3e-4 * slope.abs(), 1e-7 + 16 * U * (1 + u.abs()))
+    off = off + torch.where(slope.abs() < 0.125, torch.maximum((2.0 ** -11 + 4 * U) * slope.abs(), torch.full_like(u, 1.04 * 2.0 ** -25)), 2.0 ** -15)
+    M.check(got, slope * gd, gd.abs() * off + 2 * U * (slope * gd).abs(), "d_x")
