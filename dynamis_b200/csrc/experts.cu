@@ -207,7 +207,7 @@ static int ex_args(const dynb_expert_linear_args* in, ExArgs* e)
     if (in == nullptr) return fail_arg("null pointer");
     if (in->dtype != DYNB_F32 && in->dtype != DYNB_F16 && in->dtype != DYNB_BF16) return fail_arg("expert_linear: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
     if (in->choices < 1 || in->choices > DYNB_ROUTING_MAX_CHOICES) return fail_arg("expert_linear: choices must lie in [1, 32]");
-    if (in->n_rows < 0 || in->n_rows * in->choices >= INT32_MAX) return fail_arg("expert_linear: rows times choices must lie in [0, 2^31 - 1)");
+    if (in->n_rows < 0 || in->n_rows >= INT32_MAX || in->n_rows * in->choices >= INT32_MAX) return fail_arg("expert_linear: rows times choices must lie in [0, 2^31 - 1)");
     if (in->experts < 1 || in->experts > DYNB_ROUTING_MAX_EXPERTS) return fail_arg("expert_linear: experts must lie in [1, 1024]");
     if (in->inner < 1 || in->outer < 1 || in->inner > DYNB_TYPE_LINEAR_MAX_WIDTH || in->outer > DYNB_TYPE_LINEAR_MAX_WIDTH)
         return fail_arg("expert_linear: widths must lie in [1, 16384]");
@@ -348,7 +348,7 @@ static int ec_check(int64_t n_rows, int choices, int wide, int dtype)
 {
     if (dtype != DYNB_F32 && dtype != DYNB_F16 && dtype != DYNB_BF16) return fail_arg("expert_combine: dtype must be DYNB_F32, DYNB_F16 or DYNB_BF16");
     if (choices < 1 || choices > DYNB_ROUTING_MAX_CHOICES) return fail_arg("expert_combine: choices must lie in [1, 32]");
-    if (n_rows < 0 || n_rows * choices >= INT32_MAX) return fail_arg("expert_combine: rows times choices must lie in [0, 2^31 - 1)");
+    if (n_rows < 0 || n_rows >= INT32_MAX || n_rows * choices >= INT32_MAX) return fail_arg("expert_combine: rows times choices must lie in [0, 2^31 - 1)");
     if (wide < 1 || wide > DYNB_TYPE_LINEAR_MAX_WIDTH) return fail_arg("expert_combine: the width must lie in [1, 16384]");
     return DYNB_OK;
 }

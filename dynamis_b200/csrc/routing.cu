@@ -730,7 +730,7 @@ static int re_args(const dynb_routing* in, ReArgs* a)
     if (in->experts < 1 || in->experts > DYNB_ROUTING_MAX_EXPERTS) return fail_arg("route_experts: experts must lie in [1, 1024]");
     if (in->choices < 1 || in->choices > DYNB_ROUTING_MAX_CHOICES || in->choices > in->experts)
         return fail_arg("route_experts: choices must lie in [1, 32] and be no more than the experts");
-    if (in->n_rows < 0 || in->n_rows * in->choices >= INT32_MAX) return fail_arg("route_experts: rows times choices must lie in [0, 2^31 - 1)");
+    if (in->n_rows < 0 || in->n_rows >= INT32_MAX || in->n_rows * in->choices >= INT32_MAX) return fail_arg("route_experts: rows times choices must lie in [0, 2^31 - 1)");
     if (in->groups < 1 || in->experts % in->groups != 0 || in->kept_groups < 1 || in->kept_groups > in->groups)
         return fail_arg("route_experts: groups must divide the experts, and kept_groups lie in [1, groups]");
     if (in->score != DYNB_SCORE_SOFTMAX && in->score != DYNB_SCORE_SIGMOID) return fail_arg("route_experts: score must be DYNB_SCORE_SOFTMAX or DYNB_SCORE_SIGMOID");
