@@ -734,7 +734,7 @@ static int re_args(const dynb_routing* in, ReArgs* a)
     if (in->groups < 1 || in->experts % in->groups != 0 || in->kept_groups < 1 || in->kept_groups > in->groups)
         return fail_arg("route_experts: groups must divide the experts, and kept_groups lie in [1, groups]");
     if (in->score != DYNB_SCORE_SOFTMAX && in->score != DYNB_SCORE_SIGMOID) return fail_arg("route_experts: score must be DYNB_SCORE_SOFTMAX or DYNB_SCORE_SIGMOID");
-    if (!(in->scale > 0.0f && in->scale <= 3.0e38f)) return fail_arg("route_experts: scale must be positive and finite");
+    if (!(in->scale >= 1e-30f && in->scale <= 1e30f)) return fail_arg("route_experts: scale must lie in [1e-30, 1e30]");
     *a = ReArgs{};
     a->logits = in->logits_dev; a->row = in->logits_row; a->bias = in->bias_dev; a->n = in->n_rows;
     a->count = in->experts; a->choices = in->choices; a->groups = in->groups; a->kept = in->kept_groups;

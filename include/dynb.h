@@ -556,7 +556,7 @@ typedef struct dynb_routing {
     const float* bias_dev;                  /* [experts] or NULL */
     int64_t n_rows;
     int32_t experts, choices, dtype, score, groups, kept_groups, renormalize;
-    float scale;
+    float scale;                            /* in [1e-30, 1e30] */
 } dynb_routing;
 int dynb_route_experts_workspace_bytes(const dynb_routing* args, int64_t* bytes);
 int dynb_route_experts(const dynb_routing* args, int32_t* experts_dev, float* weights_dev, int32_t* order_dev, int32_t* start_dev, void* workspace_dev,

@@ -24,3 +24,13 @@ def test_numbers_of_rows_whose_pairs_wrap_are_refused(n_rows):
                  lambda: L.dynb_expert_combine(None, AT, AT, None, 0, n_rows, 32, 8, 0, AT, None),
                  lambda: L.dynb_expert_combine_backward(None, AT, AT, AT, 8, n_rows, 32, 8, 0, AT, None, None)):
         assert call() == -1 and b"rows times choices" in L.dynb_last_error()
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 0.99e-30, 1.01e30, 3e38])
+def test_scales_that_the_weights_do_not_survive_are_refused(scale):
+    """The gradient divides the weights by the scale: as from Python, it lies in [1e-30, 1e30]."""
+    L, n = _lib.lib(), ctypes.c_int64()
+    for value, rc in ((scale, -1), (1e-30, 0), (1e30, 0)):
+        r = _lib.RoutingArgs(logits_dev=AT, logits_row=64, n_rows=5, experts=64, choices=2, dtype=0, score=0, groups=1, kept_groups=1, renormalize=1, scale=value)
+        assert L.dynb_route_experts_workspace_bytes(ctypes.byref(r), ctypes.byref(n)) == rc
+        assert rc == 0 or b"scale" in L.dynb_last_error()
