@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/dynb.h"
 
 namespace dynb {
@@ -60,6 +62,22 @@ __device__ __forceinline__ uint32_t lanemask_lt()
     uint32_t m;
     asm("mov.u32 %0, %%lanemask_lt;" : "=r"(m));
     return m;
+}
+
+// ---- shared memory of a kernel --------------------------------------------------------------
+// Lets a kernel have up to `most` bytes of dynamic shared memory on the current device.  `most` is what its largest call needs, not what this one does: the limit belongs to the
+// kernel, and a smaller one, set by another thread between this call and its launch, makes the launch fail.  Asked for once (a call of the driver
+// at every launch costs a small call 1 to 2 us).
+static inline cudaError_t allow_shared(const void* kernel, int most)
+{
+    static std::atomic<const void*> known[64][64];   // [device][place by address]; one that is not found is asked for anew
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
+    std::atomic<const void*>* const place = dev < 0 ? nullptr : &known[dev][reinterpret_cast<uintptr_t>(kernel) / 16 % 64];
+    if (place != nullptr && place->load(std::memory_order_relaxed) == kernel) return cudaSuccess;
+    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (rc == cudaSuccess && place != nullptr) place->store(kernel, std::memory_order_relaxed);
+    return rc;
 }
 
 // ---- chained launches ----------------------------------------------------------------------

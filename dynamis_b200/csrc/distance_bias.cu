@@ -308,11 +308,15 @@ static int db_table_blocks(int64_t n)
     return (int)std::max<int64_t>(1, std::min<int64_t>((n + 1023) / 1024, 148));
 }
 
+constexpr int DB_SHARED = 224 << 10;         // of a block for both gradients
+constexpr int DB_TABLE_SHARED = 128 << 10;   // of a block for the table's alone: a copy of the largest table
+static_assert(DYNB_DISTANCE_BIAS_MAX_BUCKETS * 128 <= DB_TABLE_SHARED, "one copy of the table");
+
 // The kernel for both gradients: warps of a block, 0 where the heads or the buckets are too many for it.
 static int db_backward_warps(int buckets, int heads)
 {
     if (heads > 32) return 0;
-    const int words = buckets * 32, room = (224 << 10) / 4 - words;
+    const int words = buckets * 32, room = DB_SHARED / 4 - words;
     return std::min(22, room / (words + DB_SCRATCH));
 }
 
@@ -320,7 +324,7 @@ template <int WIDE>
 static cudaError_t db_backward(const DbArgs& a, int blocks, int warps, cudaStream_t s)
 {
     const int words = a.buckets * 32, smem = 4 * (words + warps * (words + DB_SCRATCH));
-    const cudaError_t rc = cudaFuncSetAttribute(db_backward_kernel<WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t rc = allow_shared(reinterpret_cast<const void*>(db_backward_kernel<WIDE>), DB_SHARED);
     if (rc != cudaSuccess) return rc;
     db_backward_kernel<WIDE><<<blocks, warps * 32, smem, s>>>(a);
     return cudaGetLastError();
@@ -414,9 +418,9 @@ extern "C" int dynb_distance_bias_backward(const float* dist_dev, int64_t n, con
             int wide = 1;
             while (wide < heads && wide < 32) wide *= 2;
             // as many warps as have their copies in 128 KB, and no more than 16
-            const int table_warps = std::max(1, std::min(16, (128 << 10) / (buckets * 128)));
+            const int table_warps = std::max(1, std::min(16, DB_TABLE_SHARED / (buckets * 128)));
             const int smem = table_warps * buckets * 128;
-            DYNB_CUDA_OK(cudaFuncSetAttribute(db_table_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            DYNB_CUDA_OK(allow_shared(reinterpret_cast<const void*>(db_table_kernel), DB_TABLE_SHARED));
             db_table_kernel<<<dim3(blocks, (heads + wide - 1) / wide), table_warps * 32, smem, s>>>(a, wide);
             DYNB_CUDA_OK(cudaGetLastError());
         }

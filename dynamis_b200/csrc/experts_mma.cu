@@ -16,8 +16,6 @@
 // rows and what they write, in fp32 by the chain of a stage from memory through the conversion to the multipliers.  Tiles of 64 x 64 with fused multiply-adds took
 // 4549 us for the first, 14 483 for the next three together and 5502 for the last three.
 
-#include <atomic>
-
 #include "experts.cuh"
 #include "mma_parts.cuh"
 
@@ -913,19 +911,6 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Lets a kernel have `bytes` of shared memory, once for a device (a call of the driver at every launch costs a small call 1 to 2 us).
-static cudaError_t em_allow(const void* kernel, int bytes)
-{
-    static std::atomic<const void*> known[64][64];   // [device][place by address]; one that is not found is asked for anew
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = -1;
-    std::atomic<const void*>* const place = dev < 0 ? nullptr : &known[dev][reinterpret_cast<uintptr_t>(kernel) / 16 % 64];
-    if (place != nullptr && place->load(std::memory_order_relaxed) == kernel) return cudaSuccess;
-    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (rc == cudaSuccess && place != nullptr) place->store(kernel, std::memory_order_relaxed);
-    return rc;
-}
-
 template <typename T>
 static EmPlan em_plan(const ExArgs& e, int back, bool slopes, int* tiles)   // slopes: they are brought beside the rows
 {
@@ -995,7 +980,7 @@ static cudaError_t em_rows(const ExArgs& e, int back, void* packed, cudaStream_t
     }
     const int64_t most = (a.n + TM_ROWS - 1) / TM_ROWS + a.types;
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
-    rc = em_allow(reinterpret_cast<const void*>(kernel), EM_SMEM);
+    rc = allow_shared(reinterpret_cast<const void*>(kernel), EM_SMEM);
     if (rc != cudaSuccess) return rc;
     kernel<<<grid, em_threads<T>(many ? MANY : FEW), p.smem, s>>>(e, p);
     return cudaGetLastError();
@@ -1041,7 +1026,7 @@ static cudaError_t em_weights(const ExArgs& e, cudaStream_t s)
     if constexpr (SIZE == 4) kernel = tm_on(a.x, a.x_row, SIZE, 32) && tm_on(a.dy, a.dy_row, SIZE, 32) ? em_weights_kernel<T, EM_REGISTERS, 2> : em_weights_kernel<T, EM_REGISTERS, 1>;
     else kernel = em_weights_kernel<T, EM_ASYNC, 1>;
     const int smem = 1024 + p.stages * stage, tiles_of = p.row_tiles * p.column_tiles;
-    const cudaError_t rc = em_allow(reinterpret_cast<const void*>(kernel), EW_SMEM);
+    const cudaError_t rc = allow_shared(reinterpret_cast<const void*>(kernel), EW_SMEM);
     if (rc != cudaSuccess) return rc;
     kernel<<<(unsigned)(std::max(1, ex_slices(a.inner, a.outer, sizeof(T))) * tiles_of), EW_THREADS<T>, smem, s>>>(e, p);
     return cudaGetLastError();

@@ -756,22 +756,27 @@ static void (*rt_kernel(int choices))(ReArgs, int, int)
 // Rows of `row` elements may be read, or written, by pieces of 16 bytes.
 static bool re_wide(const void* p, int64_t row, int count, int size) { return starts_on(p, 16) && row * size % 16 == 0 && count * size % 16 == 0; }
 
+// Bytes of shared memory.
+static int rt_choose_shared(int count) { return (2 * count + 1 + RT_WARPS * 32 * (count | 1)) * 4; }
+static int rt_backward_shared(int count) { return RT_WARPS * 32 * (count | 1) * 4; }
+static int re_choose_shared(int count, int groups) { return ((count + 1) * 4 + 15) / 16 * 16 + (groups > 1 ? RE_WARPS * (count + groups) * 8 : 0); }
+
 template <typename T>
 static cudaError_t re_choose(const ReArgs& a, unsigned blocks, cudaStream_t s)
 {
     if (rt_takes(a)) {
-        const int pitch = a.count | 1, smem = (2 * a.count + 1 + RT_WARPS * 32 * pitch) * 4;
+        const int pitch = a.count | 1, smem = rt_choose_shared(a.count);
         void (*const kernel)(ReArgs, int, int) = a.groups > 8 ? rt_kernel<T, 16>(a.choices) : a.groups > 1 ? rt_kernel<T, 8>(a.choices) :
                                                    a.bias != nullptr ? rt_kernel<T, 1>(a.choices) : rt_kernel<T, 0>(a.choices);
-        const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+        const cudaError_t rc = allow_shared(reinterpret_cast<const void*>(kernel), rt_choose_shared(RT_MAX_EXPERTS));
         if (rc != cudaSuccess) return rc;
         kernel<<<blocks, RT_WARPS * 32, smem, s>>>(a, pitch, re_wide(a.logits, a.row, a.count, sizeof(T)));
         return cudaGetLastError();
     }
-    const int smem = ((a.count + 1) * 4 + 15) / 16 * 16 + (a.groups > 1 ? RE_WARPS * (a.count + a.groups) * 8 : 0);
+    const int smem = re_choose_shared(a.count, a.groups);
     void (*kernel)(ReArgs) = a.count <= 32 ? re_choose_kernel<T, 1> : a.count <= 64 ? re_choose_kernel<T, 2> : a.count <= 128 ? re_choose_kernel<T, 4> :
                              a.count <= 256 ? re_choose_kernel<T, 8> : a.count <= 512 ? re_choose_kernel<T, 16> : re_choose_kernel<T, 32>;
-    const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+    const cudaError_t rc = allow_shared(reinterpret_cast<const void*>(kernel), re_choose_shared(DYNB_ROUTING_MAX_EXPERTS, DYNB_ROUTING_MAX_EXPERTS));
     if (rc != cudaSuccess) return rc;
     kernel<<<blocks, RE_WARPS * 32, smem, s>>>(a);
     return cudaGetLastError();
@@ -781,8 +786,8 @@ template <typename T>
 static cudaError_t re_backward(const ReArgs& a, const float* d_weights, void* d_logits, cudaStream_t s)
 {
     if (rt_takes(a)) {
-        const int pitch = a.count | 1, smem = RT_WARPS * 32 * pitch * 4;
-        const cudaError_t rc = smem > 48 * 1024 ? cudaFuncSetAttribute(rt_backward_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+        const int pitch = a.count | 1, smem = rt_backward_shared(a.count);
+        const cudaError_t rc = allow_shared(reinterpret_cast<const void*>(rt_backward_kernel<T>), rt_backward_shared(RT_MAX_EXPERTS));
         if (rc != cudaSuccess) return rc;
         const unsigned blocks = (unsigned)std::min<int64_t>((a.n + RT_WARPS * 32 - 1) / (RT_WARPS * 32), (int64_t)sm_count_cached() * 16);
         rt_backward_kernel<T><<<blocks, RT_WARPS * 32, smem, s>>>(a, d_weights, static_cast<T*>(d_logits), pitch, re_wide(a.logits, a.row, a.count, sizeof(T)),

@@ -514,7 +514,7 @@ static bool tm_rows(const TlArgs& a, int back, cudaStream_t s, cudaError_t* rc)
     const dim3 grid((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, sm_count_cached() / std::min(tiles, sm_count_cached()))), tiles);
     const int smem = 1024 + p.panel_bytes + p.stages * STAGE;
     void (*const kernel)(TlArgs, TmPlan) = wide ? tm_rows_kernel<T, true> : tm_rows_kernel<T, false>;
-    *rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    *rc = allow_shared(reinterpret_cast<const void*>(kernel), TM_SMEM);
     if (*rc != cudaSuccess) return true;
     kernel<<<grid, tm_threads(TM_FEED<T>), smem, s>>>(a, p);
     *rc = cudaGetLastError();
@@ -546,7 +546,7 @@ static cudaError_t tm_weights(const TlArgs& a, cudaStream_t s)
     const dim3 grid((unsigned)tl_stretches(a.n, a.types, a.stretch), (a.inner + TM_ROWS - 1) / TM_ROWS, (a.outer + p.columns - 1) / p.columns);
     const int smem = 1024 + TM_ROWS * 128 + p.stages * stage;
     void (*const kernel)(TlArgs, TwPlan) = wide ? tm_weights_kernel<T, true> : tm_weights_kernel<T, false>;
-    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t rc = allow_shared(reinterpret_cast<const void*>(kernel), TM_SMEM);
     if (rc != cudaSuccess) return rc;
     kernel<<<grid, tm_threads(TW_FEED), smem, s>>>(a, p);
     return cudaGetLastError();

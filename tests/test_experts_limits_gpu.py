@@ -1,13 +1,16 @@
 """Expert layers and rotary heads on the GPU: calls and values at the limits of what they are for.  The bounds are derived beside the plain forms
 (tests/_experts.py) and here."""
 
+import ctypes
 import math
+import threading
 
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import dynamis_b200 as D
+from dynamis_b200 import _lib
 from tests import _experts as X
 from tests import _message as M
 
@@ -113,3 +116,75 @@ def test_linear_small_slopes_keep_their_digits(cuda, dtype, activation, wide):
         off = torch.where(u < -3, 3e-4 * slope.abs(), 1e-7 + 16 * U * (1 + u.abs()))
     off = off + torch.where(slope.abs() < 0.125, torch.maximum((2.0 ** -11 + 4 * U) * slope.abs(), torch.full_like(u, 1.04 * 2.0 ** -25)), 2.0 ** -15)
     M.check(got, slope * gd, gd.abs() * off + 2 * U * (slope * gd).abs(), "d_x")
+
+
+# ------------------------------------------------------------------------------------------------ threads
+def _route_entry(experts):
+    logits, (L, n) = _normal(_gen(experts), 40, experts), (_lib.lib(), ctypes.c_int64())
+    a = _lib.RoutingArgs(logits_dev=logits.data_ptr(), logits_row=experts, n_rows=40, experts=experts, choices=4, groups=4, kept_groups=2, renormalize=1, scale=1.0)
+    assert L.dynb_route_experts_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == 0
+    out = [torch.empty(k, dtype=torch.int32, device="cuda") for k in (160, 160, 160, experts + 1)]
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    return (logits, *out, ws), lambda s: L.dynb_route_experts(ctypes.byref(a), *(t.data_ptr() for t in (*out, ws)), n.value, s), out
+
+
+def _route_backward_entry(experts):
+    logits = _normal(_gen(experts), 40, experts)
+    r = D.route_experts(logits, 4)
+    a = _lib.RoutingArgs(logits_dev=logits.data_ptr(), logits_row=experts, n_rows=40, experts=experts, choices=4, groups=1, kept_groups=1, renormalize=1, scale=1.0)
+    g, out = _normal(_gen(1), 40, 4), torch.empty_like(logits)
+    return (logits, r, g, out), lambda s: _lib.lib().dynb_route_experts_backward(ctypes.byref(a), *(t.data_ptr() for t in (r.experts, r.weights, g, out)), s), [out]
+
+
+def _type_linear_entry(inner):
+    x, w = _normal(_gen(inner), 300, inner), _normal(_gen(1), 2, inner, 64)
+    index, out = D.type_index(torch.arange(300, device="cuda") % 2, 2), torch.empty(300, 64, device="cuda")
+    a = _lib.TypeLinear(weight_dev=w.data_ptr(), order_dev=index.order.data_ptr(), start_dev=index.start.data_ptr(), n_rows=300, types=2, inner=inner, outer=64)
+    return (x, w, index, out), lambda s: _lib.lib().dynb_type_linear(ctypes.byref(a), x.data_ptr(), inner, None, out.data_ptr(), s), [out]
+
+
+def _type_linear_backward_entry(outer):
+    x, w, g = _normal(_gen(outer), 300, 64), _normal(_gen(1), 2, 64, outer), _normal(_gen(2), 300, outer)
+    index, out, n = D.type_index(torch.arange(300, device="cuda") % 2, 2), torch.empty_like(w), ctypes.c_int64()
+    a = _lib.TypeLinear(weight_dev=w.data_ptr(), order_dev=index.order.data_ptr(), start_dev=index.start.data_ptr(), n_rows=300, types=2, inner=64, outer=outer)
+    assert _lib.lib().dynb_type_linear_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    return (x, w, g, index, out, ws), lambda s: _lib.lib().dynb_type_linear_backward(ctypes.byref(a), x.data_ptr(), 64, g.data_ptr(), outer, None, out.data_ptr(), None, ws.data_ptr(),
+                                                                                  n.value, s), [out]
+
+
+def _distance_bias_entry(buckets):
+    dist, table, g = torch.rand(500, device="cuda") * 5, _normal(_gen(buckets), buckets, 8), _normal(_gen(1), 500, 8)
+    out, n = [torch.empty_like(dist), torch.empty_like(table)], ctypes.c_int64()
+    assert _lib.lib().dynb_distance_bias_workspace_bytes(500, buckets, 8, ctypes.byref(n)) == 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    return (dist, table, g, *out, ws), lambda s: _lib.lib().dynb_distance_bias_backward(dist.data_ptr(), 500, table.data_ptr(), buckets, 8, 5.0, 1, g.data_ptr(), out[0].data_ptr(),
+                                                                                     out[1].data_ptr(), ws.data_ptr(), n.value, s), out
+
+
+@pytest.mark.parametrize("entry,sizes", [(_route_entry, (128, 96)), (_route_entry, (1024, 800)), (_route_backward_entry, (128, 100)), (_type_linear_entry, (256, 64)),
+                                         (_type_linear_backward_entry, (128, 16)), (_distance_bias_entry, (64, 300)), (_distance_bias_entry, (1024, 300))])
+def test_entries_in_two_threads(cuda, entry, sizes):
+    """Calls of one kernel that need unlike amounts of shared memory: no thread takes from the other what its launch needs."""
+    cases = [entry(n) for n in sizes]
+    codes, together = [set() for _ in cases], threading.Barrier(len(cases))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+
+    def work(call, stream, seen):
+        together.wait()
+        for _ in range(3000):
+            seen.add(call(stream.cuda_stream))
+
+    threads = [threading.Thread(target=work, args=(c[1], s, seen)) for c, s, seen in zip(cases, streams, codes)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [{0}, {0}]
+    for (_, call, out), stream in zip(cases, streams):
+        beside = [t.clone() for t in out]
+        assert call(torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, beside))
