@@ -475,10 +475,10 @@ def _status_word(dev) -> int:
         _make_status_word(dev)
         found = _STATUS.get(dev.index)
         if found is None:
-            raise RuntimeError("type_linear: the first index of a device must be made before a capture, so that a wait that runs out can be told")
+            raise RuntimeError("the first TypeIndex or Routing of a device must be made before a capture, so that a wait that runs out can be told")
     if found[0].value:
         found[0].value = 0
-        raise RuntimeError("type_linear: a wait inside a kernel of an earlier call ran out; its results are not valid")
+        raise RuntimeError("type_linear or expert_linear: a wait inside a kernel of an earlier call ran out; its results are not valid")
     return found[1]
 
 

@@ -3,8 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from dynamis_b200 import _lib
+from dynamis_b200 import _lib, message
 
 AT = 4096       # an address that no refused call touches
 
@@ -34,3 +35,16 @@ def test_scales_that_the_weights_do_not_survive_are_refused(scale):
         r = _lib.RoutingArgs(logits_dev=AT, logits_row=64, n_rows=5, experts=64, choices=2, dtype=0, score=0, groups=1, kept_groups=1, renormalize=1, scale=value)
         assert L.dynb_route_experts_workspace_bytes(ctypes.byref(r), ctypes.byref(n)) == rc
         assert rc == 0 or b"scale" in L.dynb_last_error()
+
+
+def test_waits_that_ran_out_are_told_of_both_products(monkeypatch):
+    """The word of a device is set by ``type_linear`` and ``expert_linear`` alike, and either call may be the one that finds it."""
+    dev, word = torch.device("cuda:0"), ctypes.c_uint32(1)
+    monkeypatch.setattr(message, "_STATUS", {0: (word, AT)})
+    with pytest.raises(RuntimeError, match="^type_linear or expert_linear: a wait inside a kernel of an earlier call ran out"):
+        message._status_word(dev)
+    assert message._status_word(dev) == AT
+    monkeypatch.setattr(message, "_STATUS", {})
+    monkeypatch.setattr(message, "_make_status_word", lambda dev: None)          # as under a capture
+    with pytest.raises(RuntimeError, match="^the first TypeIndex or Routing of a device must be made before a capture"):
+        message._status_word(dev)
