@@ -252,9 +252,17 @@ static cudaError_t ex_combine(const Z* z, const float* weights, const int32_t* e
         const int lanes = ex_lanes((wide / piece + at_once - 1) / at_once, EX_THREADS);
         kernel<<<ex_grid(n * lanes), EX_THREADS, 0, s>>>(z, weights, experts, residual, residual_row, y, n, choices, wide, lanes);
     };
-    if (piece == MOST) start(ex_combine_kernel<Z, T, MOST, 1>, 1);
-    else if (piece == 4) start(ex_combine_kernel<Z, T, 4, 2>, 2);
-    else if (piece == 2) start(ex_combine_kernel<Z, T, 2, 4>, 4);
+    if (piece == MOST) {
+        start(ex_combine_kernel<Z, T, MOST, 1>, 1);
+        return cudaGetLastError();
+    }
+    if constexpr (MOST > 4) {
+        if (piece == 4) {
+            start(ex_combine_kernel<Z, T, 4, 2>, 2);
+            return cudaGetLastError();
+        }
+    }
+    if (piece == 2) start(ex_combine_kernel<Z, T, 2, 4>, 4);
     else start(ex_combine_kernel<Z, T, 1, 4>, 4);
     return cudaGetLastError();
 }
