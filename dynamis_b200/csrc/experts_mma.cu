@@ -520,14 +520,13 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             }
             copies_wait(0);
         } else {
-            constexpr int AHEAD = 1;
             constexpr int SLOPES = PATH == EM_SLOPE ? UNITS : 1;
             TlTile next = cursor.tile;
             int chunk = 0;
-            TmRaw<T> v[AHEAD][UNITS], slope[AHEAD][SLOPES];
-            bool live[AHEAD];
-            uint32_t row_du[AHEAD][SLOPES];         // pair whose du is kept, or a number that is none; its first column
-            int k_du[AHEAD];
+            TmRaw<T> v[UNITS], slope[SLOPES];       // of the next stage, under way
+            bool more = false;
+            uint32_t row_du[SLOPES];                // pair whose du is kept, or a number that is none; its first column
+            int k_du = 0;
             const bool keep_du = PATH == EM_SLOPE && e.du != nullptr && blockIdx.y == 0;
             auto step = [&](int stages) {           // on to a stage behind the next
                 for (int i = 0; i < stages && next.type >= 0; i++) {
@@ -542,18 +541,18 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
                     }
                 }
             };
-            auto ask = [&](TmRaw<T> (&to)[UNITS], TmRaw<T> (&to_slope)[SLOPES], uint32_t (&to_du)[SLOPES], int& to_k, bool& any) {
-                any = next.type >= 0;
-                if (!any) return;
+            auto ask = [&] {
+                more = next.type >= 0;
+                if (!more) return;
                 const int k = chunk * 64 + piece * 8, have = min(8, kk - k);
-                to_k = k;
+                k_du = k;
 #pragma unroll
                 for (int i = 0; i < UNITS; i++) {
                     const uint32_t at = row_in(rows[i]);
                     const bool ok = at < rows_in;
-                    if constexpr (PATH == EM_SLOPE) to_du[i] = keep_du && have > 0 ? at : 0xffffffffu;
-                    to[i] = em_load<WIDE>(in + (ok ? at * in_row + k : 0), 1, ok ? have : 0);
-                    if constexpr (PATH == EM_SLOPE) to_slope[i] = em_load<WIDE>(static_cast<const T*>(e.slope) + (ok ? (int64_t)at * kk + k : 0), 1, ok ? have : 0);
+                    if constexpr (PATH == EM_SLOPE) row_du[i] = keep_du && have > 0 ? at : 0xffffffffu;
+                    v[i] = em_load<WIDE>(in + (ok ? at * in_row + k : 0), 1, ok ? have : 0);
+                    if constexpr (PATH == EM_SLOPE) slope[i] = em_load<WIDE>(static_cast<const T*>(e.slope) + (ok ? (int64_t)at * kk + k : 0), 1, ok ? have : 0);
                 }
                 step(TEAMS);
             };
@@ -562,40 +561,34 @@ em_rows_kernel(const ExArgs e, const EmPlan plan)
             rows_of(cursor.tile, rows_next);
             step(team);
             stage = team;
-#pragma unroll
-            for (int s = 0; s < AHEAD; s++) ask(v[s], slope[s], row_du[s], k_du[s], live[s]);
-            bool more = true;
+            ask();
             while (more) {
+                if constexpr (PATH == EM_SLOPE) {
 #pragma unroll
-                for (int s = 0; s < AHEAD; s++) {
-                    if (!live[s]) { more = false; break; }
-                    if constexpr (PATH == EM_SLOPE) {
+                    for (int i = 0; i < UNITS; i++) {
+                        em_times(v[i], slope[i]);
+                        if (row_du[i] < rows_in) {
+                            uint4* const to = reinterpret_cast<uint4*>(static_cast<T*>(e.du) + (int64_t)row_du[i] * kk + k_du);
 #pragma unroll
-                        for (int i = 0; i < UNITS; i++) {
-                            em_times(v[s][i], slope[s][i]);
-                            if (row_du[s][i] < rows_in) {
-                                uint4* const to = reinterpret_cast<uint4*>(static_cast<T*>(e.du) + (int64_t)row_du[s][i] * kk + k_du[s]);
-#pragma unroll
-                                for (int h = 0; h < (int)(sizeof(TmRaw<T>) / 16); h++) to[h] = v[s][i].v[h];
-                            }
+                            for (int h = 0; h < (int)(sizeof(TmRaw<T>) / 16); h++) to[h] = v[i].v[h];
                         }
                     }
-                    if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); more = false; break; }
-                    unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
-                    if (tm_odd(v[s])) {
-#pragma unroll
-                        for (int i = 0; i < UNITS; i++) tm_store<true>(v[s][i], to + i * TEAM * 512, TM_ROWS * 128);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < UNITS; i++) tm_store<false>(v[s][i], to + i * TEAM * 512, TM_ROWS * 128);
-                    }
-                    fence_to_tensor();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&bars.full[stage]);
-                    stage += TEAMS;
-                    if (stage >= plan.stages) { stage -= plan.stages; phase ^= 1; }
-                    ask(v[s], slope[s], row_du[s], k_du[s], live[s]);
                 }
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+                unsigned char* const to = stage0 + stage * plan.stage_bytes + tile_piece(tid >> 3, piece);
+                if (tm_odd(v)) {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) tm_store<true>(v[i], to + i * TEAM * 512, TM_ROWS * 128);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < UNITS; i++) tm_store<false>(v[i], to + i * TEAM * 512, TM_ROWS * 128);
+                }
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[stage]);
+                stage += TEAMS;
+                if (stage >= plan.stages) { stage -= plan.stages; phase ^= 1; }
+                ask();
             }
         }
     }
@@ -868,39 +861,32 @@ em_weights_kernel(const ExArgs e, const EwPlan plan)
             copies_wait(0);
         } else {
             // the rows of the next stage are under way in registers, the number of the pair behind it
-            constexpr int AHEAD = 1;
-            TmRaw<T> v[AHEAD][UNITS] = {};
-            bool live[AHEAD];
-            auto fetch = [&](int s) {
-                units_of(id, [&](int i, const T* from, int have) { v[s][i] = em_load<WIDE>(from, 1, have); });
-                live[s] = more;
+            TmRaw<T> v[UNITS] = {};
+            bool live = false;
+            auto fetch = [&] {
+                units_of(id, [&](int i, const T* from, int have) { v[i] = em_load<WIDE>(from, 1, have); });
+                live = more;
                 more = row_of(id);
             };
+            fetch();
+            while (live) {
+                if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); break; }
+                unsigned char* const to = stage0 + stage * stage_bytes + at0;
+                if (tm_odd(v)) {
 #pragma unroll
-            for (int s = 0; s < AHEAD; s++) fetch(s);
-            bool ok = true;
-            while (ok) {
+                    for (int i = 0; i < UNITS; i++)
+                        if (i * GROUPS + group < blocks) tm_store<true>(v[i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
+                } else {
 #pragma unroll
-                for (int s = 0; s < AHEAD; s++) {
-                    if (!live[s]) { ok = false; break; }
-                    if (!bar_wait(&bars.empty[stage], phase)) { tm_ran_out(a); ok = false; break; }
-                    unsigned char* const to = stage0 + stage * stage_bytes + at0;
-                    if (tm_odd(v[s])) {
-#pragma unroll
-                        for (int i = 0; i < UNITS; i++)
-                            if (i * GROUPS + group < blocks) tm_store<true>(v[s][i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < UNITS; i++)
-                            if (i * GROUPS + group < blocks) tm_store<false>(v[s][i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
-                    }
-                    fence_to_tensor();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&bars.full[stage]);
-                    stage += TEAMS;
-                    if (stage >= plan.stages) { stage -= plan.stages; phase ^= 1; }
-                    fetch(s);   // behind the last stage: zeros
+                    for (int i = 0; i < UNITS; i++)
+                        if (i * GROUPS + group < blocks) tm_store<false>(v[i], to + i * GROUPS * PARTS * BLOCK, BLOCK);
                 }
+                fence_to_tensor();
+                __syncwarp();
+                if (lane == 0) bar_arrive(&bars.full[stage]);
+                stage += TEAMS;
+                if (stage >= plan.stages) { stage -= plan.stages; phase ^= 1; }
+                fetch();   // behind the last stage: zeros
             }
         }
     }
