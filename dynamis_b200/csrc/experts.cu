@@ -17,8 +17,10 @@ constexpr int EX_THREADS = 256;
 template <typename T, int N> struct __align__(sizeof(T) * N) ExPack { T v[N]; };
 
 // y_i = r_i + sum_j w_ij z_ij (w null: ones).  Z: type of z.  `lanes` threads (a power of two) a row, K pieces of N elements each at a time, four choices under way.
+// Blocks an SM: four, for which 64 registers are enough but for 56 spilled bytes at most; 32-bit z by whole pieces six, with 8 to 36 spilled bytes (sums of 150 k rows of 2 x 256 back: 67
+// us, with five blocks and no spills 75; of 4 x 256 forward 167 and 149).  Six for narrow 32-bit pieces spilled 448 bytes: 150 k rows of 4 x 102 121 us and now 80, of 4 x 101 176 and 113.
 template <typename Z, typename T, int N, int K>
-__global__ void __launch_bounds__(EX_THREADS, sizeof(Z) == 4 ? 6 : 4)   // blocks that their registers leave room for without spilling
+__global__ void __launch_bounds__(EX_THREADS, sizeof(Z) == 4 && K == 1 ? 6 : 4)
 ex_combine_kernel(const Z* z, const float* weights, const int32_t* experts, const T* residual, int64_t residual_row, T* y, int64_t n, int choices, int wide, int lanes)
 {
     const int in_row = threadIdx.x & (lanes - 1), rows = EX_THREADS / lanes, apart = lanes * N;
