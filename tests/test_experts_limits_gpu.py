@@ -91,6 +91,21 @@ def test_route_gradients_of_open_gates(cuda, dtype, renormalize, experts, choice
     M.check(got, *_sigmoid_gradient(logits, r.experts, g, renormalize, 1.5), "d_logits")
 
 
+@pytest.mark.parametrize("spread", [4.0, 8.0])
+@pytest.mark.parametrize("experts,choices,groups,kept", [(64, 6, 8, 4), (128, 8, 1, 1), (32, 4, 4, 2)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_peaked_logits(cuda, spread, experts, choices, groups, kept, score):
+    """Scores far below the largest decide: many rows are looked at again in 64 bits, and all choices are those of 64 bits."""
+    gen = _gen(experts + int(spread))
+    logits = _normal(gen, 700, experts) * spread
+    for bias in (None, 0.1 * _normal(gen, experts)):
+        how = dict(score=score, groups=groups, kept_groups=kept, bias=bias)
+        r, ref = D.route_experts(logits, choices, **how), X.route(logits, choices, **how)
+        for name in ("experts", "order", "start"):
+            assert torch.equal(getattr(r, name).cpu(), ref[name]), name
+        M.check(r.weights.cpu(), *ref["weights"], "weights")
+
+
 # ------------------------------------------------------------------------------------------------ products
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
@@ -116,6 +131,51 @@ def test_linear_small_slopes_keep_their_digits(cuda, dtype, activation, wide):
         off = torch.where(u < -3, 3e-4 * slope.abs(), 1e-7 + 16 * U * (1 + u.abs()))
     off = off + torch.where(slope.abs() < 0.125, torch.maximum((2.0 ** -11 + 4 * U) * slope.abs(), torch.full_like(u, 1.04 * 2.0 ** -25)), 2.0 ** -15)
     M.check(got, slope * gd, gd.abs() * off + 2 * U * (slope * gd).abs(), "d_x")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,experts,inner,outer,paired", [(50_000, 300, 64, 64, False), (17_000, 7, 1032, 520, True), (24_000, 90, 512, 128, False)])
+def test_linear_walks_of_many_tiles(cuda, dtype, rows, experts, inner, outer, paired):
+    """Blocks that take five tiles of rows and more, with changes of the expert among them, matrices that stay and that come with every stage."""
+    gen, dtype = _gen(rows), M.TYPES[dtype]
+    routing = _routing(rows, experts, 2, 0.02, inner)
+    x, g = _normal(gen, *((rows, 2) if paired else (rows,)), inner, dtype=dtype), _normal(gen, rows, 2, outer, dtype=dtype)
+    w, b = (_normal(gen, experts, inner, outer) * inner ** -0.5).to(dtype), _normal(gen, experts, outer, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    z = D.expert_linear(*leaves[:2], routing, leaves[2], "silu")
+    grads = torch.autograd.grad(z, leaves, g)
+    ref = X.linear(x, w, routing.experts, b, "silu", g)
+    for name, got in zip(("z", "d_x", "d_weight", "d_bias"), (z, *grads)):
+        M.check(got, *ref[name], name)
+    routing.check_status()
+
+
+@pytest.mark.parametrize("dtype,rows,steps", [("f32", 6000, 64), ("f16", 30_000, 470), ("bf16", 30_000, 470)])
+def test_linear_cuts_a_sum_off_once_a_step(cuda, dtype, rows, steps):
+    """Operands of one sign: the tensor cores cut a sum off towards zero at every step of 16 products, by half of its last place on average, at most 2^-23 of it.
+    Partial sums grow evenly, so over n steps this costs at most (n + 1) / 4 * 2^-23 =: c of the whole on average.  n for the matrices' gradient: the pairs of
+    a sum over 16, which are 1024 of 3000 in fp32 and a slice of 7500 in 16 bits (148 SMs, tiles of 128 x 128 and 128 x 256 of 1024 x 1024 elements); for rows
+    64.  Parts of fp32 numbers have 8 bits, and their products end above the last place of sums as short as these.  Products of 16-bit numbers reach below it, and
+    each of the 17 terms of a step may be cut off there: 17 c at most; and results in 16 bits are not to show it: an eighth of a step of the type.
+    Beside it 2^-24.  The mean of the roundings to the type does not vanish where the values lie about a power of two (the step doubles there: exact sums of
+    this kind, rounded to bfloat16, come out 2.8e-5 too small on average), so the exact sums are rounded, too.  Both roundings differ in a share c / eps of the
+    elements, by a step: the mean over 2^20 of them or more is off by sqrt(c eps / 2^20), taken five times."""
+    dtype = M.TYPES[dtype]
+    gen, wide = _gen(rows), 1024
+    experts = torch.zeros(rows, 1, dtype=torch.int32, device=cuda)
+    routing = D.Routing(experts, torch.ones(rows, 1, device=cuda), torch.arange(rows, dtype=torch.int32, device=cuda), torch.tensor([0, rows], dtype=torch.int32, device=cuda))
+    x, w, g = (torch.rand(*s, generator=gen, device="cuda").to(dtype) for s in ((rows, wide), (1, wide, wide), (rows, 1, wide)))
+    leaves = [t.detach().requires_grad_() for t in (x, w)]
+    z = D.expert_linear(*leaves, routing)
+    dx, dw = torch.autograd.grad(z, leaves, g)
+    xd, wd, gd = x.double(), w[0].double(), g[:, 0].double()
+    for name, got, ref, n in (("z", z.detach()[:, 0], xd @ wd, 64), ("d_x", dx, gd @ wd.T, 64), ("d_weight", dw[0], xd.T @ gd, steps)):
+        lost, most = float(((ref.to(dtype).double() - got.double()) / ref).mean()), (n + 1) / 4 * 2.0 ** -23
+        if dtype != torch.float32:
+            most = min(17 * most, torch.finfo(dtype).eps / 8)
+        noise = 2.0 ** -24 + 5 * math.sqrt(most * torch.finfo(dtype).eps) / wide
+        assert -noise <= lost <= most + noise, (name, lost)
+        M.check(got, ref, (1 if dtype == torch.float32 else 17) * (n + 1) * 2.0 ** -23 * ref, name)
 
 
 # ------------------------------------------------------------------------------------------------ threads
