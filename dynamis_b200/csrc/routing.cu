@@ -212,7 +212,7 @@ __device__ __forceinline__ float rt_value(uint32_t order)
     return __uint_as_float(bits ^ (uint32_t)(~((int32_t)bits >> 31) | (int32_t)0x80000000));
 }
 __device__ __forceinline__ bool rt_nan(uint32_t order) { return order == 0xff800000u; }
-// 32 rows from `row0` on to `tile` (`pitch` floats a row), rows behind the last as zeros.
+// 32 rows from `row0` on to `tile` (`pitch` floats a row).  Rows behind the last are not written, and nobody reads them.
 template <typename T>
 __device__ __forceinline__ void rt_bring(const ReArgs& a, int64_t row0, float* tile, int pitch, int wide)
 {
@@ -391,7 +391,9 @@ rt_choose_kernel(const ReArgs a, int pitch, int wide)
         for (int i = lane; i < a.count; i += 32) far = fmaxf(far, isinf(bias[i]) ? 0.0f : fabsf(bias[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) far = fmaxf(far, __shfl_xor_sync(0xffffffffu, far, o));
-    // how far a key in 32 bits may be off: a score by (experts + 16) 2^-24 (sigmoids 8: exponential and division (3 + |v|) s (1 - s) and 2), the sum with the bias by half a step
+    // how far a key in 32 bits may be off: a score by (experts + 16) 2^-24 (sigmoids 8: exponential and division (3 + |v|) s (1 - s) and 2), the sum with the bias by half a step.
+    // One bound for all keys: where those that decide are all small (a peaked softmax, sigmoids far below zero, no bias), many rows are looked at again.  200 k rows of 64
+    // experts in groups, logits of spread 1.5, 4 and 8: softmax 91, 116 and 308 us, sigmoids 69, 92 and 570; with a bias 67 to 86 at any spread.
     const float near = ((a.sigmoid ? 8.0f : a.count + 16.0f) + 2.0f * far) * 0x1p-24f;
     const int64_t first = blockIdx.x * a.chunk, last = min(first + a.chunk, a.n);
     for (int64_t row0 = first + warp * 32; row0 < last; row0 += RT_WARPS * 32) {
@@ -655,7 +657,7 @@ rt_backward_kernel(const ReArgs a, const float* d_weights, T* d_logits, int pitc
                 for (int i = 0; i < a.count; i++) top = fmaxf(top, l[i]);
 #pragma unroll 8
                 for (int i = 0; i < a.count; i++) {
-                    l[i] = l[i] == -INFINITY ? 0.0f : __expf(l[i] - top);
+                    l[i] = l[i] == -INFINITY ? 0.0f : __expf(l[i] - top);   // as in the choice
                     sum += l[i];
                 }
                 const float over = sum == 0.0f ? 0.0f : 1.0f / sum;
