@@ -751,8 +751,9 @@ static void (*rt_kernel(int choices))(ReArgs, int, int)
     if constexpr (GROUPS == 0)   // logits decide for good: nothing is looked at beside the choices
         return choices <= 1 ? rt_choose_kernel<T, 1, 0> : choices <= 2 ? rt_choose_kernel<T, 2, 0> : choices <= 4 ? rt_choose_kernel<T, 4, 0> :
                choices <= 6 ? rt_choose_kernel<T, 6, 0> : rt_choose_kernel<T, 8, 0>;
-    return choices <= 1 ? rt_choose_kernel<T, 3, GROUPS> : choices <= 2 ? rt_choose_kernel<T, 4, GROUPS> : choices <= 4 ? rt_choose_kernel<T, 6, GROUPS> :
-           choices <= 6 ? rt_choose_kernel<T, 8, GROUPS> : rt_choose_kernel<T, 10, GROUPS>;
+    else
+        return choices <= 1 ? rt_choose_kernel<T, 3, GROUPS> : choices <= 2 ? rt_choose_kernel<T, 4, GROUPS> : choices <= 4 ? rt_choose_kernel<T, 6, GROUPS> :
+               choices <= 6 ? rt_choose_kernel<T, 8, GROUPS> : rt_choose_kernel<T, 10, GROUPS>;
 }
 
 // Rows of `row` elements may be read, or written, by pieces of 16 bytes.
