@@ -11,7 +11,7 @@
 //
 // fp32 operands are three bf16 parts, six of nine products (mma_parts.cuh).
 //
-// 300 k pairs of 64 experts in bf16: 512 x 256 101 us (4.6 TB/s), 256 x 512 with SiLU and its slopes 186 us (3.7 TB/s), dx 248 us (5.0 TB/s, du for the weights' pass among it), dW 152 us.
+// 300 k pairs of 64 experts in bf16: 512 x 256 101 us (4.6 TB/s), 256 x 512 with SiLU and its slopes 184 us (3.8 TB/s), dx 242 us (5.1 TB/s, du for the weights' pass among it), dW 152 us.
 // 200 k pairs of 16 experts in fp32, 512 x 128: 163, 163 and 216 us (0.58, 0.58 and 0.44 of the six products' time).  In 16 bits the rows' passes are bound by the latency of gathered
 // rows and what they write, in fp32 by the chain of a stage from memory through the conversion to the multipliers.  Tiles of 64 x 64 with fused multiply-adds took
 // 4549 us for the first, 14 483 for the next three together and 5502 for the last three.

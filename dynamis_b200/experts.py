@@ -163,7 +163,8 @@ def route_experts(logits: torch.Tensor, choices: int, score: str = "softmax", bi
     with ``renormalize`` ``scale * s`` over the sum of the chosen ones.
 
     A logit or a bias of -inf closes an expert; places that no expert is left for have number -1 and weight 0.  A NaN comes before all numbers.  Keys are compared in
-    64 bits; without bias and groups the logits are.  The gradient of the weights goes to the logits."""
+    64 bits; without bias and groups the logits are.  The gradient of the weights goes to the logits.  The choice has none: an energy whose logits depend on
+    positions has a step where a row's choice changes."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise RuntimeError("logits must be a CUDA tensor")
     if logits.dim() != 2 or logits.dtype not in _DTYPES:
@@ -274,7 +275,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, routing: Routing, bias:
 
     Products are summed in 32 bits and rounded once behind the activation; gradients for x, weight and bias.  For 16-bit types the backward pass takes the
     activation's slope in 16 bits (to within 2^-15, below 1/8 within 2^-11 of itself or 2^-25), and the gradient in front of the activation is rounded to the
-    type before it is multiplied and summed.  float32 operands go to the tensor cores as three parts of 8 bits, which hold them whole."""
+    type before it is multiplied and summed.  float32 operands go to the tensor cores as three parts of 8 bits, which hold them whole.  Slopes (of the size of z) are
+    kept for the backward pass, which holds the gradient in front of the activation beside them and, for x of rows, that of x by pairs in 32 bits."""
     if not isinstance(routing, Routing):
         raise RuntimeError("routing must be a Routing (see route_experts)")
     if not isinstance(x, torch.Tensor) or not x.is_cuda:

@@ -84,7 +84,8 @@ def rotary_heads(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, wave: torc
     strides.  Row i of both is at ``pos[i]``: targets are the first of the rows [owned | ghost], pos [rows, axes] float32 or float64 has as many rows as the
     longer of q and k, and one to three axes.  wave [dim / 2, axes] float32: turns per unit of each axis.  Waves along one axis each are rotary positions with
     several axes; whole waves on fractional coordinates (``pos @ inv(cell)``) are the same in every image of a periodic box; pairs of zero waves stay
-    unturned.  Pair p is elements (p, p + dim / 2), or (2 p, 2 p + 1) with ``interleaved``.  q_weight, k_weight [dim] float32: ones unless given.
+    unturned.  On Cartesian
+    coordinates products of q and k depend on how the system is turned.  Pair p is elements (p, p + dim / 2), or (2 p, 2 p + 1) with ``interleaved``.  q_weight, k_weight [dim] float32: ones unless given.
 
     Turns are formed in 64 bits and whole ones dropped, all else is in 32 bits and rounded once.  Gradients for q, k, pos (forces; formed in 32
     bits, also for float64) and the weights, whose sums over rows are joined in 64 bits; waves have none."""
